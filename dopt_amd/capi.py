@@ -10,6 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdopthip.so")
 
 F32, I32 = 0, 1
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # dopt_hip_activation
 
 
 class HipError(RuntimeError):
@@ -40,6 +41,11 @@ class SplitSum(C.Structure):
 class TensorRef(C.Structure):
     _fields_ = [("w", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
                 ("vhat", C.c_void_p), ("n", C.c_size_t), ("skip_w", C.c_int)]
+
+
+class MatrixRef(C.Structure):
+    """dopt_hip_matrix_ref: a weight as a matrix, with its gradient and momentum."""
+    _fields_ = [("w", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("rows", C.c_size_t), ("cols", C.c_size_t)]
 
 
 _sz, _vp, _i, _f, _d = C.c_size_t, C.c_void_p, C.c_int, C.c_float, C.c_double
@@ -130,6 +136,13 @@ PROTOTYPES = {
                               C.POINTER(SplitSum)],
     "dopt_hip_bn_wait_limit": [C.c_uint],
     "dopt_hip_bn_infer": [_sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp],
+    "dopt_hip_group_norm": [_sz, _sz, _sz, _sz, _i, _f, _i, _vp, _vp, _vp, _vp],
+    "dopt_hip_group_norm_grad": [_sz, _sz, _sz, _sz, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "dopt_hip_dense_act": [_sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "dopt_hip_dense_act_grad": [_sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "dopt_hip_muon_create": [_i, C.POINTER(MatrixRef), C.POINTER(_vp)],
+    "dopt_hip_muon_destroy": [_vp],
+    "dopt_hip_muon_step": [_vp, _f, _f, _i, _f, _i],
     "dopt_hip_optim_create": [_i, C.POINTER(TensorRef), C.POINTER(_vp)],
     "dopt_hip_optim_destroy": [_vp],
     "dopt_hip_sgd_step": [_vp, _f, _f, _i],

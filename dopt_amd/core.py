@@ -526,6 +526,99 @@ register_operation("batchNormGrad", lambda op: True,
 register_operation("batchNormInference", lambda op: True, lambda op: (op.deps[0].dtype, op.deps[0].shape))
 
 
+# Operations without a counterpart in the reference: group norm and the dense layer, each with its activation.
+
+def _norm_sizes(x, attributes):
+    c = x.shape[-1] if attributes["channelsLast"] else x.shape[1]
+    return x.shape[0], c, int(attributes["groups"])
+
+
+def _verify_group_norm(op, x):
+    if op.deps[x].rank < 2 or op.attributes.get("activation") not in capi.ACTIVATIONS.values():
+        return False
+    _, c, groups = _norm_sizes(op.deps[x], op.attributes)
+    return (groups > 0 and c % groups == 0 and op.deps[x + 1].volume == c and op.deps[x + 2].volume == c and
+            all(d.dtype == float32_t for d in op.deps))
+
+
+def _judge_group_norm(op):
+    n, _, groups = _norm_sizes(op.deps[0], op.attributes)
+    return float32_t, (op.deps[0].volume + 2 * n * groups,)
+
+
+def _verify_dense_act(op, x):
+    a, (xs, ws) = op.attributes, op.deps[x:x + 2]
+    return (xs.rank == 2 and ws.rank == 2 and xs.shape[1] == ws.shape[1] and a.get("activation") in capi.ACTIVATIONS.values() and
+            all(d.dtype == float32_t for d in op.deps))
+
+
+def _verify_dense_act_forward(op):
+    a, m, n = op.attributes, op.deps[0].shape[0], op.deps[1].shape[0]
+    rest = [v for v, has in ((n, a["hasBias"]), (m * n, a["hasResidual"])) if has]
+    return _verify_dense_act(op, 0) and [d.volume for d in op.deps[2:]] == rest
+
+
+def _verify_dense_act_grad(op):
+    m, n = op.deps[1].shape[0], op.deps[2].shape[0]
+    return (_verify_dense_act(op, 1) and op.deps[0].volume == m * n and
+            [d.volume for d in op.deps[3:]] == ([m * n] if op.attributes["activation"] else []))
+
+
+register_operation("groupNorm", lambda op: len(op.deps) == 3 and _verify_group_norm(op, 0), _judge_group_norm)
+register_operation("groupNormGrad", lambda op: len(op.deps) == 5 and _verify_group_norm(op, 1) and
+                   _same_type(op.deps[0], op.deps[1]) and
+                   op.deps[4].volume == 2 * op.deps[1].shape[0] * op.attributes["groups"],
+                   lambda op: (float32_t, (op.deps[1].volume + op.deps[2].volume + op.deps[3].volume,)))
+register_operation("denseAct", lambda op: len(op.deps) >= 2 and _verify_dense_act_forward(op),
+                   lambda op: (float32_t, ((2 if op.attributes["keepsPre"] else 1) * op.deps[0].shape[0] * op.deps[1].shape[0],)))
+register_operation("denseActGrad", lambda op: len(op.deps) >= 3 and _verify_dense_act_grad(op),
+                   lambda op: (float32_t, (op.deps[1].volume + op.deps[2].volume + op.deps[2].shape[0],)))
+
+
+def _activation(name):
+    if name not in capi.ACTIVATIONS:
+        raise ValueError("There is no activation %r: %s" % (name, ", ".join(capi.ACTIVATIONS)))
+    return capi.ACTIVATIONS[name]
+
+
+def groupNorm(input, scale, bias, groups, epsilon=1e-5, activation="none", channelsLast=False):   # noqa: A002
+    """[y, mean, rstd]: y = activation((input - mean) * rstd * scale + bias) over `groups` groups of neighbouring channels of each
+    sample; the channels are dimension 1, or the last one.  Gradients flow through y alone."""
+    gn = Operation("groupNorm", [input, scale, bias], {"groups": int(groups), "epsilon": float(epsilon),
+                                                       "activation": _activation(activation), "channelsLast": int(bool(channelsLast))})
+    v, s = input.volume, input.shape[0] * int(groups)
+    return [slice(gn, [0], [v]).reshape(input.shape), slice(gn, [v], [v + s]), slice(gn, [v + s], [v + 2 * s])]
+
+
+def groupNormGrad(parentGrad, op):
+    x, scale, bias = op.deps
+    stats = slice(op, [x.volume], [op.volume])
+    return Operation("groupNormGrad", [parentGrad, x, scale, bias, stats],
+                     {k: op.attributes[k] for k in ("groups", "activation", "channelsLast")})
+
+
+def denseAct(input, weights, bias=None, residual=None, activation="none", keepPre=True):   # noqa: A002
+    """activation(input . weights^T + bias) + residual.  The gradient of an activation reads what it was applied to: keepPre says
+    whether that is written as well (inference does without)."""
+    act = _activation(activation)
+    op = Operation("denseAct", [input, weights] + [d for d in (bias, residual) if d is not None],
+                   {"activation": act, "hasBias": int(bias is not None), "hasResidual": int(residual is not None),
+                    "keepsPre": int(bool(keepPre and act))})
+    shape = [input.shape[0], weights.shape[0]]
+    if op.attributes["keepsPre"]:
+        op = slice(op, [0], [shape[0] * shape[1]])
+    return op.reshape(shape)
+
+
+def denseActGrad(parentGrad, op):
+    a, deps, v = op.attributes, list(op.deps[:2]), op.deps[0].shape[0] * op.deps[1].shape[0]
+    if a["activation"]:
+        if not a["keepsPre"]:
+            raise ValueError("The gradient of denseAct needs keepPre")
+        deps.append(slice(op, [v], [2 * v]))
+    return Operation("denseActGrad", [parentGrad] + deps, {"activation": a["activation"]})
+
+
 def convolution(features, filters, padding=(0, 0), stride=(1, 1)):
     return Operation("convolution", [features, filters], {"padding": list(padding), "stride": list(stride)})
 
@@ -662,6 +755,25 @@ def _reg_grads():
                 slice(packed, [v0 + v1], [v0 + v1 + v2]).reshape(bias.shape),
                 float32(op.deps[3].shape), float32(op.deps[4].shape)]
     g("batchNormTrain", bn_grad)
+
+    def parts(packed, ops):   # a packed result's pieces, shaped as the operations whose gradients they are
+        out, at = [], 0
+        for o in ops:
+            out.append(slice(packed, [at], [at + o.volume]).reshape(o.shape))
+            at += o.volume
+        return out
+
+    def gn_grad(op, pg):
+        x = op.deps[0]
+        return parts(groupNormGrad(slice(pg, [0], [x.volume]).reshape(x.shape), op), op.deps)
+    g("groupNorm", gn_grad)
+
+    def dense_act_grad(op, pg):
+        v = op.deps[0].shape[0] * op.deps[1].shape[0]
+        dy = slice(pg, [0], [v]) if op.attributes["keepsPre"] else pg
+        out = parts(denseActGrad(dy, op), op.deps[:2 + op.attributes["hasBias"]])
+        return out + ([dy.reshape(op.deps[-1].shape)] if op.attributes["hasResidual"] else [])
+    g("denseAct", dense_act_grad)
 
 
 _reg_grads()

@@ -31,6 +31,9 @@ void *workspace(size_t bytes);
 // The same for callers that can do without: null, with no error recorded, where partial sums are parked in it (open_split_set) or
 // it would have to grow while a graph is recorded.
 void *workspace_if_free(size_t bytes);
+// Until it is given back (0), the first `bytes` of the current queue's workspace belong to the caller that asked for them: other
+// requests get what lies behind them and fail rather than grow it.
+void workspace_hold(size_t bytes);
 // Changes whenever a workspace is reallocated (its address may have changed): whoever keeps the
 // address beyond one call -- a recorded HIP graph -- compares generations before using it again.
 unsigned long workspace_generation();
@@ -61,6 +64,8 @@ int product_rank1(bool written, int transA, int transB, size_t M, size_t N, size
 int product_relu_grad(bool written, int transA, int transB, size_t M, size_t N, size_t K, const float *A, const float *B, const float *x, float *C);
 int product_batch(bool written, int n, const int *transA, const int *transB, const size_t *M, const size_t *N, const size_t *K, const float *const *A,
                   const float *const *B, float *const *C);
+// Bytes of workspace that dopt_hip_sgemm_t takes for such a product.
+size_t product_scratch(int transA, int transB, size_t M, size_t N, size_t K);
 uint64_t product_order(bool written, int transA, int transB, size_t M, size_t N, size_t K);
 // sgemm.hip: dw[K][C][3][3] = filter gradient of a 3x3, pad-1 convolution over 2x2 images, from x[N][4C]
 // and dy[N][4K] in one launch.  Returns false, with nothing launched, for shapes it does not take.
@@ -100,6 +105,11 @@ int num_cus();
 // Workgroups of 256 threads that a launch of ours is given at most (a launch takes fewer than 2^32 threads along a dimension).
 constexpr size_t kLaunchBlocks = (size_t)1 << 22;
 inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
+inline bool overlaps(const void *a, size_t na, const void *b, size_t nb)   // ranges of so many bytes; a null pointer overlaps nothing
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x && y && na && nb && x < y + nb && y < x + na;
+}
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // rtc_ops.cpp: the same pointwise program over many tensors as one launch (more, when their addresses do not fit a launch's

@@ -112,6 +112,18 @@ bool need_deps(const Operation &op, size_t n)
     return false;
 }
 
+bool size_attr(const Operation &op, const char *key, size_t *value)
+{
+    const auto *v = sizes_attr(op, key);
+    if (!v) return false;
+    if (v->size() != 1) {
+        fail(DOPT_HIP_ERR_INVALID, "operation '%s': attribute '%s' must be one number", op.opType.c_str(), key);
+        return false;
+    }
+    *value = (*v)[0];
+    return true;
+}
+
 bool need_f32(const Operation &op)
 {
     if (op.dtype == DOPT_HIP_F32) return true;
@@ -126,6 +138,38 @@ void nci(const std::vector<size_t> &shape, size_t *N, size_t *C, size_t *inner)
     *C = shape.size() > 1 ? shape[1] : 1;
     *inner = 1;
     for (size_t i = 2; i < shape.size(); i++) *inner *= shape[i];
+}
+
+// What the dependencies and the result have to hold.
+bool has_volumes(const Graph &g, const Operation &op, const std::vector<size_t> &deps, size_t result)
+{
+    bool ok = op.volume() == result;
+    for (size_t i = 0; i < deps.size(); i++) ok = ok && g.ops[op.deps[i]].volume() == deps[i] && g.ops[op.deps[i]].dtype == DOPT_HIP_F32;
+    if (!ok) fail(DOPT_HIP_ERR_INVALID, "operation '%s': an operand or the result has the wrong size or type", op.opType.c_str());
+    return ok;
+}
+
+struct NormAttrs {
+    size_t N, C, inner, groups;
+    int last, act;
+};
+bool norm_attrs(const Operation &op, const std::vector<size_t> &x, NormAttrs *a)
+{
+    size_t last, act;
+    if (!size_attr(op, "groups", &a->groups) || !size_attr(op, "channelsLast", &last) || !size_attr(op, "activation", &act)) return false;
+    if (x.size() < 2) {
+        fail(DOPT_HIP_ERR_INVALID, "operation '%s': x must have rank 2 or more", op.opType.c_str());
+        return false;
+    }
+    a->last = last != 0;
+    a->act = (int)act;
+    nci(x, &a->N, &a->C, &a->inner);
+    if (last) {
+        a->inner = 1;
+        for (size_t i = 1; i + 1 < x.size(); i++) a->inner *= x[i];
+        a->C = x.back();
+    }
+    return true;
 }
 
 dopt_hip_conv_desc conv_desc(const std::vector<size_t> &x, const std::vector<size_t> &w, const std::vector<size_t> &pad,
@@ -415,6 +459,78 @@ void registerBuiltinsOnce()
         return make([=](const std::vector<const void *> &in, void *out) {
             return dopt_hip_bn_infer(N, C, inner, (const float *)in[0], (const float *)in[1], (const float *)in[2],
                                      (const float *)in[3], (const float *)in[4], (float *)out);
+        });
+    };
+
+    // No counterpart in the reference: group norm and the dense layer with their activations.  Packed results, as batchNormTrain's.
+    R["groupNorm"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps [x, scale, bias]; output [y | mean | rstd]
+        if (!need_deps(op, 3) || !need_f32(op)) return nullptr;
+        NormAttrs a;
+        if (!norm_attrs(op, g.ops[op.deps[0]].shape, &a)) return nullptr;
+        auto it = op.doubleAttrs.find("epsilon");
+        if (it == op.doubleAttrs.end()) {
+            fail(DOPT_HIP_ERR_INVALID, "groupNorm has no 'epsilon' attribute");
+            return nullptr;
+        }
+        const float eps = (float)it->second;
+        if (!has_volumes(g, op, {a.N * a.C * a.inner, a.C, a.C}, a.N * a.C * a.inner + 2 * a.N * a.groups)) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            return dopt_hip_group_norm(a.N, a.C, a.inner, a.groups, a.last, eps, a.act, (const float *)in[0], (const float *)in[1],
+                                       (const float *)in[2], (float *)out);
+        });
+    };
+    R["groupNormGrad"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps [parentGrad, x, scale, bias, stats]; output [dx | dscale | dbias]
+        if (!need_deps(op, 5) || !need_f32(op)) return nullptr;
+        NormAttrs a;
+        if (!norm_attrs(op, g.ops[op.deps[1]].shape, &a)) return nullptr;
+        const size_t total = a.N * a.C * a.inner;
+        if (!has_volumes(g, op, {total, total, a.C, a.C, 2 * a.N * a.groups}, total + 2 * a.C)) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            return dopt_hip_group_norm_grad(a.N, a.C, a.inner, a.groups, a.last, a.act, (const float *)in[0], (const float *)in[1],
+                                            (const float *)in[2], (const float *)in[3], (const float *)in[4], (float *)out);
+        });
+    };
+    R["denseAct"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps [x, w] (+ bias) (+ residual); output [y] or [y | pre]
+        size_t act, bias, residual, keep;
+        if (!size_attr(op, "activation", &act) || !size_attr(op, "hasBias", &bias) || !size_attr(op, "hasResidual", &residual) ||
+            !size_attr(op, "keepsPre", &keep) || !need_deps(op, 2 + (bias != 0) + (residual != 0)) || !need_f32(op))
+            return nullptr;
+        const auto &x = g.ops[op.deps[0]].shape, &w = g.ops[op.deps[1]].shape;
+        if (x.size() != 2 || w.size() != 2 || x[1] != w[1]) {
+            fail(DOPT_HIP_ERR_INVALID, "denseAct: operands must be x [M, K] and w [N, K]");
+            return nullptr;
+        }
+        const size_t M = x[0], K = x[1], N = w[0];
+        std::vector<size_t> volumes{M * K, N * K};
+        if (bias) volumes.push_back(N);
+        if (residual) volumes.push_back(M * N);
+        if (!has_volumes(g, op, volumes, M * N * (keep ? 2 : 1))) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            return dopt_hip_dense_act(M, N, K, (int)act, (const float *)in[0], (const float *)in[1], bias ? (const float *)in[2] : nullptr,
+                                      residual ? (const float *)in[bias ? 3 : 2] : nullptr, (float *)out,
+                                      keep ? (float *)out + M * N : nullptr);
+        });
+    };
+    R["denseActGrad"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps [parentGrad, x, w] (+ pre, with an activation); output [dx | dw | dbias]
+        size_t act;
+        if (!size_attr(op, "activation", &act) || !need_deps(op, act ? 4 : 3) || !need_f32(op)) return nullptr;
+        const auto &x = g.ops[op.deps[1]].shape, &w = g.ops[op.deps[2]].shape;
+        if (x.size() != 2 || w.size() != 2 || x[1] != w[1]) {
+            fail(DOPT_HIP_ERR_INVALID, "denseActGrad: operands must be x [M, K] and w [N, K]");
+            return nullptr;
+        }
+        const size_t M = x[0], K = x[1], N = w[0];
+        std::vector<size_t> volumes{M * N, M * K, N * K};
+        if (act) volumes.push_back(M * N);
+        if (!has_volumes(g, op, volumes, M * K + N * K + N)) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            float *const o = (float *)out;
+            return dopt_hip_dense_act_grad(M, N, K, (int)act, (const float *)in[0], act ? (const float *)in[3] : nullptr,
+                                           (const float *)in[1], (const float *)in[2], o, o + M * K, o + M * K + N * K);
         });
     };
 

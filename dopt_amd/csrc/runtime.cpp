@@ -39,6 +39,7 @@ struct Runtime {
     // workspace, one per queue: kernels of the two queues run at the same time
     void *ws[2] = {nullptr, nullptr};
     size_t ws_bytes[2] = {0, 0};
+    size_t ws_held[2] = {0, 0};        // bytes at its start that a caller keeps between two requests (workspace_hold)
     unsigned long ws_generation = 0;   // bumped whenever a workspace moves: recorded graphs hold its address
     const void *open_split[2][2] = {{nullptr, nullptr}, {nullptr, nullptr}};   // per queue: partial copies convolutions left in the workspace for their readers
 
@@ -157,7 +158,11 @@ void *workspace(size_t bytes)
                                    "that followed it: dopt_hip_split_sum_close, dopt_hip_bn_train_open, dopt_hip_bn_grad_open or dopt_hip_bn_grad_side");
         return nullptr;
     }
-    if (bytes <= r.ws_bytes[l]) return r.ws[l];
+    if (r.ws_held[l] && r.ws_held[l] + bytes > r.ws_bytes[l]) {
+        fail(DOPT_HIP_ERR_RUNTIME, "workspace: %zu bytes behind %zu that are held do not fit", bytes, r.ws_held[l]);
+        return nullptr;
+    }
+    if (bytes <= r.ws_bytes[l]) return (char *)r.ws[l] + r.ws_held[l];
     if (r.capturing) {   // allocation cannot be recorded; the plan falls back to running its kernels directly
         fail(DOPT_HIP_ERR_UNSUPPORTED, "workspace: cannot grow to %zu bytes while a graph is being captured", bytes);
         return nullptr;
@@ -181,8 +186,11 @@ void *workspace_if_free(size_t bytes)
     Runtime &r = rt();
     const int l = r.lane;
     if (r.open_split[l][0] || r.open_split[l][1] || (r.capturing && bytes > r.ws_bytes[l])) return nullptr;
+    if (r.ws_held[l] && r.ws_held[l] + bytes > r.ws_bytes[l]) return nullptr;
     return workspace(bytes);
 }
+
+void workspace_hold(size_t bytes) { rt().ws_held[rt().lane] = bytes; }
 
 // ------------------------------------------------------------------------------- hipRTC
 

@@ -1600,6 +1600,14 @@ int product_relu_grad(bool written, int transA, int transB, size_t M, size_t N, 
     return dopt_hip_relu_bwd(M * N, C, x, C);   // in place: every element is read before it is written
 }
 
+size_t product_scratch(int transA, int transB, size_t M, size_t N, size_t K)
+{
+    const Route r = sgemm_route(transA, transB, M, N, K, false);
+    size_t cuts = r.cuts;
+    if (r.kind == Route::kPanel) cuts = sgemm_route(transA, transB, M, N, K, false, false).cuts;   // operands off the 16-byte grid
+    return cuts > 1 ? cuts * M * N * sizeof(float) : 0;
+}
+
 uint64_t product_order(bool written, int transA, int transB, size_t M, size_t N, size_t K)
 {
     if (!ensure_init()) return 0;   // the cut of a reduction follows the device's size

@@ -125,6 +125,38 @@ def batchNorm(inp, momentum=0.9, gamma_decay=0.0, gamma_proj=None, beta_proj=Non
                                   Parameter(var, None, lambda ignored: var_update)])
 
 
+def groupNorm(inp, groups, activation="none", epsilon=1e-5, channels_last=False, gamma_decay=0.0, gamma_proj=None, beta_proj=None):
+    """Group norm and its activation: a norm that a sample has to itself, so training and inference compute the same.  No counterpart
+    in the reference, whose norm is layers/batchnorm.d."""
+    x, x_tr = inp.output, inp.trainOutput
+    c = x.shape[-1] if channels_last else x.shape[1]
+    gamma, beta = float32([c], np.ones(c, np.float32)), float32([c])
+
+    def norm(v):
+        return core.groupNorm(v, gamma, beta, groups, epsilon, activation, channels_last)[0]
+    y_tr = norm(x_tr)
+    y = y_tr if x is x_tr else norm(x)
+    gamma_loss = None if gamma_decay == 0.0 else gamma_decay * core.sum(gamma * gamma)
+    return Layer([inp], y, y_tr, [Parameter(gamma, gamma_loss, gamma_proj), Parameter(beta, None, beta_proj)])
+
+
+def denseAct(inp, num_outputs, init, activation="none", residual=None, use_bias=True, weight_decay=0.0, weight_proj=None,
+             bias_proj=None):
+    """A dense layer with its activation and, behind that, the sum with another layer's output: one operation.  The reference has
+    layers/dense.d and layers/relu.d."""
+    x, x_tr = inp.output, inp.trainOutput
+    x = x.reshape([x.shape[0], x.volume // x.shape[0]])
+    x_tr = x_tr.reshape([x_tr.shape[0], x_tr.volume // x_tr.shape[0]])
+    weights = float32([num_outputs, x.shape[1]])
+    init.he_gaussian(weights)
+    bias = float32([num_outputs]) if use_bias else None
+    weight_loss = None if weight_decay == 0.0 else weight_decay * core.sum(weights * weights)
+    params = [Parameter(weights, weight_loss, weight_proj)] + ([Parameter(bias, None, bias_proj)] if use_bias else [])
+    y = core.denseAct(x, weights, bias, residual.output if residual else None, activation, keepPre=False)
+    y_tr = core.denseAct(x_tr, weights, bias, residual.trainOutput if residual else None, activation)
+    return Layer([inp] + ([residual] if residual else []), y, y_tr, params)
+
+
 def relu(inp):   # layers/relu.d
     return Layer([inp], core.relu(inp.output), core.relu(inp.trainOutput), [])
 

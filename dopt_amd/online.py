@@ -97,6 +97,52 @@ def amsgrad(outputs, wrt, projs=None, alpha=None, beta1=None, beta2=None, eps=No
     return _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, True, flags)
 
 
+def _is_matrix(w):
+    """Whether a weight is updated as the matrix of its first dimension against the others."""
+    return w.rank >= 2 and w.shape[0] > 1 and w.volume > w.shape[0]
+
+
+def _orthogonalised(u, iterations):
+    rows, cols = u.shape[0], u.volume // u.shape[0]
+    x = u.reshape([rows, cols])
+    x = x / (sqrt(core.sum(x * x)) + 1e-7)
+    if rows > cols:
+        x = core.transpose(x, [1, 0])
+    for _ in range(iterations):
+        a = core.matmul(x, core.transpose(x, [1, 0]))
+        x = 3.4445 * x + core.matmul(-4.7750 * a + 2.0315 * core.matmul(a, a), x)
+    return (core.transpose(x, [1, 0]) if rows > cols else x).reshape(u.shape)
+
+
+def _wide(w):
+    return float(np.sqrt(np.maximum(1.0, w.shape[0] / (w.volume // w.shape[0]))))
+
+
+def muon(outputs, wrt, projs=None, learningRate=0.02, momentumRate=0.95, nesterov=True, decay=0.0, restRate=0.01, iterations=5,
+         flags=0):
+    """Weight matrices move along their momentum's orthogonalised form (see dopt_hip_muon_step), all other parameters as `sgd` moves
+    them with restRate and momentumRate.  No counterpart in the reference."""
+    projs = projs or {}
+    grads = grad(outputs[0], wrt)
+    momentum = [float32(g.shape) for g in grads]
+    newvals, new_momentum = [], []
+    for w, g, m in zip(wrt, grads, momentum):
+        if _is_matrix(w):
+            nm = momentumRate * m + g
+            o = _orthogonalised(g + momentumRate * nm if nesterov else nm, iterations)
+            newvals.append((1.0 - learningRate * decay) * w - (learningRate * _wide(w)) * o)
+        else:
+            nm = m * momentumRate + restRate * g
+            newvals.append(w - nm)
+        new_momentum.append(nm)
+    for i, w in enumerate(wrt):
+        if w in projs:
+            newvals[i] = projs[w](newvals[i])
+    up = _GraphUpdater(outputs, list(outputs) + newvals + new_momentum, list(wrt) + momentum, flags)
+    up.momentum = momentum
+    return up
+
+
 # ------------------------------------------------------------------------------- fused
 
 class _Placeholder:
@@ -154,8 +200,17 @@ class _FusedUpdater:
             self.state["v"] = [ops.Tensor(w.shape) for w in wrt]
         if rule == "amsgrad":
             self.state["vhat"] = [ops.Tensor(w.shape) for w in wrt]
-        self.opt = ops.FusedOptimizer(params, gviews, self.state["m"], self.state.get("v"), self.state.get("vhat"),
-                                      skip)
+        rest = list(range(len(wrt)))
+        self.muon = None
+        if rule == "muon":   # matrices are updated by a set of launches of their own, the rest as sgd
+            mats = [i for i in rest if _is_matrix(wrt[i]) and not skip[i]]
+            rest = [i for i in rest if i not in set(mats)]
+            self.muon = ops.MuonOptimizer(*[[v[i] for i in mats] for v in (params, gviews, self.state["m"])])
+
+        def of(name):
+            return [self.state[name][i] for i in rest] if name in self.state else None
+        self.opt = ops.FusedOptimizer([params[i] for i in rest], [gviews[i] for i in rest], of("m"), of("v"), of("vhat"),
+                                      [skip[i] for i in rest])
 
     def step_async(self, args=None):
         # The plan reads the OLD parameters; the fused kernel then updates them in place; projected
@@ -166,6 +221,9 @@ class _FusedUpdater:
             self.opt.sgd(h["lr"], h["mu"], h["nesterov"])
         elif self.rule == "adam":
             self.opt.adam(h["alpha"], h["beta1"], h["beta2"], h["eps"])
+        elif self.rule == "muon":
+            self.muon.step(h["lr"], h["mu"], h["nesterov"], h["decay"], h["iterations"])
+            self.opt.sgd(h["rest"], h["mu"], False)
         else:
             self.opt.amsgrad(h["alpha"], h["beta1"], h["beta2"], h["eps"])
         if self._post_plan is not None:
@@ -191,3 +249,10 @@ def fused_amsgrad(outputs, wrt, projs=None, alpha=0.001, beta1=0.9, beta2=0.999,
     return _FusedUpdater("amsgrad", outputs, wrt, projs,
                          {"alpha": float(alpha), "beta1": float(beta1), "beta2": float(beta2), "eps": float(eps)},
                          flags)
+
+
+def fused_muon(outputs, wrt, projs=None, learningRate=0.02, momentumRate=0.95, nesterov=True, decay=0.0, restRate=0.01, iterations=5,
+               flags=0):
+    return _FusedUpdater("muon", outputs, wrt, projs,
+                         {"lr": float(learningRate), "mu": float(momentumRate), "nesterov": bool(nesterov), "decay": float(decay),
+                          "rest": float(restRate), "iterations": int(iterations)}, flags)

@@ -421,7 +421,122 @@ def bn_infer(x, scale, bias, mean, var, out=None):
     return y
 
 
+# ------------------------------------------------------------------------------- group norm, dense with activation
+
+def _activation(act):
+    code = capi.ACTIVATIONS.get(act)
+    if code is None:
+        raise capi.HipError(1, "there is no activation %r: %s" % (act, ", ".join(capi.ACTIVATIONS)))
+    return code
+
+
+def _last_nci(shape):
+    return shape[0], shape[-1], _vol(shape[1:-1])
+
+
+def _norm_args(x, scale, bias, groups, channels_last):
+    if len(x.shape) < 2 or x.dtype != _F32 or scale.dtype != _F32 or bias.dtype != _F32:
+        raise capi.HipError(1, "groupNorm: x has rank 2 and more, and everything is float32")
+    N, Cc, inner = _last_nci(x.shape) if channels_last else _nci(x.shape)
+    groups = int(groups)
+    if groups < 1 or Cc % groups or scale.size != Cc or bias.size != Cc:
+        raise capi.HipError(1, "groupNorm: %d channels, %d groups, %d scales, %d biases" % (Cc, groups, scale.size, bias.size))
+    return N, Cc, inner, groups
+
+
+def group_norm(x, scale, bias, groups, eps=1e-5, act="none", channels_last=False, out=None):
+    """act(group norm(x)) of [N, C, ...], or of [N, ..., C] where channels_last: packed [y | mean | rstd], one mean and rstd
+    per sample and group.  act: "none", "relu", "gelu", "silu"."""
+    N, Cc, inner, groups = _norm_args(x, scale, bias, groups, channels_last)
+    packed = _out(out, (x.size + 2 * N * groups,))
+    _run(capi.load().dopt_hip_group_norm(N, Cc, inner, groups, 1 if channels_last else 0, eps, _activation(act), x.ptr, scale.ptr, bias.ptr,
+                                         packed.ptr))
+    return packed
+
+
+def group_norm_grad(dy, x, scale, bias, stats, groups, act="none", channels_last=False, out=None):
+    """Packed [dx | dscale | dbias] from dy and stats, the [mean | rstd] that group_norm left behind y."""
+    N, Cc, inner, groups = _norm_args(x, scale, bias, groups, channels_last)
+    if dy.shape != x.shape or stats.size != 2 * N * groups or dy.dtype != _F32 or stats.dtype != _F32:
+        raise capi.HipError(1, "groupNormGrad: dy is of x's shape, stats holds a mean and a rstd per sample and group")
+    packed = _out(out, (x.size + 2 * Cc,))
+    _run(capi.load().dopt_hip_group_norm_grad(N, Cc, inner, groups, 1 if channels_last else 0, _activation(act), dy.ptr, x.ptr, scale.ptr,
+                                              bias.ptr, stats.ptr, packed.ptr))
+    return packed
+
+
+def _dense_sizes(x, w):
+    if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1] or x.dtype != _F32 or w.dtype != _F32:
+        raise capi.HipError(1, "denseAct: x [M, K] and w [N, K] of float32")
+    return x.shape[0], w.shape[0], x.shape[1]
+
+
+def _operand(t, size, what):
+    """The address of an operand that may be missing."""
+    if t is None:
+        return None
+    if t.size != size or t.dtype != _F32:
+        raise capi.HipError(1, "denseAct: %s has the wrong size or type" % what)
+    return t.ptr
+
+
+def dense_act(x, w, bias=None, residual=None, act="none", out=None, pre=None):
+    """act(x . w^T + bias) + residual; `pre` receives what the activation is applied to, which the gradient reads."""
+    M, N, K = _dense_sizes(x, w)
+    y = _out(out, (M, N))
+    _run(capi.load().dopt_hip_dense_act(M, N, K, _activation(act), x.ptr, w.ptr, _operand(bias, N, "bias"),
+                                        _operand(residual, M * N, "residual"), y.ptr, _operand(pre, M * N, "pre")))
+    return y
+
+
+def dense_act_grad(dy, x, w, pre=None, act="none", dx=None, dw=None, dbias=None):
+    """(dx, dw, dbias); the residual's gradient is dy itself."""
+    M, N, K = _dense_sizes(x, w)
+    code = _activation(act)
+    if pre is None and code:
+        raise capi.HipError(1, "denseActGrad: the gradient of an activation reads what it was applied to")
+    dx, dw, dbias = _out(dx, (M, K)), _out(dw, (N, K)), _out(dbias, (N,))
+    _run(capi.load().dopt_hip_dense_act_grad(M, N, K, code, _operand(dy, M * N, "dy"), _operand(pre, M * N, "pre"), x.ptr, w.ptr, dx.ptr,
+                                             dw.ptr, dbias.ptr))
+    return dx, dw, dbias
+
+
 # ------------------------------------------------------------------------------- optimizers
+
+class MuonOptimizer:
+    """Updates weight matrices in place by their orthogonalised momentum (see dopt_hip_muon_step); a tensor of rank above two is
+    the matrix of its first dimension against the others."""
+
+    def __init__(self, params, grads, m):
+        n = len(params)
+        if len(grads) != n or len(m) != n:
+            raise capi.HipError(1, "MuonOptimizer: a gradient and a momentum for every matrix")
+        refs = (capi.MatrixRef * max(n, 1))()
+        for i, (p, g, q) in enumerate(zip(params, grads, m)):
+            if len(p.shape) < 2 or g.size != p.size or q.size != p.size or any(t.dtype != _F32 for t in (p, g, q)):
+                raise capi.HipError(1, "MuonOptimizer: matrix %d, its gradient or its momentum has the wrong shape or type" % i)
+            refs[i] = capi.MatrixRef(p.ptr, g.ptr, q.ptr, p.shape[0], _vol(p.shape[1:]))
+        self._keep = (params, grads, m)
+        self._h = None
+        h = C.c_void_p()
+        _run(capi.load().dopt_hip_muon_create(n, refs, C.byref(h)))
+        self._h = h
+
+    def step(self, lr=0.02, mu=0.95, nesterov=True, decay=0.0, iterations=5):
+        _run(capi.load().dopt_hip_muon_step(self._h, lr, mu, int(nesterov), decay, iterations))
+
+    def close(self):
+        if self._h:
+            capi.load().dopt_hip_muon_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 
 class FusedOptimizer:
     """Multi-tensor in-place updater over fixed parameter / gradient / state tensors."""

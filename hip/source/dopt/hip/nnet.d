@@ -32,6 +32,12 @@ package
         registerHIPKernel("batchNormTrain", toDelegate(&ctr!BatchNormTrain), true);
         registerHIPKernel("batchNormGrad", toDelegate(&ctr!BatchNormGrad), true);
         registerHIPKernel("batchNormInference", toDelegate(&ctr!BatchNormInference), true);
+
+        //Operations that dopt.core does not define (yet): the kernels wait for its definitions
+        registerHIPKernel("groupNorm", toDelegate(&ctr!GroupNorm), true);
+        registerHIPKernel("groupNormGrad", toDelegate(&ctr!GroupNormGrad), true);
+        registerHIPKernel("denseAct", toDelegate(&ctr!DenseAct), true);
+        registerHIPKernel("denseActGrad", toDelegate(&ctr!DenseActGrad), true);
     }
 }
 
@@ -300,6 +306,122 @@ private
         }
 
         size_t mN, mC, mInner;
+    }
+
+    //Shape and attributes of a group norm: size_t "groups", "channelsLast" and "activation" (dopt_hip_activation)
+    struct NormSize
+    {
+        this(Operation op, const(size_t)[] shape)
+        {
+            groups = op.attributes["groups"].get!size_t;
+            last = op.attributes["channelsLast"].get!size_t != 0 ? 1 : 0;
+            act = cast(int)op.attributes["activation"].get!size_t;
+
+            nci(shape, n, c, inner);
+
+            if(last)
+            {
+                c = shape[$ - 1];
+                inner = 1;
+
+                foreach(s; shape[1 .. $ - 1])
+                {
+                    inner *= s;
+                }
+            }
+        }
+
+        size_t n, c, inner, groups;
+        int last, act;
+    }
+
+    class GroupNorm : HIPKernel
+    {
+        this(Operation op)
+        {
+            mSize = NormSize(op, op.deps[0].shape);
+            mEps = op.attributes["epsilon"].get!double;
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: x, scale, bias; output [y | mean | rstd]
+            hipCheck(dopt_hip_group_norm(mSize.n, mSize.c, mSize.inner, mSize.groups, mSize.last, mEps, mSize.act,
+                f(inputs[0]), f(inputs[1]), f(inputs[2]), f(output)));
+        }
+
+        NormSize mSize;
+        float mEps;
+    }
+
+    class GroupNormGrad : HIPKernel
+    {
+        this(Operation op)
+        {
+            mSize = NormSize(op, op.deps[1].shape);
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: dy, x, scale, bias, [mean | rstd]; output [dx | dscale | dbias]
+            hipCheck(dopt_hip_group_norm_grad(mSize.n, mSize.c, mSize.inner, mSize.groups, mSize.last, mSize.act,
+                f(inputs[0]), f(inputs[1]), f(inputs[2]), f(inputs[3]), f(inputs[4]), f(output)));
+        }
+
+        NormSize mSize;
+    }
+
+    class DenseAct : HIPKernel
+    {
+        this(Operation op)
+        {
+            mM = op.deps[0].shape[0];
+            mK = op.deps[0].shape[1];
+            mN = op.deps[1].shape[0];
+            mAct = cast(int)op.attributes["activation"].get!size_t;
+            mBias = op.attributes["hasBias"].get!size_t != 0;
+            mResidual = op.attributes["hasResidual"].get!size_t != 0;
+            mKeep = op.attributes["keepsPre"].get!size_t != 0;
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: x, w, then the bias and the residual where there are any; output [y] or [y | pre]
+            auto bias = mBias ? f(inputs[2]) : null;
+            auto residual = mResidual ? f(inputs[mBias ? 3 : 2]) : null;
+            auto pre = mKeep ? f(output) + mM * mN : null;
+
+            hipCheck(dopt_hip_dense_act(mM, mN, mK, mAct, f(inputs[0]), f(inputs[1]), bias, residual, f(output), pre));
+        }
+
+        size_t mM, mN, mK;
+        int mAct;
+        bool mBias, mResidual, mKeep;
+    }
+
+    class DenseActGrad : HIPKernel
+    {
+        this(Operation op)
+        {
+            mM = op.deps[1].shape[0];
+            mK = op.deps[1].shape[1];
+            mN = op.deps[2].shape[0];
+            mAct = cast(int)op.attributes["activation"].get!size_t;
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: dy, x, w, then what the activation was applied to where there is one; output [dx | dw | dbias]
+            auto pre = mAct != 0 ? f(inputs[3]) : null;
+            auto dx = f(output);
+            auto dw = dx + mM * mK;
+
+            hipCheck(dopt_hip_dense_act_grad(mM, mN, mK, mAct, f(inputs[0]), pre, f(inputs[1]), f(inputs[2]), dx, dw,
+                dw + mN * mK));
+        }
+
+        size_t mM, mN, mK;
+        int mAct;
     }
 }
 

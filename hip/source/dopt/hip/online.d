@@ -32,7 +32,8 @@ private enum Rule
 {
     sgd,
     adam,
-    amsgrad
+    amsgrad,
+    muon
 }
 
 private class FusedUpdater
@@ -98,6 +99,7 @@ private class FusedUpdater
         }
 
         dopt_hip_tensor_ref[] refs;
+        dopt_hip_matrix_ref[] matrices;
 
         foreach(i, w; wrt)
         {
@@ -114,7 +116,13 @@ private class FusedUpdater
             mState ~= HIPBuffer.create(bytes);
             r.m = cast(float *)mState[$ - 1].ptr;
 
-            if(rule != Rule.sgd)
+            if(rule == Rule.muon && !skip[i] && w.shape.length >= 2 && w.shape[0] > 1 && w.volume > w.shape[0])
+            {
+                matrices ~= dopt_hip_matrix_ref(r.w, r.g, r.m, w.shape[0], w.volume / w.shape[0]);
+                continue;
+            }
+
+            if(rule == Rule.adam || rule == Rule.amsgrad)
             {
                 mState ~= HIPBuffer.create(bytes);
                 r.v = cast(float *)mState[$ - 1].ptr;
@@ -130,6 +138,11 @@ private class FusedUpdater
         }
 
         hipCheck(dopt_hip_optim_create(cast(int)refs.length, refs.ptr, &mHandle));
+
+        if(rule == Rule.muon)
+        {
+            hipCheck(dopt_hip_muon_create(cast(int)matrices.length, matrices.ptr, &mMuon));
+        }
     }
 
     ~this()
@@ -137,6 +150,11 @@ private class FusedUpdater
         if(mHandle !is null)
         {
             dopt_hip_optim_destroy(mHandle);
+        }
+
+        if(mMuon !is null)
+        {
+            dopt_hip_muon_destroy(mMuon);
         }
     }
 
@@ -159,6 +177,12 @@ private class FusedUpdater
             case Rule.amsgrad:
                 hipCheck(dopt_hip_amsgrad_step(mHandle, scalar(mHyper[0]), scalar(mHyper[1]), scalar(mHyper[2]),
                     scalar(mHyper[3]), &mB1, &mB2));
+                break;
+
+            case Rule.muon:
+                hipCheck(dopt_hip_muon_step(mMuon, scalar(mHyper[0]), scalar(mHyper[1]), mNesterov ? 1 : 0,
+                    scalar(mHyper[2]), 5));
+                hipCheck(dopt_hip_sgd_step(mHandle, scalar(mHyper[3]), scalar(mHyper[1]), 0));
                 break;
         }
 
@@ -184,7 +208,7 @@ private class FusedUpdater
     HIPPlan mPlan, mPostPlan;
     DeviceBuffer[] mRets, mPostRets;
     HIPBuffer[] mState;
-    void *mHandle;
+    void *mHandle, mMuon;
 }
 
 /**
@@ -223,6 +247,22 @@ Updater amsgrad(Operation[] outputs, Operation[] wrt, Projection[Operation] proj
 {
     auto u = new FusedUpdater(Rule.amsgrad, outputs, wrt, projs);
     u.mHyper = [alpha, beta1, beta2, eps];
+
+    return &u.update;
+}
+
+/**
+    Weight matrices (rank two and more, as their first dimension against the others) move along their momentum's
+    orthogonalised form, all other parameters as $(D sgd) moves them with $(D restRate) and $(D momentumRate).  No
+    counterpart in $(D dopt.online).
+*/
+Updater muon(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
+    Operation learningRate = float32([], [0.02f]), Operation momentumRate = float32([], [0.95f]), bool nesterov = true,
+    Operation decay = float32([], [0.0f]), Operation restRate = float32([], [0.01f]))
+{
+    auto u = new FusedUpdater(Rule.muon, outputs, wrt, projs);
+    u.mHyper = [learningRate, momentumRate, decay, restRate];
+    u.mNesterov = nesterov;
 
     return &u.update;
 }

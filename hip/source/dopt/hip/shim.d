@@ -47,6 +47,15 @@ enum
     DOPT_HIP_TINY_MATVEC = 5,
 }
 
+alias dopt_hip_activation = int;
+enum
+{
+    DOPT_HIP_ACT_NONE = 0,
+    DOPT_HIP_ACT_RELU = 1,
+    DOPT_HIP_ACT_GELU = 2,
+    DOPT_HIP_ACT_SILU = 3,
+}
+
 struct dopt_hip_tiny_node
 {
     int kind;
@@ -100,6 +109,15 @@ struct dopt_hip_tensor_ref
     float* vhat;
     size_t n;
     int skip_w;
+}
+
+struct dopt_hip_matrix_ref
+{
+    float* w;
+    const(float)* g;
+    float* m;
+    size_t rows;
+    size_t cols;
 }
 
 int dopt_hip_init(int device);
@@ -186,11 +204,18 @@ int dopt_hip_bn_grad_pool(size_t N, size_t C, size_t H, size_t W, const(float)* 
 int dopt_hip_bn_grad_side(size_t N, size_t C, size_t H, size_t W, const(float)* dy, const(dopt_hip_split_sum)* dy_open, int keep_dy, const(float)* dpooled, const(dopt_hip_split_sum)* dpooled_open, const(float)* y, const(float)* x, const(float)* scale, float* packed, float* dx_sum, const(dopt_hip_split_sum)* side);
 int dopt_hip_bn_wait_limit(uint polls);
 int dopt_hip_bn_infer(size_t N, size_t C, size_t inner, const(float)* x, const(float)* scale, const(float)* bias, const(float)* mean, const(float)* var, float* y);
+int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int channels_last, float eps, int act, const(float)* x, const(float)* scale, const(float)* bias, float* packed);
+int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, int channels_last, int act, const(float)* dy, const(float)* x, const(float)* scale, const(float)* bias, const(float)* stats, float* packed);
+int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const(float)* x, const(float)* w, const(float)* bias, const(float)* residual, float* y, float* pre);
+int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const(float)* dy, const(float)* pre, const(float)* x, const(float)* w, float* dx, float* dw, float* dbias);
 int dopt_hip_optim_create(int ntensors, const(dopt_hip_tensor_ref)* refs, void** handle);
 int dopt_hip_optim_destroy(void* handle);
 int dopt_hip_sgd_step(void* handle, float lr, float mu, int nesterov);
 int dopt_hip_adam_step(void* handle, float alpha, float beta1, float beta2, float eps, float* b1, float* b2);
 int dopt_hip_amsgrad_step(void* handle, float alpha, float beta1, float beta2, float eps, float* b1, float* b2);
+int dopt_hip_muon_create(int nmatrices, const(dopt_hip_matrix_ref)* refs, void** handle);
+int dopt_hip_muon_destroy(void* handle);
+int dopt_hip_muon_step(void* handle, float lr, float mu, int nesterov, float decay, int iterations);
 
 // ---- include/dopt_hip_plan.h
 enum

@@ -511,6 +511,41 @@ int dopt_hip_bn_infer(size_t N, size_t C, size_t inner, const float *x, const fl
                       const float *bias, const float *mean, const float *var, float *y);
 
 /* ---------------------------------------------------------------------------------------
+ * Layers that do not depend on the batch: group norm with an activation, and the dense layer
+ * with its activation and residual.  No counterpart in the reference, which has batch norm
+ * (cudnn7.d:547-654) and relu (cudnn7.d:433) and writes a dense layer as separate operations
+ * (nnet/layers/dense.d:107,143).
+ * ------------------------------------------------------------------------------------- */
+
+/* z; max(z, 0), NaN kept; z Phi(z) with the normal distribution function Phi; z / (1 + exp(-z)) */
+typedef enum {
+    DOPT_HIP_ACT_NONE = 0,
+    DOPT_HIP_ACT_RELU = 1,
+    DOPT_HIP_ACT_GELU = 2,
+    DOPT_HIP_ACT_SILU = 3
+} dopt_hip_activation;
+
+/* y = act((x - mean) * rstd * scale[c] + bias[c]) with the mean and rstd = 1 / sqrt(variance + eps) of each sample's `groups`
+   groups of C / groups neighbouring channels (biased variance).  x is [N, C, inner], or [N, inner, C] when channels_last != 0.
+   packed = [ y (N*C*inner) | mean (N*groups) | rstd (N*groups) ], y laid out as x; it may not overlap an operand. */
+int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int channels_last, float eps, int act,
+                        const float *x, const float *scale, const float *bias, float *packed);
+/* The gradients: packed = [ dx (N*C*inner) | dscale (C) | dbias (C) ].  stats = [ mean | rstd ] as the forward pass left them (the
+   tail of its packed result).  dx may not overlap an operand. */
+int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, int channels_last, int act, const float *dy,
+                             const float *x, const float *scale, const float *bias, const float *stats, float *packed);
+
+/* pre = x * w^T + bias, y = act(pre) + residual: x [M,K], w [N,K] as nnet/layers/dense.d stores it, bias [N], residual [M,N].
+   bias, residual and pre may be null; a training step keeps pre, which the gradient reads (act none needs none).  y and pre may
+   overlap neither each other nor an operand. */
+int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, const float *w, const float *bias,
+                       const float *residual, float *y, float *pre);
+/* With dz = dy * act'(pre): dx = dz * w [M,K], dw = dz^T * x [N,K], dbias = column sums of dz [N]; the residual's gradient is dy.
+   Any of the three results may be null, and w (x) with dx (dw); pre may be null for act none. */
+int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *dy, const float *pre, const float *x,
+                            const float *w, float *dx, float *dw, float *dbias);
+
+/* ---------------------------------------------------------------------------------------
  * Fused multi-tensor optimizer updates.  The reference has no such kernels: dopt.online
  * builds each rule as a graph of pointwise ops with GEMM broadcasts
  * (online/source/dopt/online/{sgd,adam,amsgrad}.d).  These kernels restate those graphs with
@@ -540,6 +575,24 @@ int dopt_hip_adam_step(void *handle, float alpha, float beta1, float beta2, floa
 /* online/amsgrad.d:52-69: ADAM's m', v', w' (w' uses v', as the reference does) plus
    vhat' = max(vhat, OLD v). */
 int dopt_hip_amsgrad_step(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2);
+
+/* A weight as a matrix [rows, cols] (a filter [K,C,R,S] is [K, C*R*S]). */
+typedef struct {
+    float *w;        /* in place */
+    const float *g;  /* gradient */
+    float *m;        /* momentum, in place */
+    size_t rows, cols;
+} dopt_hip_matrix_ref;
+
+/* The update that orthogonalises a matrix' momentum (no counterpart in the reference, whose rules are elementwise):
+     m' = mu m + g,  u = nesterov ? g + mu m' : m',  X = u / (|u| + 1e-7), |u| the 2-norm of all its values,
+     `iterations` times (five as a rule), on the side of fewer rows:  A = X X^T,  X = 3.4445 X + (-4.7750 A + 2.0315 A A) X,
+     w' = (1 - lr decay) w - lr sqrt(max(1, rows / cols)) X
+   for all matrices of the handle at once.  The handle keeps the addresses and the scratch memory that the step needs; no w or m
+   may overlap another operand of the set.  The shorter side of a matrix may have up to 16384 values. */
+int dopt_hip_muon_create(int nmatrices, const dopt_hip_matrix_ref *refs, void **handle);
+int dopt_hip_muon_destroy(void *handle);
+int dopt_hip_muon_step(void *handle, float lr, float mu, int nesterov, float decay, int iterations);
 
 #ifdef __cplusplus
 }
