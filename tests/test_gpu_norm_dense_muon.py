@@ -313,6 +313,13 @@ def test_muon(shapes, iterations):
     _run_muon(shapes, iterations, seed=len(shapes) + iterations)
 
 
+@pytest.mark.parametrize("iterations", [1, 2, 3, 5])
+def test_muon_of_many_matrices(iterations):
+    """More tiles than compute units, of matrices of many sizes; each moves as it does alone."""
+    shapes = [(64, 27), (64, 576), (128, 576), (256, 1152), (256, 2304), (512, 600), (512, 512), (10, 512)] + [(64, 130)] * 200 + [(200, 130)] * 20
+    _run_muon(shapes, iterations, seed=iterations)
+
+
 @pytest.mark.parametrize("kind", ["plain", "weak"])
 @pytest.mark.parametrize("nesterov", [False, True])
 def test_muon_momenta_alignment_and_weak_directions(nesterov, kind):
