@@ -24,10 +24,15 @@
 // 2^-14 of fp16 loses bits only against 2^-34 of the largest entry possible.  That is half the matrix work of three bf16 parts,
 // which the products of sgemm.hip need for operands of any size, and a value takes the four bytes that it takes in fp32.
 //
-// Operands lie row by row along the reduction in pieces of eight values: their h parts (16 bytes), then their l parts.  The square
-// matrices are symmetric, so all products are of that form once X is kept both as it is and transposed.
+// Operands run along the reduction: the square matrices are symmetric, and X is kept both as it is and transposed.  They lie in
+// blocks of 32 rows by 16 steps, 2 KB one after the other along a row of blocks; a row of a block is 64 bytes, h and l parts of eight
+// values (16 bytes each) and of the next eight.  So whatever a workgroup brings or stores are whole kilobytes in a line, spread
+// over all channels of the L2: row by row, at a pitch of 2 KB, the rows of a tile met in two channels of sixteen and the products
+// took three times as long.  Inside a row the four pieces lie at place piece ^ (row / 4 mod 4), in memory as in LDS, so that
+// lanes which read the same piece of neighbouring rows touch different banks.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <new>
 #include <vector>
 
@@ -53,8 +58,6 @@ struct Matrix {
     float *w;
     const float *g;
     float *m;
-    char *x[2], *xt[2];           // X and its transpose before and after a group of iterations
-    char *sq[kSquares];           // the square matrices
     float4 *partial;              // sums of parts of A's reduction
     double *parts;                // the momentum's pass: sums of squares
     int rows, cols;               // as w lies
@@ -64,10 +67,17 @@ struct Matrix {
     float wide;                   // sqrt(max(1, rows / cols))
 };
 
+// What a workgroup does, with all that it needs for its loads: looked up in a table of matrices, the addresses came a memory latency
+// later.
 struct Tile {
+    char *sq, *x;          // the square matrices; X, X after a group of iterations, and their transposes
+    int sp, lp;
     int job, i, j, big;    // job < 0: nothing to do
-    int from, to;          // the part of the reduction, in 64 steps
+    int from, to;          // the part of the reduction, in 32 steps
     int slot, parts;       // slot >= 0: where its sums wait for those of the other parts
+    __device__ char *square(int k) const { return sq + (size_t)k * sp * sp * 4; }
+    __device__ char *along(int turn) const { return x + (size_t)turn * sp * lp * 4; }
+    __device__ char *across(int turn) const { return x + (size_t)(2 + turn) * sp * lp * 4; }
 };
 
 struct Step {
@@ -168,6 +178,10 @@ __device__ __forceinline__ void join4(uint2 h, uint2 l, float *v)
     for (int e = 0; e < 4; e++) v[e] = (float)a[e] + (float)b[e];
 }
 
+// Where a row's piece lies in its block, and where the block of (row, step) lies in a matrix of `steps` steps.
+__device__ __forceinline__ int piece_at(int row, int piece) { return (row & 31) * 64 + ((piece ^ ((row >> 2) & 3)) * 16); }
+__device__ __forceinline__ size_t block_at(int row, int step, int steps) { return ((size_t)(row >> 5) * (steps >> 4) + (step >> 4)) * 2048; }
+
 // X = u / (|u| + eps), as it is and transposed, a 64 x 64 tile of w's layout per workgroup; zero outside.
 __global__ __launch_bounds__(kBlock) void muon_scale_k(const Matrix *jobs, const Tile *tiles, Step st)
 {
@@ -198,73 +212,65 @@ __global__ __launch_bounds__(kBlock) void muon_scale_k(const Matrix *jobs, const
     }
     __syncthreads();
     // rows of w's layout are rows of X, or of its transpose
-    char *const along = q.tall ? q.xt[0] : q.x[0], *const across = q.tall ? q.x[0] : q.xt[0];
-    const int along_p = q.tall ? q.sp : q.lp, across_p = q.tall ? q.lp : q.sp;   // values per row
+    char *const along = q.tall ? t.across(0) : t.along(0), *const across = q.tall ? t.along(0) : t.across(0);
+    const int along_p = q.tall ? q.sp : q.lp, across_p = q.tall ? q.lp : q.sp;   // steps of a row
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        const int r = (int)(threadIdx.x >> 3) + 32 * u, c = (int)(threadIdx.x & 7) * 8;
+    for (int u = 0; u < 2; u++) {   // a wavefront stores a block at a time
+        const int r = (int)(threadIdx.x >> 1 & 31) + 32 * u, c = (int)(threadIdx.x >> 6) * 16 + (int)(threadIdx.x & 1) * 8;
         float p[8], o[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             p[e] = tile[r][c + e];
             o[e] = tile[c + e][r];
         }
+        const int piece = 2 * (threadIdx.x & 1), h = piece_at(r, piece), l = piece_at(r, piece + 1);
         uint2 h0, l0, h1, l1;
         split4(p, h0, l0);
         split4(p + 4, h1, l1);
-        char *at = along + ((size_t)(t.i * 64 + r) * along_p + t.j * 64 + c) * 4;
-        *(v4u *)at = v4u{h0.x, h0.y, h1.x, h1.y};
-        *(v4u *)(at + 16) = v4u{l0.x, l0.y, l1.x, l1.y};
+        char *at = along + block_at(t.i * 64 + r, t.j * 64 + c, along_p);
+        *(v4u *)(at + h) = v4u{h0.x, h0.y, h1.x, h1.y};
+        *(v4u *)(at + l) = v4u{l0.x, l0.y, l1.x, l1.y};
         split4(o, h0, l0);
         split4(o + 4, h1, l1);
-        at = across + ((size_t)(t.j * 64 + r) * across_p + t.i * 64 + c) * 4;
-        *(v4u *)at = v4u{h0.x, h0.y, h1.x, h1.y};
-        *(v4u *)(at + 16) = v4u{l0.x, l0.y, l1.x, l1.y};
+        at = across + block_at(t.j * 64 + r, t.i * 64 + c, across_p);
+        *(v4u *)(at + h) = v4u{h0.x, h0.y, h1.x, h1.y};
+        *(v4u *)(at + l) = v4u{l0.x, l0.y, l1.x, l1.y};
     }
 }
 
 enum Product { kGram, kSquare, kApply, kLast };
 
-// Rows of both operands of a tile go from memory to LDS as they lie, sixteen bytes a lane, with no register in between; piece p
-// of a row's 128 or 256 bytes lies at place p ^ (row mod pieces), so that lanes which read the same piece of neighbouring rows
-// touch different banks (the lanes fetch accordingly: inside a row's line the order is theirs to choose).
-constexpr int kStage = 32768;
+// Both operands of a tile go from memory to LDS as they lie, sixteen bytes a lane, with no register in between, in stages of 16 KB:
+// four rows of blocks of 32 steps, or eight of 16.  Five stages and two workgroups share a CU's 160 KB: what is on its way,
+// 128 KB per CU, hides a memory latency of more than a microsecond.
+constexpr int kStage = 16384, kStages = 5;
 
-// 8 KB of rows from `src`, kLine bytes of each: a wavefront's share of a stage.
-template <int kLine>
-__device__ __forceinline__ void stage(const char *src, size_t pitch, int lane, char *lds)
+__device__ __forceinline__ void bring(const char *src, int kilobytes, int lane, char *lds)
 {
-    constexpr int kPieces = kLine / 16, kRows = 64 / kPieces;   // rows per instruction
-    const int row = lane / kPieces, place = lane % kPieces;
 #pragma unroll
-    for (int q = 0; q < 8; q++) {
-        const int piece = place ^ ((q * kRows + row) % kPieces);
-        __builtin_amdgcn_global_load_lds((glb_ptr)(src + (size_t)(q * kRows + row) * pitch + piece * 16), (lds_ptr)(lds + q * 1024), 16, 0, 0);
-    }
+    for (int q = 0; q < kilobytes; q++)
+        __builtin_amdgcn_global_load_lds((glb_ptr)(src + q * 1024 + lane * 16), (lds_ptr)(lds + q * 1024), 16, 0, 0);
 }
 
-template <int kLine>
-__device__ __forceinline__ v8h fragment(const char *lds, int row, int piece)
-{
-    return *(const v8h *)(lds + row * kLine + ((piece ^ (row % (kLine / 16))) * 16));
-}
+__device__ __forceinline__ v8h fragment(const char *block, int row, int piece) { return *(const v8h *)(block + piece_at(row, piece)); }
 
-// acc[i][j] += rows 32 i of A times rows 32 j of B over sixteen steps, whose first piece is `piece`.
-template <int kLine>
-__device__ __forceinline__ void multiply(const char *A, const char *B, int arow, int brow, int piece, v16f (&acc)[2][2])
+// acc[i][j] += block i of A times block j of B, `next` bytes apart.
+template <int MI>
+__device__ __forceinline__ void multiply(const char *A, const char *B, int next, int lane, v16f (&acc)[MI][MI])
 {
-    v8h ah[2], al[2], bh[2], bl[2];
+    const int row = lane & 31, piece = 2 * (lane >> 5);
+    v8h ah[MI], al[MI], bh[MI], bl[MI];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        ah[i] = fragment<kLine>(A, arow + 32 * i, piece);
-        al[i] = fragment<kLine>(A, arow + 32 * i, piece + 1);
-        bh[i] = fragment<kLine>(B, brow + 32 * i, piece);
-        bl[i] = fragment<kLine>(B, brow + 32 * i, piece + 1);
+    for (int i = 0; i < MI; i++) {
+        ah[i] = fragment(A + next * i, row, piece);
+        al[i] = fragment(A + next * i, row, piece + 1);
+        bh[i] = fragment(B + next * i, row, piece);
+        bl[i] = fragment(B + next * i, row, piece + 1);
     }
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < MI; i++)
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
+        for (int j = 0; j < MI; j++) {
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
@@ -272,7 +278,7 @@ __device__ __forceinline__ void multiply(const char *A, const char *B, int arow,
 }
 
 // Between reads and writes of the same LDS by different wavefronts.  The empty statement keeps the reads in front of the barrier: without
-// it the compiler moved those of `red` below, which ended in a branch behind the barrier, into that branch.
+// it the compiler moved reads whose values were used in a branch behind the barrier into that branch.
 __device__ __forceinline__ void meet()
 {
     asm volatile("" ::: "memory");
@@ -280,33 +286,32 @@ __device__ __forceinline__ void meet()
 }
 
 // Stage k of `steps` is in LDS, for everyone, and the stage before it has been read by everyone.  Each wavefront waits for its own
-// loads (eight a stage, of which the stages behind k may be under way) and meets the others; lgkmcnt: its fragments have left
-// the stage that is filled next.
-template <int kStages>
+// loads (four a stage, of which up to three stages behind k may be under way) and meets the others; lgkmcnt: its fragments have
+// left the stage that is filled next.
 __device__ __forceinline__ void arrive(int k, int steps)
 {
-    const int behind = min(steps - 1 - k, kStages - 2);
-    if (behind >= 2) asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
-    else if (behind == 1) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    const int behind = steps - 1 - k;
+    static_assert(kStages == 5, "three stages may be under way");
+    if (behind >= 3) asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)" ::: "memory");
+    else if (behind == 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    else if (behind == 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
-// f(stage in LDS) for each of `steps` stages, kStages - 1 of which are on their way ahead.
-template <int kLine, int kStages, class F>
-__device__ __forceinline__ void pipeline(const char *src, size_t pitch, int lane, int w, char *lds, int steps, F &&f)
+// multiply_stage(stage in LDS) for each of `steps` stages, kStages - 1 of which are on their way ahead: bring_stage(k, stage in LDS).
+template <class B, class F>
+__device__ __forceinline__ void pipeline(char *lds, int steps, B &&bring_stage, F &&multiply_stage)
 {
-    static_assert(kStages >= 2 && kStages <= 4, "arrive() counts up to two stages ahead");
-    char *const mine = lds + w * (kStage / 4);
 #pragma unroll
     for (int k = 0; k < kStages - 1; k++)
-        if (k < steps) stage<kLine>(src + (size_t)k * kLine, pitch, lane, mine + k * kStage);
+        if (k < steps) bring_stage(k, lds + k * kStage);
     int at = 0, fill = kStages - 1;
     for (int k = 0; k < steps; k++) {
-        arrive<kStages>(k, steps);
-        if (k + kStages - 1 < steps) stage<kLine>(src + (size_t)(k + kStages - 1) * kLine, pitch, lane, mine + fill * kStage);
-        f(lds + at * kStage);
+        arrive(k, steps);
+        if (k + kStages - 1 < steps) bring_stage(k + kStages - 1, lds + fill * kStage);
+        multiply_stage(lds + at * kStage);
         fill = at;
         at = at + 1 == kStages ? 0 : at + 1;
     }
@@ -330,32 +335,58 @@ __device__ __forceinline__ uint2 transpose4(uint2 v, int lane)
     return make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
 }
 
-// A 32 x 32 tile of parts, 128 bytes a row, that a wavefront puts together in LDS and stores in whole lines (eight bytes a lane
-// straight to memory took four times the requests).  The sixteen-byte pieces of a row lie at place piece ^ (row mod 8).
+// A 32 x 32 tile of parts is two blocks, which a wavefront puts together in LDS as they lie in memory (eight bytes a lane straight
+// to memory took four times the requests).  `row` runs to 32, `piece` along the columns to 8.
 __device__ __forceinline__ void put_part(char *image, int row, int piece, int half, uint2 v)
 {
-    *(uint2 *)(image + row * 128 + ((piece ^ (row & 7)) * 16) + 8 * half) = v;
+    *(uint2 *)(image + (piece >> 2) * 2048 + piece_at(row, piece & 3) + 8 * half) = v;
 }
-__device__ __forceinline__ void store_image(const char *image, char *to, size_t pitch, int lane)
+__device__ __forceinline__ void store_image(const char *image, char *to, int lane)
 {
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const int row = 8 * k + (lane >> 3), place = lane & 7;
-        *(v4u *)(to + row * pitch + ((place ^ (row & 7)) * 16)) = *(const v4u *)(image + row * 128 + place * 16);
-    }
+    for (int k = 0; k < 4; k++) *(v4u *)(to + k * 1024 + lane * 16) = *(const v4u *)(image + k * 1024 + lane * 16);
 }
 
-// The values of c that a lane adds to a square product at the end: asked for before the product.
+// What a lane adds to a 32 x 32 tile of a product at the end, asked for before it is needed: values of a square matrix in their
+// parts, or of w.
 struct Old {
     uint2 h[4], l[4];
 };
-__device__ __forceinline__ void load_old(Old &o, const Matrix &q, int c, int row0, int col0, int lane)
+struct OldW {
+    float v[16];
+};
+__device__ __forceinline__ void load_old(Old &o, const Tile &t, int c, int row0, int col0, int lane)
 {
-    const char *const at = q.sq[c] + (size_t)(col0 + (lane & 31)) * q.sp * 4 + (size_t)row0 * 4 + 8 * (lane >> 5);
+    const char *const at = t.square(c) + block_at(col0, row0, t.sp) + 8 * (lane >> 5);
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-        o.h[g] = *(const uint2 *)(at + 32 * g);
-        o.l[g] = *(const uint2 *)(at + 32 * g + 16);
+        o.h[g] = *(const uint2 *)(at + (g >> 1) * 2048 + piece_at(lane, 2 * (g & 1)));
+        o.l[g] = *(const uint2 *)(at + (g >> 1) * 2048 + piece_at(lane, 2 * (g & 1) + 1));
+    }
+}
+
+// Value v of a lane's tile in w, or null outside.
+__device__ __forceinline__ float *place_in_w(const Matrix &q, int v, int row0, int col0, int lane)
+{
+    const int r = row0 + acc_row(v, lane), c = col0 + (lane & 31);
+    if (r >= q.s || c >= q.l) return nullptr;
+    return q.w + (q.tall ? (size_t)c * q.s + r : (size_t)r * q.l + c);
+}
+__device__ __forceinline__ void load_w(OldW &o, const Matrix &q, int row0, int col0, int lane)
+{
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+        const float *const w = place_in_w(q, v, row0, col0, lane);
+        o.v[v] = w ? *w : 0.0f;
+    }
+}
+__device__ __forceinline__ void update_w(const Matrix &q, const Step &st, float alpha, const v16f &acc, const OldW &o, int row0, int col0, int lane)
+{
+    const float by = st.by * q.wide * alpha;
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+        float *const w = place_in_w(q, v, row0, col0, lane);
+        if (w) *w = st.keep * o.v[v] - by * acc[v];
     }
 }
 
@@ -363,27 +394,12 @@ __device__ __forceinline__ void load_old(Old &o, const Matrix &q, int c, int row
 // Values are stored row by row along the columns of the transpose ("across": four neighbouring values of the lane) and, exchanged
 // between four lanes, along the rows.  `images`: 8 KB of LDS of the wavefront's own.
 template <int kProduct>
-__device__ __forceinline__ void finish(const Matrix &q, const Step &st, const SquareOp &op, int turn, const v16f &acc, const Old &old, int row0,
-                                       int col0, int lane, char *images)
+__device__ __forceinline__ void finish(const Tile &t, const SquareOp &op, int turn, const v16f &acc, const Old &old, int row0, int col0, int lane,
+                                       char *images)
 {
     constexpr bool kSq = kProduct == kGram || kProduct == kSquare;
     if (kSq && row0 < col0) return;   // the other half of a tile on the diagonal stores this one
     const int c = lane & 31, col = col0 + c, half = lane >> 5;
-    if (kProduct == kLast) {
-        const float by = st.by * q.wide * op.alpha;
-        if (col >= q.l) return;
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int r = row0 + 8 * g + 4 * half + e;
-                if (r < q.s) {
-                    float *const w = q.w + (q.tall ? (size_t)col * q.s + r : (size_t)r * q.l + col);
-                    *w = st.keep * *w - by * acc[4 * g + e];
-                }
-            }
-        return;
-    }
 #pragma unroll
     for (int g = 0; g < 4; g++) {
         const int r = 8 * g + 4 * half;
@@ -403,10 +419,9 @@ __device__ __forceinline__ void finish(const Matrix &q, const Step &st, const Sq
         put_part(images + 4096, r + (lane & 3), 2 * (c >> 3), (c >> 2) & 1, transpose4(h, lane));
         put_part(images + 4096, r + (lane & 3), 2 * (c >> 3) + 1, (c >> 2) & 1, transpose4(l, lane));
     }
-    char *const along = kSq ? q.sq[op.d] : q.x[turn ^ 1], *const across = kSq ? q.sq[op.d] : q.xt[turn ^ 1];
-    const size_t along_p = (size_t)(kSq ? q.sp : q.lp) * 4, across_p = (size_t)q.sp * 4;   // bytes per row
-    store_image(images, across + (size_t)col0 * across_p + (size_t)row0 * 4, across_p, lane);
-    if (!kSq || row0 != col0) store_image(images + 4096, along + (size_t)row0 * along_p + (size_t)col0 * 4, along_p, lane);
+    char *const along = kSq ? t.square(op.d) : t.along(turn ^ 1), *const across = kSq ? t.square(op.d) : t.across(turn ^ 1);
+    store_image(images, across + block_at(col0, row0, t.sp), lane);
+    if (!kSq || row0 != col0) store_image(images + 4096, along + block_at(row0, col0, kSq ? t.sp : t.lp), lane);
 }
 
 // The sums of a 32 x 32 tile as four quads per lane.
@@ -419,79 +434,84 @@ __device__ __forceinline__ void set_quad(v16f &a, int g, float4 v)
     a[4 * g + 3] = v.w;
 }
 
-// Big tiles: 128 x 128, four wavefronts of 64 x 64 each, 32 steps a stage.  Small ones: 64 x 64, each of four wavefronts multiplies
-// the whole tile over its quarter of a stage's 64 steps, which takes half of what four tiles of 32 x 32 would read from LDS; their
-// sums meet in LDS, in the wavefronts' order.
-template <int kProduct, int kStages>
-__global__ __launch_bounds__(kBlock, kStages > 2 ? 1 : 2) void muon_product_k(const Matrix *jobs, const Tile *tiles, Step st, SquareOps ops, int turn)
+// Big tiles are 128 x 128, 64 x 64 for each of four wavefronts, small ones 64 x 64.
+template <int kProduct>
+__global__ __launch_bounds__(kBlock, 2) void muon_product_k(const Matrix *jobs, const Tile *tiles, Step st, SquareOps ops, int turn)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const Tile t = tiles[blockIdx.x];
     if (t.job < 0) return;
     const SquareOp op = ops.op[blockIdx.y];
     const Matrix &q = jobs[t.job];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), l32 = lane & 31, kh = lane >> 5;
-    const char *const left = kProduct == kGram ? q.x[turn] : q.sq[op.l];
-    const char *const right = kProduct == kGram ? q.x[turn] : kProduct == kSquare ? q.sq[op.r] : q.xt[turn];
-    const size_t pitch = (size_t)(kProduct == kGram ? q.lp : q.sp) * 4;   // of both
-    const int side = t.big ? 128 : 64;
-    // the first two wavefronts bring the left operand's rows, the others the right one's
-    const char *const src = (w < 2 ? left + (size_t)(t.i * side + w * (side / 2)) * pitch : right + (size_t)(t.j * side + (w - 2) * (side / 2)) * pitch) +
-                            (size_t)t.from * 256;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const char *const left = kProduct == kGram ? t.along(turn) : t.square(op.l);
+    const char *const right = kProduct == kGram ? t.along(turn) : kProduct == kSquare ? t.square(op.r) : t.across(turn);
+    const int steps = kProduct == kGram ? t.lp : t.sp;   // of a row of both
+    const size_t row_of_blocks = (size_t)steps * 128;
     char *const images = lds + w * 8192;
-    v16f acc[2][2];
-    zero_acc(acc);
-    if (t.big) {
+    if (t.big) {   // eight rows of blocks, two of them a wavefront's to bring; 16 steps a stage
         const int r0 = t.i * 128 + (w >> 1) * 64, c0 = t.j * 128 + (w & 1) * 64;
-        pipeline<128, kStages>(src, pitch, lane, w, lds, 2 * (t.to - t.from), [&](const char *now) {
+        const char *const src = (w < 2 ? left + (size_t)(t.i * 4 + 2 * w) * row_of_blocks : right + (size_t)(t.j * 4 + 2 * w - 4) * row_of_blocks) +
+                                (size_t)t.from * 4096;
+        v16f acc[2][2];
+        zero_acc(acc);
+        pipeline(
+            lds, 2 * (t.to - t.from),
+            [&](int k, char *to) {
+                bring(src + (size_t)k * 2048, 2, lane, to + w * 4096);
+                bring(src + row_of_blocks + (size_t)k * 2048, 2, lane, to + w * 4096 + 2048);
+            },
+            [&](const char *now) { multiply<2>(now + (w >> 1) * 4096, now + kStage / 2 + (w & 1) * 4096, 2048, lane, acc); });
+        if constexpr (kProduct == kLast) {
+            OldW old[2][2];
 #pragma unroll
-            for (int s = 0; s < 2; s++) multiply<128>(now, now + kStage / 2, (w >> 1) * 64 + l32, (w & 1) * 64 + l32, 4 * s + 2 * kh, acc);
-        });
+            for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+                for (int j = 0; j < 2; j++) load_w(old[i][j], q, r0 + 32 * i, c0 + 32 * j, lane);
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                Old old;
-                if (kProduct == kSquare) load_old(old, q, op.c, r0 + 32 * i, c0 + 32 * j, lane);
-                finish<kProduct>(q, st, op, turn, acc[i][j], old, r0 + 32 * i, c0 + 32 * j, lane, images);
-            }
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) update_w(q, st, op.alpha, acc[i][j], old[i][j], r0 + 32 * i, c0 + 32 * j, lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    Old old;
+                    if (kProduct == kSquare) load_old(old, t, op.c, r0 + 32 * i, c0 + 32 * j, lane);
+                    finish<kProduct>(t, op, turn, acc[i][j], old, r0 + 32 * i, c0 + 32 * j, lane, images);
+                }
+        }
         return;
     }
     const int row0 = t.i * 64 + (w >> 1) * 32, col0 = t.j * 64 + (w & 1) * 32;
     Old old;
-    if (kProduct == kSquare) load_old(old, q, op.c, row0, col0, lane);
-    pipeline<256, kStages>(src, pitch, lane, w, lds, t.to - t.from,
-                           [&](const char *now) { multiply<256>(now, now + kStage / 2, l32, l32, 4 * w + 2 * kh, acc); });
-    float4 *const red = (float4 *)lds;   // [wavefront][tile][quad of values][lane]
+    OldW old_w;
+    if constexpr (kProduct == kSquare) load_old(old, t, op.c, row0, col0, lane);
+    if constexpr (kProduct == kLast) load_w(old_w, q, row0, col0, lane);
+    // four rows of blocks, one for each wavefront to bring; 32 steps a stage
+    const char *const src = (w < 2 ? left + (size_t)(t.i * 2 + w) * row_of_blocks : right + (size_t)(t.j * 2 + w - 2) * row_of_blocks) +
+                            (size_t)t.from * 4096;
+    v16f acc[1][1];
+    zero_acc(acc);
+    pipeline(
+        lds, t.to - t.from, [&](int k, char *to) { bring(src + (size_t)k * 4096, 4, lane, to + w * 4096); },
+        [&](const char *now) {
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) red[((w * 4 + i * 2 + j) * 4 + g) * 64 + lane] = quad_of(acc[i][j], g);
-    meet();
-    v16f sum;
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-        float4 v = red[(w * 4 + g) * 64 + lane];
-#pragma unroll
-        for (int o = 1; o < 4; o++) {
-            const float4 p = red[((o * 4 + w) * 4 + g) * 64 + lane];
-            v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
-        }
-        set_quad(sum, g, v);
-    }
+            for (int s = 0; s < 2; s++)
+                multiply<1>(now + (w >> 1) * 4096 + s * 2048, now + kStage / 2 + (w & 1) * 4096 + s * 2048, 0, lane, acc);
+        });
     if (kProduct == kGram && t.slot >= 0) {
 #pragma unroll
-        for (int g = 0; g < 4; g++) q.partial[(((size_t)t.slot * 4 + w) * 4 + g) * 64 + lane] = quad_of(sum, g);
+        for (int g = 0; g < 4; g++) q.partial[(((size_t)t.slot * 4 + w) * 4 + g) * 64 + lane] = quad_of(acc[0][0], g);
         return;
     }
-    meet();   // the sums have been read
-    finish<kProduct>(q, st, op, turn, sum, old, row0, col0, lane, images);
+    if constexpr (kProduct == kLast) update_w(q, st, op.alpha, acc[0][0], old_w, row0, col0, lane);
+    else finish<kProduct>(t, op, turn, acc[0][0], old, row0, col0, lane, images);
 }
 
 // Adds the parts of a tile of A, in their order.
-__global__ __launch_bounds__(kBlock) void muon_meet_k(const Matrix *jobs, const Tile *tiles, Step st, SquareOps ops)
+__global__ __launch_bounds__(kBlock) void muon_meet_k(const Matrix *jobs, const Tile *tiles, SquareOps ops)
 {
     __shared__ __attribute__((aligned(16))) char images[4 * 8192];
     const Tile t = tiles[blockIdx.x];
@@ -507,7 +527,7 @@ __global__ __launch_bounds__(kBlock) void muon_meet_k(const Matrix *jobs, const 
         }
         set_quad(sum, g, v);
     }
-    finish<kGram>(q, st, ops.op[0], 0, sum, Old{}, t.i * 64 + (w >> 1) * 32, t.j * 64 + (w & 1) * 32, lane, images + w * 8192);
+    finish<kGram>(t, ops.op[0], 0, sum, Old{}, t.i * 64 + (w >> 1) * 32, t.j * 64 + (w & 1) * 32, lane, images + w * 8192);
 }
 
 // No iterations: w moves along X itself.
@@ -518,9 +538,9 @@ __global__ __launch_bounds__(kBlock) void muon_plain_k(const Matrix *jobs, const
     const size_t n = (size_t)q.rows * q.cols, from = (size_t)t.i * kChunk, to = min(from + kChunk, n);
     const float by = st.by * q.wide * (1.0f / kUp);
     for (size_t i = from + threadIdx.x; i < to; i += kBlock) {
-        const size_t r = i / q.cols, c = i % q.cols;
-        const char *const at = (q.tall ? q.xt[0] : q.x[0]) + (r * (q.tall ? q.sp : q.lp) + c / 8 * 8) * 4 + c % 8 * 2;
-        const float x = (float)*(const _Float16 *)at + (float)*(const _Float16 *)(at + 16);
+        const int r = (int)(i / q.cols), c = (int)(i % q.cols), piece = 2 * (c >> 3 & 1);
+        const char *const at = (q.tall ? t.across(0) : t.along(0)) + block_at(r, c, q.tall ? q.sp : q.lp) + 2 * (c & 7);
+        const float x = (float)*(const _Float16 *)(at + piece_at(r, piece)) + (float)*(const _Float16 *)(at + piece_at(r, piece + 1));
         q.w[i] = st.keep * q.w[i] - by * x;
     }
 }
@@ -542,12 +562,12 @@ std::vector<Tile> deal(const std::vector<Tile> &tiles, const std::vector<double>
         most = std::max(most, x.size());
     }
     std::vector<Tile> out;
+    Tile nothing{};
+    nothing.job = -1;
     for (size_t k = 0; k < most; k++)
-        for (auto &x : xcd) out.push_back(k < x.size() ? tiles[x[k]] : Tile{-1, 0, 0, 0, 0, 0, -1, 0});
+        for (auto &x : xcd) out.push_back(k < x.size() ? tiles[x[k]] : nothing);
     return out;
 }
-
-int put(const void *host, size_t bytes, void *to) { return bytes ? dopt_hip_copy_h2d(to, host, bytes) : DOPT_HIP_OK; }
 
 void release(Handle *h)
 {
@@ -557,13 +577,10 @@ void release(Handle *h)
 
 int build(Handle *h)
 {
-    std::vector<Tile> chunks, scales, grams, meets, squares, wides;
-    std::vector<double> cgram, csq, cwide;
     size_t bytes = 0;
     auto take = [&](size_t n) { const size_t at = bytes; bytes += ceil_div(n, (size_t)256) * 256; return at; };
-    std::vector<size_t> at;
-    constexpr int kBuffers = 4 + kSquares + 2;
-    size_t all = 0;   // 64-step stages of all tiles of A
+    std::vector<size_t> x_at, sq_at, partial_at, parts_at;
+    size_t all = 0;   // 32-step stages of all tiles of A
     for (Matrix &q : h->jobs) {
         q.tall = q.rows > q.cols;
         q.s = std::min(q.rows, q.cols);
@@ -574,39 +591,55 @@ int build(Handle *h)
         q.wide = std::sqrt(std::max(1.0f, (float)q.rows / (float)q.cols));
         q.nparts = (int)ceil_div((size_t)q.rows * q.cols, kChunk);
         const size_t t = q.sp / 64;
-        all += t * (t + 1) / 2 * (q.lp / 64);
+        all += t * (t + 1) / 2 * (q.lp / 32);
     }
     // A's reduction is cut where its tiles alone would not give every CU its share
-    const size_t part = std::max((size_t)16, ceil_div(all * 2, (size_t)num_cus() * 3));
-    for (size_t k = 0; k < h->jobs.size(); k++) {
-        Matrix &q = h->jobs[k];
-        const int job = (int)k, side = q.s <= 64 ? 64 : 128, big = side == 128, deep = q.lp / 64;
-        const int rp = q.tall ? q.lp : q.sp, cp = q.tall ? q.sp : q.lp, cuts = (int)ceil_div((size_t)deep, part);
-        for (int i = 0; i < q.nparts; i++) chunks.push_back(Tile{job, i, 0, 0, 0, 0, -1, 0});
+    const size_t part = std::max((size_t)32, ceil_div(all * 2, (size_t)num_cus() * 3));
+    auto cuts_of = [&](const Matrix &q) { return (int)ceil_div((size_t)q.lp / 32, part); };
+    for (const Matrix &q : h->jobs) {
+        const size_t t = q.sp / 64, cuts = cuts_of(q);
+        x_at.push_back(take((size_t)q.sp * q.lp * 4 * 4));
+        sq_at.push_back(take((size_t)q.sp * q.sp * 4 * kSquares));
+        partial_at.push_back(take(cuts > 1 ? cuts * t * (t + 1) / 2 * 64 * 64 * sizeof(float) : 0));
+        parts_at.push_back(take((size_t)q.nparts * sizeof(double)));
+    }
+    const size_t tables_at = bytes;
+    std::vector<Tile> chunks, scales, grams, meets, squares, wides;
+    std::vector<double> cgram, csq, cwide;
+    for (size_t k = 0; k < h->jobs.size(); k++) {   // (addresses are offsets until the memory is there)
+        const Matrix &q = h->jobs[k];
+        const int side = q.s <= 64 ? 64 : 128, deep = q.lp / 32, cuts = cuts_of(q);
+        const int rp = q.tall ? q.lp : q.sp, cp = q.tall ? q.sp : q.lp;
+        Tile t{(char *)sq_at[k], (char *)x_at[k], q.sp, q.lp, (int)k, 0, 0, 0, 0, q.sp / 32, -1, 0};
+        auto at = [&](int i, int j) { t.i = i; t.j = j; return t; };
+        for (int i = 0; i < q.nparts; i++) chunks.push_back(at(i, 0));
         for (int i = 0; i < rp / 64; i++)
-            for (int j = 0; j < cp / 64; j++) scales.push_back(Tile{job, i, j, 0, 0, 0, -1, 0});
+            for (int j = 0; j < cp / 64; j++) scales.push_back(at(i, j));
         int slots = 0;
         for (int i = 0; i < q.sp / 64; i++)
             for (int j = 0; j <= i; j++) {
-                squares.push_back(Tile{job, i, j, 0, 0, q.sp / 64, -1, 0});
-                csq.push_back((double)q.sp + 512);
-                if (cuts > 1) meets.push_back(Tile{job, i, j, 0, 0, 0, slots, cuts});
+                squares.push_back(at(i, j));
+                csq.push_back((double)q.sp + 256);
+                Tile g = at(i, j);
+                if (cuts > 1) {
+                    g.slot = slots;
+                    g.parts = cuts;
+                    meets.push_back(g);
+                }
                 for (int c = 0; c < cuts; c++) {
-                    const int from = deep * c / cuts, to = deep * (c + 1) / cuts;
-                    grams.push_back(Tile{job, i, j, 0, from, to, cuts > 1 ? slots++ : -1, 0});
-                    cgram.push_back((double)(to - from) + 8);
+                    g.from = (int)((size_t)deep * c / cuts);
+                    g.to = (int)((size_t)deep * (c + 1) / cuts);
+                    if (cuts > 1) g.slot = slots++;
+                    grams.push_back(g);
+                    cgram.push_back((double)(g.to - g.from) + 8);
                 }
             }
+        t.big = side == 128;
         for (int j = 0; j < q.lp / side; j++)
             for (int i = 0; i < q.sp / side; i++) {
-                wides.push_back(Tile{job, i, j, big, 0, q.sp / 64, -1, 0});
+                wides.push_back(at(i, j));
                 cwide.push_back((double)q.sp + 256);
             }
-        const size_t x = (size_t)q.sp * q.lp * 4, a = (size_t)q.sp * q.sp * 4;
-        for (int i = 0; i < 4; i++) at.push_back(take(x));
-        for (int i = 0; i < kSquares; i++) at.push_back(take(a));
-        at.push_back(take((size_t)slots * 64 * 64 * sizeof(float)));
-        at.push_back(take((size_t)q.nparts * sizeof(double)));
     }
     grams = deal(grams, cgram);
     squares = deal(squares, csq);
@@ -615,52 +648,43 @@ int build(Handle *h)
         std::vector<Tile> *tiles;
         Tile **device;
         unsigned *n;
-    } tables[] = {{&chunks, &h->chunks, &h->nchunks}, {&scales, &h->scales, &h->nscales},    {&grams, &h->grams, &h->ngrams},
-                  {&meets, &h->meets, &h->nmeets},    {&squares, &h->squares, &h->nsquares}, {&wides, &h->wides, &h->nwides}};
-    std::vector<size_t> table_at;
-    for (Table &t : tables) table_at.push_back(take(t.tiles->size() * sizeof(Tile)));
+        size_t at;
+    } tables[] = {{&chunks, &h->chunks, &h->nchunks, 0}, {&scales, &h->scales, &h->nscales, 0},    {&grams, &h->grams, &h->ngrams, 0},
+                  {&meets, &h->meets, &h->nmeets, 0},    {&squares, &h->squares, &h->nsquares, 0}, {&wides, &h->wides, &h->nwides, 0}};
+    for (Table &t : tables) t.at = take(t.tiles->size() * sizeof(Tile));
     const size_t jobs_at = take(h->jobs.size() * sizeof(Matrix));
     if (int rc = scratch_alloc(&h->memory, bytes)) return rc;
     char *const base = (char *)h->memory;
     for (size_t k = 0; k < h->jobs.size(); k++) {
-        Matrix &q = h->jobs[k];
-        const size_t *const p = &at[kBuffers * k];
-        for (int i = 0; i < 2; i++) {
-            q.x[i] = base + p[i];
-            q.xt[i] = base + p[2 + i];
-        }
-        for (int i = 0; i < kSquares; i++) q.sq[i] = base + p[4 + i];
-        q.partial = (float4 *)(base + p[4 + kSquares]);
-        q.parts = (double *)(base + p[5 + kSquares]);
+        h->jobs[k].partial = (float4 *)(base + partial_at[k]);
+        h->jobs[k].parts = (double *)(base + parts_at[k]);
     }
-    for (size_t i = 0; i < table_at.size(); i++) {
-        *tables[i].device = (Tile *)(base + table_at[i]);
-        *tables[i].n = (unsigned)tables[i].tiles->size();
-        if (int rc = put(tables[i].tiles->data(), tables[i].tiles->size() * sizeof(Tile), *tables[i].device)) return rc;
+    // the tables and the matrices lie one after the other: one copy
+    std::vector<char> host(bytes - tables_at);
+    for (Table &t : tables) {
+        for (Tile &q : *t.tiles) {
+            q.sq = base + (size_t)q.sq;
+            q.x = base + (size_t)q.x;
+        }
+        *t.device = (Tile *)(base + t.at);
+        *t.n = (unsigned)t.tiles->size();
+        if (!t.tiles->empty()) memcpy(host.data() + (t.at - tables_at), t.tiles->data(), t.tiles->size() * sizeof(Tile));
     }
     h->d_jobs = (Matrix *)(base + jobs_at);
-    return put(h->jobs.data(), h->jobs.size() * sizeof(Matrix), h->d_jobs);
-}
-
-template <int kProduct, int kStages>
-int launch_deep(const Handle *h, dim3 grid, const Tile *tiles, const Step &st, const SquareOps &ops, int turn)
-{
-    static bool raised = false;   // above 64 KB of dynamic LDS a kernel has to be told once
-    if (!raised && kStages > 2)
-        DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)muon_product_k<kProduct, kStages>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           kStages * kStage));
-    raised = true;
-    hipLaunchKernelGGL((muon_product_k<kProduct, kStages>), grid, dim3(kBlock), kStages * kStage, stream(), h->d_jobs, tiles, st, ops, turn);
-    DOPT_LAUNCH_CHECK();
-    return DOPT_HIP_OK;
+    memcpy(host.data() + (jobs_at - tables_at), h->jobs.data(), h->jobs.size() * sizeof(Matrix));
+    return dopt_hip_copy_h2d(base + tables_at, host.data(), host.size());
 }
 
 template <int kProduct>
 int launch(const Handle *h, unsigned blocks, unsigned products, const Tile *tiles, const Step &st, const SquareOps &ops, int turn)
 {
-    const dim3 grid(blocks, products);
-    return blocks * products <= (unsigned)num_cus() ? launch_deep<kProduct, 4>(h, grid, tiles, st, ops, turn)
-                                                    : launch_deep<kProduct, 2>(h, grid, tiles, st, ops, turn);
+    static bool raised = false;   // above 64 KB of dynamic LDS a kernel has to be told once
+    if (!raised)
+        DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)muon_product_k<kProduct>, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStage));
+    raised = true;
+    hipLaunchKernelGGL(muon_product_k<kProduct>, dim3(blocks, products), dim3(kBlock), kStages * kStage, stream(), h->d_jobs, tiles, st, ops, turn);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
 }
 
 // Which of the square matrices hold something that is still read, and the powers of two that they are held times.
@@ -693,7 +717,7 @@ int iterate(const Handle *h, const Step &st, int count, int turn, bool last)
     ops.op[0] = SquareOp{0, 0, a, 0, std::ldexp(1.0f, -kScaleBits), 0.0f, 0.0f};
     if (int rc = launch<kGram>(h, h->ngrams, 1, h->grams, st, ops, turn)) return rc;
     if (h->nmeets) {
-        hipLaunchKernelGGL(muon_meet_k, dim3(h->nmeets), dim3(kBlock), 0, stream(), h->d_jobs, h->meets, st, ops);
+        hipLaunchKernelGGL(muon_meet_k, dim3(h->nmeets), dim3(kBlock), 0, stream(), h->d_jobs, h->meets, ops);
         DOPT_LAUNCH_CHECK();
     }
     for (int k = 0; k < count; k++) {
