@@ -47,6 +47,16 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 using lds_ptr = __attribute__((address_space(3))) void *;
 using glb_ptr = __attribute__((address_space(1))) const void *;
+// Addresses that come out of a table: the compiler does not see that they are global memory's, and a flat access waits for LDS too.
+template <class T>
+using Global = __attribute__((address_space(1))) T *;
+template <class T>
+__device__ __forceinline__ Global<T> global(T *p)
+{
+    return (Global<T>)p;
+}
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
 constexpr size_t kChunk = 8192;   // values per workgroup of the momentum's pass
@@ -64,17 +74,20 @@ struct Matrix {
     int s, l;                     // the shorter and the longer side: X is [s][l]
     int sp, lp;                   // ... in whole tiles
     int nparts, tall;             // tall: X is w transposed
+    int quads;                    // tall, and rows of w are whole 16-byte pieces
     float wide;                   // sqrt(max(1, rows / cols))
 };
+
+enum Kind { kSmall, kMid, kWide };   // 64 x 64, 128 x 128, 128 x 256
 
 // What a workgroup does, with all that it needs for its loads: looked up in a table of matrices, the addresses came a memory latency
 // later.
 struct Tile {
     char *sq, *x;          // the square matrices; X, X after a group of iterations, and their transposes
     int sp, lp;
-    int job, i, j, big;    // job < 0: nothing to do
+    int job, i, j, kind;   // job < 0: nothing to do; kind: the tile's sides
     int from, to;          // the part of the reduction, in 32 steps
-    int slot, parts;       // slot >= 0: where its sums wait for those of the other parts
+    int slot, parts;       // slot >= 0: where its sums wait for those of the other parts, in 16 KB
     __device__ char *square(int k) const { return sq + (size_t)k * sp * sp * 4; }
     __device__ char *along(int turn) const { return x + (size_t)turn * sp * lp * 4; }
     __device__ char *across(int turn) const { return x + (size_t)(2 + turn) * sp * lp * 4; }
@@ -108,29 +121,29 @@ __device__ __forceinline__ float step_value(float g, float m, const Step &st) { 
 __global__ __launch_bounds__(kBlock) void muon_momentum_k(const Matrix *jobs, const Tile *chunks, Step st)
 {
     const Tile t = chunks[blockIdx.x];
-    const Matrix &q = jobs[t.job];
+    const Matrix q = jobs[t.job];
     const size_t n = (size_t)q.rows * q.cols, from = (size_t)t.i * kChunk, to = min(from + kChunk, n);
-    const float *const g = q.g;
-    float *const m = q.m;
+    const Global<const float> g = global(q.g);
+    const Global<float> m = global(q.m);
     double s = 0.0;
-    if ((((uintptr_t)g | (uintptr_t)m) & 15) == 0) {
+    if ((((uintptr_t)q.g | (uintptr_t)q.m) & 15) == 0) {
         constexpr int kQuads = kChunk / kBlock / 4;
         const size_t whole = from + (to - from) / 4 * 4;
-        float4 a[kQuads], b[kQuads];
+        v4f a[kQuads], b[kQuads];
 #pragma unroll
         for (int u = 0; u < kQuads; u++) {
             const size_t i = from + ((size_t)u * kBlock + threadIdx.x) * 4;
             if (i < whole) {
-                a[u] = *(const float4 *)(m + i);
-                b[u] = *(const float4 *)(g + i);
+                a[u] = *(Global<const v4f>)(m + i);
+                b[u] = *(Global<const v4f>)(g + i);
             }
         }
 #pragma unroll
         for (int u = 0; u < kQuads; u++) {
             const size_t i = from + ((size_t)u * kBlock + threadIdx.x) * 4;
             if (i < whole) {
-                float4 v = make_float4(st.mu * a[u].x + b[u].x, st.mu * a[u].y + b[u].y, st.mu * a[u].z + b[u].z, st.mu * a[u].w + b[u].w);
-                *(float4 *)(m + i) = v;
+                const v4f v = {st.mu * a[u].x + b[u].x, st.mu * a[u].y + b[u].y, st.mu * a[u].z + b[u].z, st.mu * a[u].w + b[u].w};
+                *(Global<v4f>)(m + i) = v;
                 const double p = step_value(b[u].x, v.x, st), r = step_value(b[u].y, v.y, st), y = step_value(b[u].z, v.z, st),
                              z = step_value(b[u].w, v.w, st);
                 s += (p * p + r * r) + (y * y + z * z);
@@ -155,11 +168,11 @@ __global__ __launch_bounds__(kBlock) void muon_momentum_k(const Matrix *jobs, co
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) q.parts[t.i] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) global(q.parts)[t.i] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // Four values, already times kUp, as their h and l parts.
-__device__ __forceinline__ void split4(const float *v, uint2 &h, uint2 &l)
+__device__ __forceinline__ void split4(const float *v, v2u &h, v2u &l)
 {
     v4h a, b;
 #pragma unroll
@@ -167,11 +180,11 @@ __device__ __forceinline__ void split4(const float *v, uint2 &h, uint2 &l)
         a[e] = (_Float16)v[e];
         b[e] = (_Float16)(v[e] - (float)a[e]);
     }
-    h = __builtin_bit_cast(uint2, a);
-    l = __builtin_bit_cast(uint2, b);
+    h = __builtin_bit_cast(v2u, a);
+    l = __builtin_bit_cast(v2u, b);
 }
 
-__device__ __forceinline__ void join4(uint2 h, uint2 l, float *v)
+__device__ __forceinline__ void join4(v2u h, v2u l, float *v)
 {
     const v4h a = __builtin_bit_cast(v4h, h), b = __builtin_bit_cast(v4h, l);
 #pragma unroll
@@ -188,9 +201,9 @@ __global__ __launch_bounds__(kBlock) void muon_scale_k(const Matrix *jobs, const
     __shared__ double red[kBlock / 64];
     __shared__ float tile[64][65];
     const Tile t = tiles[blockIdx.x];
-    const Matrix &q = jobs[t.job];
+    const Matrix q = jobs[t.job];
     double s = 0.0;
-    for (int i = threadIdx.x; i < q.nparts; i += kBlock) s += q.parts[i];
+    for (int i = threadIdx.x; i < q.nparts; i += kBlock) s += global(q.parts)[i];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -199,7 +212,8 @@ __global__ __launch_bounds__(kBlock) void muon_scale_k(const Matrix *jobs, const
     for (int u = 0; u < 16; u++) {
         const int r = t.i * 64 + (int)(threadIdx.x >> 6) + 4 * u, c = t.j * 64 + (int)(threadIdx.x & 63);
         const size_t at = (size_t)r * q.cols + c;
-        v[u] = r < q.rows && c < q.cols ? step_value(q.g[at], q.m[at], st) : 0.0f;
+        const size_t safe = r < q.rows && c < q.cols ? at : 0;   // (no branch: the loads go out together)
+        v[u] = step_value(global(q.g)[safe], global(q.m)[safe], st);
     }
     __syncthreads();
     const float by = (float)((double)kUp / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)kEps));
@@ -224,26 +238,27 @@ __global__ __launch_bounds__(kBlock) void muon_scale_k(const Matrix *jobs, const
             o[e] = tile[c + e][r];
         }
         const int piece = 2 * (threadIdx.x & 1), h = piece_at(r, piece), l = piece_at(r, piece + 1);
-        uint2 h0, l0, h1, l1;
+        v2u h0, l0, h1, l1;
         split4(p, h0, l0);
         split4(p + 4, h1, l1);
-        char *at = along + block_at(t.i * 64 + r, t.j * 64 + c, along_p);
-        *(v4u *)(at + h) = v4u{h0.x, h0.y, h1.x, h1.y};
-        *(v4u *)(at + l) = v4u{l0.x, l0.y, l1.x, l1.y};
+        Global<char> at = global(along + block_at(t.i * 64 + r, t.j * 64 + c, along_p));
+        *(Global<v4u>)(at + h) = v4u{h0.x, h0.y, h1.x, h1.y};
+        *(Global<v4u>)(at + l) = v4u{l0.x, l0.y, l1.x, l1.y};
         split4(o, h0, l0);
         split4(o + 4, h1, l1);
-        at = across + block_at(t.j * 64 + r, t.i * 64 + c, across_p);
-        *(v4u *)(at + h) = v4u{h0.x, h0.y, h1.x, h1.y};
-        *(v4u *)(at + l) = v4u{l0.x, l0.y, l1.x, l1.y};
+        at = global(across + block_at(t.j * 64 + r, t.i * 64 + c, across_p));
+        *(Global<v4u>)(at + h) = v4u{h0.x, h0.y, h1.x, h1.y};
+        *(Global<v4u>)(at + l) = v4u{l0.x, l0.y, l1.x, l1.y};
     }
 }
 
 enum Product { kGram, kSquare, kApply, kLast };
 
-// Both operands of a tile go from memory to LDS as they lie, sixteen bytes a lane, with no register in between, in stages of 16 KB:
-// four rows of blocks of 32 steps, or eight of 16.  Five stages and two workgroups share a CU's 160 KB: what is on its way,
-// 128 KB per CU, hides a memory latency of more than a microsecond.
-constexpr int kStage = 16384, kStages = 5;
+// Both operands of a tile go from memory to LDS as they lie, sixteen bytes a lane, with no register in between, in stages of 16 or 24 KB:
+// four rows of blocks of 32 steps, eight of 16, or twelve of 16.  Up to five stages and two workgroups share a CU's 160 KB: what
+// is on its way, about 100 KB per CU, hides a memory latency of more than a microsecond.  A CU takes in some 65 GB/s so, which is what
+// bounds small tiles and makes wide ones worth their registers: X of eight [640 x 5760], 1.1 GB in tiles of 128 x 128.
+constexpr int kLds = 81920;
 
 __device__ __forceinline__ void bring(const char *src, int kilobytes, int lane, char *lds)
 {
@@ -254,23 +269,26 @@ __device__ __forceinline__ void bring(const char *src, int kilobytes, int lane, 
 
 __device__ __forceinline__ v8h fragment(const char *block, int row, int piece) { return *(const v8h *)(block + piece_at(row, piece)); }
 
-// acc[i][j] += block i of A times block j of B, `next` bytes apart.
-template <int MI>
-__device__ __forceinline__ void multiply(const char *A, const char *B, int next, int lane, v16f (&acc)[MI][MI])
+// acc[i][j] += block i of A times block j of B.
+template <int MI, int NI>
+__device__ __forceinline__ void multiply(const char *A, const char *B, int lane, v16f (&acc)[MI][NI])
 {
     const int row = lane & 31, piece = 2 * (lane >> 5);
-    v8h ah[MI], al[MI], bh[MI], bl[MI];
+    v8h ah[MI], al[MI], bh[NI], bl[NI];
 #pragma unroll
     for (int i = 0; i < MI; i++) {
-        ah[i] = fragment(A + next * i, row, piece);
-        al[i] = fragment(A + next * i, row, piece + 1);
-        bh[i] = fragment(B + next * i, row, piece);
-        bl[i] = fragment(B + next * i, row, piece + 1);
+        ah[i] = fragment(A + 2048 * i, row, piece);
+        al[i] = fragment(A + 2048 * i, row, piece + 1);
+    }
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+        bh[j] = fragment(B + 2048 * j, row, piece);
+        bl[j] = fragment(B + 2048 * j, row, piece + 1);
     }
 #pragma unroll
     for (int i = 0; i < MI; i++)
 #pragma unroll
-        for (int j = 0; j < MI; j++) {
+        for (int j = 0; j < NI; j++) {
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
@@ -285,31 +303,32 @@ __device__ __forceinline__ void meet()
     __syncthreads();
 }
 
-// Stage k of `steps` is in LDS, for everyone, and the stage before it has been read by everyone.  Each wavefront waits for its own
-// loads (four a stage, of which up to three stages behind k may be under way) and meets the others; lgkmcnt: its fragments have
-// left the stage that is filled next.
-__device__ __forceinline__ void arrive(int k, int steps)
+// The wavefront's fragments have left LDS, and all but the last `kLoads` loads that it has asked for are there.
+template <int kLoads>
+__device__ __forceinline__ void settled()
 {
-    const int behind = steps - 1 - k;
-    static_assert(kStages == 5, "three stages may be under way");
-    if (behind >= 3) asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)" ::: "memory");
-    else if (behind == 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-    else if (behind == 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
 }
 
-// multiply_stage(stage in LDS) for each of `steps` stages, kStages - 1 of which are on their way ahead: bring_stage(k, stage in LDS).
-template <class B, class F>
+// multiply_stage(stage in LDS) for each of `steps` stages, up to kStages - 1 of which are on their way ahead, kLoads loads of a
+// wavefront each: bring_stage(k, stage in LDS).  Once a wavefront's own part of stage k is there it meets the others: then
+// all of it is, and the stage before it has been read by everyone.
+template <int kStages, int kStage, int kLoads, class B, class F>
 __device__ __forceinline__ void pipeline(char *lds, int steps, B &&bring_stage, F &&multiply_stage)
 {
+    static_assert(kStages >= 3 && kStages <= 5 && kStages * kStage <= kLds, "one to three stages may be under way behind the next one");
 #pragma unroll
     for (int k = 0; k < kStages - 1; k++)
         if (k < steps) bring_stage(k, lds + k * kStage);
     int at = 0, fill = kStages - 1;
     for (int k = 0; k < steps; k++) {
-        arrive(k, steps);
+        const int behind = min(steps - 1 - k, kStages - 2);
+        if (behind == 3) settled<3 * kLoads>();
+        else if (behind == 2) settled<2 * kLoads>();
+        else if (behind == 1) settled<kLoads>();
+        else settled<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         if (k + kStages - 1 < steps) bring_stage(k + kStages - 1, lds + fill * kStage);
         multiply_stage(lds + at * kStage);
         fill = at;
@@ -319,7 +338,7 @@ __device__ __forceinline__ void pipeline(char *lds, int steps, B &&bring_stage, 
 }
 
 // Four values in each of four neighbouring lanes: lane b gets value b of each.  `v` holds the values in pairs.
-__device__ __forceinline__ uint2 transpose4(uint2 v, int lane)
+__device__ __forceinline__ v2u transpose4(v2u v, int lane)
 {
     const bool hi = lane & 2, odd = lane & 1;
     unsigned p[4];
@@ -332,63 +351,94 @@ __device__ __forceinline__ uint2 transpose4(uint2 v, int lane)
     }
     DOPT_FROM(0) DOPT_FROM(1) DOPT_FROM(2) DOPT_FROM(3)
 #undef DOPT_FROM
-    return make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
+    return v2u{p[0] | p[1] << 16, p[2] | p[3] << 16};
 }
 
 // A 32 x 32 tile of parts is two blocks, which a wavefront puts together in LDS as they lie in memory (eight bytes a lane straight
 // to memory took four times the requests).  `row` runs to 32, `piece` along the columns to 8.
-__device__ __forceinline__ void put_part(char *image, int row, int piece, int half, uint2 v)
+__device__ __forceinline__ void put_part(char *image, int row, int piece, int half, v2u v)
 {
-    *(uint2 *)(image + (piece >> 2) * 2048 + piece_at(row, piece & 3) + 8 * half) = v;
+    *(v2u *)(image + (piece >> 2) * 2048 + piece_at(row, piece & 3) + 8 * half) = v;
 }
 __device__ __forceinline__ void store_image(const char *image, char *to, int lane)
 {
 #pragma unroll
-    for (int k = 0; k < 4; k++) *(v4u *)(to + k * 1024 + lane * 16) = *(const v4u *)(image + k * 1024 + lane * 16);
+    for (int k = 0; k < 4; k++) *(Global<v4u>)(global(to) + k * 1024 + lane * 16) = *(const v4u *)(image + k * 1024 + lane * 16);
 }
 
-// What a lane adds to a 32 x 32 tile of a product at the end, asked for before it is needed: values of a square matrix in their
-// parts, or of w.
+// What a lane adds to a 32 x 32 tile of a square product at the end, asked for before it is needed.
 struct Old {
-    uint2 h[4], l[4];
-};
-struct OldW {
-    float v[16];
+    v2u h[4], l[4];
 };
 __device__ __forceinline__ void load_old(Old &o, const Tile &t, int c, int row0, int col0, int lane)
 {
-    const char *const at = t.square(c) + block_at(col0, row0, t.sp) + 8 * (lane >> 5);
+    const Global<const char> at = global((const char *)t.square(c) + block_at(col0, row0, t.sp) + 8 * (lane >> 5));
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-        o.h[g] = *(const uint2 *)(at + (g >> 1) * 2048 + piece_at(lane, 2 * (g & 1)));
-        o.l[g] = *(const uint2 *)(at + (g >> 1) * 2048 + piece_at(lane, 2 * (g & 1) + 1));
+        o.h[g] = *(Global<const v2u>)(at + (g >> 1) * 2048 + piece_at(lane, 2 * (g & 1)));
+        o.l[g] = *(Global<const v2u>)(at + (g >> 1) * 2048 + piece_at(lane, 2 * (g & 1) + 1));
     }
 }
 
-// Value v of a lane's tile in w, or null outside.
-__device__ __forceinline__ float *place_in_w(const Matrix &q, int v, int row0, int col0, int lane)
-{
-    const int r = row0 + acc_row(v, lane), c = col0 + (lane & 31);
-    if (r >= q.s || c >= q.l) return nullptr;
-    return q.w + (q.tall ? (size_t)c * q.s + r : (size_t)r * q.l + c);
-}
-__device__ __forceinline__ void load_w(OldW &o, const Matrix &q, int row0, int col0, int lane)
-{
-#pragma unroll
-    for (int v = 0; v < 16; v++) {
-        const float *const w = place_in_w(q, v, row0, col0, lane);
-        o.v[v] = w ? *w : 0.0f;
+// What the last product reads of a matrix, in registers: from the table, every store to w would have it read again.
+struct W {
+    Global<float> w;
+    int s, l, tall, quads;
+};
+
+// A 32 x 32 tile of w, as a lane holds it.  Where all of it lies inside, there are no guards: each guarded load is waited for by
+// itself.
+struct TileOfW {
+    int row0, col0;
+    bool whole;
+    float v[16];
+    __device__ __forceinline__ Global<float> first(const W &q, int lane) const
+    {
+        const int r = row0 + 4 * (lane >> 5), c = col0 + (lane & 31);
+        return q.w + (q.tall ? (size_t)c * q.s + r : (size_t)r * q.l + c);
     }
-}
-__device__ __forceinline__ void update_w(const Matrix &q, const Step &st, float alpha, const v16f &acc, const OldW &o, int row0, int col0, int lane)
-{
-    const float by = st.by * q.wide * alpha;
+    __device__ __forceinline__ bool in(const W &q, int i, int lane) const { return row0 + acc_row(i, lane) < q.s && col0 + (lane & 31) < q.l; }
+    __device__ __forceinline__ void load(const W &q, int lane, int row, int col)
+    {
+        row0 = row;
+        col0 = col;
+        whole = row + 32 <= q.s && col + 32 <= q.l;
+        const Global<float> at = first(q, lane);
+        const size_t step = q.tall ? 1 : (size_t)q.l;
+        if (whole && q.quads) {
 #pragma unroll
-    for (int v = 0; v < 16; v++) {
-        float *const w = place_in_w(q, v, row0, col0, lane);
-        if (w) *w = st.keep * o.v[v] - by * acc[v];
+            for (int g = 0; g < 4; g++) {
+                const v4f x = *(Global<const v4f>)(at + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[4 * g + e] = x[e];
+            }
+        } else if (whole) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = at[(8 * (i >> 2) + (i & 3)) * step];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = in(q, i, lane) ? at[(8 * (i >> 2) + (i & 3)) * step] : 0.0f;
+        }
     }
-}
+    __device__ __forceinline__ void update(const W &q, int lane, float keep, float by, const v16f &acc)
+    {
+        const Global<float> at = first(q, lane);
+        const size_t step = q.tall ? 1 : (size_t)q.l;
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = keep * v[i] - by * acc[i];
+        if (whole && q.quads) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) *(Global<v4f>)(at + 8 * g) = v4f{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+        } else if (whole) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) at[(8 * (i >> 2) + (i & 3)) * step] = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (in(q, i, lane)) at[(8 * (i >> 2) + (i & 3)) * step] = v[i];
+        }
+    }
+};
 
 // The end of a 32 x 32 tile of a product at (row0, col0): a lane holds column `col` and rows r .. r + 3 of each of four groups.
 // Values are stored row by row along the columns of the transpose ("across": four neighbouring values of the lane) and, exchanged
@@ -412,7 +462,7 @@ __device__ __forceinline__ void finish(const Tile &t, const SquareOp &op, int tu
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] += op.beta * o[e] + (row0 + r + e == col ? op.gamma : 0.0f);
         }
-        uint2 h, l;
+        v2u h, l;
         split4(v, h, l);
         put_part(images, c, 2 * g, half, h);
         put_part(images, c, 2 * g + 1, half, l);
@@ -425,8 +475,8 @@ __device__ __forceinline__ void finish(const Tile &t, const SquareOp &op, int tu
 }
 
 // The sums of a 32 x 32 tile as four quads per lane.
-__device__ __forceinline__ float4 quad_of(const v16f &a, int g) { return make_float4(a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]); }
-__device__ __forceinline__ void set_quad(v16f &a, int g, float4 v)
+__device__ __forceinline__ v4f quad_of(const v16f &a, int g) { return v4f{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]}; }
+__device__ __forceinline__ void set_quad(v16f &a, int g, v4f v)
 {
     a[4 * g] = v.x;
     a[4 * g + 1] = v.y;
@@ -434,7 +484,45 @@ __device__ __forceinline__ void set_quad(v16f &a, int g, float4 v)
     a[4 * g + 3] = v.w;
 }
 
-// Big tiles are 128 x 128, 64 x 64 for each of four wavefronts, small ones 64 x 64.
+// What a wavefront does with its MI x NI tiles of 32 x 32 at (row0, col0).
+template <int kProduct, int MI, int NI>
+__device__ __forceinline__ void finish_all(const Matrix *jobs, const Tile &t, const Step &st, const SquareOp &op, int turn, const v16f (&acc)[MI][NI],
+                                           int row0, int col0, int w, int lane, char *images)
+{
+    if (kProduct == kGram && t.slot >= 0) {
+        const Global<v4f> to = (Global<v4f>)global(jobs[t.job].partial) + ((size_t)t.slot * 1024 + w * MI * NI * 256 + lane);
+#pragma unroll
+        for (int k = 0; k < MI * NI; k++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) to[(k * 4 + g) * 64] = quad_of(acc[k / NI][k % NI], g);
+        return;
+    }
+    if constexpr (kProduct == kLast) {
+        const Matrix &m = jobs[t.job];
+        const W q{global(m.w), m.s, m.l, m.tall, m.quads};
+        const float by = st.by * m.wide * op.alpha;
+        TileOfW a, b;   // one is updated while the next one arrives
+        a.load(q, lane, row0, col0);
+#pragma unroll
+        for (int k = 0; k < MI * NI; k += 2) {
+            if (k + 1 < MI * NI) b.load(q, lane, row0 + (k + 1) / NI * 32, col0 + (k + 1) % NI * 32);
+            a.update(q, lane, st.keep, by, acc[k / NI][k % NI]);
+            if (k + 2 < MI * NI) a.load(q, lane, row0 + (k + 2) / NI * 32, col0 + (k + 2) % NI * 32);
+            if (k + 1 < MI * NI) b.update(q, lane, st.keep, by, acc[(k + 1) / NI % MI][(k + 1) % NI]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+            for (int j = 0; j < NI; j++) {
+                if (kProduct == kApply && col0 + 32 * j >= t.lp) continue;   // the end of X inside a tile
+                Old old;
+                if (kProduct == kSquare) load_old(old, t, op.c, row0 + 32 * i, col0 + 32 * j, lane);
+                finish<kProduct>(t, op, turn, acc[i][j], old, row0 + 32 * i, col0 + 32 * j, lane, images);
+            }
+    }
+}
+
 template <int kProduct>
 __global__ __launch_bounds__(kBlock, 2) void muon_product_k(const Matrix *jobs, const Tile *tiles, Step st, SquareOps ops, int turn)
 {
@@ -442,91 +530,73 @@ __global__ __launch_bounds__(kBlock, 2) void muon_product_k(const Matrix *jobs, 
     const Tile t = tiles[blockIdx.x];
     if (t.job < 0) return;
     const SquareOp op = ops.op[blockIdx.y];
-    const Matrix &q = jobs[t.job];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w >> 1, wn = w & 1;
     const char *const left = kProduct == kGram ? t.along(turn) : t.square(op.l);
     const char *const right = kProduct == kGram ? t.along(turn) : kProduct == kSquare ? t.square(op.r) : t.across(turn);
     const int steps = kProduct == kGram ? t.lp : t.sp;   // of a row of both
-    const size_t row_of_blocks = (size_t)steps * 128;
+    const size_t row_of_blocks = (size_t)steps * 128, from = (size_t)t.from * 4096;
     char *const images = lds + w * 8192;
-    if (t.big) {   // eight rows of blocks, two of them a wavefront's to bring; 16 steps a stage
-        const int r0 = t.i * 128 + (w >> 1) * 64, c0 = t.j * 128 + (w & 1) * 64;
-        const char *const src = (w < 2 ? left + (size_t)(t.i * 4 + 2 * w) * row_of_blocks : right + (size_t)(t.j * 4 + 2 * w - 4) * row_of_blocks) +
-                                (size_t)t.from * 4096;
+    if (t.kind == kSmall) {   // four rows of blocks, one for each wavefront to bring; 32 steps a stage
+        const char *const src = (w < 2 ? left + (size_t)(t.i * 2 + w) * row_of_blocks : right + (size_t)(t.j * 2 + w - 2) * row_of_blocks) + from;
+        v16f acc[1][1];
+        zero_acc(acc);
+        pipeline<5, 16384, 4>(
+            lds, t.to - t.from, [&](int k, char *to) { bring(src + (size_t)k * 4096, 4, lane, to + w * 4096); },
+            [&](const char *now) {
+#pragma unroll
+                for (int s = 0; s < 2; s++) multiply(now + wm * 4096 + s * 2048, now + 8192 + wn * 4096 + s * 2048, lane, acc);
+            });
+        finish_all<kProduct>(jobs, t, st, op, turn, acc, t.i * 64 + wm * 32, t.j * 64 + wn * 32, w, lane, images);
+        return;
+    }
+    if constexpr (kProduct == kGram || kProduct == kSquare) {   // eight rows of blocks, two for each wavefront; 16 steps a stage
+        const char *const src =
+            (w < 2 ? left + (size_t)(t.i * 4 + 2 * w) * row_of_blocks : right + (size_t)(t.j * 4 + 2 * w - 4) * row_of_blocks) + from;
         v16f acc[2][2];
         zero_acc(acc);
-        pipeline(
+        pipeline<5, 16384, 4>(
             lds, 2 * (t.to - t.from),
             [&](int k, char *to) {
                 bring(src + (size_t)k * 2048, 2, lane, to + w * 4096);
                 bring(src + row_of_blocks + (size_t)k * 2048, 2, lane, to + w * 4096 + 2048);
             },
-            [&](const char *now) { multiply<2>(now + (w >> 1) * 4096, now + kStage / 2 + (w & 1) * 4096, 2048, lane, acc); });
-        if constexpr (kProduct == kLast) {
-            OldW old[2][2];
+            [&](const char *now) { multiply(now + wm * 4096, now + 8192 + wn * 4096, lane, acc); });
+        finish_all<kProduct>(jobs, t, st, op, turn, acc, t.i * 128 + wm * 64, t.j * 128 + wn * 64, w, lane, images);
+    } else {   // four rows of blocks on the left, eight on the right (the last one again where X ends), three for each wavefront
+        const int last = t.lp / 32 - 1;
+        const char *src[3];
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) load_w(old[i][j], q, r0 + 32 * i, c0 + 32 * j, lane);
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) update_w(q, st, op.alpha, acc[i][j], old[i][j], r0 + 32 * i, c0 + 32 * j, lane);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    Old old;
-                    if (kProduct == kSquare) load_old(old, t, op.c, r0 + 32 * i, c0 + 32 * j, lane);
-                    finish<kProduct>(t, op, turn, acc[i][j], old, r0 + 32 * i, c0 + 32 * j, lane, images);
-                }
+        for (int b = 0; b < 3; b++) {
+            const int r = 3 * w + b;
+            src[b] = (r < 4 ? left + (size_t)(t.i * 4 + r) * row_of_blocks : right + (size_t)min(t.j * 8 + r - 4, last) * row_of_blocks) + from;
         }
-        return;
-    }
-    const int row0 = t.i * 64 + (w >> 1) * 32, col0 = t.j * 64 + (w & 1) * 32;
-    Old old;
-    OldW old_w;
-    if constexpr (kProduct == kSquare) load_old(old, t, op.c, row0, col0, lane);
-    if constexpr (kProduct == kLast) load_w(old_w, q, row0, col0, lane);
-    // four rows of blocks, one for each wavefront to bring; 32 steps a stage
-    const char *const src = (w < 2 ? left + (size_t)(t.i * 2 + w) * row_of_blocks : right + (size_t)(t.j * 2 + w - 2) * row_of_blocks) +
-                            (size_t)t.from * 4096;
-    v16f acc[1][1];
-    zero_acc(acc);
-    pipeline(
-        lds, t.to - t.from, [&](int k, char *to) { bring(src + (size_t)k * 4096, 4, lane, to + w * 4096); },
-        [&](const char *now) {
+        v16f acc[2][4];
+        zero_acc(acc);
+        pipeline<3, 24576, 6>(
+            lds, 2 * (t.to - t.from),
+            [&](int k, char *to) {
 #pragma unroll
-            for (int s = 0; s < 2; s++)
-                multiply<1>(now + (w >> 1) * 4096 + s * 2048, now + kStage / 2 + (w & 1) * 4096 + s * 2048, 0, lane, acc);
-        });
-    if (kProduct == kGram && t.slot >= 0) {
-#pragma unroll
-        for (int g = 0; g < 4; g++) q.partial[(((size_t)t.slot * 4 + w) * 4 + g) * 64 + lane] = quad_of(acc[0][0], g);
-        return;
+                for (int b = 0; b < 3; b++) bring(src[b] + (size_t)k * 2048, 2, lane, to + (3 * w + b) * 2048);
+            },
+            [&](const char *now) { multiply(now + wm * 4096, now + 8192 + wn * 8192, lane, acc); });
+        finish_all<kProduct>(jobs, t, st, op, turn, acc, t.i * 128 + wm * 64, t.j * 256 + wn * 128, w, lane, images);
     }
-    if constexpr (kProduct == kLast) update_w(q, st, op.alpha, acc[0][0], old_w, row0, col0, lane);
-    else finish<kProduct>(t, op, turn, acc[0][0], old, row0, col0, lane, images);
 }
 
-// Adds the parts of a tile of A, in their order.
+// Adds the parts of 64 x 64 values of A, in their order.
 __global__ __launch_bounds__(kBlock) void muon_meet_k(const Matrix *jobs, const Tile *tiles, SquareOps ops)
 {
     __shared__ __attribute__((aligned(16))) char images[4 * 8192];
     const Tile t = tiles[blockIdx.x];
-    const Matrix &q = jobs[t.job];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const Global<const v4f> from = (Global<const v4f>)global((const float4 *)jobs[t.job].partial) + ((size_t)t.slot * 1024 + w * 256 + lane);
+    const size_t step = t.kind == kSmall ? 1024 : 4096;
     v16f sum;
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p = 0; p < t.parts; p++) {
-            const float4 o = q.partial[(((size_t)(t.slot + p) * 4 + w) * 4 + g) * 64 + lane];
-            v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
-        }
-        set_quad(sum, g, v);
-    }
+    for (int g = 0; g < 4; g++) set_quad(sum, g, v4f{0.0f, 0.0f, 0.0f, 0.0f});
+    for (int p = 0; p < t.parts; p++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) set_quad(sum, g, quad_of(sum, g) + from[p * step + g * 64]);
     finish<kGram>(t, ops.op[0], 0, sum, Old{}, t.i * 64 + (w >> 1) * 32, t.j * 64 + (w & 1) * 32, lane, images + w * 8192);
 }
 
@@ -534,7 +604,7 @@ __global__ __launch_bounds__(kBlock) void muon_meet_k(const Matrix *jobs, const 
 __global__ __launch_bounds__(kBlock) void muon_plain_k(const Matrix *jobs, const Tile *chunks, Step st)
 {
     const Tile t = chunks[blockIdx.x];
-    const Matrix &q = jobs[t.job];
+    const Matrix q = jobs[t.job];
     const size_t n = (size_t)q.rows * q.cols, from = (size_t)t.i * kChunk, to = min(from + kChunk, n);
     const float by = st.by * q.wide * (1.0f / kUp);
     for (size_t i = from + threadIdx.x; i < to; i += kBlock) {
@@ -580,7 +650,7 @@ int build(Handle *h)
     size_t bytes = 0;
     auto take = [&](size_t n) { const size_t at = bytes; bytes += ceil_div(n, (size_t)256) * 256; return at; };
     std::vector<size_t> x_at, sq_at, partial_at, parts_at;
-    size_t all = 0;   // 32-step stages of all tiles of A
+    size_t all = 0, mids = 0;   // stages of all tiles of A; 128 x 128 tiles of square matrices
     for (Matrix &q : h->jobs) {
         q.tall = q.rows > q.cols;
         q.s = std::min(q.rows, q.cols);
@@ -588,19 +658,23 @@ int build(Handle *h)
         const int side = q.s <= 64 ? 64 : 128;
         q.sp = (int)ceil_div((size_t)q.s, (size_t)side) * side;
         q.lp = (int)ceil_div((size_t)q.l, (size_t)side) * side;
+        q.quads = q.tall && q.cols % 4 == 0 && aligned16(q.w);
         q.wide = std::sqrt(std::max(1.0f, (float)q.rows / (float)q.cols));
         q.nparts = (int)ceil_div((size_t)q.rows * q.cols, kChunk);
-        const size_t t = q.sp / 64;
-        all += t * (t + 1) / 2 * (q.lp / 32);
+        const size_t t = q.sp / side, tiles = t * (t + 1) / 2;
+        all += tiles * (q.lp / 32) * (side / 64);   // (a stage of a 128 x 128 tile is 16 steps)
+        mids += side == 128 ? tiles : 0;
     }
-    // A's reduction is cut where its tiles alone would not give every CU its share
-    const size_t part = std::max((size_t)32, ceil_div(all * 2, (size_t)num_cus() * 3));
-    auto cuts_of = [&](const Matrix &q) { return (int)ceil_div((size_t)q.lp / 32, part); };
+    // A's reduction is cut so that two workgroups for each CU have about the same to do
+    const size_t part = std::max((size_t)32, ceil_div(all, (size_t)num_cus() * 2));
+    auto cuts_of = [&](const Matrix &q) { return (int)ceil_div((size_t)q.lp / 32 * (q.sp == 64 ? 1 : 2), part); };
+    // 64 x 64 tiles spread a short product over more CUs, 128 x 128 tiles take half the operands' traffic: 13 products of [512 x 512] ..
+    const bool mid_squares = mids >= (size_t)num_cus() * 2;
     for (const Matrix &q : h->jobs) {
-        const size_t t = q.sp / 64, cuts = cuts_of(q);
+        const size_t side = q.sp == 64 ? 64 : 128, t = q.sp / side, cuts = cuts_of(q);
         x_at.push_back(take((size_t)q.sp * q.lp * 4 * 4));
         sq_at.push_back(take((size_t)q.sp * q.sp * 4 * kSquares));
-        partial_at.push_back(take(cuts > 1 ? cuts * t * (t + 1) / 2 * 64 * 64 * sizeof(float) : 0));
+        partial_at.push_back(take(cuts > 1 ? cuts * t * (t + 1) / 2 * side * side * sizeof(float) : 0));
         parts_at.push_back(take((size_t)q.nparts * sizeof(double)));
     }
     const size_t tables_at = bytes;
@@ -608,37 +682,51 @@ int build(Handle *h)
     std::vector<double> cgram, csq, cwide;
     for (size_t k = 0; k < h->jobs.size(); k++) {   // (addresses are offsets until the memory is there)
         const Matrix &q = h->jobs[k];
-        const int side = q.s <= 64 ? 64 : 128, deep = q.lp / 32, cuts = cuts_of(q);
+        const bool small = q.sp == 64;
+        const int side = small ? 64 : 128, deep = q.lp / 32, cuts = cuts_of(q);
         const int rp = q.tall ? q.lp : q.sp, cp = q.tall ? q.sp : q.lp;
-        Tile t{(char *)sq_at[k], (char *)x_at[k], q.sp, q.lp, (int)k, 0, 0, 0, 0, q.sp / 32, -1, 0};
+        Tile t{(char *)sq_at[k], (char *)x_at[k], q.sp, q.lp, (int)k, 0, 0, kSmall, 0, q.sp / 32, -1, 0};
         auto at = [&](int i, int j) { t.i = i; t.j = j; return t; };
         for (int i = 0; i < q.nparts; i++) chunks.push_back(at(i, 0));
         for (int i = 0; i < rp / 64; i++)
             for (int j = 0; j < cp / 64; j++) scales.push_back(at(i, j));
-        int slots = 0;
-        for (int i = 0; i < q.sp / 64; i++)
+        t.kind = mid_squares && !small ? kMid : kSmall;
+        for (int i = 0; i < q.sp / (t.kind == kMid ? 128 : 64); i++)
             for (int j = 0; j <= i; j++) {
                 squares.push_back(at(i, j));
-                csq.push_back((double)q.sp + 256);
+                csq.push_back((double)(q.sp + 256) * (t.kind == kMid ? 2 : 1));
+            }
+        t.kind = small ? kSmall : kMid;
+        int slots = 0;
+        for (int i = 0; i < q.sp / side; i++)
+            for (int j = 0; j <= i; j++) {
                 Tile g = at(i, j);
-                if (cuts > 1) {
-                    g.slot = slots;
+                if (cuts > 1) {   // its quarters of 64 x 64, on and below the diagonal
                     g.parts = cuts;
-                    meets.push_back(g);
+                    for (int p = 0; p < (small ? 1 : 4); p++) {
+                        g.slot = slots + p;
+                        g.i = small ? i : 2 * i + p / 2;
+                        g.j = small ? j : 2 * j + p % 2;
+                        if (g.i >= g.j) meets.push_back(g);
+                    }
+                    g = at(i, j);
                 }
                 for (int c = 0; c < cuts; c++) {
                     g.from = (int)((size_t)deep * c / cuts);
                     g.to = (int)((size_t)deep * (c + 1) / cuts);
-                    if (cuts > 1) g.slot = slots++;
+                    if (cuts > 1) {
+                        g.slot = slots;
+                        slots += small ? 1 : 4;
+                    }
                     grams.push_back(g);
-                    cgram.push_back((double)(g.to - g.from) + 8);
+                    cgram.push_back((double)(g.to - g.from) * (small ? 1 : 2) + 8);
                 }
             }
-        t.big = side == 128;
-        for (int j = 0; j < q.lp / side; j++)
+        t.kind = small ? kSmall : kWide;
+        for (int j = 0; j < (int)ceil_div((size_t)q.lp, (size_t)(small ? 64 : 256)); j++)
             for (int i = 0; i < q.sp / side; i++) {
                 wides.push_back(at(i, j));
-                cwide.push_back((double)q.sp + 256);
+                cwide.push_back((double)(q.sp + 256) * (small ? 1 : 4));
             }
     }
     grams = deal(grams, cgram);
@@ -679,10 +767,9 @@ template <int kProduct>
 int launch(const Handle *h, unsigned blocks, unsigned products, const Tile *tiles, const Step &st, const SquareOps &ops, int turn)
 {
     static bool raised = false;   // above 64 KB of dynamic LDS a kernel has to be told once
-    if (!raised)
-        DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)muon_product_k<kProduct>, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStage));
+    if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)muon_product_k<kProduct>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
     raised = true;
-    hipLaunchKernelGGL(muon_product_k<kProduct>, dim3(blocks, products), dim3(kBlock), kStages * kStage, stream(), h->d_jobs, tiles, st, ops, turn);
+    hipLaunchKernelGGL(muon_product_k<kProduct>, dim3(blocks, products), dim3(kBlock), kLds, stream(), h->d_jobs, tiles, st, ops, turn);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
