@@ -24,6 +24,7 @@ using namespace dopt;
 
 constexpr int kBlock = 256;
 constexpr int kPiece = 8192;   // values of a part
+constexpr int kRuns = 64;      // runs of pixels of a channels-last sample, at most
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));   // sixteen bytes wherever they start
@@ -39,9 +40,22 @@ __device__ __forceinline__ void meet()
     __syncthreads();
 }
 
-__device__ __forceinline__ float lanes_sum(float v, int lanes)   // over groups of `lanes` (a power of two) lanes, in all of them
+template <int kControl>
+__device__ __forceinline__ float plus_moved(float v)
 {
-    for (int off = 1; off < lanes; off <<= 1) v += __shfl_xor(v, off, 64);
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), kControl, 0xf, 0xf, true));
+}
+
+// The sum over groups of `lanes` (a power of two, the same in all lanes) lanes, in all of them: with the neighbour, the other pair, the
+// other quad (each of whose lanes holds its sum by now: the mirrored lane's does), the other eight, sixteen and thirty-two.
+__device__ __forceinline__ float lanes_sum(float v, int lanes)
+{
+    if (lanes >= 2) v = plus_moved<0xB1>(v);
+    if (lanes >= 4) v = plus_moved<0x4E>(v);
+    if (lanes >= 8) v = plus_moved<0x141>(v);
+    if (lanes >= 16) v = plus_moved<0x140>(v);
+    if (lanes >= 32) v += __shfl_xor(v, 16, 64);
+    if (lanes >= 64) v += __shfl_xor(v, 32, 64);
     return v;
 }
 
@@ -304,6 +318,40 @@ __global__ __launch_bounds__(1024) void gn_bwd_k(Sizes s, int act, const float *
     }
 }
 
+// Adds `rows` rows of sums, C channels of `pieces` each: eight channels of a workgroup by thirty-two lanes.
+struct Fold {
+    size_t rows, C;
+    int pieces;
+    const float2 *sums;
+    float *dscale, *dbias;
+};
+__device__ __forceinline__ void fold(const Fold &f, size_t block)
+{
+    __shared__ float2 red[32][9];
+    const int col = threadIdx.x & 7, lane = threadIdx.x >> 3;
+    const size_t c = block * 8 + col;
+    float s = 0.0f, q = 0.0f;
+    if (c < f.C) {
+#pragma unroll 8
+        for (size_t i = lane; i < f.rows * f.pieces; i += 32) {
+            const float2 v = f.pieces == 1 ? f.sums[i * f.C + c] : f.sums[(i / f.pieces * f.C + c) * f.pieces + i % f.pieces];
+            s += v.x;
+            q += v.y;
+        }
+    }
+    red[lane][col] = make_float2(s, q);
+    meet();
+    if (lane == 0 && c < f.C) {
+        for (int i = 1; i < 32; i++) {
+            s += red[i][col].x;
+            q += red[i][col].y;
+        }
+        f.dbias[c] = s;
+        f.dscale[c] = q;
+    }
+}
+__global__ __launch_bounds__(kBlock) void gn_fold_k(Fold f) { fold(f, blockIdx.x); }
+
 // ------------------------------------------------------------------------------- [N, inner, C]
 
 // V channels to a thread (four where C is a multiple of four), C / V threads to a pixel, as many pixels at once as 256 threads take; more
@@ -427,22 +475,33 @@ __global__ __launch_bounds__(kBlock) void gn_last_apply_k(Rows r, float eps, int
     extern __shared__ float2 entry[];   // [group]: mean, rstd
     typedef typename Vec<V>::type vec __attribute__((aligned(4)));
     const Run run = run_of(r);
-    for (int g = threadIdx.x; g < r.G; g += kBlock) {
+    const int lane = threadIdx.x & 7;
+    for (int g = threadIdx.x >> 3; g < r.G; g += kBlock / 8) {   // a group's runs by eight lanes, eight runs to a lane
         const float2 *const of = stats + run.n * r.S * r.G + g;
-        const float all = (float)r.inner, pivot = of[0].x;
+        const float all = (float)r.inner;
+        float2 part[kRuns / 8];
+        float w[kRuns / 8];
+#pragma unroll
+        for (int i = 0; i < kRuns / 8; i++) part[i] = of[(size_t)min(lane + 8 * i, r.S - 1) * r.G];
+#pragma unroll
+        for (int i = 0; i < kRuns / 8; i++) w[i] = lane + 8 * i < r.S ? (float)pixels_in(r, lane + 8 * i) : 0.0f;
+        const float pivot = __shfl(part[0].x, 0, 8);   // equal means give that mean
         float m = 0.0f, q = 0.0f;
-        for (int i = 0; i < r.S; i++) m += (of[(size_t)i * r.G].x - pivot) * ((float)pixels_in(r, i) / all);
-        m += pivot;
-        for (int i = 0; i < r.S; i++) {
-            const float2 o = of[(size_t)i * r.G];
-            const float d = o.x - m;
-            q += o.y + (float)pixels_in(r, i) * (float)r.Cg * (d * d);
+#pragma unroll
+        for (int i = 0; i < kRuns / 8; i++) m += (part[i].x - pivot) * (w[i] / all);
+        m = pivot + lanes_sum(m, 8);
+#pragma unroll
+        for (int i = 0; i < kRuns / 8; i++) {
+            const float d = part[i].x - m;
+            q += (w[i] > 0.0f ? part[i].y : 0.0f) + w[i] * (float)r.Cg * (d * d);
         }
-        const float rstd = 1.0f / sqrtf(q / (all * (float)r.Cg) + eps);
-        entry[g] = make_float2(m, rstd);
-        if (run.k == 0) {
-            means[run.n * r.G + g] = m;
-            rstds[run.n * r.G + g] = rstd;
+        const float rstd = 1.0f / sqrtf(lanes_sum(q, 8) / (all * (float)r.Cg) + eps);
+        if (lane == 0) {
+            entry[g] = make_float2(m, rstd);
+            if (run.k == 0) {
+                means[run.n * r.G + g] = m;
+                rstds[run.n * r.G + g] = rstd;
+            }
         }
     }
     meet();
@@ -483,21 +542,32 @@ __global__ __launch_bounds__(kBlock) void gn_last_apply_k(Rows r, float eps, int
 // kDx = false: sums of dz and dz xhat over a run of pixels, per channel (sums) and, times scale, per group (gsums).  kDx: dx.
 template <int V, bool kDx>
 __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const float *dy, const float *x, const float *scale, const float *bias,
-                                                         const float *means, const float *rstds, float2 *sums, float2 *gsums, float *dx)
+                                                         const float *means, const float *rstds, float2 *sums, float2 *gsums, float *dx,
+                                                         unsigned runs, Fold f)
 {
     extern __shared__ float2 entry[];   // kDx: [group]: s1, s2; else [pixel lane][channel]
     typedef typename Vec<V>::type vec __attribute__((aligned(4)));
+    if (kDx && blockIdx.x >= runs) {   // the sums over all runs wait for nothing that this launch does: they ride behind it
+        fold(f, blockIdx.x - runs);
+        return;
+    }
     const Run run = run_of(r);
     if (kDx) {
         const float total = (float)r.inner * (float)r.Cg;
-        for (int g = threadIdx.x; g < r.G; g += kBlock) {
+        const int lane = threadIdx.x & 7;
+        for (int g = threadIdx.x >> 3; g < r.G; g += kBlock / 8) {
             float s = 0.0f, q = 0.0f;
-            for (int i = 0; i < r.S; i++) {
-                const float2 o = gsums[(run.n * r.S + i) * r.G + g];
-                s += o.x;
-                q += o.y;
+            float2 part[kRuns / 8];
+#pragma unroll
+            for (int i = 0; i < kRuns / 8; i++) part[i] = gsums[(run.n * r.S + min(lane + 8 * i, r.S - 1)) * r.G + g];
+#pragma unroll
+            for (int i = 0; i < kRuns / 8; i++) {
+                s += lane + 8 * i < r.S ? part[i].x : 0.0f;
+                q += lane + 8 * i < r.S ? part[i].y : 0.0f;
             }
-            entry[g] = make_float2(s / total, q / total);
+            s = lanes_sum(s, 8);
+            q = lanes_sum(q, 8);
+            if (lane == 0) entry[g] = make_float2(s / total, q / total);
         }
         meet();
     }
@@ -774,33 +844,6 @@ __global__ __launch_bounds__(kBlock) void gn_any_dx_k(Place p, int act, const fl
     });
 }
 
-// Adds `rows` rows of sums, C channels of `pieces` each: sixteen channels by sixteen lanes.
-__global__ __launch_bounds__(kBlock) void gn_fold_k(size_t rows, size_t C, int pieces, const float2 *sums, float *dscale, float *dbias)
-{
-    __shared__ float2 red[16][17];
-    const int col = threadIdx.x & 15, lane = threadIdx.x >> 4;
-    const size_t c = (size_t)blockIdx.x * 16 + col;
-    float s = 0.0f, q = 0.0f;
-    if (c < C) {
-#pragma unroll 4
-        for (size_t i = lane; i < rows * pieces; i += 16) {
-            const float2 v = sums[(i / pieces * C + c) * pieces + i % pieces];
-            s += v.x;
-            q += v.y;
-        }
-    }
-    red[lane][col] = make_float2(s, q);
-    meet();
-    if (lane == 0 && c < C) {
-        for (int i = 1; i < 16; i++) {
-            s += red[i][col].x;
-            q += red[i][col].y;
-        }
-        dbias[c] = s;
-        dscale[c] = q;
-    }
-}
-
 // ------------------------------------------------------------------------------- which of them
 
 // How a workgroup holds `channels` channels of `len` values: threads (0: it cannot), channels and quads of a thread.
@@ -885,7 +928,7 @@ Rows rows_of(size_t N, size_t C, size_t inner, size_t G, int V)
     r.G = (int)G;
     r.U = (int)(C / V);
     r.R = std::max(1, kBlock / r.U);
-    const size_t most = std::min((size_t)64, ceil_div(inner, (size_t)r.R * 8));   // (eight pixels to a thread, and the runs are joined by a thread each)
+    const size_t most = std::min((size_t)kRuns, ceil_div(inner, (size_t)r.R * 8));   // (eight pixels to a thread)
     r.S = (int)std::min(most, std::max((size_t)1, ceil_div((size_t)num_cus() * 4, N)));
     return r;
 }
@@ -982,9 +1025,9 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
     float *const dx = packed;
     const float *const means = stats, *const rstds = stats + N * G;
     float2 *sums = nullptr;
+    const unsigned folds = (unsigned)ceil_div(C, (size_t)8);
     auto fold = [&](size_t rows, int pieces) -> int {
-        hipLaunchKernelGGL(gn_fold_k, dim3((unsigned)ceil_div(C, (size_t)16)), dim3(kBlock), 0, stream(), rows, C, pieces, sums, packed + total,
-                           packed + total + C);
+        hipLaunchKernelGGL(gn_fold_k, dim3(folds), dim3(kBlock), 0, stream(), Fold{rows, C, pieces, sums, packed + total, packed + total + C});
         DOPT_LAUNCH_CHECK();
         return DOPT_HIP_OK;
     };
@@ -1008,14 +1051,15 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
             sums = (float2 *)workspace(N * r.S * (C + G) * sizeof(float2));
             if (!sums) return DOPT_HIP_ERR_OOM;
             float2 *const gsums = sums + N * r.S * C;
-            const dim3 grid((unsigned)(N * r.S));
-            hipLaunchKernelGGL((gn_last_grad_k<V, false>), grid, dim3(kBlock), r.R * C * sizeof(float2), stream(), r, act, dy, x, scale, bias, means,
-                               rstds, sums, gsums, dx);
+            const unsigned runs = (unsigned)(N * r.S);
+            const Fold f{N * r.S, C, 1, sums, packed + total, packed + total + C};
+            hipLaunchKernelGGL((gn_last_grad_k<V, false>), dim3(runs), dim3(kBlock), r.R * C * sizeof(float2), stream(), r, act, dy, x, scale, bias,
+                               means, rstds, sums, gsums, dx, runs, f);
             DOPT_LAUNCH_CHECK();
-            hipLaunchKernelGGL((gn_last_grad_k<V, true>), grid, dim3(kBlock), G * sizeof(float2), stream(), r, act, dy, x, scale, bias, means, rstds,
-                               sums, gsums, dx);
+            hipLaunchKernelGGL((gn_last_grad_k<V, true>), dim3(runs + folds), dim3(kBlock), G * sizeof(float2), stream(), r, act, dy, x, scale, bias,
+                               means, rstds, sums, gsums, dx, runs, f);
             DOPT_LAUNCH_CHECK();
-            return fold(N * r.S, 1);
+            return DOPT_HIP_OK;
         });
     if (!channels_last && inner >= 4) {
         const Split k = split_of(N, C, inner, G);
