@@ -3,10 +3,11 @@
 //
 //     pre = x w^T + bias,  y = act(pre) + residual
 //     dz = dy act'(pre),  dx = dz w,  dw = dz^T x,  dbias = column sums of dz;  the residual's gradient is dy
+#include <algorithm>
 #include <type_traits>
 
-#include "activation.h"
 #include "common.h"
+#include "dense.h"
 
 namespace {
 
@@ -20,31 +21,93 @@ unsigned flat_grid(size_t n)
     return (unsigned)(blocks < cap ? blocks : cap);
 }
 
-// y holds the product.
-template <int kAct>
-__global__ __launch_bounds__(kBlock) void dense_epilogue_k(size_t n, size_t N, const float *bias, const float *residual, float *y, float *pre)
+// y holds the product.  V values at a time of a row whose length is a multiple of V.
+template <int V>
+__global__ __launch_bounds__(kBlock) void dense_epilogue_k(size_t n, DenseEpilogue e, float *y)
 {
-    for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) {
-        const float z = bias ? y[i] + bias[i % N] : y[i];
-        if (pre) pre[i] = z;
-        const float v = act_value<kAct>(z);
-        y[i] = residual ? v + residual[i] : v;
+    typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
+    with_activation(e.act, [&](auto kind) {
+        for (size_t i = ((size_t)blockIdx.x * kBlock + threadIdx.x) * V; i < n; i += (size_t)gridDim.x * kBlock * V) {
+            vec z = *(const vec *)(y + i), o;
+            if (e.bias) z += *(const vec *)(e.bias + i % e.N);
+            if (e.pre) *(vec *)(e.pre + i) = z;
+#pragma unroll
+            for (int k = 0; k < V; k++) ((float *)&o)[k] = act_value<kind.value>(((float *)&z)[k]);
+            if (e.residual) o += *(const vec *)(e.residual + i);
+            *(vec *)(y + i) = o;
+        }
+    });
+}
+
+// dz = dy act'(pre), where there is an activation, and its sums over runs of rows: a workgroup takes 64 V columns by four rows at a time.
+// Bound by memory; the sums cost no pass of their own.
+template <int V>
+__global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int runs, int act, const float *dy, const float *pre, float *dz, float *sums)
+{
+    typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
+    __shared__ float red[4][64 * V];
+    const size_t tiles = (N + 64 * V - 1) / (64 * V), run = blockIdx.x / tiles, col = (blockIdx.x % tiles * 64 + (threadIdx.x & 63)) * V;
+    const size_t from = M * run / runs, to = M * (run + 1) / runs;
+    const int row = threadIdx.x >> 6;
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) s[e] = 0.0f;
+    if (col < N) {
+        with_activation(act, [&](auto kind) {
+            constexpr bool kPlain = decltype(kind)::value == DOPT_HIP_ACT_NONE;
+            auto one = [&](const float *d, const float *z, size_t at) {
+                float o[V];
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    o[e] = act_grad<kind.value>(d[e], z[e]);
+                    s[e] += o[e];
+                    if (!kPlain) dz[at + e] = o[e];
+                }
+            };
+            size_t m = from + row;
+            for (; m + 12 < to; m += 16) {
+                vec d[4], z[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    d[i] = *(const vec *)(dy + (m + 4 * i) * N + col);
+                    if (!kPlain) z[i] = *(const vec *)(pre + (m + 4 * i) * N + col);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) one((const float *)&d[i], kPlain ? (const float *)&d[i] : (const float *)&z[i], (m + 4 * i) * N + col);
+            }
+            for (; m < to; m += 4) {
+                const vec d = *(const vec *)(dy + m * N + col), z = kPlain ? d : *(const vec *)(pre + m * N + col);
+                one((const float *)&d, (const float *)&z, m * N + col);
+            }
+        });
+    }
+    if (!sums) return;
+#pragma unroll
+    for (int e = 0; e < V; e++) red[row][(threadIdx.x & 63) * V + e] = s[e];
+    __syncthreads();
+    for (size_t c = threadIdx.x; c < 64 * V; c += kBlock) {
+        const size_t at = blockIdx.x % tiles * 64 * V + c;
+        if (at < N) sums[run * N + at] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
     }
 }
 
-template <int kAct>
-__global__ __launch_bounds__(kBlock) void dense_dz_k(size_t n, const float *dy, const float *pre, float *dz)
+// Adds the runs: eight columns of a workgroup by thirty-two lanes.
+__global__ __launch_bounds__(kBlock) void dense_fold_k(size_t runs, size_t N, const float *sums, float *dbias)
 {
-    for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) dz[i] = act_grad<kAct>(dy[i], pre[i]);
-}
-
-__global__ __launch_bounds__(kBlock) void dense_columns_k(size_t M, size_t N, const float *dz, float *dbias)
-{
-    const size_t c = (size_t)blockIdx.x * kBlock + threadIdx.x;
-    if (c >= N) return;
+    __shared__ float red[32][9];
+    const int col = threadIdx.x & 7, lane = threadIdx.x >> 3;
+    const size_t c = (size_t)blockIdx.x * 8 + col;
     float s = 0.0f;
-    for (size_t m = 0; m < M; m++) s += dz[m * N + c];
-    dbias[c] = s;
+    if (c < N) {
+#pragma unroll 4
+        for (size_t i = lane; i < runs; i += 32) s += sums[i * N + c];
+    }
+    red[lane][col] = s;
+    __syncthreads();
+    if (lane == 0 && c < N) {
+        for (int i = 1; i < 32; i++) s += red[i][col];
+        dbias[c] = s;
+    }
 }
 
 int check(const char *who, size_t M, size_t N, size_t K, int act)
@@ -57,6 +120,18 @@ int check(const char *who, size_t M, size_t N, size_t K, int act)
 }
 
 }  // namespace
+
+namespace dopt {
+
+int dense_finish(size_t M, size_t N, const DenseEpilogue &e, float *y)
+{
+    if (N % 4 == 0) hipLaunchKernelGGL(dense_epilogue_k<4>, dim3(flat_grid(M * N / 4)), dim3(kBlock), 0, stream(), M * N, e, y);
+    else hipLaunchKernelGGL(dense_epilogue_k<1>, dim3(flat_grid(M * N)), dim3(kBlock), 0, stream(), M * N, e, y);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+}  // namespace dopt
 
 extern "C" {
 
@@ -71,12 +146,7 @@ int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, co
         DOPT_REQUIRE(!overlaps(o, out, x, M * K * f) && !overlaps(o, out, w, N * K * f) && !overlaps(o, out, bias, N * f) && !overlaps(o, out, residual, out),
                      "dopt_hip_dense_act: a result overlaps an operand");
     DOPT_REQUIRE(!overlaps(y, out, pre, out), "dopt_hip_dense_act: y and pre overlap");
-    if (int rc = dopt_hip_sgemm_t(0, 1, M, N, K, x, w, y)) return rc;
-    return with_activation(act, [&](auto a) -> int {
-        hipLaunchKernelGGL(dense_epilogue_k<a.value>, dim3(flat_grid(M * N)), dim3(kBlock), 0, stream(), M * N, N, bias, residual, y, pre);
-        DOPT_LAUNCH_CHECK();
-        return DOPT_HIP_OK;
-    });
+    return product_dense(M, N, K, x, w, DenseEpilogue{bias, residual, pre, act, N}, y);
 }
 
 int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *dy, const float *pre, const float *x, const float *w,
@@ -95,30 +165,41 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
         for (int j = 0; j < i; j++) DOPT_REQUIRE(!overlaps(results[i], sizes[i], results[j], sizes[j]), "dopt_hip_dense_act_grad: two results overlap");
     }
     DOPT_ENSURE_INIT();
+    const bool plain = act == DOPT_HIP_ACT_NONE;
     const float *dz = dy;
-    if (act != DOPT_HIP_ACT_NONE && M * N > 0) {
-        // dz and what the products park beside it share one request, which none of them has to grow
-        const size_t own = ceil_div(M * N * sizeof(float), (size_t)256) * 256;
+    float *sums = nullptr;
+    const int V = N % 4 == 0 ? 4 : 1;
+    const size_t tiles = ceil_div(std::max(N, (size_t)1), (size_t)(64 * V));
+    // enough workgroups to fill the chip, of sixteen rows and more
+    const int runs = (int)std::max((size_t)1, std::min(ceil_div(M, (size_t)16), ceil_div((size_t)num_cus() * 8, tiles)));
+    size_t held = 0;
+    if (M * N > 0 && (!plain || dbias)) {
+        // dz, its sums and what the products park beside them share one request, which none of them has to grow
+        auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
+        const size_t first = plain ? 0 : rounded(M * N * sizeof(float));
+        held = first + rounded((size_t)runs * N * sizeof(float));
         const size_t more = std::max(dx ? product_scratch(0, 0, M, K, N) : 0, dw ? product_scratch(1, 0, N, K, M) : 0);
-        float *const to = (float *)workspace(own + more);
+        char *const to = (char *)workspace(held + more);
         if (!to) return DOPT_HIP_ERR_OOM;
-        with_activation(act, [&](auto a) {
-            hipLaunchKernelGGL(dense_dz_k<a.value>, dim3(flat_grid(M * N)), dim3(kBlock), 0, stream(), M * N, dy, pre, to);
-        });
+        if (!plain) dz = (float *)to;
+        sums = (float *)(to + first);
+        const dim3 grid((unsigned)(tiles * runs));
+        if (V == 4)
+            hipLaunchKernelGGL(dense_dz_k<4>, grid, dim3(kBlock), 0, stream(), M, N, runs, act, dy, pre, (float *)to, dbias ? sums : nullptr);
+        else
+            hipLaunchKernelGGL(dense_dz_k<1>, grid, dim3(kBlock), 0, stream(), M, N, runs, act, dy, pre, (float *)to, dbias ? sums : nullptr);
         DOPT_LAUNCH_CHECK();
-        workspace_hold(own);
-        dz = to;
     }
+    if (dbias && N > 0) {
+        hipLaunchKernelGGL(dense_fold_k, dim3((unsigned)ceil_div(N, (size_t)8)), dim3(kBlock), 0, stream(), sums ? (size_t)runs : 0, N, sums, dbias);
+        DOPT_LAUNCH_CHECK();
+    }
+    workspace_hold(held);
     int rc = DOPT_HIP_OK;
     if (dx && M * K > 0) rc = dopt_hip_sgemm_t(0, 0, M, K, N, dz, w, dx);
     if (!rc && dw && N * K > 0) rc = dopt_hip_sgemm_t(1, 0, N, K, M, dz, x, dw);
     workspace_hold(0);
-    if (rc) return rc;
-    if (dbias && N > 0) {
-        hipLaunchKernelGGL(dense_columns_k, dim3((unsigned)ceil_div(N, (size_t)kBlock)), dim3(kBlock), 0, stream(), M, N, dz, dbias);
-        DOPT_LAUNCH_CHECK();
-    }
-    return DOPT_HIP_OK;
+    return rc;
 }
 
 }  // extern "C"

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "common.h"
+#include "dense.h"
 #include "mfma_core.h"
 
 namespace {
@@ -256,8 +257,8 @@ struct RowsTile {
     static_assert(WM * WN * 64 == kRowsThreads && BM % 64 == 0 && BN % 64 == 0 && BM + BN <= kRowsThreads, "one block of four rows by four steps per thread");
 };
 
-template <class T, bool kTA, bool kTB, bool kCut>
-__global__ __launch_bounds__(kRowsThreads, 2) void sgemm_rows_k(Gemm p)
+template <class T, bool kTA, bool kTB, bool kCut, class E>
+__global__ __launch_bounds__(kRowsThreads, 2) void sgemm_rows_k(Gemm p, E ep)
 {
     constexpr int MI = T::MI, NI = T::NI, kBuf = T::kBuf;
     extern __shared__ __attribute__((aligned(16))) char rows_lds[];
@@ -384,6 +385,51 @@ __global__ __launch_bounds__(kRowsThreads, 2) void sgemm_rows_k(Gemm p)
                 }
             }
     };
+    // The same with a dense layer's end behind the sums (uncut reductions only).
+    auto put_dense = [&](bool add) {
+        if constexpr (E::kOn) {
+            int pitch = p.N;
+            asm volatile("" : "+s"(pitch));
+#pragma unroll
+            for (int j = 0; j < NI; j++) {
+                const int col = n0 + brow + 32 * j;
+                const float bias = ep.bias_of(min(col, p.N - 1));
+#pragma unroll
+                for (int i = 0; i < MI; i++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {   // four rows at a time, no address held longer: the accumulators leave no registers
+                        asm volatile("" : "+s"(pitch));
+                        const int row = m0 + wm * 32 * MI + i * 32 + 8 * g + 4 * kh;
+                        const size_t first = (size_t)row * pitch + col;
+                        auto in = [&](int e) { return whole || (row + e < p.M && col < p.N); };
+                        float old[4], z[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) z[e] = acc[i][j][4 * g + e];
+                        if (add) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) old[e] = in(e) ? p.C[first + (size_t)e * pitch] : 0.0f;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) z[e] += old[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) old[e] = ep.residual && in(e) ? ep.residual[first + (size_t)e * pitch] : 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            z[e] += bias;
+                            if (ep.pre && in(e)) ep.pre[first + (size_t)e * pitch] = z[e];
+                        }
+                        with_activation(ep.act, [&](auto kind) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) z[e] = act_value<kind.value>(z[e]);
+                        });
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (in(e)) p.C[first + (size_t)e * pitch] = ep.residual ? z[e] + old[e] : z[e];
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+        }
+    };
     // A split's sum is formed in passes (sgemm_route says how long they are), all but the last of which wait in `total` or in C.
     float top = 0.0f;   // NaN once anything is not finite: x * 0 is 0 for finite x only
 #pragma clang loop unroll(disable)
@@ -451,6 +497,10 @@ __global__ __launch_bounds__(kRowsThreads, 2) void sgemm_rows_k(Gemm p)
                     top = __fmaf_rn(acc[i][j][v], 0.0f, top);
                     acc[i][j][v] *= kSplitDown;
                 }
+        if (E::kOn && to == k_end && !__any(top != 0.0f)) {
+            put_dense(from != k_begin);
+            return;
+        }
         put(from != k_begin);
     }
     if (!__any(top != 0.0f)) return;
@@ -487,7 +537,10 @@ __global__ __launch_bounds__(kRowsThreads, 2) void sgemm_rows_k(Gemm p)
             for (int v = 0; v < 16; v++) {
                 const int m = m0 + wm * 32 * MI + i * 32 + acc_row(v, lane);
                 float *const c = outp + (size_t)(i * 32 + 4 * kh + 8 * (v >> 2) + (v & 3)) * p.N + 32 * j;
-                if (m < p.M && n0 + brow + 32 * j < p.N && *c * 0.0f != 0.0f) *c = acc[i][j][v];
+                if (m < p.M && n0 + brow + 32 * j < p.N) {
+                    if (*c * 0.0f != 0.0f) *c = acc[i][j][v];
+                    if constexpr (E::kOn) *c = ep(*c, c - p.C);
+                }
             }
 }
 
@@ -535,11 +588,11 @@ __device__ __forceinline__ float small_value(const float (&v)[4], int e, int kk,
 }
 
 // kCut: a k-contiguous operand's rows are no whole quads.
-template <bool kTA, bool kTB, bool kCut>
+template <bool kTA, bool kTB, bool kCut, class E = NoEpilogue>
 __device__ __forceinline__ void sgemm_small_body(int M, int N, int K, int lda, int ldb, int kslice, const float *A,
                                                  const float *B, float *C, const float *colbias, int bias_shift,
                                                  const float *rowvec, int relu, const float *mask, int bx, int by, int k0, int k1,
-                                                 float (*red)[32 * 33])
+                                                 float (*red)[32 * 33], const E &ep = E{})
 {
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, r = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // the same in every lane: loop bounds stay scalar
@@ -596,6 +649,7 @@ __device__ __forceinline__ void sgemm_small_body(int M, int N, int K, int lda, i
 #pragma unroll
         for (int w = 1; w < kSmallWaves; w++) sum += red[w][rr * 33 + cc];
         if (m0 + rr < M && n0 + cc < N) {
+            if constexpr (E::kOn) sum = ep(sum, (size_t)(m0 + rr) * N + n0 + cc);
             if (colbias) {   // one value per group of 2^bias_shift columns, times the row's factor when there is one
                 float add = colbias[(n0 + cc) >> bias_shift];
                 if (rowvec) add = __fmul_rn(rowvec[m0 + rr], add);   // rounded on its own, as the separate product is
@@ -619,6 +673,16 @@ __global__ __launch_bounds__(64 * kSmallWaves) void sgemm_small_k(int M, int N, 
     const int k0 = (int)blockIdx.z * kSmallWaves * kslice;
     sgemm_small_body<kTA, kTB, kCut>(M, N, K, lda, ldb, kslice, A, B, C + (size_t)blockIdx.z * M * N, colbias, bias_shift, rowvec, relu,
                                      mask, (int)blockIdx.x, (int)blockIdx.y, k0, min(K, k0 + kSmallWaves * kslice), red);
+}
+
+// A dense layer: x [M, K] times w [N, K] transposed, and its end.
+template <bool kCut>
+__global__ __launch_bounds__(64 * kSmallWaves) void sgemm_small_dense_k(int M, int N, int K, int kslice, const float *x, const float *w, float *y,
+                                                                         DenseEpilogue ep)
+{
+    __shared__ float red[kSmallWaves][32 * 33];
+    sgemm_small_body<false, true, kCut, DenseEpilogue>(M, N, K, K, K, kslice, x, w, y, nullptr, 0, nullptr, 0, nullptr, (int)blockIdx.x,
+                                                       (int)blockIdx.y, 0, K, red, ep);
 }
 
 // Short reductions over large outputs with both operands stored k-major (A as [K][M], B as [K][N]:
@@ -802,6 +866,21 @@ __global__ __launch_bounds__(256) void splitk_epilogue_k(size_t M, size_t N, int
     }
 }
 
+// ... and a dense layer's end.
+__global__ __launch_bounds__(256) void splitk_dense_k(size_t n, int splits, const float *partial, float *out, DenseEpilogue ep)
+{
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        float acc = 0.f;
+        const int last = splits - 1;
+        for (int s = 0; s < splits; s += 4) {
+            const float v0 = partial[(size_t)s * n + i], v1 = partial[(size_t)min(s + 1, last) * n + i];
+            const float v2 = partial[(size_t)min(s + 2, last) * n + i], v3 = partial[(size_t)min(s + 3, last) * n + i];
+            acc = (((acc + v0) + (s + 1 <= last ? v1 : 0.f)) + (s + 2 <= last ? v2 : 0.f)) + (s + 3 <= last ? v3 : 0.f);
+        }
+        out[i] = ep(acc, i);
+    }
+}
+
 // K == 1: C[m][n] = a[m] * b[n] -- the broadcast product.  One rounding per element, so a
 // product with 1.0f reproduces the broadcast value exactly.
 __global__ __launch_bounds__(256) void outer_k(size_t M, size_t N, const float *a, const float *b, float *c)
@@ -841,8 +920,8 @@ struct VectorEpilogue {   // + rowvec[row] * colbias[col >> shift], relu, mask, 
 // kSteps > 0: at most so many steps of 64, where all of the loops below is only what a wavefront has to go through.  Up to four one
 // after the other (3 000 000 rows of 2 steps 437 us with the loops, 314 so; 30000 of 64 6.7 and 4.5, of 129 7.7 and 5.4), more all
 // together (8333 rows of 512 4.5 us one after the other, 3.8 with the loops, 3.6 so; 6057 of 429 3.8, 3.8 and 3.1; 25648 of 272 9.1, 8.2 and 6.5).
-template <int kSteps>
-__global__ __launch_bounds__(256) void gemv_rows_k(size_t M, size_t K, const float *A, const float *b, float *c, VectorEpilogue ep)
+template <int kSteps, class E>
+__global__ __launch_bounds__(256) void gemv_rows_k(size_t M, size_t K, const float *A, const float *b, float *c, E ep)
 {
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= M) return;
@@ -1122,10 +1201,21 @@ namespace dopt {
 struct Extras {
     const float *mask = nullptr;
     bool written = false;   // see sgemm_route
+    const DenseEpilogue *dense = nullptr;   // of x w^T alone (transA = 0, transB = 1), instead of the others
 };
 
 // Whether a matrix times a vector finds the matrix stored row by row along the reduction (where both sides are vectors it does).
 bool gemv_by_rows(int transA, int transB, size_t M, size_t N) { return (N == 1 && !transA) || (M == 1 && transB) || (M == 1 && N == 1); }
+
+template <class E>
+void launch_gemv_rows(size_t R, size_t K, const float *mat, const float *vec, float *c, const E &ep)
+{
+    const dim3 grid((unsigned)ceil_div(R, (size_t)4));
+    if (K <= 256) hipLaunchKernelGGL((gemv_rows_k<4, E>), grid, dim3(256), 0, stream(), R, K, mat, vec, c, ep);
+    else if (K <= 384) hipLaunchKernelGGL((gemv_rows_k<6, E>), grid, dim3(256), 0, stream(), R, K, mat, vec, c, ep);
+    else if (K <= 512) hipLaunchKernelGGL((gemv_rows_k<8, E>), grid, dim3(256), 0, stream(), R, K, mat, vec, c, ep);
+    else hipLaunchKernelGGL((gemv_rows_k<0, E>), grid, dim3(256), 0, stream(), R, K, mat, vec, c, ep);
+}
 
 template <int kGroups, int kLive = kGemvSlice>
 void launch_gemv_groups(int K, int N, size_t slices, const float *a, const float *B, float *c, const VectorEpilogue &ep)
@@ -1165,25 +1255,27 @@ struct Route {
     size_t bm = 128, bn = 128;   // the tile engines' tile (no part of the order: every tile of a kind adds its elements' terms alike)
 };
 
-template <class T, bool kTA, bool kTB, bool kCut>
-int rows_launch_one(dim3 grid, const Gemm &g)
+template <class T, bool kTA, bool kTB, bool kCut, class E>
+int rows_launch_one(dim3 grid, const Gemm &g, const E &ep)
 {
     static bool raised = false;   // above 64 KB of dynamic LDS a kernel has to be told once
     if (!raised)
-        DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)sgemm_rows_k<T, kTA, kTB, kCut>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)sgemm_rows_k<T, kTA, kTB, kCut, E>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                            2 * T::kBuf));
     raised = true;
-    hipLaunchKernelGGL((sgemm_rows_k<T, kTA, kTB, kCut>), grid, dim3(kRowsThreads), 2 * T::kBuf, stream(), g);
+    hipLaunchKernelGGL((sgemm_rows_k<T, kTA, kTB, kCut, E>), grid, dim3(kRowsThreads), 2 * T::kBuf, stream(), g, ep);
     return DOPT_HIP_OK;
 }
 
-template <bool kTA, bool kTB, bool kCut>
-int rows_launch(const Route &r, dim3 grid, const Gemm &g)
+template <bool kTA, bool kTB, bool kCut, class E = NoEpilogue>
+int rows_launch(const Route &r, dim3 grid, const Gemm &g, const E &ep = E{})
 {
-    if (r.bm == 256 && r.bn == 256) return rows_launch_one<RowsTile<2, 4, 4, 2>, kTA, kTB, kCut>(grid, g);
-    if (r.bm == 256) return rows_launch_one<RowsTile<4, 2, 2, 2>, kTA, kTB, kCut>(grid, g);
-    if (r.bn == 256) return rows_launch_one<RowsTile<2, 4, 2, 2>, kTA, kTB, kCut>(grid, g);
-    return rows_launch_one<RowsTile<2, 4, 2, 1>, kTA, kTB, kCut>(grid, g);
+    if constexpr (!E::kOn) {
+        if (r.bm == 256 && r.bn == 256) return rows_launch_one<RowsTile<2, 4, 4, 2>, kTA, kTB, kCut>(grid, g, ep);
+    }
+    if (r.bm == 256) return rows_launch_one<RowsTile<4, 2, 2, 2>, kTA, kTB, kCut>(grid, g, ep);
+    if (r.bn == 256) return rows_launch_one<RowsTile<2, 4, 2, 2>, kTA, kTB, kCut>(grid, g, ep);
+    return rows_launch_one<RowsTile<2, 4, 2, 1>, kTA, kTB, kCut>(grid, g, ep);
 }
 
 
@@ -1355,11 +1447,8 @@ int sgemm_epilogue(int transA, int transB, size_t M, size_t N, size_t K, const f
         const VectorEpilogue ep{colbias, rowvec, ex.mask, bias_shift, relu, N}, none{nullptr, nullptr, nullptr, 0, 0, 1};
         *biased = true;
         if (gemv_by_rows(transA, transB, M, N)) {
-            const dim3 grid((unsigned)ceil_div(R, (size_t)4));
-            if (K <= 256) hipLaunchKernelGGL(gemv_rows_k<4>, grid, dim3(256), 0, stream(), R, K, mat, vec, C, ep);
-            else if (K <= 384) hipLaunchKernelGGL(gemv_rows_k<6>, grid, dim3(256), 0, stream(), R, K, mat, vec, C, ep);
-            else if (K <= 512) hipLaunchKernelGGL(gemv_rows_k<8>, grid, dim3(256), 0, stream(), R, K, mat, vec, C, ep);
-            else hipLaunchKernelGGL(gemv_rows_k<0>, grid, dim3(256), 0, stream(), R, K, mat, vec, C, ep);
+            if (ex.dense) launch_gemv_rows(R, K, mat, vec, C, *ex.dense);
+            else launch_gemv_rows(R, K, mat, vec, C, ep);
             DOPT_LAUNCH_CHECK();
             return DOPT_HIP_OK;
         }
@@ -1390,13 +1479,19 @@ int sgemm_epilogue(int transA, int transB, size_t M, size_t N, size_t K, const f
                        A, B, to, fused ? colbias : nullptr, bias_shift, fused ? rowvec : nullptr, fused ? relu : 0,      \
                        fused ? ex.mask : nullptr)
         const bool cut = K % 4 != 0;
-        if (transA && transB) { if (cut) DOPT_SMALL(true, true, true); else DOPT_SMALL(true, true, false); }
+        if (ex.dense && fused) {
+            if (cut) hipLaunchKernelGGL(sgemm_small_dense_k<true>, grid, block, 0, stream(), (int)M, (int)N, (int)K, kslice, A, B, C, *ex.dense);
+            else hipLaunchKernelGGL(sgemm_small_dense_k<false>, grid, block, 0, stream(), (int)M, (int)N, (int)K, kslice, A, B, C, *ex.dense);
+        } else if (transA && transB) { if (cut) DOPT_SMALL(true, true, true); else DOPT_SMALL(true, true, false); }
         else if (transA) DOPT_SMALL(true, false, false);   // nothing k-contiguous to cut
         else if (transB) { if (cut) DOPT_SMALL(false, true, true); else DOPT_SMALL(false, true, false); }
         else { if (cut) DOPT_SMALL(false, false, true); else DOPT_SMALL(false, false, false); }
 #undef DOPT_SMALL
         DOPT_LAUNCH_CHECK();
-        if (!fused) {
+        if (!fused && ex.dense) {
+            hipLaunchKernelGGL(splitk_dense_k, dim3(flat_grid(M * N)), dim3(256), 0, stream(), M * N, (int)cuts, to, C, *ex.dense);
+            DOPT_LAUNCH_CHECK();
+        } else if (!fused) {
             hipLaunchKernelGGL(splitk_epilogue_k, dim3(flat_grid(M * N)), dim3(256), 0, stream(), M, N, (int)cuts, to, C, colbias,
                                bias_shift, rowvec, relu, ex.mask);
             DOPT_LAUNCH_CHECK();
@@ -1446,6 +1541,15 @@ int sgemm_epilogue(int transA, int transB, size_t M, size_t N, size_t K, const f
     } while (0)
     if (kind == Route::kRows || kind == Route::kRowsBig) {
         const bool cut = K % 4 != 0;
+        // (the largest tile has no registers left for it: with 150 of them spilled [8192 x 4096] from 4096 steps took 1520 us, with a pass
+        // behind the product 1425)
+        if (ex.dense && splits == 1 && kind == Route::kRows) {
+            if (int rc = cut ? rows_launch<false, true, true>(route, grid, g, *ex.dense) : rows_launch<false, true, false>(route, grid, g, *ex.dense))
+                return rc;
+            *biased = true;
+            DOPT_LAUNCH_CHECK();
+            return DOPT_HIP_OK;
+        }
 #define DOPT_ROWS(TA, TB)                                                                                \
     do {                                                                                                 \
         if (int rc = cut ? rows_launch<TA, TB, true>(route, grid, g) : rows_launch<TA, TB, false>(route, grid, g)) return rc; \
@@ -1460,7 +1564,11 @@ int sgemm_epilogue(int transA, int transB, size_t M, size_t N, size_t K, const f
 #undef DOPT_SGEMM_T
 #undef DOPT_SGEMM
     DOPT_LAUNCH_CHECK();
-    if (splits > 1) {
+    if (splits > 1 && ex.dense) {
+        hipLaunchKernelGGL(splitk_dense_k, dim3(flat_grid(g.out_elems)), dim3(256), 0, stream(), g.out_elems, splits, partial, C, *ex.dense);
+        DOPT_LAUNCH_CHECK();
+        *biased = true;
+    } else if (splits > 1) {
         hipLaunchKernelGGL(splitk_reduce_k, dim3(flat_grid(g.out_elems)), dim3(256), 0, stream(), g.out_elems, splits,
                            partial, C);
         DOPT_LAUNCH_CHECK();
@@ -1598,6 +1706,15 @@ int product_relu_grad(bool written, int transA, int transB, size_t M, size_t N, 
     if (int rc = sgemm_epilogue(transA, transB, M, N, K, A, B, C, nullptr, 0, nullptr, 0, &applied, ex)) return rc;
     if (applied || M * N == 0) return DOPT_HIP_OK;
     return dopt_hip_relu_bwd(M * N, C, x, C);   // in place: every element is read before it is written
+}
+
+int product_dense(size_t M, size_t N, size_t K, const float *x, const float *w, const DenseEpilogue &e, float *y)
+{
+    Extras ex;
+    ex.dense = &e;
+    bool applied = false;
+    if (int rc = sgemm_epilogue(0, 1, M, N, K, x, w, y, nullptr, 0, nullptr, 0, &applied, ex)) return rc;
+    return applied ? DOPT_HIP_OK : dense_finish(M, N, e, y);
 }
 
 size_t product_scratch(int transA, int transB, size_t M, size_t N, size_t K)
