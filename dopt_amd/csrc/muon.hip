@@ -113,6 +113,7 @@ struct Handle {
     Matrix *d_jobs = nullptr;
     Tile *chunks = nullptr, *scales = nullptr, *grams = nullptr, *meets = nullptr, *squares = nullptr, *wides = nullptr;   // device
     unsigned nchunks = 0, nscales = 0, ngrams = 0, nmeets = 0, nsquares = 0, nwides = 0;
+    bool small = false;   // no shorter side of more than 64
 };
 
 __device__ __forceinline__ float step_value(float g, float m, const Step &st) { return st.nesterov ? g + st.mu * m : m; }
@@ -600,6 +601,73 @@ __global__ __launch_bounds__(kBlock) void muon_meet_k(const Matrix *jobs, const 
     finish<kGram>(t, ops.op[0], 0, sum, Old{}, t.i * 64 + (w >> 1) * 32, t.j * 64 + (w & 1) * 32, lane, images + w * 8192);
 }
 
+// The square products of a group of iterations for matrices whose shorter side is at most 64: everything in one workgroup's LDS, a
+// product and a barrier after the other, where thirteen launches of a tile each took 3.6 us.  Adds the parts of A first; the
+// last product goes to memory.
+constexpr int kChainOps = 16;
+struct Chain {
+    SquareOp op[kChainOps];
+    int n, a, q;   // how many; where A goes, and which one is wanted
+};
+__global__ __launch_bounds__(kBlock) void muon_chain_k(const Matrix *jobs, const Tile *tiles, Chain ch)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];   // kSquares matrices of 16 KB: four blocks along, two down
+    const Tile t = tiles[blockIdx.x];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w >> 1, wn = w & 1;
+    const int c = lane & 31, half = lane >> 5;
+    // (row, col) lies in blocks 4 (row / 32) + col / 16; what is below the diagonal is stored twice, what is above not formed
+    auto store = [&](char *to, const v16f &acc, float alpha, float beta, const char *old, float gamma) {
+        if (wm < wn) return;
+        char *const across = to + wn * 8192 + wm * 4096, *const along = to + wm * 8192 + wn * 4096;
+        const char *const at = old + wn * 8192 + wm * 4096;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int r = 8 * g + 4 * half, place = (g >> 1) * 2048 + 8 * half;
+            const int hp = piece_at(c, 2 * (g & 1)), lp = piece_at(c, 2 * (g & 1) + 1);
+            float o[4], v[4];
+            join4(*(const v2u *)(at + place + hp), *(const v2u *)(at + place + lp), o);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = acc[4 * g + e] * alpha + (beta * o[e] + (wm == wn && r + e == c ? gamma : 0.0f));
+            v2u h, l;
+            split4(v, h, l);
+            put_part(across, c, 2 * g, half, h);
+            put_part(across, c, 2 * g + 1, half, l);
+            if (wm == wn) continue;
+            put_part(along, r + (lane & 3), 2 * (c >> 3), (c >> 2) & 1, transpose4(h, lane));
+            put_part(along, r + (lane & 3), 2 * (c >> 3) + 1, (c >> 2) & 1, transpose4(l, lane));
+        }
+    };
+    {   // A: the sum of its parts
+        const Global<const v4f> from = (Global<const v4f>)global((const float4 *)jobs[t.job].partial) + ((size_t)t.slot * 1024 + w * 256 + lane);
+        v16f sum;
+#pragma unroll
+        for (int g = 0; g < 4; g++) set_quad(sum, g, v4f{0.0f, 0.0f, 0.0f, 0.0f});
+        for (int p = 0; p < t.parts; p++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) set_quad(sum, g, quad_of(sum, g) + from[p * 1024 + g * 64]);
+        // (beta is zero: what is read beside it only has to be a number)
+        for (int i = threadIdx.x; i < kSquares * 1024; i += kBlock) ((v4u *)lds)[i] = v4u{0, 0, 0, 0};
+        meet();
+        store(lds + ch.a * 16384, sum, ch.op[0].gamma, 0.0f, lds + ch.a * 16384, 0.0f);
+    }
+    for (int k = 1; k < ch.n; k++) {
+        meet();
+        const SquareOp op = ch.op[k];
+        v16f acc[1][1];
+        zero_acc(acc);
+        if (wm >= wn) {
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+                multiply(lds + op.l * 16384 + wm * 8192 + s * 2048, lds + op.r * 16384 + wn * 8192 + s * 2048, lane, acc);
+        }
+        store(lds + op.d * 16384, acc[0][0], op.alpha, op.beta, lds + op.c * 16384, op.gamma);
+    }
+    meet();
+    const Global<char> to = global(t.square(ch.q));
+#pragma unroll
+    for (int i = 0; i < 4; i++) *(Global<v4u>)(to + (i * kBlock + threadIdx.x) * 16) = *(const v4u *)(lds + ch.q * 16384 + (i * kBlock + threadIdx.x) * 16);
+}
+
 // No iterations: w moves along X itself.
 __global__ __launch_bounds__(kBlock) void muon_plain_k(const Matrix *jobs, const Tile *chunks, Step st)
 {
@@ -651,6 +719,7 @@ int build(Handle *h)
     auto take = [&](size_t n) { const size_t at = bytes; bytes += ceil_div(n, (size_t)256) * 256; return at; };
     std::vector<size_t> x_at, sq_at, partial_at, parts_at;
     size_t all = 0, mids = 0;   // stages of all tiles of A; 128 x 128 tiles of square matrices
+    h->small = true;
     for (Matrix &q : h->jobs) {
         q.tall = q.rows > q.cols;
         q.s = std::min(q.rows, q.cols);
@@ -664,9 +733,10 @@ int build(Handle *h)
         const size_t t = q.sp / side, tiles = t * (t + 1) / 2;
         all += tiles * (q.lp / 32) * (side / 64);   // (a stage of a 128 x 128 tile is 16 steps)
         mids += side == 128 ? tiles : 0;
+        h->small = h->small && side == 64;
     }
     // A's reduction is cut so that two workgroups for each CU have about the same to do
-    const size_t part = std::max((size_t)32, ceil_div(all, (size_t)num_cus() * 2));
+    const size_t part = std::max((size_t)(h->small ? 4 : 32), ceil_div(all, (size_t)num_cus() * 2));
     auto cuts_of = [&](const Matrix &q) { return (int)ceil_div((size_t)q.lp / 32 * (q.sp == 64 ? 1 : 2), part); };
     // 64 x 64 tiles spread a short product over more CUs, 128 x 128 tiles take half the operands' traffic: 13 products of [512 x 512] ..
     const bool mid_squares = mids >= (size_t)num_cus() * 2;
@@ -674,7 +744,7 @@ int build(Handle *h)
         const size_t side = q.sp == 64 ? 64 : 128, t = q.sp / side, cuts = cuts_of(q);
         x_at.push_back(take((size_t)q.sp * q.lp * 4 * 4));
         sq_at.push_back(take((size_t)q.sp * q.sp * 4 * kSquares));
-        partial_at.push_back(take(cuts > 1 ? cuts * t * (t + 1) / 2 * side * side * sizeof(float) : 0));
+        partial_at.push_back(take(cuts > 1 || h->small ? cuts * t * (t + 1) / 2 * side * side * sizeof(float) : 0));
         parts_at.push_back(take((size_t)q.nparts * sizeof(double)));
     }
     const size_t tables_at = bytes;
@@ -701,7 +771,7 @@ int build(Handle *h)
         for (int i = 0; i < q.sp / side; i++)
             for (int j = 0; j <= i; j++) {
                 Tile g = at(i, j);
-                if (cuts > 1) {   // its quarters of 64 x 64, on and below the diagonal
+                if (cuts > 1 || h->small) {   // its quarters of 64 x 64, on and below the diagonal
                     g.parts = cuts;
                     for (int p = 0; p < (small ? 1 : 4); p++) {
                         g.slot = slots + p;
@@ -714,7 +784,7 @@ int build(Handle *h)
                 for (int c = 0; c < cuts; c++) {
                     g.from = (int)((size_t)deep * c / cuts);
                     g.to = (int)((size_t)deep * (c + 1) / cuts);
-                    if (cuts > 1) {
+                    if (cuts > 1 || h->small) {
                         g.slot = slots;
                         slots += small ? 1 : 4;
                     }
@@ -794,23 +864,17 @@ struct Buffers {
     }
 };
 
-// `count` iterations on X[turn]: into X[turn ^ 1], or into w.
-int iterate(const Handle *h, const Step &st, int count, int turn, bool last)
+// The square products of `count` iterations, in their order: f(operations, how many of them do not wait for each other).  Returns where
+// Q is left.
+template <class F>
+int squares_of(int count, Buffers &b, int a, F &&f, int *q_out)
 {
-    Buffers b;
-    auto squares = [&](const SquareOps &ops, unsigned n) { return launch<kSquare>(h, h->nsquares, n, h->squares, st, ops, turn); };
-    int a = b.take(kScaleBits), q = -1;
     SquareOps ops{};
-    ops.op[0] = SquareOp{0, 0, a, 0, std::ldexp(1.0f, -kScaleBits), 0.0f, 0.0f};
-    if (int rc = launch<kGram>(h, h->ngrams, 1, h->grams, st, ops, turn)) return rc;
-    if (h->nmeets) {
-        hipLaunchKernelGGL(muon_meet_k, dim3(h->nmeets), dim3(kBlock), 0, stream(), h->d_jobs, h->meets, ops);
-        DOPT_LAUNCH_CHECK();
-    }
+    int q = -1;
     for (int k = 0; k < count; k++) {
         const int p = b.take(kScaleBits);
         ops.op[0] = b.op(kC, a, a, kB, a, kA, p);   // P
-        if (int rc = squares(ops, 1)) return rc;
+        if (int rc = f(ops, 1)) return rc;
         unsigned n = 0;
         const int before = q;
         if (q >= 0) {   // Q <- P Q
@@ -823,20 +887,62 @@ int iterate(const Handle *h, const Step &st, int count, int turn, bool last)
         if (k + 1 < count) {   // A <- P A P
             const int t = b.take(kScaleBits);
             ops.op[n++] = b.op(1.0f, p, a, 0.0f, a, 0.0f, t);
-            if (int rc = squares(ops, n)) return rc;
+            if (int rc = f(ops, n)) return rc;
             const int next = b.take(kScaleBits);
             ops.op[0] = b.op(1.0f, t, p, 0.0f, a, 0.0f, next);
-            if (int rc = squares(ops, 1)) return rc;
+            if (int rc = f(ops, 1)) return rc;
             b.drop(a);
             b.drop(t);
             a = next;
         } else if (n) {
-            if (int rc = squares(ops, n)) return rc;
+            if (int rc = f(ops, n)) return rc;
         }
         if (before >= 0) {
             b.drop(before);
             b.drop(p);
         }
+    }
+    *q_out = q;
+    return DOPT_HIP_OK;
+}
+
+// `count` iterations on X[turn]: into X[turn ^ 1], or into w.
+int iterate(const Handle *h, const Step &st, int count, int turn, bool last)
+{
+    Buffers b;
+    const int a = b.take(kScaleBits);
+    int q = a;
+    SquareOps ops{};
+    const float alpha = std::ldexp(1.0f, -kScaleBits);
+    ops.op[0] = SquareOp{0, 0, a, 0, alpha, 0.0f, 0.0f};
+    if (int rc = launch<kGram>(h, h->ngrams, 1, h->grams, st, ops, turn)) return rc;
+    if (h->small) {
+        Chain ch{};
+        ch.a = a;
+        ch.op[ch.n++].gamma = alpha;
+        static_assert(1 + 3 * kGroup + (kGroup - 1) <= kChainOps, "an iteration has up to four products");
+        if (int rc = squares_of(
+                count, b, a,
+                [&](const SquareOps &o, unsigned n) {
+                    for (unsigned i = 0; i < n; i++) ch.op[ch.n++] = o.op[i];
+                    return (int)DOPT_HIP_OK;
+                },
+                &q))
+            return rc;
+        ch.q = q;
+        static bool raised = false;
+        if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)muon_chain_k, hipFuncAttributeMaxDynamicSharedMemorySize, kSquares * 16384));
+        raised = true;
+        hipLaunchKernelGGL(muon_chain_k, dim3(h->nmeets), dim3(kBlock), kSquares * 16384, stream(), h->d_jobs, h->meets, ch);
+        DOPT_LAUNCH_CHECK();
+    } else {
+        if (h->nmeets) {
+            hipLaunchKernelGGL(muon_meet_k, dim3(h->nmeets), dim3(kBlock), 0, stream(), h->d_jobs, h->meets, ops);
+            DOPT_LAUNCH_CHECK();
+        }
+        if (int rc = squares_of(
+                count, b, a, [&](const SquareOps &o, unsigned n) { return launch<kSquare>(h, h->nsquares, n, h->squares, st, o, turn); }, &q))
+            return rc;
     }
     ops.op[0] = SquareOp{q, 0, 0, 0, std::ldexp(1.0f, (last ? -kScaleBits : 0) - b.bits[q]), 0.0f, 0.0f};
     return last ? launch<kLast>(h, h->nwides, 1, h->wides, st, ops, turn) : launch<kApply>(h, h->nwides, 1, h->wides, st, ops, turn);
