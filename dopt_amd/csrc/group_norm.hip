@@ -7,10 +7,10 @@
 //     dx = rstd (dz scale[c] - s1 - xhat s2),  s1, s2 the group's means of dz scale and dz scale xhat
 //
 // All of it is bound by memory: 8 bytes a value forward, 12 backward.  A group of an [N, C, inner] tensor lies in one piece, and up to
-// 32768 values of it stay in the registers of one workgroup, which so reads and writes everything once.  Longer groups, and
-// those of too few samples to fill the chip, are parted: a first launch leaves each part's statistics (or sums), a second one joins
-// them and reads the part again.  Channels-last groups lie in pieces of C / G values: workgroups take runs of pixels with all their
-// channels, in two launches likewise.  Means are taken before variances everywhere - of a part in registers, then of the parts - so
+// 32768 values of it (of the gradient 16384 of both tensors) stay in the registers of one workgroup, which so reads and writes everything
+// once.  Longer groups are parted: a first launch leaves each part's statistics (or sums), a second one joins them and reads the part again.
+// Channels-last groups lie in pieces of C / G values; those of 32 bytes and more are held likewise, otherwise workgroups take
+// runs of pixels with all their channels, in two launches.  Means are taken before variances everywhere - of a part in registers, then of the parts - so
 // nothing cancels however far from zero the values lie.  No atomics: every sum has one order.
 #include <algorithm>
 #include <type_traits>
@@ -649,6 +649,127 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
     }
 }
 
+// ------------------------------------------------------------------------------- [N, inner, C], a group in one workgroup
+
+// Groups of 8 to 64 channels, a power of two of them: `1 << bits` threads to a pixel's quads, and the group's values in registers as above.
+// A pixel's piece may be less than a line of 128 bytes, which then belongs to several groups: blocks of one XCD, whose L2
+// holds it meanwhile, take groups that lie side by side.
+struct Held {
+    size_t C, inner;
+    int Cg, G, bits;
+    unsigned groups, per;   // all of them, an XCD's
+};
+__device__ __forceinline__ size_t held_group(const Held &h) { return (size_t)(blockIdx.x & 7) * h.per + (blockIdx.x >> 3); }
+
+template <int kQ>
+__global__ __launch_bounds__(1024) void gn_held_fwd_k(Held h, float eps, int act, const float *x, const float *scale, const float *bias, float *y,
+                                                      float *means, float *rstds)
+{
+    __shared__ float red[16];
+    const size_t group = held_group(h);
+    if (group >= h.groups) return;
+    const int quad = threadIdx.x & ((1 << h.bits) - 1), row = threadIdx.x >> h.bits, rows = blockDim.x >> h.bits, last = (int)h.inner - 1;
+    const int c = (int)(group % h.G) * h.Cg + 4 * quad;
+    const size_t base = group / h.G * h.inner * h.C + c;
+    v4f v[kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; i++) v[i] = load4(x + base + (size_t)min(row + i * rows, last) * h.C);
+    const v4f a0 = load4(scale + c), b = load4(bias + c);
+    const float total = (float)h.Cg * (float)h.inner;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kQ; i++) s += own_sum(v[i], row + i * rows <= last ? 0 : 4);
+    const float mean = block_sum(s, red) / total;
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kQ; i++) {
+        const v4f d = v[i] - mean;
+        q += own_sum(d * d, row + i * rows <= last ? 0 : 4);
+    }
+    const float rstd = 1.0f / sqrtf(block_sum(q, red) / total + eps);
+    if (threadIdx.x == 0) {
+        means[group] = mean;
+        rstds[group] = rstd;
+    }
+    const v4f a = rstd * a0;
+    with_activation(act, [&](auto kind) {
+#pragma unroll
+        for (int i = 0; i < kQ; i++) {
+            v4f o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = act_value<kind.value>((v[i][e] - mean) * a[e] + b[e]);
+            if (row + i * rows <= last) store4(y + base + (size_t)(row + i * rows) * h.C, o);
+        }
+    });
+}
+
+// `sums`: of dz and dz xhat over each sample's channels.
+template <int kQ>
+__global__ __launch_bounds__(1024) void gn_held_bwd_k(Held h, int act, const float *dy, const float *x, const float *scale, const float *bias,
+                                                      const float *means, const float *rstds, float2 *sums, float *dx)
+{
+    __shared__ float red[16];
+    __shared__ float2 waves[16][64];
+    const size_t group = held_group(h);
+    if (group >= h.groups) return;
+    const int quad = threadIdx.x & ((1 << h.bits) - 1), row = threadIdx.x >> h.bits, rows = blockDim.x >> h.bits, last = (int)h.inner - 1;
+    const int c = (int)(group % h.G) * h.Cg + 4 * quad;
+    const size_t base = group / h.G * h.inner * h.C + c;
+    v4f v[kQ], d[kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; i++) {
+        const size_t at = base + (size_t)min(row + i * rows, last) * h.C;
+        v[i] = load4(x + at);
+        d[i] = load4(dy + at);
+    }
+    const v4f a = load4(scale + c), b = load4(bias + c);
+    const float mean = means[group], rstd = rstds[group];
+    v4f t{0.0f, 0.0f, 0.0f, 0.0f}, u = t;
+    with_activation(act, [&](auto kind) {
+#pragma unroll
+        for (int i = 0; i < kQ; i++) {
+            const bool own = row + i * rows <= last;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[i][e] = (v[i][e] - mean) * rstd;
+                d[i][e] = act_grad<kind.value>(d[i][e], v[i][e] * a[e] + b[e]);
+                t[e] += own ? d[i][e] : 0.0f;
+                u[e] += own ? d[i][e] * v[i][e] : 0.0f;
+            }
+        }
+    });
+#pragma unroll
+    for (int e = 0; e < 4; e++)   // the wavefront's pixels, then the wavefronts
+        for (int m = 32; m >> h.bits; m >>= 1) {
+            t[e] += __shfl_xor(t[e], m, 64);
+            u[e] += __shfl_xor(u[e], m, 64);
+        }
+    if ((threadIdx.x & 63) == quad) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) waves[threadIdx.x >> 6][4 * quad + e] = make_float2(t[e], u[e]);
+    }
+    meet();
+    float s1 = 0.0f, s2 = 0.0f;
+    if ((int)threadIdx.x < h.Cg) {
+        float2 o = waves[0][threadIdx.x];
+        for (unsigned i = 1; i < blockDim.x / 64; i++) o = make_float2(o.x + waves[i][threadIdx.x].x, o.y + waves[i][threadIdx.x].y);
+        const size_t at = group % h.G * h.Cg + threadIdx.x;
+        sums[group / h.G * h.C + at] = o;
+        s1 = scale[at] * o.x;
+        s2 = scale[at] * o.y;
+    }
+    const float total = (float)h.Cg * (float)h.inner;
+    s1 = block_sum(s1, red) / total;
+    s2 = block_sum(s2, red) / total;
+#pragma unroll
+    for (int i = 0; i < kQ; i++) {
+        v4f o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = rstd * (d[i][e] * a[e] - s1 - v[i][e] * s2);
+        if (row + i * rows <= last) store4(dx + base + (size_t)(row + i * rows) * h.C, o);
+    }
+}
+
 // ------------------------------------------------------------------------------- one value to a channel: rows of a dense layer
 
 constexpr int kRowValues = 16;   // of a lane: groups of up to 1024 channels
@@ -846,23 +967,29 @@ __global__ __launch_bounds__(kBlock) void gn_any_dx_k(Place p, int act, const fl
 
 // ------------------------------------------------------------------------------- which of them
 
-// How a workgroup holds `channels` channels of `len` values: threads (0: it cannot), channels and quads of a thread.
+// The most quads that a thread holds of a tensor: 1024 threads leave each 128 registers, of which the gradient's eight quads of both its
+// tensors spilled 800 values ([64, 512, 32 x 32] in 16 groups, whole: 361 us, in parts 134).
+constexpr int kMost = 8, kMostGrad = 4;
+
+// How a workgroup holds `channels` channels of `len` values, up to `most` quads to a thread: threads (0: it cannot), channels and quads
+// of a thread.
 struct Hold {
     int threads = 0, c = 1, q = 1, P = 1, rows = 1;
 };
-Hold hold_for(int channels, size_t len)
+Hold hold_for(int channels, size_t len, int most)
 {
     Hold best;
     size_t least = 0;
     const size_t quads = ceil_div(len, (size_t)4);
-    for (int q = 1; q <= 8; q *= 2)
-        for (int c = 1; c * q <= 8; c *= 2) {
+    for (int q = 1; q <= most; q *= 2)
+        for (int c = 1; c * q <= most; c *= 2) {
             int P = 1;
             while ((size_t)P * q < quads && P <= 1024) P *= 2;
             const int rows = (channels + c - 1) / c, threads = (int)ceil_div((size_t)rows * P, (size_t)64) * 64;
             if (P > 1024 || rows > 1024 || threads > 1024) continue;
-            // places that stay empty cost what full ones do; four quads to a thread keep enough loads on their way
-            const size_t cost = (size_t)threads * c * q * 16 + (size_t)std::abs(c * q - 4) * threads;
+            // Places that stay empty cost what full ones do.  Four quads of one tensor to a thread, two of two, and more wavefronts with the
+            // registers that this saves: the gradient of [128, 320, 16 x 16] in sixteen groups takes 38.5 us with two, 48.1 with four.
+            const size_t cost = (size_t)threads * (c * q * 16 + std::abs(c * q - most / 2) * 4);
             if (best.threads && cost >= least) continue;
             least = cost;
             best.threads = threads;
@@ -880,7 +1007,7 @@ struct Split {
     Hold h;
     bool whole;
 };
-Split split_of(size_t N, size_t C, size_t inner, size_t G)
+Split split_of(size_t C, size_t inner, size_t G, int most)
 {
     Split r;
     Sizes &s = r.s;
@@ -892,29 +1019,62 @@ Split split_of(size_t N, size_t C, size_t inner, size_t G)
     s.per = s.Cg;
     s.parts = 1;
     const size_t L = C / G * inner;
-    r.h = L <= 32768 ? hold_for(s.Cg, inner) : Hold{};
-    // a few long groups leave most of the chip idle: [1, 64, 64 x 64] in two groups ..
-    r.whole = r.h.threads && (L <= kPiece || N * G * 2 > (size_t)num_cus());
+    r.h = L <= (size_t)4096 * most ? hold_for(s.Cg, inner, most) : Hold{};
+    // (also where a few of them leave most of the chip idle: sixteen of 32768 values take 8.9 us, in parts 9.2; 128 of them 11.3 and 14.2)
+    r.whole = r.h.threads != 0;
     if (!r.whole) {
         s.pieces = (int)ceil_div(inner, (size_t)kPiece);
         s.per = s.pieces > 1 ? 1 : std::max(1, std::min(s.Cg, (int)(kPiece / inner)));
         s.parts = s.pieces * (int)ceil_div((size_t)s.Cg, (size_t)s.per);
-        r.h = hold_for(s.per, ceil_div(inner, (size_t)s.pieces));
+        r.h = hold_for(s.per, ceil_div(inner, (size_t)s.pieces), most);
     }
     s.P = r.h.P;
     s.rows = r.h.rows;
     return r;
 }
 
-template <class F>
+template <int kMax, class F>
 int with_hold(const Hold &h, F &&f)
 {
 #define DOPT_HOLD(C, Q) \
-    if (h.c == C && h.q == Q) return f(std::integral_constant<int, C>{}, std::integral_constant<int, Q>{});
+    if constexpr (C * Q <= kMax) \
+        if (h.c == C && h.q == Q) return f(std::integral_constant<int, C>{}, std::integral_constant<int, Q>{});
     DOPT_HOLD(1, 1) DOPT_HOLD(1, 2) DOPT_HOLD(1, 4) DOPT_HOLD(1, 8) DOPT_HOLD(2, 1)
     DOPT_HOLD(2, 2) DOPT_HOLD(2, 4) DOPT_HOLD(4, 1) DOPT_HOLD(4, 2) DOPT_HOLD(8, 1)
 #undef DOPT_HOLD
     return fail(DOPT_HIP_ERR_UNSUPPORTED, "group norm: no kernel holds such a group");
+}
+
+// Channels-last groups in registers: threads (0: not these), quads of a thread.
+struct HeldHold {
+    Held h;
+    int threads = 0, q = 1;
+};
+HeldHold held_for(size_t N, size_t C, size_t inner, size_t G, bool grad)
+{
+    HeldHold r;
+    const int most = grad ? kMostGrad : kMost;
+    const size_t Cg = C / G;
+    if (Cg < 8 || Cg > 64 || (Cg & (Cg - 1)) || Cg * inner > (size_t)4096 * most) return r;
+    // The gradient's runs read everything twice, but the second time from a cache of 256 MB, and in whole lines.  In registers [64, 1024, 128]
+    // in 16 groups takes 37.8 us, by runs 32.0; four times as many samples 116 and 134; [37, 957, 200] in 25 groups
+    // 29.3 and 30.7; [8, 256, 256] in 32 groups 9.2 and 11.0; [8, 2048, 64] in 8 groups 12.3 and 10.7.  Forward, where [64, 1024, 128]
+    // takes 16.6 and 23.7 us, registers win throughout.
+    const size_t in = 2 * N * C * inner * sizeof(float);
+    if (grad && in < (size_t)200 << 20 && (in > (size_t)60 << 20 || Cg * inner > kPiece)) return r;
+    r.h = Held{C, inner, (int)Cg, (int)G, 0, (unsigned)(N * G), (unsigned)ceil_div(N * G, (size_t)8)};
+    while ((size_t)4 << r.h.bits < Cg) r.h.bits++;
+    size_t least = 0;
+    for (int q = 1; q <= most; q *= 2) {
+        const size_t threads = ceil_div(ceil_div(inner, (size_t)q) << r.h.bits, (size_t)64) * 64;
+        if (threads > 1024) continue;
+        const size_t cost = threads * (q * 16 + std::abs(q - 4) * 4);   // as in hold_for
+        if (r.threads && cost >= least) continue;
+        least = cost;
+        r.threads = (int)threads;
+        r.q = q;
+    }
+    return r;
 }
 
 constexpr size_t kLastChannels = 8192;   // LDS of a run of pixels
@@ -931,6 +1091,15 @@ Rows rows_of(size_t N, size_t C, size_t inner, size_t G, int V)
     const size_t most = std::min((size_t)kRuns, ceil_div(inner, (size_t)r.R * 8));   // (eight pixels to a thread)
     r.S = (int)std::min(most, std::max((size_t)1, ceil_div((size_t)num_cus() * 4, N)));
     return r;
+}
+
+template <int kMax, class F>
+int with_quads(int q, F &&f)
+{
+    if (q == 1) return f(std::integral_constant<int, 1>{});
+    if (q == 2) return f(std::integral_constant<int, 2>{});
+    if (q == 4 || kMax == 4) return f(std::integral_constant<int, 4>{});
+    return f(std::integral_constant<int, kMax>{});
 }
 
 template <class F>
@@ -972,6 +1141,14 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
         DOPT_LAUNCH_CHECK();
         return DOPT_HIP_OK;
     }
+    const HeldHold held = channels_last && inner > 1 ? held_for(N, C, inner, G, false) : HeldHold{};
+    if (held.threads)
+        return with_quads<kMost>(held.q, [&](auto q) -> int {
+            hipLaunchKernelGGL(gn_held_fwd_k<decltype(q)::value>, dim3(8 * held.h.per), dim3(held.threads), 0, stream(), held.h, eps, act, x, scale,
+                               bias, y, means, rstds);
+            DOPT_LAUNCH_CHECK();
+            return DOPT_HIP_OK;
+        });
     if (channels_last && inner > 1 && C <= kLastChannels)
         return with_vec(C, [&](auto v) -> int {
             constexpr int V = decltype(v)::value;
@@ -987,10 +1164,10 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
             return DOPT_HIP_OK;
         });
     if (!channels_last && inner >= 4) {
-        const Split k = split_of(N, C, inner, G);
+        const Split k = split_of(C, inner, G, kMost);
         float2 *stats = nullptr;
         if (!k.whole && !(stats = (float2 *)workspace(N * G * k.s.parts * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
-        return with_hold(k.h, [&](auto c, auto q) -> int {
+        return with_hold<kMost>(k.h, [&](auto c, auto q) -> int {
             constexpr int kC = decltype(c)::value, kQ = decltype(q)::value;
             const dim3 grid((unsigned)(N * G * k.s.parts)), block(k.h.threads);
             if (k.whole) {
@@ -1044,6 +1221,18 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
         DOPT_LAUNCH_CHECK();
         return fold(S, 1);
     }
+    const HeldHold held = channels_last && inner > 1 ? held_for(N, C, inner, G, true) : HeldHold{};
+    if (held.threads) {
+        if (!(sums = (float2 *)workspace(N * C * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
+        if (int rc = with_quads<kMostGrad>(held.q, [&](auto q) -> int {
+                hipLaunchKernelGGL(gn_held_bwd_k<decltype(q)::value>, dim3(8 * held.h.per), dim3(held.threads), 0, stream(), held.h, act, dy, x,
+                                   scale, bias, means, rstds, sums, dx);
+                DOPT_LAUNCH_CHECK();
+                return DOPT_HIP_OK;
+            }))
+            return rc;
+        return fold(N, 1);
+    }
     if (channels_last && inner > 1 && C <= kLastChannels)
         return with_vec(C, [&](auto v) -> int {
             constexpr int V = decltype(v)::value;
@@ -1062,9 +1251,9 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
             return DOPT_HIP_OK;
         });
     if (!channels_last && inner >= 4) {
-        const Split k = split_of(N, C, inner, G);
+        const Split k = split_of(C, inner, G, kMostGrad);
         if (!(sums = (float2 *)workspace(N * C * k.s.pieces * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
-        if (int rc = with_hold(k.h, [&](auto c, auto q) -> int {
+        if (int rc = with_hold<kMostGrad>(k.h, [&](auto c, auto q) -> int {
                 constexpr int kC = decltype(c)::value, kQ = decltype(q)::value;
                 const dim3 grid((unsigned)(N * G * k.s.parts)), block(k.h.threads);
                 if (k.whole) {

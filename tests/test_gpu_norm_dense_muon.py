@@ -73,6 +73,26 @@ def test_group_norm(size, last):
     _check_norm_grad(dy, x, scale, bias, groups, name, last)
 
 
+# groups of a power of two of channels, on both sides of what a workgroup holds of them forward (32768 values) and backward (16384)
+HELD = [(2, 64, 30, 31, 8), (3, 48, 13, 19, 3), (2, 64, 11, 23, 2), (2, 128, 9, 29, 2), (3, 24, 1, 2, 3), (1, 8, 63, 65, 1), (2, 16, 45, 45, 2),
+        (9, 8, 3, 3, 1), (2, 16, 64, 65, 2), (2, 16, 40, 45, 1), (2, 20, 16, 16, 1), (1, 12, 37, 37, 1)]
+
+
+@pytest.mark.parametrize("last", [False, True], ids=["first", "last"])
+@pytest.mark.parametrize("size", HELD, ids=lambda s: "x".join(map(str, s)))
+def test_group_norm_of_groups_that_a_workgroup_holds(size, last):
+    n, c, h, w, groups = size
+    x, scale, bias, dy = _norm_case(n, c, h, w, last, sum(size))
+    for name, up in (("silu", ops.tensor), ("gelu", _off_grid)):
+        _check_norm(x, scale, bias, groups, name, last, up)
+        _check_norm_grad(dy, x, scale, bias, groups, name, last, up)
+
+
+def test_group_norm_gradient_of_more_than_the_caches_hold():
+    x, scale, bias, dy = _norm_case(54, 256, 32, 64, True, 9)
+    _check_norm_grad(dy, x, scale, bias, 32, "none", True)
+
+
 @pytest.mark.parametrize("name", R.ACTS)
 @pytest.mark.parametrize("last", [False, True], ids=["first", "last"])
 def test_group_norm_activations_and_alignment(name, last):
