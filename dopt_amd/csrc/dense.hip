@@ -146,7 +146,9 @@ int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, co
         DOPT_REQUIRE(!overlaps(o, out, x, M * K * f) && !overlaps(o, out, w, N * K * f) && !overlaps(o, out, bias, N * f) && !overlaps(o, out, residual, out),
                      "dopt_hip_dense_act: a result overlaps an operand");
     DOPT_REQUIRE(!overlaps(y, out, pre, out), "dopt_hip_dense_act: y and pre overlap");
-    return product_dense(M, N, K, x, w, DenseEpilogue{bias, residual, pre, act, N}, y);
+    const DenseEpilogue e{bias, residual, pre, act, N};
+    if (dense_wide_takes(M, N, K)) return dense_wide(M, N, K, x, w, e, y);
+    return product_dense(M, N, K, x, w, e, y);
 }
 
 int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *dy, const float *pre, const float *x, const float *w,

@@ -37,26 +37,11 @@
 #include <vector>
 
 #include "common.h"
-#include "mfma_core.h"
+#include "half_parts.h"
 
 namespace {
 
 using namespace dopt;
-
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-using lds_ptr = __attribute__((address_space(3))) void *;
-using glb_ptr = __attribute__((address_space(1))) const void *;
-// Addresses that come out of a table: the compiler does not see that they are global memory's, and a flat access waits for LDS too.
-template <class T>
-using Global = __attribute__((address_space(1))) T *;
-template <class T>
-__device__ __forceinline__ Global<T> global(T *p)
-{
-    return (Global<T>)p;
-}
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
 constexpr size_t kChunk = 8192;   // values per workgroup of the momentum's pass
@@ -172,30 +157,6 @@ __global__ __launch_bounds__(kBlock) void muon_momentum_k(const Matrix *jobs, co
     if (threadIdx.x == 0) global(q.parts)[t.i] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Four values, already times kUp, as their h and l parts.
-__device__ __forceinline__ void split4(const float *v, v2u &h, v2u &l)
-{
-    v4h a, b;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        a[e] = (_Float16)v[e];
-        b[e] = (_Float16)(v[e] - (float)a[e]);
-    }
-    h = __builtin_bit_cast(v2u, a);
-    l = __builtin_bit_cast(v2u, b);
-}
-
-__device__ __forceinline__ void join4(v2u h, v2u l, float *v)
-{
-    const v4h a = __builtin_bit_cast(v4h, h), b = __builtin_bit_cast(v4h, l);
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = (float)a[e] + (float)b[e];
-}
-
-// Where a row's piece lies in its block, and where the block of (row, step) lies in a matrix of `steps` steps.
-__device__ __forceinline__ int piece_at(int row, int piece) { return (row & 31) * 64 + ((piece ^ ((row >> 2) & 3)) * 16); }
-__device__ __forceinline__ size_t block_at(int row, int step, int steps) { return ((size_t)(row >> 5) * (steps >> 4) + (step >> 4)) * 2048; }
-
 // X = u / (|u| + eps), as it is and transposed, a 64 x 64 tile of w's layout per workgroup; zero outside.
 __global__ __launch_bounds__(kBlock) void muon_scale_k(const Matrix *jobs, const Tile *tiles, Step st)
 {
@@ -260,83 +221,6 @@ enum Product { kGram, kSquare, kApply, kLast };
 // is on its way, about 100 KB per CU, hides a memory latency of more than a microsecond.  A CU takes in some 65 GB/s so, which is what
 // bounds small tiles and makes wide ones worth their registers: X of eight [640 x 5760], 1.1 GB in tiles of 128 x 128.
 constexpr int kLds = 81920;
-
-__device__ __forceinline__ void bring(const char *src, int kilobytes, int lane, char *lds)
-{
-#pragma unroll
-    for (int q = 0; q < kilobytes; q++)
-        __builtin_amdgcn_global_load_lds((glb_ptr)(src + q * 1024 + lane * 16), (lds_ptr)(lds + q * 1024), 16, 0, 0);
-}
-
-__device__ __forceinline__ v8h fragment(const char *block, int row, int piece) { return *(const v8h *)(block + piece_at(row, piece)); }
-
-// acc[i][j] += block i of A times block j of B.
-template <int MI, int NI>
-__device__ __forceinline__ void multiply(const char *A, const char *B, int lane, v16f (&acc)[MI][NI])
-{
-    const int row = lane & 31, piece = 2 * (lane >> 5);
-    v8h ah[MI], al[MI], bh[NI], bl[NI];
-#pragma unroll
-    for (int i = 0; i < MI; i++) {
-        ah[i] = fragment(A + 2048 * i, row, piece);
-        al[i] = fragment(A + 2048 * i, row, piece + 1);
-    }
-#pragma unroll
-    for (int j = 0; j < NI; j++) {
-        bh[j] = fragment(B + 2048 * j, row, piece);
-        bl[j] = fragment(B + 2048 * j, row, piece + 1);
-    }
-#pragma unroll
-    for (int i = 0; i < MI; i++)
-#pragma unroll
-        for (int j = 0; j < NI; j++) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
-        }
-}
-
-// Between reads and writes of the same LDS by different wavefronts.  The empty statement keeps the reads in front of the barrier: without
-// it the compiler moved reads whose values were used in a branch behind the barrier into that branch.
-__device__ __forceinline__ void meet()
-{
-    asm volatile("" ::: "memory");
-    __syncthreads();
-}
-
-// The wavefront's fragments have left LDS, and all but the last `kLoads` loads that it has asked for are there.
-template <int kLoads>
-__device__ __forceinline__ void settled()
-{
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
-}
-
-// multiply_stage(stage in LDS) for each of `steps` stages, up to kStages - 1 of which are on their way ahead, kLoads loads of a
-// wavefront each: bring_stage(k, stage in LDS).  Once a wavefront's own part of stage k is there it meets the others: then
-// all of it is, and the stage before it has been read by everyone.
-template <int kStages, int kStage, int kLoads, class B, class F>
-__device__ __forceinline__ void pipeline(char *lds, int steps, B &&bring_stage, F &&multiply_stage)
-{
-    static_assert(kStages >= 3 && kStages <= 5 && kStages * kStage <= kLds, "one to three stages may be under way behind the next one");
-#pragma unroll
-    for (int k = 0; k < kStages - 1; k++)
-        if (k < steps) bring_stage(k, lds + k * kStage);
-    int at = 0, fill = kStages - 1;
-    for (int k = 0; k < steps; k++) {
-        const int behind = min(steps - 1 - k, kStages - 2);
-        if (behind == 3) settled<3 * kLoads>();
-        else if (behind == 2) settled<2 * kLoads>();
-        else if (behind == 1) settled<kLoads>();
-        else settled<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (k + kStages - 1 < steps) bring_stage(k + kStages - 1, lds + fill * kStage);
-        multiply_stage(lds + at * kStage);
-        fill = at;
-        at = at + 1 == kStages ? 0 : at + 1;
-    }
-    meet();   // the last stage has been read
-}
 
 // Four values in each of four neighbouring lanes: lane b gets value b of each.  `v` holds the values in pairs.
 __device__ __forceinline__ v2u transpose4(v2u v, int lane)
