@@ -9,6 +9,7 @@
 //
 // Bound by the matrix instructions: 6 M N K operations.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "dense.h"
@@ -21,7 +22,7 @@ using namespace dopt;
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 
-constexpr int kBlock = 256, kTile = 256, kThreads = 512, kStages = 4, kStage = 32768;
+constexpr int kTile = 256, kThreads = 512, kStages = 4, kStage = 32768;
 constexpr int kInf = 1 << 20, kNan = 1 << 21;   // in a row's shift: it holds infinities, NaN
 
 struct Operand {
@@ -34,67 +35,82 @@ struct Operand {
 // (by value: of an element of a vector the builtin takes the first one's bits)
 __device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
-// Four rows per workgroup: a wavefront finds its row's largest value, then all of them lay out the four.  Bound by memory; the second
-// reading finds most of the four rows in the L2.  Padding and rows that are not finite become zeros.
-__global__ __launch_bounds__(kBlock) void wide_split_k(Operand a, Operand b, unsigned blocks_a, size_t K, size_t steps)
+// Four rows per workgroup, eight values of a row to each of its threads and those of kUnits further places, in registers between the
+// search for the rows' largest values and the layout: sixteen steps of the four rows are stored by eight threads, 256 bytes
+// in a line.  Bound by memory; read twice, through an L2 that holds no row for so long, [8192 + 4096] rows of 4096 took 106 us.
+// Longer rows than the registers hold are.  Padding and rows that are not finite become zeros.
+constexpr int kUnits = 8;
+__global__ __launch_bounds__(1024) void wide_split_k(Operand a, Operand b, unsigned blocks_a, size_t K, size_t steps)
 {
-    __shared__ int shifts[4];
+    __shared__ unsigned tops[16][4];
     const Operand o = blockIdx.x < blocks_a ? a : b;
     const size_t row0 = (size_t)(blockIdx.x < blocks_a ? blockIdx.x : blockIdx.x - blocks_a) * 4;
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const size_t row = row0 + w;
+    const int lane = threadIdx.x & 63, r = threadIdx.x >> 1 & 3, half = threadIdx.x & 1, waves = blockDim.x >> 6;
+    const size_t stride = blockDim.x / 8, s0 = threadIdx.x / 8;
+    const bool inside = row0 + r < o.rows;
+    const float *const x = o.x + min(row0 + r, o.rows - 1) * K;
+    v4f v[kUnits][2];
     unsigned top = 0;   // of the values' magnitudes as integers, whose order is theirs, infinity and NaN last
-    if (row < o.rows) {
-        const float *const x = o.x + row * K;
-        const size_t whole = K / 4 * 4;
-#pragma unroll 8
-        for (size_t k = lane * 4; k < whole; k += 256) {
-            const v4f v = *(const v4f_any *)(x + k);
+    auto load = [&](size_t step, bool whole, v4f *to) {   // whole: all of the workgroup's steps lie inside
+        const size_t k = step * 16 + half * 8;
+        if (whole) {
+            to[0] = *(const v4f_any *)(x + k);
+            to[1] = *(const v4f_any *)(x + k + 4);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) top = max(top, magnitude(v[e]));
+            for (int e = 0; e < 8; e++) to[e / 4][e % 4] = k + e < K ? x[k + e] : 0.0f;
         }
-        for (size_t k = whole + lane; k < K; k += 64) top = max(top, magnitude(x[k]));
+    };
+    auto see = [&](const v4f *of) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = max(top, magnitude(of[e / 4][e % 4]));
+    };
+#pragma unroll
+    for (int i = 0; i < kUnits; i++)
+        if (i * stride < steps) load(s0 + i * stride, (i + 1) * stride * 16 <= K, v[i]);
+#pragma unroll
+    for (int i = 0; i < kUnits; i++)
+        if (i * stride < steps) see(v[i]);
+    for (size_t i = kUnits; i * stride < steps; i++) {
+        v4f more[2];
+        load(s0 + i * stride, (i + 1) * stride * 16 <= K, more);
+        see(more);
     }
 #pragma unroll
-    for (int m = 32; m; m >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, m, 64));
+    for (int m = 32; m; m >>= 1)
+        if (m != 2 && m != 4) top = max(top, (unsigned)__shfl_xor((int)top, m, 64));
+    if ((lane & ~6) == 0) tops[threadIdx.x >> 6][r] = top;
+    __syncthreads();
+    top = tops[0][r];
+    for (int i = 1; i < waves; i++) top = max(top, tops[i][r]);
     int shift = 0;
-    if (top > 0x7f800000u) shift = kNan;
+    if (!inside) shift = 0;
+    else if (top > 0x7f800000u) shift = kNan;
     else if (top == 0x7f800000u) shift = kInf;
     else if (top >= 0x800000u) shift = 14 + 127 - (int)(top >> 23);
     else if (top) shift = 14 + 149 - (31 - __builtin_clz(top));
-    if (lane == 0) {
-        shifts[w] = shift;
-        if (row < o.padded) o.shift[row] = shift;
-    }
-    __syncthreads();
-    // sixteen steps of the four rows by eight threads, which store 256 bytes in a line
-    const int r = threadIdx.x >> 1 & 3, half = threadIdx.x & 1;
-    const int by = shifts[r];
-    const bool live = row0 + r < o.rows && by < kInf;
-    const float *const x = o.x + (row0 + r) * K;
-    for (size_t s = threadIdx.x >> 3; s < steps; s += kBlock / 8) {
-        const size_t k = s * 16 + half * 8;
-        float v[8];
-        if (live && k + 8 <= K) {
-            const v4f p = *(const v4f_any *)(x + k), q = *(const v4f_any *)(x + k + 4);
+    if (threadIdx.x < 8 && half == 0) o.shift[row0 + r] = shift;
+    const bool live = inside && shift < kInf;
+    auto put = [&](size_t step, const v4f *of) {
+        if (step >= steps) return;
+        float u[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[e] = p[e];
-                v[4 + e] = q[e];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = live && k + e < K ? x[k + e] : 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = __builtin_ldexpf(v[e], by < kInf ? by : 0);
+        for (int e = 0; e < 8; e++) u[e] = live ? __builtin_ldexpf(of[e / 4][e % 4], shift) : 0.0f;
         v2u h0, l0, h1, l1;
-        split4(v, h0, l0);
-        split4(v + 4, h1, l1);
-        char *const at = o.parts + ((row0 >> 5) * steps + s) * 2048;
+        split4(u, h0, l0);
+        split4(u + 4, h1, l1);
+        char *const at = o.parts + ((row0 >> 5) * steps + step) * 2048;
         const int in = (int)(row0 & 31) + r;
         *(v4u *)(at + piece_at(in, 2 * half)) = v4u{h0.x, h0.y, h1.x, h1.y};
         *(v4u *)(at + piece_at(in, 2 * half + 1)) = v4u{l0.x, l0.y, l1.x, l1.y};
+    };
+#pragma unroll
+    for (int i = 0; i < kUnits; i++)
+        if (i * stride < steps) put(s0 + i * stride, v[i]);
+    for (size_t i = kUnits; i * stride < steps; i++) {
+        v4f more[2];
+        load(s0 + i * stride, (i + 1) * stride * 16 <= K, more);
+        put(s0 + i * stride, more);
     }
 }
 
@@ -107,7 +123,7 @@ struct Wide {
 };
 
 // What is not finite in a tile's operands: the sums of those rows and columns as fp32 instructions make them.
-__device__ __noinline__ void rough_sums(const Wide &q, const DenseEpilogue &ep, float *y, size_t m0, size_t n0, const int *shift)
+__device__ __noinline__ void rough_sums(Wide q, DenseEpilogue ep, float *y, size_t m0, size_t n0, const int *shift)
 {
     for (int i = threadIdx.x; i < kTile * kTile; i += kThreads) {
         const size_t m = m0 + i / kTile, n = n0 + i % kTile;
@@ -119,6 +135,15 @@ __device__ __noinline__ void rough_sums(const Wide &q, const DenseEpilogue &ep, 
             for (size_t k = 0; k < q.K; k++) s += q.x[m * q.K + k] * q.w[n * q.K + k];
         y[m * q.N + n] = ep(s, m * q.N + n);
     }
+}
+
+__device__ __forceinline__ void phase()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // A tile of 256 x 256 by eight wavefronts of 128 x 64: the accumulators are half of the registers, and a stage of 16 steps, 32 KB, feeds
@@ -136,13 +161,39 @@ __global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilo
     const char *const left = q.xp + (mt * 8 + w) * row_of_blocks, *const right = q.wp + (nt * 8 + w) * row_of_blocks;
     v16f acc[4][2];
     zero_acc(acc);
-    pipeline<kStages, kStage, 4>(
-        lds, (int)q.steps,
-        [&](int k, char *to) {
-            bring(left + (size_t)k * 2048, 2, lane, to + w * 2048);
-            bring(right + (size_t)k * 2048, 2, lane, to + 16384 + w * 2048);
-        },
-        [&](const char *now) { multiply(now + wm * 8192, now + 16384 + wn * 4096, lane, acc); });
+    auto bring_stage = [&](int k) {
+        char *const to = lds + (k & 3) * kStage;
+        bring(left + (size_t)k * 2048, 2, lane, to + w * 2048);
+        bring(right + (size_t)k * 2048, 2, lane, to + 16384 + w * 2048);
+    };
+    auto arrived = [&](int ahead) {   // all loads but those of the last `ahead` stages asked for
+        if (ahead >= 2) settled<8>();
+        else if (ahead == 1) settled<4>();
+        else settled<0>();
+    };
+    const int steps = (int)q.steps;
+    for (int k = 0; k < min(steps, 3); k++) bring_stage(k);
+    arrived(min(steps, 3) - 1);
+    phase();
+    if (wm) phase();
+    for (int k = 0; k < steps; k++) {
+        Side<4> a;
+        Side<2> b;
+        const char *const now = lds + (k & 3) * kStage;
+        a.read(now + wm * 8192, lane);
+        b.read(now + 16384 + wn * 4096, lane);
+        if (k + 3 < steps) bring_stage(k + 3);
+        if (wm) arrived(min(steps - 2 - k, 2));
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        phase();
+        __builtin_amdgcn_s_setprio(1);
+        multiply(a, b, acc);
+        __builtin_amdgcn_s_setprio(0);
+        if (!wm) arrived(min(steps - 2 - k, 2));
+        phase();
+    }
+    if (!wm) phase();
+    meet();
 
     int *const shift = (int *)lds;
     const size_t m0 = (size_t)mt * kTile, n0 = (size_t)nt * kTile;
@@ -151,51 +202,69 @@ __global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilo
     const bool rough = __syncthreads_or(mine >= kInf);
     // 32 rows at a time through LDS, so that a row's 64 values are stored by sixteen lanes
     float *const image = (float *)(lds + 2048) + w * (32 * 68);
-    const int col = 4 * (lane & 15);
-    const size_t n = n0 + wn * 64 + col;
     const bool inside = m0 + kTile <= q.M && n0 + kTile <= q.N && !rough;
-    const v4i sn = *(const v4i *)(shift + kTile + wn * 64 + col);
+    const size_t left_col = n0 + wn * 64;   // of the wavefront's 64
+    // values one by one: beside values that are not finite, and where the matrix ends within the wavefront's first three columns
+    const bool single = rough || (left_col < q.N && left_col + 4 > q.N);
+    // quads end with the matrix: the lanes that would pass its end take its last quad once more
+    const int col = single ? 4 * (lane & 15) : (int)(min(left_col + 4 * (lane & 15), q.N - 4) - left_col);
+    const size_t n = left_col + col;
+    int sn[4];
     v4f bias{0.0f, 0.0f, 0.0f, 0.0f};
-    if (ep.bias) {
+    if (left_col < q.N && !single) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) bias[e] = n + e < q.N ? ep.bias[n + e] : 0.0f;
+        for (int e = 0; e < 4; e++) sn[e] = shift[kTile + wn * 64 + col + e];
+        if (ep.bias) bias = *(const v4f_any *)(ep.bias + n);
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
+    // (a loop, whose sums move down: its code unrolled, for each activation, costs more to fetch than 96 moves)
+#pragma unroll 1
+    for (int i = 0; i < 4 && left_col < q.N; i++) {
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) image[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * 68 + 32 * j + (lane & 31)] = acc[i][j][e];
+            for (int e = 0; e < 16; e++) image[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * 68 + 32 * j + (lane & 31)] = acc[0][j][e];
         asm volatile("" ::: "memory");   // (a wavefront's LDS accesses stay in their order)
         const int r0 = wm * 128 + i * 32 + (lane >> 4);
         with_activation(ep.act, [&](auto kind) {
-            if (inside) {
+            auto quads = [&](auto whole) {   // whole: nothing ends within the tile
+                constexpr bool kWhole = decltype(whole)::value;
                 v4f res[8];
                 if (ep.residual) {
 #pragma unroll
-                    for (int t = 0; t < 8; t++) res[t] = *(const v4f_any *)(ep.residual + (m0 + r0 + 4 * t) * q.N + n);
+                    for (int t = 0; t < 8; t++) res[t] = *(const v4f_any *)(ep.residual + (kWhole ? m0 + r0 + 4 * t : min(m0 + r0 + 4 * t, q.M - 1)) * q.N + n);
                 }
 #pragma unroll
                 for (int t = 0; t < 8; t++) {
-                    v4f z = *(const v4f *)(image + (4 * t + (lane >> 4)) * 68 + col), o;
+                    const float *const from = image + (4 * t + (lane >> 4)) * 68 + col;
                     const int sm = shift[r0 + 4 * t];
-                    const size_t at = (m0 + r0 + 4 * t) * q.N + n;
+                    const size_t m = m0 + r0 + 4 * t, at = m * q.N + n;
+                    v4f z, o;
+                    if (kWhole) z = *(const v4f *)from;
+                    else z = v4f{from[0], from[1], from[2], from[3]};
 #pragma unroll
                     for (int e = 0; e < 4; e++) z[e] = __builtin_ldexpf(z[e], -(sm + sn[e])) + bias[e];
-                    if (ep.pre) *(v4f_any *)(ep.pre + at) = z;
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[e] = act_value<kind.value>(z[e]);
                     if (ep.residual) o += res[t];
-                    *(v4f_any *)(y + at) = o;
+                    if (kWhole || m < q.M) {
+                        if (ep.pre) *(v4f_any *)(ep.pre + at) = z;
+                        *(v4f_any *)(y + at) = o;
+                    }
                 }
+            };
+            if (inside) {
+                quads(std::true_type{});
+            } else if (!single) {
+                quads(std::false_type{});
             } else {
                 for (int t = 0; t < 8; t++) {
                     const int sm = shift[r0 + 4 * t];
                     const size_t m = m0 + r0 + 4 * t;
                     if (m >= q.M || sm >= kInf) continue;
                     for (int e = 0; e < 4; e++) {
+                        if (n + e >= q.N) break;
                         const int s = shift[kTile + wn * 64 + col + e];
-                        if (n + e >= q.N || s >= kInf) continue;
+                        if (s >= kInf) continue;
                         const size_t at = m * q.N + n + e;
                         const float z = __builtin_ldexpf(image[(4 * t + (lane >> 4)) * 68 + col + e], -(sm + s)) + ep.bias_of(n + e);
                         if (ep.pre) ep.pre[at] = z;
@@ -206,6 +275,10 @@ __global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilo
             }
         });
         asm volatile("" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) acc[k][j] = acc[k + 1][j];
     }
     if (rough) rough_sums(q, ep, y, m0, n0, shift);
 }
@@ -214,9 +287,13 @@ __global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilo
 
 namespace dopt {
 
+// Where a third of the chip's places for tiles are taken.  us here and on three bf16 parts, with 128, 512 and 1024 steps:
+//     [1024 x 4096] 36 57 84 and 29 51 85    [1500 x 4096] 37 63 93 and 36 69 113    [4096 x 2500] 55 77 109 and 91 153 198
+//     [4096 x 4097] 96 142 210 and 140 234 362    [8192 x 4096] 130 187 268 and 160 308 472
 bool dense_wide_takes(size_t M, size_t N, size_t K)
 {
-    return M >= 1024 && N >= 1024 && K >= 512 && ceil_div(M, (size_t)kTile) < ((size_t)1 << 20) && ceil_div(N, (size_t)kTile) < ((size_t)1 << 10);
+    const size_t tiles = ceil_div(M, (size_t)kTile) * ceil_div(N, (size_t)kTile), rounds = ceil_div(tiles, (size_t)num_cus());
+    return M >= 512 && N >= 512 && K >= 128 && tiles < ((size_t)1 << 30) && M * N * 3 >= rounds * num_cus() * kTile * kTile;
 }
 
 int dense_wide(size_t M, size_t N, size_t K, const float *x, const float *w, const DenseEpilogue &e, float *y)
@@ -226,8 +303,8 @@ int dense_wide(size_t M, size_t N, size_t K, const float *x, const float *w, con
     if (!to) return DOPT_HIP_ERR_OOM;
     char *const xp = to, *const wp = xp + mp * steps * 64;
     int *const xs = (int *)(wp + np * steps * 64), *const ws = xs + mp;
-    const unsigned blocks = (unsigned)(mp / 4);
-    hipLaunchKernelGGL(wide_split_k, dim3(blocks + (unsigned)(np / 4)), dim3(kBlock), 0, stream(), Operand{x, M, mp, xp, xs}, Operand{w, N, np, wp, ws}, blocks,
+    const unsigned blocks = (unsigned)(mp / 4), threads = steps > 512 ? 1024 : steps > 256 ? 512 : 256;   // rows in registers up to 16384
+    hipLaunchKernelGGL(wide_split_k, dim3(blocks + (unsigned)(np / 4)), dim3(threads), 0, stream(), Operand{x, M, mp, xp, xs}, Operand{w, N, np, wp, ws}, blocks,
                        K, steps);
     DOPT_LAUNCH_CHECK();
     static bool raised = false;

@@ -62,30 +62,42 @@ __device__ __forceinline__ void bring(const char *src, int kilobytes, int lane, 
 
 __device__ __forceinline__ v8h fragment(const char *block, int row, int piece) { return *(const v8h *)(block + piece_at(row, piece)); }
 
-// acc[i][j] += block i of A times block j of B.
+// Blocks of a wavefront's side of a product, as its lanes hold them.
+template <int N>
+struct Side {
+    v8h h[N], l[N];
+    __device__ __forceinline__ void read(const char *blocks, int lane)
+    {
+        const int row = lane & 31, piece = 2 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            h[i] = fragment(blocks + 2048 * i, row, piece);
+            l[i] = fragment(blocks + 2048 * i, row, piece + 1);
+        }
+    }
+};
+
+// acc[i][j] += block i of a times block j of b.
 template <int MI, int NI>
-__device__ __forceinline__ void multiply(const char *A, const char *B, int lane, v16f (&acc)[MI][NI])
+__device__ __forceinline__ void multiply(const Side<MI> &a, const Side<NI> &b, v16f (&acc)[MI][NI])
 {
-    const int row = lane & 31, piece = 2 * (lane >> 5);
-    v8h ah[MI], al[MI], bh[NI], bl[NI];
-#pragma unroll
-    for (int i = 0; i < MI; i++) {
-        ah[i] = fragment(A + 2048 * i, row, piece);
-        al[i] = fragment(A + 2048 * i, row, piece + 1);
-    }
-#pragma unroll
-    for (int j = 0; j < NI; j++) {
-        bh[j] = fragment(B + 2048 * j, row, piece);
-        bl[j] = fragment(B + 2048 * j, row, piece + 1);
-    }
 #pragma unroll
     for (int i = 0; i < MI; i++)
 #pragma unroll
         for (int j = 0; j < NI; j++) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l[i], b.h[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h[i], b.l[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h[i], b.h[j], acc[i][j], 0, 0, 0);
         }
+}
+template <int MI, int NI>
+__device__ __forceinline__ void multiply(const char *A, const char *B, int lane, v16f (&acc)[MI][NI])
+{
+    Side<MI> a;
+    Side<NI> b;
+    a.read(A, lane);
+    b.read(B, lane);
+    multiply(a, b, acc);
 }
 
 // Between reads and writes of the same LDS by different wavefronts.  The empty statement keeps the reads in front of the barrier: without

@@ -206,7 +206,7 @@ def test_group_norm_refusals():
 # m, n, k
 DENSES = [(1, 1, 1), (1, 10, 16), (1, 4096, 512), (1, 333, 1025), (2, 3, 5), (7, 64, 100), (33, 65, 127), (64, 512, 784), (130, 70, 1), (256, 10, 512),
           (300, 1, 77), (129, 257, 130), (512, 512, 512), (1000, 130, 260), (257, 300, 2050), (64, 2000, 1030), (520, 1030, 1500), (1024, 1024, 512), (1030, 1100, 530),
-          (1300, 1281, 1111)]
+          (1300, 1281, 1111), (2560, 2304, 512), (2497, 2370, 131), (2370, 2497, 400)]
 
 
 def _dense_case(m, n, k, seed):
@@ -270,7 +270,7 @@ def test_dense_act_of_nothing():
     assert dx.size == 0 and not dw.numpy().any() and not db.numpy().any()
 
 
-@pytest.mark.parametrize("size", [(1, 64, 300), (40, 50, 300), (300, 300, 300), (300, 520, 1200), (1030, 1100, 530)], ids=str)
+@pytest.mark.parametrize("size", [(1, 64, 300), (40, 50, 300), (300, 300, 300), (300, 520, 1200), (1030, 1100, 530), (2500, 2403, 140)], ids=str)
 def test_dense_act_with_values_that_are_not_finite(size):
     m, n, k = size
     x, w, b, res, _ = _dense_case(m, n, k, 12)
@@ -289,7 +289,7 @@ def test_dense_act_with_values_that_are_not_finite(size):
 
 def test_dense_act_of_large_layers_with_rows_of_any_size():
     """Rows 2^160 apart, rows of zeros, and rows whose largest value meets zeros only: what is below 2^-40 of it may be lost."""
-    m, n, k = 1025, 1030, 640
+    m, n, k = 2401, 2562, 640
     r = np.random.default_rng(14)
     x, w, _, _, _ = _dense_case(m, n, k, 13)
     x = _f(x * 2.0 ** r.integers(-80, 41, (m, 1)))
@@ -303,6 +303,14 @@ def test_dense_act_of_large_layers_with_rows_of_any_size():
     want, bound = R.product(x, w)
     top = np.outer(np.abs(x).max(1).astype(np.float64), np.abs(w).max(1).astype(np.float64))
     R.close(y, (want, bound + 2.0 ** -39 * k * top + E_TINY), "rows of small values and a large one")
+
+
+def test_dense_act_of_long_rows():
+    m, n, k = 2368, 2504, 17001
+    x, w, b, _, _ = _dense_case(m, n, k, 15)
+    x[:, 17000] += F32(300.0)   # the largest value is the last one
+    y = ops.dense_act(ops.tensor(x), ops.tensor(w), ops.tensor(b), act="silu").numpy()
+    R.close(y, R.dense_act(x, w, b, None, "silu")[0], "y")
 
 
 def test_dense_act_refusals():
