@@ -33,9 +33,14 @@ struct DenseEpilogue {
 
 // dense.hip: the same for a product that lies in y already.
 int dense_finish(size_t M, size_t N, const DenseEpilogue &e, float *y);
-// dense_wide.hip: x w^T with that epilogue for large sizes.
+// dense_wide.hip: x w^T with that epilogue for large sizes; either may lie across, [K][rows].
+struct WideSide {
+    const float *values;
+    bool across;
+};
 bool dense_wide_takes(size_t M, size_t N, size_t K);
-int dense_wide(size_t M, size_t N, size_t K, const float *x, const float *w, const DenseEpilogue &e, float *y);
+size_t dense_wide_scratch(size_t M, size_t N, size_t K);
+int dense_wide(size_t M, size_t N, size_t K, const WideSide &x, const WideSide &w, const DenseEpilogue &e, float *y);
 // sgemm.hip: x w^T with that epilogue, x [M, K], w [N, K].
 int product_dense(size_t M, size_t N, size_t K, const float *x, const float *w, const DenseEpilogue &e, float *y);
 

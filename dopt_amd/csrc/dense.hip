@@ -147,7 +147,7 @@ int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, co
                      "dopt_hip_dense_act: a result overlaps an operand");
     DOPT_REQUIRE(!overlaps(y, out, pre, out), "dopt_hip_dense_act: y and pre overlap");
     const DenseEpilogue e{bias, residual, pre, act, N};
-    if (dense_wide_takes(M, N, K)) return dense_wide(M, N, K, x, w, e, y);
+    if (dense_wide_takes(M, N, K)) return dense_wide(M, N, K, {x, false}, {w, false}, e, y);
     return product_dense(M, N, K, x, w, e, y);
 }
 
@@ -174,13 +174,15 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     const size_t tiles = ceil_div(std::max(N, (size_t)1), (size_t)(64 * V));
     // enough workgroups to fill the chip, of sixteen rows and more
     const int runs = (int)std::max((size_t)1, std::min(ceil_div(M, (size_t)16), ceil_div((size_t)num_cus() * 8, tiles)));
+    const bool wide_x = dense_wide_takes(M, K, N), wide_w = dense_wide_takes(N, K, M);
     size_t held = 0;
     if (M * N > 0 && (!plain || dbias)) {
         // dz, its sums and what the products park beside them share one request, which none of them has to grow
         auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
         const size_t first = plain ? 0 : rounded(M * N * sizeof(float));
         held = first + rounded((size_t)runs * N * sizeof(float));
-        const size_t more = std::max(dx ? product_scratch(0, 0, M, K, N) : 0, dw ? product_scratch(1, 0, N, K, M) : 0);
+        const size_t more = std::max(!dx ? 0 : wide_x ? dense_wide_scratch(M, K, N) : product_scratch(0, 0, M, K, N),
+                                     !dw ? 0 : wide_w ? dense_wide_scratch(N, K, M) : product_scratch(1, 0, N, K, M));
         char *const to = (char *)workspace(held + more);
         if (!to) return DOPT_HIP_ERR_OOM;
         if (!plain) dz = (float *)to;
@@ -198,8 +200,9 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     }
     workspace_hold(held);
     int rc = DOPT_HIP_OK;
-    if (dx && M * K > 0) rc = dopt_hip_sgemm_t(0, 0, M, K, N, dz, w, dx);
-    if (!rc && dw && N * K > 0) rc = dopt_hip_sgemm_t(1, 0, N, K, M, dz, x, dw);
+    const DenseEpilogue none{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K};
+    if (dx && M * K > 0) rc = wide_x ? dense_wide(M, K, N, {dz, false}, {w, true}, none, dx) : dopt_hip_sgemm_t(0, 0, M, K, N, dz, w, dx);
+    if (!rc && dw && N * K > 0) rc = wide_w ? dense_wide(N, K, M, {dz, true}, {x, true}, none, dw) : dopt_hip_sgemm_t(1, 0, N, K, M, dz, x, dw);
     workspace_hold(0);
     return rc;
 }

@@ -1,5 +1,5 @@
-// Large dense layers forward: both operands are laid out once as two fp16 parts and go to the matrix instruction from there, the layer's end
-// rides in the product.
+// Products of large dense layers, forward and backward: both operands are laid out once as two fp16 parts and go to the matrix instruction
+// from there, the layer's end rides in the product.
 //
 // Rows are scaled by powers of two, each to a largest value in [2^14, 2^15), so h + l is off by at most 2^-22 of a value and 2^-40 of
 // the largest one of its row (fp16's last subnormal place).  l l is left out, 2^-22 of a product at most.  Together with sums in fp32
@@ -34,6 +34,25 @@ struct Operand {
 
 // (by value: of an element of a vector the builtin takes the first one's bits)
 __device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+
+// What a row is held times, from its largest magnitude.
+__device__ __forceinline__ int shift_of(unsigned top)
+{
+    if (top > 0x7f800000u) return kNan;
+    if (top == 0x7f800000u) return kInf;
+    if (top >= 0x800000u) return 14 + 127 - (int)(top >> 23);
+    return top ? 14 + 149 - (31 - __builtin_clz(top)) : 0;
+}
+
+// Eight steps of a row of a block.
+__device__ __forceinline__ void store_parts(char *block, int row, int half, const float *v)
+{
+    v2u h0, l0, h1, l1;
+    split4(v, h0, l0);
+    split4(v + 4, h1, l1);
+    *(v4u *)(block + piece_at(row, 2 * half)) = v4u{h0.x, h0.y, h1.x, h1.y};
+    *(v4u *)(block + piece_at(row, 2 * half + 1)) = v4u{l0.x, l0.y, l1.x, l1.y};
+}
 
 // Four rows per workgroup, eight values of a row to each of its threads and those of kUnits further places, in registers between the
 // search for the rows' largest values and the layout: sixteen steps of the four rows are stored by eight threads, 256 bytes
@@ -83,12 +102,7 @@ __global__ __launch_bounds__(1024) void wide_split_k(Operand a, Operand b, unsig
     __syncthreads();
     top = tops[0][r];
     for (int i = 1; i < waves; i++) top = max(top, tops[i][r]);
-    int shift = 0;
-    if (!inside) shift = 0;
-    else if (top > 0x7f800000u) shift = kNan;
-    else if (top == 0x7f800000u) shift = kInf;
-    else if (top >= 0x800000u) shift = 14 + 127 - (int)(top >> 23);
-    else if (top) shift = 14 + 149 - (31 - __builtin_clz(top));
+    const int shift = inside ? shift_of(top) : 0;
     if (threadIdx.x < 8 && half == 0) o.shift[row0 + r] = shift;
     const bool live = inside && shift < kInf;
     auto put = [&](size_t step, const v4f *of) {
@@ -96,13 +110,7 @@ __global__ __launch_bounds__(1024) void wide_split_k(Operand a, Operand b, unsig
         float u[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) u[e] = live ? __builtin_ldexpf(of[e / 4][e % 4], shift) : 0.0f;
-        v2u h0, l0, h1, l1;
-        split4(u, h0, l0);
-        split4(u + 4, h1, l1);
-        char *const at = o.parts + ((row0 >> 5) * steps + step) * 2048;
-        const int in = (int)(row0 & 31) + r;
-        *(v4u *)(at + piece_at(in, 2 * half)) = v4u{h0.x, h0.y, h1.x, h1.y};
-        *(v4u *)(at + piece_at(in, 2 * half + 1)) = v4u{l0.x, l0.y, l1.x, l1.y};
+        store_parts(o.parts + ((row0 >> 5) * steps + step) * 2048, (int)(row0 & 31) + r, half, u);
     };
 #pragma unroll
     for (int i = 0; i < kUnits; i++)
@@ -114,9 +122,86 @@ __global__ __launch_bounds__(1024) void wide_split_k(Operand a, Operand b, unsig
     }
 }
 
+// Operands that lie across the reduction, [K][rows]: the largest values of runs of K for each column, then a tile of 64 steps by 64 columns
+// per workgroup, turned in LDS.
+constexpr int kRuns = 32;
+struct Across {
+    Operand o;
+    unsigned *tops;   // [run][row]
+    unsigned tiles;   // of 256 columns; of 64 columns, padding included
+};
+
+__global__ __launch_bounds__(256) void wide_tops_k(Across a, size_t K, int runs)
+{
+    __shared__ unsigned red[4][256];
+    const size_t col = min((size_t)(blockIdx.x % a.tiles) * 256 + (threadIdx.x & 63) * 4, a.o.rows - 4), run = blockIdx.x / a.tiles;
+    const size_t from = K * run / runs, to = K * (run + 1) / runs;
+    const int row = threadIdx.x >> 6;
+    unsigned top[4] = {0, 0, 0, 0};
+    size_t k = from + row;
+    auto see = [&](v4f v) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) top[e] = max(top[e], magnitude(v[e]));
+    };
+    for (; k + 28 < to; k += 32) {
+        v4f v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = *(const v4f_any *)(a.o.x + (k + 4 * i) * a.o.rows + col);
+#pragma unroll
+        for (int i = 0; i < 8; i++) see(v[i]);
+    }
+    for (; k < to; k += 4) see(*(const v4f_any *)(a.o.x + k * a.o.rows + col));
+#pragma unroll
+    for (int e = 0; e < 4; e++) red[row][(threadIdx.x & 63) * 4 + e] = top[e];
+    __syncthreads();
+    if (row) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int c = (threadIdx.x & 63) * 4 + e;
+        a.tops[run * a.o.rows + col + e] = max(max(red[0][c], red[1][c]), max(red[2][c], red[3][c]));
+    }
+}
+
+__global__ __launch_bounds__(256) void wide_turn_k(Across a, size_t K, size_t steps, int runs)
+{
+    __shared__ float tile[64][65];
+    __shared__ unsigned tops[4][64];
+    const size_t c0 = (size_t)(blockIdx.x % a.tiles) * 64, k0 = (size_t)(blockIdx.x / a.tiles) * 64;
+    const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const size_t col = min(c0 + c, a.o.rows - 1);
+    float v[16];
+#pragma unroll
+    for (int u = 0; u < 16; u++) v[u] = a.o.x[min(k0 + w + 4 * u, K - 1) * a.o.rows + col];
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < kRuns / 4; i++) top = max(top, a.tops[min(w + 4 * i, runs - 1) * a.o.rows + col]);
+    tops[w][c] = top;
+    __syncthreads();
+    const bool inside = c0 + c < a.o.rows;
+    const int shift = inside ? shift_of(max(max(tops[0][c], tops[1][c]), max(tops[2][c], tops[3][c]))) : 0;
+    if (k0 == 0 && w == 0) a.o.shift[c0 + c] = shift;
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+        const int k = w + 4 * u;
+        tile[k][c] = inside && shift < kInf && k0 + k < K ? __builtin_ldexpf(v[u], shift) : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; u++) {   // a wavefront stores a block at a time
+        const int r = (threadIdx.x >> 1 & 31) + 32 * u, half = threadIdx.x & 1;
+        const size_t step = k0 / 16 + w;
+        if (step >= steps) break;
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) p[e] = tile[w * 16 + half * 8 + e][r];
+        store_parts(a.o.parts + ((c0 + r) / 32 * steps + step) * 2048, r & 31, half, p);
+    }
+}
+
 struct Wide {
     size_t M, N, K, steps;
     const float *x, *w;
+    size_t xm, xk, wn, wk;   // between rows, between steps
     const char *xp, *wp;
     const int *xs, *ws;
     unsigned tiles, mtiles, ntiles;
@@ -132,7 +217,7 @@ __device__ __noinline__ void rough_sums(Wide q, DenseEpilogue ep, float *y, size
         const bool nan = most == kNan;
         float s = nan ? __builtin_nanf("") : 0.0f;
         if (!nan)
-            for (size_t k = 0; k < q.K; k++) s += q.x[m * q.K + k] * q.w[n * q.K + k];
+            for (size_t k = 0; k < q.K; k++) s += q.x[m * q.xm + k * q.xk] * q.w[n * q.wn + k * q.wk];
         y[m * q.N + n] = ep(s, m * q.N + n);
     }
 }
@@ -296,23 +381,53 @@ bool dense_wide_takes(size_t M, size_t N, size_t K)
     return M >= 512 && N >= 512 && K >= 128 && tiles < ((size_t)1 << 30) && M * N * 3 >= rounds * num_cus() * kTile * kTile;
 }
 
-int dense_wide(size_t M, size_t N, size_t K, const float *x, const float *w, const DenseEpilogue &e, float *y)
+size_t dense_wide_scratch(size_t M, size_t N, size_t K)
+{
+    const size_t mp = ceil_div(M, (size_t)kTile) * kTile, np = ceil_div(N, (size_t)kTile) * kTile;
+    return (mp + np) * (ceil_div(K, (size_t)16) * 64 + sizeof(int)) + kRuns * std::max(M, N) * sizeof(unsigned);
+}
+
+int dense_wide(size_t M, size_t N, size_t K, const WideSide &x, const WideSide &w, const DenseEpilogue &e, float *y)
 {
     const size_t mp = ceil_div(M, (size_t)kTile) * kTile, np = ceil_div(N, (size_t)kTile) * kTile, steps = ceil_div(K, (size_t)16);
-    char *const to = (char *)workspace((mp + np) * (steps * 64 + sizeof(int)));
+    char *const to = (char *)workspace(dense_wide_scratch(M, N, K));
     if (!to) return DOPT_HIP_ERR_OOM;
     char *const xp = to, *const wp = xp + mp * steps * 64;
     int *const xs = (int *)(wp + np * steps * 64), *const ws = xs + mp;
-    const unsigned blocks = (unsigned)(mp / 4), threads = steps > 512 ? 1024 : steps > 256 ? 512 : 256;   // rows in registers up to 16384
-    hipLaunchKernelGGL(wide_split_k, dim3(blocks + (unsigned)(np / 4)), dim3(threads), 0, stream(), Operand{x, M, mp, xp, xs}, Operand{w, N, np, wp, ws}, blocks,
-                       K, steps);
-    DOPT_LAUNCH_CHECK();
+    unsigned *const tops = (unsigned *)(ws + np);
+    const Operand both[] = {{x.values, M, mp, xp, xs}, {w.values, N, np, wp, ws}};
+    const unsigned threads = steps > 512 ? 1024 : steps > 256 ? 512 : 256;   // rows in registers up to 16384
+    if (!x.across && !w.across) {   // in one launch
+        const unsigned blocks = (unsigned)(mp / 4);
+        hipLaunchKernelGGL(wide_split_k, dim3(blocks + (unsigned)(np / 4)), dim3(threads), 0, stream(), both[0], both[1], blocks, K, steps);
+        DOPT_LAUNCH_CHECK();
+    } else {
+        const bool across[] = {x.across, w.across};
+        for (int i = 0; i < 2; i++) {
+            const Operand &o = both[i];
+            if (!across[i]) {
+                const unsigned blocks = (unsigned)(o.padded / 4);
+                hipLaunchKernelGGL(wide_split_k, dim3(blocks), dim3(threads), 0, stream(), o, o, blocks, K, steps);
+                DOPT_LAUNCH_CHECK();
+                continue;
+            }
+            const int runs = (int)std::min((size_t)kRuns, ceil_div(K, (size_t)64));
+            Across a{o, tops, (unsigned)ceil_div(o.rows, (size_t)256)};
+            hipLaunchKernelGGL(wide_tops_k, dim3(a.tiles * runs), dim3(256), 0, stream(), a, K, runs);
+            DOPT_LAUNCH_CHECK();
+            a.tiles = (unsigned)(o.padded / 64);
+            hipLaunchKernelGGL(wide_turn_k, dim3(a.tiles * (unsigned)ceil_div(steps, (size_t)4)), dim3(256), 0, stream(), a, K, steps, runs);
+            DOPT_LAUNCH_CHECK();
+        }
+    }
     static bool raised = false;
     if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)wide_product_k, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStage));
     raised = true;
     const unsigned mt = (unsigned)(mp / kTile), nt = (unsigned)(np / kTile);
     hipLaunchKernelGGL(wide_product_k, dim3(xcd_grid(mt * nt)), dim3(kThreads), kStages * kStage, stream(),
-                       Wide{M, N, K, steps, x, w, xp, wp, xs, ws, mt * nt, mt, nt}, e, y);
+                       Wide{M, N, K, steps, x.values, w.values, x.across ? 1 : K, x.across ? M : 1, w.across ? 1 : K, w.across ? N : 1, xp, wp, xs, ws, mt * nt,
+                            mt, nt},
+                       e, y);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }

@@ -313,6 +313,27 @@ def test_dense_act_of_long_rows():
     R.close(y, R.dense_act(x, w, b, None, "silu")[0], "y")
 
 
+@pytest.mark.parametrize("size", [(2400, 2411, 2421), (2563, 300, 2500), (2499, 2305, 130)], ids=str)
+def test_dense_act_gradient_of_large_layers(size):
+    m, n, k = size
+    x, w, _, pre, dy = _dense_case(m, n, k, 16)
+    x = _f(x * 2.0 ** np.random.default_rng(17).integers(-20, 21, (1, k)))   # each column of its own size
+    for name, up in (("silu", ops.tensor), ("none", _off_grid)):
+        got = ops.dense_act_grad(up(dy), up(x), up(w), up(pre), name)
+        for t, v, what in zip(got, R.dense_act_grad(dy, x, w, pre, name), ("dx", "dw", "dbias")):
+            R.close(t.numpy(), v, name + " " + what)
+    x[5, 7], dy[9, 11] = np.inf, np.nan
+    dy[5] = np.abs(dy[5]) + F32(0.1)
+    with np.errstate(invalid="ignore"):
+        dx, dw = (t.numpy() for t in ops.dense_act_grad(ops.tensor(dy), ops.tensor(x), ops.tensor(w))[:2])
+    want_x, want_w = np.zeros((m, k), bool), np.zeros((n, k), bool)
+    want_x[9], want_w[11] = True, True
+    assert np.array_equal(np.isnan(dx), want_x) and np.array_equal(np.isnan(dw), want_w)
+    want_w[:, 7] ^= True
+    want_w[11] = False
+    assert np.array_equal(np.isposinf(dw), want_w) and not np.isinf(dx).any()
+
+
 def test_dense_act_refusals():
     x, w, y = ops.Tensor((4, 6)), ops.Tensor((5, 6)), ops.Tensor((4, 5))
     for bad in (lambda: ops.dense_act(x, ops.Tensor((5, 7))), lambda: ops.dense_act(x, w, ops.Tensor((4,))), lambda: ops.dense_act(x, w, None, x),
