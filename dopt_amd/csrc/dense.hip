@@ -91,24 +91,7 @@ __global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int run
     }
 }
 
-// Adds the runs: eight columns of a workgroup by thirty-two lanes.
-__global__ __launch_bounds__(kBlock) void dense_fold_k(size_t runs, size_t N, const float *sums, float *dbias)
-{
-    __shared__ float red[32][9];
-    const int col = threadIdx.x & 7, lane = threadIdx.x >> 3;
-    const size_t c = (size_t)blockIdx.x * 8 + col;
-    float s = 0.0f;
-    if (c < N) {
-#pragma unroll 4
-        for (size_t i = lane; i < runs; i += 32) s += sums[i * N + c];
-    }
-    red[lane][col] = s;
-    __syncthreads();
-    if (lane == 0 && c < N) {
-        for (int i = 1; i < 32; i++) s += red[i][col];
-        dbias[c] = s;
-    }
-}
+__global__ __launch_bounds__(kBlock) void dense_fold_k(DenseFold f) { dense_fold(f, blockIdx.x); }
 
 int check(const char *who, size_t M, size_t N, size_t K, int act)
 {
@@ -147,7 +130,10 @@ int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, co
                      "dopt_hip_dense_act: a result overlaps an operand");
     DOPT_REQUIRE(!overlaps(y, out, pre, out), "dopt_hip_dense_act: y and pre overlap");
     const DenseEpilogue e{bias, residual, pre, act, N};
-    if (dense_wide_takes(M, N, K)) return dense_wide(M, N, K, {x, false}, {w, false}, e, y);
+    if (dense_wide_takes(M, N, K)) {
+        const WideProduct p{M, N, K, {x, false}, {w, false}, y};
+        return dense_wide(&p, 1, e, DenseFold{});
+    }
     return product_dense(M, N, K, x, w, e, y);
 }
 
@@ -174,15 +160,21 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     const size_t tiles = ceil_div(std::max(N, (size_t)1), (size_t)(64 * V));
     // enough workgroups to fill the chip, of sixteen rows and more
     const int runs = (int)std::max((size_t)1, std::min(ceil_div(M, (size_t)16), ceil_div((size_t)num_cus() * 8, tiles)));
-    const bool wide_x = dense_wide_takes(M, K, N), wide_w = dense_wide_takes(N, K, M);
+    // the products that dense_wide.hip takes, in its launches
+    WideProduct wide[2];
+    int wides = 0;
+    if (dx && dense_wide_takes(M, K, N)) wide[wides++] = WideProduct{M, K, N, {dz, false}, {w, true}, dx};
+    const bool wide_x = wides > 0;
+    if (dw && dense_wide_takes(N, K, M)) wide[wides++] = WideProduct{N, K, M, {dz, true}, {x, true}, dw};
+    const bool wide_w = wides > (int)wide_x;
     size_t held = 0;
     if (M * N > 0 && (!plain || dbias)) {
         // dz, its sums and what the products park beside them share one request, which none of them has to grow
         auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
         const size_t first = plain ? 0 : rounded(M * N * sizeof(float));
         held = first + rounded((size_t)runs * N * sizeof(float));
-        const size_t more = std::max(!dx ? 0 : wide_x ? dense_wide_scratch(M, K, N) : product_scratch(0, 0, M, K, N),
-                                     !dw ? 0 : wide_w ? dense_wide_scratch(N, K, M) : product_scratch(1, 0, N, K, M));
+        const size_t more = std::max({dense_wide_scratch(wide, wides), !dx || wide_x ? 0 : product_scratch(0, 0, M, K, N),
+                                      !dw || wide_w ? 0 : product_scratch(1, 0, N, K, M)});
         char *const to = (char *)workspace(held + more);
         if (!to) return DOPT_HIP_ERR_OOM;
         if (!plain) dz = (float *)to;
@@ -194,15 +186,19 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
             hipLaunchKernelGGL(dense_dz_k<1>, grid, dim3(kBlock), 0, stream(), M, N, runs, act, dy, pre, (float *)to, dbias ? sums : nullptr);
         DOPT_LAUNCH_CHECK();
     }
-    if (dbias && N > 0) {
-        hipLaunchKernelGGL(dense_fold_k, dim3((unsigned)ceil_div(N, (size_t)8)), dim3(kBlock), 0, stream(), sums ? (size_t)runs : 0, N, sums, dbias);
+    const DenseFold fold{sums ? (size_t)runs : 0, N, sums, N > 0 ? dbias : nullptr};
+    if (fold.dbias && !wides) {
+        hipLaunchKernelGGL(dense_fold_k, dim3((unsigned)ceil_div(N, (size_t)8)), dim3(kBlock), 0, stream(), fold);
         DOPT_LAUNCH_CHECK();
     }
     workspace_hold(held);
     int rc = DOPT_HIP_OK;
-    const DenseEpilogue none{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K};
-    if (dx && M * K > 0) rc = wide_x ? dense_wide(M, K, N, {dz, false}, {w, true}, none, dx) : dopt_hip_sgemm_t(0, 0, M, K, N, dz, w, dx);
-    if (!rc && dw && N * K > 0) rc = wide_w ? dense_wide(N, K, M, {dz, true}, {x, true}, none, dw) : dopt_hip_sgemm_t(1, 0, N, K, M, dz, x, dw);
+    if (wides) {
+        for (int i = 0; i < wides; i++) wide[i].x.values = dz;
+        rc = dense_wide(wide, wides, DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, fold);
+    }
+    if (!rc && dx && !wide_x && M * K > 0) rc = dopt_hip_sgemm_t(0, 0, M, K, N, dz, w, dx);
+    if (!rc && dw && !wide_w && N * K > 0) rc = dopt_hip_sgemm_t(1, 0, N, K, M, dz, x, dw);
     workspace_hold(0);
     return rc;
 }

@@ -22,14 +22,17 @@ using namespace dopt;
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 256, kThreads = 512, kStages = 4, kStage = 32768;
+constexpr int kBig = 256, kSmall = 128;   // sides of tiles
 constexpr int kInf = 1 << 20, kNan = 1 << 21;   // in a row's shift: it holds infinities, NaN
 
 struct Operand {
     const float *x;
-    size_t rows, padded;
+    size_t rows, padded, K, steps;
     char *parts;
-    int *shift;   // of each row: it is held times 2^shift
+    int *shift;         // of each row: it is held times 2^shift
+    unsigned *tops;     // of one that lies across: the largest magnitudes of its runs, [run][row]
+    int runs;
+    unsigned blocks;    // of a launch
 };
 
 // (by value: of an element of a vector the builtin takes the first one's bits)
@@ -59,11 +62,10 @@ __device__ __forceinline__ void store_parts(char *block, int row, int half, cons
 // in a line.  Bound by memory; read twice, through an L2 that holds no row for so long, [8192 + 4096] rows of 4096 took 106 us.
 // Longer rows than the registers hold are.  Padding and rows that are not finite become zeros.
 constexpr int kUnits = 8;
-__global__ __launch_bounds__(1024) void wide_split_k(Operand a, Operand b, unsigned blocks_a, size_t K, size_t steps)
+__device__ __forceinline__ void split_rows(const Operand &o, unsigned block)
 {
     __shared__ unsigned tops[16][4];
-    const Operand o = blockIdx.x < blocks_a ? a : b;
-    const size_t row0 = (size_t)(blockIdx.x < blocks_a ? blockIdx.x : blockIdx.x - blocks_a) * 4;
+    const size_t row0 = (size_t)block * 4, K = o.K, steps = o.steps;
     const int lane = threadIdx.x & 63, r = threadIdx.x >> 1 & 3, half = threadIdx.x & 1, waves = blockDim.x >> 6;
     const size_t stride = blockDim.x / 8, s0 = threadIdx.x / 8;
     const bool inside = row0 + r < o.rows;
@@ -124,18 +126,27 @@ __global__ __launch_bounds__(1024) void wide_split_k(Operand a, Operand b, unsig
 
 // Operands that lie across the reduction, [K][rows]: the largest values of runs of K for each column, then a tile of 64 steps by 64 columns
 // per workgroup, turned in LDS.
-constexpr int kRuns = 32;
-struct Across {
-    Operand o;
-    unsigned *tops;   // [run][row]
-    unsigned tiles;   // of 256 columns; of 64 columns, padding included
+constexpr int kRuns = 32, kAcross = 3;
+struct Tops {
+    Operand o[kAcross];
+    int n;
+};
+struct Layout {
+    Operand rows[2], across[kAcross];
+    int nrows, nacross;
+    DenseFold fold;   // rides behind them
 };
 
-__global__ __launch_bounds__(256) void wide_tops_k(Across a, size_t K, int runs)
+__global__ __launch_bounds__(256) void wide_tops_k(Tops t)
 {
     __shared__ unsigned red[4][256];
-    const size_t col = min((size_t)(blockIdx.x % a.tiles) * 256 + (threadIdx.x & 63) * 4, a.o.rows - 4), run = blockIdx.x / a.tiles;
-    const size_t from = K * run / runs, to = K * (run + 1) / runs;
+    unsigned block = blockIdx.x;
+    int which = 0;
+    while (which + 1 < t.n && block >= t.o[which].blocks) block -= t.o[which++].blocks;
+    const Operand &o = t.o[which];
+    const unsigned tiles = (unsigned)((o.rows + 255) / 256);
+    const size_t col = min((size_t)(block % tiles) * 256 + (threadIdx.x & 63) * 4, o.rows - 4), run = block / tiles;
+    const size_t from = o.K * run / o.runs, to = o.K * (run + 1) / o.runs;
     const int row = threadIdx.x >> 6;
     unsigned top[4] = {0, 0, 0, 0};
     size_t k = from + row;
@@ -146,11 +157,11 @@ __global__ __launch_bounds__(256) void wide_tops_k(Across a, size_t K, int runs)
     for (; k + 28 < to; k += 32) {
         v4f v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = *(const v4f_any *)(a.o.x + (k + 4 * i) * a.o.rows + col);
+        for (int i = 0; i < 8; i++) v[i] = *(const v4f_any *)(o.x + (k + 4 * i) * o.rows + col);
 #pragma unroll
         for (int i = 0; i < 8; i++) see(v[i]);
     }
-    for (; k < to; k += 4) see(*(const v4f_any *)(a.o.x + k * a.o.rows + col));
+    for (; k < to; k += 4) see(*(const v4f_any *)(o.x + k * o.rows + col));
 #pragma unroll
     for (int e = 0; e < 4; e++) red[row][(threadIdx.x & 63) * 4 + e] = top[e];
     __syncthreads();
@@ -158,28 +169,29 @@ __global__ __launch_bounds__(256) void wide_tops_k(Across a, size_t K, int runs)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const int c = (threadIdx.x & 63) * 4 + e;
-        a.tops[run * a.o.rows + col + e] = max(max(red[0][c], red[1][c]), max(red[2][c], red[3][c]));
+        o.tops[run * o.rows + col + e] = max(max(red[0][c], red[1][c]), max(red[2][c], red[3][c]));
     }
 }
 
-__global__ __launch_bounds__(256) void wide_turn_k(Across a, size_t K, size_t steps, int runs)
+__device__ __forceinline__ void turn_tile(const Operand &o, unsigned block)
 {
     __shared__ float tile[64][65];
     __shared__ unsigned tops[4][64];
-    const size_t c0 = (size_t)(blockIdx.x % a.tiles) * 64, k0 = (size_t)(blockIdx.x / a.tiles) * 64;
+    const unsigned tiles = (unsigned)(o.padded / 64);
+    const size_t K = o.K, steps = o.steps, c0 = (size_t)(block % tiles) * 64, k0 = (size_t)(block / tiles) * 64;
     const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const size_t col = min(c0 + c, a.o.rows - 1);
+    const size_t col = min(c0 + c, o.rows - 1);
     float v[16];
 #pragma unroll
-    for (int u = 0; u < 16; u++) v[u] = a.o.x[min(k0 + w + 4 * u, K - 1) * a.o.rows + col];
+    for (int u = 0; u < 16; u++) v[u] = o.x[min(k0 + w + 4 * u, K - 1) * o.rows + col];
     unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < kRuns / 4; i++) top = max(top, a.tops[min(w + 4 * i, runs - 1) * a.o.rows + col]);
+    for (int i = 0; i < kRuns / 4; i++) top = max(top, o.tops[min(w + 4 * i, o.runs - 1) * o.rows + col]);
     tops[w][c] = top;
     __syncthreads();
-    const bool inside = c0 + c < a.o.rows;
+    const bool inside = c0 + c < o.rows;
     const int shift = inside ? shift_of(max(max(tops[0][c], tops[1][c]), max(tops[2][c], tops[3][c]))) : 0;
-    if (k0 == 0 && w == 0) a.o.shift[c0 + c] = shift;
+    if (k0 == 0 && w == 0) o.shift[c0 + c] = shift;
 #pragma unroll
     for (int u = 0; u < 16; u++) {
         const int k = w + 4 * u;
@@ -194,8 +206,22 @@ __global__ __launch_bounds__(256) void wide_turn_k(Across a, size_t K, size_t st
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) p[e] = tile[w * 16 + half * 8 + e][r];
-        store_parts(a.o.parts + ((c0 + r) / 32 * steps + step) * 2048, r & 31, half, p);
+        store_parts(o.parts + ((c0 + r) / 32 * steps + step) * 2048, r & 31, half, p);
     }
+}
+
+__global__ __launch_bounds__(1024) void wide_layout_k(Layout l)
+{
+    unsigned block = blockIdx.x;
+    for (int i = 0; i < l.nrows; i++) {
+        if (block < l.rows[i].blocks) return split_rows(l.rows[i], block);
+        block -= l.rows[i].blocks;
+    }
+    for (int i = 0; i < l.nacross; i++) {
+        if (block < l.across[i].blocks) return turn_tile(l.across[i], block);
+        block -= l.across[i].blocks;
+    }
+    dense_fold(l.fold, block);
 }
 
 struct Wide {
@@ -204,20 +230,26 @@ struct Wide {
     size_t xm, xk, wn, wk;   // between rows, between steps
     const char *xp, *wp;
     const int *xs, *ws;
-    unsigned tiles, mtiles, ntiles;
+    float *y, *to;           // the result; the sums of splits, [split][M][N], where there are several
+    unsigned tiles, mtiles, ntiles, splits;
+};
+struct Wides {
+    Wide q[2];
+    unsigned blocks;   // of both
 };
 
 // What is not finite in a tile's operands: the sums of those rows and columns as fp32 instructions make them.
-__device__ __noinline__ void rough_sums(Wide q, DenseEpilogue ep, float *y, size_t m0, size_t n0, const int *shift)
+template <int kTile>
+__device__ __noinline__ void rough_sums(Wide q, DenseEpilogue ep, float *y, size_t m0, size_t n0, size_t from, size_t to, const int *shift)
 {
-    for (int i = threadIdx.x; i < kTile * kTile; i += kThreads) {
+    for (int i = threadIdx.x; i < kTile * kTile; i += 2 * kTile) {
         const size_t m = m0 + i / kTile, n = n0 + i % kTile;
         const int most = max(shift[i / kTile], shift[kTile + i % kTile]);
         if (m >= q.M || n >= q.N || most < kInf) continue;
         const bool nan = most == kNan;
         float s = nan ? __builtin_nanf("") : 0.0f;
         if (!nan)
-            for (size_t k = 0; k < q.K; k++) s += q.x[m * q.xm + k * q.xk] * q.w[n * q.wn + k * q.wk];
+            for (size_t k = from; k < to; k++) s += q.x[m * q.xm + k * q.xk] * q.w[n * q.wn + k * q.wk];
         y[m * q.N + n] = ep(s, m * q.N + n);
     }
 }
@@ -231,43 +263,36 @@ __device__ __forceinline__ void phase()
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// A tile of 256 x 256 by eight wavefronts of 128 x 64: the accumulators are half of the registers, and a stage of 16 steps, 32 KB, feeds
-// 24 matrix instructions of each.  Three stages are on their way behind the one in use.
-__global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilogue ep, float *y)
+// A stage of 16 steps of both sides of a tile: a wavefront brings a row of blocks of each.
+__device__ __forceinline__ void bring_both(const char *left, const char *right, int k, int w, int lane, int sides, char *to)
 {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    unsigned id;
-    if (!xcd_remap(blockIdx.x, q.tiles, &id)) return;
-    // eight rows of tiles together, column by column: what an XCD works on at a time shares rows and columns
-    const unsigned band = 8 * q.ntiles, first = id / band * 8, high = min(8u, q.mtiles - first);
-    const unsigned mt = first + id % band % high, nt = id % band / high;
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w >> 2, wn = w & 3;
-    const size_t row_of_blocks = q.steps * 2048;
-    const char *const left = q.xp + (mt * 8 + w) * row_of_blocks, *const right = q.wp + (nt * 8 + w) * row_of_blocks;
-    v16f acc[4][2];
-    zero_acc(acc);
-    auto bring_stage = [&](int k) {
-        char *const to = lds + (k & 3) * kStage;
-        bring(left + (size_t)k * 2048, 2, lane, to + w * 2048);
-        bring(right + (size_t)k * 2048, 2, lane, to + 16384 + w * 2048);
-    };
+    bring(left + (size_t)k * 2048, 2, lane, to + w * 2048);
+    bring(right + (size_t)k * 2048, 2, lane, to + sides + w * 2048);
+}
+
+// Tiles of 256 x 256 by eight wavefronts of 128 x 64: the accumulators are half of the registers, and a stage, 32 KB, feeds 24 matrix
+// instructions of each.  The halves of the workgroup, which share the CU's four SIMDs, read and multiply in turn; three
+// stages are on their way.
+__device__ __forceinline__ void sums(const char *left, const char *right, int steps, int w, int lane, char *lds, v16f (&acc)[4][2])
+{
+    const int wm = w >> 2, wn = w & 3;
     auto arrived = [&](int ahead) {   // all loads but those of the last `ahead` stages asked for
         if (ahead >= 2) settled<8>();
         else if (ahead == 1) settled<4>();
         else settled<0>();
     };
-    const int steps = (int)q.steps;
-    for (int k = 0; k < min(steps, 3); k++) bring_stage(k);
+    for (int k = 0; k < min(steps, 3); k++) bring_both(left, right, k, w, lane, 16384, lds + k * 32768);
     arrived(min(steps, 3) - 1);
     phase();
     if (wm) phase();
     for (int k = 0; k < steps; k++) {
         Side<4> a;
         Side<2> b;
-        const char *const now = lds + (k & 3) * kStage;
+        const char *const now = lds + (k & 3) * 32768;
         a.read(now + wm * 8192, lane);
         b.read(now + 16384 + wn * 4096, lane);
-        if (k + 3 < steps) bring_stage(k + 3);
+        // (into the stage that the other half read before this phase)
+        if (k + 3 < steps) bring_both(left, right, k + 3, w, lane, 16384, lds + ((k + 3) & 3) * 32768);
         if (wm) arrived(min(steps - 2 - k, 2));
         else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         phase();
@@ -279,14 +304,64 @@ __global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilo
     }
     if (!wm) phase();
     meet();
+}
+
+// Tiles of 128 x 128 by four of 64 x 64, two workgroups to a CU.
+__device__ __forceinline__ void sums(const char *left, const char *right, int steps, int w, int lane, char *lds, v16f (&acc)[2][2])
+{
+    pipeline<5, 16384, 4, 2, 2>(
+        lds, steps, [&](int k, char *to) { bring_both(left, right, k, w, lane, 8192, to); },
+        [&](const char *now, Side<2> &a, Side<2> &b) {
+            a.read(now + (w >> 1) * 4096, lane);
+            b.read(now + 8192 + (w & 1) * 4096, lane);
+        },
+        [&](const Side<2> &a, const Side<2> &b) { multiply(a, b, acc); });
+}
+
+template <int kTile>
+constexpr int kLdsOf = kTile == kBig ? 4 * 32768 : 5 * 16384;
+
+template <int kTile>
+__global__ __launch_bounds__(2 * kTile, 2) void wide_product_k(Wides both, DenseEpilogue ep)
+{
+    constexpr int MI = kTile / 64, kBlocks = kTile / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    unsigned id;
+    if (!xcd_remap(blockIdx.x, both.blocks, &id)) return;
+    const unsigned before = both.q[0].tiles * both.q[0].splits;
+    const bool second = id >= before;
+    const Wide q = both.q[second];
+    if (second) id -= before;
+    const unsigned split = id / q.tiles;
+    id %= q.tiles;
+    const size_t from = q.steps * split / q.splits, to = q.steps * (split + 1) / q.splits;
+    float *const y = q.splits > 1 ? q.to + split * q.M * q.N : q.y;
+    if (q.splits > 1) ep = DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, q.N};   // it rides in the sum over the splits
+    // eight rows of tiles together, column by column: what an XCD works on at a time shares rows and columns
+    const unsigned band = 8 * q.ntiles, first = id / band * 8, high = min(8u, q.mtiles - first);
+    const unsigned mt = first + id % band % high, nt = id % band / high;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wm = kTile == kBig ? w >> 2 : w >> 1, wn = kTile == kBig ? w & 3 : w & 1;
+    const size_t row_of_blocks = q.steps * 2048;
+    v16f acc[MI][2];
+    zero_acc(acc);
+    sums(q.xp + (mt * kBlocks + w) * row_of_blocks + from * 2048, q.wp + (nt * kBlocks + w) * row_of_blocks + from * 2048, (int)(to - from), w, lane, lds,
+         acc);
 
     int *const shift = (int *)lds;
     const size_t m0 = (size_t)mt * kTile, n0 = (size_t)nt * kTile;
     const int mine = threadIdx.x < kTile ? q.xs[m0 + threadIdx.x] : q.ws[n0 + threadIdx.x - kTile];
     shift[threadIdx.x] = mine;
-    const bool rough = __syncthreads_or(mine >= kInf);
+    // (whether any is not finite; the library's vote over a workgroup has LDS of its own, which would leave a CU one of them)
+    const bool some = __any(mine >= kInf);
+    if (lane == 0) shift[2 * kTile + w] = some;
+    meet();
+    bool rough = false;
+#pragma unroll
+    for (int i = 0; i < kTile / 32; i++) rough = rough || shift[2 * kTile + i];
+    rough = __builtin_amdgcn_readfirstlane(rough);
     // 32 rows at a time through LDS, so that a row's 64 values are stored by sixteen lanes
-    float *const image = (float *)(lds + 2048) + w * (32 * 68);
+    float *const image = (float *)(lds + 2304) + w * (32 * 68);
     const bool inside = m0 + kTile <= q.M && n0 + kTile <= q.N && !rough;
     const size_t left_col = n0 + wn * 64;   // of the wavefront's 64
     // values one by one: beside values that are not finite, and where the matrix ends within the wavefront's first three columns
@@ -303,13 +378,13 @@ __global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilo
     }
     // (a loop, whose sums move down: its code unrolled, for each activation, costs more to fetch than 96 moves)
 #pragma unroll 1
-    for (int i = 0; i < 4 && left_col < q.N; i++) {
+    for (int i = 0; i < MI && left_col < q.N; i++) {
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) image[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * 68 + 32 * j + (lane & 31)] = acc[0][j][e];
         asm volatile("" ::: "memory");   // (a wavefront's LDS accesses stay in their order)
-        const int r0 = wm * 128 + i * 32 + (lane >> 4);
+        const int r0 = wm * (kTile / 2) + i * 32 + (lane >> 4);
         with_activation(ep.act, [&](auto kind) {
             auto quads = [&](auto whole) {   // whole: nothing ends within the tile
                 constexpr bool kWhole = decltype(whole)::value;
@@ -361,11 +436,102 @@ __global__ __launch_bounds__(kThreads, 2) void wide_product_k(Wide q, DenseEpilo
         });
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int k = 0; k < 3; k++)
+        for (int k = 0; k + 1 < MI; k++)
 #pragma unroll
             for (int j = 0; j < 2; j++) acc[k][j] = acc[k + 1][j];
     }
-    if (rough) rough_sums(q, ep, y, m0, n0, shift);
+    if (rough) rough_sums<kTile>(q, ep, y, m0, n0, from * 16, min(to * 16, q.K), shift);
+}
+
+// Adds the splits of up to two products and ends them, four values at a time; the last four end with the product, whatever of them the
+// quad before has written too.
+__global__ __launch_bounds__(256) void wide_join_k(Wides both, DenseEpilogue ep)
+{
+    auto quads_of = [](const Wide &q) { return q.splits > 1 ? (q.M * q.N + 3) / 4 : 0; };
+    const size_t n0 = quads_of(both.q[0]), n1 = quads_of(both.q[1]);
+    with_activation(ep.act, [&](auto kind) {
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n0 + n1; i += (size_t)gridDim.x * 256) {
+            const Wide &q = both.q[i >= n0];
+            const size_t n = q.M * q.N, at = min(4 * (i >= n0 ? i - n0 : i), n - 4);
+            v4f z = *(const v4f_any *)(q.to + at), o;
+#pragma unroll 4
+            for (unsigned p = 1; p < q.splits; p++) z += *(const v4f_any *)(q.to + p * n + at);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (ep.bias) z[e] += ep.bias[(at + e) % q.N];
+                o[e] = act_value<kind.value>(z[e]);
+            }
+            if (ep.pre) *(v4f_any *)(ep.pre + at) = z;
+            if (ep.residual) o += *(const v4f_any *)(ep.residual + at);
+            *(v4f_any *)(q.y + at) = o;
+        }
+    });
+}
+
+// The side of the tiles that suit a product; 0: none here.
+int tile_for(size_t M, size_t N, size_t K)
+{
+    const size_t tiles = ceil_div(M, (size_t)kBig) * ceil_div(N, (size_t)kBig), rounds = ceil_div(tiles, (size_t)num_cus());
+    if (K < 128 || tiles >= (size_t)1 << 28) return 0;
+    if (M >= 512 && N >= 512 && M * N * 3 >= rounds * num_cus() * kBig * kBig) return kBig;
+    return std::min(M, N) >= 256 && K <= 8 * std::min(M, N) && M * N * K >= (size_t)900000000 ? kSmall : 0;
+}
+
+template <int kTile>
+int launch_tiles(const Wides &both, const DenseEpilogue &e)
+{
+    static bool raised = false;
+    if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)wide_product_k<kTile>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsOf<kTile>));
+    raised = true;
+    hipLaunchKernelGGL(wide_product_k<kTile>, dim3(xcd_grid(both.blocks)), dim3(2 * kTile), kLdsOf<kTile>, stream(), both, e);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+int launch_products(int tile, const Wide *q, int n, const DenseEpilogue &e)
+{
+    Wides both{{q[0], q[n - 1]}, q[0].tiles * q[0].splits + (n == 2 ? q[1].tiles * q[1].splits : 0)};
+    if (int rc = tile == kBig ? launch_tiles<kBig>(both, e) : launch_tiles<kSmall>(both, e)) return rc;
+    if (n == 1) both.q[1].splits = 1;
+    size_t values = 0;
+    for (const Wide &p : both.q) values += p.splits > 1 ? p.M * p.N : 0;
+    if (!values) return DOPT_HIP_OK;
+    hipLaunchKernelGGL(wide_join_k, dim3((unsigned)std::min(ceil_div(values, (size_t)1024), (size_t)num_cus() * 16)), dim3(256), 0, stream(), both, e);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+// Into how many parts the reductions of products in tiles of 128 x 128 are cut.  A stage takes 0.4 us where a CU has one workgroup, two
+// of them 0.6; the sums of parts are written and read at about 6 TB/s, and adding them is a launch.  ([1024 x 1024] from 4096
+// steps in eight parts 56 us, in one 112; [2048 x 2048] from 512 steps in two 47, in one 36.)
+void cut(const WideProduct *p, int n, unsigned *splits)
+{
+    size_t stages[2] = {0, 0}, tiles[2] = {0, 0};
+    unsigned now[2] = {1, 1};
+    for (int i = 0; i < n; i++) {
+        splits[i] = 1;
+        if (tile_for(p[i].M, p[i].N, p[i].K) != kSmall) continue;
+        stages[i] = ceil_div(p[i].K, (size_t)16);
+        tiles[i] = ceil_div(p[i].M, (size_t)kSmall) * ceil_div(p[i].N, (size_t)kSmall);
+    }
+    double least = 0.0;
+    for (;;) {   // the longest one is cut further
+        size_t blocks = 0, longest = 0, bytes = 0;
+        for (int i = 0; i < n; i++) {
+            blocks += tiles[i] * now[i];
+            longest = std::max(longest, ceil_div(stages[i], (size_t)now[i]));
+            bytes += now[i] > 1 ? (2 * now[i] + 1) * p[i].M * p[i].N * sizeof(float) : 0;
+        }
+        const double us = (double)longest * (blocks <= (size_t)num_cus() ? 0.4 : 0.6 * (double)ceil_div(blocks, (size_t)num_cus() * 2)) +
+                          (bytes ? 5.0 + (double)bytes / 6e6 : 0.0);
+        if (least == 0.0 || us < least) {
+            least = us;
+            for (int i = 0; i < n; i++) splits[i] = now[i];
+        }
+        const int i = n == 2 && stages[1] * now[0] > stages[0] * now[1];
+        if (blocks + tiles[i] > (size_t)num_cus() * 2 || stages[i] < (size_t)16 * (now[i] + 1)) return;
+        now[i]++;
+    }
 }
 
 }  // namespace
@@ -375,60 +541,88 @@ namespace dopt {
 // Where a third of the chip's places for tiles are taken.  us here and on three bf16 parts, with 128, 512 and 1024 steps:
 //     [1024 x 4096] 36 57 84 and 29 51 85    [1500 x 4096] 37 63 93 and 36 69 113    [4096 x 2500] 55 77 109 and 91 153 198
 //     [4096 x 4097] 96 142 210 and 140 234 362    [8192 x 4096] 130 187 268 and 160 308 472
-bool dense_wide_takes(size_t M, size_t N, size_t K)
-{
-    const size_t tiles = ceil_div(M, (size_t)kTile) * ceil_div(N, (size_t)kTile), rounds = ceil_div(tiles, (size_t)num_cus());
-    return M >= 512 && N >= 512 && K >= 128 && tiles < ((size_t)1 << 30) && M * N * 3 >= rounds * num_cus() * kTile * kTile;
-}
+bool dense_wide_takes(size_t M, size_t N, size_t K) { return tile_for(M, N, K) != 0; }
 
-size_t dense_wide_scratch(size_t M, size_t N, size_t K)
+size_t dense_wide_scratch(const WideProduct *p, int n)
 {
-    const size_t mp = ceil_div(M, (size_t)kTile) * kTile, np = ceil_div(N, (size_t)kTile) * kTile;
-    return (mp + np) * (ceil_div(K, (size_t)16) * 64 + sizeof(int)) + kRuns * std::max(M, N) * sizeof(unsigned);
-}
-
-int dense_wide(size_t M, size_t N, size_t K, const WideSide &x, const WideSide &w, const DenseEpilogue &e, float *y)
-{
-    const size_t mp = ceil_div(M, (size_t)kTile) * kTile, np = ceil_div(N, (size_t)kTile) * kTile, steps = ceil_div(K, (size_t)16);
-    char *const to = (char *)workspace(dense_wide_scratch(M, N, K));
-    if (!to) return DOPT_HIP_ERR_OOM;
-    char *const xp = to, *const wp = xp + mp * steps * 64;
-    int *const xs = (int *)(wp + np * steps * 64), *const ws = xs + mp;
-    unsigned *const tops = (unsigned *)(ws + np);
-    const Operand both[] = {{x.values, M, mp, xp, xs}, {w.values, N, np, wp, ws}};
-    const unsigned threads = steps > 512 ? 1024 : steps > 256 ? 512 : 256;   // rows in registers up to 16384
-    if (!x.across && !w.across) {   // in one launch
-        const unsigned blocks = (unsigned)(mp / 4);
-        hipLaunchKernelGGL(wide_split_k, dim3(blocks + (unsigned)(np / 4)), dim3(threads), 0, stream(), both[0], both[1], blocks, K, steps);
-        DOPT_LAUNCH_CHECK();
-    } else {
-        const bool across[] = {x.across, w.across};
-        for (int i = 0; i < 2; i++) {
-            const Operand &o = both[i];
-            if (!across[i]) {
-                const unsigned blocks = (unsigned)(o.padded / 4);
-                hipLaunchKernelGGL(wide_split_k, dim3(blocks), dim3(threads), 0, stream(), o, o, blocks, K, steps);
-                DOPT_LAUNCH_CHECK();
-                continue;
-            }
-            const int runs = (int)std::min((size_t)kRuns, ceil_div(K, (size_t)64));
-            Across a{o, tops, (unsigned)ceil_div(o.rows, (size_t)256)};
-            hipLaunchKernelGGL(wide_tops_k, dim3(a.tiles * runs), dim3(256), 0, stream(), a, K, runs);
-            DOPT_LAUNCH_CHECK();
-            a.tiles = (unsigned)(o.padded / 64);
-            hipLaunchKernelGGL(wide_turn_k, dim3(a.tiles * (unsigned)ceil_div(steps, (size_t)4)), dim3(256), 0, stream(), a, K, steps, runs);
-            DOPT_LAUNCH_CHECK();
-        }
+    size_t bytes = 0;
+    unsigned splits[2];
+    cut(p, n, splits);
+    for (int i = 0; i < n; i++) {
+        const size_t tile = tile_for(p[i].M, p[i].N, p[i].K), K = ceil_div(p[i].K, (size_t)16) * 64 + sizeof(int);
+        const size_t mp = ceil_div(p[i].M, tile) * tile, np = ceil_div(p[i].N, tile) * tile;
+        if (splits[i] > 1) bytes += (splits[i] * p[i].M * p[i].N * sizeof(float) + 255) / 256 * 256;
+        bytes += (mp + np) * K + kRuns * ((p[i].x.across ? mp : 0) + (p[i].w.across ? np : 0)) * sizeof(unsigned);
     }
-    static bool raised = false;
-    if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)wide_product_k, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStage));
-    raised = true;
-    const unsigned mt = (unsigned)(mp / kTile), nt = (unsigned)(np / kTile);
-    hipLaunchKernelGGL(wide_product_k, dim3(xcd_grid(mt * nt)), dim3(kThreads), kStages * kStage, stream(),
-                       Wide{M, N, K, steps, x.values, w.values, x.across ? 1 : K, x.across ? M : 1, w.across ? 1 : K, w.across ? N : 1, xp, wp, xs, ws, mt * nt,
-                            mt, nt},
-                       e, y);
-    DOPT_LAUNCH_CHECK();
+    return bytes;
+}
+
+int dense_wide(const WideProduct *p, int n, const DenseEpilogue &e, const DenseFold &fold)
+{
+    char *to = (char *)workspace(dense_wide_scratch(p, n));
+    if (!to) return DOPT_HIP_ERR_OOM;
+    Layout l{};
+    Tops tops{};
+    Wide q[2];
+    int tile[2];
+    unsigned splits[2];
+    cut(p, n, splits);
+    unsigned top_blocks = 0, row_blocks = 0, blocks = 0;
+    size_t longest = 0;
+    for (int i = 0; i < n; i++) {
+        const WideProduct &g = p[i];
+        tile[i] = tile_for(g.M, g.N, g.K);
+        Operand sides[2];
+        for (int k = 0; k < 2; k++) {
+            const WideSide &side = k ? g.w : g.x;
+            const size_t rows = k ? g.N : g.M, padded = ceil_div(rows, (size_t)tile[i]) * tile[i], steps = ceil_div(g.K, (size_t)16);
+            Operand o{side.values, rows, padded, g.K, steps, to, (int *)(to + padded * steps * 64), nullptr, 0, 0};
+            to += padded * (steps * 64 + sizeof(int));
+            if (side.across) {
+                o.runs = (int)std::min((size_t)kRuns, ceil_div(g.K, (size_t)64));
+                o.tops = (unsigned *)to;
+                to += kRuns * padded * sizeof(unsigned);
+                o.blocks = (unsigned)(ceil_div(rows, (size_t)256) * o.runs);
+                top_blocks += o.blocks;
+                tops.o[tops.n++] = o;
+                o.blocks = (unsigned)(padded / 64 * ceil_div(steps, (size_t)4));
+                blocks += o.blocks;
+                l.across[l.nacross++] = o;
+            } else {
+                o.blocks = (unsigned)(padded / 4);
+                row_blocks += o.blocks;
+                longest = std::max(longest, steps);
+                l.rows[l.nrows++] = o;
+            }
+            sides[k] = o;
+        }
+        const unsigned mt = (unsigned)(sides[0].padded / tile[i]), nt = (unsigned)(sides[1].padded / tile[i]);
+        q[i] = Wide{g.M, g.N, g.K, sides[0].steps, g.x.values, g.w.values, g.x.across ? 1 : g.K, g.x.across ? g.M : 1, g.w.across ? 1 : g.K,
+                    g.w.across ? g.N : 1, sides[0].parts, sides[1].parts, sides[0].shift, sides[1].shift, g.y, (float *)to, mt * nt, mt, nt, splits[i]};
+        if (splits[i] > 1) to += (splits[i] * g.M * g.N * sizeof(float) + 255) / 256 * 256;
+    }
+    if (tops.n) {
+        hipLaunchKernelGGL(wide_tops_k, dim3(top_blocks), dim3(256), 0, stream(), tops);
+        DOPT_LAUNCH_CHECK();
+    }
+    l.fold = fold;
+    blocks += fold.dbias ? (unsigned)ceil_div(fold.N, (size_t)8) : 0;
+    const unsigned threads = longest > 512 ? 1024 : longest > 256 ? 512 : 256;   // rows in registers up to 16384 steps
+    if (threads > 256) {   // by themselves
+        Layout rows = l;
+        rows.nacross = 0;
+        hipLaunchKernelGGL(wide_layout_k, dim3(row_blocks), dim3(threads), 0, stream(), rows);
+        DOPT_LAUNCH_CHECK();
+        l.nrows = 0;
+        row_blocks = 0;
+    }
+    if (row_blocks + blocks) {
+        hipLaunchKernelGGL(wide_layout_k, dim3(row_blocks + blocks), dim3(256), 0, stream(), l);
+        DOPT_LAUNCH_CHECK();
+    }
+    if (n == 2 && tile[0] == tile[1]) return launch_products(tile[0], q, 2, e);
+    for (int i = 0; i < n; i++)
+        if (int rc = launch_products(tile[i], q + i, 1, e)) return rc;
     return DOPT_HIP_OK;
 }
 

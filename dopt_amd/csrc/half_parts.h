@@ -77,6 +77,13 @@ struct Side {
     }
 };
 
+__device__ __forceinline__ v16f product(v8h ah, v8h al, v8h bh, v8h bl, v16f acc)
+{
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+}
+
 // acc[i][j] += block i of a times block j of b.
 template <int MI, int NI>
 __device__ __forceinline__ void multiply(const Side<MI> &a, const Side<NI> &b, v16f (&acc)[MI][NI])
@@ -84,11 +91,7 @@ __device__ __forceinline__ void multiply(const Side<MI> &a, const Side<NI> &b, v
 #pragma unroll
     for (int i = 0; i < MI; i++)
 #pragma unroll
-        for (int j = 0; j < NI; j++) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l[i], b.h[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h[i], b.l[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h[i], b.h[j], acc[i][j], 0, 0, 0);
-        }
+        for (int j = 0; j < NI; j++) acc[i][j] = product(a.h[i], a.l[i], b.h[j], b.l[j], acc[i][j]);
 }
 template <int MI, int NI>
 __device__ __forceinline__ void multiply(const char *A, const char *B, int lane, v16f (&acc)[MI][NI])
@@ -115,29 +118,44 @@ __device__ __forceinline__ void settled()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
 }
 
-// multiply_stage(stage in LDS) for each of `steps` stages, up to kStages - 1 of which are on their way ahead, kLoads loads of a
-// wavefront each: bring_stage(k, stage in LDS).  Once a wavefront's own part of stage k is there it meets the others: then
-// all of it is, and the stage before it has been read by everyone.
-template <int kStages, int kStage, int kLoads, class B, class F>
-__device__ __forceinline__ void pipeline(char *lds, int steps, B &&bring_stage, F &&multiply_stage)
+// multiply(a, b) for each of `steps` stages, which bring(k, stage in LDS) asks for, kLoads loads of a wavefront each, and of which
+// read(stage in LDS, a, b) takes the wavefront's blocks.  While a stage is multiplied the next one is read into other
+// registers; kStages - 1 further ones are on their way.  Once a wavefront's own part of stage k + 1 is there it meets the others: then
+// all of it is, and stage k has been read by everyone.
+template <int kStages, int kStage, int kLoads, int MI, int NI, class B, class R, class M>
+__device__ __forceinline__ void pipeline(char *lds, int steps, B &&bring_stage, R &&read, M &&multiply_blocks)
 {
     static_assert(kStages >= 3 && kStages <= 5 && kStages * kStage <= 163840, "one to three stages may be under way behind the next one");
-#pragma unroll
-    for (int k = 0; k < kStages - 1; k++)
-        if (k < steps) bring_stage(k, lds + k * kStage);
-    int at = 0, fill = kStages - 1;
-    for (int k = 0; k < steps; k++) {
-        const int behind = min(steps - 1 - k, kStages - 2);
-        if (behind == 3) settled<3 * kLoads>();
-        else if (behind == 2) settled<2 * kLoads>();
-        else if (behind == 1) settled<kLoads>();
+    auto arrived = [&](int behind) {   // all loads but those of the last `behind` stages asked for
+        if (kStages > 4 && behind >= 3) settled<3 * kLoads>();
+        else if (kStages > 3 && behind >= 2) settled<2 * kLoads>();
+        else if (behind >= 1) settled<kLoads>();
         else settled<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k + kStages - 1 < steps) bring_stage(k + kStages - 1, lds + fill * kStage);
-        multiply_stage(lds + at * kStage);
-        fill = at;
-        at = at + 1 == kStages ? 0 : at + 1;
+    };
+#pragma unroll
+    for (int k = 0; k < kStages - 1; k++)
+        if (k < steps) bring_stage(k, lds + k * kStage);
+    int at = 0, fill = kStages - 1;   // where the stage that was read last lies, and the next one asked for
+    arrived(min(steps - 1, kStages - 2));
+    Side<MI> a0, a1;
+    Side<NI> b0, b1;
+    read(lds, a0, b0);
+    if (kStages - 1 < steps) bring_stage(kStages - 1, lds + fill * kStage);
+    auto one = [&](int k, const Side<MI> &a, const Side<NI> &b, Side<MI> &next_a, Side<NI> &next_b) {
+        if (k + 1 < steps) {
+            arrived(min(steps - 2 - k, kStages - 2));
+            fill = at;
+            at = at + 1 == kStages ? 0 : at + 1;
+            read(lds + at * kStage, next_a, next_b);
+            if (k + kStages < steps) bring_stage(k + kStages, lds + fill * kStage);
+        }
+        multiply_blocks(a, b);
+    };
+    for (int k = 0; k < steps; k += 2) {
+        one(k, a0, b0, a1, b1);
+        if (k + 1 < steps) one(k + 1, a1, b1, a0, b0);
     }
     meet();   // the last stage has been read
 }

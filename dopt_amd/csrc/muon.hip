@@ -425,11 +425,15 @@ __global__ __launch_bounds__(kBlock, 2) void muon_product_k(const Matrix *jobs, 
         const char *const src = (w < 2 ? left + (size_t)(t.i * 2 + w) * row_of_blocks : right + (size_t)(t.j * 2 + w - 2) * row_of_blocks) + from;
         v16f acc[1][1];
         zero_acc(acc);
-        pipeline<5, 16384, 4>(
+        pipeline<5, 16384, 4, 2, 2>(   // (two blocks of steps at a time)
             lds, t.to - t.from, [&](int k, char *to) { bring(src + (size_t)k * 4096, 4, lane, to + w * 4096); },
-            [&](const char *now) {
+            [&](const char *now, Side<2> &a, Side<2> &b) {
+                a.read(now + wm * 4096, lane);
+                b.read(now + 8192 + wn * 4096, lane);
+            },
+            [&](const Side<2> &a, const Side<2> &b) {
 #pragma unroll
-                for (int s = 0; s < 2; s++) multiply(now + wm * 4096 + s * 2048, now + 8192 + wn * 4096 + s * 2048, lane, acc);
+                for (int s = 0; s < 2; s++) acc[0][0] = product(a.h[s], a.l[s], b.h[s], b.l[s], acc[0][0]);
             });
         finish_all<kProduct>(jobs, t, st, op, turn, acc, t.i * 64 + wm * 32, t.j * 64 + wn * 32, w, lane, images);
         return;
@@ -439,13 +443,17 @@ __global__ __launch_bounds__(kBlock, 2) void muon_product_k(const Matrix *jobs, 
             (w < 2 ? left + (size_t)(t.i * 4 + 2 * w) * row_of_blocks : right + (size_t)(t.j * 4 + 2 * w - 4) * row_of_blocks) + from;
         v16f acc[2][2];
         zero_acc(acc);
-        pipeline<5, 16384, 4>(
+        pipeline<5, 16384, 4, 2, 2>(
             lds, 2 * (t.to - t.from),
             [&](int k, char *to) {
                 bring(src + (size_t)k * 2048, 2, lane, to + w * 4096);
                 bring(src + row_of_blocks + (size_t)k * 2048, 2, lane, to + w * 4096 + 2048);
             },
-            [&](const char *now) { multiply(now + wm * 4096, now + 8192 + wn * 4096, lane, acc); });
+            [&](const char *now, Side<2> &a, Side<2> &b) {
+                a.read(now + wm * 4096, lane);
+                b.read(now + 8192 + wn * 4096, lane);
+            },
+            [&](const Side<2> &a, const Side<2> &b) { multiply(a, b, acc); });
         finish_all<kProduct>(jobs, t, st, op, turn, acc, t.i * 128 + wm * 64, t.j * 128 + wn * 64, w, lane, images);
     } else {   // four rows of blocks on the left, eight on the right (the last one again where X ends), three for each wavefront
         const int last = t.lp / 32 - 1;
@@ -457,13 +465,17 @@ __global__ __launch_bounds__(kBlock, 2) void muon_product_k(const Matrix *jobs, 
         }
         v16f acc[2][4];
         zero_acc(acc);
-        pipeline<3, 24576, 6>(
+        pipeline<3, 24576, 6, 2, 4>(
             lds, 2 * (t.to - t.from),
             [&](int k, char *to) {
 #pragma unroll
                 for (int b = 0; b < 3; b++) bring(src[b] + (size_t)k * 2048, 2, lane, to + (3 * w + b) * 2048);
             },
-            [&](const char *now) { multiply(now + wm * 4096, now + 8192 + wn * 8192, lane, acc); });
+            [&](const char *now, Side<2> &a, Side<4> &b) {
+                a.read(now + wm * 4096, lane);
+                b.read(now + 8192 + wn * 8192, lane);
+            },
+            [&](const Side<2> &a, const Side<4> &b) { multiply(a, b, acc); });
         finish_all<kProduct>(jobs, t, st, op, turn, acc, t.i * 128 + wm * 64, t.j * 256 + wn * 128, w, lane, images);
     }
 }

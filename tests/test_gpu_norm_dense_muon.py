@@ -206,7 +206,8 @@ def test_group_norm_refusals():
 # m, n, k
 DENSES = [(1, 1, 1), (1, 10, 16), (1, 4096, 512), (1, 333, 1025), (2, 3, 5), (7, 64, 100), (33, 65, 127), (64, 512, 784), (130, 70, 1), (256, 10, 512),
           (300, 1, 77), (129, 257, 130), (512, 512, 512), (1000, 130, 260), (257, 300, 2050), (64, 2000, 1030), (520, 1030, 1500), (1024, 1024, 512), (1030, 1100, 530),
-          (1300, 1281, 1111), (2560, 2304, 512), (2497, 2370, 131), (2370, 2497, 400)]
+          (1300, 1281, 1111), (2560, 2304, 512), (2497, 2370, 131), (2370, 2497, 400),
+          (1024, 1024, 2100), (300, 2001, 2000)]
 
 
 def _dense_case(m, n, k, seed):
@@ -270,7 +271,7 @@ def test_dense_act_of_nothing():
     assert dx.size == 0 and not dw.numpy().any() and not db.numpy().any()
 
 
-@pytest.mark.parametrize("size", [(1, 64, 300), (40, 50, 300), (300, 300, 300), (300, 520, 1200), (1030, 1100, 530), (2500, 2403, 140)], ids=str)
+@pytest.mark.parametrize("size", [(1, 64, 300), (40, 50, 300), (300, 300, 300), (300, 520, 1200), (1030, 1100, 530), (1030, 1100, 1000), (2500, 2403, 140)], ids=str)
 def test_dense_act_with_values_that_are_not_finite(size):
     m, n, k = size
     x, w, b, res, _ = _dense_case(m, n, k, 12)
@@ -313,7 +314,7 @@ def test_dense_act_of_long_rows():
     R.close(y, R.dense_act(x, w, b, None, "silu")[0], "y")
 
 
-@pytest.mark.parametrize("size", [(2400, 2411, 2421), (2563, 300, 2500), (2499, 2305, 130)], ids=str)
+@pytest.mark.parametrize("size", [(2400, 2411, 2421), (2563, 300, 2500), (2499, 2305, 130), (1000, 1777, 1111)], ids=str)
 def test_dense_act_gradient_of_large_layers(size):
     m, n, k = size
     x, w, _, pre, dy = _dense_case(m, n, k, 16)
