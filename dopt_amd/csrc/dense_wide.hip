@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256) void wide_join_k(Wides both, DenseEpilogue ep)
 int tile_for(size_t M, size_t N, size_t K)
 {
     const size_t tiles = ceil_div(M, (size_t)kBig) * ceil_div(N, (size_t)kBig), rounds = ceil_div(tiles, (size_t)num_cus());
-    if (K < 128 || tiles >= (size_t)1 << 28) return 0;
+    if (K < 128 || std::max(M, N) > (size_t)1 << 24) return 0;
     if (M >= 512 && N >= 512 && M * N * 3 >= rounds * num_cus() * kBig * kBig) return kBig;
     return std::min(M, N) >= 256 && K <= 8 * std::min(M, N) && M * N * K >= (size_t)900000000 ? kSmall : 0;
 }

@@ -40,6 +40,14 @@ __device__ __forceinline__ void meet()
     __syncthreads();
 }
 
+// A launch counts its threads in 32 bits along each side of its grid: more workgroups than this go into rows of as many.
+constexpr unsigned kGridRow = 1 << 20;
+__device__ __forceinline__ size_t block_id() { return (size_t)blockIdx.y * kGridRow + blockIdx.x; }
+dim3 grid_of(size_t blocks)
+{
+    return blocks <= kGridRow ? dim3((unsigned)blocks) : dim3(kGridRow, (unsigned)ceil_div(blocks, (size_t)kGridRow));
+}
+
 template <int kControl>
 __device__ __forceinline__ float plus_moved(float v)
 {
@@ -114,6 +122,7 @@ struct Sizes {
     int per;               // channels of a part
     int parts;             // of a group
     int P, rows;
+    size_t blocks;         // of a launch
 };
 
 __device__ __forceinline__ Part part_of(const Sizes &s, size_t n, int g, int k)
@@ -188,15 +197,16 @@ __global__ __launch_bounds__(1024) void gn_fwd_k(Sizes s, float eps, int act, co
                                                  float *means, float *rstds, float2 *stats)
 {
     __shared__ float red[16];
-    const size_t group = kMode == kWhole ? blockIdx.x : blockIdx.x / s.parts;
-    const int k = kMode == kWhole ? 0 : (int)(blockIdx.x % s.parts), g = (int)(group % s.G);
+    const size_t block = block_id(), group = kMode == kWhole ? block : block / s.parts;
+    if (block >= s.blocks) return;
+    const int k = kMode == kWhole ? 0 : (int)(block % s.parts), g = (int)(group % s.G);
     const Part p = part_of(s, group / s.G, g, k);
     v4f v[kC][kQ];
     load_part(p, x, v);
     float mean, m2;
     if (kMode != kSecond) moments(p, v, red, mean, m2);
     if (kMode == kFirst) {
-        if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(mean, m2);
+        if (threadIdx.x == 0) stats[block] = make_float2(mean, m2);
         return;
     }
     const float total = (float)s.Cg * (float)s.inner;
@@ -236,8 +246,9 @@ __global__ __launch_bounds__(1024) void gn_bwd_k(Sizes s, int act, const float *
 {
     __shared__ float red[16];
     __shared__ float2 waves[kC * 16];
-    const size_t group = kMode == kWhole ? blockIdx.x : blockIdx.x / s.parts, n = group / s.G;
-    const int k = kMode == kWhole ? 0 : (int)(blockIdx.x % s.parts), g = (int)(group % s.G);
+    const size_t block = block_id(), group = kMode == kWhole ? block : block / s.parts, n = group / s.G;
+    if (block >= s.blocks) return;
+    const int k = kMode == kWhole ? 0 : (int)(block % s.parts), g = (int)(group % s.G);
     const Part p = part_of(s, n, g, k);
     v4f v[kC][kQ], d[kC][kQ];
     load_part(p, x, v);
@@ -350,7 +361,7 @@ __device__ __forceinline__ void fold(const Fold &f, size_t block)
         f.dscale[c] = q;
     }
 }
-__global__ __launch_bounds__(kBlock) void gn_fold_k(Fold f) { fold(f, blockIdx.x); }
+__global__ __launch_bounds__(kBlock) void gn_fold_k(Fold f) { fold(f, block_id()); }
 
 // ------------------------------------------------------------------------------- [N, inner, C]
 
@@ -360,6 +371,7 @@ struct Rows {
     size_t C, inner;
     int Cg, G, S;       // S: runs of pixels of a sample
     int U, R;           // threads to a pixel, pixels at once
+    size_t runs;        // of all samples
 };
 
 template <int V>
@@ -384,8 +396,8 @@ struct Run {
 __device__ __forceinline__ Run run_of(const Rows &r)
 {
     Run u;
-    u.n = blockIdx.x / r.S;
-    u.k = (int)(blockIdx.x % r.S);
+    u.n = block_id() / r.S;
+    u.k = (int)(block_id() % r.S);
     u.p0 = r.inner * u.k / r.S;
     u.count = (int)(r.inner * (u.k + 1) / r.S - u.p0);
     u.at = (u.n * r.inner + u.p0) * r.C;
@@ -399,6 +411,7 @@ __global__ __launch_bounds__(kBlock) void gn_last_stats_k(Rows r, const float *x
 {
     extern __shared__ float2 entry[];   // [pixel lane][channel]: mean, sum of squared differences
     typedef typename Vec<V>::type vec __attribute__((aligned(4)));
+    if (block_id() >= r.runs) return;
     const Run run = run_of(r);
     const int row = r.R > 1 ? threadIdx.x / r.U : 0, u0 = r.R > 1 ? threadIdx.x % r.U : threadIdx.x;
     const int mine = row < r.R && row < run.count ? (run.count - row + r.R - 1) / r.R : 0;
@@ -458,7 +471,7 @@ __global__ __launch_bounds__(kBlock) void gn_last_stats_k(Rows r, const float *x
             q += o.y + held(i / r.Cg) * (d * d);
         }
         q = lanes_sum(q, 8);
-        if (lane == 0) stats[(size_t)blockIdx.x * r.G + g] = make_float2(m, q);
+        if (lane == 0) stats[block_id() * r.G + g] = make_float2(m, q);
     }
 }
 
@@ -474,6 +487,7 @@ __global__ __launch_bounds__(kBlock) void gn_last_apply_k(Rows r, float eps, int
 {
     extern __shared__ float2 entry[];   // [group]: mean, rstd
     typedef typename Vec<V>::type vec __attribute__((aligned(4)));
+    if (block_id() >= r.runs) return;
     const Run run = run_of(r);
     const int lane = threadIdx.x & 7;
     for (int g = threadIdx.x >> 3; g < r.G; g += kBlock / 8) {   // a group's runs by eight lanes, eight runs to a lane
@@ -543,12 +557,12 @@ __global__ __launch_bounds__(kBlock) void gn_last_apply_k(Rows r, float eps, int
 template <int V, bool kDx>
 __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const float *dy, const float *x, const float *scale, const float *bias,
                                                          const float *means, const float *rstds, float2 *sums, float2 *gsums, float *dx,
-                                                         unsigned runs, Fold f)
+                                                         Fold f)
 {
     extern __shared__ float2 entry[];   // kDx: [group]: s1, s2; else [pixel lane][channel]
     typedef typename Vec<V>::type vec __attribute__((aligned(4)));
-    if (kDx && blockIdx.x >= runs) {   // the sums over all runs wait for nothing that this launch does: they ride behind it
-        fold(f, blockIdx.x - runs);
+    if (block_id() >= r.runs) {   // the sums over all runs wait for nothing that this launch does: they ride behind it
+        if (kDx) fold(f, block_id() - r.runs);
         return;
     }
     const Run run = run_of(r);
@@ -631,7 +645,7 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
             const float2 o = entry[(size_t)i * r.C + c];
             t = make_float2(t.x + o.x, t.y + o.y);
         }
-        sums[(size_t)blockIdx.x * r.C + c] = t;
+        sums[block_id() * r.C + c] = t;
         const float a = scale[c];
         entry[c] = make_float2(a * t.x, a * t.y);
     }
@@ -645,7 +659,7 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
         }
         s = lanes_sum(s, 8);
         q = lanes_sum(q, 8);
-        if (lane == 0) gsums[(size_t)blockIdx.x * r.G + g] = make_float2(s, q);
+        if (lane == 0) gsums[block_id() * r.G + g] = make_float2(s, q);
     }
 }
 
@@ -659,7 +673,7 @@ struct Held {
     int Cg, G, bits;
     unsigned groups, per;   // all of them, an XCD's
 };
-__device__ __forceinline__ size_t held_group(const Held &h) { return (size_t)(blockIdx.x & 7) * h.per + (blockIdx.x >> 3); }
+__device__ __forceinline__ size_t held_group(const Held &h) { return (block_id() & 7) * h.per + (block_id() >> 3); }
 
 template <int kQ>
 __global__ __launch_bounds__(1024) void gn_held_fwd_k(Held h, float eps, int act, const float *x, const float *scale, const float *bias, float *y,
@@ -667,7 +681,7 @@ __global__ __launch_bounds__(1024) void gn_held_fwd_k(Held h, float eps, int act
 {
     __shared__ float red[16];
     const size_t group = held_group(h);
-    if (group >= h.groups) return;
+    if (block_id() >= 8 * (size_t)h.per || group >= h.groups) return;
     const int quad = threadIdx.x & ((1 << h.bits) - 1), row = threadIdx.x >> h.bits, rows = blockDim.x >> h.bits, last = (int)h.inner - 1;
     const int c = (int)(group % h.G) * h.Cg + 4 * quad;
     const size_t base = group / h.G * h.inner * h.C + c;
@@ -711,7 +725,7 @@ __global__ __launch_bounds__(1024) void gn_held_bwd_k(Held h, int act, const flo
     __shared__ float red[16];
     __shared__ float2 waves[16][64];
     const size_t group = held_group(h);
-    if (group >= h.groups) return;
+    if (block_id() >= 8 * (size_t)h.per || group >= h.groups) return;
     const int quad = threadIdx.x & ((1 << h.bits) - 1), row = threadIdx.x >> h.bits, rows = blockDim.x >> h.bits, last = (int)h.inner - 1;
     const int c = (int)(group % h.G) * h.Cg + 4 * quad;
     const size_t base = group / h.G * h.inner * h.C + c;
@@ -778,7 +792,7 @@ constexpr int kRowValues = 16;   // of a lane: groups of up to 1024 channels
 __global__ __launch_bounds__(kBlock) void gn_row_fwd_k(size_t groups, int Cg, int G, float eps, int act, const float *x, const float *scale,
                                                        const float *bias, float *y, float *means, float *rstds)
 {
-    const size_t group = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const size_t group = block_id() * 4 + (threadIdx.x >> 6);
     if (group >= groups) return;
     const int lane = threadIdx.x & 63, c0 = (int)(group % G) * Cg;
     const size_t at = group * Cg;
@@ -814,7 +828,7 @@ __global__ __launch_bounds__(kBlock) void gn_row_fwd_k(size_t groups, int Cg, in
 __global__ __launch_bounds__(kBlock) void gn_row_dx_k(size_t groups, int Cg, int G, int act, const float *dy, const float *x, const float *scale,
                                                       const float *bias, const float *means, const float *rstds, float *dx)
 {
-    const size_t group = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const size_t group = block_id() * 4 + (threadIdx.x >> 6);
     if (group >= groups) return;
     const int lane = threadIdx.x & 63, c0 = (int)(group % G) * Cg;
     const size_t at = group * Cg;
@@ -853,7 +867,8 @@ __global__ __launch_bounds__(kBlock) void gn_row_sums_k(size_t N, size_t C, int 
                                                         const float *scale, const float *bias, const float *means, const float *rstds, float2 *sums)
 {
     __shared__ float2 red[4][64];
-    const size_t tiles = (C + 63) / 64, c = blockIdx.x % tiles * 64 + (threadIdx.x & 63), run = blockIdx.x / tiles;
+    const size_t tiles = (C + 63) / 64, c = block_id() % tiles * 64 + (threadIdx.x & 63), run = block_id() / tiles;
+    if (run >= (size_t)S) return;
     const size_t from = N * run / S, to = N * (run + 1) / S;
     float s = 0.0f, q = 0.0f;
     if (c < C) {
@@ -882,7 +897,7 @@ __global__ __launch_bounds__(kBlock) void gn_row_sums_k(size_t N, size_t C, int 
 
 // Rows of two and three values, groups of more than 1024 channels of one value, more than 8192 channels last.
 struct Place {
-    size_t C, inner, Cg, G;
+    size_t N, C, inner, Cg, G;
     int last;
     __device__ size_t at(size_t n, size_t g, size_t i) const
     {
@@ -897,7 +912,8 @@ __global__ __launch_bounds__(kBlock) void gn_any_fwd_k(Place p, float eps, int a
                                                        float *means, float *rstds)
 {
     __shared__ float red[16];
-    const size_t n = blockIdx.x / p.G, g = blockIdx.x % p.G, L = p.Cg * p.inner;
+    const size_t group = block_id(), n = group / p.G, g = group % p.G, L = p.Cg * p.inner;
+    if (n >= p.N) return;
     float s = 0.0f;
     for (size_t i = threadIdx.x; i < L; i += kBlock) s += x[p.at(n, g, i)];
     const float mean = L ? block_sum(s, red) / (float)L : 0.0f;
@@ -914,8 +930,8 @@ __global__ __launch_bounds__(kBlock) void gn_any_fwd_k(Place p, float eps, int a
         }
     });
     if (threadIdx.x == 0) {
-        means[blockIdx.x] = mean;
-        rstds[blockIdx.x] = rstd;
+        means[group] = mean;
+        rstds[group] = rstd;
     }
 }
 
@@ -924,7 +940,8 @@ __global__ __launch_bounds__(kBlock) void gn_any_sums_k(Place p, int act, const 
                                                         const float *means, const float *rstds, float2 *sums)
 {
     __shared__ float red[16];
-    const size_t n = blockIdx.x / p.C, c = blockIdx.x % p.C, g = c / p.Cg;
+    const size_t n = block_id() / p.C, c = block_id() % p.C, g = c / p.Cg;
+    if (n >= p.N) return;
     const float mean = means[n * p.G + g], rstd = rstds[n * p.G + g], a = scale[c], b = bias[c];
     float s = 0.0f, q = 0.0f;
     with_activation(act, [&](auto kind) {
@@ -937,7 +954,7 @@ __global__ __launch_bounds__(kBlock) void gn_any_sums_k(Place p, int act, const 
     });
     s = block_sum(s, red);
     q = block_sum(q, red);
-    if (threadIdx.x == 0) sums[blockIdx.x] = make_float2(s, q);
+    if (threadIdx.x == 0) sums[n * p.C + c] = make_float2(s, q);
 }
 
 // A workgroup per group.
@@ -945,8 +962,9 @@ __global__ __launch_bounds__(kBlock) void gn_any_dx_k(Place p, int act, const fl
                                                       const float *means, const float *rstds, const float2 *sums, float *dx)
 {
     __shared__ float red[16];
-    const size_t n = blockIdx.x / p.G, g = blockIdx.x % p.G, L = p.Cg * p.inner;
-    const float mean = means[blockIdx.x], rstd = rstds[blockIdx.x];
+    const size_t group = block_id(), n = group / p.G, g = group % p.G, L = p.Cg * p.inner;
+    if (n >= p.N) return;
+    const float mean = means[group], rstd = rstds[group];
     float s1 = 0.0f, s2 = 0.0f;
     for (size_t c = g * p.Cg + threadIdx.x; c < (g + 1) * p.Cg; c += kBlock) {
         const float2 v = sums[n * p.C + c];
@@ -1007,7 +1025,7 @@ struct Split {
     Hold h;
     bool whole;
 };
-Split split_of(size_t C, size_t inner, size_t G, int most)
+Split split_of(size_t N, size_t C, size_t inner, size_t G, int most)
 {
     Split r;
     Sizes &s = r.s;
@@ -1030,6 +1048,7 @@ Split split_of(size_t C, size_t inner, size_t G, int most)
     }
     s.P = r.h.P;
     s.rows = r.h.rows;
+    s.blocks = N * G * s.parts;
     return r;
 }
 
@@ -1090,6 +1109,7 @@ Rows rows_of(size_t N, size_t C, size_t inner, size_t G, int V)
     r.R = std::max(1, kBlock / r.U);
     const size_t most = std::min((size_t)kRuns, ceil_div(inner, (size_t)r.R * 8));   // (eight pixels to a thread)
     r.S = (int)std::min(most, std::max((size_t)1, ceil_div((size_t)num_cus() * 4, N)));
+    r.runs = N * r.S;
     return r;
 }
 
@@ -1136,7 +1156,7 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
     float *const y = packed, *const means = packed + total, *const rstds = means + N * G;
     const bool rows = inner == 1 && C / G <= 64 * kRowValues;
     if (rows) {
-        hipLaunchKernelGGL(gn_row_fwd_k, dim3((unsigned)ceil_div(N * G, (size_t)4)), dim3(kBlock), 0, stream(), N * G, (int)(C / G), (int)G, eps,
+        hipLaunchKernelGGL(gn_row_fwd_k, grid_of(ceil_div(N * G, (size_t)4)), dim3(kBlock), 0, stream(), N * G, (int)(C / G), (int)G, eps,
                            act, x, scale, bias, y, means, rstds);
         DOPT_LAUNCH_CHECK();
         return DOPT_HIP_OK;
@@ -1144,7 +1164,7 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
     const HeldHold held = channels_last && inner > 1 ? held_for(N, C, inner, G, false) : HeldHold{};
     if (held.threads)
         return with_quads<kMost>(held.q, [&](auto q) -> int {
-            hipLaunchKernelGGL(gn_held_fwd_k<decltype(q)::value>, dim3(8 * held.h.per), dim3(held.threads), 0, stream(), held.h, eps, act, x, scale,
+            hipLaunchKernelGGL(gn_held_fwd_k<decltype(q)::value>, grid_of(8 * (size_t)held.h.per), dim3(held.threads), 0, stream(), held.h, eps, act, x, scale,
                                bias, y, means, rstds);
             DOPT_LAUNCH_CHECK();
             return DOPT_HIP_OK;
@@ -1153,9 +1173,9 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
         return with_vec(C, [&](auto v) -> int {
             constexpr int V = decltype(v)::value;
             const Rows r = rows_of(N, C, inner, G, V);
-            float2 *const stats = (float2 *)workspace(N * r.S * G * sizeof(float2));
+            float2 *const stats = (float2 *)workspace(r.runs * G * sizeof(float2));
             if (!stats) return DOPT_HIP_ERR_OOM;
-            const dim3 grid((unsigned)(N * r.S));
+            const dim3 grid = grid_of(r.runs);
             hipLaunchKernelGGL(gn_last_stats_k<V>, grid, dim3(kBlock), r.R * C * sizeof(float2), stream(), r, x, stats);
             DOPT_LAUNCH_CHECK();
             hipLaunchKernelGGL(gn_last_apply_k<V>, grid, dim3(kBlock), G * sizeof(float2), stream(), r, eps, act, x, scale, bias, y, means, rstds,
@@ -1164,12 +1184,12 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
             return DOPT_HIP_OK;
         });
     if (!channels_last && inner >= 4) {
-        const Split k = split_of(C, inner, G, kMost);
+        const Split k = split_of(N, C, inner, G, kMost);
         float2 *stats = nullptr;
         if (!k.whole && !(stats = (float2 *)workspace(N * G * k.s.parts * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
         return with_hold<kMost>(k.h, [&](auto c, auto q) -> int {
             constexpr int kC = decltype(c)::value, kQ = decltype(q)::value;
-            const dim3 grid((unsigned)(N * G * k.s.parts)), block(k.h.threads);
+            const dim3 grid = grid_of(k.s.blocks), block(k.h.threads);
             if (k.whole) {
                 hipLaunchKernelGGL((gn_fwd_k<kC, kQ, kWhole>), grid, block, 0, stream(), k.s, eps, act, x, scale, bias, y, means, rstds, stats);
             } else {
@@ -1181,8 +1201,8 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
             return DOPT_HIP_OK;
         });
     }
-    const Place p{C, inner, C / G, G, channels_last != 0};
-    hipLaunchKernelGGL(gn_any_fwd_k, dim3((unsigned)(N * G)), dim3(kBlock), 0, stream(), p, eps, act, x, scale, bias, y, means, rstds);
+    const Place p{N, C, inner, C / G, G, channels_last != 0};
+    hipLaunchKernelGGL(gn_any_fwd_k, grid_of(N * G), dim3(kBlock), 0, stream(), p, eps, act, x, scale, bias, y, means, rstds);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
@@ -1202,9 +1222,9 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
     float *const dx = packed;
     const float *const means = stats, *const rstds = stats + N * G;
     float2 *sums = nullptr;
-    const unsigned folds = (unsigned)ceil_div(C, (size_t)8);
+    const size_t folds = ceil_div(C, (size_t)8);
     auto fold = [&](size_t rows, int pieces) -> int {
-        hipLaunchKernelGGL(gn_fold_k, dim3(folds), dim3(kBlock), 0, stream(), Fold{rows, C, pieces, sums, packed + total, packed + total + C});
+        hipLaunchKernelGGL(gn_fold_k, grid_of(folds), dim3(kBlock), 0, stream(), Fold{rows, C, pieces, sums, packed + total, packed + total + C});
         DOPT_LAUNCH_CHECK();
         return DOPT_HIP_OK;
     };
@@ -1213,10 +1233,10 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
         const size_t tiles = ceil_div(C, (size_t)64);
         const int S = (int)std::min(std::max((size_t)1, (size_t)num_cus() * 4 / tiles), ceil_div(N, (size_t)32));
         if (!(sums = (float2 *)workspace((size_t)S * C * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
-        hipLaunchKernelGGL(gn_row_dx_k, dim3((unsigned)ceil_div(N * G, (size_t)4)), dim3(kBlock), 0, stream(), N * G, (int)(C / G), (int)G, act, dy,
+        hipLaunchKernelGGL(gn_row_dx_k, grid_of(ceil_div(N * G, (size_t)4)), dim3(kBlock), 0, stream(), N * G, (int)(C / G), (int)G, act, dy,
                            x, scale, bias, means, rstds, dx);
         DOPT_LAUNCH_CHECK();
-        hipLaunchKernelGGL(gn_row_sums_k, dim3((unsigned)(tiles * S)), dim3(kBlock), 0, stream(), N, C, (int)(C / G), (int)G, S, act, dy, x, scale,
+        hipLaunchKernelGGL(gn_row_sums_k, grid_of(tiles * S), dim3(kBlock), 0, stream(), N, C, (int)(C / G), (int)G, S, act, dy, x, scale,
                            bias, means, rstds, sums);
         DOPT_LAUNCH_CHECK();
         return fold(S, 1);
@@ -1225,7 +1245,7 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
     if (held.threads) {
         if (!(sums = (float2 *)workspace(N * C * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
         if (int rc = with_quads<kMostGrad>(held.q, [&](auto q) -> int {
-                hipLaunchKernelGGL(gn_held_bwd_k<decltype(q)::value>, dim3(8 * held.h.per), dim3(held.threads), 0, stream(), held.h, act, dy, x,
+                hipLaunchKernelGGL(gn_held_bwd_k<decltype(q)::value>, grid_of(8 * (size_t)held.h.per), dim3(held.threads), 0, stream(), held.h, act, dy, x,
                                    scale, bias, means, rstds, sums, dx);
                 DOPT_LAUNCH_CHECK();
                 return DOPT_HIP_OK;
@@ -1237,25 +1257,24 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
         return with_vec(C, [&](auto v) -> int {
             constexpr int V = decltype(v)::value;
             const Rows r = rows_of(N, C, inner, G, V);
-            sums = (float2 *)workspace(N * r.S * (C + G) * sizeof(float2));
+            sums = (float2 *)workspace(r.runs * (C + G) * sizeof(float2));
             if (!sums) return DOPT_HIP_ERR_OOM;
-            float2 *const gsums = sums + N * r.S * C;
-            const unsigned runs = (unsigned)(N * r.S);
-            const Fold f{N * r.S, C, 1, sums, packed + total, packed + total + C};
-            hipLaunchKernelGGL((gn_last_grad_k<V, false>), dim3(runs), dim3(kBlock), r.R * C * sizeof(float2), stream(), r, act, dy, x, scale, bias,
-                               means, rstds, sums, gsums, dx, runs, f);
+            float2 *const gsums = sums + r.runs * C;
+            const Fold f{r.runs, C, 1, sums, packed + total, packed + total + C};
+            hipLaunchKernelGGL((gn_last_grad_k<V, false>), grid_of(r.runs), dim3(kBlock), r.R * C * sizeof(float2), stream(), r, act, dy, x, scale, bias,
+                               means, rstds, sums, gsums, dx, f);
             DOPT_LAUNCH_CHECK();
-            hipLaunchKernelGGL((gn_last_grad_k<V, true>), dim3(runs + folds), dim3(kBlock), G * sizeof(float2), stream(), r, act, dy, x, scale, bias,
-                               means, rstds, sums, gsums, dx, runs, f);
+            hipLaunchKernelGGL((gn_last_grad_k<V, true>), grid_of(r.runs + folds), dim3(kBlock), G * sizeof(float2), stream(), r, act, dy, x, scale, bias,
+                               means, rstds, sums, gsums, dx, f);
             DOPT_LAUNCH_CHECK();
             return DOPT_HIP_OK;
         });
     if (!channels_last && inner >= 4) {
-        const Split k = split_of(C, inner, G, kMostGrad);
+        const Split k = split_of(N, C, inner, G, kMostGrad);
         if (!(sums = (float2 *)workspace(N * C * k.s.pieces * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
         if (int rc = with_hold<kMostGrad>(k.h, [&](auto c, auto q) -> int {
                 constexpr int kC = decltype(c)::value, kQ = decltype(q)::value;
-                const dim3 grid((unsigned)(N * G * k.s.parts)), block(k.h.threads);
+                const dim3 grid = grid_of(k.s.blocks), block(k.h.threads);
                 if (k.whole) {
                     hipLaunchKernelGGL((gn_bwd_k<kC, kQ, kWhole>), grid, block, 0, stream(), k.s, act, dy, x, scale, bias, means, rstds, sums, dx);
                 } else {
@@ -1269,11 +1288,11 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
             return rc;
         return fold(N, k.s.pieces);
     }
-    const Place p{C, inner, C / G, G, channels_last != 0};
+    const Place p{N, C, inner, C / G, G, channels_last != 0};
     if (!(sums = (float2 *)workspace(N * C * sizeof(float2)))) return DOPT_HIP_ERR_OOM;
-    hipLaunchKernelGGL(gn_any_sums_k, dim3((unsigned)(N * C)), dim3(kBlock), 0, stream(), p, act, dy, x, scale, bias, means, rstds, sums);
+    hipLaunchKernelGGL(gn_any_sums_k, grid_of(N * C), dim3(kBlock), 0, stream(), p, act, dy, x, scale, bias, means, rstds, sums);
     DOPT_LAUNCH_CHECK();
-    hipLaunchKernelGGL(gn_any_dx_k, dim3((unsigned)(N * G)), dim3(kBlock), 0, stream(), p, act, dy, x, scale, bias, means, rstds, sums, dx);
+    hipLaunchKernelGGL(gn_any_dx_k, grid_of(N * G), dim3(kBlock), 0, stream(), p, act, dy, x, scale, bias, means, rstds, sums, dx);
     DOPT_LAUNCH_CHECK();
     return fold(N, 1);
 }

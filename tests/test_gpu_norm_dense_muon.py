@@ -89,6 +89,16 @@ def test_group_norm_of_groups_that_a_workgroup_holds(size, last):
         _check_norm_grad(dy, x, scale, bias, groups, name, last, up)
 
 
+# one launch counts 2^32 threads along a side of its grid: whole groups, held ones, runs of pixels, rows, and the rest
+@pytest.mark.parametrize("size,last", [((2 ** 20 + 3, 2, 2, 2, 1), False), ((2 ** 20 + 9, 8, 1, 2, 1), True), ((2 ** 20 + 5, 4, 1, 3, 1), True),
+                                       ((2 ** 22 + 7, 8, 1, 1, 1), False), ((2 ** 20 + 5, 4, 1, 2, 1), False)], ids=str)
+def test_group_norm_of_more_groups_than_a_row_of_a_grid(size, last):
+    n, c, h, w, groups = size
+    x, scale, bias, dy = _norm_case(n, c, h, w, last, 18)
+    _check_norm(x, scale, bias, groups, "none", last)
+    _check_norm_grad(dy, x, scale, bias, groups, "none", last)
+
+
 def test_group_norm_gradient_of_more_than_the_caches_hold():
     x, scale, bias, dy = _norm_case(54, 256, 32, 64, True, 9)
     _check_norm_grad(dy, x, scale, bias, 32, "none", True)
