@@ -614,7 +614,7 @@ int build(Handle *h)
     size_t bytes = 0;
     auto take = [&](size_t n) { const size_t at = bytes; bytes += ceil_div(n, (size_t)256) * 256; return at; };
     std::vector<size_t> x_at, sq_at, partial_at, parts_at;
-    size_t all = 0, mids = 0;   // stages of all tiles of A; 128 x 128 tiles of square matrices
+    size_t all = 0, longest = 0, mids = 0;   // stages of all tiles of A, of one; 128 x 128 tiles of square matrices
     h->small = true;
     for (Matrix &q : h->jobs) {
         q.tall = q.rows > q.cols;
@@ -627,15 +627,21 @@ int build(Handle *h)
         q.wide = std::sqrt(std::max(1.0f, (float)q.rows / (float)q.cols));
         q.nparts = (int)ceil_div((size_t)q.rows * q.cols, kChunk);
         const size_t t = q.sp / side, tiles = t * (t + 1) / 2;
-        all += tiles * (q.lp / 32) * (side / 64);   // (a stage of a 128 x 128 tile is 16 steps)
+        const size_t stages = (size_t)(q.lp / 32) * (side / 64);   // (one of a 128 x 128 tile is 16 steps)
+        all += tiles * stages;
+        longest = std::max(longest, stages);
         mids += side == 128 ? tiles : 0;
         h->small = h->small && side == 64;
     }
-    // A's reduction is cut so that two workgroups for each CU have about the same to do
-    const size_t part = std::max((size_t)(h->small ? 4 : 32), ceil_div(all, (size_t)num_cus() * 2));
+    // A's reduction is cut so that three workgroups for every two CUs have about the same to do (us for VGG-16's matrices and for eight of
+    // [640 x 5760]: one for each CU 456 and 785, three for two 449 and 776, two 468 and 809).  Where one workgroup adds the
+    // parts for its whole chain there are sixteen at most: eight of [64 x 8192] take 110 us, in sixty-four parts each 140.
+    const size_t part = std::max(h->small ? std::max((size_t)4, longest / 16) : (size_t)32, ceil_div(all * 2, (size_t)num_cus() * 3));
     auto cuts_of = [&](const Matrix &q) { return (int)ceil_div((size_t)q.lp / 32 * (q.sp == 64 ? 1 : 2), part); };
-    // 64 x 64 tiles spread a short product over more CUs, 128 x 128 tiles take half the operands' traffic: 13 products of [512 x 512] ..
-    const bool mid_squares = mids >= (size_t)num_cus() * 2;
+    // 64 x 64 tiles spread a short product over more CUs, 128 x 128 tiles take half the operands' traffic (whole updates, us, in the former
+    // and the latter: one [512 x 512] 207 and 343, eight [640 x 5760] 827 and 929, eight [1024 x 1024], 288 of the large
+    // tiles, 901 and 874, two [2048 x 2048] 1555 and 1449).
+    const bool mid_squares = mids >= (size_t)num_cus();
     for (const Matrix &q : h->jobs) {
         const size_t side = q.sp == 64 ? 64 : 128, t = q.sp / side, cuts = cuts_of(q);
         x_at.push_back(take((size_t)q.sp * q.lp * 4 * 4));
