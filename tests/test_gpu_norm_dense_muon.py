@@ -400,6 +400,12 @@ def test_muon_of_many_matrices(iterations):
     _run_muon(shapes, iterations, seed=iterations)
 
 
+def test_muon_of_large_matrices():
+    """More tiles of X than compute units: sides of odd numbers of 128 rows, and a side of at most 64 among them."""
+    _run_muon([(300, 9000), (9000, 700), (40, 5001), (515, 900), (64, 64), (1000, 130)], 5, seed=11)
+    _run_muon([(300, 9000), (9001, 700), (40, 5000)], 2, False, 12, up=_off_grid)
+
+
 @pytest.mark.parametrize("kind", ["plain", "weak"])
 @pytest.mark.parametrize("nesterov", [False, True])
 def test_muon_momenta_alignment_and_weak_directions(nesterov, kind):
