@@ -1,13 +1,16 @@
-// Products of large dense layers, forward and backward: both operands are laid out once as two fp16 parts and go to the matrix instruction
-// from there, the layer's end rides in the product.
+// Products of dense layers of middling and large sizes, forward and backward: both operands are laid out once as two fp16 parts and go to
+// the matrix instruction from there, the layer's end rides in the product.
 //
-// Rows are scaled by powers of two, each to a largest value in [2^14, 2^15), so h + l is off by at most 2^-22 of a value and 2^-40 of
+// Rows are scaled by powers of two, each to a largest value in [2^14, 2^15), so h + l is off by at most 2^-22 of a value or 2^-39 of
 // the largest one of its row (fp16's last subnormal place).  l l is left out, 2^-22 of a product at most.  Together with sums in fp32
-//     |error| <= (K 2^-24 + 2^-20) sum |x| |w| + 2^-39 K max |x row| max |w row|
-// that is, fp32's own rounding of a long sum unless a row spans more than fifteen binary orders and its largest values meet zeros.
+//     |error| <= (K 2^-24 + 2^-20) sum |x| |w| + 2^-38 K max |x row| max |w row|
+// that is, fp32's own rounding of a long sum unless a row spans more than seventeen binary orders and its largest values meet zeros.
 // Three bf16 parts, which sgemm.hip uses for operands of any kind, keep 24 bits and take twice the matrix work.
 //
-// Bound by the matrix instructions: 6 M N K operations.
+// Bound by the matrix instructions, 6 M N K operations, where tiles are large: [8192 x 4096] from 4096 steps, 824 GFLOP, takes 745 us, 86 of
+// them for the layout (402 MB, 4.7 TB/s) and 660 for the product (1250 TFLOP/s; a library's bf16 product of 4096 cubed reaches 1157).
+// The matrix instructions are busy 72 % of its cycles, at the clock that is left when they are.  With tiles of 128 x 128 the bound is
+// what a CU takes in, some 45 GB/s whoever asks for it.
 #include <algorithm>
 #include <type_traits>
 
@@ -59,8 +62,8 @@ __device__ __forceinline__ void store_parts(char *block, int row, int half, cons
 
 // Four rows per workgroup, eight values of a row to each of its threads and those of kUnits further places, in registers between the
 // search for the rows' largest values and the layout: sixteen steps of the four rows are stored by eight threads, 256 bytes
-// in a line.  Bound by memory; read twice, through an L2 that holds no row for so long, [8192 + 4096] rows of 4096 took 106 us.
-// Longer rows than the registers hold are.  Padding and rows that are not finite become zeros.
+// in a line.  Bound by memory: [8192 + 4096] rows of 4096 take 86 us, read twice, which the L2 does not shorten, 106.  Longer rows than
+// the registers hold are read twice.  Padding and rows that are not finite become zeros.
 constexpr int kUnits = 8;
 __device__ __forceinline__ void split_rows(const Operand &o, unsigned block)
 {
@@ -126,7 +129,7 @@ __device__ __forceinline__ void split_rows(const Operand &o, unsigned block)
 
 // Operands that lie across the reduction, [K][rows]: the largest values of runs of K for each column, then a tile of 64 steps by 64 columns
 // per workgroup, turned in LDS.
-constexpr int kRuns = 32, kAcross = 3;
+constexpr int kRuns = 32, kAcross = 3;   // (dz, w and x of [1000, 1777] from 1111: 7 us and 13 us, with dz as it lies)
 struct Tops {
     Operand o[kAcross];
     int n;
@@ -271,8 +274,8 @@ __device__ __forceinline__ void bring_both(const char *left, const char *right, 
 }
 
 // Tiles of 256 x 256 by eight wavefronts of 128 x 64: the accumulators are half of the registers, and a stage, 32 KB, feeds 24 matrix
-// instructions of each.  The halves of the workgroup, which share the CU's four SIMDs, read and multiply in turn; three
-// stages are on their way.
+// instructions of each.  The halves of the workgroup, which share the CU's four SIMDs, read and multiply in turn; three stages are on
+// their way.  (Reading and multiplying together, between one barrier per stage, took 908 us where this takes 815.)
 __device__ __forceinline__ void sums(const char *left, const char *right, int steps, int w, int lane, char *lds, v16f (&acc)[4][2])
 {
     const int wm = w >> 2, wn = w & 3;
@@ -444,7 +447,7 @@ __global__ __launch_bounds__(2 * kTile, 2) void wide_product_k(Wides both, Dense
 }
 
 // Adds the splits of up to two products and ends them, four values at a time; the last four end with the product, whatever of them the
-// quad before has written too.
+// quad before has written too.  Bound by memory ([1000 x 1111] of three and [1777 x 1111] of two: 41 MB, 8 us).
 __global__ __launch_bounds__(256) void wide_join_k(Wides both, DenseEpilogue ep)
 {
     auto quads_of = [](const Wide &q) { return q.splits > 1 ? (q.M * q.N + 3) / 4 : 0; };
@@ -468,7 +471,14 @@ __global__ __launch_bounds__(256) void wide_join_k(Wides both, DenseEpilogue ep)
     });
 }
 
-// The side of the tiles that suit a product; 0: none here.
+// The side of the tiles that suit a product; 0: none here.  Large ones where they take a third of the chip's places; small ones from
+// two gigaflops on, unless the reduction is long and the sides short.  us here and on three bf16 parts, large tiles with 128, 512
+// and 1024 steps:
+//     [1500 x 4096] 37 63 93 and 36 69 113    [4096 x 2500] 55 77 109 and 91 153 198    [4096 x 4097] 96 142 210 and 140 234 362
+//     [8192 x 4096] 130 187 268 and 160 308 472
+// small ones with 512, 1024 and 4096:
+//     [1024 x 1024] 28 30 56 and 22 38 65    [2048 x 1024] 32 40 89 and 39 49 113    [1024 x 4096] 37 51 155 and 50 82 199
+//     [256 x 4096] 29 33 76 and 21 39 69
 int tile_for(size_t M, size_t N, size_t K)
 {
     const size_t tiles = ceil_div(M, (size_t)kBig) * ceil_div(N, (size_t)kBig), rounds = ceil_div(tiles, (size_t)num_cus());
@@ -538,9 +548,6 @@ void cut(const WideProduct *p, int n, unsigned *splits)
 
 namespace dopt {
 
-// Where a third of the chip's places for tiles are taken.  us here and on three bf16 parts, with 128, 512 and 1024 steps:
-//     [1024 x 4096] 36 57 84 and 29 51 85    [1500 x 4096] 37 63 93 and 36 69 113    [4096 x 2500] 55 77 109 and 91 153 198
-//     [4096 x 4097] 96 142 210 and 140 234 362    [8192 x 4096] 130 187 268 and 160 308 472
 bool dense_wide_takes(size_t M, size_t N, size_t K) { return tile_for(M, N, K) != 0; }
 
 size_t dense_wide_scratch(const WideProduct *p, int n)

@@ -30,6 +30,10 @@
 // over all channels of the L2: row by row, at a pitch of 2 KB, the rows of a tile met in two channels of sixteen and the products
 // took three times as long.  Inside a row the four pieces lie at place piece ^ (row / 4 mod 4), in memory as in LDS, so that
 // lanes which read the same piece of neighbouring rows touch different banks.
+//
+// Measured: VGG-16's sixteen matrices 448 us (39 for the momenta and 49 for X, at 5 TB/s; 72 for the two A, 140 for X after
+// three and five iterations, 13 x 13.6 for square products, each a launch and what a CU takes in of its operands), eight of up to [640 x 5760]
+// 760 to 810 by the machine (68, 85, 146, 300, 13 x 17.5), one [64 x 576] 53.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

@@ -537,11 +537,15 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
 
 /* pre = x * w^T + bias, y = act(pre) + residual: x [M,K], w [N,K] as nnet/layers/dense.d stores it, bias [N], residual [M,N].
    bias, residual and pre may be null; a training step keeps pre, which the gradient reads (act none needs none).  y and pre may
-   overlap neither each other nor an operand. */
+   overlap neither each other nor an operand.
+   Products of 9e8 multiplications and more (both sides 256 and more) are formed from two fp16 parts of each value, scaled row by row:
+   a value keeps 22 bits, or 2^-39 of its row's largest one where that is more.  They take workspace: four bytes a value of
+   both operands, rows counted up to a multiple of 256.  Values that are not finite reach the results that fp32 would give them. */
 int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, const float *w, const float *bias,
                        const float *residual, float *y, float *pre);
 /* With dz = dy * act'(pre): dx = dz * w [M,K], dw = dz^T * x [N,K], dbias = column sums of dz [N]; the residual's gradient is dy.
-   Any of the three results may be null, and w (x) with dx (dw); pre may be null for act none. */
+   Any of the three results may be null, and w (x) with dx (dw); pre may be null for act none.  The products are formed as above,
+   "row by row" of dz and by the columns of w for dx, by the columns of dz and x for dw. */
 int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *dy, const float *pre, const float *x,
                             const float *w, float *dx, float *dw, float *dbias);
 
@@ -588,8 +592,9 @@ typedef struct {
      m' = mu m + g,  u = nesterov ? g + mu m' : m',  X = u / (|u| + 1e-7), |u| the 2-norm of all its values,
      `iterations` times (five as a rule), on the side of fewer rows:  A = X X^T,  X = 3.4445 X + (-4.7750 A + 2.0315 A A) X,
      w' = (1 - lr decay) w - lr sqrt(max(1, rows / cols)) X
-   for all matrices of the handle at once.  The handle keeps the addresses and the scratch memory that the step needs; no w or m
-   may overlap another operand of the set.  The shorter side of a matrix may have up to 16384 values. */
+   for all matrices of the handle at once.  The handle keeps the addresses and the scratch memory that the step needs, sixteen bytes
+   a value with both sides counted up to multiples of 128 (of 64, where the shorter one is no longer) and 24 a value of A; no w
+   or m may overlap another operand of the set.  The shorter side of a matrix may have up to 16384 values, all of it 2^28. */
 int dopt_hip_muon_create(int nmatrices, const dopt_hip_matrix_ref *refs, void **handle);
 int dopt_hip_muon_destroy(void *handle);
 int dopt_hip_muon_step(void *handle, float lr, float mu, int nesterov, float decay, int iterations);
