@@ -93,6 +93,7 @@ struct Part {
     size_t inner;
     int c0, channels, len, P, rows;
     size_t i0;
+    int row, lane;    // of the thread
 };
 
 struct Where {
@@ -105,13 +106,12 @@ struct Where {
 // beyond the last quad or channel repeats it, so that nothing is guarded but the sums.
 __device__ __forceinline__ Where where(const Part &p, int ci, int qi)
 {
-    const int lane = threadIdx.x & (p.P - 1), row = threadIdx.x / p.P;
-    const int c = row + ci * p.rows, q = lane + qi * p.P;
+    const int c = p.row + ci * p.rows, q = p.lane + qi * p.P;
     const int start = min(4 * q, p.len - 4);
     Where w;
     w.c = p.c0 + min(c, p.channels - 1);
     w.at = p.base + (size_t)w.c * p.inner + p.i0 + start;
-    w.first = c < p.channels && row < p.rows ? min(4 * q - start, 4) : 4;
+    w.first = c < p.channels && p.row < p.rows ? min(4 * q - start, 4) : 4;
     return w;
 }
 
@@ -142,6 +142,8 @@ __device__ __forceinline__ Part part_of(const Sizes &s, size_t n, int g, int k)
     p.len = (int)(s.inner * (piece + 1) / s.pieces - p.i0);
     p.P = s.P;
     p.rows = s.rows;
+    p.row = (int)threadIdx.x / s.P;
+    p.lane = (int)threadIdx.x - p.row * s.P;
     return p;
 }
 
@@ -290,8 +292,8 @@ __global__ __launch_bounds__(1024) void gn_bwd_k(Sizes s, int act, const float *
             if (p.P > 64 && (threadIdx.x & 63) == 0) waves[ci * 16 + (threadIdx.x >> 6)] = own[ci];
         }
         if (p.P > 64) meet();
-        const int row = threadIdx.x / p.P;
-        const bool leads = (threadIdx.x & (p.P - 1)) == 0 && row < p.rows;
+        const int row = p.row;
+        const bool leads = p.lane == 0 && row < p.rows;
 #pragma unroll
         for (int ci = 0; ci < kC; ci++) {
             const int c = row + ci * p.rows;
@@ -1006,8 +1008,10 @@ Hold hold_for(int channels, size_t len, int most)
     const size_t quads = ceil_div(len, (size_t)4);
     for (int q = 1; q <= most; q *= 2)
         for (int c = 1; c * q <= most; c *= 2) {
+            // lanes to a channel: a power of two, or whole wavefronts ([87, 160, 39 x 28] in 16 groups backward, 273 quads to a channel,
+            // 70 us; with 512 lanes, or half of them to spare, 101)
             int P = 1;
-            while ((size_t)P * q < quads && P <= 1024) P *= 2;
+            while ((size_t)P * q < quads && P <= 1024) P += P < 64 ? P : 64;
             const int rows = (channels + c - 1) / c, threads = (int)ceil_div((size_t)rows * P, (size_t)64) * 64;
             if (P > 1024 || rows > 1024 || threads > 1024) continue;
             // Places that stay empty cost what full ones do.  Four quads of one tensor to a thread, two of two, and more wavefronts with the
@@ -1048,6 +1052,7 @@ Split split_of(size_t N, size_t C, size_t inner, size_t G, int most)
     if (!r.whole) {
         s.pieces = (int)ceil_div(inner, (size_t)kPiece);
         s.per = s.pieces > 1 ? 1 : std::max(1, std::min(s.Cg, (int)(kPiece / inner)));
+        s.per = (int)ceil_div((size_t)s.Cg, ceil_div((size_t)s.Cg, (size_t)s.per));   // (of about the same size)
         s.parts = s.pieces * (int)ceil_div((size_t)s.Cg, (size_t)s.per);
         r.h = hold_for(s.per, ceil_div(inner, (size_t)s.pieces), most);
     }
