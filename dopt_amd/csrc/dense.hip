@@ -43,56 +43,73 @@ __global__ __launch_bounds__(kBlock) void dense_epilogue_k(size_t n, DenseEpilog
     });
 }
 
-// dz = dy act'(pre), where there is an activation, and its sums over runs of rows: a workgroup takes 64 V columns by four rows at a time.
+// dz = dy act'(pre), where there is an activation, and its sums over runs of rows: a workgroup takes 64 V columns by four rows at a time.  The
+// last V columns end with the matrix, whatever of them other lanes form as well, to the same bits.  Likewise the largest magnitudes of
+// the runs, and, behind them, those of matrices that wait for nothing here.
 // Bound by memory, [1000 x 1777] 21 MB in 6.6 us; the sums cost no pass of their own.
 template <int V>
-__global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int runs, int act, const float *dy, const float *pre, float *dz, float *sums)
+__global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int runs, int act, const float *dy, const float *pre, float *dz, float *sums,
+                                                     unsigned *tops, Tops others)
 {
     typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
     __shared__ float red[4][64 * V];
-    const size_t tiles = (N + 64 * V - 1) / (64 * V), run = blockIdx.x / tiles, col = (blockIdx.x % tiles * 64 + (threadIdx.x & 63)) * V;
+    const size_t tiles = (N + 64 * V - 1) / (64 * V), run = blockIdx.x / tiles, first = blockIdx.x % tiles * 64 * V;
+    if (run >= (size_t)runs) {
+        column_tops(others, (unsigned)(blockIdx.x - tiles * runs));
+        return;
+    }
+    const size_t col = min(first + (threadIdx.x & 63) * V, N - V);
     const size_t from = M * run / runs, to = M * (run + 1) / runs;
     const int row = threadIdx.x >> 6;
     float s[V];
+    unsigned top[V];
 #pragma unroll
-    for (int e = 0; e < V; e++) s[e] = 0.0f;
-    if (col < N) {
-        with_activation(act, [&](auto kind) {
-            constexpr bool kPlain = decltype(kind)::value == DOPT_HIP_ACT_NONE;
-            auto one = [&](const float *d, const float *z, size_t at) {
-                float o[V];
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    o[e] = act_grad<kind.value>(d[e], z[e]);
-                    s[e] += o[e];
-                    if (!kPlain) dz[at + e] = o[e];
-                }
-            };
-            size_t m = from + row;
-            for (; m + 12 < to; m += 16) {
-                vec d[4], z[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    d[i] = *(const vec *)(dy + (m + 4 * i) * N + col);
-                    if (!kPlain) z[i] = *(const vec *)(pre + (m + 4 * i) * N + col);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) one((const float *)&d[i], kPlain ? (const float *)&d[i] : (const float *)&z[i], (m + 4 * i) * N + col);
-            }
-            for (; m < to; m += 4) {
-                const vec d = *(const vec *)(dy + m * N + col), z = kPlain ? d : *(const vec *)(pre + m * N + col);
-                one((const float *)&d, (const float *)&z, m * N + col);
-            }
-        });
+    for (int e = 0; e < V; e++) {
+        s[e] = 0.0f;
+        top[e] = 0;
     }
-    if (!sums) return;
+    with_activation(act, [&](auto kind) {
+        constexpr bool kPlain = decltype(kind)::value == DOPT_HIP_ACT_NONE;
+        auto one = [&](const float *d, const float *z, size_t at) {
+            float o[V];
 #pragma unroll
-    for (int e = 0; e < V; e++) red[row][(threadIdx.x & 63) * V + e] = s[e];
+            for (int e = 0; e < V; e++) {
+                o[e] = act_grad<kind.value>(d[e], z[e]);
+                s[e] += o[e];
+                top[e] = max(top[e], magnitude(o[e]));
+                if (!kPlain) dz[at + e] = o[e];
+            }
+        };
+        size_t m = from + row;
+        for (; m + 12 < to; m += 16) {
+            vec d[4], z[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                d[i] = *(const vec *)(dy + (m + 4 * i) * N + col);
+                if (!kPlain) z[i] = *(const vec *)(pre + (m + 4 * i) * N + col);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) one((const float *)&d[i], kPlain ? (const float *)&d[i] : (const float *)&z[i], (m + 4 * i) * N + col);
+        }
+        for (; m < to; m += 4) {
+            const vec d = *(const vec *)(dy + m * N + col), z = kPlain ? d : *(const vec *)(pre + m * N + col);
+            one((const float *)&d, (const float *)&z, m * N + col);
+        }
+    });
+    auto place = [&](size_t c) { return run * N + min(first + c / V * V, N - V) + c % V; };
+    if (sums) {
+#pragma unroll
+        for (int e = 0; e < V; e++) red[row][(threadIdx.x & 63) * V + e] = s[e];
+        __syncthreads();
+        for (size_t c = threadIdx.x; c < 64 * V; c += kBlock) sums[place(c)] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+    }
+    if (!tops) return;
     __syncthreads();
-    for (size_t c = threadIdx.x; c < 64 * V; c += kBlock) {
-        const size_t at = blockIdx.x % tiles * 64 * V + c;
-        if (at < N) sums[run * N + at] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-    }
+#pragma unroll
+    for (int e = 0; e < V; e++) red[row][(threadIdx.x & 63) * V + e] = __builtin_bit_cast(float, top[e]);
+    __syncthreads();
+    for (size_t c = threadIdx.x; c < 64 * V; c += kBlock)
+        tops[place(c)] = max(max(magnitude(red[0][c]), magnitude(red[1][c])), max(magnitude(red[2][c]), magnitude(red[3][c])));
 }
 
 __global__ __launch_bounds__(kBlock) void dense_fold_k(DenseFold f) { dense_fold(f, blockIdx.x); }
@@ -136,7 +153,7 @@ int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, co
     const DenseEpilogue e{bias, residual, pre, act, N};
     if (dense_wide_takes(M, N, K)) {
         const WideProduct p{M, N, K, {x, false}, {w, false}, y};
-        return dense_wide(&p, 1, e, DenseFold{});
+        return dense_wide(&p, 1, e, DenseFold{}, false);
     }
     return product_dense(M, N, K, x, w, e, y);
 }
@@ -160,7 +177,7 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     const bool plain = act == DOPT_HIP_ACT_NONE;
     const float *dz = dy;
     float *sums = nullptr;
-    const int V = N % 4 == 0 ? 4 : 1;
+    const int V = N >= 4 ? 4 : 1;
     const size_t tiles = ceil_div(std::max(N, (size_t)1), (size_t)(64 * V));
     // enough workgroups to fill the chip, of sixteen rows and more
     const int runs = (int)std::max((size_t)1, std::min(ceil_div(M, (size_t)16), ceil_div((size_t)num_cus() * 8, tiles)));
@@ -169,10 +186,11 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     int wides = 0;
     if (dx && dense_wide_takes(M, K, N)) wide[wides++] = WideProduct{M, K, N, {dz, false}, {w, true}, dx};
     const bool wide_x = wides > 0;
-    if (dw && dense_wide_takes(N, K, M)) wide[wides++] = WideProduct{N, K, M, {dz, true}, {x, true}, dw};
+    const bool pass = M * N > 0 && (!plain || dbias);   // over dz, which then finds what the products need of it
+    if (dw && dense_wide_takes(N, K, M)) wide[wides++] = WideProduct{N, K, M, {dz, true, pass ? runs : 0}, {x, true}, dw};
     const bool wide_w = wides > (int)wide_x;
     size_t held = 0;
-    if (M * N > 0 && (!plain || dbias)) {
+    if (pass) {
         // dz, its sums and what the products park beside them share one request, which none of them has to grow
         auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
         const size_t first = plain ? 0 : rounded(M * N * sizeof(float));
@@ -183,11 +201,14 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
         if (!to) return DOPT_HIP_ERR_OOM;
         if (!plain) dz = (float *)to;
         sums = (float *)(to + first);
-        const dim3 grid((unsigned)(tiles * runs));
+        for (int i = 0; i < wides; i++) wide[i].x.values = dz;
+        Tops others{};
+        unsigned *const tops = wides ? dense_wide_tops(wide, wides, to + held, &others) : nullptr;
+        const dim3 grid((unsigned)(tiles * runs) + others.blocks);
         if (V == 4)
-            hipLaunchKernelGGL(dense_dz_k<4>, grid, dim3(kBlock), 0, stream(), M, N, runs, act, dy, pre, (float *)to, dbias ? sums : nullptr);
+            hipLaunchKernelGGL(dense_dz_k<4>, grid, dim3(kBlock), 0, stream(), M, N, runs, act, dy, pre, (float *)to, dbias ? sums : nullptr, tops, others);
         else
-            hipLaunchKernelGGL(dense_dz_k<1>, grid, dim3(kBlock), 0, stream(), M, N, runs, act, dy, pre, (float *)to, dbias ? sums : nullptr);
+            hipLaunchKernelGGL(dense_dz_k<1>, grid, dim3(kBlock), 0, stream(), M, N, runs, act, dy, pre, (float *)to, dbias ? sums : nullptr, tops, others);
         DOPT_LAUNCH_CHECK();
     }
     const DenseFold fold{sums ? (size_t)runs : 0, N, sums, N > 0 ? dbias : nullptr};
@@ -197,10 +218,7 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     }
     workspace_hold(held);
     int rc = DOPT_HIP_OK;
-    if (wides) {
-        for (int i = 0; i < wides; i++) wide[i].x.values = dz;
-        rc = dense_wide(wide, wides, DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, fold);
-    }
+    if (wides) rc = dense_wide(wide, wides, DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, fold, pass);
     if (!rc && dx && !wide_x && M * K > 0) rc = dopt_hip_sgemm_t(0, 0, M, K, N, dz, w, dx);
     if (!rc && dw && !wide_w && N * K > 0) rc = dopt_hip_sgemm_t(1, 0, N, K, M, dz, x, dw);
     workspace_hold(0);

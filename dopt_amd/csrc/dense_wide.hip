@@ -38,9 +38,6 @@ struct Operand {
     unsigned blocks;    // of a launch
 };
 
-// (by value: of an element of a vector the builtin takes the first one's bits)
-__device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
-
 // What a row is held times, from its largest magnitude.
 __device__ __forceinline__ int shift_of(unsigned top)
 {
@@ -130,51 +127,13 @@ __device__ __forceinline__ void split_rows(const Operand &o, unsigned block)
 // Operands that lie across the reduction, [K][rows]: the largest values of runs of K for each column, then a tile of 64 steps by 64 columns
 // per workgroup, turned in LDS.
 constexpr int kRuns = 32, kAcross = 3;   // (dz, w and x of [1000, 1777] from 1111: 7 us and 13 us, with dz as it lies)
-struct Tops {
-    Operand o[kAcross];
-    int n;
-};
 struct Layout {
     Operand rows[2], across[kAcross];
     int nrows, nacross;
     DenseFold fold;   // rides behind them
 };
 
-__global__ __launch_bounds__(256) void wide_tops_k(Tops t)
-{
-    __shared__ unsigned red[4][256];
-    unsigned block = blockIdx.x;
-    int which = 0;
-    while (which + 1 < t.n && block >= t.o[which].blocks) block -= t.o[which++].blocks;
-    const Operand &o = t.o[which];
-    const unsigned tiles = (unsigned)((o.rows + 255) / 256);
-    const size_t col = min((size_t)(block % tiles) * 256 + (threadIdx.x & 63) * 4, o.rows - 4), run = block / tiles;
-    const size_t from = o.K * run / o.runs, to = o.K * (run + 1) / o.runs;
-    const int row = threadIdx.x >> 6;
-    unsigned top[4] = {0, 0, 0, 0};
-    size_t k = from + row;
-    auto see = [&](v4f v) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) top[e] = max(top[e], magnitude(v[e]));
-    };
-    for (; k + 28 < to; k += 32) {
-        v4f v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = *(const v4f_any *)(o.x + (k + 4 * i) * o.rows + col);
-#pragma unroll
-        for (int i = 0; i < 8; i++) see(v[i]);
-    }
-    for (; k < to; k += 4) see(*(const v4f_any *)(o.x + k * o.rows + col));
-#pragma unroll
-    for (int e = 0; e < 4; e++) red[row][(threadIdx.x & 63) * 4 + e] = top[e];
-    __syncthreads();
-    if (row) return;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const int c = (threadIdx.x & 63) * 4 + e;
-        o.tops[run * o.rows + col + e] = max(max(red[0][c], red[1][c]), max(red[2][c], red[3][c]));
-    }
-}
+__global__ __launch_bounds__(256) void wide_tops_k(Tops t) { column_tops(t, blockIdx.x); }
 
 __device__ __forceinline__ void turn_tile(const Operand &o, unsigned block)
 {
@@ -188,8 +147,8 @@ __device__ __forceinline__ void turn_tile(const Operand &o, unsigned block)
 #pragma unroll
     for (int u = 0; u < 16; u++) v[u] = o.x[min(k0 + w + 4 * u, K - 1) * o.rows + col];
     unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < kRuns / 4; i++) top = max(top, o.tops[min(w + 4 * i, o.runs - 1) * o.rows + col]);
+#pragma unroll 8
+    for (int i = w; i < o.runs; i += 4) top = max(top, o.tops[i * o.rows + col]);
     tops[w][c] = top;
     __syncthreads();
     const bool inside = c0 + c < o.rows;
@@ -484,7 +443,7 @@ int tile_for(size_t M, size_t N, size_t K)
     const size_t tiles = ceil_div(M, (size_t)kBig) * ceil_div(N, (size_t)kBig), rounds = ceil_div(tiles, (size_t)num_cus());
     if (K < 128 || std::max(M, N) > (size_t)1 << 24) return 0;
     if (M >= 512 && N >= 512 && M * N * 3 >= rounds * num_cus() * kBig * kBig) return kBig;
-    return std::min(M, N) >= 256 && K <= 8 * std::min(M, N) && M * N * K >= (size_t)900000000 ? kSmall : 0;
+    return std::min(M, N) >= 256 && K <= 12 * std::min(M, N) && M * N * K >= (size_t)900000000 ? kSmall : 0;
 }
 
 template <int kTile>
@@ -544,92 +503,107 @@ void cut(const WideProduct *p, int n, unsigned *splits)
     }
 }
 
+// The launches of up to two products, in scratch from `to` on.
+struct Plan {
+    Layout l{};
+    Tops tops{};
+    Wide q[2];
+    int tile[2];
+    unsigned *callers = nullptr;   // largest magnitudes that the caller finds
+    unsigned row_blocks = 0, blocks = 0;
+    size_t longest = 0, bytes = 0;
+};
+Plan arrange(const WideProduct *p, int n, char *const scratch)
+{
+    Plan r;
+    auto take = [&](size_t bytes) {
+        char *const at = scratch + r.bytes;
+        r.bytes += ceil_div(bytes, (size_t)256) * 256;
+        return at;
+    };
+    unsigned splits[2];
+    cut(p, n, splits);
+    for (int i = 0; i < n; i++) {
+        const WideProduct &g = p[i];
+        const size_t tile = r.tile[i] = tile_for(g.M, g.N, g.K), steps = ceil_div(g.K, (size_t)16);
+        Operand sides[2];
+        for (int k = 0; k < 2; k++) {
+            const WideSide &side = k ? g.w : g.x;
+            const size_t rows = k ? g.N : g.M, padded = ceil_div(rows, tile) * tile;
+            Operand &o = sides[k] = Operand{side.values, rows, padded, g.K, steps, nullptr, nullptr, nullptr, 0, 0};
+            o.parts = take(padded * steps * 64);
+            o.shift = (int *)take(padded * sizeof(int));
+            if (!side.across) {
+                o.blocks = (unsigned)(padded / 4);
+                r.row_blocks += o.blocks;
+                r.longest = std::max(r.longest, steps);
+                r.l.rows[r.l.nrows++] = o;
+                continue;
+            }
+            o.runs = side.runs ? side.runs : (int)std::min((size_t)kRuns, ceil_div(g.K, (size_t)64));
+            o.tops = (unsigned *)take(o.runs * rows * sizeof(unsigned));
+            if (side.runs) {
+                r.callers = o.tops;
+            } else {
+                const unsigned blocks = (unsigned)(ceil_div(rows, (size_t)256) * o.runs);
+                r.tops.o[r.tops.n++] = Tops::One{o.x, rows, g.K, o.tops, o.runs, blocks};
+                r.tops.blocks += blocks;
+            }
+            o.blocks = (unsigned)(padded / 64 * ceil_div(steps, (size_t)4));
+            r.blocks += o.blocks;
+            r.l.across[r.l.nacross++] = o;
+        }
+        float *const partial = splits[i] > 1 ? (float *)take(splits[i] * g.M * g.N * sizeof(float)) : nullptr;
+        const unsigned mt = (unsigned)(sides[0].padded / tile), nt = (unsigned)(sides[1].padded / tile);
+        r.q[i] = Wide{g.M, g.N, g.K, steps, g.x.values, g.w.values, g.x.across ? 1 : g.K, g.x.across ? g.M : 1, g.w.across ? 1 : g.K, g.w.across ? g.N : 1,
+                      sides[0].parts, sides[1].parts, sides[0].shift, sides[1].shift, g.y, partial, mt * nt, mt, nt, splits[i]};
+    }
+    return r;
+}
+
 }  // namespace
 
 namespace dopt {
 
 bool dense_wide_takes(size_t M, size_t N, size_t K) { return tile_for(M, N, K) != 0; }
 
-size_t dense_wide_scratch(const WideProduct *p, int n)
+size_t dense_wide_scratch(const WideProduct *p, int n) { return arrange(p, n, nullptr).bytes; }
+
+unsigned *dense_wide_tops(const WideProduct *p, int n, char *scratch, Tops *others)
 {
-    size_t bytes = 0;
-    unsigned splits[2];
-    cut(p, n, splits);
-    for (int i = 0; i < n; i++) {
-        const size_t tile = tile_for(p[i].M, p[i].N, p[i].K), K = ceil_div(p[i].K, (size_t)16) * 64 + sizeof(int);
-        const size_t mp = ceil_div(p[i].M, tile) * tile, np = ceil_div(p[i].N, tile) * tile;
-        if (splits[i] > 1) bytes += (splits[i] * p[i].M * p[i].N * sizeof(float) + 255) / 256 * 256;
-        bytes += (mp + np) * K + kRuns * ((p[i].x.across ? mp : 0) + (p[i].w.across ? np : 0)) * sizeof(unsigned);
-    }
-    return bytes;
+    const Plan plan = arrange(p, n, scratch);
+    *others = plan.tops;
+    return plan.callers;
 }
 
-int dense_wide(const WideProduct *p, int n, const DenseEpilogue &e, const DenseFold &fold)
+int dense_wide(const WideProduct *p, int n, const DenseEpilogue &e, const DenseFold &fold, bool found)
 {
-    char *to = (char *)workspace(dense_wide_scratch(p, n));
-    if (!to) return DOPT_HIP_ERR_OOM;
-    Layout l{};
-    Tops tops{};
-    Wide q[2];
-    int tile[2];
-    unsigned splits[2];
-    cut(p, n, splits);
-    unsigned top_blocks = 0, row_blocks = 0, blocks = 0;
-    size_t longest = 0;
-    for (int i = 0; i < n; i++) {
-        const WideProduct &g = p[i];
-        tile[i] = tile_for(g.M, g.N, g.K);
-        Operand sides[2];
-        for (int k = 0; k < 2; k++) {
-            const WideSide &side = k ? g.w : g.x;
-            const size_t rows = k ? g.N : g.M, padded = ceil_div(rows, (size_t)tile[i]) * tile[i], steps = ceil_div(g.K, (size_t)16);
-            Operand o{side.values, rows, padded, g.K, steps, to, (int *)(to + padded * steps * 64), nullptr, 0, 0};
-            to += padded * (steps * 64 + sizeof(int));
-            if (side.across) {
-                o.runs = (int)std::min((size_t)kRuns, ceil_div(g.K, (size_t)64));
-                o.tops = (unsigned *)to;
-                to += kRuns * padded * sizeof(unsigned);
-                o.blocks = (unsigned)(ceil_div(rows, (size_t)256) * o.runs);
-                top_blocks += o.blocks;
-                tops.o[tops.n++] = o;
-                o.blocks = (unsigned)(padded / 64 * ceil_div(steps, (size_t)4));
-                blocks += o.blocks;
-                l.across[l.nacross++] = o;
-            } else {
-                o.blocks = (unsigned)(padded / 4);
-                row_blocks += o.blocks;
-                longest = std::max(longest, steps);
-                l.rows[l.nrows++] = o;
-            }
-            sides[k] = o;
-        }
-        const unsigned mt = (unsigned)(sides[0].padded / tile[i]), nt = (unsigned)(sides[1].padded / tile[i]);
-        q[i] = Wide{g.M, g.N, g.K, sides[0].steps, g.x.values, g.w.values, g.x.across ? 1 : g.K, g.x.across ? g.M : 1, g.w.across ? 1 : g.K,
-                    g.w.across ? g.N : 1, sides[0].parts, sides[1].parts, sides[0].shift, sides[1].shift, g.y, (float *)to, mt * nt, mt, nt, splits[i]};
-        if (splits[i] > 1) to += (splits[i] * g.M * g.N * sizeof(float) + 255) / 256 * 256;
-    }
-    if (tops.n) {
-        hipLaunchKernelGGL(wide_tops_k, dim3(top_blocks), dim3(256), 0, stream(), tops);
+    char *const scratch = (char *)workspace(dense_wide_scratch(p, n));
+    if (!scratch) return DOPT_HIP_ERR_OOM;
+    Plan plan = arrange(p, n, scratch);
+    Layout &l = plan.l;
+    if (plan.tops.n && !found) {
+        hipLaunchKernelGGL(wide_tops_k, dim3(plan.tops.blocks), dim3(256), 0, stream(), plan.tops);
         DOPT_LAUNCH_CHECK();
     }
     l.fold = fold;
-    blocks += fold.dbias ? (unsigned)ceil_div(fold.N, (size_t)8) : 0;
-    const unsigned threads = longest > 512 ? 1024 : longest > 256 ? 512 : 256;   // rows in registers up to 16384 steps
+    unsigned rows = plan.row_blocks, blocks = plan.blocks + (fold.dbias ? (unsigned)ceil_div(fold.N, (size_t)8) : 0);
+    const unsigned threads = plan.longest > 512 ? 1024 : plan.longest > 256 ? 512 : 256;   // rows in registers up to 16384 steps
     if (threads > 256) {   // by themselves
-        Layout rows = l;
-        rows.nacross = 0;
-        hipLaunchKernelGGL(wide_layout_k, dim3(row_blocks), dim3(threads), 0, stream(), rows);
+        Layout alone = l;
+        alone.nacross = 0;
+        hipLaunchKernelGGL(wide_layout_k, dim3(rows), dim3(threads), 0, stream(), alone);
         DOPT_LAUNCH_CHECK();
         l.nrows = 0;
-        row_blocks = 0;
+        rows = 0;
     }
-    if (row_blocks + blocks) {
-        hipLaunchKernelGGL(wide_layout_k, dim3(row_blocks + blocks), dim3(256), 0, stream(), l);
+    if (rows + blocks) {
+        hipLaunchKernelGGL(wide_layout_k, dim3(rows + blocks), dim3(256), 0, stream(), l);
         DOPT_LAUNCH_CHECK();
     }
-    if (n == 2 && tile[0] == tile[1]) return launch_products(tile[0], q, 2, e);
+    if (n == 2 && plan.tile[0] == plan.tile[1]) return launch_products(plan.tile[0], plan.q, 2, e);
     for (int i = 0; i < n; i++)
-        if (int rc = launch_products(tile[i], q + i, 1, e)) return rc;
+        if (int rc = launch_products(plan.tile[i], plan.q + i, 1, e)) return rc;
     return DOPT_HIP_OK;
 }
 
