@@ -197,7 +197,7 @@ struct Wide {
 };
 struct Wides {
     Wide q[2];
-    unsigned blocks;   // of both
+    unsigned per[2];   // an XCD's workgroups of each
 };
 
 // What is not finite in a tile's operands: the sums of those rows and columns as fp32 instructions make them.
@@ -288,12 +288,12 @@ __global__ __launch_bounds__(2 * kTile, 2) void wide_product_k(Wides both, Dense
 {
     constexpr int MI = kTile / 64, kBlocks = kTile / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    unsigned id;
-    if (!xcd_remap(blockIdx.x, both.blocks, &id)) return;
-    const unsigned before = both.q[0].tiles * both.q[0].splits;
-    const bool second = id >= before;
+    // an XCD takes an eighth of each product, side by side; the one with the longer reduction first
+    const unsigned xcd = blockIdx.x & 7, place = blockIdx.x >> 3;
+    const bool second = place >= both.per[0];
     const Wide q = both.q[second];
-    if (second) id -= before;
+    unsigned id = second ? xcd * both.per[1] + place - both.per[0] : xcd * both.per[0] + place;
+    if (id >= q.tiles * q.splits) return;
     const unsigned split = id / q.tiles;
     id %= q.tiles;
     const size_t from = q.steps * split / q.splits, to = q.steps * (split + 1) / q.splits;
@@ -452,14 +452,16 @@ int launch_tiles(const Wides &both, const DenseEpilogue &e)
     static bool raised = false;
     if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)wide_product_k<kTile>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsOf<kTile>));
     raised = true;
-    hipLaunchKernelGGL(wide_product_k<kTile>, dim3(xcd_grid(both.blocks)), dim3(2 * kTile), kLdsOf<kTile>, stream(), both, e);
+    hipLaunchKernelGGL(wide_product_k<kTile>, dim3(8 * (both.per[0] + both.per[1])), dim3(2 * kTile), kLdsOf<kTile>, stream(), both, e);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
 
 int launch_products(int tile, const Wide *q, int n, const DenseEpilogue &e)
 {
-    Wides both{{q[0], q[n - 1]}, q[0].tiles * q[0].splits + (n == 2 ? q[1].tiles * q[1].splits : 0)};
+    Wides both{{q[0], q[n - 1]}, {0, 0}};
+    if (n == 2 && q[1].steps * q[0].splits > q[0].steps * q[1].splits) std::swap(both.q[0], both.q[1]);
+    for (int i = 0; i < n; i++) both.per[i] = (unsigned)ceil_div((size_t)both.q[i].tiles * both.q[i].splits, (size_t)8);
     if (int rc = tile == kBig ? launch_tiles<kBig>(both, e) : launch_tiles<kSmall>(both, e)) return rc;
     if (n == 1) both.q[1].splits = 1;
     size_t values = 0;
