@@ -46,7 +46,8 @@ __global__ __launch_bounds__(kBlock) void dense_epilogue_k(size_t n, DenseEpilog
 // dz = dy act'(pre), where there is an activation, and its sums over runs of rows: a workgroup takes 64 V columns by four rows at a time.  The
 // last V columns end with the matrix, whatever of them other lanes form as well, to the same bits.  Likewise the largest magnitudes of
 // the runs, and, behind them, those of matrices that wait for nothing here.
-// Bound by memory, [1000 x 1777] 21 MB in 6.6 us; the sums cost no pass of their own.
+// Bound by memory: [2066 x 4431], 110 MB, took 29 us by single columns and, with the magnitudes of w and x, 27 by four; [1000 x 1777] with
+// them, 34 MB, takes 8.8 us, where a launch of their own took 7.  The sums cost no pass.
 template <int V>
 __global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int runs, int act, const float *dy, const float *pre, float *dz, float *sums,
                                                      unsigned *tops, Tops others)
@@ -179,15 +180,18 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     float *sums = nullptr;
     const int V = N >= 4 ? 4 : 1;
     const size_t tiles = ceil_div(std::max(N, (size_t)1), (size_t)(64 * V));
-    // enough workgroups to fill the chip, of sixteen rows and more
-    const int runs = (int)std::max((size_t)1, std::min(ceil_div(M, (size_t)16), ceil_div((size_t)num_cus() * 8, tiles)));
+    // Enough workgroups to fill the chip, of sixteen rows and more; no more than 64 runs where every tile of dz' layout reads their largest
+    // magnitudes ([2066 x 462] from 4431 and its like in 114 runs 147 us, in 64 or 32 of them 136).
+    const bool turns = dw && dense_wide_takes(N, K, M);
+    const size_t most = turns ? std::min((size_t)64, ceil_div(M, (size_t)16)) : ceil_div(M, (size_t)16);
+    const int runs = (int)std::max((size_t)1, std::min(most, ceil_div((size_t)num_cus() * 8, tiles)));
     // the products that dense_wide.hip takes, in its launches
     WideProduct wide[2];
     int wides = 0;
     if (dx && dense_wide_takes(M, K, N)) wide[wides++] = WideProduct{M, K, N, {dz, false}, {w, true}, dx};
     const bool wide_x = wides > 0;
     const bool pass = M * N > 0 && (!plain || dbias);   // over dz, which then finds what the products need of it
-    if (dw && dense_wide_takes(N, K, M)) wide[wides++] = WideProduct{N, K, M, {dz, true, pass ? runs : 0}, {x, true}, dw};
+    if (turns) wide[wides++] = WideProduct{N, K, M, {dz, true, pass ? runs : 0}, {x, true}, dw};
     const bool wide_w = wides > (int)wide_x;
     size_t held = 0;
     if (pass) {

@@ -7,10 +7,11 @@
 // that is, fp32's own rounding of a long sum unless a row spans more than seventeen binary orders and its largest values meet zeros.
 // Three bf16 parts, which sgemm.hip uses for operands of any kind, keep 24 bits and take twice the matrix work.
 //
-// Bound by the matrix instructions, 6 M N K operations, where tiles are large: [8192 x 4096] from 4096 steps, 824 GFLOP, takes 745 us, 86 of
-// them for the layout (402 MB, 4.7 TB/s) and 660 for the product (1250 TFLOP/s; a library's bf16 product of 4096 cubed reaches 1157).
+// Bound by the matrix instructions, 6 M N K operations, where tiles are large: [8192 x 4096] from 4096 steps, 824 GFLOP, takes 728 us, 86 of
+// them for the layout (402 MB, 4.7 TB/s) and 640 for the product (1290 TFLOP/s; a library's bf16 product of 4096 cubed reaches 1157).
 // The matrix instructions are busy 72 % of its cycles, at the clock that is left when they are.  With tiles of 128 x 128 the bound is
-// what a CU takes in, some 45 GB/s whoever asks for it.
+// what a CU takes in, some 45 GB/s whoever asks for it: both gradients of [1000 x 1777] from 1111 take 63 us, 33 of them for the
+// products, 9 for dz, 17 for the layout and 8 to add parts.
 #include <algorithm>
 #include <type_traits>
 
@@ -72,15 +73,20 @@ __device__ __forceinline__ void split_rows(const Operand &o, unsigned block)
     const float *const x = o.x + min(row0 + r, o.rows - 1) * K;
     v4f v[kUnits][2];
     unsigned top = 0;   // of the values' magnitudes as integers, whose order is theirs, infinity and NaN last
-    auto load = [&](size_t step, bool whole, v4f *to) {   // whole: all of the workgroup's steps lie inside
+    // the loads of all places go out together, whatever lies behind the row's end; then the end is put right
+    auto load = [&](size_t step, v4f *to) {
+        const size_t k = min(step * 16 + half * 8, K - 8);
+        to[0] = *(const v4f_any *)(x + k);
+        to[1] = *(const v4f_any *)(x + k + 4);
+    };
+    auto end = [&](size_t step, v4f *of) {
         const size_t k = step * 16 + half * 8;
-        if (whole) {
-            to[0] = *(const v4f_any *)(x + k);
-            to[1] = *(const v4f_any *)(x + k + 4);
-        } else {
+        if (k + 8 <= K) return;
+        float t[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) to[e / 4][e % 4] = k + e < K ? x[k + e] : 0.0f;
-        }
+        for (int e = 0; e < 8; e++) t[e] = x[min(k + e, K - 1)];
+#pragma unroll
+        for (int e = 0; e < 8; e++) of[e / 4][e % 4] = k + e < K ? t[e] : 0.0f;
     };
     auto see = [&](const v4f *of) {
 #pragma unroll
@@ -88,13 +94,17 @@ __device__ __forceinline__ void split_rows(const Operand &o, unsigned block)
     };
 #pragma unroll
     for (int i = 0; i < kUnits; i++)
-        if (i * stride < steps) load(s0 + i * stride, (i + 1) * stride * 16 <= K, v[i]);
+        if (i * stride < steps) load(s0 + i * stride, v[i]);
 #pragma unroll
     for (int i = 0; i < kUnits; i++)
-        if (i * stride < steps) see(v[i]);
+        if (i * stride < steps) {
+            if ((i + 1) * stride * 16 > K) end(s0 + i * stride, v[i]);
+            see(v[i]);
+        }
     for (size_t i = kUnits; i * stride < steps; i++) {
         v4f more[2];
-        load(s0 + i * stride, (i + 1) * stride * 16 <= K, more);
+        load(s0 + i * stride, more);
+        end(s0 + i * stride, more);
         see(more);
     }
 #pragma unroll
@@ -119,14 +129,15 @@ __device__ __forceinline__ void split_rows(const Operand &o, unsigned block)
         if (i * stride < steps) put(s0 + i * stride, v[i]);
     for (size_t i = kUnits; i * stride < steps; i++) {
         v4f more[2];
-        load(s0 + i * stride, (i + 1) * stride * 16 <= K, more);
+        load(s0 + i * stride, more);
+        end(s0 + i * stride, more);
         put(s0 + i * stride, more);
     }
 }
 
 // Operands that lie across the reduction, [K][rows]: the largest values of runs of K for each column, then a tile of 64 steps by 64 columns
 // per workgroup, turned in LDS.
-constexpr int kRuns = 32, kAcross = 3;   // (dz, w and x of [1000, 1777] from 1111: 7 us and 13 us, with dz as it lies)
+constexpr int kRuns = 32, kAcross = 3;
 struct Layout {
     Operand rows[2], across[kAcross];
     int nrows, nacross;
@@ -431,7 +442,7 @@ __global__ __launch_bounds__(256) void wide_join_k(Wides both, DenseEpilogue ep)
 }
 
 // The side of the tiles that suit a product; 0: none here.  Large ones where they take a third of the chip's places; small ones from
-// two gigaflops on, unless the reduction is long and the sides short.  us here and on three bf16 parts, large tiles with 128, 512
+// two gigaflops on, unless the reduction is more than twelve times as long as the shorter side.  us here and on three bf16 parts, large tiles with 128, 512
 // and 1024 steps:
 //     [1500 x 4096] 37 63 93 and 36 69 113    [4096 x 2500] 55 77 109 and 91 153 198    [4096 x 4097] 96 142 210 and 140 234 362
 //     [8192 x 4096] 130 187 268 and 160 308 472
@@ -519,7 +530,7 @@ Plan arrange(const WideProduct *p, int n, char *const scratch)
 {
     Plan r;
     auto take = [&](size_t bytes) {
-        char *const at = scratch + r.bytes;
+        char *const at = scratch ? scratch + r.bytes : nullptr;   // (null: for the size alone)
         r.bytes += ceil_div(bytes, (size_t)256) * 256;
         return at;
     };
