@@ -575,6 +575,30 @@ def test_inference_of_the_block_matches_its_training_pass():
     assert np.array_equal(a, b)   # neither norm nor dense layer depends on the batch or on what is kept
 
 
+@pytest.mark.parametrize("size", [(1100, 1203, 1000), (2600, 2304, 2500)], ids=str)
+def test_a_recorded_plan_of_a_large_layer(size):
+    """Replays, with other users of the workspace between them, give the bits of the entry points called one by one."""
+    m, n, k = size
+    x, w, b, _, dy = _dense_case(m, n, k, 19)
+    vx, vt, vw, vb = core.float32([m, k]), core.float32([m, n]), core.float32([n, k], w), core.float32([n], b)
+    y = core.denseAct(vx, vw, vb, None, "gelu")
+    plan = core.compile([y] + core.grad(core.sum(y * vt), [vw, vb, vx]), REWRITES | core.PLAN_GRAPH)
+    outs = [ops.Tensor(o.shape) for o in plan.outputs]
+    dev = {vx: ops.tensor(x), vt: ops.tensor(dy)}
+    tw, pre = ops.tensor(w), ops.Tensor((m, n))
+    want = [ops.dense_act(dev[vx], tw, ops.tensor(b), None, "gelu", pre=pre).numpy()]
+    dx, dw, db = ops.dense_act_grad(dev[vt], dev[vx], tw, pre, "gelu")
+    want += [dw.numpy(), db.numpy(), dx.numpy()]
+    for _ in range(4):
+        for t in outs:
+            t.set(np.full(t.shape, 7.0, F32))
+        plan.execute(dev, outs)
+        for a, t in zip(want, outs):
+            assert np.array_equal(a, t.numpy().reshape(a.shape))
+        ops.dense_act(ops.tensor(dy), ops.tensor(np.ascontiguousarray(dy[:900])))
+    assert plan.recordings()["replays"] >= 2
+
+
 def test_two_plans_share_the_workspace():
     """Two recorded plans and eager calls that need scratch memory, one after the other: every replay gives the eager values."""
     blocks = [_block(8, 48, 96), _block(9, 130, 64)]
