@@ -379,6 +379,7 @@ struct Rows {
     int Cg, G, S;       // S: runs of pixels of a sample
     int U, R;           // threads to a pixel, pixels at once
     size_t runs;        // of all samples
+    int per_group, per_channel;   // lanes that join what a workgroup's threads have of one, powers of two
 };
 
 template <int V>
@@ -413,6 +414,7 @@ __device__ __forceinline__ Run run_of(const Rows &r)
 __device__ __forceinline__ int pixels_in(const Rows &r, int i) { return (int)(r.inner * (i + 1) / r.S - r.inner * i / r.S); }
 
 // Statistics of a run of pixels, group by group: eight pixels at a time in registers, joined per channel, then per group.
+// (Few groups have many lanes each: [64, 32 x 32, 64] in one group takes 17.5 us, with eight lanes 71; [215, 63 x 51, 4] in two 16 and 42.)
 template <int V>
 __global__ __launch_bounds__(kBlock) void gn_last_stats_k(Rows r, const float *x, float2 *stats)
 {
@@ -464,20 +466,20 @@ __global__ __launch_bounds__(kBlock) void gn_last_stats_k(Rows r, const float *x
         for (int e = 0; e < V; e++) entry[(size_t)row * r.C + (size_t)u * V + e] = make_float2(mean[e], m2[e]);
     }
     meet();
-    const int rows = min(r.R, run.count), n = rows * r.Cg, lane = threadIdx.x & 7;
+    const int rows = min(r.R, run.count), n = rows * r.Cg, lane = threadIdx.x & (r.per_group - 1);
     const float total = (float)run.count * (float)r.Cg;
     auto held = [&](int row) { return (float)((run.count - row + r.R - 1) / r.R); };
-    for (int g = threadIdx.x >> 3; g < r.G; g += kBlock / 8) {
+    for (int g = threadIdx.x / r.per_group; g < r.G; g += kBlock / r.per_group) {
         const float pivot = entry[g * r.Cg].x;
         float m = 0.0f, q = 0.0f;
-        for (int i = lane; i < n; i += 8) m += (entry[(size_t)(i / r.Cg) * r.C + g * r.Cg + i % r.Cg].x - pivot) * (held(i / r.Cg) / total);
-        m = pivot + lanes_sum(m, 8);
-        for (int i = lane; i < n; i += 8) {
+        for (int i = lane; i < n; i += r.per_group) m += (entry[(size_t)(i / r.Cg) * r.C + g * r.Cg + i % r.Cg].x - pivot) * (held(i / r.Cg) / total);
+        m = pivot + lanes_sum(m, r.per_group);
+        for (int i = lane; i < n; i += r.per_group) {
             const float2 o = entry[(size_t)(i / r.Cg) * r.C + g * r.Cg + i % r.Cg];
             const float d = o.x - m;
             q += o.y + held(i / r.Cg) * (d * d);
         }
-        q = lanes_sum(q, 8);
+        q = lanes_sum(q, r.per_group);
         if (lane == 0) stats[block_id() * r.G + g] = make_float2(m, q);
     }
 }
@@ -646,12 +648,15 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
     });
     if (kDx) return;
     meet();
-    for (size_t c = threadIdx.x; c < r.C; c += kBlock) {
-        float2 t = entry[c];
-        for (int i = 1; i < r.R; i++) {
+    const int part = threadIdx.x & (r.per_channel - 1);
+    for (size_t c = threadIdx.x / r.per_channel; c < r.C; c += kBlock / r.per_channel) {
+        float2 t = make_float2(0.0f, 0.0f);
+        for (int i = part; i < r.R; i += r.per_channel) {
             const float2 o = entry[(size_t)i * r.C + c];
             t = make_float2(t.x + o.x, t.y + o.y);
         }
+        t = make_float2(lanes_sum(t.x, r.per_channel), lanes_sum(t.y, r.per_channel));
+        if (part) continue;
         sums[block_id() * r.C + c] = t;
         const float a = scale[c];
         entry[c] = make_float2(a * t.x, a * t.y);
@@ -1120,6 +1125,13 @@ Rows rows_of(size_t N, size_t C, size_t inner, size_t G, int V)
     const size_t most = std::min((size_t)kRuns, ceil_div(inner, (size_t)r.R * 8));   // (eight pixels to a thread)
     r.S = (int)std::min(most, std::max((size_t)1, ceil_div((size_t)num_cus() * 4, N)));
     r.runs = N * r.S;
+    auto lanes = [](size_t n, int least) {   // of 256 threads to each of n
+        int l = 64;
+        while (l > least && l * n > (size_t)kBlock) l /= 2;
+        return l;
+    };
+    r.per_group = lanes(G, 8);
+    r.per_channel = lanes(C, 1);
     return r;
 }
 
