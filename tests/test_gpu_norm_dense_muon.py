@@ -78,7 +78,8 @@ def test_group_norm(size, last):
 HELD = [(2, 64, 30, 31, 8), (3, 48, 13, 19, 3), (2, 64, 11, 23, 2), (2, 128, 9, 29, 2), (3, 24, 1, 2, 3), (1, 8, 63, 65, 1), (2, 16, 45, 45, 2),
         (9, 8, 3, 3, 1), (2, 16, 64, 65, 2), (2, 16, 40, 45, 1), (2, 20, 16, 16, 1), (1, 12, 37, 37, 1),
         (2, 30, 39, 28, 3), (1, 40, 39, 28, 1), (1, 1, 100, 101, 1), (2, 6, 50, 52, 2), (3, 4, 63, 51, 2), (2, 64, 32, 33, 1),
-        (2, 3, 40, 41, 3), (1, 520, 9, 7, 130)]
+        (2, 3, 40, 41, 3), (1, 520, 9, 7, 130), (40, 99, 1, 3, 3),
+        (2, 8448, 9, 15, 12)]
 
 
 @pytest.mark.parametrize("last", [False, True], ids=["first", "last"])
