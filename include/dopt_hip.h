@@ -538,7 +538,7 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
 /* pre = x * w^T + bias, y = act(pre) + residual: x [M,K], w [N,K] as nnet/layers/dense.d stores it, bias [N], residual [M,N].
    bias, residual and pre may be null; a training step keeps pre, which the gradient reads (act none needs none).  y and pre may
    overlap neither each other nor an operand.
-   Products of 9e8 multiplications and more (both sides 256 and more) are formed from two fp16 parts of each value, scaled row by row:
+   Large products (from some 8e8 multiplications on, both sides 256 and more) are formed from two fp16 parts of each value, scaled row by row:
    a value keeps 22 bits, or 2^-39 of its row's largest one where that is more.  They take workspace: four bytes a value of
    both operands, rows counted up to a multiple of 256.  Values that are not finite reach the results that fp32 would give them. */
 int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, const float *w, const float *bias,
