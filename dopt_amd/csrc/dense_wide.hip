@@ -27,6 +27,12 @@ typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int kBig = 256, kSmall = 128;   // sides of tiles
+// Blocks of 16 steps that are added in one accumulator: 4096 steps.  The instruction rounds down what lies below its guard bits, so a long sum
+// of one sign drifts, and every instruction rounds a sum that is longer by then.  Products of non-negative values, off by on average and
+// in the root mean square, relative to the result: 4096 steps -1.2e-7 and 5.3e-7 (a library's fp32 product 8.4e-7), 17001 in one accumulator
+// -5.0e-7 and 1.2e-6 (1.7e-6), in five passes -1.0e-7 and 2.6e-7.  (Where half of both operands is zero the fp32 instruction rounds half as often:
+// 4096 steps 5.7e-7 and a library's 4.9e-7.)  A pass more costs some 2 % of a product.
+constexpr size_t kPass = 256;
 constexpr int kInf = 1 << 20, kNan = 1 << 21;   // in a row's shift: it holds infinities, NaN
 
 struct Operand {
@@ -204,6 +210,7 @@ struct Wide {
     const char *xp, *wp;
     const int *xs, *ws;
     float *y, *to;           // the result; the sums of splits, [split][M][N], where there are several
+    char *waiting;           // each workgroup's sums between its passes
     unsigned tiles, mtiles, ntiles, splits;
 };
 struct Wides {
@@ -291,6 +298,29 @@ __device__ __forceinline__ void sums(const char *left, const char *right, int st
         [&](const Side<2> &a, const Side<2> &b) { multiply(a, b, acc); });
 }
 
+// Between two passes a wavefront's sums wait in memory, where each lane finds its own again.
+template <int MI>
+__device__ __forceinline__ void waiting_sums(v16f (&acc)[MI][2], char *at, bool add, bool put)
+{
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            v4f *const to = (v4f *)at + (i * 2 + j) * 256;
+            if (add) {
+                v4f old[4];
+#pragma unroll
+                for (int g = 0; g < 4; g++) old[g] = to[g * 64];
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][j][e] += old[e >> 2][e & 3];
+            }
+            if (put) {
+#pragma unroll
+                for (int g = 0; g < 4; g++) to[g * 64] = v4f{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            }
+        }
+}
+
 template <int kTile>
 constexpr int kLdsOf = kTile == kBig ? 4 * 32768 : 5 * 16384;
 
@@ -305,7 +335,7 @@ __global__ __launch_bounds__(2 * kTile, 2) void wide_product_k(Wides both, Dense
     const Wide q = both.q[second];
     unsigned id = second ? xcd * both.per[1] + place - both.per[0] : xcd * both.per[0] + place;
     if (id >= q.tiles * q.splits) return;
-    const unsigned split = id / q.tiles;
+    const unsigned split = id / q.tiles, place_of_tile = id;
     id %= q.tiles;
     const size_t from = q.steps * split / q.splits, to = q.steps * (split + 1) / q.splits;
     float *const y = q.splits > 1 ? q.to + split * q.M * q.N : q.y;
@@ -316,13 +346,21 @@ __global__ __launch_bounds__(2 * kTile, 2) void wide_product_k(Wides both, Dense
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = kTile == kBig ? w >> 2 : w >> 1, wn = kTile == kBig ? w & 3 : w & 1;
     const size_t row_of_blocks = q.steps * 2048;
+    const char *const left = q.xp + (mt * kBlocks + w) * row_of_blocks, *const right = q.wp + (nt * kBlocks + w) * row_of_blocks;
+    const size_t m0 = (size_t)mt * kTile, n0 = (size_t)nt * kTile;
     v16f acc[MI][2];
-    zero_acc(acc);
-    sums(q.xp + (mt * kBlocks + w) * row_of_blocks + from * 2048, q.wp + (nt * kBlocks + w) * row_of_blocks + from * 2048, (int)(to - from), w, lane, lds,
-         acc);
+    const unsigned passes = (unsigned)((to - from + kPass - 1) / kPass);
+#pragma unroll 1
+    for (unsigned pass = 0;; pass++) {
+        const size_t at = from + (to - from) * pass / passes, next = from + (to - from) * (pass + 1) / passes;
+        zero_acc(acc);
+        sums(left + at * 2048, right + at * 2048, (int)(next - at), w, lane, lds, acc);
+        if (passes == 1) break;
+        waiting_sums(acc, q.waiting + ((size_t)place_of_tile * (kTile / 32) + w) * (MI * 8192) + lane * 16, pass > 0, pass + 1 < passes);
+        if (pass + 1 == passes) break;
+    }
 
     int *const shift = (int *)lds;
-    const size_t m0 = (size_t)mt * kTile, n0 = (size_t)nt * kTile;
     const int mine = threadIdx.x < kTile ? q.xs[m0 + threadIdx.x] : q.ws[n0 + threadIdx.x - kTile];
     shift[threadIdx.x] = mine;
     // (whether any is not finite; the library's vote over a workgroup has LDS of its own, which would leave a CU one of them)
@@ -567,9 +605,11 @@ Plan arrange(const WideProduct *p, int n, char *const scratch)
             r.l.across[r.l.nacross++] = o;
         }
         float *const partial = splits[i] > 1 ? (float *)take(splits[i] * g.M * g.N * sizeof(float)) : nullptr;
+        const size_t waits = ceil_div(steps, (size_t)splits[i]) > kPass ? splits[i] * sides[0].padded * sides[1].padded * sizeof(float) : 0;
+        char *const waiting = waits ? take(waits) : nullptr;
         const unsigned mt = (unsigned)(sides[0].padded / tile), nt = (unsigned)(sides[1].padded / tile);
         r.q[i] = Wide{g.M, g.N, g.K, steps, g.x.values, g.w.values, g.x.across ? 1 : g.K, g.x.across ? g.M : 1, g.w.across ? 1 : g.K, g.w.across ? g.N : 1,
-                      sides[0].parts, sides[1].parts, sides[0].shift, sides[1].shift, g.y, partial, mt * nt, mt, nt, splits[i]};
+                      sides[0].parts, sides[1].parts, sides[0].shift, sides[1].shift, g.y, partial, waiting, mt * nt, mt, nt, splits[i]};
     }
     return r;
 }
