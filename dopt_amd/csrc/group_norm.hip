@@ -336,16 +336,16 @@ __global__ __launch_bounds__(1024) void gn_bwd_k(Sizes s, int act, const float *
     }
 }
 
-// Adds `rows` rows of sums, C channels of `pieces` each: eight channels of a workgroup by thirty-two lanes.
+// Adds `rows` rows of sums, C channels of `pieces` each: eight channels of a workgroup by thirty-two lanes.  red: kFoldRed values of LDS.
+constexpr int kFoldRed = 32 * 9;
 struct Fold {
     size_t rows, C;
     int pieces;
     const float2 *sums;
     float *dscale, *dbias;
 };
-__device__ __forceinline__ void fold(const Fold &f, size_t block)
+__device__ __forceinline__ void fold(const Fold &f, size_t block, float2 *red)
 {
-    __shared__ float2 red[32][9];
     const int col = threadIdx.x & 7, lane = threadIdx.x >> 3;
     const size_t c = block * 8 + col;
     float s = 0.0f, q = 0.0f;
@@ -357,18 +357,22 @@ __device__ __forceinline__ void fold(const Fold &f, size_t block)
             q += v.y;
         }
     }
-    red[lane][col] = make_float2(s, q);
+    red[lane * 9 + col] = make_float2(s, q);
     meet();
     if (lane == 0 && c < f.C) {
         for (int i = 1; i < 32; i++) {
-            s += red[i][col].x;
-            q += red[i][col].y;
+            s += red[i * 9 + col].x;
+            q += red[i * 9 + col].y;
         }
         f.dbias[c] = s;
         f.dscale[c] = q;
     }
 }
-__global__ __launch_bounds__(kBlock) void gn_fold_k(Fold f) { fold(f, block_id()); }
+__global__ __launch_bounds__(kBlock) void gn_fold_k(Fold f)
+{
+    __shared__ float2 red[kFoldRed];
+    fold(f, block_id(), red);
+}
 
 // ------------------------------------------------------------------------------- [N, inner, C]
 
@@ -568,10 +572,10 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
                                                          const float *means, const float *rstds, float2 *sums, float2 *gsums, float *dx,
                                                          Fold f)
 {
-    extern __shared__ float2 entry[];   // kDx: [group]: s1, s2; else [pixel lane][channel]
+    extern __shared__ float2 entry[];   // kDx: [group]: s1, s2, or the fold's; else [pixel lane][channel]
     typedef typename Vec<V>::type vec __attribute__((aligned(4)));
     if (block_id() >= r.runs) {   // the sums over all runs wait for nothing that this launch does: they ride behind it
-        if (kDx) fold(f, block_id() - r.runs);
+        if (kDx) fold(f, block_id() - r.runs, entry);
         return;
     }
     const Run run = run_of(r);
@@ -1116,7 +1120,7 @@ HeldHold held_for(size_t N, size_t C, size_t inner, size_t G, bool grad)
     return r;
 }
 
-constexpr size_t kLastChannels = 8192;   // LDS of a run of pixels
+constexpr size_t kLastChannels = 8192;   // 64 KB of LDS for a run of pixels, which every launch may ask for
 
 Rows rows_of(size_t N, size_t C, size_t inner, size_t G, int V)
 {
@@ -1291,7 +1295,7 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
             hipLaunchKernelGGL((gn_last_grad_k<V, false>), grid_of(r.runs), dim3(kBlock), r.R * C * sizeof(float2), stream(), r, act, dy, x, scale, bias,
                                means, rstds, sums, gsums, dx, f);
             DOPT_LAUNCH_CHECK();
-            hipLaunchKernelGGL((gn_last_grad_k<V, true>), grid_of(r.runs + folds), dim3(kBlock), G * sizeof(float2), stream(), r, act, dy, x, scale, bias,
+            hipLaunchKernelGGL((gn_last_grad_k<V, true>), grid_of(r.runs + folds), dim3(kBlock), std::max(G, (size_t)kFoldRed) * sizeof(float2), stream(), r, act, dy, x, scale, bias,
                                means, rstds, sums, gsums, dx, f);
             DOPT_LAUNCH_CHECK();
             return DOPT_HIP_OK;
