@@ -923,7 +923,7 @@ struct VectorEpilogue {   // + rowvec[row] * colbias[col >> shift], relu, mask, 
 template <int kSteps, class E>
 __global__ __launch_bounds__(256) void gemv_rows_k(size_t M, size_t K, const float *A, const float *b, float *c, E ep)
 {
-    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const size_t row = ((size_t)blockIdx.y * kLaunchBlocks + blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (row >= M) return;
     const int lane = threadIdx.x & 63;
     const float *ar = A + row * K;
@@ -1210,7 +1210,8 @@ bool gemv_by_rows(int transA, int transB, size_t M, size_t N) { return (N == 1 &
 template <class E>
 void launch_gemv_rows(size_t R, size_t K, const float *mat, const float *vec, float *c, const E &ep)
 {
-    const dim3 grid((unsigned)ceil_div(R, (size_t)4));
+    const size_t blocks = ceil_div(R, (size_t)4);   // in rows of as many as a launch is given
+    const dim3 grid((unsigned)std::min(blocks, kLaunchBlocks), (unsigned)ceil_div(blocks, kLaunchBlocks));
     if (K <= 256) hipLaunchKernelGGL((gemv_rows_k<4, E>), grid, dim3(256), 0, stream(), R, K, mat, vec, c, ep);
     else if (K <= 384) hipLaunchKernelGGL((gemv_rows_k<6, E>), grid, dim3(256), 0, stream(), R, K, mat, vec, c, ep);
     else if (K <= 512) hipLaunchKernelGGL((gemv_rows_k<8, E>), grid, dim3(256), 0, stream(), R, K, mat, vec, c, ep);
