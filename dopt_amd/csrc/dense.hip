@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int run
         tops[place(c)] = max(max(magnitude(red[0][c]), magnitude(red[1][c])), max(magnitude(red[2][c]), magnitude(red[3][c])));
 }
 
-__global__ __launch_bounds__(kBlock) void dense_fold_k(DenseFold f) { dense_fold(f, blockIdx.x); }
+__global__ __launch_bounds__(kBlock) void dense_fold_k(DenseFold f) { dense_fold(f, (size_t)blockIdx.y * kLaunchBlocks + blockIdx.x); }
 
 int check(const char *who, size_t M, size_t N, size_t K, int act)
 {
@@ -217,7 +217,9 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
     }
     const DenseFold fold{sums ? (size_t)runs : 0, N, sums, N > 0 ? dbias : nullptr};
     if (fold.dbias && !wides) {
-        hipLaunchKernelGGL(dense_fold_k, dim3((unsigned)ceil_div(N, (size_t)8)), dim3(kBlock), 0, stream(), fold);
+        const size_t blocks = ceil_div(N, (size_t)8);
+        hipLaunchKernelGGL(dense_fold_k, dim3((unsigned)std::min(blocks, kLaunchBlocks), (unsigned)ceil_div(blocks, kLaunchBlocks)), dim3(kBlock), 0, stream(),
+                           fold);
         DOPT_LAUNCH_CHECK();
     }
     workspace_hold(held);

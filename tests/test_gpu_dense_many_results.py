@@ -22,3 +22,13 @@ def test_a_wavefront_per_result():
     assert np.array_equal(ops.dense_act(tv, tw, tb).numpy()[:, 0], want)
     assert np.array_equal(ops.dense_act(tw, tv, act="relu").numpy()[0], np.maximum(want - 1, 0))
     assert np.array_equal(ops.matmul_t(tv, tw, False, True).numpy()[:, 0], want - 1)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_column_sums(rows):
+    n = (1 << 27) + 3
+    dy = _whole(np.random.default_rng(2), (rows, n))
+    td, out = ops.tensor(dy), ops.tensor(np.full(n + 8, 99.0, F32))
+    capi.check(capi.load().dopt_hip_dense_act_grad(rows, n, 1, 0, td.ptr, None, None, None, None, None, out.ptr))
+    got = out.numpy()
+    assert np.array_equal(got[:n], dy.sum(0)) and (got[n:] == 99.0).all()
