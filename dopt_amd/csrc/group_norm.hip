@@ -86,6 +86,18 @@ __device__ __forceinline__ float block_sum(float v, float *red)
     return s;
 }
 
+// A sum of any length with what its roundings have left out (Kahan): many equal values are rounded the same way again and again, 135168 of
+// 0.1 to a mean that is 1e-3 off.
+struct LongSum {
+    float sum = 0.0f, over = 0.0f;
+    __device__ __forceinline__ void add(float v)
+    {
+        const float more = v - over, next = sum + more;
+        over = __builtin_fabsf(next) <= 3.402823466e38f ? (next - sum) - more : 0.0f;   // (infinity stays one)
+        sum = next;
+    }
+};
+
 // What a workgroup holds of a group: `channels` of them from the group's channel c0 on, `len` values of each from `i0` on, P lanes to a
 // channel; a thread has channels row, row + rows, .. (kC of them) and quads lane, lane + P, .. (kQ) of each.
 struct Part {
@@ -930,15 +942,14 @@ __global__ __launch_bounds__(kBlock) void gn_any_fwd_k(Place p, float eps, int a
     __shared__ float red[16];
     const size_t group = block_id(), n = group / p.G, g = group % p.G, L = p.Cg * p.inner;
     if (n >= p.N) return;
-    float s = 0.0f;
-    for (size_t i = threadIdx.x; i < L; i += kBlock) s += x[p.at(n, g, i)];
-    const float mean = L ? block_sum(s, red) / (float)L : 0.0f;
-    float q = 0.0f;
+    LongSum s, q;
+    for (size_t i = threadIdx.x; i < L; i += kBlock) s.add(x[p.at(n, g, i)]);
+    const float mean = L ? block_sum(s.sum, red) / (float)L : 0.0f;
     for (size_t i = threadIdx.x; i < L; i += kBlock) {
         const float d = x[p.at(n, g, i)] - mean;
-        q += d * d;
+        q.add(d * d);
     }
-    const float rstd = 1.0f / sqrtf((L ? block_sum(q, red) / (float)L : 0.0f) + eps);
+    const float rstd = 1.0f / sqrtf((L ? block_sum(q.sum, red) / (float)L : 0.0f) + eps);
     with_activation(act, [&](auto kind) {
         for (size_t i = threadIdx.x; i < L; i += kBlock) {
             const size_t at = p.at(n, g, i), c = p.channel(g, i);
