@@ -360,15 +360,16 @@ __device__ __forceinline__ void fold(const Fold &f, size_t block, float2 *red)
 {
     const int col = threadIdx.x & 7, lane = threadIdx.x >> 3;
     const size_t c = block * 8 + col;
-    float s = 0.0f, q = 0.0f;
+    LongSum sum_x, sum_y;
     if (c < f.C) {
 #pragma unroll 8
         for (size_t i = lane; i < f.rows * f.pieces; i += 32) {
             const float2 v = f.pieces == 1 ? f.sums[i * f.C + c] : f.sums[(i / f.pieces * f.C + c) * f.pieces + i % f.pieces];
-            s += v.x;
-            q += v.y;
+            sum_x.add(v.x);
+            sum_y.add(v.y);
         }
     }
+    float s = sum_x.sum, q = sum_y.sum;
     red[lane * 9 + col] = make_float2(s, q);
     meet();
     if (lane == 0 && c < f.C) {
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
     const int mine = row < r.R && row < run.count ? (run.count - row + r.R - 1) / r.R : 0;
     with_activation(act, [&](auto kind) {
         for (int u = u0; u < r.U && row < r.R; u += kBlock) {
-            float mean[V], rstd[V], a[V], b[V], s[V], q[V];
+            float mean[V], rstd[V], a[V], b[V], s[V], q[V], all_s[V], all_q[V];
 #pragma unroll
             for (int e = 0; e < V; e++) {
                 const int c = u * V + e, g = c / r.Cg;
@@ -624,6 +625,7 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
                 b[e] = bias[c];
                 s[e] = kDx ? entry[g].x : 0.0f;
                 q[e] = kDx ? entry[g].y : 0.0f;
+                all_s[e] = all_q[e] = 0.0f;
             }
             const size_t first = run.at + (size_t)row * r.C + (size_t)u * V, step = (size_t)r.R * r.C;
             auto one = [&](vec v, vec d, size_t at) {
@@ -641,8 +643,17 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
                 }
                 if (kDx) *(vec *)(dx + at) = o;
             };
+            auto put_aside = [&]() {
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    all_s[e] += s[e];
+                    all_q[e] += q[e];
+                    s[e] = q[e] = 0.0f;
+                }
+            };
             int j = 0;
             for (; j + 4 <= mine; j += 4) {
+                if (!kDx && (j & 63) == 0) put_aside();   // sums of 64 values each, so that many like ones do not round the same way for long
                 vec v[4], d[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -657,8 +668,9 @@ __global__ __launch_bounds__(kBlock) void gn_last_grad_k(Rows r, int act, const 
                 one(*(const vec *)(x + at), *(const vec *)(dy + at), at);
             }
             if (!kDx) {
+                put_aside();
 #pragma unroll
-                for (int e = 0; e < V; e++) entry[(size_t)row * r.C + (size_t)u * V + e] = make_float2(s[e], q[e]);
+                for (int e = 0; e < V; e++) entry[(size_t)row * r.C + (size_t)u * V + e] = make_float2(all_s[e], all_q[e]);
             }
         }
     });
@@ -903,12 +915,18 @@ __global__ __launch_bounds__(kBlock) void gn_row_sums_k(size_t N, size_t C, int 
         const float a = scale[c], b = bias[c];
         const size_t g = c / Cg;
         with_activation(act, [&](auto kind) {
+            for (size_t first = from + (threadIdx.x >> 6); first < to; first += 256) {   // (of 64 values each, as below)
+                const size_t end = min(first + 256, to);
+                float t = 0.0f, u = 0.0f;
 #pragma unroll 4
-            for (size_t n = from + (threadIdx.x >> 6); n < to; n += 4) {
-                const float xhat = (x[n * C + c] - means[n * G + g]) * rstds[n * G + g];
-                const float dz = act_grad<kind.value>(dy[n * C + c], xhat * a + b);
-                s += dz;
-                q += dz * xhat;
+                for (size_t n = first; n < end; n += 4) {
+                    const float xhat = (x[n * C + c] - means[n * G + g]) * rstds[n * G + g];
+                    const float dz = act_grad<kind.value>(dy[n * C + c], xhat * a + b);
+                    t += dz;
+                    u += dz * xhat;
+                }
+                s += t;
+                q += u;
             }
         });
     }
@@ -997,14 +1015,13 @@ __global__ __launch_bounds__(kBlock) void gn_any_dx_k(Place p, int act, const fl
     const size_t group = block_id(), n = group / p.G, g = group % p.G, L = p.Cg * p.inner;
     if (n >= p.N) return;
     const float mean = means[group], rstd = rstds[group];
-    float s1 = 0.0f, s2 = 0.0f;
+    LongSum t, u;
     for (size_t c = g * p.Cg + threadIdx.x; c < (g + 1) * p.Cg; c += kBlock) {
         const float2 v = sums[n * p.C + c];
-        s1 += v.x * scale[c];
-        s2 += v.y * scale[c];
+        t.add(v.x * scale[c]);
+        u.add(v.y * scale[c]);
     }
-    s1 = block_sum(s1, red) / (float)L;
-    s2 = block_sum(s2, red) / (float)L;
+    const float s1 = block_sum(t.sum, red) / (float)L, s2 = block_sum(u.sum, red) / (float)L;
     with_activation(act, [&](auto kind) {
         for (size_t i = threadIdx.x; i < L; i += kBlock) {
             const size_t at = p.at(n, g, i), c = p.channel(g, i);
