@@ -62,11 +62,11 @@ __global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int run
     const size_t col = min(first + (threadIdx.x & 63) * V, N - V);
     const size_t from = M * run / runs, to = M * (run + 1) / runs;
     const int row = threadIdx.x >> 6;
-    float s[V];
+    float s[V], all[V];
     unsigned top[V];
 #pragma unroll
     for (int e = 0; e < V; e++) {
-        s[e] = 0.0f;
+        s[e] = all[e] = 0.0f;
         top[e] = 0;
     }
     with_activation(act, [&](auto kind) {
@@ -83,6 +83,13 @@ __global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int run
         };
         size_t m = from + row;
         for (; m + 12 < to; m += 16) {
+            if (((m - from) & 255) < 4) {   // sums of 64 values each: 1024 equal ones in a row are rounded the same way to 1.5e-5 of their sum
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    all[e] += s[e];
+                    s[e] = 0.0f;
+                }
+            }
             vec d[4], z[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -100,7 +107,7 @@ __global__ __launch_bounds__(kBlock) void dense_dz_k(size_t M, size_t N, int run
     auto place = [&](size_t c) { return run * N + min(first + c / V * V, N - V) + c % V; };
     if (sums) {
 #pragma unroll
-        for (int e = 0; e < V; e++) red[row][(threadIdx.x & 63) * V + e] = s[e];
+        for (int e = 0; e < V; e++) red[row][(threadIdx.x & 63) * V + e] = all[e] + s[e];
         __syncthreads();
         for (size_t c = threadIdx.x; c < 64 * V; c += kBlock) sums[place(c)] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
     }

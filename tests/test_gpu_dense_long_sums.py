@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from dopt_amd import ops
+from dopt_amd import capi, ops
 
 pytestmark = pytest.mark.gpu
 F32 = np.float32
@@ -52,3 +52,15 @@ def test_gradients(size, kind):
     _held(dx, dy @ w, "dx")
     _held(dw, dy.T @ x, "dw")
     _held(db, dy.sum(0), "dbias")
+
+
+@pytest.mark.parametrize("size", [(1 << 18, 8192), (1 << 20, 1001), (1 << 20, 3)], ids=str)
+def test_column_sums_of_equal_values(size):
+    """Each column of one value, whose roundings all go the same way: chains of 64, 64 and 64 additions, each off by half a step of its sum."""
+    m, n = size
+    v = np.random.default_rng(3).uniform(0.05, 1.0, n).astype(F32)
+    td = ops.tensor(np.broadcast_to(v, (m, n)))
+    db = ops.Tensor((n,))
+    capi.check(capi.load().dopt_hip_dense_act_grad(m, n, 1, 0, td.ptr, None, None, None, None, None, db.ptr))
+    off = db.numpy().astype(np.float64) / (v.astype(np.float64) * m) - 1
+    assert np.abs(off).max() <= 192 * E, np.abs(off).max()
