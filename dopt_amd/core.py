@@ -552,16 +552,26 @@ def _verify_dense_act(op, x):
             all(d.dtype == float32_t for d in op.deps))
 
 
+def _rows(t, m):
+    """Whether the values lie in m rows, or in one: a matrix the other way round holds as many."""
+    return t.rank < 2 or t.shape[0] == m
+
+
 def _verify_dense_act_forward(op):
-    a, m, n = op.attributes, op.deps[0].shape[0], op.deps[1].shape[0]
+    a = op.attributes
+    if not _verify_dense_act(op, 0):
+        return False
+    m, n = op.deps[0].shape[0], op.deps[1].shape[0]
     rest = [v for v, has in ((n, a["hasBias"]), (m * n, a["hasResidual"])) if has]
-    return _verify_dense_act(op, 0) and [d.volume for d in op.deps[2:]] == rest
+    return [d.volume for d in op.deps[2:]] == rest and (not a["hasResidual"] or _rows(op.deps[-1], m))
 
 
 def _verify_dense_act_grad(op):
+    if not _verify_dense_act(op, 1):
+        return False
     m, n = op.deps[1].shape[0], op.deps[2].shape[0]
-    return (_verify_dense_act(op, 1) and op.deps[0].volume == m * n and
-            [d.volume for d in op.deps[3:]] == ([m * n] if op.attributes["activation"] else []))
+    return (op.deps[0].volume == m * n and [d.volume for d in op.deps[3:]] == ([m * n] if op.attributes["activation"] else []) and
+            all(_rows(d, m) for d in op.deps[:1] + op.deps[3:]))
 
 
 register_operation("groupNorm", lambda op: len(op.deps) == 3 and _verify_group_norm(op, 0), _judge_group_norm)

@@ -471,11 +471,11 @@ def _dense_sizes(x, w):
     return x.shape[0], w.shape[0], x.shape[1]
 
 
-def _operand(t, size, what):
-    """The address of an operand that may be missing."""
+def _operand(t, size, what, rows=None):
+    """The address of an operand that may be missing; `rows`: of a matrix, which the other way round holds as many values."""
     if t is None:
         return None
-    if t.size != size or t.dtype != _F32:
+    if t.size != size or t.dtype != _F32 or (rows is not None and len(t.shape) > 1 and t.shape[0] != rows):
         raise capi.HipError(1, "denseAct: %s has the wrong size or type" % what)
     return t.ptr
 
@@ -485,7 +485,7 @@ def dense_act(x, w, bias=None, residual=None, act="none", out=None, pre=None):
     M, N, K = _dense_sizes(x, w)
     y = _out(out, (M, N))
     _run(capi.load().dopt_hip_dense_act(M, N, K, _activation(act), x.ptr, w.ptr, _operand(bias, N, "bias"),
-                                        _operand(residual, M * N, "residual"), y.ptr, _operand(pre, M * N, "pre")))
+                                        _operand(residual, M * N, "residual", M), y.ptr, _operand(pre, M * N, "pre", M)))
     return y
 
 
@@ -496,7 +496,7 @@ def dense_act_grad(dy, x, w, pre=None, act="none", dx=None, dw=None, dbias=None)
     if pre is None and code:
         raise capi.HipError(1, "denseActGrad: the gradient of an activation reads what it was applied to")
     dx, dw, dbias = _out(dx, (M, K)), _out(dw, (N, K)), _out(dbias, (N,))
-    _run(capi.load().dopt_hip_dense_act_grad(M, N, K, code, _operand(dy, M * N, "dy"), _operand(pre, M * N, "pre"), x.ptr, w.ptr, dx.ptr,
+    _run(capi.load().dopt_hip_dense_act_grad(M, N, K, code, _operand(dy, M * N, "dy", M), _operand(pre, M * N, "pre", M), x.ptr, w.ptr, dx.ptr,
                                              dw.ptr, dbias.ptr))
     return dx, dw, dbias
 
