@@ -181,7 +181,7 @@ private class FusedUpdater
 
             case Rule.muon:
                 hipCheck(dopt_hip_muon_step(mMuon, scalar(mHyper[0]), scalar(mHyper[1]), mNesterov ? 1 : 0,
-                    scalar(mHyper[2]), 5));
+                    scalar(mHyper[2]), mIterations));
                 hipCheck(dopt_hip_sgd_step(mHandle, scalar(mHyper[3]), scalar(mHyper[1]), 0));
                 break;
         }
@@ -204,6 +204,7 @@ private class FusedUpdater
     Operation[] mOutputs;
     Operation[] mHyper;
     bool mNesterov;
+    int mIterations;
     float mB1 = 1.0f, mB2 = 1.0f;   //the running products beta^t of online/adam.d:44-46
     HIPPlan mPlan, mPostPlan;
     DeviceBuffer[] mRets, mPostRets;
@@ -258,11 +259,13 @@ Updater amsgrad(Operation[] outputs, Operation[] wrt, Projection[Operation] proj
 */
 Updater muon(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
     Operation learningRate = float32([], [0.02f]), Operation momentumRate = float32([], [0.95f]), bool nesterov = true,
-    Operation decay = float32([], [0.0f]), Operation restRate = float32([], [0.01f]))
+    Operation decay = float32([], [0.0f]), Operation restRate = float32([], [0.01f]),
+    int iterations = 5)
 {
     auto u = new FusedUpdater(Rule.muon, outputs, wrt, projs);
     u.mHyper = [learningRate, momentumRate, decay, restRate];
     u.mNesterov = nesterov;
+    u.mIterations = iterations;
 
     return &u.update;
 }
