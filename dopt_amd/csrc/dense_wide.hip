@@ -324,7 +324,9 @@ __device__ __forceinline__ void waiting_sums(v16f (&acc)[MI][2], char *at, bool 
 template <int kTile>
 constexpr int kLdsOf = kTile == kBig ? 4 * 32768 : 5 * 16384;
 
-template <int kTile>
+// kPasses: some part of a reduction is longer than a pass.  (The loop by itself, with its registers, takes 1.6 % of both gradients of
+// [1000 x 1777] from 1111 where it runs once.)
+template <int kTile, bool kPasses>
 __global__ __launch_bounds__(2 * kTile, 2) void wide_product_k(Wides both, DenseEpilogue ep)
 {
     constexpr int MI = kTile / 64, kBlocks = kTile / 32;
@@ -349,15 +351,21 @@ __global__ __launch_bounds__(2 * kTile, 2) void wide_product_k(Wides both, Dense
     const char *const left = q.xp + (mt * kBlocks + w) * row_of_blocks, *const right = q.wp + (nt * kBlocks + w) * row_of_blocks;
     const size_t m0 = (size_t)mt * kTile, n0 = (size_t)nt * kTile;
     v16f acc[MI][2];
-    const unsigned passes = (unsigned)((to - from + kPass - 1) / kPass);
+    if constexpr (kPasses) {
+        const unsigned passes = (unsigned)((to - from + kPass - 1) / kPass);
+        char *const waiting = q.waiting + ((size_t)place_of_tile * (kTile / 32) + w) * (MI * 8192) + lane * 16;
 #pragma unroll 1
-    for (unsigned pass = 0;; pass++) {
-        const size_t at = from + (to - from) * pass / passes, next = from + (to - from) * (pass + 1) / passes;
+        for (unsigned pass = 0;; pass++) {
+            const size_t at = from + (to - from) * pass / passes, next = from + (to - from) * (pass + 1) / passes;
+            zero_acc(acc);
+            sums(left + at * 2048, right + at * 2048, (int)(next - at), w, lane, lds, acc);
+            if (passes == 1) break;
+            waiting_sums(acc, waiting, pass > 0, pass + 1 < passes);
+            if (pass + 1 == passes) break;
+        }
+    } else {
         zero_acc(acc);
-        sums(left + at * 2048, right + at * 2048, (int)(next - at), w, lane, lds, acc);
-        if (passes == 1) break;
-        waiting_sums(acc, q.waiting + ((size_t)place_of_tile * (kTile / 32) + w) * (MI * 8192) + lane * 16, pass > 0, pass + 1 < passes);
-        if (pass + 1 == passes) break;
+        sums(left + from * 2048, right + from * 2048, (int)(to - from), w, lane, lds, acc);
     }
 
     int *const shift = (int *)lds;
@@ -495,13 +503,13 @@ int tile_for(size_t M, size_t N, size_t K)
     return std::min(M, N) >= 256 && K <= 12 * std::min(M, N) && M * N * K >= (size_t)900000000 ? kSmall : 0;
 }
 
-template <int kTile>
+template <int kTile, bool kPasses>
 int launch_tiles(const Wides &both, const DenseEpilogue &e)
 {
     static bool raised = false;
-    if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)wide_product_k<kTile>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsOf<kTile>));
+    if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)wide_product_k<kTile, kPasses>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsOf<kTile>));
     raised = true;
-    hipLaunchKernelGGL(wide_product_k<kTile>, dim3(8 * (both.per[0] + both.per[1])), dim3(2 * kTile), kLdsOf<kTile>, stream(), both, e);
+    hipLaunchKernelGGL((wide_product_k<kTile, kPasses>), dim3(8 * (both.per[0] + both.per[1])), dim3(2 * kTile), kLdsOf<kTile>, stream(), both, e);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
@@ -511,7 +519,11 @@ int launch_products(int tile, const Wide *q, int n, const DenseEpilogue &e)
     Wides both{{q[0], q[n - 1]}, {0, 0}};
     if (n == 2 && q[1].steps * q[0].splits > q[0].steps * q[1].splits) std::swap(both.q[0], both.q[1]);
     for (int i = 0; i < n; i++) both.per[i] = (unsigned)ceil_div((size_t)both.q[i].tiles * both.q[i].splits, (size_t)8);
-    if (int rc = tile == kBig ? launch_tiles<kBig>(both, e) : launch_tiles<kSmall>(both, e)) return rc;
+    const bool passes = q[0].waiting || q[n - 1].waiting;
+    int rc;
+    if (tile == kBig) rc = passes ? launch_tiles<kBig, true>(both, e) : launch_tiles<kBig, false>(both, e);
+    else rc = passes ? launch_tiles<kSmall, true>(both, e) : launch_tiles<kSmall, false>(both, e);
+    if (rc) return rc;
     if (n == 1) both.q[1].splits = 1;
     size_t values = 0;
     for (const Wide &p : both.q) values += p.splits > 1 ? p.M * p.N : 0;
