@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from dopt_amd import capi, ops
+from dopt_amd import capi, core, ops
 
 pytestmark = pytest.mark.gpu
 F32 = np.float32
@@ -64,3 +64,42 @@ def test_column_sums_of_equal_values(size):
     capi.check(capi.load().dopt_hip_dense_act_grad(m, n, 1, 0, td.ptr, None, None, None, None, None, db.ptr))
     off = db.numpy().astype(np.float64) / (v.astype(np.float64) * m) - 1
     assert np.abs(off).max() <= 192 * E, np.abs(off).max()
+
+
+@pytest.mark.parametrize("size", [(2400, 2411, 5000), (2001, 2000, 9001)], ids=str)
+def test_values_that_are_not_finite(size):
+    """They reach their row and column whichever pass they are in, and no others."""
+    m, n, k = size
+    r = np.random.default_rng(5)
+    x, w = _operand(r, (m, k), "uniform"), _operand(r, (n, k), "uniform")
+    # no zeros for an infinity to meet
+    x[:, 4500], w[:, k - 1] = np.maximum(x[:, 4500], F32(1e-3)), np.maximum(w[:, k - 1], F32(1e-3))
+    clean = ops.dense_act(ops.tensor(x), ops.tensor(w), act="relu").numpy()
+    x[7, 3], x[m - 1, k - 1], w[n - 1, 4500] = np.nan, np.inf, np.inf
+    y = ops.dense_act(ops.tensor(x), ops.tensor(w), act="relu").numpy()
+    nan, inf = np.zeros((m, n), bool), np.zeros((m, n), bool)
+    inf[m - 1], inf[:, n - 1] = True, True
+    inf[7], nan[7] = False, True
+    assert np.array_equal(np.isnan(y), nan) and np.array_equal(np.isposinf(y), inf)
+    rest = ~(nan | inf)
+    assert np.array_equal(y[rest], clean[rest])
+
+
+@pytest.mark.parametrize("size", [(2400, 2411, 5000), (2000, 2000, 9001)], ids=str)
+def test_recorded_passes(size):
+    """Replays, with other users of the workspace between them, give the bits of the call."""
+    m, n, k = size
+    r = np.random.default_rng(6)
+    x, w = _operand(r, (m, k), "relu"), _operand(r, (n, k), "uniform")
+    vx, vw = core.float32([m, k]), core.float32([n, k], w)
+    plan = core.compile([core.denseAct(vx, vw, None, None, "silu")], core.PLAN_VIEWS | core.PLAN_FUSE | core.PLAN_GRAPH)
+    out = ops.tensor(np.full(m * n + 64, 3.0, F32))
+    dev = {vx: ops.tensor(x)}
+    want = ops.dense_act(dev[vx], ops.tensor(w), act="silu").numpy()
+    for _ in range(4):
+        out.set(np.full(out.shape, 3.0, F32))
+        plan.execute(dev, [out.view(0, (m, n))])
+        got = out.numpy()
+        assert np.array_equal(got[:m * n].reshape(m, n), want) and (got[m * n:] == 3.0).all()
+        ops.dense_act(ops.tensor(x[:900]), ops.tensor(w[:900]))
+    assert plan.recordings()["replays"] >= 2
