@@ -7,10 +7,11 @@
 // that is, fp32's own rounding of a long sum unless a row spans more than seventeen binary orders and its largest values meet zeros.
 // Three bf16 parts, which sgemm.hip uses for operands of any kind, keep 24 bits and take twice the matrix work.
 //
-// Bound by the matrix instructions, 6 M N K operations, where tiles are large: [8192 x 4096] from 4096 steps, 824 GFLOP, takes 728 us, 86 of
-// them for the layout (402 MB, 4.7 TB/s) and 640 for the product (1290 TFLOP/s; a library's bf16 product of 4096 cubed reaches 1157).
+// Bound by the matrix instructions, 6 M N K operations, where tiles are large: [8192 x 4096] from 4096 steps, 824 GFLOP, takes 730 us, 79 of
+// them for the layout (402 MB, 5.1 TB/s) and 660 for the product (1250 TFLOP/s; a library's bf16 product of 4096 cubed reaches 1157) - once the
+// card's clock has settled: in the first thirty products after a pause it takes up to 880.
 // The matrix instructions are busy 72 % of its cycles, at the clock that is left when they are.  With tiles of 128 x 128 the bound is
-// what a CU takes in, some 45 GB/s whoever asks for it: both gradients of [1000 x 1777] from 1111 take 63 us, 33 of them for the
+// what a CU takes in, some 45 GB/s whoever asks for it: both gradients of [1000 x 1777] from 1111 take 66 us, 33 of them for the
 // products, 9 for dz, 17 for the layout and 8 to add parts.
 #include <algorithm>
 #include <type_traits>
@@ -66,7 +67,7 @@ __device__ __forceinline__ void store_parts(char *block, int row, int half, cons
 
 // Four rows per workgroup, eight values of a row to each of its threads and those of kUnits further places, in registers between the
 // search for the rows' largest values and the layout: sixteen steps of the four rows are stored by eight threads, 256 bytes
-// in a line.  Bound by memory: [8192 + 4096] rows of 4096 take 86 us, read twice, which the L2 does not shorten, 106.  Longer rows than
+// in a line.  Bound by memory: [8192 + 4096] rows of 4096 take 79 to 86 us, read twice, which the L2 does not shorten, 106.  Longer rows than
 // the registers hold are read twice.  Padding and rows that are not finite become zeros.
 constexpr int kUnits = 8;
 __device__ __forceinline__ void split_rows(const Operand &o, unsigned block)

@@ -9,14 +9,15 @@
 // All of it is bound by memory: 8 bytes a value forward, 12 backward.  A group of an [N, C, inner] tensor lies in one piece, and up to
 // 32768 values of it (of the gradient 16384 of both tensors) stay in the registers of one workgroup, which so reads and writes everything
 // once.  Longer groups are parted: a first launch leaves each part's statistics (or sums), a second one joins them and reads the part again.
-// Channels-last groups lie in pieces of C / G values; those of 32 bytes and more are held likewise, otherwise workgroups take
-// runs of pixels with all their channels, in two launches.  Means are taken before variances everywhere - of a part in registers, then
-// of the parts - so nothing cancels however far from zero the values lie.  No atomics: every sum has one order.
+// Channels-last groups lie in pieces of C / G values; those of 8 to 64 channels, a power of two, are held likewise (gradients where that is
+// faster, see held_for), otherwise workgroups take runs of pixels with all their channels, in two launches.  Means are taken before variances everywhere - of a part in registers, then
+// of the parts - so nothing cancels however far from zero the values lie; sums of any length are taken in pieces or keep what their roundings leave out.
+// No atomics: every sum has one order.
 //
-// Measured: [128, 160, 32 x 32] in 32 groups 34 us (168 MB, 4.9 TB/s), its like of 320 channels of 16 x 16 backward 34.5 us (126 MB), of
-// which the sums over samples take 4.6; channels last [37, 29 x 33, 200] in 25 groups 15.4 us (57 MB; in two launches by runs 25),
-// [64, 32 x 32, 128] in 16 groups backward 32 us by runs (101 MB; two passes over x and dy, the second from the last cache);
-// one sample of [64, 8 x 8] 5.4 us, a launch.
+// Measured: [128, 160, 32 x 32] in 32 groups 34 us (168 MB, 4.9 TB/s), its like of 320 channels of 16 x 16 backward 35 us (126 MB), of
+// which the sums over samples take 5; channels last [37, 29 x 33, 200] in 25 groups 15.4 us (57 MB; in two launches by runs 25),
+// [64, 32 x 32, 128] in 16 groups backward 33 us by runs (101 MB; two passes over x and dy, the second from the last cache);
+// one sample of [64, 8 x 8] 5.5 us, a launch.
 #include <algorithm>
 #include <type_traits>
 

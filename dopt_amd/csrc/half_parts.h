@@ -1,5 +1,6 @@
 // Products of fp32 values as two fp16 parts each: h = fp16(v) and l = fp16(v - h), 22 bits in four bytes, and the three products h h + h l + l h
-// on the fp16 matrix instruction, in fp32 sums.  The caller scales its values into fp16's range.
+// on the fp16 matrix instruction, in fp32 sums.  The caller scales its values into fp16's range, and bounds how many steps are added in one accumulator: all three
+// products go there, and the instruction rounds down what lies below its guard bits.
 //
 // Operands run along the reduction.  They lie in blocks of 32 rows by 16 steps, 2 KB one after the other along a row of blocks; a row of a
 // block is 64 bytes, h and l parts of eight values (16 bytes each) and of the next eight.  Inside a row the four pieces lie at

@@ -14,7 +14,8 @@
 // symmetric (half of its tiles are formed, and stored twice), and X is read and written once per group: 6 s^2 l + 14 s^3
 // operations for five iterations on [s, l] instead of 15 s^2 l + 5 s^3.  An error of A, 2^-24 of its largest eigenvalue, grows by
 // a^2 with each iteration that A is carried on rather than formed again: within three by 142, to 1e-5 of a direction that is
-// still weak; all five at once would make it 1e-2.
+// still weak; all five at once would make it 1e-2.  (A's diagonal is a sum of squares, which the matrix instruction lets drift downwards: parts of
+// 262144 steps, those of [1 x 4194304], leave an update 4e-6 off, of 16384 steps 1e-6.)
 //
 // The products run on the fp16 matrix instruction with every value as the sum of two fp16 numbers, h = fp16(v) and
 // l = fp16(v - h), of the three products h h + h l + l h that matter, in fp32 sums.  Two parts hold 22 bits, and l l is 2^-24 of
@@ -31,9 +32,9 @@
 // took three times as long.  Inside a row the four pieces lie at place piece ^ (row / 4 mod 4), in memory as in LDS, so that
 // lanes which read the same piece of neighbouring rows touch different banks.
 //
-// Measured: VGG-16's sixteen matrices 448 us (39 for the momenta and 49 for X, at 5 TB/s; 72 for the two A, 140 for X after
-// three and five iterations, 13 x 13.6 for square products, each a launch and what a CU takes in of its operands), eight of up to [640 x 5760]
-// 760 to 810 by the machine (68, 85, 146, 300, 13 x 17.5), one [64 x 576] 53.
+// Measured: VGG-16's sixteen matrices 448 to 465 us by the machine (39 for the momenta and 44 for X, at 5 TB/s; 66 for the two A and 15 for
+// their parts, 129 for X after three and five iterations, 13 x 12.1 for square products, each a launch and what a CU takes in of its
+// operands), eight of up to [640 x 5760] 760 to 810 (67, 83, 132, 18, 276, 13 x 15), one [64 x 576] 53.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

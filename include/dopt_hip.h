@@ -538,9 +538,12 @@ int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, in
 /* pre = x * w^T + bias, y = act(pre) + residual: x [M,K], w [N,K] as nnet/layers/dense.d stores it, bias [N], residual [M,N].
    bias, residual and pre may be null; a training step keeps pre, which the gradient reads (act none needs none).  y and pre may
    overlap neither each other nor an operand.
-   Large products (from some 8e8 multiplications on, both sides 256 and more) are formed from two fp16 parts of each value, scaled row by row:
-   a value keeps 22 bits, or 2^-39 of its row's largest one where that is more.  They take workspace: four bytes a value of
-   both operands, rows counted up to a multiple of 256.  Values that are not finite reach the results that fp32 would give them. */
+   Large products (from 9e8 multiplications on with both sides 256 and more, or with tiles of 256 x 256 for a third of the compute units, and
+   reductions of 128 and more) are formed from two fp16 parts of each value, scaled row by row: a value keeps 22 bits, or 2^-39 of its row's
+   largest one where that is more; at most 4096 products are added in one accumulator.  They take workspace: four bytes a value of both
+   operands, rows counted up to a multiple of 256 and their lengths to one of 16, four bytes a value of the result for each part that a long
+   reduction over few tiles is cut into, and as much again where a part is longer than 4096.  Values that are not finite reach the results that
+   fp32 would give them.  residual lies as y does. */
 int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, const float *w, const float *bias,
                        const float *residual, float *y, float *pre);
 /* With dz = dy * act'(pre): dx = dz * w [M,K], dw = dz^T * x [N,K], dbias = column sums of dz [N]; the residual's gradient is dy.
@@ -593,8 +596,8 @@ typedef struct {
      `iterations` times (five as a rule), on the side of fewer rows:  A = X X^T,  X = 3.4445 X + (-4.7750 A + 2.0315 A A) X,
      w' = (1 - lr decay) w - lr sqrt(max(1, rows / cols)) X
    for all matrices of the handle at once.  The handle keeps the addresses and the scratch memory that the step needs, sixteen bytes
-   a value with both sides counted up to multiples of 128 (of 64, where the shorter one is no longer) and 24 a value of A; no w
-   or m may overlap another operand of the set.  The shorter side of a matrix may have up to 16384 values, all of it 2^28. */
+   a value with both sides counted up to multiples of 128 (of 64, where the shorter one is no longer), 24 a value of A, and four a value
+   of A's lower half for each part that its reduction is cut into; no w or m may overlap another operand of the set.  The shorter side of a matrix may have up to 16384 values, all of it 2^28. */
 int dopt_hip_muon_create(int nmatrices, const dopt_hip_matrix_ref *refs, void **handle);
 int dopt_hip_muon_destroy(void *handle);
 int dopt_hip_muon_step(void *handle, float lr, float mu, int nesterov, float decay, int iterations);
