@@ -87,3 +87,39 @@ def test_three_steps_of_a_network_follow_the_formula(make, nesterov):
                 mom[i] = mu * mom[i] + rest * g[i]
                 want, bound = before[i] - mom[i], off * np.linalg.norm(mom[i])
             assert np.linalg.norm(p.value - want) <= bound + 4 * R.E * np.linalg.norm(want), (i, p.shape)
+
+
+@pytest.mark.parametrize("make", [online.muon, online.fused_muon], ids=["graph", "fused"])
+@pytest.mark.parametrize("which", ["matrices", "rest", "projected"])
+def test_sets_without_a_rest_or_without_matrices(make, which):
+    """Only matrices, none at all, and two whose projections change the updated value and replace it."""
+    r = np.random.default_rng(8)
+    lr, mu, rest, iterations = 0.1, 0.5, 0.2, 2
+    shapes = {"matrices": [(6, 9), (12, 5)], "rest": [(7,), (1, 9), (5, 1)], "projected": [(6, 9), (8, 4), (4,)]}[which]
+    start, targets = [r.standard_normal(s, F32) for s in shapes], [r.standard_normal(s, F32) for s in shapes]
+    ps = [core.float32(list(s), v) for s, v in zip(shapes, start)]
+    ts = [core.float32(list(s)) for s in shapes]
+    loss = None
+    for p, t in zip(ps, ts):
+        d = p - t
+        term = core.sum(d * d).reshape([])
+        loss = term if loss is None else loss + term
+    projs = {ps[0]: lambda v: 0.5 * v, ps[1]: lambda ignored: 2.0 * ts[1]} if which == "projected" else {}
+    step = make([loss], ps, projs, learningRate=lr, momentumRate=mu, nesterov=False, restRate=rest, iterations=iterations)
+    dev = {t: ops.tensor(v) for t, v in zip(ts, targets)}
+    want, mom = [s.astype(np.float64) for s in start], [np.zeros(s) for s in shapes]
+    for _ in range(3):
+        step(dev)
+        for i, s in enumerate(shapes):
+            g = 2 * (want[i] - targets[i])
+            if len(s) > 1 and s[0] > 1 and np.prod(s) > s[0]:
+                new, mom[i], o = R.muon(want[i], g, mom[i], lr, mu, False, 0.0, iterations)
+                bound = lr * (R.muon_bound(iterations) + 12 * 64 * R.E) * np.linalg.norm(o)
+            else:
+                mom[i] = mu * mom[i] + rest * g
+                new, bound = want[i] - mom[i], 64 * R.E * np.linalg.norm(mom[i])
+            if which == "projected" and i < 2:
+                new = 0.5 * new if i == 0 else 2.0 * targets[1].astype(np.float64)
+            got = ps[i].value.astype(np.float64)
+            assert np.linalg.norm(got - new) <= bound + 8 * R.E * np.linalg.norm(new), (i, s)
+            want[i] = got   # (the next step starts from the values that are there)
