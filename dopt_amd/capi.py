@@ -48,6 +48,11 @@ class MatrixRef(C.Structure):
     _fields_ = [("w", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("rows", C.c_size_t), ("cols", C.c_size_t)]
 
 
+class GradientRef(C.Structure):
+    """dopt_hip_gradient_ref: a gradient and where it goes when it is clipped."""
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("n", C.c_size_t)]
+
+
 _sz, _vp, _i, _f, _d = C.c_size_t, C.c_void_p, C.c_int, C.c_float, C.c_double
 _szp = C.POINTER(C.c_size_t)
 
@@ -148,6 +153,14 @@ PROTOTYPES = {
     "dopt_hip_sgd_step": [_vp, _f, _f, _i],
     "dopt_hip_adam_step": [_vp, _f, _f, _f, _f, C.POINTER(_f), C.POINTER(_f)],
     "dopt_hip_amsgrad_step": [_vp, _f, _f, _f, _f, C.POINTER(_f), C.POINTER(_f)],
+    "dopt_hip_sgd_step_scaled": [_vp, _f, _f, _i, _vp],
+    "dopt_hip_adam_step_scaled": [_vp, _f, _f, _f, _f, C.POINTER(_f), C.POINTER(_f), _vp],
+    "dopt_hip_amsgrad_step_scaled": [_vp, _f, _f, _f, _f, C.POINTER(_f), C.POINTER(_f), _vp],
+    "dopt_hip_muon_step_scaled": [_vp, _f, _f, _i, _f, _i, _vp],
+    "dopt_hip_gradient_norm_create": [_i, C.POINTER(GradientRef), C.POINTER(_vp)],
+    "dopt_hip_gradient_norm_destroy": [_vp],
+    "dopt_hip_gradient_norm": [_vp, _f, _vp],
+    "dopt_hip_gradient_clip": [_vp, _f, _vp],
 }
 _SPECIAL = {
     "dopt_hip_last_error": ([], C.c_char_p),

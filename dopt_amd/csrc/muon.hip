@@ -86,6 +86,8 @@ struct Tile {
 struct Step {
     float mu, by, keep;
     int nesterov;
+    const float *factor;   // of the gradients; null: one
+    __device__ __forceinline__ float gradient_factor() const { return factor ? *factor : 1.0f; }
 };
 
 // d = alpha l r + beta c + gamma I, in square matrices by number; the factors take the matrices' scales along.
@@ -116,6 +118,7 @@ __global__ __launch_bounds__(kBlock) void muon_momentum_k(const Matrix *jobs, co
     const size_t n = (size_t)q.rows * q.cols, from = (size_t)t.i * kChunk, to = min(from + kChunk, n);
     const Global<const float> g = global(q.g);
     const Global<float> m = global(q.m);
+    const float by = st.gradient_factor();
     double s = 0.0;
     if ((((uintptr_t)q.g | (uintptr_t)q.m) & 15) == 0) {
         constexpr int kQuads = kChunk / kBlock / 4;
@@ -126,7 +129,7 @@ __global__ __launch_bounds__(kBlock) void muon_momentum_k(const Matrix *jobs, co
             const size_t i = from + ((size_t)u * kBlock + threadIdx.x) * 4;
             if (i < whole) {
                 a[u] = *(Global<const v4f>)(m + i);
-                b[u] = *(Global<const v4f>)(g + i);
+                b[u] = *(Global<const v4f>)(g + i) * by;
             }
         }
 #pragma unroll
@@ -141,16 +144,16 @@ __global__ __launch_bounds__(kBlock) void muon_momentum_k(const Matrix *jobs, co
             }
         }
         for (size_t i = whole + threadIdx.x; i < to; i += kBlock) {
-            const float v = st.mu * m[i] + g[i];
+            const float d = g[i] * by, v = st.mu * m[i] + d;
             m[i] = v;
-            const double p = step_value(g[i], v, st);
+            const double p = step_value(d, v, st);
             s += p * p;
         }
     } else {
         for (size_t i = from + threadIdx.x; i < to; i += kBlock) {
-            const float v = st.mu * m[i] + g[i];
+            const float d = g[i] * by, v = st.mu * m[i] + d;
             m[i] = v;
-            const double p = step_value(g[i], v, st);
+            const double p = step_value(d, v, st);
             s += p * p;
         }
     }
@@ -175,12 +178,13 @@ __global__ __launch_bounds__(kBlock) void muon_scale_k(const Matrix *jobs, const
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     float v[16];
+    const float by_g = st.gradient_factor();
 #pragma unroll
     for (int u = 0; u < 16; u++) {
         const int r = t.i * 64 + (int)(threadIdx.x >> 6) + 4 * u, c = t.j * 64 + (int)(threadIdx.x & 63);
         const size_t at = (size_t)r * q.cols + c;
         const size_t safe = r < q.rows && c < q.cols ? at : 0;   // (no branch: the loads go out together)
-        v[u] = step_value(global(q.g)[safe], global(q.m)[safe], st);
+        v[u] = step_value(global(q.g)[safe] * by_g, global(q.m)[safe], st);
     }
     __syncthreads();
     const float by = (float)((double)kUp / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)kEps));
@@ -919,11 +923,16 @@ int dopt_hip_muon_destroy(void *handle)
 
 int dopt_hip_muon_step(void *handle, float lr, float mu, int nesterov, float decay, int iterations)
 {
+    return dopt_hip_muon_step_scaled(handle, lr, mu, nesterov, decay, iterations, nullptr);
+}
+
+int dopt_hip_muon_step_scaled(void *handle, float lr, float mu, int nesterov, float decay, int iterations, const float *factor)
+{
     DOPT_REQUIRE(handle != nullptr, "dopt_hip_muon_step: handle is null");
     DOPT_REQUIRE(iterations >= 0 && iterations <= 100, "dopt_hip_muon_step: %d iterations", iterations);
     const Handle *const h = (const Handle *)handle;
     if (h->jobs.empty()) return DOPT_HIP_OK;
-    const Step st{mu, lr, 1.0f - lr * decay, nesterov != 0};
+    const Step st{mu, lr, 1.0f - lr * decay, nesterov != 0, factor};
     hipLaunchKernelGGL(muon_momentum_k, dim3(h->nchunks), dim3(kBlock), 0, stream(), h->d_jobs, h->chunks, st);
     hipLaunchKernelGGL(muon_scale_k, dim3(h->nscales), dim3(kBlock), 0, stream(), h->d_jobs, h->scales, st);
     DOPT_LAUNCH_CHECK();

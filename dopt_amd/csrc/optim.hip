@@ -90,8 +90,9 @@ __device__ inline void update1(const Scalars &s, float &w, float g, float &m, fl
 
 template <int kRule>
 __global__ __launch_bounds__(kBlock) void optim_k(const TensorDev *tensors, const ChunkDev *chunks, size_t nchunks,
-                                                   Scalars s)
+                                                   Scalars s, const float *factor)
 {
+    const float by = factor ? *factor : 1.0f;   // (times one a gradient keeps its bits)
     constexpr bool kHasV = kRule >= kAdam;
     constexpr bool kHasVhat = kRule == kAmsgrad;
     for (size_t ci = blockIdx.x; ci < nchunks; ci += gridDim.x) {
@@ -114,10 +115,10 @@ __global__ __launch_bounds__(kBlock) void optim_k(const TensorDev *tensors, cons
 #pragma unroll
             for (int u = 0; u < kVecPerThread; u++) {
                 size_t i = b4 + (size_t)u * kBlock + threadIdx.x;
-                update1<kRule>(s, w[u].x, g[u].x, m[u].x, v[u].x, vh[u].x);
-                update1<kRule>(s, w[u].y, g[u].y, m[u].y, v[u].y, vh[u].y);
-                update1<kRule>(s, w[u].z, g[u].z, m[u].z, v[u].z, vh[u].z);
-                update1<kRule>(s, w[u].w, g[u].w, m[u].w, v[u].w, vh[u].w);
+                update1<kRule>(s, w[u].x, g[u].x * by, m[u].x, v[u].x, vh[u].x);
+                update1<kRule>(s, w[u].y, g[u].y * by, m[u].y, v[u].y, vh[u].y);
+                update1<kRule>(s, w[u].z, g[u].z * by, m[u].z, v[u].z, vh[u].z);
+                update1<kRule>(s, w[u].w, g[u].w * by, m[u].w, v[u].w, vh[u].w);
                 if (!t.skip_w) ((float4 *)t.w)[i] = w[u];
                 ((float4 *)t.m)[i] = m[u];
                 if (kHasV) ((float4 *)t.v)[i] = v[u];
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(kBlock) void optim_k(const TensorDev *tensors, cons
             }
         } else {
             for (size_t i = begin + threadIdx.x; i < end; i += kBlock) {
-                float w = t.w[i], g = t.g[i], m = t.m[i];
+                float w = t.w[i], g = t.g[i] * by, m = t.m[i];
                 float v = kHasV ? t.v[i] : 0.0f, vh = kHasVhat ? t.vhat[i] : 0.0f;
                 update1<kRule>(s, w, g, m, v, vh);
                 if (!t.skip_w) t.w[i] = w;
@@ -138,12 +139,12 @@ __global__ __launch_bounds__(kBlock) void optim_k(const TensorDev *tensors, cons
 }
 
 template <int kRule>
-int launch(Handle *h, const Scalars &s)
+int launch(Handle *h, const Scalars &s, const float *factor)
 {
     if (h->nchunks == 0) return DOPT_HIP_OK;
     size_t cap = (size_t)num_cus() * 16;
     unsigned grid = (unsigned)(h->nchunks < cap ? h->nchunks : cap);
-    hipLaunchKernelGGL(optim_k<kRule>, dim3(grid), dim3(kBlock), 0, stream(), h->tensors, h->chunks, h->nchunks, s);
+    hipLaunchKernelGGL(optim_k<kRule>, dim3(grid), dim3(kBlock), 0, stream(), h->tensors, h->chunks, h->nchunks, s, factor);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
@@ -238,32 +239,47 @@ int dopt_hip_optim_destroy(void *handle)
 
 int dopt_hip_sgd_step(void *handle, float lr, float mu, int nesterov)
 {
+    return dopt_hip_sgd_step_scaled(handle, lr, mu, nesterov, nullptr);
+}
+
+int dopt_hip_sgd_step_scaled(void *handle, float lr, float mu, int nesterov, const float *factor)
+{
     DOPT_REQUIRE(handle != nullptr, "dopt_hip_sgd_step: handle is null");
     Handle *h = (Handle *)handle;
     Scalars s{};
     s.lr = lr;
     s.mu = mu;
-    return nesterov ? launch<kSgdNesterov>(h, s) : launch<kSgd>(h, s);
+    return nesterov ? launch<kSgdNesterov>(h, s, factor) : launch<kSgd>(h, s, factor);
 }
 
 int dopt_hip_adam_step(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2)
+{
+    return dopt_hip_adam_step_scaled(handle, alpha, beta1, beta2, eps, b1, b2, nullptr);
+}
+
+int dopt_hip_adam_step_scaled(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2, const float *factor)
 {
     DOPT_REQUIRE(handle && b1 && b2, "dopt_hip_adam_step: null argument");
     Handle *h = (Handle *)handle;
     DOPT_REQUIRE(h->has_v, "dopt_hip_adam_step: every tensor needs a second-moment buffer v");
     Scalars s{};
     adam_scalars(alpha, beta1, beta2, eps, b1, b2, &s);
-    return launch<kAdam>(h, s);
+    return launch<kAdam>(h, s, factor);
 }
 
 int dopt_hip_amsgrad_step(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2)
+{
+    return dopt_hip_amsgrad_step_scaled(handle, alpha, beta1, beta2, eps, b1, b2, nullptr);
+}
+
+int dopt_hip_amsgrad_step_scaled(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2, const float *factor)
 {
     DOPT_REQUIRE(handle && b1 && b2, "dopt_hip_amsgrad_step: null argument");
     Handle *h = (Handle *)handle;
     DOPT_REQUIRE(h->has_v && h->has_vhat, "dopt_hip_amsgrad_step: every tensor needs v and vhat buffers");
     Scalars s{};
     adam_scalars(alpha, beta1, beta2, eps, b1, b2, &s);
-    return launch<kAmsgrad>(h, s);
+    return launch<kAmsgrad>(h, s, factor);
 }
 
 }  // extern "C"

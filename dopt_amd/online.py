@@ -23,6 +23,24 @@ def _newbufs(variables):
     return [v.device_ptr()[0] for v in variables]
 
 
+def clipped(grads, maxNorm):
+    """The gradients times min(1, maxNorm / norm), norm the square root of the sum of all their squares; as they are where maxNorm
+    is None.  A gradient that stands for several parameters counts for each.  No counterpart in the reference."""
+    if maxNorm is not None and not maxNorm >= 0:
+        raise ValueError("The largest norm is %r" % (maxNorm,))
+    if maxNorm is None or np.isinf(maxNorm) or not grads:
+        return list(grads)
+    total = None
+    for g in grads:
+        s = core.sum(g * g)
+        total = s if total is None else total + s
+    norm = sqrt(total)
+    # (one where the norm is in bounds, whatever maxNorm / norm is there)
+    over = core.gt(norm, float32([], [maxNorm]))
+    factor = over * (float32([], [maxNorm]) / core.max(norm, float32([], [np.finfo(np.float32).tiny]))) + (1.0 - over)
+    return [g * factor for g in grads]
+
+
 class _GraphUpdater:
     def __init__(self, outputs, plan_outputs, targets, flags):
         self.outputs = outputs
@@ -40,12 +58,12 @@ class _GraphUpdater:
         self.plan.execute(args, self._rets)
 
 
-def sgd(outputs, wrt, projs=None, learningRate=None, momentumRate=None, nesterov=False, flags=0):
-    """online/sgd.d:28-94."""
+def sgd(outputs, wrt, projs=None, learningRate=None, momentumRate=None, nesterov=False, flags=0, maxNorm=None):
+    """online/sgd.d:28-94.  maxNorm (here and below; no counterpart there): the gradients are clipped to that norm of them all."""
     projs = projs or {}
     learningRate = learningRate if learningRate is not None else float32([], [0.01])
     momentumRate = momentumRate if momentumRate is not None else float32([], [0.0])
-    grads = grad(outputs[0], wrt)
+    grads = clipped(grad(outputs[0], wrt), maxNorm)
     momentum = [float32(g.shape) for g in grads]
     if nesterov:
         new_momentum = [m * momentumRate - learningRate * g for g, m in zip(grads, momentum)]
@@ -61,13 +79,13 @@ def sgd(outputs, wrt, projs=None, learningRate=None, momentumRate=None, nesterov
     return up
 
 
-def _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, with_varhat, flags):
+def _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, with_varhat, flags, maxNorm):
     projs = projs or {}
     alpha = alpha if alpha is not None else float32([], [0.001])
     beta1 = beta1 if beta1 is not None else float32([], [0.9])
     beta2 = beta2 if beta2 is not None else float32([], [0.999])
     eps = eps if eps is not None else float32([], [1e-8])
-    grads = grad(outputs[0], wrt)
+    grads = clipped(grad(outputs[0], wrt), maxNorm)
     means = [float32(w.shape) for w in wrt]
     vars_ = [float32(w.shape) for w in wrt]
     varhats = [float32(w.shape) for w in wrt] if with_varhat else []
@@ -87,14 +105,14 @@ def _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, with_varhat, flag
     return up
 
 
-def adam(outputs, wrt, projs=None, alpha=None, beta1=None, beta2=None, eps=None, flags=0):
+def adam(outputs, wrt, projs=None, alpha=None, beta1=None, beta2=None, eps=None, flags=0, maxNorm=None):
     """online/adam.d:32-93."""
-    return _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, False, flags)
+    return _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, False, flags, maxNorm)
 
 
-def amsgrad(outputs, wrt, projs=None, alpha=None, beta1=None, beta2=None, eps=None, flags=0):
+def amsgrad(outputs, wrt, projs=None, alpha=None, beta1=None, beta2=None, eps=None, flags=0, maxNorm=None):
     """online/amsgrad.d:32-99."""
-    return _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, True, flags)
+    return _adam_graph(outputs, wrt, projs, alpha, beta1, beta2, eps, True, flags, maxNorm)
 
 
 def _is_matrix(w):
@@ -119,11 +137,11 @@ def _wide(w):
 
 
 def muon(outputs, wrt, projs=None, learningRate=0.02, momentumRate=0.95, nesterov=True, decay=0.0, restRate=0.01, iterations=5,
-         flags=0):
+         flags=0, maxNorm=None):
     """Weight matrices move along their momentum's orthogonalised form (see dopt_hip_muon_step), all other parameters as `sgd` moves
     them with restRate and momentumRate.  No counterpart in the reference."""
     projs = projs or {}
-    grads = grad(outputs[0], wrt)
+    grads = clipped(grad(outputs[0], wrt), maxNorm)
     momentum = [float32(g.shape) for g in grads]
     newvals, new_momentum = [], []
     for w, g, m in zip(wrt, grads, momentum):
@@ -150,7 +168,7 @@ class _Placeholder:
 
 
 class _FusedUpdater:
-    def __init__(self, rule, outputs, wrt, projs, hyper, flags):
+    def __init__(self, rule, outputs, wrt, projs, hyper, flags, maxNorm=None):
         projs = projs or {}
         self.rule, self.hyper, self.outputs, self.wrt = rule, hyper, list(outputs), list(wrt)
         grads = grad(outputs[0], wrt)
@@ -195,6 +213,11 @@ class _FusedUpdater:
 
         params = [view(w, w.device_ptr()[0]) for w in wrt]
         gviews = [view(g, self.plan.result_ptr(g)[0]) for g in grads]
+        self.maxNorm, self._factor, self.norm = maxNorm, None, None
+        if maxNorm is not None:
+            self._gradientNorm = ops.GradientNorm(gviews)
+            self.norm = ops.Tensor((2,))   # of the last step's gradients; what they were multiplied by
+            self._factor = self.norm.view(1, (1,))
         self.state = {"m": [ops.Tensor(w.shape) for w in wrt]}
         if rule in ("adam", "amsgrad"):
             self.state["v"] = [ops.Tensor(w.shape) for w in wrt]
@@ -216,16 +239,18 @@ class _FusedUpdater:
         # The plan reads the OLD parameters; the fused kernel then updates them in place; projected
         # parameters were written by the plan's return copies (they are skipped by the kernel).
         self.plan.execute(args, self._rets)
-        h = self.hyper
+        h, f = self.hyper, self._factor
+        if f is not None:
+            self._gradientNorm.norm(self.maxNorm, out=self.norm)
         if self.rule == "sgd":
-            self.opt.sgd(h["lr"], h["mu"], h["nesterov"])
+            self.opt.sgd(h["lr"], h["mu"], h["nesterov"], f)
         elif self.rule == "adam":
-            self.opt.adam(h["alpha"], h["beta1"], h["beta2"], h["eps"])
+            self.opt.adam(h["alpha"], h["beta1"], h["beta2"], h["eps"], f)
         elif self.rule == "muon":
-            self.muon.step(h["lr"], h["mu"], h["nesterov"], h["decay"], h["iterations"])
-            self.opt.sgd(h["rest"], h["mu"], False)
+            self.muon.step(h["lr"], h["mu"], h["nesterov"], h["decay"], h["iterations"], f)
+            self.opt.sgd(h["rest"], h["mu"], False, f)
         else:
-            self.opt.amsgrad(h["alpha"], h["beta1"], h["beta2"], h["eps"])
+            self.opt.amsgrad(h["alpha"], h["beta1"], h["beta2"], h["eps"], f)
         if self._post_plan is not None:
             self._post_plan.execute(None, self._post_rets)
 
@@ -234,25 +259,25 @@ class _FusedUpdater:
         return [t.numpy() for t in self._out_bufs]
 
 
-def fused_sgd(outputs, wrt, projs=None, learningRate=0.01, momentumRate=0.0, nesterov=False, flags=0):
+def fused_sgd(outputs, wrt, projs=None, learningRate=0.01, momentumRate=0.0, nesterov=False, flags=0, maxNorm=None):
     return _FusedUpdater("sgd", outputs, wrt, projs,
-                         {"lr": float(learningRate), "mu": float(momentumRate), "nesterov": bool(nesterov)}, flags)
+                         {"lr": float(learningRate), "mu": float(momentumRate), "nesterov": bool(nesterov)}, flags, maxNorm)
 
 
-def fused_adam(outputs, wrt, projs=None, alpha=0.001, beta1=0.9, beta2=0.999, eps=1e-8, flags=0):
+def fused_adam(outputs, wrt, projs=None, alpha=0.001, beta1=0.9, beta2=0.999, eps=1e-8, flags=0, maxNorm=None):
     return _FusedUpdater("adam", outputs, wrt, projs,
                          {"alpha": float(alpha), "beta1": float(beta1), "beta2": float(beta2), "eps": float(eps)},
-                         flags)
+                         flags, maxNorm)
 
 
-def fused_amsgrad(outputs, wrt, projs=None, alpha=0.001, beta1=0.9, beta2=0.999, eps=1e-8, flags=0):
+def fused_amsgrad(outputs, wrt, projs=None, alpha=0.001, beta1=0.9, beta2=0.999, eps=1e-8, flags=0, maxNorm=None):
     return _FusedUpdater("amsgrad", outputs, wrt, projs,
                          {"alpha": float(alpha), "beta1": float(beta1), "beta2": float(beta2), "eps": float(eps)},
-                         flags)
+                         flags, maxNorm)
 
 
 def fused_muon(outputs, wrt, projs=None, learningRate=0.02, momentumRate=0.95, nesterov=True, decay=0.0, restRate=0.01, iterations=5,
-               flags=0):
+               flags=0, maxNorm=None):
     return _FusedUpdater("muon", outputs, wrt, projs,
                          {"lr": float(learningRate), "mu": float(momentumRate), "nesterov": bool(nesterov), "decay": float(decay),
-                          "rest": float(restRate), "iterations": int(iterations)}, flags)
+                          "rest": float(restRate), "iterations": int(iterations)}, flags, maxNorm)

@@ -522,8 +522,8 @@ class MuonOptimizer:
         _run(capi.load().dopt_hip_muon_create(n, refs, C.byref(h)))
         self._h = h
 
-    def step(self, lr=0.02, mu=0.95, nesterov=True, decay=0.0, iterations=5):
-        _run(capi.load().dopt_hip_muon_step(self._h, lr, mu, int(nesterov), decay, iterations))
+    def step(self, lr=0.02, mu=0.95, nesterov=True, decay=0.0, iterations=5, factor=None):
+        _run(capi.load().dopt_hip_muon_step_scaled(self._h, lr, mu, int(nesterov), decay, iterations, _factor(factor)))
 
     def close(self):
         if self._h:
@@ -538,8 +538,60 @@ class MuonOptimizer:
 
 
 
+def _factor(t):
+    """The address of what an update multiplies its gradients by: one value on the device, or none."""
+    if t is None:
+        return None
+    if t.size != 1 or t.dtype != _F32:
+        raise capi.HipError(1, "a step's factor is one float32 value")
+    return t.ptr
+
+
+class GradientNorm:
+    """The norm of a fixed set of gradients, and clipping (see dopt_hip_gradient_norm): `outs` says where the clipped ones go, the
+    gradients themselves for clipping in place.  Both calls give {norm, factor}, two values on the device; a step of an optimizer
+    takes the second one (`.view(1, (1,))`) and reads the gradients as if they were clipped."""
+
+    def __init__(self, grads, outs=None):
+        n = len(grads)
+        if outs is not None and len(outs) != n:
+            raise capi.HipError(1, "GradientNorm: a result for every gradient")
+        refs = (capi.GradientRef * max(n, 1))()
+        for i, g in enumerate(grads):
+            if g.dtype != _F32 or (outs is not None and (outs[i].dtype != _F32 or outs[i].size != g.size)):
+                raise capi.HipError(1, "GradientNorm: gradient %d or its result has the wrong size or type" % i)
+            refs[i] = capi.GradientRef(g.ptr, outs[i].ptr if outs is not None else None, g.size)
+        self._keep = (grads, outs)
+        self._h = None
+        h = C.c_void_p()
+        _run(capi.load().dopt_hip_gradient_norm_create(n, refs, C.byref(h)))
+        self._h = h
+
+    def norm(self, max_norm=float("inf"), out=None):
+        out = _out(out, (2,))
+        _run(capi.load().dopt_hip_gradient_norm(self._h, max_norm, out.ptr))
+        return out
+
+    def clip(self, max_norm, out=None):
+        out = _out(out, (2,))
+        _run(capi.load().dopt_hip_gradient_clip(self._h, max_norm, out.ptr))
+        return out
+
+    def close(self):
+        if self._h:
+            capi.load().dopt_hip_gradient_norm_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class FusedOptimizer:
-    """Multi-tensor in-place updater over fixed parameter / gradient / state tensors."""
+    """Multi-tensor in-place updater over fixed parameter / gradient / state tensors.  `factor` of a step: one value on the device
+    that the gradients are multiplied by."""
 
     def __init__(self, params, grads, m, v=None, vhat=None, skip=None):
         n = len(params)
@@ -555,16 +607,16 @@ class FusedOptimizer:
         self.b1 = C.c_float(1.0)   # online/adam.d:44-45: b1, b2 start at 1
         self.b2 = C.c_float(1.0)
 
-    def sgd(self, lr=0.01, mu=0.0, nesterov=False):
-        _run(capi.load().dopt_hip_sgd_step(self._h, lr, mu, int(nesterov)))
+    def sgd(self, lr=0.01, mu=0.0, nesterov=False, factor=None):
+        _run(capi.load().dopt_hip_sgd_step_scaled(self._h, lr, mu, int(nesterov), _factor(factor)))
 
-    def adam(self, alpha=1e-3, beta1=0.9, beta2=0.999, eps=1e-8):
-        _run(capi.load().dopt_hip_adam_step(self._h, alpha, beta1, beta2, eps, C.byref(self.b1),
-                                                  C.byref(self.b2)))
+    def adam(self, alpha=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, factor=None):
+        _run(capi.load().dopt_hip_adam_step_scaled(self._h, alpha, beta1, beta2, eps, C.byref(self.b1), C.byref(self.b2),
+                                                   _factor(factor)))
 
-    def amsgrad(self, alpha=1e-3, beta1=0.9, beta2=0.999, eps=1e-8):
-        _run(capi.load().dopt_hip_amsgrad_step(self._h, alpha, beta1, beta2, eps, C.byref(self.b1),
-                                                     C.byref(self.b2)))
+    def amsgrad(self, alpha=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, factor=None):
+        _run(capi.load().dopt_hip_amsgrad_step_scaled(self._h, alpha, beta1, beta2, eps, C.byref(self.b1), C.byref(self.b2),
+                                                      _factor(factor)))
 
     def close(self):
         if self._h:

@@ -15,6 +15,8 @@
     nnet/lipschitz.d) runs as a second small plan after the kernel; one that also reads this batch's activations (the
     max-gain projections) can only be ordered correctly inside a single plan, so use $(D dopt.online) for those.
 
+    All of them clip the gradients to the norm $(D maxNorm) of them all, if that is finite; $(D dopt.online) has nothing of the kind.
+
     Written where no D compiler exists: never compiled.
 */
 module dopt.hip.online;
@@ -38,9 +40,10 @@ private enum Rule
 
 private class FusedUpdater
 {
-    this(Rule rule, Operation[] outputs, Operation[] wrt, Projection[Operation] projs)
+    this(Rule rule, Operation[] outputs, Operation[] wrt, Projection[Operation] projs, float maxNorm)
     {
         mRule = rule;
+        mMaxNorm = maxNorm;
         mOutputs = outputs.dup;
 
         auto grads = grad(outputs[0], wrt);
@@ -100,6 +103,7 @@ private class FusedUpdater
 
         dopt_hip_tensor_ref[] refs;
         dopt_hip_matrix_ref[] matrices;
+        dopt_hip_gradient_ref[] gradients;
 
         foreach(i, w; wrt)
         {
@@ -110,6 +114,7 @@ private class FusedUpdater
             r.w = cast(float *)wbuf.ptr;
             r.g = cast(const(float) *)mPlan.result(grads[i]).ptr;
             r.n = w.volume;
+            gradients ~= dopt_hip_gradient_ref(r.g, null, r.n);
             r.skip_w = skip[i] ? 1 : 0;
 
             auto bytes = w.volume * float.sizeof;
@@ -143,6 +148,12 @@ private class FusedUpdater
         {
             hipCheck(dopt_hip_muon_create(cast(int)matrices.length, matrices.ptr, &mMuon));
         }
+
+        if(maxNorm < float.infinity)
+        {
+            hipCheck(dopt_hip_gradient_norm_create(cast(int)gradients.length, gradients.ptr, &mNorm));
+            mNormResult = HIPBuffer.create(2 * float.sizeof);
+        }
     }
 
     ~this()
@@ -156,6 +167,11 @@ private class FusedUpdater
         {
             dopt_hip_muon_destroy(mMuon);
         }
+
+        if(mNorm !is null)
+        {
+            dopt_hip_gradient_norm_destroy(mNorm);
+        }
     }
 
     DeviceBuffer[] update(DeviceBuffer[Operation] args)
@@ -163,6 +179,25 @@ private class FusedUpdater
         //The plan reads the OLD parameters; the kernel then updates them in place
         mPlan.execute(args, mRets);
 
+        if(mNorm is null)
+        {
+            step();
+        }
+        else
+        {
+            clippedStep();
+        }
+
+        if(mPostPlan !is null)
+        {
+            mPostPlan.execute(null, mPostRets);
+        }
+
+        return mRets[0 .. mOutputs.length];
+    }
+
+    void step()
+    {
         final switch(mRule)
         {
             case Rule.sgd:
@@ -185,13 +220,37 @@ private class FusedUpdater
                 hipCheck(dopt_hip_sgd_step(mHandle, scalar(mHyper[3]), scalar(mHyper[1]), 0));
                 break;
         }
+    }
 
-        if(mPostPlan !is null)
+    //The kernels multiply the gradients by the second value of { norm, factor } as they read them
+    void clippedStep()
+    {
+        auto result = cast(float *)mNormResult.ptr;
+        auto factor = cast(const(float) *)(result + 1);
+        hipCheck(dopt_hip_gradient_norm(mNorm, mMaxNorm, result));
+
+        final switch(mRule)
         {
-            mPostPlan.execute(null, mPostRets);
-        }
+            case Rule.sgd:
+                hipCheck(dopt_hip_sgd_step_scaled(mHandle, scalar(mHyper[0]), scalar(mHyper[1]), mNesterov ? 1 : 0, factor));
+                break;
 
-        return mRets[0 .. mOutputs.length];
+            case Rule.adam:
+                hipCheck(dopt_hip_adam_step_scaled(mHandle, scalar(mHyper[0]), scalar(mHyper[1]), scalar(mHyper[2]),
+                    scalar(mHyper[3]), &mB1, &mB2, factor));
+                break;
+
+            case Rule.amsgrad:
+                hipCheck(dopt_hip_amsgrad_step_scaled(mHandle, scalar(mHyper[0]), scalar(mHyper[1]), scalar(mHyper[2]),
+                    scalar(mHyper[3]), &mB1, &mB2, factor));
+                break;
+
+            case Rule.muon:
+                hipCheck(dopt_hip_muon_step_scaled(mMuon, scalar(mHyper[0]), scalar(mHyper[1]), mNesterov ? 1 : 0,
+                    scalar(mHyper[2]), mIterations, factor));
+                hipCheck(dopt_hip_sgd_step_scaled(mHandle, scalar(mHyper[3]), scalar(mHyper[1]), 0, factor));
+                break;
+        }
     }
 
     //Hyper-parameters are scalar Operations, as in dopt.online: their current value is read at every step
@@ -209,16 +268,19 @@ private class FusedUpdater
     HIPPlan mPlan, mPostPlan;
     DeviceBuffer[] mRets, mPostRets;
     HIPBuffer[] mState;
-    void *mHandle, mMuon;
+    float mMaxNorm;
+    HIPBuffer mNormResult;
+    void *mHandle, mMuon, mNorm;
 }
 
 /**
     Stochastic gradient descent with momentum; see $(D dopt.online.sgd) (online/sgd.d:28-94) for the parameters.
 */
 Updater sgd(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
-    Operation learningRate = float32([], [0.01f]), Operation momentumRate = float32([], [0.0f]), bool nesterov = false)
+    Operation learningRate = float32([], [0.01f]), Operation momentumRate = float32([], [0.0f]), bool nesterov = false,
+    float maxNorm = float.infinity)
 {
-    auto u = new FusedUpdater(Rule.sgd, outputs, wrt, projs);
+    auto u = new FusedUpdater(Rule.sgd, outputs, wrt, projs, maxNorm);
     u.mHyper = [learningRate, momentumRate];
     u.mNesterov = nesterov;
 
@@ -230,9 +292,9 @@ Updater sgd(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
 */
 Updater adam(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
     Operation alpha = float32([], [0.001f]), Operation beta1 = float32([], [0.9f]),
-    Operation beta2 = float32([], [0.999f]), Operation eps = float32([], [1e-8]))
+    Operation beta2 = float32([], [0.999f]), Operation eps = float32([], [1e-8]), float maxNorm = float.infinity)
 {
-    auto u = new FusedUpdater(Rule.adam, outputs, wrt, projs);
+    auto u = new FusedUpdater(Rule.adam, outputs, wrt, projs, maxNorm);
     u.mHyper = [alpha, beta1, beta2, eps];
 
     return &u.update;
@@ -244,9 +306,9 @@ Updater adam(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
 */
 Updater amsgrad(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
     Operation alpha = float32([], [0.001f]), Operation beta1 = float32([], [0.9f]),
-    Operation beta2 = float32([], [0.999f]), Operation eps = float32([], [1e-8]))
+    Operation beta2 = float32([], [0.999f]), Operation eps = float32([], [1e-8]), float maxNorm = float.infinity)
 {
-    auto u = new FusedUpdater(Rule.amsgrad, outputs, wrt, projs);
+    auto u = new FusedUpdater(Rule.amsgrad, outputs, wrt, projs, maxNorm);
     u.mHyper = [alpha, beta1, beta2, eps];
 
     return &u.update;
@@ -262,7 +324,14 @@ Updater muon(Operation[] outputs, Operation[] wrt, Projection[Operation] projs,
     Operation decay = float32([], [0.0f]), Operation restRate = float32([], [0.01f]),
     int iterations = 5)
 {
-    auto u = new FusedUpdater(Rule.muon, outputs, wrt, projs);
+    return muon(outputs, wrt, projs, learningRate, momentumRate, nesterov, decay, restRate, iterations, float.infinity);
+}
+
+///ditto
+Updater muon(Operation[] outputs, Operation[] wrt, Projection[Operation] projs, Operation learningRate,
+    Operation momentumRate, bool nesterov, Operation decay, Operation restRate, int iterations, float maxNorm)
+{
+    auto u = new FusedUpdater(Rule.muon, outputs, wrt, projs, maxNorm);
     u.mHyper = [learningRate, momentumRate, decay, restRate];
     u.mNesterov = nesterov;
     u.mIterations = iterations;

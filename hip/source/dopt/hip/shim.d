@@ -120,6 +120,13 @@ struct dopt_hip_matrix_ref
     size_t cols;
 }
 
+struct dopt_hip_gradient_ref
+{
+    const(float)* g;
+    float* out_;
+    size_t n;
+}
+
 int dopt_hip_init(int device);
 int dopt_hip_shutdown();
 const(char)* dopt_hip_last_error();
@@ -213,9 +220,17 @@ int dopt_hip_optim_destroy(void* handle);
 int dopt_hip_sgd_step(void* handle, float lr, float mu, int nesterov);
 int dopt_hip_adam_step(void* handle, float alpha, float beta1, float beta2, float eps, float* b1, float* b2);
 int dopt_hip_amsgrad_step(void* handle, float alpha, float beta1, float beta2, float eps, float* b1, float* b2);
+int dopt_hip_sgd_step_scaled(void* handle, float lr, float mu, int nesterov, const(float)* factor);
+int dopt_hip_adam_step_scaled(void* handle, float alpha, float beta1, float beta2, float eps, float* b1, float* b2, const(float)* factor);
+int dopt_hip_amsgrad_step_scaled(void* handle, float alpha, float beta1, float beta2, float eps, float* b1, float* b2, const(float)* factor);
 int dopt_hip_muon_create(int nmatrices, const(dopt_hip_matrix_ref)* refs, void** handle);
 int dopt_hip_muon_destroy(void* handle);
 int dopt_hip_muon_step(void* handle, float lr, float mu, int nesterov, float decay, int iterations);
+int dopt_hip_muon_step_scaled(void* handle, float lr, float mu, int nesterov, float decay, int iterations, const(float)* factor);
+int dopt_hip_gradient_norm_create(int ntensors, const(dopt_hip_gradient_ref)* refs, void** handle);
+int dopt_hip_gradient_norm_destroy(void* handle);
+int dopt_hip_gradient_norm(void* handle, float max_norm, float* result);
+int dopt_hip_gradient_clip(void* handle, float max_norm, float* result);
 
 // ---- include/dopt_hip_plan.h
 enum

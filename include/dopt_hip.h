@@ -582,6 +582,13 @@ int dopt_hip_adam_step(void *handle, float alpha, float beta1, float beta2, floa
 /* online/amsgrad.d:52-69: ADAM's m', v', w' (w' uses v', as the reference does) plus
    vhat' = max(vhat, OLD v). */
 int dopt_hip_amsgrad_step(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2);
+/* The same with every gradient multiplied by *factor (device), rounded, before the rule sees it: clipping, see
+   dopt_hip_gradient_norm, without a pass over the gradients.  A null factor is one. */
+int dopt_hip_sgd_step_scaled(void *handle, float lr, float mu, int nesterov, const float *factor);
+int dopt_hip_adam_step_scaled(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2,
+                              const float *factor);
+int dopt_hip_amsgrad_step_scaled(void *handle, float alpha, float beta1, float beta2, float eps, float *b1, float *b2,
+                                 const float *factor);
 
 /* A weight as a matrix [rows, cols] (a filter [K,C,R,S] is [K, C*R*S]). */
 typedef struct {
@@ -601,6 +608,28 @@ typedef struct {
 int dopt_hip_muon_create(int nmatrices, const dopt_hip_matrix_ref *refs, void **handle);
 int dopt_hip_muon_destroy(void *handle);
 int dopt_hip_muon_step(void *handle, float lr, float mu, int nesterov, float decay, int iterations);
+/* ... with every gradient multiplied by *factor, as dopt_hip_sgd_step_scaled. */
+int dopt_hip_muon_step_scaled(void *handle, float lr, float mu, int nesterov, float decay, int iterations,
+                              const float *factor);
+
+/* The norm of all gradients of a step, and clipping.  No counterpart in the reference. */
+typedef struct {
+    const float *g;  /* gradient */
+    float *out;      /* the clipped gradient: g itself, memory of its own, or null where dopt_hip_gradient_clip is not called */
+    size_t n;        /* element count */
+} dopt_hip_gradient_ref;
+
+/* Keeps the addresses of a fixed set of gradients; reuse it every step.  A gradient may be listed twice (and counts twice); no
+   result may overlap another one, or a gradient other than its own. */
+int dopt_hip_gradient_norm_create(int ntensors, const dopt_hip_gradient_ref *refs, void **handle);
+int dopt_hip_gradient_norm_destroy(void *handle);
+/* result (device, two floats) = { norm, factor }: the square root of the sum of all gradients' squares, formed in 64 bits, and
+   norm <= max_norm ? 1 : max_norm / norm (NaN for a norm that is NaN, zero where a gradient is infinite).  The factor is formed from
+   the norm in 64 bits, also where that is beyond a float's range and written as infinity.  max_norm is zero or more; infinity clips
+   nothing.  result may lie in no tensor of the set. */
+int dopt_hip_gradient_norm(void *handle, float max_norm, float *result);
+/* ... and out = factor * g for every tensor of the set. */
+int dopt_hip_gradient_clip(void *handle, float max_norm, float *result);
 
 #ifdef __cplusplus
 }
