@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(HERE, "libdopthip.so")
 
 F32, I32 = 0, 1
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # dopt_hip_activation
+ROW_NORMS = {"none": 0, "layer": 1, "rms": 2}                # dopt_hip_row_norm
 
 
 class HipError(RuntimeError):
@@ -46,6 +47,12 @@ class TensorRef(C.Structure):
 class MatrixRef(C.Structure):
     """dopt_hip_matrix_ref: a weight as a matrix, with its gradient and momentum."""
     _fields_ = [("w", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("rows", C.c_size_t), ("cols", C.c_size_t)]
+
+
+class ResidualNormDesc(C.Structure):
+    """dopt_hip_residual_norm_desc: rows, gates, the norms of the branch and of the sum."""
+    _fields_ = [("rows", C.c_size_t), ("cols", C.c_size_t), ("gates", C.c_size_t), ("post", C.c_int), ("pre", C.c_int),
+                ("eps", C.c_float), ("residual_scale", C.c_float)]
 
 
 class GradientRef(C.Structure):
@@ -143,6 +150,8 @@ PROTOTYPES = {
     "dopt_hip_bn_infer": [_sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp],
     "dopt_hip_group_norm": [_sz, _sz, _sz, _sz, _i, _f, _i, _vp, _vp, _vp, _vp],
     "dopt_hip_group_norm_grad": [_sz, _sz, _sz, _sz, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "dopt_hip_residual_norm": [C.POINTER(ResidualNormDesc)] + [_vp] * 10,
+    "dopt_hip_residual_norm_grad": [C.POINTER(ResidualNormDesc)] + [_vp] * 16,
     "dopt_hip_dense_act": [_sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     "dopt_hip_dense_act_grad": [_sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "dopt_hip_muon_create": [_i, C.POINTER(MatrixRef), C.POINTER(_vp)],

@@ -17,6 +17,7 @@ import numpy as np
 from . import capi
 
 _bmax = builtins.max   # several reference op names (max, min, sum, abs, pow, slice) shadow builtins below
+_bsum = builtins.sum
 float32_t = np.dtype(np.float32)
 int32_t = np.dtype(np.int32)
 _CODE = {float32_t: capi.F32, int32_t: capi.I32}
@@ -629,6 +630,115 @@ def denseActGrad(parentGrad, op):
     return Operation("denseActGrad", [parentGrad] + deps, {"activation": a["activation"]})
 
 
+# What lies between two blocks of a residual network; "operands" has a bit for each optional one, in this order.
+_JOIN_OPERANDS = ("stream", "branch", "gate", "postScale", "postBias", "preScale", "preBias")
+_JOIN_STATS = (0, 2, 1)   # values of a row by its norm
+
+
+def _join_parts(op, first):
+    """{name: dependency} from the `first` one on; None where their number is not that of the bits."""
+    names = [n for i, n in enumerate(_JOIN_OPERANDS) if op.attributes["operands"] >> i & 1]
+    return dict(zip(names, op.deps[first:])) if len(names) == len(op.deps) - first else None
+
+
+def _verify_join(op):
+    a, parts = op.attributes, _join_parts(op, 0)
+    if parts is None or not ("stream" in parts or "branch" in parts):
+        return False
+    like = op.deps[0]
+    if like.rank < 1 or like.volume == 0 or not {a["post"], a["pre"]} <= set(capi.ROW_NORMS.values()):
+        return False
+    cols = like.shape[-1]
+    rows = like.volume // cols
+    for name, d in parts.items():
+        if d.dtype != float32_t:
+            return False
+        if name in ("stream", "branch"):
+            ok = d.shape == like.shape
+        elif name == "gate":
+            ok = "branch" in parts and d.volume > 0 and d.volume % cols == 0 and rows % (d.volume // cols) == 0
+        else:
+            ok = d.volume == cols and a["post" if name.startswith("post") else "pre"] != 0
+        if not ok:
+            return False
+    return a["post"] == 0 or "branch" in parts
+
+
+def _judge_join(op):
+    v, cols, a = op.deps[0].volume, op.deps[0].shape[-1], op.attributes
+    return float32_t, (v * (2 if a["pre"] else 1) + v // cols * (_JOIN_STATS[a["post"]] + _JOIN_STATS[a["pre"]]),)
+
+
+def _judge_join_grad(op):
+    a, cols = op.attributes, op.attributes["columns"]
+    v, sizes = a["rows"] * cols, {"gate": a["gates"] * cols}
+    names = [n for i, n in enumerate(_JOIN_OPERANDS) if a["operands"] >> i & 1]
+    return float32_t, (_bsum(v if n in ("stream", "branch") else sizes.get(n, cols) for n in names),)
+
+
+register_operation("residualNorm", _verify_join, _judge_join)
+register_operation("residualNormGrad", lambda op: all(d.dtype == float32_t for d in op.deps), _judge_join_grad)
+
+
+def _row_norm(name):
+    if name not in capi.ROW_NORMS:
+        raise ValueError("There is no norm %r: %s" % (name, ", ".join(capi.ROW_NORMS)))
+    return capi.ROW_NORMS[name]
+
+
+def residualNorm(stream=None, branch=None, gate=None, post="none", postScale=None, postBias=None, pre="none", preScale=None,
+                 preBias=None, residualScale=1.0, epsilon=1e-5):
+    """[y, h]: y = residualScale stream + gate (post(branch) postScale + postBias) and h = pre(y) preScale + preBias, norms over the
+    last dimension ("none", "layer", "rms"); h is None where there is no norm of y.  A gate has rows for one sample, all rows, or each.
+    Gradients flow through y and h."""
+    parts = (stream, branch, gate, postScale, postBias, preScale, preBias)
+    if stream is None and branch is None:
+        raise ValueError("residualNorm needs a stream or a branch")
+    op = Operation("residualNorm", [p for p in parts if p is not None],
+                   {"operands": _bsum(1 << i for i, p in enumerate(parts) if p is not None), "post": _row_norm(post), "pre": _row_norm(pre),
+                    "residualScale": float(residualScale), "epsilon": float(epsilon)})
+    like = op.deps[0]
+    v = like.volume
+    return [slice(op, [0], [v]).reshape(like.shape), slice(op, [v], [2 * v]).reshape(like.shape) if op.attributes["pre"] else None]
+
+
+def _gradient_of(pg, start, stop):
+    """The part [start, stop) of a packed result's gradient, or None where it is zero: the sum of what its readers gave, without the
+    zeros that each of them was padded with."""
+    if pg.opType == "add":
+        found = [g for g in (_gradient_of(d, start, stop) for d in pg.deps) if g is not None]
+        return found[0] + found[1] if len(found) == 2 else found[0] if found else None
+    if pg.opType == "pad":
+        begin = pg.attributes["before"][0]
+        end = begin + pg.deps[0].volume
+        if end <= start or begin >= stop:
+            return None
+        if begin == start and end == stop:
+            return pg.deps[0]
+    return slice(pg, [start], [stop])
+
+
+def residualNormGrad(parentGrad, op):
+    """The packed gradients of op's operands, in their order."""
+    a, parts, like = op.attributes, _join_parts(op, 0), op.deps[0]
+    v, cols = like.volume, like.shape[-1]
+    dy = _gradient_of(parentGrad, 0, v)
+    dh = _gradient_of(parentGrad, v, 2 * v) if a["pre"] else None
+    if a["pre"] and dh is None:   # nobody reads h, but its norm's scale and bias are parameters
+        dh = float32([v])
+    if dy is None and dh is None:
+        dy = float32([v])
+    deps = [d for d in (dy, dh) if d is not None]
+    if a["pre"]:
+        deps.append(slice(op, [0], [v]))
+    deps += [parts[n] for n in _JOIN_OPERANDS[1:6] if n in parts]
+    if a["post"] or a["pre"]:
+        deps.append(slice(op, [v * (2 if a["pre"] else 1)], [op.volume]))
+    return Operation("residualNormGrad", deps, {"operands": a["operands"], "post": a["post"], "pre": a["pre"],
+                                                "residualScale": a["residualScale"], "hasDy": int(dy is not None), "rows": v // cols,
+                                                "columns": cols, "gates": parts["gate"].volume // cols if "gate" in parts else 0})
+
+
 def convolution(features, filters, padding=(0, 0), stride=(1, 1)):
     return Operation("convolution", [features, filters], {"padding": list(padding), "stride": list(stride)})
 
@@ -784,6 +894,7 @@ def _reg_grads():
         out = parts(denseActGrad(dy, op), op.deps[:2 + op.attributes["hasBias"]])
         return out + ([dy.reshape(op.deps[-1].shape)] if op.attributes["hasResidual"] else [])
     g("denseAct", dense_act_grad)
+    g("residualNorm", lambda op, pg: parts(residualNormGrad(pg, op), op.deps))
 
 
 _reg_grads()

@@ -172,6 +172,31 @@ bool norm_attrs(const Operation &op, const std::vector<size_t> &x, NormAttrs *a)
     return true;
 }
 
+// The optional operands of a residualNorm, by the bits of its attribute, and the descriptor (but for the rows).
+enum JoinOperand { kStream, kBranch, kGate, kPostScale, kPostBias, kPreScale, kPreBias, kJoinOperands };
+struct JoinAttrs {
+    dopt_hip_residual_norm_desc d{};
+    size_t operands;
+    bool has(int i) const { return operands >> i & 1; }
+    size_t stats() const { return ((d.post == DOPT_HIP_NORM_LAYER) + (d.post != 0) + (d.pre == DOPT_HIP_NORM_LAYER) + (d.pre != 0)) * d.rows; }
+    // values of an operand (and of its gradient)
+    size_t volume(int i) const { return i <= kBranch ? d.rows * d.cols : i == kGate ? d.gates * d.cols : d.cols; }
+};
+bool join_attrs(const Operation &op, JoinAttrs *a)
+{
+    size_t post, pre;
+    if (!size_attr(op, "operands", &a->operands) || !size_attr(op, "post", &post) || !size_attr(op, "pre", &pre)) return false;
+    auto it = op.doubleAttrs.find("residualScale");
+    if (it == op.doubleAttrs.end() || a->operands >> kJoinOperands) {
+        fail(DOPT_HIP_ERR_INVALID, "operation '%s' has no attribute 'residualScale', or more operands than there are", op.opType.c_str());
+        return false;
+    }
+    a->d.post = (int)post;
+    a->d.pre = (int)pre;
+    a->d.residual_scale = (float)it->second;
+    return true;
+}
+
 dopt_hip_conv_desc conv_desc(const std::vector<size_t> &x, const std::vector<size_t> &w, const std::vector<size_t> &pad,
                              const std::vector<size_t> &stride)
 {
@@ -490,6 +515,71 @@ void registerBuiltinsOnce()
         return make([=](const std::vector<const void *> &in, void *out) {
             return dopt_hip_group_norm_grad(a.N, a.C, a.inner, a.groups, a.last, a.act, (const float *)in[0], (const float *)in[1],
                                             (const float *)in[2], (const float *)in[3], (const float *)in[4], (float *)out);
+        });
+    };
+    R["residualNorm"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps: the operands that there are; output [y | h | stats]
+        JoinAttrs a;
+        if (!need_f32(op) || !join_attrs(op, &a) || !need_deps(op, (size_t)__builtin_popcountll(a.operands))) return nullptr;
+        auto it = op.doubleAttrs.find("epsilon");
+        if (it == op.doubleAttrs.end() || op.deps.empty() || g.ops[op.deps[0]].shape.empty() || g.ops[op.deps[0]].volume() == 0 ||
+            !(a.has(kStream) || a.has(kBranch))) {
+            fail(DOPT_HIP_ERR_INVALID, "residualNorm: no 'epsilon' attribute, or neither a stream nor a branch of at least one value");
+            return nullptr;
+        }
+        a.d.eps = (float)it->second;
+        const auto &like = g.ops[op.deps[0]].shape;
+        a.d.cols = like.back();
+        a.d.rows = g.ops[op.deps[0]].volume() / a.d.cols;
+        std::vector<size_t> volumes;
+        for (int i = 0; i < kJoinOperands; i++) {
+            if (!a.has(i)) continue;
+            if (i == kGate) a.d.gates = g.ops[op.deps[volumes.size()]].volume() / a.d.cols;
+            volumes.push_back(a.volume(i));
+        }
+        const size_t v = a.d.rows * a.d.cols;
+        if (!has_volumes(g, op, volumes, v * (a.d.pre ? 2 : 1) + a.stats())) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            const float *o[kJoinOperands] = {};
+            for (int i = 0, k = 0; i < kJoinOperands; i++)
+                if (a.has(i)) o[i] = (const float *)in[k++];
+            float *const y = (float *)out, *const h = a.d.pre ? y + v : nullptr;
+            return dopt_hip_residual_norm(&a.d, o[kStream], o[kBranch], o[kGate], o[kPostScale], o[kPostBias], o[kPreScale], o[kPreBias], y, h,
+                                          a.stats() ? y + v * (a.d.pre ? 2 : 1) : nullptr);
+        });
+    };
+    R["residualNormGrad"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps [dy] [dh, y], branch to preScale as there are, [stats]; output the operands' gradients in their order
+        JoinAttrs a;
+        size_t has_dy;
+        if (!need_f32(op) || !join_attrs(op, &a) || !size_attr(op, "hasDy", &has_dy) || !size_attr(op, "rows", &a.d.rows) ||
+            !size_attr(op, "columns", &a.d.cols) || !size_attr(op, "gates", &a.d.gates))
+            return nullptr;
+        const size_t v = a.d.rows * a.d.cols;
+        std::vector<size_t> volumes(has_dy ? 1 : 0, v);
+        if (a.d.pre) volumes.insert(volumes.end(), 2, v);
+        for (int i = kBranch; i <= kPreScale; i++)
+            if (a.has(i)) volumes.push_back(a.volume(i));
+        if (a.stats()) volumes.push_back(a.stats());
+        size_t result = 0;
+        for (int i = 0; i < kJoinOperands; i++)
+            if (a.has(i)) result += a.volume(i);
+        if (!need_deps(op, volumes.size()) || !has_volumes(g, op, volumes, result)) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            const float *o[kJoinOperands] = {};
+            size_t k = 0;
+            auto next = [&](bool there) { return there ? (const float *)in[k++] : nullptr; };
+            const float *const dy = next(has_dy), *const dh = next(a.d.pre != 0), *const y = next(a.d.pre != 0);
+            for (int i = kBranch; i <= kPreScale; i++) o[i] = next(a.has(i));
+            const float *const stats = next(a.stats() != 0);
+            float *d[kJoinOperands] = {}, *to = (float *)out;
+            for (int i = 0; i < kJoinOperands; i++)
+                if (a.has(i)) {
+                    d[i] = to;
+                    to += a.volume(i);
+                }
+            return dopt_hip_residual_norm_grad(&a.d, dy, dh, y, o[kBranch], o[kGate], o[kPostScale], o[kPostBias], o[kPreScale], stats, d[kStream],
+                                               d[kBranch], d[kGate], d[kPostScale], d[kPostBias], d[kPreScale], d[kPreBias]);
         });
     };
     R["denseAct"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {

@@ -1,0 +1,817 @@
+// What lies between two blocks of a residual network: the norm behind the one, its gate, the sum with the stream, and the norm before the
+// other, forward and backward, over rows of `cols` values.  No counterpart in the reference, whose only norm is over the batch
+// (cuda/source/dopt/cuda/nnet/cudnn7.d:547-654).
+//
+//     zb = norm(branch),  u = zb ps + pb,  y = s x + gate u,  zy = norm(y),  h = zy qs + qb
+//     norm(v) = (v - mean) rstd with rstd = 1 / sqrt(variance + eps), or v rstd with rstd = 1 / sqrt(mean of v^2 + eps)
+//
+//     e = dh qs,  t = dy + ry (e - mean(e) - zy mean(e zy)),  dx = s t,  dgate = sum over the gate's rows of t u,  du = t gate
+//     f = du ps,  dbranch = rb (f - mean(f) - zb mean(f zb))          (no mean(e), mean(f) where a norm takes no mean out)
+//     dqs = sum of dh zy,  dqb = sum of dh,  dps = sum of du zb,  dpb = sum of du over all rows
+//
+// Bound by memory: 16 bytes a value forward, 24 backward.  A row stays in the registers of the team of lanes that has it: 16, 32 or 64 lanes
+// of a wavefront for up to 1024 values, a workgroup for up to 16384, so everything is read and written once; longer rows are
+// read several times by a workgroup.  Means come before squared differences from them, so nothing cancels.  Backward a team takes a
+// run of rows and adds up the columns in registers; a second launch adds the runs.  No atomics: every sum has one order.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.h"
+
+namespace {
+
+using namespace dopt;
+
+constexpr int kBlock = 256;          // of teams within a wavefront
+constexpr size_t kHeld = 16384;      // values of a row that a workgroup holds at most
+constexpr size_t kRunRows = 128;     // of a run at most: sums of more values that are alike are rounded the same way for long
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));   // sixteen bytes wherever they start
+
+// Between reads and writes of the same LDS by different wavefronts; the empty statement keeps reads in front of it that are used behind
+// it in a branch.
+__device__ __forceinline__ void meet()
+{
+    asm volatile("" ::: "memory");
+    __syncthreads();
+}
+
+template <int kControl>
+__device__ __forceinline__ float plus_moved(float v)
+{
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), kControl, 0xf, 0xf, true));
+}
+
+// The sum over groups of kLanes lanes, in all of them.
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v)
+{
+    v = plus_moved<0xB1>(v);    // the neighbour
+    v = plus_moved<0x4E>(v);    // the other pair
+    v = plus_moved<0x141>(v);   // the other quad: each of its lanes holds its sum by now
+    v = plus_moved<0x140>(v);   // the other eight
+    if (kLanes >= 32) v += __shfl_xor(v, 16, 64);
+    if (kLanes >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+struct Norms {
+    size_t rows;
+    int cols;
+    size_t per_gate;     // consecutive rows with one gate; 0: there is none
+    int post, pre;
+    float eps, scale;
+    const float *x, *branch, *gate, *ps, *pb, *qs, *qb;
+    float *y, *h;
+    float *mb, *rb, *my, *ry;    // the rows' statistics
+};
+struct Grads {
+    Norms n;             // y and branch as the forward pass read and left them; statistics as it left them
+    const float *dy, *dh;
+    float *dx, *db, *dgate;
+    float *sums;         // of each block: kinds x cols, see Kind; then the gate's, cols for each run
+    int kinds;           // a bit for each kind that is wanted
+};
+enum Kind { kPreScale, kPreBias, kPostScale, kPostBias, kKinds };
+
+// Rows in runs: of a gate's rows, `splits` runs for each gate; or of `gates` whole gates each, whose gradients then need no second launch.
+struct Runs {
+    size_t count, rows, per_gate, splits, gates;
+    __device__ __forceinline__ void range(size_t run, size_t &from, size_t &to) const
+    {
+        if (gates) {
+            from = min(rows, run * gates * per_gate);
+            to = min(rows, from + gates * per_gate);
+            return;
+        }
+        const size_t first = run / splits * per_gate, part = run % splits;
+        from = first + per_gate * part / splits;
+        to = first + per_gate * (part + 1) / splits;
+    }
+};
+
+// A row's values of one thread: quad lane + i * lanes of the row; values beyond its end are zero.
+__device__ __forceinline__ v4f load_quad(const float *row, int col, int cols)
+{
+    if (col + 4 <= cols) return *(const v4f_any *)(row + col);
+    v4f v{0.0f, 0.0f, 0.0f, 0.0f};
+    if (col < cols) v.x = row[col];
+    if (col + 1 < cols) v.y = row[col + 1];
+    if (col + 2 < cols) v.z = row[col + 2];
+    return v;
+}
+__device__ __forceinline__ void store_quad(float *row, int col, int cols, v4f v)
+{
+    if (col + 4 <= cols) {
+        *(v4f_any *)(row + col) = v;
+        return;
+    }
+    if (col < cols) row[col] = v.x;
+    if (col + 1 < cols) row[col + 1] = v.y;
+    if (col + 2 < cols) row[col + 2] = v.z;
+}
+__device__ __forceinline__ v4f inside(v4f v, int col, int cols)   // zero beyond the row's end
+{
+    if (col + 4 > cols) {
+        if (col >= cols) v.x = 0.0f;
+        if (col + 1 >= cols) v.y = 0.0f;
+        if (col + 2 >= cols) v.z = 0.0f;
+        v.w = 0.0f;
+    }
+    return v;
+}
+__device__ __forceinline__ float sum4(v4f v) { return (v.x + v.y) + (v.z + v.w); }
+__device__ __forceinline__ v4f splat(float v) { return v4f{v, v, v, v}; }
+
+// The lanes that share a row: kLanes of a wavefront, or (0) the workgroup.
+template <int kLanes>
+struct Team {
+    static constexpr bool kBlockwide = kLanes == 0;
+    float *red;   // of a workgroup: twice 32 values
+    int turn = 0;
+    __device__ __forceinline__ int lane() const { return kBlockwide ? (int)threadIdx.x : (int)threadIdx.x & (kLanes - 1); }
+    __device__ __forceinline__ int lanes() const { return kBlockwide ? (int)blockDim.x : kLanes; }
+    __device__ __forceinline__ void sum(float &a, float &b)   // both over the team, in all of its lanes
+    {
+        a = lanes_sum<kBlockwide ? 64 : kLanes>(a);
+        b = lanes_sum<kBlockwide ? 64 : kLanes>(b);
+        if (!kBlockwide || blockDim.x == 64) return;
+        float *const r = red + turn * 32;   // two places in turn: a barrier apiece is enough
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) {
+            r[threadIdx.x >> 6] = a;
+            r[16 + (threadIdx.x >> 6)] = b;
+        }
+        meet();
+        const int waves = (int)blockDim.x >> 6;
+        a = r[0];
+        b = r[16];
+        for (int i = 1; i < waves; i++) {
+            a += r[i];
+            b += r[16 + i];
+        }
+    }
+    __device__ __forceinline__ float sum(float a)
+    {
+        float none = 0.0f;
+        sum(a, none);
+        return a;
+    }
+};
+
+// A row's mean (where the norm takes it out) and rstd.
+template <int Q, class T>
+__device__ __forceinline__ void row_stats(T &team, const v4f (&v)[Q], int kind, int cols, float eps, float &mean, float &rstd)
+{
+    mean = 0.0f;
+    const float n = (float)cols;
+    if (kind == DOPT_HIP_NORM_LAYER) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Q; i++) s += sum4(v[i]);
+        mean = team.sum(s) / n;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Q; i++) {
+        const v4f d = inside(v[i] - splat(mean), 4 * (team.lane() + i * team.lanes()), cols);
+        q += sum4(d * d);
+    }
+    rstd = 1.0f / sqrtf(team.sum(q) / n + eps);
+}
+
+template <int Q>
+__device__ __forceinline__ void load_row(const float *p, float missing, int lane, int lanes, int cols, v4f (&v)[Q])
+{
+#pragma unroll
+    for (int i = 0; i < Q; i++) v[i] = p ? load_quad(p, 4 * (lane + i * lanes), cols) : splat(missing);
+}
+
+template <int kLanes, int Q>
+__global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
+{
+    __shared__ float red[64];
+    Team<kLanes> team{red};
+    constexpr int kTeams = kLanes ? kBlock / (kLanes ? kLanes : 1) : 1;
+    const int lane = team.lane(), lanes = team.lanes(), cols = n.cols;
+    v4f gate[Q], ps[Q], pb[Q], qs[Q], qb[Q];
+    load_row(n.ps, 1.0f, lane, lanes, cols, ps);
+    load_row(n.pb, 0.0f, lane, lanes, cols, pb);
+    load_row(n.qs, 1.0f, lane, lanes, cols, qs);
+    load_row(n.qb, 0.0f, lane, lanes, cols, qb);
+    const bool one_gate = n.per_gate == 0 || n.per_gate == n.rows;
+    if (one_gate) load_row(n.gate, 1.0f, lane, lanes, cols, gate);
+    const size_t first = (size_t)blockIdx.x * kTeams + (kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0);
+    for (size_t r = first; r < n.rows; r += (size_t)gridDim.x * kTeams) {
+        const size_t at = r * (size_t)cols;
+        v4f x[Q], v[Q];
+        load_row(n.branch ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, v);
+        load_row(n.x ? n.x + at : nullptr, 0.0f, lane, lanes, cols, x);
+        if (!one_gate) load_row(n.gate + r / n.per_gate * (size_t)cols, 1.0f, lane, lanes, cols, gate);
+        if (n.post) {
+            float mean, rstd;
+            row_stats(team, v, n.post, cols, n.eps, mean, rstd);
+            if (lane == 0 && n.rb) {
+                if (n.mb) n.mb[r] = mean;
+                n.rb[r] = rstd;
+            }
+#pragma unroll
+            for (int i = 0; i < Q; i++) v[i] = (v[i] - splat(mean)) * splat(rstd) * ps[i] + pb[i];
+        }
+#pragma unroll
+        for (int i = 0; i < Q; i++) {
+            const int col = 4 * (lane + i * lanes);
+            v[i] = inside(splat(n.scale) * x[i] + gate[i] * v[i], col, cols);
+            if (n.y) store_quad(n.y + at, col, cols, v[i]);
+        }
+        if (!n.pre) continue;
+        float mean, rstd;
+        row_stats(team, v, n.pre, cols, n.eps, mean, rstd);
+        if (lane == 0 && n.ry) {
+            if (n.my) n.my[r] = mean;
+            n.ry[r] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < Q; i++)
+            store_quad(n.h + at, 4 * (lane + i * lanes), cols, (v[i] - splat(mean)) * splat(rstd) * qs[i] + qb[i]);
+    }
+}
+
+// What of a row's gradient belongs to one column.
+struct Column {
+    float gate, ps, pb, qs;
+};
+struct RowStats {
+    float mb, rb, my, ry;
+};
+__device__ __forceinline__ RowStats stats_of(const Norms &n, size_t r)
+{
+    RowStats s{0.0f, 1.0f, 0.0f, 1.0f};
+    if (n.post) {
+        s.rb = n.rb[r];
+        if (n.mb) s.mb = n.mb[r];
+    }
+    if (n.pre) {
+        s.ry = n.ry[r];
+        if (n.my) s.my = n.my[r];
+    }
+    return s;
+}
+
+// The columns' sums of a block's teams, added in LDS and written to its place.  One kind after the other.
+template <int kLanes, int Q>
+__device__ __forceinline__ void put_sums(const v4f (&acc)[Q], float *lds, int lane, int lanes, int cols, float *to)
+{
+    if constexpr (kLanes == 0) {
+#pragma unroll
+        for (int i = 0; i < Q; i++) store_quad(to, 4 * (lane + i * lanes), cols, acc[i]);
+    } else {
+        constexpr int kTeams = kBlock / kLanes, kWidth = 4 * kLanes * Q;
+        const int team = (int)threadIdx.x / kLanes;
+        meet();
+#pragma unroll
+        for (int i = 0; i < Q; i++) *(v4f *)(lds + team * kWidth + 4 * (lane + i * lanes)) = acc[i];
+        meet();
+        for (int c = (int)threadIdx.x; c < cols; c += kBlock) {
+            float s = lds[c];
+#pragma unroll
+            for (int t = 1; t < kTeams; t++) s += lds[t * kWidth + c];
+            to[c] = s;
+        }
+    }
+}
+
+template <int kLanes, int Q>
+__global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, Runs runs)
+{
+    constexpr int kTeams = kLanes ? kBlock / (kLanes ? kLanes : 1) : 1;
+    __shared__ float red[64];
+    __shared__ __attribute__((aligned(16))) float lds[kLanes ? kBlock * 4 * Q : 4];
+    Team<kLanes> team{red};
+    const Norms &n = g.n;
+    const int lane = team.lane(), lanes = team.lanes(), cols = n.cols;
+    const float over = 1.0f / (float)cols;
+    v4f gate[Q], ps[Q], pb[Q], qs[Q], acc[kKinds][Q], sum_gate[Q];
+    load_row(n.ps, 1.0f, lane, lanes, cols, ps);
+    load_row(n.pb, 0.0f, lane, lanes, cols, pb);
+    load_row(n.qs, 1.0f, lane, lanes, cols, qs);
+#pragma unroll
+    for (int i = 0; i < Q; i++) {
+#pragma unroll
+        for (int k = 0; k < kKinds; k++) acc[k][i] = splat(0.0f);
+        sum_gate[i] = splat(0.0f);
+        gate[i] = splat(1.0f);
+    }
+    const size_t run = (size_t)blockIdx.x * kTeams + (kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0);
+    size_t from = 0, to = 0;
+    if (run < runs.count) runs.range(run, from, to);
+    size_t left = 0;   // rows until the next gate
+    for (size_t r = from; r < to; r++) {
+        const size_t at = r * (size_t)cols;
+        v4f t[Q], e[Q], y[Q], b[Q];
+        load_row(g.dy ? g.dy + at : nullptr, 0.0f, lane, lanes, cols, t);
+        load_row(n.branch ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, b);
+        if (n.pre) {
+            load_row(g.dh + at, 0.0f, lane, lanes, cols, e);
+            load_row(n.y + at, 0.0f, lane, lanes, cols, y);
+        }
+        if (n.gate && left == 0) {
+            load_row(n.gate + r / n.per_gate * (size_t)cols, 1.0f, lane, lanes, cols, gate);
+            left = n.per_gate - r % n.per_gate;
+        }
+        const RowStats s = stats_of(n, r);
+        if (n.pre) {
+            float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < Q; i++) {
+                y[i] = (y[i] - splat(s.my)) * splat(s.ry);
+                acc[kPreBias][i] += e[i];
+                acc[kPreScale][i] += e[i] * y[i];
+                e[i] *= qs[i];
+                s1 += sum4(e[i]);
+                s2 += sum4(e[i] * y[i]);
+            }
+            team.sum(s1, s2);
+            s1 = n.pre == DOPT_HIP_NORM_LAYER ? s1 * over : 0.0f;
+            s2 *= over;
+#pragma unroll
+            for (int i = 0; i < Q; i++) t[i] += splat(s.ry) * (e[i] - splat(s1) - y[i] * splat(s2));
+        }
+#pragma unroll
+        for (int i = 0; i < Q; i++) {
+            const int col = 4 * (lane + i * lanes);
+            t[i] = inside(t[i], col, cols);
+            if (g.dx) store_quad(g.dx + at, col, cols, splat(n.scale) * t[i]);
+        }
+        if (!n.branch) continue;
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Q; i++) {
+            b[i] = (b[i] - splat(s.mb)) * splat(s.rb);
+            sum_gate[i] += t[i] * (b[i] * ps[i] + pb[i]);
+            t[i] *= gate[i];
+            acc[kPostBias][i] += t[i];
+            acc[kPostScale][i] += t[i] * b[i];
+            t[i] *= ps[i];
+            s1 += sum4(t[i]);
+            s2 += sum4(t[i] * b[i]);
+        }
+        if (n.post) {
+            team.sum(s1, s2);
+            s1 = n.post == DOPT_HIP_NORM_LAYER ? s1 * over : 0.0f;
+            s2 *= over;
+#pragma unroll
+            for (int i = 0; i < Q; i++) t[i] = splat(s.rb) * (t[i] - splat(s1) - b[i] * splat(s2));
+        }
+        if (g.db) {
+#pragma unroll
+            for (int i = 0; i < Q; i++) store_quad(g.db + at, 4 * (lane + i * lanes), cols, t[i]);
+        }
+        if (n.gate && --left == 0 && runs.gates && g.dgate) {   // a whole gate's rows
+#pragma unroll
+            for (int i = 0; i < Q; i++) {
+                store_quad(g.dgate + r / n.per_gate * (size_t)cols, 4 * (lane + i * lanes), cols, sum_gate[i]);
+                sum_gate[i] = splat(0.0f);
+            }
+        }
+    }
+    float *sums = g.sums + (size_t)blockIdx.x * cols;
+#pragma unroll
+    for (int k = 0; k < kKinds; k++)
+        if (g.kinds >> k & 1) {
+            put_sums<kLanes>(acc[k], lds, lane, lanes, cols, sums);
+            sums += (size_t)gridDim.x * cols;
+        }
+    if (n.gate && g.dgate && !runs.gates && run < runs.count) {
+        sums = g.sums + (size_t)__builtin_popcount(g.kinds) * gridDim.x * cols + run * cols;
+#pragma unroll
+        for (int i = 0; i < Q; i++) store_quad(sums, 4 * (lane + i * lanes), cols, sum_gate[i]);
+    }
+}
+
+// Rows of more than a workgroup holds, a workgroup each, read again for each of what follows from all of a row.
+constexpr int kLong = 1024;
+__global__ __launch_bounds__(kLong) void join_long_k(Norms n)
+{
+    __shared__ float red[64];
+    Team<0> team{red};
+    const float count = (float)n.cols;
+    auto stats = [&](auto &&value, int kind, float &mean, float &rstd) {
+        mean = 0.0f;
+        if (kind == DOPT_HIP_NORM_LAYER) {
+            float all = 0.0f;
+            for (int c = threadIdx.x; c < n.cols; c += 64 * kLong) {   // sums of 64 values each
+                float s = 0.0f;
+                for (int i = c; i < min(n.cols, c + 64 * kLong); i += kLong) s += value(i);
+                all += s;
+            }
+            mean = team.sum(all) / count;
+        }
+        float all = 0.0f;
+        for (int c = threadIdx.x; c < n.cols; c += 64 * kLong) {
+            float s = 0.0f;
+            for (int i = c; i < min(n.cols, c + 64 * kLong); i += kLong) {
+                const float d = value(i) - mean;
+                s += d * d;
+            }
+            all += s;
+        }
+        rstd = 1.0f / sqrtf(team.sum(all) / count + n.eps);
+    };
+    for (size_t r = blockIdx.x; r < n.rows; r += gridDim.x) {
+        const size_t at = r * (size_t)n.cols;
+        const float *const gate = n.gate ? n.gate + r / n.per_gate * (size_t)n.cols : nullptr;
+        float mb = 0.0f, rb = 1.0f;
+        if (n.post) stats([&](int c) { return n.branch[at + c]; }, n.post, mb, rb);
+        auto y_of = [&](int c) {
+            float v = n.branch ? n.branch[at + c] : 0.0f;
+            if (n.post) v = (v - mb) * rb * (n.ps ? n.ps[c] : 1.0f) + (n.pb ? n.pb[c] : 0.0f);
+            return n.scale * (n.x ? n.x[at + c] : 0.0f) + (gate ? gate[c] : 1.0f) * v;
+        };
+        float my = 0.0f, ry = 1.0f;
+        if (n.pre) stats(y_of, n.pre, my, ry);
+        for (int c = threadIdx.x; c < n.cols; c += kLong) {   // (y or h may lie where x or the branch does)
+            const float v = y_of(c);
+            if (n.y) n.y[at + c] = v;
+            if (n.pre) n.h[at + c] = (v - my) * ry * (n.qs ? n.qs[c] : 1.0f) + (n.qb ? n.qb[c] : 0.0f);
+        }
+        if (threadIdx.x == 0) {
+            if (n.post && n.rb) {
+                if (n.mb) n.mb[r] = mb;
+                n.rb[r] = rb;
+            }
+            if (n.pre && n.ry) {
+                if (n.my) n.my[r] = my;
+                n.ry[r] = ry;
+            }
+        }
+    }
+}
+
+// ... and their gradients: dx and dbranch, and the rows' four means, for the columns' sums behind it.
+struct Means {
+    float e, ez, f, fz;
+};
+__device__ __forceinline__ float stream_grad(const Grads &g, const RowStats &s, const Means &m, size_t i, int c, float &zy)
+{
+    const Norms &n = g.n;
+    const float t = g.dy ? g.dy[i] : 0.0f;
+    if (!n.pre) return t;
+    zy = (n.y[i] - s.my) * s.ry;
+    return t + s.ry * (g.dh[i] * (n.qs ? n.qs[c] : 1.0f) - m.e - zy * m.ez);
+}
+__global__ __launch_bounds__(kLong) void join_grad_long_k(Grads g, Means *means)
+{
+    __shared__ float red[64];
+    Team<0> team{red};
+    const Norms &n = g.n;
+    const float over = 1.0f / (float)n.cols;
+    for (size_t r = blockIdx.x; r < n.rows; r += gridDim.x) {
+        const size_t at = r * (size_t)n.cols;
+        const float *const gate = n.gate ? n.gate + r / n.per_gate * (size_t)n.cols : nullptr;
+        const RowStats s = stats_of(n, r);
+        Means m{0.0f, 0.0f, 0.0f, 0.0f};
+        auto both = [&](auto &&values, float &a, float &b) {   // sums of 64 values each
+            float all_a = 0.0f, all_b = 0.0f;
+            for (int c = threadIdx.x; c < n.cols; c += 64 * kLong) {
+                float sa = 0.0f, sb = 0.0f;
+                for (int i = c; i < min(n.cols, c + 64 * kLong); i += kLong) values(i, sa, sb);
+                all_a += sa;
+                all_b += sb;
+            }
+            team.sum(all_a, all_b);
+            a = all_a * over;
+            b = all_b * over;
+        };
+        if (n.pre) {
+            both(
+                [&](int c, float &a, float &b) {
+                    const float e = g.dh[at + c] * (n.qs ? n.qs[c] : 1.0f);
+                    a += e;
+                    b += e * ((n.y[at + c] - s.my) * s.ry);
+                },
+                m.e, m.ez);
+            if (n.pre != DOPT_HIP_NORM_LAYER) m.e = 0.0f;
+        }
+        float zy;
+        auto f_of = [&](int c) {
+            return stream_grad(g, s, m, at + c, c, zy) * (gate ? gate[c] : 1.0f) * (n.post && n.ps ? n.ps[c] : 1.0f);
+        };
+        if (n.branch && n.post) {
+            both(
+                [&](int c, float &a, float &b) {
+                    const float f = f_of(c);
+                    a += f;
+                    b += f * ((n.branch[at + c] - s.mb) * s.rb);
+                },
+                m.f, m.fz);
+            if (n.post != DOPT_HIP_NORM_LAYER) m.f = 0.0f;
+        }
+        for (int c = threadIdx.x; c < n.cols; c += kLong) {
+            if (g.dx) g.dx[at + c] = n.scale * stream_grad(g, s, m, at + c, c, zy);
+            if (g.db) {
+                const float f = f_of(c);
+                g.db[at + c] = n.post ? s.rb * (f - m.f - (n.branch[at + c] - s.mb) * s.rb * m.fz) : f;
+            }
+        }
+        if (threadIdx.x == 0) means[r] = m;
+    }
+}
+// A thread's column over a run of rows.
+__global__ __launch_bounds__(kBlock) void join_columns_k(Grads g, Runs runs, const Means *means)
+{
+    const Norms &n = g.n;
+    const size_t tiles = ((size_t)n.cols + kBlock - 1) / kBlock, run = blockIdx.x / tiles;
+    const int c = (int)(blockIdx.x % tiles) * kBlock + (int)threadIdx.x;
+    if (c >= n.cols || run >= runs.count) return;
+    size_t from, to;
+    runs.range(run, from, to);
+    float acc[kKinds] = {0.0f, 0.0f, 0.0f, 0.0f}, sum_gate = 0.0f;
+    for (size_t r = from; r < to; r++) {
+        const size_t i = r * (size_t)n.cols + c;
+        const RowStats s = stats_of(n, r);
+        float zy = 0.0f;
+        const float t = stream_grad(g, s, means[r], i, c, zy);
+        if (n.pre) {
+            acc[kPreBias] += g.dh[i];
+            acc[kPreScale] += g.dh[i] * zy;
+        }
+        if (!n.branch) continue;
+        const float zb = (n.branch[i] - s.mb) * s.rb;
+        sum_gate += t * (zb * (n.ps ? n.ps[c] : 1.0f) + (n.pb ? n.pb[c] : 0.0f));
+        const float du = n.gate ? t * n.gate[r / n.per_gate * (size_t)n.cols + c] : t;
+        acc[kPostBias] += du;
+        acc[kPostScale] += du * zb;
+        if (n.gate && runs.gates && g.dgate && (r + 1) % n.per_gate == 0) {
+            g.dgate[r / n.per_gate * (size_t)n.cols + c] = sum_gate;
+            sum_gate = 0.0f;
+        }
+    }
+    float *sums = g.sums + run * n.cols + c;
+    for (int k = 0; k < kKinds; k++)
+        if (g.kinds >> k & 1) {
+            *sums = acc[k];
+            sums += runs.count * n.cols;
+        }
+    if (n.gate && g.dgate && !runs.gates) *sums = sum_gate;
+}
+
+// Adds the runs: sixteen columns of one result by sixteen lanes.
+struct Fold {
+    const float *from[kKinds + 1];
+    float *to[kKinds + 1];
+    size_t runs[kKinds + 1], rows[kKinds + 1];   // of a result's row; rows of a result
+    int n, cols;
+    size_t tiles;
+};
+__global__ __launch_bounds__(kBlock) void join_fold_k(Fold f)
+{
+    __shared__ float red[16][17];
+    size_t row = blockIdx.x / f.tiles;
+    int k = 0;
+    while (k + 1 < f.n && row >= f.rows[k]) row -= f.rows[k++];
+    const int c = (int)(blockIdx.x % f.tiles) * 16 + (int)(threadIdx.x & 15), lane = (int)threadIdx.x >> 4;
+    float all = 0.0f;
+    if (c < f.cols) {
+        const float *const from = f.from[k] + row * f.runs[k] * f.cols + c;
+        for (size_t i0 = lane; i0 < f.runs[k]; i0 += 64 * 16) {   // sums of 64 values each
+            float s = 0.0f;
+            const size_t end = min(f.runs[k], i0 + 64 * 16);
+#pragma unroll 4
+            for (size_t i = i0; i < end; i += 16) s += from[i * f.cols];
+            all += s;
+        }
+    }
+    red[lane][threadIdx.x & 15] = all;
+    __syncthreads();
+    if (lane || c >= f.cols) return;
+    for (int i = 1; i < 16; i++) all += red[i][threadIdx.x];
+    f.to[k][row * f.cols + c] = all;
+}
+
+// Which kernel holds a row: lanes of a wavefront (0: a workgroup) and quads of a lane.
+struct Form {
+    int lanes, quads;
+    unsigned threads;
+};
+Form form_of(size_t cols)
+{
+    const size_t quads = ceil_div(cols, (size_t)4);
+    if (quads <= 16) return Form{16, 1, kBlock};
+    if (quads <= 32) return Form{32, 1, kBlock};
+    if (quads <= 64) return Form{64, 1, kBlock};
+    if (quads <= 128) return Form{64, 2, kBlock};
+    if (quads <= 256) return Form{64, 4, kBlock};
+    if (quads <= 2048) return Form{0, 2, (unsigned)(64 * ceil_div(quads, (size_t)128))};
+    return Form{0, 4, (unsigned)(64 * ceil_div(quads, (size_t)256))};
+}
+template <class F>
+void with_form(const Form &f, F &&call)
+{
+    auto c = [](auto v) { return v; };
+    if (f.lanes == 16) call(c(std::integral_constant<int, 16>{}), c(std::integral_constant<int, 1>{}));
+    else if (f.lanes == 32) call(c(std::integral_constant<int, 32>{}), c(std::integral_constant<int, 1>{}));
+    else if (f.lanes == 64 && f.quads == 1) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 1>{}));
+    else if (f.lanes == 64 && f.quads == 2) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 2>{}));
+    else if (f.lanes == 64) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 4>{}));
+    else if (f.quads == 2) call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 2>{}));
+    else call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 4>{}));
+}
+
+bool known_norm(int kind) { return kind >= DOPT_HIP_NORM_NONE && kind <= DOPT_HIP_NORM_RMS; }
+
+int check(const char *who, const dopt_hip_residual_norm_desc *d, bool branch, const float *gate, const float *ps, const float *pb, const float *qs,
+          const float *qb)
+{
+    DOPT_REQUIRE(d != nullptr, "%s: null argument", who);
+    DOPT_REQUIRE(known_norm(d->post) && known_norm(d->pre), "%s: there is no norm %d", who, known_norm(d->post) ? d->pre : d->post);
+    DOPT_REQUIRE(d->rows < (size_t)1 << 31 && d->cols < (size_t)1 << 30 && d->rows * d->cols < (size_t)1 << 40, "%s: dimensions too large", who);
+    DOPT_REQUIRE(d->gates <= d->rows && (d->gates == 0 || d->rows % d->gates == 0), "%s: %zu rows do not share %zu gates evenly", who, d->rows, d->gates);
+    DOPT_REQUIRE((d->gates == 0) == (gate == nullptr) || d->rows == 0, "%s: %zu gates, and %s", who, d->gates, gate ? "an operand for them" : "no operand");
+    DOPT_REQUIRE(d->eps >= 0.0f, "%s: eps is %g", who, (double)d->eps);
+    DOPT_REQUIRE(d->post || (!ps && !pb), "%s: a scale or bias of a norm that is not there", who);
+    DOPT_REQUIRE(d->pre || (!qs && !qb), "%s: a scale or bias of a norm that is not there", who);
+    DOPT_REQUIRE(branch || d->rows == 0 || (!d->post && !d->gates), "%s: a norm or gate of a branch that is not there", who);
+    return DOPT_HIP_OK;
+}
+
+size_t stats_of_norm(int kind) { return kind == DOPT_HIP_NORM_LAYER ? 2 : kind == DOPT_HIP_NORM_RMS ? 1 : 0; }
+
+void place_stats(const dopt_hip_residual_norm_desc *d, float *stats, Norms *n)
+{
+    if (!stats) return;
+    if (d->post == DOPT_HIP_NORM_LAYER) n->mb = stats, stats += d->rows;
+    if (d->post) n->rb = stats, stats += d->rows;
+    if (d->pre == DOPT_HIP_NORM_LAYER) n->my = stats, stats += d->rows;
+    if (d->pre) n->ry = stats;
+}
+
+struct Span {
+    const void *p;
+    size_t bytes;
+};
+
+}  // namespace
+
+extern "C" {
+
+int dopt_hip_residual_norm(const dopt_hip_residual_norm_desc *d, const float *x, const float *branch, const float *gate, const float *post_scale,
+                           const float *post_bias, const float *pre_scale, const float *pre_bias, float *y, float *h, float *stats)
+{
+    const char *const who = "dopt_hip_residual_norm";
+    if (int rc = check(who, d, branch != nullptr, gate, post_scale, post_bias, pre_scale, pre_bias)) return rc;
+    if (d->rows * d->cols == 0) return DOPT_HIP_OK;
+    DOPT_REQUIRE(x || branch, "%s: neither a stream nor a branch", who);
+    DOPT_REQUIRE((d->pre == 0) == (h == nullptr), "%s: h and the norm that gives it belong together", who);
+    DOPT_REQUIRE(y || h, "%s: no result", who);
+    const size_t f = sizeof(float), all = d->rows * d->cols * f, row = d->cols * f;
+    const Span in[] = {{x, all}, {branch, all}, {gate, d->gates * row}, {post_scale, row}, {post_bias, row}, {pre_scale, row}, {pre_bias, row}};
+    const size_t stats_bytes = (stats_of_norm(d->post) + stats_of_norm(d->pre)) * d->rows * f;
+    const Span out[] = {{y, all}, {h, all}, {stats, stats_bytes}};
+    for (int i = 0; i < 3; i++) {
+        for (int k = 0; k < 7; k++)   // (a value of y or h is written by the thread that has read its operands, behind all of the row)
+            DOPT_REQUIRE(!overlaps(out[i].p, out[i].bytes, in[k].p, in[k].bytes) || (i < 2 && k < 2 && out[i].p == in[k].p),
+                         "%s: a result overlaps an operand", who);
+        for (int k = 0; k < i; k++) DOPT_REQUIRE(!overlaps(out[i].p, out[i].bytes, out[k].p, out[k].bytes), "%s: two results overlap", who);
+    }
+    DOPT_ENSURE_INIT();
+    Norms n{};
+    n.rows = d->rows;
+    n.cols = (int)d->cols;
+    n.per_gate = d->gates ? d->rows / d->gates : 0;
+    n.post = d->post;
+    n.pre = d->pre;
+    n.eps = d->eps;
+    n.scale = d->residual_scale;
+    n.x = x;
+    n.branch = branch;
+    n.gate = gate;
+    n.ps = post_scale;
+    n.pb = post_bias;
+    n.qs = pre_scale;
+    n.qb = pre_bias;
+    n.y = y;
+    n.h = h;
+    place_stats(d, stats, &n);
+    const size_t most = (size_t)num_cus() * 8;
+    if (d->cols > kHeld) {
+        hipLaunchKernelGGL(join_long_k, dim3((unsigned)std::min(d->rows, most)), dim3(kLong), 0, stream(), n);
+    } else {
+        const Form form = form_of(d->cols);
+        const size_t blocks = form.lanes ? ceil_div(d->rows, (size_t)(kBlock / form.lanes)) : d->rows;
+        with_form(form, [&](auto lanes, auto quads) {
+            hipLaunchKernelGGL((join_k<lanes.value, quads.value>), dim3((unsigned)std::min(blocks, most)), dim3(form.threads), 0, stream(), n);
+        });
+    }
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const float *dy, const float *dh, const float *y, const float *branch,
+                                const float *gate, const float *post_scale, const float *post_bias, const float *pre_scale, const float *stats,
+                                float *dx, float *dbranch, float *dgate, float *dpost_scale, float *dpost_bias, float *dpre_scale, float *dpre_bias)
+{
+    const char *const who = "dopt_hip_residual_norm_grad";
+    if (int rc = check(who, d, branch != nullptr, gate, post_scale, post_bias, pre_scale, nullptr)) return rc;
+    if (d->cols == 0) return DOPT_HIP_OK;
+    const size_t f = sizeof(float), all = d->rows * d->cols * f, row = d->cols * f;
+    const size_t stats_bytes = (stats_of_norm(d->post) + stats_of_norm(d->pre)) * d->rows * f;
+    DOPT_REQUIRE(d->rows == 0 || (d->pre ? dh && y : dy && !dh), "%s: the gradient of h and y where there is a norm of y, and that of y elsewhere", who);
+    DOPT_REQUIRE(d->rows == 0 || stats || !(d->post || d->pre), "%s: the statistics are missing", who);
+    DOPT_REQUIRE(branch || d->rows == 0 || !dbranch, "%s: the gradient of a branch that is not there", who);
+    DOPT_REQUIRE(d->gates || !dgate, "%s: the gradient of a gate that is not there", who);
+    DOPT_REQUIRE(d->post || (!dpost_scale && !dpost_bias), "%s: the gradient of a norm that is not there", who);
+    DOPT_REQUIRE(d->pre || (!dpre_scale && !dpre_bias), "%s: the gradient of a norm that is not there", who);
+    const Span in[] = {{dy, all}, {dh, all}, {y, all}, {branch, all}, {gate, d->gates * row}, {post_scale, row}, {post_bias, row}, {pre_scale, row},
+                       {stats, stats_bytes}};
+    const Span out[] = {{dx, all}, {dbranch, all}, {dgate, d->gates * row}, {dpost_scale, row}, {dpost_bias, row}, {dpre_scale, row}, {dpre_bias, row}};
+    for (int i = 0; i < 7; i++) {
+        for (const Span &s : in) DOPT_REQUIRE(!overlaps(out[i].p, out[i].bytes, s.p, s.bytes), "%s: a result overlaps an operand", who);
+        for (int k = 0; k < i; k++) DOPT_REQUIRE(!overlaps(out[i].p, out[i].bytes, out[k].p, out[k].bytes), "%s: two results overlap", who);
+    }
+    DOPT_ENSURE_INIT();
+    Grads g{};
+    Norms &n = g.n;
+    n.rows = d->rows;
+    n.cols = (int)d->cols;
+    n.per_gate = d->gates ? d->rows / d->gates : 0;
+    n.post = d->post;
+    n.pre = d->pre;
+    n.scale = d->residual_scale;
+    n.branch = branch;
+    n.gate = gate;
+    n.ps = post_scale;
+    n.pb = post_bias;
+    n.qs = pre_scale;
+    n.y = const_cast<float *>(y);
+    place_stats(d, const_cast<float *>(stats), &n);
+    g.dy = dy;
+    g.dh = dh;
+    g.dx = dx;
+    g.db = dbranch;
+    g.dgate = dgate;
+    float *const results[kKinds] = {dpre_scale, dpre_bias, dpost_scale, dpost_bias};
+    for (int k = 0; k < kKinds; k++) g.kinds |= results[k] ? 1 << k : 0;
+
+    const bool held = d->cols <= kHeld;
+    const Form form = form_of(std::min(d->cols, kHeld));
+    const size_t teams = held && form.lanes ? kBlock / form.lanes : 1;
+    // as many runs as there are teams on the chip, of a few rows at least, so that the runs' sums stay small beside the rows
+    const size_t places = (size_t)num_cus() * (held && form.lanes ? 4 * teams : std::max((size_t)1, (size_t)2048 / form.threads));
+    const size_t wanted = std::min(kRunRows, std::max((size_t)4, ceil_div(std::max(d->rows, (size_t)1), places)));
+    Runs runs{0, d->rows, n.per_gate ? n.per_gate : d->rows, 1, 0};
+    if (d->rows) {
+        if (d->gates && runs.per_gate < wanted) {
+            runs.gates = wanted / runs.per_gate;
+            runs.count = ceil_div(d->gates, runs.gates);
+        } else {
+            runs.splits = ceil_div(runs.per_gate, wanted);
+            runs.count = std::max(d->gates, (size_t)1) * runs.splits;
+        }
+    }
+    const size_t blocks = ceil_div(runs.count, teams), kinds = (size_t)__builtin_popcount((unsigned)g.kinds);
+    DOPT_REQUIRE(blocks < (size_t)1 << 24, "%s: dimensions too large", who);
+    const bool gate_sums = dgate && !runs.gates;
+    const size_t sums = (kinds * blocks + (gate_sums ? runs.count : 0)) * row, means = held ? 0 : ceil_div(d->rows * sizeof(Means), (size_t)256) * 256;
+    char *const scratch = sums + means ? (char *)workspace(sums + means) : nullptr;
+    if (sums + means && !scratch) return DOPT_HIP_ERR_OOM;
+    g.sums = (float *)(scratch + means);
+    if (d->rows && held) {
+        with_form(form, [&](auto lanes, auto quads) {
+            hipLaunchKernelGGL((join_grad_k<lanes.value, quads.value>), dim3((unsigned)blocks), dim3(form.threads), 0, stream(), g, runs);
+        });
+        DOPT_LAUNCH_CHECK();
+    } else if (d->rows) {
+        hipLaunchKernelGGL(join_grad_long_k, dim3((unsigned)std::min(d->rows, (size_t)num_cus() * 8)), dim3(kLong), 0, stream(), g, (Means *)scratch);
+        const size_t tiles = ceil_div(d->cols, (size_t)kBlock);
+        DOPT_REQUIRE(tiles * runs.count < (size_t)1 << 24, "%s: dimensions too large", who);
+        if (kinds || dgate) hipLaunchKernelGGL(join_columns_k, dim3((unsigned)(tiles * runs.count)), dim3(kBlock), 0, stream(), g, runs, (const Means *)scratch);
+        DOPT_LAUNCH_CHECK();
+    }
+    Fold fold{};
+    fold.cols = (int)d->cols;
+    fold.tiles = ceil_div(d->cols, (size_t)16);
+    size_t rows = 0;
+    auto add = [&](const float *from, float *to, size_t count, size_t results_rows) {
+        fold.from[fold.n] = from;
+        fold.to[fold.n] = to;
+        fold.runs[fold.n] = count;
+        fold.rows[fold.n++] = results_rows;
+        rows += results_rows;
+    };
+    const float *at = g.sums;
+    for (int k = 0; k < kKinds; k++)
+        if (results[k]) {
+            add(at, results[k], blocks, 1);
+            at += blocks * d->cols;
+        }
+    if (gate_sums && d->gates) add(at, dgate, d->rows ? runs.splits : 0, d->gates);
+    if (!rows) return DOPT_HIP_OK;
+    DOPT_REQUIRE(rows * fold.tiles < (size_t)1 << 24, "%s: dimensions too large", who);
+    hipLaunchKernelGGL(join_fold_k, dim3((unsigned)(rows * fold.tiles)), dim3(kBlock), 0, stream(), fold);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+}  // extern "C"

@@ -157,6 +157,41 @@ def denseAct(inp, num_outputs, init, activation="none", residual=None, use_bias=
     return Layer([inp] + ([residual] if residual else []), y, y_tr, params)
 
 
+def residualNorm(stream, branch=None, gate=None, post="none", pre="none", residual_scale=1.0, epsilon=1e-5, scale_decay=0.0):
+    """What lies between two blocks of a residual network: (the stream behind the one, what the other one reads).  The branch's norm, with its gate, is
+    added to the stream, whose norm is the second layer (the stream itself where there is none).  gate: None, a starting value
+    for a gate that is learnt and the same for all rows, or the layer that gives one for each sample.  Norms: "none", "layer" with scale
+    and bias, "rms" with a scale."""
+    first = stream if stream is not None else branch
+    c = first.output.shape[-1]
+    params, shared = [], {}
+    for name, kind in (("post", post), ("pre", pre)):
+        if kind != "none":
+            scale = float32([c], np.ones(c, np.float32))
+            params.append(Parameter(scale, None if scale_decay == 0.0 else scale_decay * core.sum(scale * scale), None))
+            shared[name + "Scale"] = scale
+        if kind == "layer":
+            shared[name + "Bias"] = float32([c])
+            params.append(Parameter(shared[name + "Bias"], None, None))
+    inputs = [l for l in (stream, branch) if l is not None]
+    gate_of = dict.fromkeys(("output", "trainOutput"))
+    if isinstance(gate, Layer):
+        inputs.append(gate)
+        gate_of = {k: getattr(gate, k) for k in gate_of}
+    elif gate is not None:
+        symbol = float32([c], np.full(c, gate, np.float32))
+        params.append(Parameter(symbol, None, None))
+        gate_of = dict.fromkeys(gate_of, symbol)
+
+    def join(which):
+        return core.residualNorm(*[getattr(l, which) if l is not None else None for l in (stream, branch)], gate_of[which], post=post, pre=pre,
+                                 residualScale=residual_scale, epsilon=epsilon, **shared)
+    tr = join("trainOutput")
+    out = tr if all(getattr(l, "output") is getattr(l, "trainOutput") for l in inputs) else join("output")
+    y = Layer(inputs, out[0], tr[0], params)
+    return y, y if pre == "none" else Layer([y], out[1], tr[1], [])
+
+
 def relu(inp):   # layers/relu.d
     return Layer([inp], core.relu(inp.output), core.relu(inp.trainOutput), [])
 

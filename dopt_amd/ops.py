@@ -465,6 +465,94 @@ def group_norm_grad(dy, x, scale, bias, stats, groups, act="none", channels_last
     return packed
 
 
+def _row_norm(kind):
+    code = capi.ROW_NORMS.get(kind)
+    if code is None:
+        raise capi.HipError(1, "there is no norm %r: %s" % (kind, ", ".join(capi.ROW_NORMS)))
+    return code
+
+
+@functools.lru_cache(maxsize=4096)
+def _residual_desc(rows, cols, gates, post, pre, eps, residual_scale):
+    return capi.ResidualNormDesc(rows, cols, gates, post, pre, eps, residual_scale)
+
+
+_STATS = (0, 2, 1)   # values of a row by its norm: mean and rstd of the layer norm, rstd alone of the rms norm
+
+
+def _row_stats(rows, post, pre):
+    return rows * (_STATS[post] + _STATS[pre])
+
+
+def _residual_args(like, operands, gate, vectors, post, pre, eps, residual_scale):
+    """The descriptor and the addresses of the optional operands: tensors of like's shape, the gate, one row each."""
+    if len(like.shape) < 1 or like.shape[-1] < 1:
+        raise capi.HipError(1, "residualNorm: rows of at least one value")
+    cols = like.shape[-1]
+    for t in operands:
+        if t is not None and (t.size != like.size or t.shape[-1:] != like.shape[-1:] or t.dtype != _F32):
+            raise capi.HipError(1, "residualNorm: an operand has the wrong size or type")
+    for t in vectors:
+        if t is not None and (t.size != cols or t.dtype != _F32):
+            raise capi.HipError(1, "residualNorm: a scale or bias has the wrong size or type")
+    if gate is not None and (gate.size % cols or gate.size == 0 or gate.dtype != _F32):
+        raise capi.HipError(1, "residualNorm: the gate has the wrong size or type")
+    rows = like.size // cols
+    return rows, cols, _residual_desc(rows, cols, gate.size // cols if gate is not None else 0, _row_norm(post), _row_norm(pre), eps,
+                                      residual_scale)
+
+
+def _ptr(t):
+    return None if t is None else t.ptr
+
+
+def residual_norm(x=None, branch=None, gate=None, post="none", post_scale=None, post_bias=None, pre="none", pre_scale=None,
+                  pre_bias=None, residual_scale=1.0, eps=1e-5, y=None, h=None, stats=None):
+    """y = residual_scale x + gate (post(branch) post_scale + post_bias) and h = pre(y) pre_scale + pre_bias over the last dimension;
+    post, pre: "none", "layer", "rms".  What is None is missing.  gate: rows of the last dimension, each for as many consecutive rows of x.
+    (y, h, stats); h is None without a norm of y; stats holds [post mean | post rstd | pre mean | pre rstd] as far as there are any."""
+    like = x if x is not None else branch
+    if like is None:
+        raise capi.HipError(1, "residualNorm: neither a stream nor a branch")
+    rows, _, d = _residual_args(like, (x, branch, y, h), gate, (post_scale, post_bias, pre_scale, pre_bias), post, pre, eps, residual_scale)
+    y = _out(y, like.shape)
+    if d.pre:
+        h = _out(h, like.shape)
+    stats = _out(stats, (_row_stats(rows, d.post, d.pre),))
+    _run(capi.load().dopt_hip_residual_norm(C.byref(d), _ptr(x), _ptr(branch), _ptr(gate), _ptr(post_scale), _ptr(post_bias), _ptr(pre_scale),
+                                            _ptr(pre_bias), y.ptr, _ptr(h), stats.ptr or None))
+    return y, h, stats
+
+
+def residual_norm_grad(dy, dh, y, branch, stats, gate=None, post="none", post_scale=None, post_bias=None, pre="none", pre_scale=None,
+                       pre_bias=None, residual_scale=1.0, out=None):
+    """The gradients of residual_norm's operands as a dict: dx, and dbranch, dgate, dpost_scale, dpost_bias, dpre_scale, dpre_bias of
+    those that are there.  dy: y's gradient from elsewhere, or None with dh.  `out`: tensors for the results that are to be formed (all of
+    them where it is None)."""
+    like = next((t for t in (dy, dh, branch) if t is not None), None)
+    if like is None:
+        raise capi.HipError(1, "residualNormGrad: no gradient")
+    rows, cols, d = _residual_args(like, (dy, dh, y, branch), gate, (post_scale, post_bias, pre_scale, pre_bias), post, pre, 0.0,
+                                   residual_scale)
+    if d.post or d.pre:
+        if stats is None or stats.size != _row_stats(rows, d.post, d.pre) or stats.dtype != _F32:
+            raise capi.HipError(1, "residualNormGrad: stats holds what residual_norm left of each row")
+    vectors = {"dpost_scale": post_scale, "dpost_bias": post_bias, "dpre_scale": pre_scale, "dpre_bias": pre_bias}
+    shapes = {"dx": like.shape}
+    if branch is not None:
+        shapes["dbranch"] = like.shape
+    if gate is not None:
+        shapes["dgate"] = gate.shape
+    shapes.update({k: v.shape for k, v in vectors.items() if v is not None})
+    if out is not None and not set(out) <= set(shapes):
+        raise capi.HipError(1, "residualNormGrad: there is no %s" % ", ".join(sorted(set(out) - set(shapes))))
+    made = {k: _out(out[k] if out is not None else None, s) for k, s in shapes.items() if out is None or k in out}
+    _run(capi.load().dopt_hip_residual_norm_grad(
+        C.byref(d), _ptr(dy), _ptr(dh), _ptr(y), _ptr(branch), _ptr(gate), _ptr(post_scale), _ptr(post_bias), _ptr(pre_scale), _ptr(stats),
+        *[_ptr(made.get(k)) for k in ("dx", "dbranch", "dgate", "dpost_scale", "dpost_bias", "dpre_scale", "dpre_bias")]))
+    return made
+
+
 def _dense_sizes(x, w):
     if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1] or x.dtype != _F32 or w.dtype != _F32:
         raise capi.HipError(1, "denseAct: x [M, K] and w [N, K] of float32")

@@ -38,6 +38,8 @@ package
         registerHIPKernel("groupNormGrad", toDelegate(&ctr!GroupNormGrad), true);
         registerHIPKernel("denseAct", toDelegate(&ctr!DenseAct), true);
         registerHIPKernel("denseActGrad", toDelegate(&ctr!DenseActGrad), true);
+        registerHIPKernel("residualNorm", toDelegate(&ctr!ResidualNorm), true);
+        registerHIPKernel("residualNormGrad", toDelegate(&ctr!ResidualNormGrad), true);
     }
 }
 
@@ -369,6 +371,126 @@ private
         }
 
         NormSize mSize;
+    }
+
+    //The optional operands of a residualNorm, by the bits of its size_t attribute "operands": stream, branch, gate,
+    //postScale, postBias, preScale, preBias; "post" and "pre" are dopt_hip_row_norm
+    struct JoinSize
+    {
+        enum { stream, branch, gate, postScale, postBias, preScale, preBias, count }
+
+        this(Operation op)
+        {
+            operands = op.attributes["operands"].get!size_t;
+            desc.post = cast(int)op.attributes["post"].get!size_t;
+            desc.pre = cast(int)op.attributes["pre"].get!size_t;
+            desc.residual_scale = op.attributes["residualScale"].get!double;
+        }
+
+        bool has(int i) const
+        {
+            return (operands >> i & 1) != 0;
+        }
+
+        size_t stats() const
+        {
+            size_t perRow(int kind)
+            {
+                return kind == 1 ? 2 : kind == 2 ? 1 : 0;
+            }
+
+            return desc.rows * (perRow(desc.post) + perRow(desc.pre));
+        }
+
+        size_t volume(int i) const
+        {
+            return i <= branch ? desc.rows * desc.cols : i == gate ? desc.gates * desc.cols : desc.cols;
+        }
+
+        size_t operands;
+        dopt_hip_residual_norm_desc desc;
+    }
+
+    class ResidualNorm : HIPKernel
+    {
+        this(Operation op)
+        {
+            mSize = JoinSize(op);
+            mSize.desc.eps = op.attributes["epsilon"].get!double;
+            mSize.desc.cols = op.deps[0].shape[$ - 1];
+            mSize.desc.rows = op.deps[0].volume / mSize.desc.cols;
+
+            if(mSize.has(JoinSize.gate))
+            {
+                auto place = (mSize.has(JoinSize.stream) ? 1 : 0) + (mSize.has(JoinSize.branch) ? 1 : 0);
+                mSize.desc.gates = op.deps[place].volume / mSize.desc.cols;
+            }
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: the operands that there are; output [y | h | stats]
+            const(float) *[JoinSize.count] o;
+            size_t k = 0;
+
+            foreach(i; 0 .. cast(int)JoinSize.count)
+            {
+                o[i] = mSize.has(i) ? f(inputs[k++]) : null;
+            }
+
+            auto v = mSize.desc.rows * mSize.desc.cols;
+            auto y = f(output);
+            auto h = mSize.desc.pre != 0 ? y + v : null;
+            auto stats = mSize.stats != 0 ? y + v * (mSize.desc.pre != 0 ? 2 : 1) : null;
+
+            hipCheck(dopt_hip_residual_norm(&mSize.desc, o[0], o[1], o[2], o[3], o[4], o[5], o[6], y, h, stats));
+        }
+
+        JoinSize mSize;
+    }
+
+    class ResidualNormGrad : HIPKernel
+    {
+        this(Operation op)
+        {
+            mSize = JoinSize(op);
+            mSize.desc.rows = op.attributes["rows"].get!size_t;
+            mSize.desc.cols = op.attributes["columns"].get!size_t;
+            mSize.desc.gates = op.attributes["gates"].get!size_t;
+            mHasDy = op.attributes["hasDy"].get!size_t != 0;
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: [dy] [dh, y], branch to preScale as there are, [stats]; output the operands' gradients in their order
+            const(float) *[JoinSize.count] o;
+            float *[JoinSize.count] d;
+            size_t k = 0;
+
+            auto dy = mHasDy ? f(inputs[k++]) : null;
+            auto dh = mSize.desc.pre != 0 ? f(inputs[k++]) : null;
+            auto y = mSize.desc.pre != 0 ? f(inputs[k++]) : null;
+
+            foreach(i; cast(int)JoinSize.branch .. JoinSize.preScale + 1)
+            {
+                o[i] = mSize.has(i) ? f(inputs[k++]) : null;
+            }
+
+            auto stats = mSize.stats != 0 ? f(inputs[k++]) : null;
+            auto to = f(output);
+
+            foreach(i; 0 .. cast(int)JoinSize.count)
+            {
+                d[i] = mSize.has(i) ? to : null;
+                to += mSize.has(i) ? mSize.volume(i) : 0;
+            }
+
+            hipCheck(dopt_hip_residual_norm_grad(&mSize.desc, dy, dh, y, o[1], o[2], o[3], o[4], o[5], stats, d[0], d[1],
+                d[2], d[3], d[4], d[5], d[6]));
+        }
+
+        JoinSize mSize;
+        bool mHasDy;
     }
 
     class DenseAct : HIPKernel

@@ -56,6 +56,14 @@ enum
     DOPT_HIP_ACT_SILU = 3,
 }
 
+alias dopt_hip_row_norm = int;
+enum
+{
+    DOPT_HIP_NORM_NONE = 0,
+    DOPT_HIP_NORM_LAYER = 1,
+    DOPT_HIP_NORM_RMS = 2,
+}
+
 struct dopt_hip_tiny_node
 {
     int kind;
@@ -98,6 +106,17 @@ struct dopt_hip_split_sum
     const(float)* bias;
     float* value;
     int lanes;
+}
+
+struct dopt_hip_residual_norm_desc
+{
+    size_t rows;
+    size_t cols;
+    size_t gates;
+    int post;
+    int pre;
+    float eps;
+    float residual_scale;
 }
 
 struct dopt_hip_tensor_ref
@@ -213,6 +232,8 @@ int dopt_hip_bn_wait_limit(uint polls);
 int dopt_hip_bn_infer(size_t N, size_t C, size_t inner, const(float)* x, const(float)* scale, const(float)* bias, const(float)* mean, const(float)* var, float* y);
 int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int channels_last, float eps, int act, const(float)* x, const(float)* scale, const(float)* bias, float* packed);
 int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, int channels_last, int act, const(float)* dy, const(float)* x, const(float)* scale, const(float)* bias, const(float)* stats, float* packed);
+int dopt_hip_residual_norm(const(dopt_hip_residual_norm_desc)* desc, const(float)* x, const(float)* branch, const(float)* gate, const(float)* post_scale, const(float)* post_bias, const(float)* pre_scale, const(float)* pre_bias, float* y, float* h, float* stats);
+int dopt_hip_residual_norm_grad(const(dopt_hip_residual_norm_desc)* desc, const(float)* dy, const(float)* dh, const(float)* y, const(float)* branch, const(float)* gate, const(float)* post_scale, const(float)* post_bias, const(float)* pre_scale, const(float)* stats, float* dx, float* dbranch, float* dgate, float* dpost_scale, float* dpost_bias, float* dpre_scale, float* dpre_bias);
 int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const(float)* x, const(float)* w, const(float)* bias, const(float)* residual, float* y, float* pre);
 int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const(float)* dy, const(float)* pre, const(float)* x, const(float)* w, float* dx, float* dw, float* dbias);
 int dopt_hip_optim_create(int ntensors, const(dopt_hip_tensor_ref)* refs, void** handle);

@@ -535,6 +535,40 @@ int dopt_hip_group_norm(size_t N, size_t C, size_t inner, size_t groups, int cha
 int dopt_hip_group_norm_grad(size_t N, size_t C, size_t inner, size_t groups, int channels_last, int act, const float *dy,
                              const float *x, const float *scale, const float *bias, const float *stats, float *packed);
 
+/* The norms of a row: none; (v - mean) / sqrt(variance + eps), the variance biased; v / sqrt(mean of v^2 + eps) */
+typedef enum {
+    DOPT_HIP_NORM_NONE = 0,
+    DOPT_HIP_NORM_LAYER = 1,
+    DOPT_HIP_NORM_RMS = 2
+} dopt_hip_row_norm;
+
+typedef struct {
+    size_t rows, cols;
+    size_t gates;          /* rows of the gate, each for rows / gates consecutive rows; 0: there is none */
+    int post, pre;         /* dopt_hip_row_norm of the branch, and of the sum */
+    float eps;
+    float residual_scale;
+} dopt_hip_residual_norm_desc;
+
+/* What lies between two blocks of a residual network: the norm behind the one, its gate, the sum with the stream, and the norm before
+   the other, in one pass over rows of cols values:
+     y = residual_scale * x + gate * (post(branch) * post_scale + post_bias),  h = pre(y) * pre_scale + pre_bias
+   x or branch may be null (a term that is missing), gate, scales and biases too (one, one, zero), y where it is not wanted, h where
+   there is no norm of y, stats in inference.  A row of the gate belongs to one sample, to all rows, or (gates == rows) to one row.
+   stats = [ mean of the branch | rstd of the branch | mean of y | rstd of y ], `rows` values each, of which a norm that is not there
+   has none and the rms norm no mean.  y and h may take the place of x or of the branch (the same address); otherwise no result may
+   overlap an operand. */
+int dopt_hip_residual_norm(const dopt_hip_residual_norm_desc *desc, const float *x, const float *branch, const float *gate,
+                           const float *post_scale, const float *post_bias, const float *pre_scale, const float *pre_bias,
+                           float *y, float *h, float *stats);
+/* The gradients, from that of h (dh; none without a norm of y) and that of y from elsewhere (dy, may be null with dh); y and stats as
+   the forward pass left them.  dgate sums over the rows of a gate, the scales' and biases' gradients over all rows.  Any
+   result may be null; none may overlap an operand. */
+int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *desc, const float *dy, const float *dh, const float *y,
+                                const float *branch, const float *gate, const float *post_scale, const float *post_bias,
+                                const float *pre_scale, const float *stats, float *dx, float *dbranch, float *dgate,
+                                float *dpost_scale, float *dpost_bias, float *dpre_scale, float *dpre_bias);
+
 /* pre = x * w^T + bias, y = act(pre) + residual: x [M,K], w [N,K] as nnet/layers/dense.d stores it, bias [N], residual [M,N].
    bias, residual and pre may be null; a training step keeps pre, which the gradient reads (act none needs none).  y and pre may
    overlap neither each other nor an operand.
