@@ -24,7 +24,7 @@ using namespace dopt;
 
 constexpr int kBlock = 256;          // of teams within a wavefront
 constexpr size_t kHeld = 16384;      // values of a row that a workgroup holds at most
-constexpr size_t kRunRows = 128;     // of a run at most: sums of more values that are alike are rounded the same way for long
+constexpr size_t kTeamRows = 128;    // rows that a team adds up at most: sums of more values that are alike are rounded the same way for long
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));   // sixteen bytes wherever they start
@@ -75,9 +75,11 @@ struct Grads {
 };
 enum Kind { kPreScale, kPreBias, kPostScale, kPostBias, kKinds };
 
-// Rows in runs: of a gate's rows, `splits` runs for each gate; or of `gates` whole gates each, whose gradients then need no second launch.
+// A workgroup's rows: of a gate's rows one of `splits` runs; or, where kWhole, `gates` whole gates.  Its teams take every teams-th row of
+// a run, or every teams-th gate.
 struct Runs {
     size_t count, rows, per_gate, splits, gates;
+    __device__ __forceinline__ size_t gate_of(size_t run) const { return run / splits; }
     __device__ __forceinline__ void range(size_t run, size_t &from, size_t &to) const
     {
         if (gates) {
@@ -124,19 +126,22 @@ __device__ __forceinline__ v4f inside(v4f v, int col, int cols)   // zero beyond
 __device__ __forceinline__ float sum4(v4f v) { return (v.x + v.y) + (v.z + v.w); }
 __device__ __forceinline__ v4f splat(float v) { return v4f{v, v, v, v}; }
 
-// The lanes that share a row: kLanes of a wavefront, or (0) the workgroup.
+// The lanes that share a row: kLanes of a wavefront, or (0) `waves` wavefronts of a workgroup, whose teams then sum together.
 template <int kLanes>
 struct Team {
-    static constexpr bool kBlockwide = kLanes == 0;
-    float *red;   // of a workgroup: twice 32 values
+    static constexpr bool kWide = kLanes == 0;
+    float *red;   // of wide teams: twice 32 values
+    int waves;
     int turn = 0;
-    __device__ __forceinline__ int lane() const { return kBlockwide ? (int)threadIdx.x : (int)threadIdx.x & (kLanes - 1); }
-    __device__ __forceinline__ int lanes() const { return kBlockwide ? (int)blockDim.x : kLanes; }
+    __device__ __forceinline__ int lanes() const { return kWide ? 64 * waves : kLanes; }
+    __device__ __forceinline__ int index() const { return kWide ? (int)threadIdx.x / lanes() : (int)threadIdx.x / (kLanes ? kLanes : 1); }
+    __device__ __forceinline__ int lane() const { return kWide ? (int)threadIdx.x - index() * lanes() : (int)threadIdx.x & (kLanes - 1); }
+    __device__ __forceinline__ int teams() const { return kWide ? (int)blockDim.x / lanes() : kBlock / (kLanes ? kLanes : 1); }
     __device__ __forceinline__ void sum(float &a, float &b)   // both over the team, in all of its lanes
     {
-        a = lanes_sum<kBlockwide ? 64 : kLanes>(a);
-        b = lanes_sum<kBlockwide ? 64 : kLanes>(b);
-        if (!kBlockwide || blockDim.x == 64) return;
+        a = lanes_sum<kWide ? 64 : kLanes>(a);
+        b = lanes_sum<kWide ? 64 : kLanes>(b);
+        if (!kWide || waves == 1) return;
         float *const r = red + turn * 32;   // two places in turn: a barrier apiece is enough
         turn ^= 1;
         if ((threadIdx.x & 63) == 0) {
@@ -144,12 +149,12 @@ struct Team {
             r[16 + (threadIdx.x >> 6)] = b;
         }
         meet();
-        const int waves = (int)blockDim.x >> 6;
-        a = r[0];
-        b = r[16];
+        const int first = index() * waves;
+        a = r[first];
+        b = r[16 + first];
         for (int i = 1; i < waves; i++) {
-            a += r[i];
-            b += r[16 + i];
+            a += r[first + i];
+            b += r[16 + first + i];
         }
     }
     __device__ __forceinline__ float sum(float a)
@@ -192,8 +197,7 @@ template <int kLanes, int Q>
 __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
 {
     __shared__ float red[64];
-    Team<kLanes> team{red};
-    constexpr int kTeams = kLanes ? kBlock / (kLanes ? kLanes : 1) : 1;
+    Team<kLanes> team{red, (int)blockDim.x >> 6};
     const int lane = team.lane(), lanes = team.lanes(), cols = n.cols;
     v4f gate[Q], ps[Q], pb[Q], qs[Q], qb[Q];
     load_row(n.ps, 1.0f, lane, lanes, cols, ps);
@@ -202,8 +206,8 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
     load_row(n.qb, 0.0f, lane, lanes, cols, qb);
     const bool one_gate = n.per_gate == 0 || n.per_gate == n.rows;
     if (one_gate) load_row(n.gate, 1.0f, lane, lanes, cols, gate);
-    const size_t first = (size_t)blockIdx.x * kTeams + (kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0);
-    for (size_t r = first; r < n.rows; r += (size_t)gridDim.x * kTeams) {
+    const size_t first = (size_t)blockIdx.x * team.teams() + team.index();
+    for (size_t r = first; r < n.rows; r += (size_t)gridDim.x * team.teams()) {
         const size_t at = r * (size_t)cols;
         v4f x[Q], v[Q];
         load_row(n.branch ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, v);
@@ -238,10 +242,6 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
     }
 }
 
-// What of a row's gradient belongs to one column.
-struct Column {
-    float gate, ps, pb, qs;
-};
 struct RowStats {
     float mb, rb, my, ry;
 };
@@ -259,76 +259,89 @@ __device__ __forceinline__ RowStats stats_of(const Norms &n, size_t r)
     return s;
 }
 
-// The columns' sums of a block's teams, added in LDS and written to its place.  One kind after the other.
-template <int kLanes, int Q>
-__device__ __forceinline__ void put_sums(const v4f (&acc)[Q], float *lds, int lane, int lanes, int cols, float *to)
+// Adds what the workgroup's teams hold, in team 0.
+template <int Q, class T>
+__device__ __forceinline__ void join_teams(const T &team, v4f (&acc)[Q], float *lds, int lane, int lanes)
 {
-    if constexpr (kLanes == 0) {
+    if (team.teams() == 1) return;
+    const int width = 4 * lanes * Q;
+    meet();
 #pragma unroll
-        for (int i = 0; i < Q; i++) store_quad(to, 4 * (lane + i * lanes), cols, acc[i]);
-    } else {
-        constexpr int kTeams = kBlock / kLanes, kWidth = 4 * kLanes * Q;
-        const int team = (int)threadIdx.x / kLanes;
-        meet();
+    for (int i = 0; i < Q; i++) *(v4f *)(lds + team.index() * width + 4 * (lane + i * lanes)) = acc[i];
+    meet();
+    if (team.index()) return;
+    for (int t = 1; t < team.teams(); t++)
 #pragma unroll
-        for (int i = 0; i < Q; i++) *(v4f *)(lds + team * kWidth + 4 * (lane + i * lanes)) = acc[i];
-        meet();
-        for (int c = (int)threadIdx.x; c < cols; c += kBlock) {
-            float s = lds[c];
+        for (int i = 0; i < Q; i++) acc[i] += *(const v4f *)(lds + t * width + 4 * (lane + i * lanes));
+}
+template <int Q>
+__device__ __forceinline__ void store_row(float *to, int lane, int lanes, int cols, const v4f (&v)[Q])
+{
 #pragma unroll
-            for (int t = 1; t < kTeams; t++) s += lds[t * kWidth + c];
-            to[c] = s;
-        }
-    }
+    for (int i = 0; i < Q; i++) store_quad(to, 4 * (lane + i * lanes), cols, v[i]);
 }
 
-template <int kLanes, int Q>
-__global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, Runs runs)
+// Within a gate's rows the sums of t zb and of t are all that the branch's columns need: dps = gate a, dpb = gate b, dgate = ps a + pb b.
+// Scales lie in LDS where they fit (kStaged), for the registers' sake.
+template <int kLanes, int Q, bool kWhole, bool kStaged>
+__global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, Runs runs, int waves)
 {
-    constexpr int kTeams = kLanes ? kBlock / (kLanes ? kLanes : 1) : 1;
     __shared__ float red[64];
-    __shared__ __attribute__((aligned(16))) float lds[kLanes ? kBlock * 4 * Q : 4];
-    Team<kLanes> team{red};
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    Team<kLanes> team{red, waves};
     const Norms &n = g.n;
-    const int lane = team.lane(), lanes = team.lanes(), cols = n.cols;
+    const int lane = team.lane(), lanes = team.lanes(), cols = n.cols, width = 4 * lanes * Q;
     const float over = 1.0f / (float)cols;
-    v4f gate[Q], ps[Q], pb[Q], qs[Q], acc[kKinds][Q], sum_gate[Q];
-    load_row(n.ps, 1.0f, lane, lanes, cols, ps);
-    load_row(n.pb, 0.0f, lane, lanes, cols, pb);
-    load_row(n.qs, 1.0f, lane, lanes, cols, qs);
-#pragma unroll
-    for (int i = 0; i < Q; i++) {
-#pragma unroll
-        for (int k = 0; k < kKinds; k++) acc[k][i] = splat(0.0f);
-        sum_gate[i] = splat(0.0f);
-        gate[i] = splat(1.0f);
+    const size_t run = blockIdx.x;
+    size_t from, to;
+    runs.range(run, from, to);
+    const float *gate = n.gate ? n.gate + (kWhole ? 0 : runs.gate_of(run)) * (size_t)cols : nullptr;
+    if constexpr (kStaged) {
+        for (int c = (int)threadIdx.x; c < width; c += (int)blockDim.x) {
+            const bool in = c < cols;
+            lds[c] = n.qs && in ? n.qs[c] : 1.0f;
+            lds[width + c] = n.ps && in ? n.ps[c] : 1.0f;
+            if (!kWhole) lds[2 * width + c] = gate && in ? gate[c] : 1.0f;
+        }
+        meet();
     }
-    const size_t run = (size_t)blockIdx.x * kTeams + (kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0);
-    size_t from = 0, to = 0;
-    if (run < runs.count) runs.range(run, from, to);
-    size_t left = 0;   // rows until the next gate
-    for (size_t r = from; r < to; r++) {
-        const size_t at = r * (size_t)cols;
-        v4f t[Q], e[Q], y[Q], b[Q];
-        load_row(g.dy ? g.dy + at : nullptr, 0.0f, lane, lanes, cols, t);
-        load_row(n.branch ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, b);
+    auto scale = [&](const float *p, int staged, int col) {
+        return kStaged ? *(const v4f *)(lds + staged * width + col) : p ? load_quad(p, col, cols) : splat(1.0f);
+    };
+    auto gates = [&](int col) { return kWhole ? gate ? load_quad(gate, col, cols) : splat(1.0f) : scale(gate, 2, col); };
+
+    v4f dqs[Q], dqb[Q], a[Q], b[Q], dps[kWhole ? Q : 1], dpb[kWhole ? Q : 1];
+#pragma unroll
+    for (int i = 0; i < Q; i++) dqs[i] = dqb[i] = a[i] = b[i] = splat(0.0f);
+    if (kWhole) {
+#pragma unroll
+        for (int i = 0; i < Q; i++) dps[i] = dpb[i] = splat(0.0f);
+    }
+    const int teams = team.teams();
+    const size_t mine = team.index();
+    size_t r = kWhole ? from + mine * runs.per_gate : from + mine;
+    size_t left = runs.per_gate;   // kWhole: rows of this gate that are left
+    const size_t turns = kWhole ? (runs.gates + teams - 1) / teams * runs.per_gate : (to - from + teams - 1) / teams;
+    for (size_t turn = 0; turn < turns; turn++) {
+        const bool live = r < to;   // (a team without a row keeps the others company)
+        const size_t at = live ? r * (size_t)cols : 0;
+        v4f t[Q], e[Q], y[Q], z[Q];
+        load_row(live && g.dy ? g.dy + at : nullptr, 0.0f, lane, lanes, cols, t);
+        load_row(live && n.branch && (n.post || gate) ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, z);
         if (n.pre) {
-            load_row(g.dh + at, 0.0f, lane, lanes, cols, e);
-            load_row(n.y + at, 0.0f, lane, lanes, cols, y);
+            load_row(live ? g.dh + at : nullptr, 0.0f, lane, lanes, cols, e);
+            load_row(live ? n.y + at : nullptr, 0.0f, lane, lanes, cols, y);
         }
-        if (n.gate && left == 0) {
-            load_row(n.gate + r / n.per_gate * (size_t)cols, 1.0f, lane, lanes, cols, gate);
-            left = n.per_gate - r % n.per_gate;
-        }
-        const RowStats s = stats_of(n, r);
+        RowStats s{0.0f, 1.0f, 0.0f, 1.0f};
+        if (live) s = stats_of(n, r);
         if (n.pre) {
             float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
             for (int i = 0; i < Q; i++) {
-                y[i] = (y[i] - splat(s.my)) * splat(s.ry);
-                acc[kPreBias][i] += e[i];
-                acc[kPreScale][i] += e[i] * y[i];
-                e[i] *= qs[i];
+                y[i] = inside((y[i] - splat(s.my)) * splat(s.ry), 4 * (lane + i * lanes), cols);
+                dqb[i] += e[i];
+                dqs[i] += e[i] * y[i];
+                e[i] *= scale(n.qs, 0, 4 * (lane + i * lanes));
                 s1 += sum4(e[i]);
                 s2 += sum4(e[i] * y[i]);
             }
@@ -342,51 +355,87 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, R
         for (int i = 0; i < Q; i++) {
             const int col = 4 * (lane + i * lanes);
             t[i] = inside(t[i], col, cols);
-            if (g.dx) store_quad(g.dx + at, col, cols, splat(n.scale) * t[i]);
+            if (g.dx && live) store_quad(g.dx + at, col, cols, splat(n.scale) * t[i]);
         }
-        if (!n.branch) continue;
-        float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < Q; i++) {
-            b[i] = (b[i] - splat(s.mb)) * splat(s.rb);
-            sum_gate[i] += t[i] * (b[i] * ps[i] + pb[i]);
-            t[i] *= gate[i];
-            acc[kPostBias][i] += t[i];
-            acc[kPostScale][i] += t[i] * b[i];
-            t[i] *= ps[i];
-            s1 += sum4(t[i]);
-            s2 += sum4(t[i] * b[i]);
-        }
-        if (n.post) {
-            team.sum(s1, s2);
-            s1 = n.post == DOPT_HIP_NORM_LAYER ? s1 * over : 0.0f;
-            s2 *= over;
-#pragma unroll
-            for (int i = 0; i < Q; i++) t[i] = splat(s.rb) * (t[i] - splat(s1) - b[i] * splat(s2));
-        }
-        if (g.db) {
-#pragma unroll
-            for (int i = 0; i < Q; i++) store_quad(g.db + at, 4 * (lane + i * lanes), cols, t[i]);
-        }
-        if (n.gate && --left == 0 && runs.gates && g.dgate) {   // a whole gate's rows
+        if (n.branch) {
+            if (kWhole && gate) gate = n.gate + (live ? r / runs.per_gate : 0) * (size_t)cols;
+            float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
             for (int i = 0; i < Q; i++) {
-                store_quad(g.dgate + r / n.per_gate * (size_t)cols, 4 * (lane + i * lanes), cols, sum_gate[i]);
-                sum_gate[i] = splat(0.0f);
+                const int col = 4 * (lane + i * lanes);
+                z[i] = inside((z[i] - splat(s.mb)) * splat(s.rb), col, cols);
+                b[i] += t[i];
+                a[i] += t[i] * z[i];
+                t[i] *= gates(col) * scale(n.ps, 1, col);
+                s1 += sum4(t[i]);
+                s2 += sum4(t[i] * z[i]);
             }
+            if (n.post) {
+                team.sum(s1, s2);
+                s1 = n.post == DOPT_HIP_NORM_LAYER ? s1 * over : 0.0f;
+                s2 *= over;
+#pragma unroll
+                for (int i = 0; i < Q; i++) t[i] = splat(s.rb) * (t[i] - splat(s1) - z[i] * splat(s2));
+            }
+            if (g.db && live) store_row(g.db + at, lane, lanes, cols, t);
+        }
+        r += kWhole ? 1 : teams;
+        if (kWhole && --left == 0) {
+            left = runs.per_gate;
+#pragma unroll
+            for (int i = 0; i < Q && live; i++) {
+                const int col = 4 * (lane + i * lanes);
+                const v4f g4 = gates(col);
+                dps[i] += g4 * a[i];
+                dpb[i] += g4 * b[i];
+                if (g.dgate)
+                    store_quad(g.dgate + (r - 1) / runs.per_gate * (size_t)cols, col, cols,
+                               scale(n.ps, 1, col) * a[i] + (n.pb ? load_quad(n.pb, col, cols) * b[i] : splat(0.0f)));
+                a[i] = b[i] = splat(0.0f);
+            }
+            r += (teams - 1) * runs.per_gate;
         }
     }
-    float *sums = g.sums + (size_t)blockIdx.x * cols;
+    float *sums = g.sums + run * cols;
+    const size_t next = (size_t)gridDim.x * cols;
+    if (g.kinds >> kPreScale & 1) {
+        join_teams(team, dqs, lds + 3 * width, lane, lanes);
+        if (mine == 0) store_row(sums, lane, lanes, cols, dqs);
+        sums += next;
+    }
+    if (g.kinds >> kPreBias & 1) {
+        join_teams(team, dqb, lds + 3 * width, lane, lanes);
+        if (mine == 0) store_row(sums, lane, lanes, cols, dqb);
+        sums += next;
+    }
+    const bool of_gate = !kWhole && g.dgate;
+    if (!(g.kinds >> kPostScale) && !of_gate) return;
+    if (kWhole) {
 #pragma unroll
-    for (int k = 0; k < kKinds; k++)
-        if (g.kinds >> k & 1) {
-            put_sums<kLanes>(acc[k], lds, lane, lanes, cols, sums);
-            sums += (size_t)gridDim.x * cols;
+        for (int i = 0; i < Q; i++) {
+            a[i] = dps[i];
+            b[i] = dpb[i];
         }
-    if (n.gate && g.dgate && !runs.gates && run < runs.count) {
-        sums = g.sums + (size_t)__builtin_popcount(g.kinds) * gridDim.x * cols + run * cols;
+    }
+    join_teams(team, a, lds + 3 * width, lane, lanes);
+    join_teams(team, b, lds + 3 * width, lane, lanes);
+    if (mine) return;
 #pragma unroll
-        for (int i = 0; i < Q; i++) store_quad(sums, 4 * (lane + i * lanes), cols, sum_gate[i]);
+    for (int i = 0; i < Q; i++) {
+        const int col = 4 * (lane + i * lanes);
+        const v4f g4 = kWhole ? splat(1.0f) : gates(col);
+        float *at = sums;
+        if (g.kinds >> kPostScale & 1) {
+            store_quad(at, col, cols, g4 * a[i]);
+            at += next;
+        }
+        if (g.kinds >> kPostBias & 1) {
+            store_quad(at, col, cols, g4 * b[i]);
+            at += next;
+        }
+        if (of_gate)
+            store_quad(runs.splits == 1 ? g.dgate + run * cols : at, col, cols,
+                       scale(n.ps, 1, col) * a[i] + (n.pb ? load_quad(n.pb, col, cols) * b[i] : splat(0.0f)));
     }
 }
 
@@ -395,7 +444,7 @@ constexpr int kLong = 1024;
 __global__ __launch_bounds__(kLong) void join_long_k(Norms n)
 {
     __shared__ float red[64];
-    Team<0> team{red};
+    Team<0> team{red, kLong / 64};
     const float count = (float)n.cols;
     auto stats = [&](auto &&value, int kind, float &mean, float &rstd) {
         mean = 0.0f;
@@ -464,7 +513,7 @@ __device__ __forceinline__ float stream_grad(const Grads &g, const RowStats &s, 
 __global__ __launch_bounds__(kLong) void join_grad_long_k(Grads g, Means *means)
 {
     __shared__ float red[64];
-    Team<0> team{red};
+    Team<0> team{red, kLong / 64};
     const Norms &n = g.n;
     const float over = 1.0f / (float)n.cols;
     for (size_t r = blockIdx.x; r < n.rows; r += gridDim.x) {
@@ -554,10 +603,10 @@ __global__ __launch_bounds__(kBlock) void join_columns_k(Grads g, Runs runs, con
             *sums = acc[k];
             sums += runs.count * n.cols;
         }
-    if (n.gate && g.dgate && !runs.gates) *sums = sum_gate;
+    if (n.gate && g.dgate && !runs.gates) *(runs.splits == 1 ? g.dgate + run * n.cols + c : sums) = sum_gate;
 }
 
-// Adds the runs: sixteen columns of one result by sixteen lanes.
+// Adds the runs: 32 columns of one result by 32 lanes.
 struct Fold {
     const float *from[kKinds + 1];
     float *to[kKinds + 1];
@@ -565,28 +614,28 @@ struct Fold {
     int n, cols;
     size_t tiles;
 };
-__global__ __launch_bounds__(kBlock) void join_fold_k(Fold f)
+__global__ __launch_bounds__(1024) void join_fold_k(Fold f)
 {
-    __shared__ float red[16][17];
+    __shared__ float red[32][33];
     size_t row = blockIdx.x / f.tiles;
     int k = 0;
     while (k + 1 < f.n && row >= f.rows[k]) row -= f.rows[k++];
-    const int c = (int)(blockIdx.x % f.tiles) * 16 + (int)(threadIdx.x & 15), lane = (int)threadIdx.x >> 4;
+    const int c = (int)(blockIdx.x % f.tiles) * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
     float all = 0.0f;
     if (c < f.cols) {
         const float *const from = f.from[k] + row * f.runs[k] * f.cols + c;
-        for (size_t i0 = lane; i0 < f.runs[k]; i0 += 64 * 16) {   // sums of 64 values each
+        for (size_t i0 = lane; i0 < f.runs[k]; i0 += 64 * 32) {   // sums of 64 values each
             float s = 0.0f;
-            const size_t end = min(f.runs[k], i0 + 64 * 16);
-#pragma unroll 4
-            for (size_t i = i0; i < end; i += 16) s += from[i * f.cols];
+            const size_t end = min(f.runs[k], i0 + 64 * 32);
+#pragma unroll 8
+            for (size_t i = i0; i < end; i += 32) s += from[i * f.cols];
             all += s;
         }
     }
-    red[lane][threadIdx.x & 15] = all;
+    red[lane][threadIdx.x & 31] = all;
     __syncthreads();
-    if (lane || c >= f.cols) return;
-    for (int i = 1; i < 16; i++) all += red[i][threadIdx.x];
+    if (threadIdx.x >= 32 || c >= f.cols) return;
+    for (int i = 1; i < 32; i++) all += red[i][threadIdx.x];
     f.to[k][row * f.cols + c] = all;
 }
 
@@ -617,6 +666,20 @@ void with_form(const Form &f, F &&call)
     else if (f.lanes == 64) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 4>{}));
     else if (f.quads == 2) call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 2>{}));
     else call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 4>{}));
+}
+
+template <int kLanes, int Q, bool kWhole, bool kStaged>
+int launch_grad(unsigned blocks, unsigned threads, size_t lds, const Grads &g, const Runs &runs, int waves)
+{
+    const auto kernel = join_grad_k<kLanes, Q, kWhole, kStaged>;
+    static bool raised = false;
+    if (!raised && lds > 65536 - 1024) {
+        DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 159 * 1024));
+        raised = true;
+    }
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), lds, stream(), g, runs, waves);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
 }
 
 bool known_norm(int kind) { return kind >= DOPT_HIP_NORM_NONE && kind <= DOPT_HIP_NORM_RMS; }
@@ -756,32 +819,42 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
 
     const bool held = d->cols <= kHeld;
     const Form form = form_of(std::min(d->cols, kHeld));
-    const size_t teams = held && form.lanes ? kBlock / form.lanes : 1;
-    // as many runs as there are teams on the chip, of a few rows at least, so that the runs' sums stay small beside the rows
-    const size_t places = (size_t)num_cus() * (held && form.lanes ? 4 * teams : std::max((size_t)1, (size_t)2048 / form.threads));
-    const size_t wanted = std::min(kRunRows, std::max((size_t)4, ceil_div(std::max(d->rows, (size_t)1), places)));
-    Runs runs{0, d->rows, n.per_gate ? n.per_gate : d->rows, 1, 0};
+    // Teams of a workgroup: of several wavefronts each, as many as make half of the largest one.
+    const int waves = (int)form.threads / 64;
+    const size_t teams = !held ? 1 : form.lanes ? (size_t)(kBlock / form.lanes) : std::max(1, 8 / waves);
+    const unsigned threads = form.lanes ? form.threads : form.threads * (unsigned)teams;
+    // As many runs as there are workgroups on the chip at a time, of a few rows for each team at least, so that their sums stay small beside
+    // the rows.  Gates of a few rows go to teams as a whole.
+    const unsigned at_a_time = form.lanes ? form.quads == 4 ? 512 : form.quads == 2 ? 1024 : 1536 : 1024;   // threads of a CU, by their registers
+    const size_t places = (size_t)num_cus() * std::max(1u, at_a_time / threads);
+    const size_t wanted = std::min(kTeamRows * teams, std::max(4 * teams, ceil_div(std::max(d->rows, (size_t)1), places)));
+    Runs runs{0, d->rows, n.per_gate ? n.per_gate : std::max(d->rows, (size_t)1), 1, 0};
     if (d->rows) {
-        if (d->gates && runs.per_gate < wanted) {
-            runs.gates = wanted / runs.per_gate;
+        if (d->gates && runs.per_gate < std::min(wanted, (size_t)16)) {
+            runs.gates = ceil_div(ceil_div(wanted, runs.per_gate), teams) * teams;
             runs.count = ceil_div(d->gates, runs.gates);
         } else {
             runs.splits = ceil_div(runs.per_gate, wanted);
             runs.count = std::max(d->gates, (size_t)1) * runs.splits;
         }
     }
-    const size_t blocks = ceil_div(runs.count, teams), kinds = (size_t)__builtin_popcount((unsigned)g.kinds);
-    DOPT_REQUIRE(blocks < (size_t)1 << 24, "%s: dimensions too large", who);
-    const bool gate_sums = dgate && !runs.gates;
-    const size_t sums = (kinds * blocks + (gate_sums ? runs.count : 0)) * row, means = held ? 0 : ceil_div(d->rows * sizeof(Means), (size_t)256) * 256;
+    const size_t blocks = runs.count, kinds = (size_t)__builtin_popcount((unsigned)g.kinds);
+    DOPT_REQUIRE(blocks < (size_t)1 << 22, "%s: dimensions too large", who);
+    const bool gate_sums = dgate && !runs.gates && (runs.splits > 1 || d->rows == 0);
+    const size_t sums = (kinds * blocks + (gate_sums ? blocks : 0)) * row, means = held ? 0 : ceil_div(d->rows * sizeof(Means), (size_t)256) * 256;
     char *const scratch = sums + means ? (char *)workspace(sums + means) : nullptr;
     if (sums + means && !scratch) return DOPT_HIP_ERR_OOM;
     g.sums = (float *)(scratch + means);
     if (d->rows && held) {
+        int rc = DOPT_HIP_OK;
         with_form(form, [&](auto lanes, auto quads) {
-            hipLaunchKernelGGL((join_grad_k<lanes.value, quads.value>), dim3((unsigned)blocks), dim3(form.threads), 0, stream(), g, runs);
+            constexpr bool kStaged = lanes.value || quads.value < 4;
+            const size_t width = 4 * (lanes.value ? (size_t)lanes.value : (size_t)form.threads) * quads.value;
+            const size_t bytes = (3 + (teams > 1 ? teams : 0)) * width * f;
+            rc = runs.gates ? launch_grad<lanes.value, quads.value, true, kStaged>((unsigned)blocks, threads, kStaged ? bytes : 0, g, runs, waves)
+                            : launch_grad<lanes.value, quads.value, false, kStaged>((unsigned)blocks, threads, kStaged ? bytes : 0, g, runs, waves);
         });
-        DOPT_LAUNCH_CHECK();
+        if (rc) return rc;
     } else if (d->rows) {
         hipLaunchKernelGGL(join_grad_long_k, dim3((unsigned)std::min(d->rows, (size_t)num_cus() * 8)), dim3(kLong), 0, stream(), g, (Means *)scratch);
         const size_t tiles = ceil_div(d->cols, (size_t)kBlock);
@@ -791,7 +864,7 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     }
     Fold fold{};
     fold.cols = (int)d->cols;
-    fold.tiles = ceil_div(d->cols, (size_t)16);
+    fold.tiles = ceil_div(d->cols, (size_t)32);
     size_t rows = 0;
     auto add = [&](const float *from, float *to, size_t count, size_t results_rows) {
         fold.from[fold.n] = from;
@@ -808,8 +881,8 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
         }
     if (gate_sums && d->gates) add(at, dgate, d->rows ? runs.splits : 0, d->gates);
     if (!rows) return DOPT_HIP_OK;
-    DOPT_REQUIRE(rows * fold.tiles < (size_t)1 << 24, "%s: dimensions too large", who);
-    hipLaunchKernelGGL(join_fold_k, dim3((unsigned)(rows * fold.tiles)), dim3(kBlock), 0, stream(), fold);
+    DOPT_REQUIRE(rows * fold.tiles < (size_t)1 << 22, "%s: dimensions too large", who);
+    hipLaunchKernelGGL(join_fold_k, dim3((unsigned)(rows * fold.tiles)), dim3(1024), 0, stream(), fold);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
