@@ -24,6 +24,7 @@ using namespace dopt;
 
 constexpr int kBlock = 256;          // of teams within a wavefront
 constexpr size_t kHeld = 16384;      // values of a row that a workgroup holds at most
+constexpr size_t kWholeRows = 16;    // of a gate
 constexpr size_t kTeamRows = 128;    // rows that a team adds up at most: sums of more values that are alike are rounded the same way for long
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -57,9 +58,9 @@ __device__ __forceinline__ float lanes_sum(float v)
 }
 
 struct Norms {
-    size_t rows;
+    unsigned rows;
     int cols;
-    size_t per_gate;     // consecutive rows with one gate; 0: there is none
+    unsigned per_gate;   // consecutive rows with one gate; 0: there is none
     int post, pre;
     float eps, scale;
     const float *x, *branch, *gate, *ps, *pb, *qs, *qb;
@@ -78,18 +79,18 @@ enum Kind { kPreScale, kPreBias, kPostScale, kPostBias, kKinds };
 // A workgroup's rows: of a gate's rows one of `splits` runs; or, where kWhole, `gates` whole gates.  Its teams take every teams-th row of
 // a run, or every teams-th gate.
 struct Runs {
-    size_t count, rows, per_gate, splits, gates;
-    __device__ __forceinline__ size_t gate_of(size_t run) const { return run / splits; }
-    __device__ __forceinline__ void range(size_t run, size_t &from, size_t &to) const
+    unsigned count, rows, per_gate, splits, gates;
+    __device__ __forceinline__ unsigned gate_of(unsigned run) const { return run / splits; }
+    __device__ __forceinline__ void range(unsigned run, unsigned &from, unsigned &to) const
     {
         if (gates) {
-            from = min(rows, run * gates * per_gate);
-            to = min(rows, from + gates * per_gate);
+            from = (unsigned)min((size_t)rows, (size_t)run * gates * per_gate);
+            to = (unsigned)min((size_t)rows, from + (size_t)gates * per_gate);
             return;
         }
-        const size_t first = run / splits * per_gate, part = run % splits;
-        from = first + per_gate * part / splits;
-        to = first + per_gate * (part + 1) / splits;
+        const unsigned first = run / splits * per_gate, part = run % splits;
+        from = first + (unsigned)((size_t)per_gate * part / splits);
+        to = first + (unsigned)((size_t)per_gate * (part + 1) / splits);
     }
 };
 
@@ -196,23 +197,47 @@ __device__ __forceinline__ void load_row(const float *p, float missing, int lane
 template <int kLanes, int Q>
 __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
 {
+    constexpr bool kHeldScales = kLanes || Q < 4;   // in registers; else read from the L2 for each row
+    constexpr bool kAhead = !kLanes;                // the next row is on its way while one is worked on
     __shared__ float red[64];
     Team<kLanes> team{red, (int)blockDim.x >> 6};
     const int lane = team.lane(), lanes = team.lanes(), cols = n.cols;
-    v4f gate[Q], ps[Q], pb[Q], qs[Q], qb[Q];
-    load_row(n.ps, 1.0f, lane, lanes, cols, ps);
-    load_row(n.pb, 0.0f, lane, lanes, cols, pb);
-    load_row(n.qs, 1.0f, lane, lanes, cols, qs);
-    load_row(n.qb, 0.0f, lane, lanes, cols, qb);
-    const bool one_gate = n.per_gate == 0 || n.per_gate == n.rows;
+    constexpr int H = kHeldScales ? Q : 1;
+    v4f ps[H], pb[H], qs[H], qb[H], gate[Q];
+    if constexpr (kHeldScales) {
+        load_row(n.ps, 1.0f, lane, lanes, cols, ps);
+        load_row(n.pb, 0.0f, lane, lanes, cols, pb);
+        load_row(n.qs, 1.0f, lane, lanes, cols, qs);
+        load_row(n.qb, 0.0f, lane, lanes, cols, qb);
+    }
+    auto held = [&](const v4f(&v)[H], const float *p, float missing, int i) {
+        if constexpr (kHeldScales) return v[i];
+        else return p ? load_quad(p, 4 * (lane + i * lanes), cols) : splat(missing);
+    };
+    const bool one_gate = kHeldScales && (n.per_gate == 0 || n.per_gate == n.rows);
     if (one_gate) load_row(n.gate, 1.0f, lane, lanes, cols, gate);
-    const size_t first = (size_t)blockIdx.x * team.teams() + team.index();
-    for (size_t r = first; r < n.rows; r += (size_t)gridDim.x * team.teams()) {
+    const unsigned step = gridDim.x * team.teams();
+    const unsigned first = blockIdx.x * team.teams() + team.index();
+    auto fetch = [&](unsigned r, v4f(&x)[Q], v4f(&v)[Q]) {
         const size_t at = r * (size_t)cols;
-        v4f x[Q], v[Q];
         load_row(n.branch ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, v);
         load_row(n.x ? n.x + at : nullptr, 0.0f, lane, lanes, cols, x);
-        if (!one_gate) load_row(n.gate + r / n.per_gate * (size_t)cols, 1.0f, lane, lanes, cols, gate);
+    };
+    v4f x[Q], v[Q], x_ahead[Q], v_ahead[Q];
+    if (kAhead && first < n.rows) fetch(first, x_ahead, v_ahead);
+    for (unsigned r = first; r < n.rows; r += step) {
+        const size_t at = r * (size_t)cols;
+        if (kAhead) {
+#pragma unroll
+            for (int i = 0; i < Q; i++) {
+                x[i] = x_ahead[i];
+                v[i] = v_ahead[i];
+            }
+            if (r + step < n.rows) fetch(r + step, x_ahead, v_ahead);
+        } else {
+            fetch(r, x, v);
+        }
+        if (!one_gate) load_row(n.gate ? n.gate + (n.per_gate ? r / n.per_gate : 0) * (size_t)cols : nullptr, 1.0f, lane, lanes, cols, gate);
         if (n.post) {
             float mean, rstd;
             row_stats(team, v, n.post, cols, n.eps, mean, rstd);
@@ -221,7 +246,7 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
                 n.rb[r] = rstd;
             }
 #pragma unroll
-            for (int i = 0; i < Q; i++) v[i] = (v[i] - splat(mean)) * splat(rstd) * ps[i] + pb[i];
+            for (int i = 0; i < Q; i++) v[i] = (v[i] - splat(mean)) * splat(rstd) * held(ps, n.ps, 1.0f, i) + held(pb, n.pb, 0.0f, i);
         }
 #pragma unroll
         for (int i = 0; i < Q; i++) {
@@ -238,14 +263,14 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
         }
 #pragma unroll
         for (int i = 0; i < Q; i++)
-            store_quad(n.h + at, 4 * (lane + i * lanes), cols, (v[i] - splat(mean)) * splat(rstd) * qs[i] + qb[i]);
+            store_quad(n.h + at, 4 * (lane + i * lanes), cols, (v[i] - splat(mean)) * splat(rstd) * held(qs, n.qs, 1.0f, i) + held(qb, n.qb, 0.0f, i));
     }
 }
 
 struct RowStats {
     float mb, rb, my, ry;
 };
-__device__ __forceinline__ RowStats stats_of(const Norms &n, size_t r)
+__device__ __forceinline__ RowStats stats_of(const Norms &n, unsigned r)
 {
     RowStats s{0.0f, 1.0f, 0.0f, 1.0f};
     if (n.post) {
@@ -281,19 +306,29 @@ __device__ __forceinline__ void store_row(float *to, int lane, int lanes, int co
     for (int i = 0; i < Q; i++) store_quad(to, 4 * (lane + i * lanes), cols, v[i]);
 }
 
+// What a thread has of a row.
+template <int Q>
+struct Row {
+    v4f t[Q], e[Q], y[Q], z[Q];
+    RowStats s;
+};
+
 // Within a gate's rows the sums of t zb and of t are all that the branch's columns need: dps = gate a, dpb = gate b, dgate = ps a + pb b.
 // Scales lie in LDS where they fit (kStaged), for the registers' sake.
-template <int kLanes, int Q, bool kWhole, bool kStaged>
-__global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, Runs runs, int waves)
+template <int kLanes, int Q, bool kWhole, int kThreads>
+__global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int waves)
 {
+    constexpr bool kStaged = kLanes || Q < 4;
+    constexpr bool kAhead = kLanes ? Q <= 2 : kThreads <= 768;   // the next row is on its way while one is worked on
+    constexpr bool kSumsInLds = !kLanes && Q == 4;               // those of dh: the registers hold the others
     __shared__ float red[64];
     extern __shared__ __attribute__((aligned(16))) float lds[];
     Team<kLanes> team{red, waves};
     const Norms &n = g.n;
     const int lane = team.lane(), lanes = team.lanes(), cols = n.cols, width = 4 * lanes * Q;
     const float over = 1.0f / (float)cols;
-    const size_t run = blockIdx.x;
-    size_t from, to;
+    const unsigned run = blockIdx.x;
+    unsigned from, to;
     runs.range(run, from, to);
     const float *gate = n.gate ? n.gate + (kWhole ? 0 : runs.gate_of(run)) * (size_t)cols : nullptr;
     if constexpr (kStaged) {
@@ -310,37 +345,61 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, R
     };
     auto gates = [&](int col) { return kWhole ? gate ? load_quad(gate, col, cols) : splat(1.0f) : scale(gate, 2, col); };
 
-    v4f dqs[Q], dqb[Q], a[Q], b[Q], dps[kWhole ? Q : 1], dpb[kWhole ? Q : 1];
+    constexpr int S = kSumsInLds ? 1 : Q;
+    v4f dqs[S], dqb[S], a[Q], b[Q], dps[kWhole ? Q : 1], dpb[kWhole ? Q : 1];
+    v4f *const apart = (v4f *)lds + lane;   // dqs and dqb of the thread, where they are in LDS
 #pragma unroll
-    for (int i = 0; i < Q; i++) dqs[i] = dqb[i] = a[i] = b[i] = splat(0.0f);
+    for (int i = 0; i < Q; i++) {
+        a[i] = b[i] = splat(0.0f);
+        if constexpr (kSumsInLds) apart[i * lanes] = apart[(Q + i) * lanes] = splat(0.0f);
+        else dqs[i] = dqb[i] = splat(0.0f);
+    }
     if (kWhole) {
 #pragma unroll
         for (int i = 0; i < Q; i++) dps[i] = dpb[i] = splat(0.0f);
     }
     const int teams = team.teams();
-    const size_t mine = team.index();
-    size_t r = kWhole ? from + mine * runs.per_gate : from + mine;
-    size_t left = runs.per_gate;   // kWhole: rows of this gate that are left
-    const size_t turns = kWhole ? (runs.gates + teams - 1) / teams * runs.per_gate : (to - from + teams - 1) / teams;
-    for (size_t turn = 0; turn < turns; turn++) {
-        const bool live = r < to;   // (a team without a row keeps the others company)
-        const size_t at = live ? r * (size_t)cols : 0;
-        v4f t[Q], e[Q], y[Q], z[Q];
-        load_row(live && g.dy ? g.dy + at : nullptr, 0.0f, lane, lanes, cols, t);
-        load_row(live && n.branch && (n.post || gate) ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, z);
+    const unsigned mine = team.index();
+    unsigned r = kWhole ? from + mine * runs.per_gate : from + mine;   // (beyond the rows by fewer than 2^12: 32 bits hold it)
+    unsigned left = runs.per_gate;   // kWhole: rows of this gate that are left
+    const unsigned turns = kWhole ? (runs.gates + teams - 1) / teams * runs.per_gate : (to - from + teams - 1) / teams;
+    auto fetch = [&](unsigned row, Row<Q> &v) {   // (a team without a row keeps the others company)
+        const bool live = row < to;
+        const size_t at = live ? row * (size_t)cols : 0;
+        load_row(live && g.dy ? g.dy + at : nullptr, 0.0f, lane, lanes, cols, v.t);
+        load_row(live && n.branch && (n.post || gate) ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, v.z);
         if (n.pre) {
-            load_row(live ? g.dh + at : nullptr, 0.0f, lane, lanes, cols, e);
-            load_row(live ? n.y + at : nullptr, 0.0f, lane, lanes, cols, y);
+            load_row(live ? g.dh + at : nullptr, 0.0f, lane, lanes, cols, v.e);
+            load_row(live ? n.y + at : nullptr, 0.0f, lane, lanes, cols, v.y);
         }
-        RowStats s{0.0f, 1.0f, 0.0f, 1.0f};
-        if (live) s = stats_of(n, r);
+        v.s = RowStats{0.0f, 1.0f, 0.0f, 1.0f};
+        if (live) v.s = stats_of(n, row);
+    };
+    Row<Q> v, ahead;
+    if (kAhead && turns) fetch(r, ahead);
+    for (unsigned turn = 0; turn < turns; turn++) {
+        const bool live = r < to;
+        const size_t at = live ? r * (size_t)cols : 0;
+        if (kAhead) {
+            v = ahead;
+            if (turn + 1 < turns) fetch(!kWhole ? r + teams : left > 1 ? r + 1 : r + 1 + (teams - 1) * runs.per_gate, ahead);
+        } else {
+            fetch(r, v);
+        }
+        v4f(&t)[Q] = v.t, (&e)[Q] = v.e, (&y)[Q] = v.y, (&z)[Q] = v.z;
+        const RowStats s = v.s;
         if (n.pre) {
             float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
             for (int i = 0; i < Q; i++) {
                 y[i] = inside((y[i] - splat(s.my)) * splat(s.ry), 4 * (lane + i * lanes), cols);
-                dqb[i] += e[i];
-                dqs[i] += e[i] * y[i];
+                if constexpr (kSumsInLds) {
+                    apart[i * lanes] += e[i] * y[i];
+                    apart[(Q + i) * lanes] += e[i];
+                } else {
+                    dqb[i] += e[i];
+                    dqs[i] += e[i] * y[i];
+                }
                 e[i] *= scale(n.qs, 0, 4 * (lane + i * lanes));
                 s1 += sum4(e[i]);
                 s2 += sum4(e[i] * y[i]);
@@ -396,18 +455,20 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, R
             r += (teams - 1) * runs.per_gate;
         }
     }
-    float *sums = g.sums + run * cols;
+    float *sums = g.sums + run * (size_t)cols;
     const size_t next = (size_t)gridDim.x * cols;
-    if (g.kinds >> kPreScale & 1) {
-        join_teams(team, dqs, lds + 3 * width, lane, lanes);
-        if (mine == 0) store_row(sums, lane, lanes, cols, dqs);
+    auto put = [&](v4f(&v)[S], int in_lds) {
+        if constexpr (kSumsInLds) {   // (a team by itself)
+#pragma unroll
+            for (int i = 0; i < Q; i++) store_quad(sums, 4 * (lane + i * lanes), cols, apart[(in_lds + i) * lanes]);
+        } else {
+            join_teams(team, v, lds + 3 * width, lane, lanes);
+            if (mine == 0) store_row(sums, lane, lanes, cols, v);
+        }
         sums += next;
-    }
-    if (g.kinds >> kPreBias & 1) {
-        join_teams(team, dqb, lds + 3 * width, lane, lanes);
-        if (mine == 0) store_row(sums, lane, lanes, cols, dqb);
-        sums += next;
-    }
+    };
+    if (g.kinds >> kPreScale & 1) put(dqs, 0);
+    if (g.kinds >> kPreBias & 1) put(dqb, Q);
     const bool of_gate = !kWhole && g.dgate;
     if (!(g.kinds >> kPostScale) && !of_gate) return;
     if (kWhole) {
@@ -434,7 +495,7 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_grad_k(Grads g, R
             at += next;
         }
         if (of_gate)
-            store_quad(runs.splits == 1 ? g.dgate + run * cols : at, col, cols,
+            store_quad(runs.splits == 1 ? g.dgate + run * (size_t)cols : at, col, cols,
                        scale(n.ps, 1, col) * a[i] + (n.pb ? load_quad(n.pb, col, cols) * b[i] : splat(0.0f)));
     }
 }
@@ -468,7 +529,7 @@ __global__ __launch_bounds__(kLong) void join_long_k(Norms n)
         }
         rstd = 1.0f / sqrtf(team.sum(all) / count + n.eps);
     };
-    for (size_t r = blockIdx.x; r < n.rows; r += gridDim.x) {
+    for (unsigned r = blockIdx.x; r < n.rows; r += gridDim.x) {
         const size_t at = r * (size_t)n.cols;
         const float *const gate = n.gate ? n.gate + r / n.per_gate * (size_t)n.cols : nullptr;
         float mb = 0.0f, rb = 1.0f;
@@ -516,7 +577,7 @@ __global__ __launch_bounds__(kLong) void join_grad_long_k(Grads g, Means *means)
     Team<0> team{red, kLong / 64};
     const Norms &n = g.n;
     const float over = 1.0f / (float)n.cols;
-    for (size_t r = blockIdx.x; r < n.rows; r += gridDim.x) {
+    for (unsigned r = blockIdx.x; r < n.rows; r += gridDim.x) {
         const size_t at = r * (size_t)n.cols;
         const float *const gate = n.gate ? n.gate + r / n.per_gate * (size_t)n.cols : nullptr;
         const RowStats s = stats_of(n, r);
@@ -571,13 +632,13 @@ __global__ __launch_bounds__(kLong) void join_grad_long_k(Grads g, Means *means)
 __global__ __launch_bounds__(kBlock) void join_columns_k(Grads g, Runs runs, const Means *means)
 {
     const Norms &n = g.n;
-    const size_t tiles = ((size_t)n.cols + kBlock - 1) / kBlock, run = blockIdx.x / tiles;
-    const int c = (int)(blockIdx.x % tiles) * kBlock + (int)threadIdx.x;
+    const size_t tiles = ((size_t)n.cols + kBlock - 1) / kBlock, run = blockIdx.x / (unsigned)tiles;
+    const int c = (int)(blockIdx.x % (unsigned)tiles) * kBlock + (int)threadIdx.x;
     if (c >= n.cols || run >= runs.count) return;
-    size_t from, to;
-    runs.range(run, from, to);
+    unsigned from, to;
+    runs.range((unsigned)run, from, to);
     float acc[kKinds] = {0.0f, 0.0f, 0.0f, 0.0f}, sum_gate = 0.0f;
-    for (size_t r = from; r < to; r++) {
+    for (unsigned r = from; r < to; r++) {
         const size_t i = r * (size_t)n.cols + c;
         const RowStats s = stats_of(n, r);
         float zy = 0.0f;
@@ -606,37 +667,45 @@ __global__ __launch_bounds__(kBlock) void join_columns_k(Grads g, Runs runs, con
     if (n.gate && g.dgate && !runs.gates) *(runs.splits == 1 ? g.dgate + run * n.cols + c : sums) = sum_gate;
 }
 
-// Adds the runs: 32 columns of one result by 32 lanes.
+// Adds the runs: 32 columns of one result's row by 32 lanes, or of four rows by eight lanes each where there are few runs.
 struct Fold {
-    const float *from[kKinds + 1];
-    float *to[kKinds + 1];
-    size_t runs[kKinds + 1], rows[kKinds + 1];   // of a result's row; rows of a result
+    struct One {
+        const float *from;
+        float *to;
+        size_t runs, rows;   // of a row of the result; of the result
+        int at_once;         // rows of a workgroup
+        size_t blocks;       // for 32 columns
+    } one[kKinds + 1];
     int n, cols;
     size_t tiles;
 };
 __global__ __launch_bounds__(1024) void join_fold_k(Fold f)
 {
     __shared__ float red[32][33];
-    size_t row = blockIdx.x / f.tiles;
+    size_t block = blockIdx.x / f.tiles;
     int k = 0;
-    while (k + 1 < f.n && row >= f.rows[k]) row -= f.rows[k++];
-    const int c = (int)(blockIdx.x % f.tiles) * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
+    while (k + 1 < f.n && block >= f.one[k].blocks) block -= f.one[k++].blocks;
+    const Fold::One &o = f.one[k];
+    const int lanes = 32 / o.at_once, group = (int)threadIdx.x >> 5, lane = group % lanes;
+    const int c = (int)(blockIdx.x % f.tiles) * 32 + (int)(threadIdx.x & 31);
+    const size_t row = block * o.at_once + group / lanes;
+    const bool in = c < f.cols && row < o.rows;
     float all = 0.0f;
-    if (c < f.cols) {
-        const float *const from = f.from[k] + row * f.runs[k] * f.cols + c;
-        for (size_t i0 = lane; i0 < f.runs[k]; i0 += 64 * 32) {   // sums of 64 values each
+    if (in) {
+        const float *const from = o.from + row * o.runs * f.cols + c;
+        for (size_t i0 = lane; i0 < o.runs; i0 += 64 * lanes) {   // sums of 64 values each
             float s = 0.0f;
-            const size_t end = min(f.runs[k], i0 + 64 * 32);
+            const size_t end = min(o.runs, i0 + 64 * lanes);
 #pragma unroll 8
-            for (size_t i = i0; i < end; i += 32) s += from[i * f.cols];
+            for (size_t i = i0; i < end; i += lanes) s += from[i * f.cols];
             all += s;
         }
     }
-    red[lane][threadIdx.x & 31] = all;
+    red[group][threadIdx.x & 31] = all;
     __syncthreads();
-    if (threadIdx.x >= 32 || c >= f.cols) return;
-    for (int i = 1; i < 32; i++) all += red[i][threadIdx.x];
-    f.to[k][row * f.cols + c] = all;
+    if (lane || !in) return;
+    for (int i = 1; i < lanes; i++) all += red[group + i][threadIdx.x & 31];
+    o.to[row * f.cols + c] = all;
 }
 
 // Which kernel holds a row: lanes of a wavefront (0: a workgroup) and quads of a lane.
@@ -652,8 +721,12 @@ Form form_of(size_t cols)
     if (quads <= 64) return Form{64, 1, kBlock};
     if (quads <= 128) return Form{64, 2, kBlock};
     if (quads <= 256) return Form{64, 4, kBlock};
-    if (quads <= 2048) return Form{0, 2, (unsigned)(64 * ceil_div(quads, (size_t)128))};
-    return Form{0, 4, (unsigned)(64 * ceil_div(quads, (size_t)256))};
+    // wavefronts in numbers that a CU's four SIMDs share evenly, by themselves or with the teams that a workgroup has of them
+    if (quads <= 2048) {
+        const unsigned waves = (unsigned)ceil_div(quads, (size_t)128);
+        return Form{0, 2, 64 * (waves <= 4 ? waves : waves <= 6 ? 6 : waves <= 8 ? 8 : waves <= 12 ? 12 : 16)};
+    }
+    return Form{0, 4, quads <= 256 * 12 ? 768u : 1024u};
 }
 template <class F>
 void with_form(const Form &f, F &&call)
@@ -668,17 +741,38 @@ void with_form(const Form &f, F &&call)
     else call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 4>{}));
 }
 
-template <int kLanes, int Q, bool kWhole, bool kStaged>
-int launch_grad(unsigned blocks, unsigned threads, size_t lds, const Grads &g, const Runs &runs, int waves)
+// How many workgroups of a kernel the chip holds at a time (0: the runtime does not say).  Asked once for each number of wavefronts.
+template <class K>
+size_t places_of(K kernel, unsigned threads, size_t lds)
 {
-    const auto kernel = join_grad_k<kLanes, Q, kWhole, kStaged>;
+    static size_t known[17] = {};
+    size_t &places = known[threads / 64];
+    if (!places) {
+        int of_cu = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&of_cu, reinterpret_cast<const void *>(kernel), (int)threads, lds) != hipSuccess) {
+            (void)hipGetLastError();
+            of_cu = 0;
+        }
+        places = (size_t)num_cus() * (size_t)std::max(1, of_cu);
+    }
+    return places;
+}
+
+struct Launch {
+    const void *kernel;
+    unsigned threads;
+    size_t lds, places;
+};
+template <int kLanes, int Q, bool kWhole, int kThreads>
+int grad_launch(unsigned threads, size_t lds, Launch *l)
+{
+    const auto kernel = join_grad_k<kLanes, Q, kWhole, kThreads>;
     static bool raised = false;
     if (!raised && lds > 65536 - 1024) {
         DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 159 * 1024));
         raised = true;
     }
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), lds, stream(), g, runs, waves);
-    DOPT_LAUNCH_CHECK();
+    *l = Launch{(const void *)kernel, threads, lds, places_of(kernel, threads, lds)};
     return DOPT_HIP_OK;
 }
 
@@ -740,9 +834,9 @@ int dopt_hip_residual_norm(const dopt_hip_residual_norm_desc *d, const float *x,
     }
     DOPT_ENSURE_INIT();
     Norms n{};
-    n.rows = d->rows;
+    n.rows = (unsigned)d->rows;
     n.cols = (int)d->cols;
-    n.per_gate = d->gates ? d->rows / d->gates : 0;
+    n.per_gate = d->gates ? (unsigned)(d->rows / d->gates) : 0;
     n.post = d->post;
     n.pre = d->pre;
     n.eps = d->eps;
@@ -757,14 +851,16 @@ int dopt_hip_residual_norm(const dopt_hip_residual_norm_desc *d, const float *x,
     n.y = y;
     n.h = h;
     place_stats(d, stats, &n);
-    const size_t most = (size_t)num_cus() * 8;
     if (d->cols > kHeld) {
-        hipLaunchKernelGGL(join_long_k, dim3((unsigned)std::min(d->rows, most)), dim3(kLong), 0, stream(), n);
+        hipLaunchKernelGGL(join_long_k, dim3((unsigned)std::min(d->rows, (size_t)num_cus() * 8)), dim3(kLong), 0, stream(), n);
     } else {
         const Form form = form_of(d->cols);
         const size_t blocks = form.lanes ? ceil_div(d->rows, (size_t)(kBlock / form.lanes)) : d->rows;
         with_form(form, [&](auto lanes, auto quads) {
-            hipLaunchKernelGGL((join_k<lanes.value, quads.value>), dim3((unsigned)std::min(blocks, most)), dim3(form.threads), 0, stream(), n);
+            const auto kernel = join_k<lanes.value, quads.value>;
+            // every workgroup loads the scales once: no more of them than run at a time, and as many rows for each
+            const size_t rounds = ceil_div(blocks, places_of(kernel, form.threads, 0));
+            hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(blocks, rounds)), dim3(form.threads), 0, stream(), n);
         });
     }
     DOPT_LAUNCH_CHECK();
@@ -796,9 +892,9 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     DOPT_ENSURE_INIT();
     Grads g{};
     Norms &n = g.n;
-    n.rows = d->rows;
+    n.rows = (unsigned)d->rows;
     n.cols = (int)d->cols;
-    n.per_gate = d->gates ? d->rows / d->gates : 0;
+    n.per_gate = d->gates ? (unsigned)(d->rows / d->gates) : 0;
     n.post = d->post;
     n.pre = d->pre;
     n.scale = d->residual_scale;
@@ -819,23 +915,48 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
 
     const bool held = d->cols <= kHeld;
     const Form form = form_of(std::min(d->cols, kHeld));
-    // Teams of a workgroup: of several wavefronts each, as many as make half of the largest one.
+    // Teams of a workgroup: of three wavefronts four, of four and six two.
     const int waves = (int)form.threads / 64;
-    const size_t teams = !held ? 1 : form.lanes ? (size_t)(kBlock / form.lanes) : std::max(1, 8 / waves);
+    const size_t teams = !held ? 1 : form.lanes ? (size_t)(kBlock / form.lanes) : waves == 3 ? 4 : waves <= 6 ? 2 : 1;
     const unsigned threads = form.lanes ? form.threads : form.threads * (unsigned)teams;
-    // As many runs as there are workgroups on the chip at a time, of a few rows for each team at least, so that their sums stay small beside
-    // the rows.  Gates of a few rows go to teams as a whole.
-    const unsigned at_a_time = form.lanes ? form.quads == 4 ? 512 : form.quads == 2 ? 1024 : 1536 : 1024;   // threads of a CU, by their registers
-    const size_t places = (size_t)num_cus() * std::max(1u, at_a_time / threads);
-    const size_t wanted = std::min(kTeamRows * teams, std::max(4 * teams, ceil_div(std::max(d->rows, (size_t)1), places)));
-    Runs runs{0, d->rows, n.per_gate ? n.per_gate : std::max(d->rows, (size_t)1), 1, 0};
+    const size_t width = 4 * (form.lanes ? (size_t)form.lanes : (size_t)form.threads) * form.quads;
+    const bool staged = form.lanes || form.quads < 4;
+    const size_t lds = (staged ? 3 + (teams > 1 ? teams : 0) : 2) * width * f;   // scales and what teams add, or sums
+    Runs runs{0, (unsigned)d->rows, n.per_gate ? n.per_gate : (unsigned)std::max(d->rows, (size_t)1), 1, 0};
+    Launch launch{nullptr, kBlock, 0, (size_t)num_cus() * 8};
+    // Gates of fewer rows than this go to teams as a whole.
+    const bool whole = d->gates && runs.per_gate < std::min(kWholeRows, 4 * teams);
+    if (held) {
+        int rc = DOPT_HIP_OK;
+        with_form(form, [&](auto lanes, auto quads) {
+            auto with = [&](auto most) {
+                rc = whole ? grad_launch<lanes.value, quads.value, true, most.value>(threads, lds, &launch)
+                           : grad_launch<lanes.value, quads.value, false, most.value>(threads, lds, &launch);
+            };
+            if constexpr (lanes.value) with(std::integral_constant<int, kBlock>{});
+            else if (threads <= 768 && quads.value == 2) with(std::integral_constant<int, quads.value == 2 ? 768 : 1024>{});
+            else with(std::integral_constant<int, 1024>{});
+        });
+        if (rc) return rc;
+    }
     if (d->rows) {
-        if (d->gates && runs.per_gate < std::min(wanted, (size_t)16)) {
-            runs.gates = ceil_div(ceil_div(wanted, runs.per_gate), teams) * teams;
-            runs.count = ceil_div(d->gates, runs.gates);
+        const size_t gates = std::max(d->gates, (size_t)1);
+        if (whole) {
+            const size_t most = std::max((size_t)1, kTeamRows / runs.per_gate);   // gates of a team
+            runs.gates = (unsigned)(std::min(most, ceil_div(gates, launch.places * teams)) * teams);
+            runs.count = (unsigned)ceil_div(gates, (size_t)runs.gates);
         } else {
-            runs.splits = ceil_div(runs.per_gate, wanted);
-            runs.count = std::max(d->gates, (size_t)1) * runs.splits;
+            // One to three rounds of all places, whichever leaves the fewest turns of a team; a workgroup's beginning and end cost some two of them.
+            const size_t least = ceil_div((size_t)runs.per_gate, kTeamRows * teams), most = ceil_div((size_t)runs.per_gate, 2 * teams);
+            size_t best = 0;
+            for (size_t rounds = 1; rounds <= 3; rounds++) {
+                const size_t splits = std::max(least, std::min(most, std::max((size_t)1, rounds * launch.places / gates)));
+                const size_t turns = ceil_div(gates * splits, launch.places) * (ceil_div(ceil_div((size_t)runs.per_gate, splits), teams) + 2);
+                if (best && turns >= best) continue;
+                best = turns;
+                runs.splits = (unsigned)splits;
+            }
+            runs.count = (unsigned)std::min(gates * runs.splits, (size_t)1 << 31);
         }
     }
     const size_t blocks = runs.count, kinds = (size_t)__builtin_popcount((unsigned)g.kinds);
@@ -846,15 +967,9 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     if (sums + means && !scratch) return DOPT_HIP_ERR_OOM;
     g.sums = (float *)(scratch + means);
     if (d->rows && held) {
-        int rc = DOPT_HIP_OK;
-        with_form(form, [&](auto lanes, auto quads) {
-            constexpr bool kStaged = lanes.value || quads.value < 4;
-            const size_t width = 4 * (lanes.value ? (size_t)lanes.value : (size_t)form.threads) * quads.value;
-            const size_t bytes = (3 + (teams > 1 ? teams : 0)) * width * f;
-            rc = runs.gates ? launch_grad<lanes.value, quads.value, true, kStaged>((unsigned)blocks, threads, kStaged ? bytes : 0, g, runs, waves)
-                            : launch_grad<lanes.value, quads.value, false, kStaged>((unsigned)blocks, threads, kStaged ? bytes : 0, g, runs, waves);
-        });
-        if (rc) return rc;
+        int of_team = waves;
+        void *arguments[] = {&g, &runs, &of_team};
+        DOPT_HIP_CHECK(hipLaunchKernel(launch.kernel, dim3((unsigned)blocks), dim3(launch.threads), arguments, launch.lds, stream()));
     } else if (d->rows) {
         hipLaunchKernelGGL(join_grad_long_k, dim3((unsigned)std::min(d->rows, (size_t)num_cus() * 8)), dim3(kLong), 0, stream(), g, (Means *)scratch);
         const size_t tiles = ceil_div(d->cols, (size_t)kBlock);
@@ -865,13 +980,12 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     Fold fold{};
     fold.cols = (int)d->cols;
     fold.tiles = ceil_div(d->cols, (size_t)32);
-    size_t rows = 0;
-    auto add = [&](const float *from, float *to, size_t count, size_t results_rows) {
-        fold.from[fold.n] = from;
-        fold.to[fold.n] = to;
-        fold.runs[fold.n] = count;
-        fold.rows[fold.n++] = results_rows;
-        rows += results_rows;
+    size_t fold_blocks = 0;
+    auto add = [&](const float *from, float *to, size_t count, size_t rows) {
+        const int at_once = rows > 1 && count <= 64 ? 4 : 1;
+        const size_t of_it = ceil_div(rows, (size_t)at_once);
+        fold.one[fold.n++] = Fold::One{from, to, count, rows, at_once, of_it};
+        fold_blocks += of_it;
     };
     const float *at = g.sums;
     for (int k = 0; k < kKinds; k++)
@@ -880,9 +994,9 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
             at += blocks * d->cols;
         }
     if (gate_sums && d->gates) add(at, dgate, d->rows ? runs.splits : 0, d->gates);
-    if (!rows) return DOPT_HIP_OK;
-    DOPT_REQUIRE(rows * fold.tiles < (size_t)1 << 22, "%s: dimensions too large", who);
-    hipLaunchKernelGGL(join_fold_k, dim3((unsigned)(rows * fold.tiles)), dim3(1024), 0, stream(), fold);
+    if (!fold_blocks) return DOPT_HIP_OK;
+    DOPT_REQUIRE(fold_blocks * fold.tiles < (size_t)1 << 22, "%s: dimensions too large", who);
+    hipLaunchKernelGGL(join_fold_k, dim3((unsigned)(fold_blocks * fold.tiles)), dim3(1024), 0, stream(), fold);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
