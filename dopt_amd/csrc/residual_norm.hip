@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "mfma_core.h"
 
 namespace {
 
@@ -71,8 +72,8 @@ struct Grads {
     Norms n;             // y and branch as the forward pass read and left them; statistics as it left them
     const float *dy, *dh;
     float *dx, *db, *dgate;
-    float *sums;         // of each block: kinds x cols, see Kind; then the gate's, cols for each run
-    int kinds;           // a bit for each kind that is wanted
+    float *sums[4];      // by Kind, a row for each run, null where not wanted: scratch, or the result itself where there is one run
+    float *gate_sums;    // likewise of the gate, where its rows are several runs
 };
 enum Kind { kPreScale, kPreBias, kPostScale, kPostBias, kKinds };
 
@@ -137,7 +138,7 @@ struct Team {
     __device__ __forceinline__ int lanes() const { return kWide ? 64 * waves : kLanes; }
     __device__ __forceinline__ int index() const { return kWide ? (int)threadIdx.x / lanes() : (int)threadIdx.x / (kLanes ? kLanes : 1); }
     __device__ __forceinline__ int lane() const { return kWide ? (int)threadIdx.x - index() * lanes() : (int)threadIdx.x & (kLanes - 1); }
-    __device__ __forceinline__ int teams() const { return kWide ? (int)blockDim.x / lanes() : kBlock / (kLanes ? kLanes : 1); }
+    __device__ __forceinline__ int teams() const { return (int)blockDim.x / lanes(); }
     __device__ __forceinline__ void sum(float &a, float &b)   // both over the team, in all of its lanes
     {
         a = lanes_sum<kWide ? 64 : kLanes>(a);
@@ -194,11 +195,45 @@ __device__ __forceinline__ void load_row(const float *p, float missing, int lane
     for (int i = 0; i < Q; i++) v[i] = p ? load_quad(p, 4 * (lane + i * lanes), cols) : splat(missing);
 }
 
+// Rows that belong to whole wavefronts go through a buffer resource of the row's bytes: what lies beyond its end reads as zero and is not
+// written, dword by dword (measured), without a branch - with branches one wavefront that stuck out of the row held up all of its
+// workgroup ([2048 x 7936] took 69 us, [2048 x 8192] 57).
+template <bool kWaves, int Q>
+__device__ __forceinline__ void fetch_row(const float *p, int lane, int lanes, int cols, v4f (&v)[Q])   // null: zeros
+{
+    if constexpr (kWaves) {
+        const __amdgpu_buffer_rsrc_t row = make_rsrc(p, p ? (size_t)cols * sizeof(float) : 0);
+#pragma unroll
+        for (int i = 0; i < Q; i++) v[i] = __builtin_bit_cast(v4f, buffer_load_f32x4(row, 16u * (lane + i * lanes), 0));
+    } else {
+        load_row(p, 0.0f, lane, lanes, cols, v);
+    }
+}
+template <bool kWaves, int Q>
+__device__ __forceinline__ void put_row(float *p, int lane, int lanes, int cols, const v4f (&v)[Q])
+{
+    if constexpr (kWaves) {
+        const __amdgpu_buffer_rsrc_t row = make_rsrc(p, (size_t)cols * sizeof(float));
+#pragma unroll
+        for (int i = 0; i < Q; i++) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v[i]), row, 16 * (lane + i * lanes), 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Q; i++) store_quad(p, 4 * (lane + i * lanes), cols, v[i]);
+    }
+}
+// What is the same in all lanes of a team of whole wavefronts, for the scalar registers.
+template <bool kWaves>
+__device__ __forceinline__ unsigned alike(unsigned v)
+{
+    return kWaves ? (unsigned)__builtin_amdgcn_readfirstlane((int)v) : v;
+}
+
 template <int kLanes, int Q>
 __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
 {
     constexpr bool kHeldScales = kLanes || Q < 4;   // in registers; else read from the L2 for each row
     constexpr bool kAhead = !kLanes;                // the next row is on its way while one is worked on
+    constexpr bool kWaves = kLanes == 0 || kLanes == 64;
     __shared__ float red[64];
     Team<kLanes> team{red, (int)blockDim.x >> 6};
     const int lane = team.lane(), lanes = team.lanes(), cols = n.cols;
@@ -217,11 +252,11 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
     const bool one_gate = kHeldScales && (n.per_gate == 0 || n.per_gate == n.rows);
     if (one_gate) load_row(n.gate, 1.0f, lane, lanes, cols, gate);
     const unsigned step = gridDim.x * team.teams();
-    const unsigned first = blockIdx.x * team.teams() + team.index();
+    const unsigned first = alike<kWaves>(blockIdx.x * team.teams() + team.index());
     auto fetch = [&](unsigned r, v4f(&x)[Q], v4f(&v)[Q]) {
         const size_t at = r * (size_t)cols;
-        load_row(n.branch ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, v);
-        load_row(n.x ? n.x + at : nullptr, 0.0f, lane, lanes, cols, x);
+        fetch_row<kWaves>(n.branch ? n.branch + at : nullptr, lane, lanes, cols, v);
+        fetch_row<kWaves>(n.x ? n.x + at : nullptr, lane, lanes, cols, x);
     };
     v4f x[Q], v[Q], x_ahead[Q], v_ahead[Q];
     if (kAhead && first < n.rows) fetch(first, x_ahead, v_ahead);
@@ -237,7 +272,10 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
         } else {
             fetch(r, x, v);
         }
-        if (!one_gate) load_row(n.gate ? n.gate + (n.per_gate ? r / n.per_gate : 0) * (size_t)cols : nullptr, 1.0f, lane, lanes, cols, gate);
+        if (!one_gate) {
+            if (n.gate) fetch_row<kWaves>(n.gate + r / n.per_gate * (size_t)cols, lane, lanes, cols, gate);
+            else load_row(nullptr, 1.0f, lane, lanes, cols, gate);
+        }
         if (n.post) {
             float mean, rstd;
             row_stats(team, v, n.post, cols, n.eps, mean, rstd);
@@ -252,8 +290,8 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
         for (int i = 0; i < Q; i++) {
             const int col = 4 * (lane + i * lanes);
             v[i] = inside(splat(n.scale) * x[i] + gate[i] * v[i], col, cols);
-            if (n.y) store_quad(n.y + at, col, cols, v[i]);
         }
+        if (n.y) put_row<kWaves>(n.y + at, lane, lanes, cols, v);
         if (!n.pre) continue;
         float mean, rstd;
         row_stats(team, v, n.pre, cols, n.eps, mean, rstd);
@@ -262,8 +300,8 @@ __global__ __launch_bounds__(kLanes ? kBlock : 1024) void join_k(Norms n)
             n.ry[r] = rstd;
         }
 #pragma unroll
-        for (int i = 0; i < Q; i++)
-            store_quad(n.h + at, 4 * (lane + i * lanes), cols, (v[i] - splat(mean)) * splat(rstd) * held(qs, n.qs, 1.0f, i) + held(qb, n.qb, 0.0f, i));
+        for (int i = 0; i < Q; i++) v[i] = (v[i] - splat(mean)) * splat(rstd) * held(qs, n.qs, 1.0f, i) + held(qb, n.qb, 0.0f, i);
+        put_row<kWaves>(n.h + at, lane, lanes, cols, v);
     }
 }
 
@@ -320,6 +358,7 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
 {
     constexpr bool kStaged = kLanes || Q < 4;
     constexpr bool kAhead = kLanes ? Q <= 2 : kThreads <= 768;   // the next row is on its way while one is worked on
+    constexpr bool kWaves = kLanes == 0 || kLanes == 64;
     constexpr bool kSumsInLds = !kLanes && Q == 4;               // those of dh: the registers hold the others
     __shared__ float red[64];
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -359,18 +398,18 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
         for (int i = 0; i < Q; i++) dps[i] = dpb[i] = splat(0.0f);
     }
     const int teams = team.teams();
-    const unsigned mine = team.index();
+    const unsigned mine = alike<kWaves>(team.index());
     unsigned r = kWhole ? from + mine * runs.per_gate : from + mine;   // (beyond the rows by fewer than 2^12: 32 bits hold it)
     unsigned left = runs.per_gate;   // kWhole: rows of this gate that are left
     const unsigned turns = kWhole ? (runs.gates + teams - 1) / teams * runs.per_gate : (to - from + teams - 1) / teams;
     auto fetch = [&](unsigned row, Row<Q> &v) {   // (a team without a row keeps the others company)
         const bool live = row < to;
         const size_t at = live ? row * (size_t)cols : 0;
-        load_row(live && g.dy ? g.dy + at : nullptr, 0.0f, lane, lanes, cols, v.t);
-        load_row(live && n.branch && (n.post || gate) ? n.branch + at : nullptr, 0.0f, lane, lanes, cols, v.z);
+        fetch_row<kWaves>(live && g.dy ? g.dy + at : nullptr, lane, lanes, cols, v.t);
+        fetch_row<kWaves>(live && n.branch && (n.post || gate) ? n.branch + at : nullptr, lane, lanes, cols, v.z);
         if (n.pre) {
-            load_row(live ? g.dh + at : nullptr, 0.0f, lane, lanes, cols, v.e);
-            load_row(live ? n.y + at : nullptr, 0.0f, lane, lanes, cols, v.y);
+            fetch_row<kWaves>(live ? g.dh + at : nullptr, lane, lanes, cols, v.e);
+            fetch_row<kWaves>(live ? n.y + at : nullptr, lane, lanes, cols, v.y);
         }
         v.s = RowStats{0.0f, 1.0f, 0.0f, 1.0f};
         if (live) v.s = stats_of(n, row);
@@ -412,10 +451,10 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
         }
 #pragma unroll
         for (int i = 0; i < Q; i++) {
-            const int col = 4 * (lane + i * lanes);
-            t[i] = inside(t[i], col, cols);
-            if (g.dx && live) store_quad(g.dx + at, col, cols, splat(n.scale) * t[i]);
+            t[i] = inside(t[i], 4 * (lane + i * lanes), cols);
+            e[i] = splat(n.scale) * t[i];
         }
+        if (g.dx && live) put_row<kWaves>(g.dx + at, lane, lanes, cols, e);
         if (n.branch) {
             if (kWhole && gate) gate = n.gate + (live ? r / runs.per_gate : 0) * (size_t)cols;
             float s1 = 0.0f, s2 = 0.0f;
@@ -436,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
 #pragma unroll
                 for (int i = 0; i < Q; i++) t[i] = splat(s.rb) * (t[i] - splat(s1) - z[i] * splat(s2));
             }
-            if (g.db && live) store_row(g.db + at, lane, lanes, cols, t);
+            if (g.db && live) put_row<kWaves>(g.db + at, lane, lanes, cols, t);
         }
         r += kWhole ? 1 : teams;
         if (kWhole && --left == 0) {
@@ -455,9 +494,8 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
             r += (teams - 1) * runs.per_gate;
         }
     }
-    float *sums = g.sums + run * (size_t)cols;
-    const size_t next = (size_t)gridDim.x * cols;
-    auto put = [&](v4f(&v)[S], int in_lds) {
+    const size_t place = run * (size_t)cols;
+    auto put = [&](v4f(&v)[S], int in_lds, float *sums) {
         if constexpr (kSumsInLds) {   // (a team by itself)
 #pragma unroll
             for (int i = 0; i < Q; i++) store_quad(sums, 4 * (lane + i * lanes), cols, apart[(in_lds + i) * lanes]);
@@ -465,12 +503,11 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
             join_teams(team, v, lds + 3 * width, lane, lanes);
             if (mine == 0) store_row(sums, lane, lanes, cols, v);
         }
-        sums += next;
     };
-    if (g.kinds >> kPreScale & 1) put(dqs, 0);
-    if (g.kinds >> kPreBias & 1) put(dqb, Q);
+    if (g.sums[kPreScale]) put(dqs, 0, g.sums[kPreScale] + place);
+    if (g.sums[kPreBias]) put(dqb, Q, g.sums[kPreBias] + place);
     const bool of_gate = !kWhole && g.dgate;
-    if (!(g.kinds >> kPostScale) && !of_gate) return;
+    if (!g.sums[kPostScale] && !g.sums[kPostBias] && !of_gate) return;
     if (kWhole) {
 #pragma unroll
         for (int i = 0; i < Q; i++) {
@@ -485,17 +522,10 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
     for (int i = 0; i < Q; i++) {
         const int col = 4 * (lane + i * lanes);
         const v4f g4 = kWhole ? splat(1.0f) : gates(col);
-        float *at = sums;
-        if (g.kinds >> kPostScale & 1) {
-            store_quad(at, col, cols, g4 * a[i]);
-            at += next;
-        }
-        if (g.kinds >> kPostBias & 1) {
-            store_quad(at, col, cols, g4 * b[i]);
-            at += next;
-        }
+        if (g.sums[kPostScale]) store_quad(g.sums[kPostScale] + place, col, cols, g4 * a[i]);
+        if (g.sums[kPostBias]) store_quad(g.sums[kPostBias] + place, col, cols, g4 * b[i]);
         if (of_gate)
-            store_quad(runs.splits == 1 ? g.dgate + run * (size_t)cols : at, col, cols,
+            store_quad((runs.splits == 1 ? g.dgate : g.gate_sums) + place, col, cols,
                        scale(n.ps, 1, col) * a[i] + (n.pb ? load_quad(n.pb, col, cols) * b[i] : splat(0.0f)));
     }
 }
@@ -658,13 +688,10 @@ __global__ __launch_bounds__(kBlock) void join_columns_k(Grads g, Runs runs, con
             sum_gate = 0.0f;
         }
     }
-    float *sums = g.sums + run * n.cols + c;
+    const size_t place = run * (size_t)n.cols + c;
     for (int k = 0; k < kKinds; k++)
-        if (g.kinds >> k & 1) {
-            *sums = acc[k];
-            sums += runs.count * n.cols;
-        }
-    if (n.gate && g.dgate && !runs.gates) *(runs.splits == 1 ? g.dgate + run * n.cols + c : sums) = sum_gate;
+        if (g.sums[k]) g.sums[k][place] = acc[k];
+    if (n.gate && g.dgate && !runs.gates) (runs.splits == 1 ? g.dgate : g.gate_sums)[place] = sum_gate;
 }
 
 // Adds the runs: 32 columns of one result's row by 32 lanes, or of four rows by eight lanes each where there are few runs.
@@ -713,14 +740,14 @@ struct Form {
     int lanes, quads;
     unsigned threads;
 };
-Form form_of(size_t cols)
+Form form_of(size_t cols, bool back)
 {
     const size_t quads = ceil_div(cols, (size_t)4);
     if (quads <= 16) return Form{16, 1, kBlock};
     if (quads <= 32) return Form{32, 1, kBlock};
     if (quads <= 64) return Form{64, 1, kBlock};
-    if (quads <= 128) return Form{64, 2, kBlock};
-    if (quads <= 256) return Form{64, 4, kBlock};
+    if (quads <= 128 && !back) return Form{64, 2, kBlock};
+    if (quads <= 256 && !back) return Form{64, 4, kBlock};   // (of the gradient four quads leave registers for two wavefronts of a SIMD: 105 us for 94)
     // wavefronts in numbers that a CU's four SIMDs share evenly, by themselves or with the teams that a workgroup has of them
     if (quads <= 2048) {
         const unsigned waves = (unsigned)ceil_div(quads, (size_t)128);
@@ -854,7 +881,7 @@ int dopt_hip_residual_norm(const dopt_hip_residual_norm_desc *d, const float *x,
     if (d->cols > kHeld) {
         hipLaunchKernelGGL(join_long_k, dim3((unsigned)std::min(d->rows, (size_t)num_cus() * 8)), dim3(kLong), 0, stream(), n);
     } else {
-        const Form form = form_of(d->cols);
+        const Form form = form_of(d->cols, false);
         const size_t blocks = form.lanes ? ceil_div(d->rows, (size_t)(kBlock / form.lanes)) : d->rows;
         with_form(form, [&](auto lanes, auto quads) {
             const auto kernel = join_k<lanes.value, quads.value>;
@@ -911,14 +938,15 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     g.db = dbranch;
     g.dgate = dgate;
     float *const results[kKinds] = {dpre_scale, dpre_bias, dpost_scale, dpost_bias};
-    for (int k = 0; k < kKinds; k++) g.kinds |= results[k] ? 1 << k : 0;
+    size_t kinds = 0;
+    for (const float *r : results) kinds += r != nullptr;
 
     const bool held = d->cols <= kHeld;
-    const Form form = form_of(std::min(d->cols, kHeld));
-    // Teams of a workgroup: of three wavefronts four, of four and six two.
+    const Form form = form_of(std::min(d->cols, kHeld), true);
+    // Teams of a workgroup: of two wavefronts two, of three four, of six two, so that the SIMDs share them evenly.
     const int waves = (int)form.threads / 64;
-    const size_t teams = !held ? 1 : form.lanes ? (size_t)(kBlock / form.lanes) : waves == 3 ? 4 : waves <= 6 ? 2 : 1;
-    const unsigned threads = form.lanes ? form.threads : form.threads * (unsigned)teams;
+    const size_t teams = !held ? 1 : form.lanes ? (size_t)(768 / form.lanes) : waves > 12 ? 1 : 12 / waves;
+    const unsigned threads = form.lanes ? 768 : form.threads * (unsigned)teams;
     const size_t width = 4 * (form.lanes ? (size_t)form.lanes : (size_t)form.threads) * form.quads;
     const bool staged = form.lanes || form.quads < 4;
     const size_t lds = (staged ? 3 + (teams > 1 ? teams : 0) : 2) * width * f;   // scales and what teams add, or sums
@@ -933,7 +961,7 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
                 rc = whole ? grad_launch<lanes.value, quads.value, true, most.value>(threads, lds, &launch)
                            : grad_launch<lanes.value, quads.value, false, most.value>(threads, lds, &launch);
             };
-            if constexpr (lanes.value) with(std::integral_constant<int, kBlock>{});
+            if constexpr (lanes.value) with(std::integral_constant<int, 768>{});
             else if (threads <= 768 && quads.value == 2) with(std::integral_constant<int, quads.value == 2 ? 768 : 1024>{});
             else with(std::integral_constant<int, 1024>{});
         });
@@ -947,7 +975,8 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
             runs.count = (unsigned)ceil_div(gates, (size_t)runs.gates);
         } else {
             // One to three rounds of all places, whichever leaves the fewest turns of a team; a workgroup's beginning and end cost some two of them.
-            const size_t least = ceil_div((size_t)runs.per_gate, kTeamRows * teams), most = ceil_div((size_t)runs.per_gate, 2 * teams);
+            const size_t least = ceil_div((size_t)runs.per_gate, kTeamRows * teams);
+            const size_t most = ceil_div((size_t)runs.per_gate, (form.lanes ? 6 : 2) * teams);
             size_t best = 0;
             for (size_t rounds = 1; rounds <= 3; rounds++) {
                 const size_t splits = std::max(least, std::min(most, std::max((size_t)1, rounds * launch.places / gates)));
@@ -959,13 +988,21 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
             runs.count = (unsigned)std::min(gates * runs.splits, (size_t)1 << 31);
         }
     }
-    const size_t blocks = runs.count, kinds = (size_t)__builtin_popcount((unsigned)g.kinds);
+    const size_t blocks = runs.count;
     DOPT_REQUIRE(blocks < (size_t)1 << 22, "%s: dimensions too large", who);
     const bool gate_sums = dgate && !runs.gates && (runs.splits > 1 || d->rows == 0);
-    const size_t sums = (kinds * blocks + (gate_sums ? blocks : 0)) * row, means = held ? 0 : ceil_div(d->rows * sizeof(Means), (size_t)256) * 256;
+    const size_t to_add = blocks == 1 ? 0 : kinds;   // (one run's sums are the results)
+    const size_t sums = (to_add + gate_sums) * blocks * row, means = held ? 0 : ceil_div(d->rows * sizeof(Means), (size_t)256) * 256;
     char *const scratch = sums + means ? (char *)workspace(sums + means) : nullptr;
     if (sums + means && !scratch) return DOPT_HIP_ERR_OOM;
-    g.sums = (float *)(scratch + means);
+    float *at = (float *)(scratch + means);
+    for (int k = 0; k < kKinds; k++) {
+        g.sums[k] = results[k];
+        if (!results[k] || !to_add) continue;
+        g.sums[k] = at;
+        at += blocks * d->cols;
+    }
+    g.gate_sums = at;
     if (d->rows && held) {
         int of_team = waves;
         void *arguments[] = {&g, &runs, &of_team};
@@ -987,13 +1024,9 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
         fold.one[fold.n++] = Fold::One{from, to, count, rows, at_once, of_it};
         fold_blocks += of_it;
     };
-    const float *at = g.sums;
     for (int k = 0; k < kKinds; k++)
-        if (results[k]) {
-            add(at, results[k], blocks, 1);
-            at += blocks * d->cols;
-        }
-    if (gate_sums && d->gates) add(at, dgate, d->rows ? runs.splits : 0, d->gates);
+        if (results[k] && to_add) add(g.sums[k], results[k], blocks, 1);
+    if (gate_sums && d->gates) add(g.gate_sums, dgate, d->rows ? runs.splits : 0, d->gates);
     if (!fold_blocks) return DOPT_HIP_OK;
     DOPT_REQUIRE(fold_blocks * fold.tiles < (size_t)1 << 22, "%s: dimensions too large", who);
     hipLaunchKernelGGL(join_fold_k, dim3((unsigned)(fold_blocks * fold.tiles)), dim3(1024), 0, stream(), fold);

@@ -472,38 +472,45 @@ def _row_norm(kind):
     return code
 
 
-@functools.lru_cache(maxsize=4096)
-def _residual_desc(rows, cols, gates, post, pre, eps, residual_scale):
-    return capi.ResidualNormDesc(rows, cols, gates, post, pre, eps, residual_scale)
-
-
 _STATS = (0, 2, 1)   # values of a row by its norm: mean and rstd of the layer norm, rstd alone of the rms norm
 
 
-def _row_stats(rows, post, pre):
-    return rows * (_STATS[post] + _STATS[pre])
-
-
-def _residual_args(like, operands, gate, vectors, post, pre, eps, residual_scale):
-    """The descriptor and the addresses of the optional operands: tensors of like's shape, the gate, one row each."""
-    if len(like.shape) < 1 or like.shape[-1] < 1:
+@functools.lru_cache(maxsize=4096)
+def _residual_desc(shape, gate, post, pre, eps, residual_scale):
+    """The descriptor for operands of that shape, a gate of so many values (or None), and the shape of the statistics."""
+    if not shape or shape[-1] < 1:
         raise capi.HipError(1, "residualNorm: rows of at least one value")
-    cols = like.shape[-1]
-    for t in operands:
-        if t is not None and (t.size != like.size or t.shape[-1:] != like.shape[-1:] or t.dtype != _F32):
-            raise capi.HipError(1, "residualNorm: an operand has the wrong size or type")
-    for t in vectors:
-        if t is not None and (t.size != cols or t.dtype != _F32):
-            raise capi.HipError(1, "residualNorm: a scale or bias has the wrong size or type")
-    if gate is not None and (gate.size % cols or gate.size == 0 or gate.dtype != _F32):
+    cols, rows = shape[-1], _vol(shape[:-1])
+    if gate is not None and (gate % cols or gate == 0):
         raise capi.HipError(1, "residualNorm: the gate has the wrong size or type")
-    rows = like.size // cols
-    return rows, cols, _residual_desc(rows, cols, gate.size // cols if gate is not None else 0, _row_norm(post), _row_norm(pre), eps,
-                                      residual_scale)
+    post, pre = _row_norm(post), _row_norm(pre)
+    d = capi.ResidualNormDesc(rows, cols, 0 if gate is None else gate // cols, post, pre, eps, residual_scale)
+    return d, (rows * (_STATS[post] + _STATS[pre]),)
 
 
-def _ptr(t):
-    return None if t is None else t.ptr
+def _of_shape(t, shape):
+    """The address of an operand that may be missing and else has as many values, in rows as long."""
+    if t is None:
+        return None
+    if t.shape != shape and (t.size != _vol(shape) or t.shape[-1:] != shape[-1:]) or t.dtype is not _F32 and t.dtype != _F32:
+        raise capi.HipError(1, "residualNorm: an operand has the wrong size or type")
+    return t.ptr
+
+
+def _of_row(t, cols):
+    if t is None:
+        return None
+    if t.size != cols or t.dtype is not _F32 and t.dtype != _F32:
+        raise capi.HipError(1, "residualNorm: a scale or bias has the wrong size or type")
+    return t.ptr
+
+
+def _gate_size(gate):
+    if gate is None:
+        return None
+    if gate.dtype is not _F32 and gate.dtype != _F32:
+        raise capi.HipError(1, "residualNorm: the gate has the wrong size or type")
+    return gate.size
 
 
 def residual_norm(x=None, branch=None, gate=None, post="none", post_scale=None, post_bias=None, pre="none", pre_scale=None,
@@ -514,13 +521,16 @@ def residual_norm(x=None, branch=None, gate=None, post="none", post_scale=None, 
     like = x if x is not None else branch
     if like is None:
         raise capi.HipError(1, "residualNorm: neither a stream nor a branch")
-    rows, _, d = _residual_args(like, (x, branch, y, h), gate, (post_scale, post_bias, pre_scale, pre_bias), post, pre, eps, residual_scale)
-    y = _out(y, like.shape)
+    shape = like.shape
+    d, stats_shape = _residual_desc(shape, _gate_size(gate), post, pre, eps, residual_scale)
+    cols = shape[-1]
+    y = _out(y, shape)
     if d.pre:
-        h = _out(h, like.shape)
-    stats = _out(stats, (_row_stats(rows, d.post, d.pre),))
-    _run(capi.load().dopt_hip_residual_norm(C.byref(d), _ptr(x), _ptr(branch), _ptr(gate), _ptr(post_scale), _ptr(post_bias), _ptr(pre_scale),
-                                            _ptr(pre_bias), y.ptr, _ptr(h), stats.ptr or None))
+        h = _out(h, shape)
+    stats = _out(stats, stats_shape)
+    _run(capi.load().dopt_hip_residual_norm(d, _of_shape(x, shape), _of_shape(branch, shape), gate.ptr if gate is not None else None,
+                                            _of_row(post_scale, cols), _of_row(post_bias, cols), _of_row(pre_scale, cols), _of_row(pre_bias, cols),
+                                            y.ptr, _of_shape(h, shape), stats.ptr or None))
     return y, h, stats
 
 
@@ -529,27 +539,31 @@ def residual_norm_grad(dy, dh, y, branch, stats, gate=None, post="none", post_sc
     """The gradients of residual_norm's operands as a dict: dx, and dbranch, dgate, dpost_scale, dpost_bias, dpre_scale, dpre_bias of
     those that are there.  dy: y's gradient from elsewhere, or None with dh.  `out`: tensors for the results that are to be formed (all of
     them where it is None)."""
-    like = next((t for t in (dy, dh, branch) if t is not None), None)
+    like = dy if dy is not None else dh if dh is not None else branch
     if like is None:
         raise capi.HipError(1, "residualNormGrad: no gradient")
-    rows, cols, d = _residual_args(like, (dy, dh, y, branch), gate, (post_scale, post_bias, pre_scale, pre_bias), post, pre, 0.0,
-                                   residual_scale)
-    if d.post or d.pre:
-        if stats is None or stats.size != _row_stats(rows, d.post, d.pre) or stats.dtype != _F32:
-            raise capi.HipError(1, "residualNormGrad: stats holds what residual_norm left of each row")
-    vectors = {"dpost_scale": post_scale, "dpost_bias": post_bias, "dpre_scale": pre_scale, "dpre_bias": pre_bias}
-    shapes = {"dx": like.shape}
-    if branch is not None:
-        shapes["dbranch"] = like.shape
-    if gate is not None:
-        shapes["dgate"] = gate.shape
-    shapes.update({k: v.shape for k, v in vectors.items() if v is not None})
-    if out is not None and not set(out) <= set(shapes):
-        raise capi.HipError(1, "residualNormGrad: there is no %s" % ", ".join(sorted(set(out) - set(shapes))))
-    made = {k: _out(out[k] if out is not None else None, s) for k, s in shapes.items() if out is None or k in out}
+    shape = like.shape
+    d, stats_shape = _residual_desc(shape, _gate_size(gate), post, pre, 0.0, residual_scale)
+    cols = shape[-1]
+    if stats_shape[0] and (stats is None or stats.size != stats_shape[0] or stats.dtype != _F32):
+        raise capi.HipError(1, "residualNormGrad: stats holds what residual_norm left of each row")
+    _of_row(pre_bias, cols)   # (read only for its shape)
+    made = {}
+    there = (("dx", like), ("dbranch", branch), ("dgate", gate), ("dpost_scale", post_scale), ("dpost_bias", post_bias),
+             ("dpre_scale", pre_scale), ("dpre_bias", pre_bias))
+    results = []
+    for name, operand in there:
+        given = None if out is None else out.get(name)
+        if operand is None or (out is not None and given is None):
+            if given is not None:
+                raise capi.HipError(1, "residualNormGrad: there is no %s" % name)
+            results.append(None)
+            continue
+        made[name] = t = _out(given, operand.shape)
+        results.append(t.ptr)
     _run(capi.load().dopt_hip_residual_norm_grad(
-        C.byref(d), _ptr(dy), _ptr(dh), _ptr(y), _ptr(branch), _ptr(gate), _ptr(post_scale), _ptr(post_bias), _ptr(pre_scale), _ptr(stats),
-        *[_ptr(made.get(k)) for k in ("dx", "dbranch", "dgate", "dpost_scale", "dpost_bias", "dpre_scale", "dpre_bias")]))
+        d, _of_shape(dy, shape), _of_shape(dh, shape), _of_shape(y, shape), _of_shape(branch, shape), gate.ptr if gate is not None else None,
+        _of_row(post_scale, cols), _of_row(post_bias, cols), _of_row(pre_scale, cols), stats.ptr if stats_shape[0] else None, *results))
     return made
 
 
