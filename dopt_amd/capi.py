@@ -154,6 +154,8 @@ PROTOTYPES = {
     "dopt_hip_residual_norm_grad": [C.POINTER(ResidualNormDesc)] + [_vp] * 16,
     "dopt_hip_dense_act": [_sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     "dopt_hip_dense_act_grad": [_sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "dopt_hip_dense_groups": [_sz, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "dopt_hip_dense_groups_grad": [_sz, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "dopt_hip_muon_create": [_i, C.POINTER(MatrixRef), C.POINTER(_vp)],
     "dopt_hip_muon_destroy": [_vp],
     "dopt_hip_muon_step": [_vp, _f, _f, _i, _f, _i],

@@ -630,6 +630,59 @@ def denseActGrad(parentGrad, op):
     return Operation("denseActGrad", [parentGrad] + deps, {"activation": a["activation"]})
 
 
+def _group_operands(op, first):
+    """Whether the dependencies from `first` on are x [M, K], w [G, N, K] and G + 1 offsets."""
+    if len(op.deps) < first + 3:
+        return False
+    x, w, offsets = op.deps[first:first + 3]
+    return (x.rank == 2 and w.rank == 3 and x.shape[1] == w.shape[2] and offsets.dtype == int32_t and offsets.volume == w.shape[0] + 1 and
+            op.attributes.get("activation") in capi.ACTIVATIONS.values() and
+            all(d.dtype == float32_t for d in op.deps if d is not offsets))
+
+
+def _verify_dense_groups(op):
+    if not _group_operands(op, 0):
+        return False
+    w = op.deps[1]
+    rest = [w.shape[0] * w.shape[1]] if op.attributes["hasBias"] else []
+    return [d.volume for d in op.deps[3:]] == rest and all(_rows(d, w.shape[0]) for d in op.deps[3:])
+
+
+def _verify_dense_groups_grad(op):
+    if not _group_operands(op, 1):
+        return False
+    v = op.deps[1].shape[0] * op.deps[2].shape[1]
+    return (op.deps[0].volume == v and [d.volume for d in op.deps[4:]] == ([v] if op.attributes["activation"] else []) and
+            all(_rows(d, op.deps[1].shape[0]) for d in op.deps[:1] + op.deps[4:]))
+
+
+register_operation("denseGroups", _verify_dense_groups,
+                   lambda op: (float32_t, ((2 if op.attributes["keepsPre"] else 1) * op.deps[0].shape[0] * op.deps[1].shape[1],)))
+register_operation("denseGroupsGrad", _verify_dense_groups_grad,
+                   lambda op: (float32_t, (op.deps[1].volume + op.deps[2].volume + op.deps[2].shape[0] * op.deps[2].shape[1],)))
+
+
+def denseGroups(input, weights, offsets, bias=None, activation="none", keepPre=True):   # noqa: A002
+    """activation(input . weights[g]^T + bias[g]) for the rows offsets[g] .. offsets[g + 1] - 1 of input, zeros for rows of no group;
+    weights [G, N, K], offsets [G + 1] of int32, bias [G, N].  keepPre as denseAct's.  No gradient of the offsets."""
+    act = _activation(activation)
+    op = Operation("denseGroups", [input, weights, offsets] + ([bias] if bias is not None else []),
+                   {"activation": act, "hasBias": int(bias is not None), "keepsPre": int(bool(keepPre and act))})
+    shape = [input.shape[0], weights.shape[1]]
+    if op.attributes["keepsPre"]:
+        op = slice(op, [0], [shape[0] * shape[1]])
+    return op.reshape(shape)
+
+
+def denseGroupsGrad(parentGrad, op):
+    a, deps, v = op.attributes, list(op.deps[:3]), op.deps[0].shape[0] * op.deps[1].shape[1]
+    if a["activation"]:
+        if not a["keepsPre"]:
+            raise ValueError("The gradient of denseGroups needs keepPre")
+        deps.append(slice(op, [v], [2 * v]))
+    return Operation("denseGroupsGrad", [parentGrad] + deps, {"activation": a["activation"]})
+
+
 # What lies between two blocks of a residual network; "operands" has a bit for each optional one, in this order.
 _JOIN_OPERANDS = ("stream", "branch", "gate", "postScale", "postBias", "preScale", "preBias")
 _JOIN_STATS = (0, 2, 1)   # values of a row by its norm
@@ -894,6 +947,17 @@ def _reg_grads():
         out = parts(denseActGrad(dy, op), op.deps[:2 + op.attributes["hasBias"]])
         return out + ([dy.reshape(op.deps[-1].shape)] if op.attributes["hasResidual"] else [])
     g("denseAct", dense_act_grad)
+
+    def dense_groups_grad(op, pg):
+        x, w = op.deps[:2]
+        dy = slice(pg, [0], [x.shape[0] * w.shape[1]]) if op.attributes["keepsPre"] else pg
+        packed, v = denseGroupsGrad(dy, op), x.volume + w.volume
+        out = parts(packed, [x, w])
+        if not op.attributes["hasBias"]:
+            return out
+        bias = op.deps[3]
+        return out + [None, slice(packed, [v], [v + bias.volume]).reshape(bias.shape)]   # (none of the offsets)
+    g("denseGroups", dense_groups_grad)
     g("residualNorm", lambda op, pg: parts(residualNormGrad(pg, op), op.deps))
 
 
@@ -914,6 +978,8 @@ def grad(objective, wrt):
         if fn is None or op_grad is None:
             continue
         for d, g in zip(op.deps, fn(op, op_grad)):
+            if g is None:
+                continue
             cur = grads.get(id(d))
             grads[id(d)] = g if cur is None else cur + g
     for i, w in enumerate(wrt):

@@ -1,0 +1,295 @@
+// Dense layers whose rows fall into groups of consecutive rows with a weight matrix and a bias of their own, forward and backward: the
+// layers of experts, domains or heads, where the sizes of the groups are known to the device alone.  No counterpart in the reference
+// (its one dense layer is nnet/source/dopt/nnet/layers/dense.d).
+//
+//     rows o[g] .. o[g + 1] - 1:  pre = x w_g^T + bias_g,  y = act(pre);  rows of no group: zeros
+//     dz = dy act'(pre),  dx = dz w_g,  dw_g = dz^T x and dbias_g = column sums of dz over the group's rows;  dx of no group's rows: zeros
+//
+// A workgroup finds its rows in the offsets itself: the grid has room for any sizes, workgroups beyond what there is end at once.
+#include <algorithm>
+
+#include "common.h"
+#include "dense.h"
+#include "groups.h"
+#include "small_product.h"
+
+namespace {
+
+using namespace dopt;
+
+constexpr int kTileShift = 5;    // rows of a tile: 32
+constexpr int kRunShift = 6;     // rows that a thread adds up for dbias before it rounds to memory: 64
+constexpr unsigned kGridRow = 65535;   // units along the second side of a grid; more go to the third
+
+__device__ __forceinline__ unsigned unit_id() { return blockIdx.z * kGridRow + blockIdx.y; }
+// x: as many as there are tiles side by side, a multiple of eight, so that a tile of columns - and what it reads of a weight - stays on one XCD
+dim3 grid_of(size_t tiles, size_t units)
+{
+    const size_t x = ceil_div(tiles, (size_t)8) * 8;
+    return dim3((unsigned)x, (unsigned)std::min(units, (size_t)kGridRow), (unsigned)ceil_div(units, (size_t)kGridRow));
+}
+
+struct Layer {
+    Groups q;
+    int N, K;   // of w_g [N, K]
+};
+
+typedef float SmallSums[32 * 33];
+
+// y = act(x w^T + bias): a tile of 32 rows of a group by 32 columns.
+template <bool kCut>
+__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(Layer l, int kslice, const float *x, const float *w, const float *bias, float *y,
+                                                                    float *pre, int act)
+{
+    __shared__ SmallSums red[kSmallWaves];
+    const int n0 = (int)blockIdx.x * 32;
+    if (n0 >= l.N) return;
+    const Segment s = find_unit<true>(l.q, kTileShift, unit_id());
+    if (s.group < 0) return;
+    const size_t row = s.begin + ((size_t)s.unit << kTileShift);
+    const int rows = (int)min(s.end - row, (size_t)32);
+    if (s.group == (int)l.q.G) {
+        for (int i = threadIdx.x; i < 32 * rows; i += 64 * kSmallWaves) {
+            const int c = n0 + (i & 31);
+            if (c >= l.N) continue;
+            const size_t at = (row + (i >> 5)) * l.N + c;
+            y[at] = 0.0f;
+            if (pre) pre[at] = 0.0f;
+        }
+        return;
+    }
+    const DenseEpilogue ep{bias ? bias + (size_t)s.group * l.N : nullptr, nullptr, pre ? pre + row * l.N : nullptr, act, (size_t)l.N};
+    sgemm_small_body<false, true, kCut, DenseEpilogue>(rows, l.N, l.K, l.K, l.K, kslice, x + row * l.K, w + (size_t)s.group * l.N * l.K, y + row * l.N,
+                                                       nullptr, 0, nullptr, 0, nullptr, (int)blockIdx.x, 0, 0, l.K, red, ep);
+}
+
+// dx = dz w: a tile of 32 rows of a group by 32 of the K columns.
+template <bool kCut>
+__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dx_k(Layer l, int kslice, const float *dz, const float *w, float *dx)
+{
+    __shared__ SmallSums red[kSmallWaves];
+    const int k0 = (int)blockIdx.x * 32;
+    if (k0 >= l.K) return;
+    const Segment s = find_unit<true>(l.q, kTileShift, unit_id());
+    if (s.group < 0) return;
+    const size_t row = s.begin + ((size_t)s.unit << kTileShift);
+    const int rows = (int)min(s.end - row, (size_t)32);
+    if (s.group == (int)l.q.G) {
+        for (int i = threadIdx.x; i < 32 * rows; i += 64 * kSmallWaves)
+            if (k0 + (i & 31) < l.K) dx[(row + (i >> 5)) * l.K + k0 + (i & 31)] = 0.0f;
+        return;
+    }
+    sgemm_small_body<false, false, kCut>(rows, l.K, l.N, l.N, l.K, kslice, dz + row * l.N, w + (size_t)s.group * l.N * l.K, dx + row * l.K, nullptr, 0,
+                                         nullptr, 0, nullptr, (int)blockIdx.x, 0, 0, l.N, red);
+}
+
+// dw = dz^T x over 2^shift rows of a group: a tile of 32 of the N rows by 32 of the K columns.  Where a group is several such parts, they
+// wait for groups_join_k in `parts`, one matrix after the other.
+__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dw_k(Layer l, int shift, bool direct, const float *dz, const float *x, float *dw, float *parts)
+{
+    __shared__ SmallSums red[kSmallWaves];
+    const unsigned tiles = (unsigned)(l.K + 31) / 32, bx = blockIdx.x % tiles, by = blockIdx.x / tiles;
+    if ((int)by * 32 >= l.N) return;
+    const Segment s = find_unit<false, true>(l.q, shift, unit_id());
+    if (s.group < 0) return;
+    const size_t row = s.begin + ((size_t)s.unit << shift), matrix = (size_t)l.N * l.K;
+    const int rows = (int)min((size_t)s.end - row, (size_t)1 << shift);
+    const int kslice = ((rows + kSmallWaves - 1) / kSmallWaves + 7) / 8 * 8;
+    float *const to = direct ? dw + s.group * matrix : parts + unit_id() * matrix;
+    sgemm_small_body<true, false, false>(l.N, l.K, rows, l.N, l.K, kslice, dz + row * l.N, x + row * l.K, to, nullptr, 0, nullptr, 0, nullptr, (int)bx,
+                                         (int)by, 0, rows, red);
+}
+// Adds a group's parts, of which an empty one has a matrix of zeros.
+__global__ __launch_bounds__(256) void groups_join_k(Layer l, int shift, const float *parts, float *dw)
+{
+    const size_t matrix = (size_t)l.N * l.K;
+    const Segment s = find_group<true>(l.q, shift, unit_id());
+    if (s.group < 0) return;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < matrix; i += (size_t)gridDim.x * 256) {
+        const float *const from = parts + s.first * matrix + i;
+        float all = 0.0f;
+        for (unsigned p0 = 0; p0 < s.unit; p0 += 64) {   // sums of 64 values each
+            float sum = 0.0f;
+#pragma unroll 4
+            for (unsigned p = p0; p < min(s.unit, p0 + 64); p++) sum += from[p * matrix];
+            all += sum;
+        }
+        dw[s.group * matrix + i] = all;
+    }
+}
+
+// dz of 64 rows of a group by 256 columns, and their sums.
+__global__ __launch_bounds__(256) void groups_dz_k(Layer l, int act, const float *dy, const float *pre, float *dz, float *sums)
+{
+    const int c = (int)blockIdx.x * 256 + (int)threadIdx.x;
+    if ((int)blockIdx.x * 256 >= l.N) return;
+    const Segment s = find_unit<false>(l.q, kRunShift, unit_id());
+    if (s.group < 0 || c >= l.N) return;
+    const size_t row = s.begin + ((size_t)s.unit << kRunShift);
+    const int rows = (int)min((size_t)s.end - row, (size_t)1 << kRunShift);
+    const size_t at = row * l.N + c;
+    float sum = 0.0f;
+    with_activation(act, [&](auto kind) {
+        constexpr bool kPlain = decltype(kind)::value == DOPT_HIP_ACT_NONE;
+#pragma unroll 8
+        for (int r = 0; r < rows; r++) {
+            const size_t i = at + (size_t)r * l.N;
+            const float v = kPlain ? dy[i] : act_grad<kind.value>(dy[i], pre[i]);
+            sum += v;
+            if (!kPlain) dz[i] = v;
+        }
+    });
+    if (sums) sums[(size_t)unit_id() * l.N + c] = sum;
+}
+// dbias: 32 columns of a group by 32 lanes.
+__global__ __launch_bounds__(1024) void groups_fold_k(Layer l, const float *sums, float *dbias)
+{
+    __shared__ float red[32][33];
+    const int c = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
+    const Segment s = find_group(l.q, kRunShift, unit_id());
+    if (s.group < 0) return;
+    float all = 0.0f;
+    if (c < l.N) {
+        const float *const from = sums + (size_t)s.first * l.N + c;
+        for (unsigned i0 = (unsigned)lane; i0 < s.unit; i0 += 64 * 32) {   // sums of 64 values each
+            float sum = 0.0f;
+#pragma unroll 4
+            for (unsigned i = i0; i < min(s.unit, i0 + 64 * 32); i += 32) sum += from[(size_t)i * l.N];
+            all += sum;
+        }
+    }
+    red[lane][threadIdx.x & 31] = all;
+    __syncthreads();
+    if (lane || c >= l.N) return;
+    for (int i = 1; i < 32; i++) all += red[i][threadIdx.x];
+    dbias[(size_t)s.group * l.N + c] = all;
+}
+
+__global__ __launch_bounds__(256) void groups_zero_k(size_t n, float *p)
+{
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0.0f;
+}
+int clear(float *p, size_t n)
+{
+    if (!p || !n) return DOPT_HIP_OK;
+    hipLaunchKernelGGL(groups_zero_k, dim3((unsigned)std::min(ceil_div(n, (size_t)256), (size_t)num_cus() * 16)), dim3(256), 0, stream(), n, p);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+constexpr size_t kBytes = (size_t)1 << 31;   // what a buffer resource of the small products covers
+
+int check(const char *who, size_t G, size_t M, size_t N, size_t K, int act)
+{
+    DOPT_REQUIRE(known_activation(act), "%s: there is no activation %d", who, act);
+    // the small products reach 2 GB of one group's w and of 256 rows
+    DOPT_REQUIRE(G <= ((size_t)1 << 20) && M < ((size_t)1 << 31) && N <= ((size_t)1 << 20) && K <= ((size_t)1 << 20) &&
+                     std::max(N, (size_t)1) * std::max(K, (size_t)1) < kBytes / 4 && M * std::max(N, K) < ((size_t)1 << 40) &&
+                     G * N * K < ((size_t)1 << 40),
+                 "%s: dimensions too large", who);
+    return DOPT_HIP_OK;
+}
+
+size_t slice_of(size_t depth) { return ceil_div(ceil_div(depth, (size_t)kSmallWaves), (size_t)8) * 8; }
+
+struct Span {
+    const void *p;
+    size_t bytes;
+};
+template <size_t I, size_t O>
+int apart(const char *who, const Span (&in)[I], const Span (&out)[O])
+{
+    for (size_t i = 0; i < O; i++) {
+        for (const Span &s : in) DOPT_REQUIRE(!overlaps(out[i].p, out[i].bytes, s.p, s.bytes), "%s: a result overlaps an operand", who);
+        for (size_t k = 0; k < i; k++) DOPT_REQUIRE(!overlaps(out[i].p, out[i].bytes, out[k].p, out[k].bytes), "%s: two results overlap", who);
+    }
+    return DOPT_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const int32_t *offsets, const float *x, const float *w, const float *bias,
+                          float *y, float *pre)
+{
+    const char *const who = "dopt_hip_dense_groups";
+    if (int rc = check(who, G, M, N, K, act)) return rc;
+    if (M * N == 0) return DOPT_HIP_OK;
+    DOPT_REQUIRE(y && (G == 0 || (offsets && (K == 0 || (x && w)))), "%s: null argument", who);
+    const size_t f = sizeof(float), out = M * N * f;
+    const Span in[] = {{offsets, (G + 1) * sizeof(int32_t)}, {x, M * K * f}, {w, G * N * K * f}, {bias, G * N * f}};
+    const Span results[] = {{y, out}, {pre, out}};
+    if (int rc = apart(who, in, results)) return rc;
+    DOPT_ENSURE_INIT();
+    const Layer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    const dim3 grid = grid_of(ceil_div(N, (size_t)32), most_units(M, G + 2, kTileShift));
+    const int slice = (int)slice_of(K);
+    if (K % 4) hipLaunchKernelGGL(groups_small_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
+    else hipLaunchKernelGGL(groups_small_k<false>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, const int32_t *offsets, const float *dy, const float *pre,
+                               const float *x, const float *w, float *dx, float *dw, float *dbias)
+{
+    const char *const who = "dopt_hip_dense_groups_grad";
+    if (int rc = check(who, G, M, N, K, act)) return rc;
+    const bool some = G > 0 && M * N > 0;
+    DOPT_REQUIRE(!some || (offsets && dy && (act == DOPT_HIP_ACT_NONE || pre)), "%s: null argument", who);
+    DOPT_REQUIRE(!some || K == 0 || !dx || w, "%s: the gradient of x needs w", who);
+    DOPT_REQUIRE(!some || K == 0 || !dw || x, "%s: the gradient of w needs x", who);
+    DOPT_REQUIRE(G == 0 || offsets || M == 0, "%s: null argument", who);
+    const size_t f = sizeof(float);
+    const Span in[] = {{offsets, (G + 1) * sizeof(int32_t)}, {dy, M * N * f}, {pre, M * N * f}, {x, M * K * f}, {w, G * N * K * f}};
+    const Span results[] = {{dx, M * K * f}, {dw, G * N * K * f}, {dbias, G * N * f}};
+    if (int rc = apart(who, in, results)) return rc;
+    DOPT_ENSURE_INIT();
+    if (K == 0 || M * K == 0) dx = nullptr;
+    if (G * N * K == 0) dw = nullptr;
+    if (G * N == 0) dbias = nullptr;
+    if (!dx && !dw && !dbias) return DOPT_HIP_OK;
+    if (!some) {   // nothing to sum up
+        if (int rc = clear(dx, M * K)) return rc;
+        if (int rc = clear(dw, G * N * K)) return rc;
+        return clear(dbias, G * N);
+    }
+    const Layer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    // Rows of a part of a group's reduction: at most 8192, 1024 for each wavefront, so that sums of one sign are not rounded the same way for
+    // long; fewer where the tiles would not fill the chip (a part's matrix is written and read).
+    const size_t tiles = ceil_div(N, (size_t)32) * ceil_div(K, (size_t)32);
+    int shift = 13;
+    if (dw)
+        while (shift > 8 && (most_units(M, G, shift) * tiles < (size_t)num_cus() * 4 || ((size_t)1 << shift) * std::max(N, K) * f >= kBytes)) shift--;
+    const bool direct = ((size_t)1 << shift) >= M;
+    const size_t dw_units = most_units(M, G, shift), runs = most_units(M, G, kRunShift);
+    auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
+    const bool plain = act == DOPT_HIP_ACT_NONE;
+    const size_t dz_bytes = plain || !(dx || dw) ? 0 : rounded(M * N * f), sum_bytes = dbias ? rounded(runs * N * f) : 0,
+                 part_bytes = dw && !direct ? dw_units * N * K * f : 0;
+    char *const scratch = dz_bytes + sum_bytes + part_bytes ? (char *)workspace(dz_bytes + sum_bytes + part_bytes) : nullptr;
+    if (dz_bytes + sum_bytes + part_bytes && !scratch) return DOPT_HIP_ERR_OOM;
+    float *const dz_to = (float *)scratch, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
+    const float *const dz = plain ? dy : dz_to;
+    if (!plain || dbias) {
+        hipLaunchKernelGGL(groups_dz_k, grid_of(ceil_div(N, (size_t)256), runs), dim3(256), 0, stream(), l, act, dy, pre, dz_to, dbias ? sums : nullptr);
+        DOPT_LAUNCH_CHECK();
+    }
+    if (dx) {
+        const dim3 grid = grid_of(ceil_div(K, (size_t)32), most_units(M, G + 2, kTileShift));
+        const int slice = (int)slice_of(N);
+        if (N % 4) hipLaunchKernelGGL(groups_small_dx_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, dz, w, dx);
+        else hipLaunchKernelGGL(groups_small_dx_k<false>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, dz, w, dx);
+    }
+    if (dw) {
+        hipLaunchKernelGGL(groups_small_dw_k, grid_of(tiles, dw_units), dim3(64 * kSmallWaves), 0, stream(), l, shift, direct, dz, x, dw, parts);
+        if (!direct)
+            hipLaunchKernelGGL(groups_join_k, grid_of(std::min(ceil_div(N * K, (size_t)256), (size_t)num_cus() * 8), G), dim3(256), 0, stream(), l, shift, parts, dw);
+    }
+    if (dbias) hipLaunchKernelGGL(groups_fold_k, grid_of(ceil_div(N, (size_t)32), G), dim3(1024), 0, stream(), l, sums, dbias);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+}  // extern "C"

@@ -172,6 +172,30 @@ bool norm_attrs(const Operation &op, const std::vector<size_t> &x, NormAttrs *a)
     return true;
 }
 
+// x [M, K], w [G, N, K] and offsets [G + 1] of int32, dependencies `first` and on.
+struct GroupsSize {
+    size_t G, M, N, K;
+};
+bool groups_size(const Graph &g, const Operation &op, int first, GroupsSize *z)
+{
+    const auto &x = g.ops[op.deps[first]].shape, &w = g.ops[op.deps[first + 1]].shape;
+    const Operation &offsets = g.ops[op.deps[first + 2]];
+    if (x.size() != 2 || w.size() != 3 || x[1] != w[2] || offsets.dtype != DOPT_HIP_I32 || offsets.volume() != w[0] + 1) {
+        fail(DOPT_HIP_ERR_INVALID, "operation '%s': operands must be x [M, K], w [G, N, K] and G + 1 offsets of int32", op.opType.c_str());
+        return false;
+    }
+    *z = GroupsSize{w[0], x[0], w[1], x[1]};
+    return true;
+}
+// ... and the float32 operands beside the offsets: {dependency, volume}.
+bool groups_volumes(const Graph &g, const Operation &op, const std::vector<std::pair<int, size_t>> &deps, size_t result)
+{
+    bool ok = op.volume() == result;
+    for (const auto &d : deps) ok = ok && g.ops[op.deps[d.first]].volume() == d.second && g.ops[op.deps[d.first]].dtype == DOPT_HIP_F32;
+    if (!ok) fail(DOPT_HIP_ERR_INVALID, "operation '%s': an operand or the result has the wrong size or type", op.opType.c_str());
+    return ok;
+}
+
 // The optional operands of a residualNorm, by the bits of its attribute, and the descriptor (but for the rows).
 enum JoinOperand { kStream, kBranch, kGate, kPostScale, kPostBias, kPreScale, kPreBias, kJoinOperands };
 struct JoinAttrs {
@@ -515,6 +539,36 @@ void registerBuiltinsOnce()
         return make([=](const std::vector<const void *> &in, void *out) {
             return dopt_hip_group_norm_grad(a.N, a.C, a.inner, a.groups, a.last, a.act, (const float *)in[0], (const float *)in[1],
                                             (const float *)in[2], (const float *)in[3], (const float *)in[4], (float *)out);
+        });
+    };
+    R["denseGroups"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps [x, w, offsets] (+ bias); output [y] or [y | pre]
+        size_t act, bias, keep;
+        GroupsSize z;
+        if (!size_attr(op, "activation", &act) || !size_attr(op, "hasBias", &bias) || !size_attr(op, "keepsPre", &keep) ||
+            !need_deps(op, 3 + (bias != 0)) || !need_f32(op) || !groups_size(g, op, 0, &z))
+            return nullptr;
+        std::vector<std::pair<int, size_t>> volumes{{0, z.M * z.K}, {1, z.G * z.N * z.K}};
+        if (bias) volumes.push_back({3, z.G * z.N});
+        if (!groups_volumes(g, op, volumes, z.M * z.N * (keep ? 2 : 1))) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            return dopt_hip_dense_groups(z.G, z.M, z.N, z.K, (int)act, (const int32_t *)in[2], (const float *)in[0], (const float *)in[1],
+                                         bias ? (const float *)in[3] : nullptr, (float *)out, keep ? (float *)out + z.M * z.N : nullptr);
+        });
+    };
+    R["denseGroupsGrad"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {
+        const Operation &op = g.ops[id];  // deps [parentGrad, x, w, offsets] (+ pre, with an activation); output [dx | dw | dbias]
+        size_t act;
+        GroupsSize z;
+        if (!size_attr(op, "activation", &act) || !need_deps(op, act ? 5 : 4) || !need_f32(op) || !groups_size(g, op, 1, &z)) return nullptr;
+        std::vector<std::pair<int, size_t>> volumes{{0, z.M * z.N}, {1, z.M * z.K}, {2, z.G * z.N * z.K}};
+        if (act) volumes.push_back({4, z.M * z.N});
+        if (!groups_volumes(g, op, volumes, z.M * z.K + z.G * z.N * z.K + z.G * z.N)) return nullptr;
+        return make([=](const std::vector<const void *> &in, void *out) {
+            float *const dx = (float *)out, *const dw = dx + z.M * z.K;
+            return dopt_hip_dense_groups_grad(z.G, z.M, z.N, z.K, (int)act, (const int32_t *)in[3], (const float *)in[0],
+                                              act ? (const float *)in[4] : nullptr, (const float *)in[1], (const float *)in[2], dx, dw,
+                                              dw + z.G * z.N * z.K);
         });
     };
     R["residualNorm"] = [](const Graph &g, int id) -> std::unique_ptr<HIPKernel> {

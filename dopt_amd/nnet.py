@@ -157,6 +157,19 @@ def denseAct(inp, num_outputs, init, activation="none", residual=None, use_bias=
     return Layer([inp] + ([residual] if residual else []), y, y_tr, params)
 
 
+def denseGroups(inp, offsets, groups, num_outputs, init, activation="none", use_bias=True, weight_decay=0.0):
+    """A dense layer with a weight matrix for each of `groups` groups of consecutive rows: offsets (an operation of groups + 1 int32
+    values, an argument of each step as a rule) says where they begin.  No counterpart in the reference."""
+    x, x_tr = inp.output, inp.trainOutput
+    weights = float32([groups, num_outputs, x.shape[1]])
+    weights.set_value((init.rng.standard_normal(weights.shape) * np.sqrt(2.0 / x.shape[1])).astype(np.float32))
+    bias = float32([groups, num_outputs]) if use_bias else None
+    weight_loss = None if weight_decay == 0.0 else weight_decay * core.sum(weights * weights)
+    params = [Parameter(weights, weight_loss, None)] + ([Parameter(bias, None, None)] if use_bias else [])
+    y = core.denseGroups(x, weights, offsets, bias, activation, keepPre=False)
+    return Layer([inp], y, core.denseGroups(x_tr, weights, offsets, bias, activation), params)
+
+
 def residualNorm(stream, branch=None, gate=None, post="none", pre="none", residual_scale=1.0, epsilon=1e-5, scale_decay=0.0):
     """What lies between two blocks of a residual network: (the stream behind the one, what the other one reads).  The branch's norm, with its gate, is
     added to the stream, whose norm is the second layer (the stream itself where there is none).  gate: None, a starting value

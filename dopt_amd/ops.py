@@ -603,6 +603,44 @@ def dense_act_grad(dy, x, w, pre=None, act="none", dx=None, dw=None, dbias=None)
     return dx, dw, dbias
 
 
+def _group_sizes(x, w, offsets):
+    if len(x.shape) != 2 or len(w.shape) != 3 or x.shape[1] != w.shape[2] or x.dtype != _F32 or w.dtype != _F32:
+        raise capi.HipError(1, "denseGroups: x [M, K] and w [G, N, K] of float32")
+    if offsets.size != w.shape[0] + 1 or offsets.dtype != np.int32:
+        raise capi.HipError(1, "denseGroups: the offsets are G + 1 values of int32")
+    return w.shape[0], x.shape[0], w.shape[1], x.shape[1]
+
+
+def _group_operand(t, size, what, rows):
+    if t is None:
+        return None
+    if t.size != size or t.dtype != _F32 or (len(t.shape) > 1 and t.shape[0] != rows):
+        raise capi.HipError(1, "denseGroups: %s has the wrong size or type" % what)
+    return t.ptr
+
+
+def dense_groups(x, w, offsets, bias=None, act="none", out=None, pre=None):
+    """act(x . w[g]^T + bias[g]) for the rows offsets[g] .. offsets[g + 1] - 1 of x, zeros for rows of no group; w [G, N, K], offsets
+    [G + 1] of int32; `pre` receives what the activation is applied to, which the gradient reads."""
+    G, M, N, K = _group_sizes(x, w, offsets)
+    y = _out(out, (M, N))
+    _run(capi.load().dopt_hip_dense_groups(G, M, N, K, _activation(act), offsets.ptr, x.ptr, w.ptr, _group_operand(bias, G * N, "bias", G),
+                                           _group_operand(y, M * N, "the result", M), _group_operand(pre, M * N, "pre", M)))
+    return y
+
+
+def dense_groups_grad(dy, x, w, offsets, pre=None, act="none", dx=None, dw=None, dbias=None):
+    """(dx, dw, dbias) of dense_groups."""
+    G, M, N, K = _group_sizes(x, w, offsets)
+    code = _activation(act)
+    if pre is None and code:
+        raise capi.HipError(1, "denseGroupsGrad: the gradient of an activation reads what it was applied to")
+    dx, dw, dbias = _out(dx, (M, K)), _out(dw, (G, N, K)), _out(dbias, (G, N))
+    _run(capi.load().dopt_hip_dense_groups_grad(G, M, N, K, code, offsets.ptr, _group_operand(dy, M * N, "dy", M), _group_operand(pre, M * N, "pre", M),
+                                                x.ptr, w.ptr, dx.ptr, dw.ptr, dbias.ptr))
+    return dx, dw, dbias
+
+
 # ------------------------------------------------------------------------------- optimizers
 
 class MuonOptimizer:

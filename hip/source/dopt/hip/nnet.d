@@ -38,6 +38,8 @@ package
         registerHIPKernel("groupNormGrad", toDelegate(&ctr!GroupNormGrad), true);
         registerHIPKernel("denseAct", toDelegate(&ctr!DenseAct), true);
         registerHIPKernel("denseActGrad", toDelegate(&ctr!DenseActGrad), true);
+        registerHIPKernel("denseGroups", toDelegate(&ctr!DenseGroups), true);
+        registerHIPKernel("denseGroupsGrad", toDelegate(&ctr!DenseGroupsGrad), true);
         registerHIPKernel("residualNorm", toDelegate(&ctr!ResidualNorm), true);
         registerHIPKernel("residualNormGrad", toDelegate(&ctr!ResidualNormGrad), true);
     }
@@ -371,6 +373,60 @@ private
         }
 
         NormSize mSize;
+    }
+
+    class DenseGroups : HIPKernel
+    {
+        this(Operation op)
+        {
+            mM = op.deps[0].shape[0];
+            mG = op.deps[1].shape[0];
+            mN = op.deps[1].shape[1];
+            mK = op.deps[1].shape[2];
+            mAct = cast(int)op.attributes["activation"].get!size_t;
+            mBias = op.attributes["hasBias"].get!size_t != 0;
+            mKeep = op.attributes["keepsPre"].get!size_t != 0;
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: x, w, offsets, then the bias where there is one; output [y] or [y | pre]
+            auto bias = mBias ? f(inputs[3]) : null;
+            auto pre = mKeep ? f(output) + mM * mN : null;
+
+            hipCheck(dopt_hip_dense_groups(mG, mM, mN, mK, mAct, cast(const(int) *)inputs[2].ptr, f(inputs[0]), f(inputs[1]),
+                bias, f(output), pre));
+        }
+
+        size_t mG, mM, mN, mK;
+        int mAct;
+        bool mBias, mKeep;
+    }
+
+    class DenseGroupsGrad : HIPKernel
+    {
+        this(Operation op)
+        {
+            mM = op.deps[1].shape[0];
+            mG = op.deps[2].shape[0];
+            mN = op.deps[2].shape[1];
+            mK = op.deps[2].shape[2];
+            mAct = cast(int)op.attributes["activation"].get!size_t;
+        }
+
+        override void execute(const(HIPBuffer)[] inputs, HIPBuffer output)
+        {
+            //deps: dy, x, w, offsets, then what the activation was applied to where there is one; output [dx | dw | dbias]
+            auto pre = mAct != 0 ? f(inputs[4]) : null;
+            auto dx = f(output);
+            auto dw = dx + mM * mK;
+
+            hipCheck(dopt_hip_dense_groups_grad(mG, mM, mN, mK, mAct, cast(const(int) *)inputs[3].ptr, f(inputs[0]), pre,
+                f(inputs[1]), f(inputs[2]), dx, dw, dw + mG * mN * mK));
+        }
+
+        size_t mG, mM, mN, mK;
+        int mAct;
     }
 
     //The optional operands of a residualNorm, by the bits of its size_t attribute "operands": stream, branch, gate,

@@ -236,6 +236,8 @@ int dopt_hip_residual_norm(const(dopt_hip_residual_norm_desc)* desc, const(float
 int dopt_hip_residual_norm_grad(const(dopt_hip_residual_norm_desc)* desc, const(float)* dy, const(float)* dh, const(float)* y, const(float)* branch, const(float)* gate, const(float)* post_scale, const(float)* post_bias, const(float)* pre_scale, const(float)* stats, float* dx, float* dbranch, float* dgate, float* dpost_scale, float* dpost_bias, float* dpre_scale, float* dpre_bias);
 int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const(float)* x, const(float)* w, const(float)* bias, const(float)* residual, float* y, float* pre);
 int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const(float)* dy, const(float)* pre, const(float)* x, const(float)* w, float* dx, float* dw, float* dbias);
+int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const(int)* offsets, const(float)* x, const(float)* w, const(float)* bias, float* y, float* pre);
+int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, const(int)* offsets, const(float)* dy, const(float)* pre, const(float)* x, const(float)* w, float* dx, float* dw, float* dbias);
 int dopt_hip_optim_create(int ntensors, const(dopt_hip_tensor_ref)* refs, void** handle);
 int dopt_hip_optim_destroy(void* handle);
 int dopt_hip_sgd_step(void* handle, float lr, float mu, int nesterov);

@@ -586,6 +586,20 @@ int dopt_hip_dense_act(size_t M, size_t N, size_t K, int act, const float *x, co
 int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *dy, const float *pre, const float *x,
                             const float *w, float *dx, float *dw, float *dbias);
 
+/* Dense layers whose rows fall into G groups of consecutive rows, each with a w [N,K] and a bias [N] of its own (experts, domains,
+   heads): for the rows m of group g, offsets[g] <= m < offsets[g + 1],
+     pre = x * w[g]^T + bias[g],  y = act(pre)
+   x [M,K], w [G,N,K], bias [G,N] (may be null), y and pre (may be null) [M,N]; offsets holds G + 1 row numbers on the device.  A boundary
+   counts as the largest one up to it, and as no more than M, whatever is there; rows in front of the first group and
+   behind the last one belong to none: y and pre are zero there.  No result may overlap an operand or the other one. */
+int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const int32_t *offsets, const float *x, const float *w,
+                          const float *bias, float *y, float *pre);
+/* With dz = dy * act'(pre): dx = dz * w[g] [M,K], zero for rows of no group; dw[g] = dz^T * x [G,N,K] and dbias[g] = column sums of dz
+   [G,N] over the group's rows, zero for a group without rows.  Any of the three results may be null, and w (x) with dx (dw); pre
+   may be null for act none. */
+int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, const int32_t *offsets, const float *dy,
+                               const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
+
 /* ---------------------------------------------------------------------------------------
  * Fused multi-tensor optimizer updates.  The reference has no such kernels: dopt.online
  * builds each rule as a graph of pointwise ops with GEMM broadcasts

@@ -1,0 +1,215 @@
+"""Dense layers of groups of rows on the device against their float64 form."""
+import numpy as np
+import pytest
+
+import dense_groups as D
+import norm_dense_muon as R
+from dopt_amd import capi, core, nnet, online, ops
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+
+
+def _f(a):
+    return np.asarray(a, F32)
+
+
+def _off_grid(a):
+    """A device copy that starts four bytes behind a 16-byte boundary."""
+    return ops.Tensor((a.size + 1,), a.dtype).view(1, a.shape).set(a)
+
+
+def _case(sizes, n, k, seed, before=0, after=0):
+    r = np.random.default_rng(seed)
+    m, g = before + sum(sizes) + after, len(sizes)
+    offsets = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32) + np.int32(before)
+    return {"offsets": offsets, "x": _f(r.standard_normal((m, k))), "w": _f(r.standard_normal((g, n, k)) * np.sqrt(2.0 / max(k, 1))),
+            "bias": _f(0.3 * r.standard_normal((g, n))), "dy": _f(r.standard_normal((m, n))), "pre": _f(1.4 * r.standard_normal((m, n)))}
+
+
+def _place(shape, up):
+    """A result buffer that holds something already."""
+    return up(np.full(shape, 7, F32))
+
+
+def _check(t, name, up=ops.tensor, keep=True, bias=True):
+    d = {k: up(v) for k, v in t.items()}
+    (m, k), (g, n) = t["x"].shape, t["w"].shape[:2]
+    y, pre = _place((m, n), up), _place((m, n), up) if keep else None
+    ops.dense_groups(d["x"], d["w"], d["offsets"], d["bias"] if bias else None, name, out=y, pre=pre)
+    want = D.forward(t["x"], t["w"], t["bias"] if bias else None, t["offsets"], name)
+    R.close(y.numpy(), want[0], "y")
+    if keep:
+        R.close(pre.numpy(), want[1], "pre")
+    _check_grad(t, name, d, up)
+
+
+def _check_grad(t, name, d=None, up=ops.tensor):
+    d = d or {k: up(v) for k, v in t.items()}
+    p = t["pre"] if name != "none" else None
+    got = ops.dense_groups_grad(d["dy"], d["x"], d["w"], d["offsets"], d["pre"] if name != "none" else None, name, dx=_place(t["x"].shape, up),
+                                dw=_place(t["w"].shape, up), dbias=_place(t["w"].shape[:2], up))
+    want = D.backward(t["dy"], t["x"], t["w"], p, t["offsets"], name)
+    for a, b, what in zip(got, want, ("dx", "dw", "dbias")):
+        R.close(a.numpy(), b, what)
+    return got
+
+
+SIZES = [[1], [0], [5], [0, 0, 3, 0], [31, 32, 33], [9, 0, 17, 3, 11, 8, 14, 2], [64] * 4, [130, 1, 0, 77], [200, 63, 65], [1] * 70, [0] * 64 + [5] + [0] * 70 + [3]]
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: "%dx%d" % (len(s), sum(s)))
+@pytest.mark.parametrize("n,k", [(1, 1), (3, 5), (32, 32), (33, 65), (10, 200), (129, 31), (70, 128)])
+def test_sizes(sizes, n, k):
+    name = R.ACTS[(len(sizes) + n) % 4]
+    _check(_case(sizes, n, k, n + k), name, up=_off_grid if k % 2 else ops.tensor, keep=n % 2 == 0, bias=n != 10)
+
+
+@pytest.mark.parametrize("name", R.ACTS)
+def test_rows_of_no_group(name):
+    for before, after in ((3, 0), (0, 70), (40, 33)):
+        t = _case([20, 0, 45], 50, 40, 3, before, after)
+        t["x"][:before], t["dy"][:before], t["pre"][:before] = np.nan, np.inf, np.nan
+        if after:
+            t["x"][-after:], t["dy"][-after:], t["pre"][-after:] = np.inf, np.nan, np.nan
+        _check(t, name)
+
+
+@pytest.mark.parametrize("offsets", [[0, 0, 0, 0], [7, 7, 7, 7], [-5, 3, 9, 40], [0, 10, 4, 30], [50, 20, 30, 40], [0, 30, 30, 2 ** 31 - 1], [-2 ** 31, 5, -1, 29],
+                                     [60, 60, 60, 60], [100, 200, 300, 400], [30, 20, 10, 0]])
+def test_offsets_of_any_value(offsets):
+    """Boundaries beyond the rows and ones that fall are taken as the rules say; nothing outside the operands is read or written."""
+    t = _case([10, 20, 30], 24, 36, 4)
+    t["offsets"] = np.asarray(offsets, np.int32)
+    _check(t, "silu")
+
+
+def test_no_groups_and_no_rows():
+    t = _case([5], 8, 12, 1)
+    y = ops.tensor(np.full((5, 8), 3, F32))
+    lib = capi.load()
+    x, w, o = ops.tensor(t["x"]), ops.tensor(t["w"]), ops.tensor(t["offsets"])
+    capi.check(lib.dopt_hip_dense_groups(0, 5, 8, 12, 0, None, x.ptr, None, None, y.ptr, None))
+    assert not y.numpy().any()
+    dx, dw, db = ops.tensor(np.ones((5, 12), F32)), ops.tensor(np.ones((1, 8, 12), F32)), ops.tensor(np.ones((1, 8), F32))
+    capi.check(lib.dopt_hip_dense_groups_grad(0, 5, 8, 12, 0, None, y.ptr, None, x.ptr, None, dx.ptr, None, None))
+    assert not dx.numpy().any()
+    capi.check(lib.dopt_hip_dense_groups_grad(1, 0, 8, 12, 0, o.ptr, None, None, None, None, None, dw.ptr, db.ptr))
+    assert not dw.numpy().any() and not db.numpy().any()
+    capi.check(lib.dopt_hip_dense_groups(1, 5, 8, 0, 0, o.ptr, None, None, ops.tensor(t["bias"]).ptr, y.ptr, None))
+    assert np.array_equal(y.numpy(), np.tile(t["bias"], (5, 1)))
+    db.set(np.ones((1, 8), F32))
+    capi.check(lib.dopt_hip_dense_groups_grad(1, 5, 8, 0, 0, o.ptr, ops.tensor(t["dy"]).ptr, None, None, None, None, None, db.ptr))
+    R.close(db.numpy(), D.backward(t["dy"], t["x"], t["w"], None, t["offsets"], "none")[2], "dbias")
+
+
+def test_some_of_the_gradients():
+    t = _case([33, 0, 50, 12], 45, 70, 6, 2, 5)
+    d = {k: ops.tensor(v) for k, v in t.items()}
+    whole = [v.numpy() for v in _check_grad(t, "gelu", d)]
+    for want in range(1, 8):
+        out = [ops.Tensor(v.shape) if want >> i & 1 else None for i, v in enumerate(whole)]
+        capi.check(capi.load().dopt_hip_dense_groups_grad(4, len(t["x"]), 45, 70, 2, d["offsets"].ptr, d["dy"].ptr, d["pre"].ptr,
+                                                          d["x"].ptr if want & 2 else None, d["w"].ptr if want & 1 else None, *[o.ptr if o else None for o in out]))
+        assert all(o is None or np.array_equal(o.numpy(), v) for o, v in zip(out, whole))
+
+
+# reductions over many rows, in parts and by many groups; sizes of training
+@pytest.mark.parametrize("sizes,n,k", [([3000, 1, 700], 40, 24), ([20000], 17, 33), ([9000, 0, 9000], 64, 64), ([512, 311, 905, 77], 256, 200),
+                                       ([131, 0, 77, 200, 1, 64, 0, 45, 150, 33, 9, 120, 101], 333, 231), ([40] * 200, 64, 48), ([1024, 700, 90], 520, 384),
+                                       ([700, 1300], 1030, 260), ([300, 0, 5, 1500], 512, 1040)])
+def test_training_sizes(sizes, n, k):
+    t = _case(sizes, n, k, n, 1, 9)
+    _check(t, R.ACTS[n % 4])
+
+
+def test_a_group_that_is_not_finite_is_alone():
+    t = _case([40, 200, 30], 70, 90, 8)
+    clean = [ops.dense_groups(*[ops.tensor(t[k]) for k in ("x", "w", "offsets", "bias")], "gelu").numpy()] + [v.numpy() for v in _check_grad(t, "gelu")]
+    t["x"][50, 3], t["w"][1, 5, 7], t["dy"][60, 9] = np.nan, np.inf, -np.inf
+    d = {k: ops.tensor(v) for k, v in t.items()}
+    y = ops.dense_groups(d["x"], d["w"], d["offsets"], d["bias"], "gelu").numpy()
+    dx, dw, db = (v.numpy() for v in ops.dense_groups_grad(d["dy"], d["x"], d["w"], d["offsets"], d["pre"], "gelu"))
+    others = np.r_[0:40, 240:270]
+    assert np.array_equal(y[others], clean[0][others]) and np.array_equal(dx[others], clean[1][others])
+    assert np.array_equal(dw[[0, 2]], clean[2][[0, 2]]) and np.array_equal(db[[0, 2]], clean[3][[0, 2]])
+    assert np.isnan(y[50]).all() and not np.isfinite(y[40:240, 5]).any()
+
+
+def test_many_equal_values():
+    """A column of 0.1 summed over 100000 rows, and its products with ones: sums of at most 64 and 1024 values in a row."""
+    t = _case([100000, 5], 8, 8, 1)
+    t["dy"][:], t["x"][:] = 0.1, 1.0
+    dx, dw, db = (v.numpy() for v in ops.dense_groups_grad(*[ops.tensor(t[k]) for k in ("dy", "x", "w", "offsets")]))
+    assert np.abs(db[0] / (100000 * np.float64(F32(0.1))) - 1).max() <= 100 * R.E
+    assert np.abs(dw[0] / (100000 * np.float64(F32(0.1))) - 1).max() <= 600 * R.E
+
+
+def test_repeated_calls_give_the_same_bits():
+    t = _case([300, 1, 0, 512, 90], 200, 150, 2)
+    d = {k: ops.tensor(v) for k, v in t.items()}
+    first = [v.numpy() for v in _check_grad(t, "silu", d)]
+    for _ in range(5):
+        again = ops.dense_groups_grad(d["dy"], d["x"], d["w"], d["offsets"], d["pre"], "silu")
+        assert all(np.array_equal(a, b.numpy()) for a, b in zip(first, again))
+
+
+# ------------------------------------------------------------------------------------------------ in graphs
+
+FLAGS = [0, core.PLAN_VIEWS | core.PLAN_FUSE, core.PLAN_VIEWS | core.PLAN_FUSE | core.PLAN_GRAPH, core.PLAN_VIEWS | core.PLAN_OVERLAP]
+
+
+@pytest.mark.parametrize("flags", FLAGS)
+@pytest.mark.parametrize("name", R.ACTS)
+def test_in_a_graph(name, flags):
+    """The same plan with offsets that change from step to step: what no group has is zero each time."""
+    t = _case([10, 5, 0, 25], 30, 20, 5, 0, 8)
+    f = {k: core.float32(t[k].shape) for k in ("x", "w", "bias", "dy")}
+    o = core.int32(t["offsets"].shape)
+    y = core.denseGroups(f["x"], f["w"], o, f["bias"], name)
+    wrt = [f[k] for k in ("x", "w", "bias")]
+    outputs = [y] + core.grad(core.sum(y * f["dy"], [0, 1]).reshape([]), wrt)
+    plan = core.compile(outputs, flags)
+    rets = [ops.Tensor(v.shape) for v in outputs]
+    args = {f[k]: ops.tensor(t[k]) for k in f}
+    args[o] = ops.tensor(t["offsets"])
+    for offsets in ([0, 10, 15, 15, 40], [3, 3, 20, 48, 48], [0, 10, 15, 15, 40], [0, 0, 0, 0, 0], [0, 12, 24, 36, 48]):
+        t["offsets"] = np.asarray(offsets, np.int32)
+        args[o].set(t["offsets"])
+        plan.execute(args, rets)
+        got = [r.numpy() for r in rets]
+        (want, bound), (pre, _) = D.forward(t["x"], t["w"], t["bias"], t["offsets"], name)
+        R.close(got[0], (want, bound), "y")
+        if name == "relu":   # (where pre is within a rounding of zero either gradient is one)
+            assert np.abs(pre[want > 0]).min(initial=1.0) > 1e-5
+        _, p = ops.dense_groups(*[args[f[k]] for k in ("x", "w")], args[o], args[f["bias"]], name), ops.Tensor(want.shape)
+        ops.dense_groups(*[args[f[k]] for k in ("x", "w")], args[o], args[f["bias"]], name, pre=p)
+        grads = D.backward(t["dy"], t["x"], t["w"], p.numpy() if name != "none" else None, t["offsets"], name)
+        for a, b, what in zip(got[1:], grads, ("dx", "dw", "dbias")):
+            R.close(a, b, what)
+
+
+def test_a_network_of_blocks_with_groups_trains():
+    """Norms around blocks of two layers of groups, gradients clipped: with and without rewrites the same losses, and the clipped norm is as asked."""
+    losses = []
+    for flags in (0, core.PLAN_VIEWS | core.PLAN_FUSE | core.PLAN_GRAPH):
+        init = nnet.Init(3)
+        x, y, o = core.float32([60, 24]), core.float32([60, 24]), core.int32([5])
+        stream = nnet.dataSource(x)
+        _, h = nnet.residualNorm(stream, pre="rms")
+        for _ in range(2):
+            body = nnet.denseGroups(nnet.denseGroups(h, o, 4, 48, init, "gelu"), o, 4, 24, init)
+            stream, h = nnet.residualNorm(stream, body, gate=0.5, post="layer", pre="rms")
+        net = nnet.DAGNetwork([x], [h])
+        d = h.trainOutput - y
+        loss = core.sum(d * d, [0, 1]).reshape([])
+        up = online.fused_adam([loss], net.params, net.paramProj, flags=flags, maxNorm=2.0)
+        r = np.random.default_rng(2)
+        feed = {x: ops.tensor(_f(r.standard_normal((60, 24)))), y: ops.tensor(_f(r.standard_normal((60, 24)))), o: ops.tensor(np.asarray([0, 9, 9, 40, 57], np.int32))}
+        run = []
+        for _ in range(5):
+            run.append(float(up(feed)[0]))
+            norm, factor = up.norm.numpy()
+            assert norm > 2.0 and abs(factor * norm / 2.0 - 1) < 4 * R.E
+        losses.append(run)
+    assert np.array_equal(*losses) and np.isfinite(losses).all()
