@@ -1,0 +1,34 @@
+// What the kernels of dense layers of groups share (dense_groups.hip, dense_groups_wide.hip).
+#pragma once
+
+#include "common.h"
+#include "dense.h"
+#include "groups.h"
+
+namespace dopt {
+
+struct GroupLayer {
+    Groups q;
+    int N, K;   // of w_g [N, K]
+};
+
+// Large products, of two fp16 parts of each value.
+bool groups_wide_takes(size_t G, size_t M, size_t N, size_t K);        // y [M, N] from K steps
+bool groups_wide_takes_grad(size_t G, size_t M, size_t N, size_t K);   // dx and dw
+int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
+// dy and pre give dz, which is written where there is an activation; any result may be null.
+int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
+
+// dense_groups.hip: dbias from the sums of runs of 2^shift rows of a group.
+int groups_fold(const GroupLayer &l, int shift, const float *sums, float *dbias);
+
+constexpr unsigned kGridRow = 65535;   // units along the second side of a grid; more go to the third
+__device__ __forceinline__ unsigned unit_id() { return blockIdx.z * kGridRow + blockIdx.y; }
+// x: as many as there are tiles side by side, a multiple of eight, so that a tile of columns - and what it reads of a weight - stays on one XCD
+inline dim3 grid_of(size_t tiles, size_t units)
+{
+    const size_t x = ceil_div(tiles, (size_t)8) * 8;
+    return dim3((unsigned)x, (unsigned)(units < kGridRow ? units : kGridRow), (unsigned)ceil_div(units, (size_t)kGridRow));
+}
+
+}  // namespace dopt

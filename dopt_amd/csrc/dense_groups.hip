@@ -8,9 +8,7 @@
 // A workgroup finds its rows in the offsets itself: the grid has room for any sizes, workgroups beyond what there is end at once.
 #include <algorithm>
 
-#include "common.h"
-#include "dense.h"
-#include "groups.h"
+#include "dense_groups.h"
 #include "small_product.h"
 
 namespace {
@@ -19,26 +17,11 @@ using namespace dopt;
 
 constexpr int kTileShift = 5;    // rows of a tile: 32
 constexpr int kRunShift = 6;     // rows that a thread adds up for dbias before it rounds to memory: 64
-constexpr unsigned kGridRow = 65535;   // units along the second side of a grid; more go to the third
-
-__device__ __forceinline__ unsigned unit_id() { return blockIdx.z * kGridRow + blockIdx.y; }
-// x: as many as there are tiles side by side, a multiple of eight, so that a tile of columns - and what it reads of a weight - stays on one XCD
-dim3 grid_of(size_t tiles, size_t units)
-{
-    const size_t x = ceil_div(tiles, (size_t)8) * 8;
-    return dim3((unsigned)x, (unsigned)std::min(units, (size_t)kGridRow), (unsigned)ceil_div(units, (size_t)kGridRow));
-}
-
-struct Layer {
-    Groups q;
-    int N, K;   // of w_g [N, K]
-};
-
 typedef float SmallSums[32 * 33];
 
 // y = act(x w^T + bias): a tile of 32 rows of a group by 32 columns.
 template <bool kCut>
-__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(Layer l, int kslice, const float *x, const float *w, const float *bias, float *y,
+__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(GroupLayer l, int kslice, const float *x, const float *w, const float *bias, float *y,
                                                                     float *pre, int act)
 {
     __shared__ SmallSums red[kSmallWaves];
@@ -65,7 +48,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(Layer l, int 
 
 // dx = dz w: a tile of 32 rows of a group by 32 of the K columns.
 template <bool kCut>
-__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dx_k(Layer l, int kslice, const float *dz, const float *w, float *dx)
+__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dx_k(GroupLayer l, int kslice, const float *dz, const float *w, float *dx)
 {
     __shared__ SmallSums red[kSmallWaves];
     const int k0 = (int)blockIdx.x * 32;
@@ -85,7 +68,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dx_k(Layer l, i
 
 // dw = dz^T x over 2^shift rows of a group: a tile of 32 of the N rows by 32 of the K columns.  Where a group is several such parts, they
 // wait for groups_join_k in `parts`, one matrix after the other.
-__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dw_k(Layer l, int shift, bool direct, const float *dz, const float *x, float *dw, float *parts)
+__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dw_k(GroupLayer l, int shift, bool direct, const float *dz, const float *x, float *dw, float *parts)
 {
     __shared__ SmallSums red[kSmallWaves];
     const unsigned tiles = (unsigned)(l.K + 31) / 32, bx = blockIdx.x % tiles, by = blockIdx.x / tiles;
@@ -100,7 +83,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dw_k(Layer l, i
                                          (int)by, 0, rows, red);
 }
 // Adds a group's parts, of which an empty one has a matrix of zeros.
-__global__ __launch_bounds__(256) void groups_join_k(Layer l, int shift, const float *parts, float *dw)
+__global__ __launch_bounds__(256) void groups_join_k(GroupLayer l, int shift, const float *parts, float *dw)
 {
     const size_t matrix = (size_t)l.N * l.K;
     const Segment s = find_group<true>(l.q, shift, unit_id());
@@ -118,8 +101,8 @@ __global__ __launch_bounds__(256) void groups_join_k(Layer l, int shift, const f
     }
 }
 
-// dz of 64 rows of a group by 256 columns, and their sums.
-__global__ __launch_bounds__(256) void groups_dz_k(Layer l, int act, const float *dy, const float *pre, float *dz, float *sums)
+// dz (or null) of 64 rows of a group by 256 columns, and their sums.
+__global__ __launch_bounds__(256) void groups_dz_k(GroupLayer l, int act, const float *dy, const float *pre, float *dz, float *sums)
 {
     const int c = (int)blockIdx.x * 256 + (int)threadIdx.x;
     if ((int)blockIdx.x * 256 >= l.N) return;
@@ -136,17 +119,17 @@ __global__ __launch_bounds__(256) void groups_dz_k(Layer l, int act, const float
             const size_t i = at + (size_t)r * l.N;
             const float v = kPlain ? dy[i] : act_grad<kind.value>(dy[i], pre[i]);
             sum += v;
-            if (!kPlain) dz[i] = v;
+            if (!kPlain && dz) dz[i] = v;
         }
     });
     if (sums) sums[(size_t)unit_id() * l.N + c] = sum;
 }
 // dbias: 32 columns of a group by 32 lanes.
-__global__ __launch_bounds__(1024) void groups_fold_k(Layer l, const float *sums, float *dbias)
+__global__ __launch_bounds__(1024) void groups_fold_k(GroupLayer l, int shift, const float *sums, float *dbias)
 {
     __shared__ float red[32][33];
     const int c = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
-    const Segment s = find_group(l.q, kRunShift, unit_id());
+    const Segment s = find_group(l.q, shift, unit_id());
     if (s.group < 0) return;
     float all = 0.0f;
     if (c < l.N) {
@@ -208,6 +191,17 @@ int apart(const char *who, const Span (&in)[I], const Span (&out)[O])
 
 }  // namespace
 
+namespace dopt {
+
+int groups_fold(const GroupLayer &l, int shift, const float *sums, float *dbias)
+{
+    hipLaunchKernelGGL(groups_fold_k, grid_of(ceil_div((size_t)l.N, (size_t)32), l.q.G), dim3(1024), 0, stream(), l, shift, sums, dbias);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+}  // namespace dopt
+
 extern "C" {
 
 int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const int32_t *offsets, const float *x, const float *w, const float *bias,
@@ -222,7 +216,8 @@ int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const
     const Span results[] = {{y, out}, {pre, out}};
     if (int rc = apart(who, in, results)) return rc;
     DOPT_ENSURE_INIT();
-    const Layer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    if (G > 0 && groups_wide_takes(G, M, N, K)) return groups_wide(l, x, w, bias, act, y, pre);
     const dim3 grid = grid_of(ceil_div(N, (size_t)32), most_units(M, G + 2, kTileShift));
     const int slice = (int)slice_of(K);
     if (K % 4) hipLaunchKernelGGL(groups_small_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
@@ -255,7 +250,8 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
         if (int rc = clear(dw, G * N * K)) return rc;
         return clear(dbias, G * N);
     }
-    const Layer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    if ((dx || dw) && groups_wide_takes_grad(G, M, N, K)) return groups_wide_grad(l, act, dy, pre, x, w, dx, dw, dbias);
     // Rows of a part of a group's reduction: at most 8192, 1024 for each wavefront, so that sums of one sign are not rounded the same way for
     // long; fewer where the tiles would not fill the chip (a part's matrix is written and read).
     const size_t tiles = ceil_div(N, (size_t)32) * ceil_div(K, (size_t)32);
@@ -270,7 +266,7 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
                  part_bytes = dw && !direct ? dw_units * N * K * f : 0;
     char *const scratch = dz_bytes + sum_bytes + part_bytes ? (char *)workspace(dz_bytes + sum_bytes + part_bytes) : nullptr;
     if (dz_bytes + sum_bytes + part_bytes && !scratch) return DOPT_HIP_ERR_OOM;
-    float *const dz_to = (float *)scratch, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
+    float *const dz_to = dz_bytes ? (float *)scratch : nullptr, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
     const float *const dz = plain ? dy : dz_to;
     if (!plain || dbias) {
         hipLaunchKernelGGL(groups_dz_k, grid_of(ceil_div(N, (size_t)256), runs), dim3(256), 0, stream(), l, act, dy, pre, dz_to, dbias ? sums : nullptr);
@@ -287,9 +283,8 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
         if (!direct)
             hipLaunchKernelGGL(groups_join_k, grid_of(std::min(ceil_div(N * K, (size_t)256), (size_t)num_cus() * 8), G), dim3(256), 0, stream(), l, shift, parts, dw);
     }
-    if (dbias) hipLaunchKernelGGL(groups_fold_k, grid_of(ceil_div(N, (size_t)32), G), dim3(1024), 0, stream(), l, sums, dbias);
     DOPT_LAUNCH_CHECK();
-    return DOPT_HIP_OK;
+    return dbias ? groups_fold(l, kRunShift, sums, dbias) : DOPT_HIP_OK;
 }
 
 }  // extern "C"

@@ -32,12 +32,17 @@ def _place(shape, up):
     return up(np.full(shape, 7, F32))
 
 
+def _parts(t):
+    """Whether the products may be of two fp16 parts: the large ones."""
+    return t["x"].size * t["w"].shape[1] >= 900000000
+
+
 def _check(t, name, up=ops.tensor, keep=True, bias=True):
     d = {k: up(v) for k, v in t.items()}
     (m, k), (g, n) = t["x"].shape, t["w"].shape[:2]
     y, pre = _place((m, n), up), _place((m, n), up) if keep else None
     ops.dense_groups(d["x"], d["w"], d["offsets"], d["bias"] if bias else None, name, out=y, pre=pre)
-    want = D.forward(t["x"], t["w"], t["bias"] if bias else None, t["offsets"], name)
+    want = D.forward(t["x"], t["w"], t["bias"] if bias else None, t["offsets"], name, _parts(t))
     R.close(y.numpy(), want[0], "y")
     if keep:
         R.close(pre.numpy(), want[1], "pre")
@@ -49,7 +54,7 @@ def _check_grad(t, name, d=None, up=ops.tensor):
     p = t["pre"] if name != "none" else None
     got = ops.dense_groups_grad(d["dy"], d["x"], d["w"], d["offsets"], d["pre"] if name != "none" else None, name, dx=_place(t["x"].shape, up),
                                 dw=_place(t["w"].shape, up), dbias=_place(t["w"].shape[:2], up))
-    want = D.backward(t["dy"], t["x"], t["w"], p, t["offsets"], name)
+    want = D.backward(t["dy"], t["x"], t["w"], p, t["offsets"], name, _parts(t))
     for a, b, what in zip(got, want, ("dx", "dw", "dbias")):
         R.close(a.numpy(), b, what)
     return got
@@ -213,3 +218,101 @@ def test_a_network_of_blocks_with_groups_trains():
             assert norm > 2.0 and abs(factor * norm / 2.0 - 1) < 4 * R.E
         losses.append(run)
     assert np.array_equal(*losses) and np.isfinite(losses).all()
+
+
+# ------------------------------------------------------------------------------------------------ large products
+
+LARGE = [([512, 311, 905, 77, 640, 388, 1001, 262], 1024, 300), ([1300, 0, 200, 3000], 700, 513), ([4200, 5000], 300, 384), ([128] * 40, 520, 530),
+         ([2000, 1], 1030, 1100), ([300, 256, 255, 257, 1], 1500, 1024)]
+
+
+@pytest.mark.parametrize("sizes,n,k", LARGE, ids=lambda v: "%dx%d" % (len(v), sum(v)) if isinstance(v, list) else str(v))
+def test_large(sizes, n, k):
+    for i, (before, after) in enumerate(((0, 0), (5, 300))):
+        t = _case(sizes, n, k, n + i, before, after)
+        _check(t, R.ACTS[(n + i) % 4], up=_off_grid if i else ops.tensor, keep=i == 0, bias=i == 0)
+
+
+def test_large_with_a_long_reduction():
+    """More steps than one accumulator takes, of every product."""
+    _check(_case([5000, 300, 4500], 200, 4600, 1), "gelu")
+    _check(_case([300, 700], 5000, 260, 2), "silu")
+
+
+@pytest.mark.parametrize("offsets", [[0, 0, 0, 0, 0], [2000, 2000, 2000, 2000, 2000], [-5, 300, 900, 5000, 700], [0, 1500, 400, 3000, 2900],
+                                     [900, 100, 300, 200, 2 ** 31 - 1], [7000, 1, 1, 1, 1]])
+def test_large_with_offsets_of_any_value(offsets):
+    t = _case([500, 500, 500, 500], 800, 640, 4, 0, 100)
+    t["offsets"] = np.asarray(offsets, np.int32)
+    _check(t, "silu")
+
+
+def test_large_with_values_that_are_not_finite():
+    t = _case([600, 0, 900, 500], 700, 640, 9, 10, 20)
+    clean = [ops.dense_groups(*[ops.tensor(t[k]) for k in ("x", "w", "offsets", "bias")], "gelu").numpy()] + [v.numpy() for v in _check_grad(t, "gelu")]
+    t["x"][700, 3], t["x"][900, 5], t["w"][2, 5, 7], t["dy"][1000, 9] = np.nan, np.inf, np.inf, -np.inf
+    t["x"][:10], t["x"][-20:], t["w"][1] = np.nan, np.inf, np.nan
+    d = {k: ops.tensor(v) for k, v in t.items()}
+    y = ops.dense_groups(d["x"], d["w"], d["offsets"], d["bias"], "gelu").numpy()
+    dx, dw, db = (v.numpy() for v in ops.dense_groups_grad(d["dy"], d["x"], d["w"], d["offsets"], d["pre"], "gelu"))
+    others = np.r_[0:610, 1510:2030]
+    assert np.array_equal(y[others], clean[0][others]) and np.array_equal(dx[others], clean[1][others])
+    assert np.array_equal(dw[[0, 1, 3]], clean[2][[0, 1, 3]]) and np.array_equal(db[[0, 1, 3]], clean[3][[0, 1, 3]])
+    assert np.isnan(y[700]).all() and not np.isfinite(y[610:1510, 5]).any()
+    fine = np.delete(np.arange(610, 1510), [90, 290])
+    cols = np.delete(np.arange(700), 5)
+    assert np.array_equal(y[np.ix_(fine, cols)], clean[0][np.ix_(fine, cols)])
+    assert not np.isfinite(dw[2][:, [3, 5]]).any() and not np.isfinite(dw[2][9]).any() and not np.isfinite(db[2, 9])
+    rows, cols = np.delete(np.arange(700), 9), np.delete(np.arange(640), [3, 5])
+    assert np.array_equal(dw[2][np.ix_(rows, cols)], clean[2][2][np.ix_(rows, cols)])
+    assert not np.isfinite(dx[1000]).any() and not np.isfinite(dx[610:1510, 7]).any()
+
+
+def test_large_some_of_the_gradients():
+    t = _case([600, 300, 900], 600, 640, 6, 2, 5)
+    d = {k: ops.tensor(v) for k, v in t.items()}
+    for name in ("gelu", "none"):
+        whole = [v.numpy() for v in _check_grad(t, name, d)]
+        for want in range(1, 8):
+            out = [ops.Tensor(v.shape) if want >> i & 1 else None for i, v in enumerate(whole)]
+            capi.check(capi.load().dopt_hip_dense_groups_grad(3, len(t["x"]), 600, 640, capi.ACTIVATIONS[name], d["offsets"].ptr, d["dy"].ptr,
+                                                              d["pre"].ptr if name != "none" else None, d["x"].ptr if want & 2 else None,
+                                                              d["w"].ptr if want & 1 else None, *[o.ptr if o else None for o in out]))
+            for o, v, what in zip(out, whole, ("dx", "dw", "dbias")):
+                if o is not None and what == "dbias":   # (alone its sums go by other runs)
+                    R.close(o.numpy(), D.backward(t["dy"], t["x"], t["w"], t["pre"] if name != "none" else None, t["offsets"], name)[2], what)
+                elif o is not None:
+                    assert np.array_equal(o.numpy(), v) or np.abs(o.numpy() - v).max() <= 2.0 ** -18 * np.abs(v).max(), what
+
+
+def test_large_values_over_many_orders():
+    """Rows whose largest values differ by 2^60, and values far below their row's largest: each keeps 22 bits, or 2^-39 of that."""
+    t = _case([500, 700], 600, 640, 3)
+    r = np.random.default_rng(4)
+    t["x"] *= _f(2.0 ** r.integers(-30, 30, (1200, 1)))
+    t["w"] *= _f(2.0 ** r.integers(-20, 0, t["w"].shape))
+    y = ops.dense_groups(*[ops.tensor(t[k]) for k in ("x", "w", "offsets")]).numpy()
+    for g, s in enumerate((slice(0, 500), slice(500, 1200))):
+        x, w = t["x"][s].astype(np.float64), t["w"][g].astype(np.float64)
+        bound = (640 * 2.0 ** -24 + 2.0 ** -20) * (np.abs(x) @ np.abs(w).T) + 2.0 ** -38 * 640 * np.outer(np.abs(x).max(1), np.abs(w).max(1))
+        assert (np.abs(y[s] - x @ w.T) <= bound).all()
+
+
+def test_large_in_a_recorded_plan():
+    t = _case([700, 0, 900, 300], 512, 640, 5, 0, 60)
+    f = {k: core.float32(t[k].shape) for k in ("x", "w", "bias", "dy")}
+    o = core.int32(t["offsets"].shape)
+    y = core.denseGroups(f["x"], f["w"], o, f["bias"], "silu")
+    outputs = [y] + core.grad(core.sum(y * f["dy"], [0, 1]).reshape([]), [f[k] for k in ("x", "w", "bias")])
+    plan = core.compile(outputs, core.PLAN_VIEWS | core.PLAN_FUSE | core.PLAN_GRAPH)
+    rets = [ops.Tensor(v.shape) for v in outputs]
+    args = {f[k]: ops.tensor(t[k]) for k in f}
+    args[o] = ops.tensor(t["offsets"])
+    for offsets in ([0, 700, 700, 1600, 1900], [3, 3, 1200, 1480, 1960], [0, 0, 0, 0, 0], [0, 700, 700, 1600, 1900]):
+        args[o].set(np.asarray(offsets, np.int32))
+        pre = ops.Tensor(y.shape)
+        want = [ops.dense_groups(args[f["x"]], args[f["w"]], args[o], args[f["bias"]], "silu", pre=pre).numpy()]
+        want += [v.numpy() for v in ops.dense_groups_grad(args[f["dy"]], args[f["x"]], args[f["w"]], args[o], pre, "silu")]
+        plan.execute(args, rets)
+        assert all(np.array_equal(r.numpy(), w) for r, w in zip(rets, want))
+    assert plan.stats()["kernels"] and plan.recordings()["replays"] > 0
