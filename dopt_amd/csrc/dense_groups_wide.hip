@@ -5,6 +5,7 @@
 // Rows of a group are laid out from a tile's boundary on, so that a tile holds rows of one group; the steps of dw's reductions from a boundary of
 // 64 rows on.  How many tiles there are is found on the device: an XCD takes an eighth of them, side by side.
 #include <algorithm>
+#include <cstdlib>
 
 #include "dense_groups.h"
 #include "dense_wide.h"
@@ -21,7 +22,8 @@ __device__ __forceinline__ bool surely_empty(const Groups &q, unsigned g) { retu
 // ------------------------------------------------------------------------------------------------ columns: dz, sums, largest magnitudes
 
 // 256 columns of a run of rows: of 2^shift rows of a group, or of 256 rows of a group's w.  Of dy and pre dz, its sums and its largest
-// magnitudes; of x and w the magnitudes.  Bound by memory.
+// magnitudes; of x and w the magnitudes.  A lane has four columns, a wavefront every fourth row; the last four columns end with the matrix, whatever of
+// them other lanes form as well, to the same bits.  Bound by memory.
 struct Columns {
     const float *x, *pre;
     float *dz, *sums;
@@ -38,12 +40,15 @@ constexpr int kWeightRun = 256;
 
 __global__ __launch_bounds__(256) void groups_columns_k(Groups q, ColumnJobs jobs)
 {
+    __shared__ v4f_any red_sum[4][64];
+    __shared__ unsigned red_top[4][64][4];
     unsigned block = blockIdx.x;
     int which = 0;
     while (which + 1 < jobs.n && block >= jobs.j[which].blocks) block -= jobs.j[which++].blocks;
     const Columns &j = jobs.j[which];
     const unsigned unit = block / j.tiles;
-    const int c = (int)(block % j.tiles) * 256 + (int)threadIdx.x;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int c = min((int)(block % j.tiles) * 256 + 4 * lane, j.cols - 4);
     size_t row;
     int rows;
     if (j.runs) {
@@ -57,33 +62,60 @@ __global__ __launch_bounds__(256) void groups_columns_k(Groups q, ColumnJobs job
         row = s.begin + ((size_t)s.unit << jobs.shift);
         rows = (int)min((size_t)s.end - row, (size_t)1 << jobs.shift);
     }
-    if (c >= j.cols) return;
-    const size_t at = row * j.cols + c;
-    float all = 0.0f;
-    unsigned top = 0;
-    if (j.sums || j.dz) {
-        with_activation(j.act, [&](auto kind) {
-            constexpr bool kPlain = decltype(kind)::value == DOPT_HIP_ACT_NONE;
-            for (int r0 = 0; r0 < rows; r0 += 64) {   // sums of 64 values each
-                float sum = 0.0f;
-                const int end = min(rows, r0 + 64);
-#pragma unroll 8
-                for (int r = r0; r < end; r++) {
-                    const size_t i = at + (size_t)r * j.cols;
-                    const float v = kPlain ? j.x[i] : act_grad<kind.value>(j.x[i], j.pre[i]);
-                    sum += v;
-                    top = max(top, magnitude(v));
-                    if (!kPlain) j.dz[i] = v;
-                }
-                all += sum;
+    const size_t pitch = (size_t)j.cols, at = row * pitch + c;
+    float all[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    unsigned top[4] = {0, 0, 0, 0};
+    with_activation(j.act, [&](auto kind) {
+        constexpr bool kPlain = decltype(kind)::value == DOPT_HIP_ACT_NONE;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto one = [&](const v4f_any &d, const v4f_any &z, size_t i) {
+            v4f_any o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float v = act_grad<kind.value>(d[e], z[e]);
+                o[e] = v;
+                sum[e] += v;
+                top[e] = max(top[e], magnitude(v));
             }
-        });
-        if (j.sums) j.sums[(size_t)unit * j.cols + c] = all;
-    } else {
-#pragma unroll 8
-        for (int r = 0; r < rows; r++) top = max(top, magnitude(j.x[at + (size_t)r * j.cols]));
+            if (!kPlain) *(v4f_any *)(j.dz + i) = o;
+        };
+        int r = wave;
+        for (; r + 12 < rows; r += 16) {
+            if ((r & 255) < 4) {   // sums of 64 values each
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    all[e] += sum[e];
+                    sum[e] = 0.0f;
+                }
+            }
+            v4f_any d[4], z[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                d[i] = *(const v4f_any *)(j.x + at + (r + 4 * i) * pitch);
+                if (!kPlain) z[i] = *(const v4f_any *)(j.pre + at + (r + 4 * i) * pitch);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) one(d[i], kPlain ? d[i] : z[i], at + (r + 4 * i) * pitch);
+        }
+        for (; r < rows; r += 4) {
+            const v4f_any d = *(const v4f_any *)(j.x + at + r * pitch);
+            one(d, kPlain ? d : *(const v4f_any *)(j.pre + at + r * pitch), at + r * pitch);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) all[e] += sum[e];
+    });
+    red_sum[wave][lane] = v4f_any{all[0], all[1], all[2], all[3]};
+#pragma unroll
+    for (int e = 0; e < 4; e++) red_top[wave][lane][e] = top[e];
+    __syncthreads();
+    if (wave) return;
+    const size_t to = (size_t)unit * pitch + c;
+    if (j.sums) *(v4f_any *)(j.sums + to) = (red_sum[0][lane] + red_sum[1][lane]) + (red_sum[2][lane] + red_sum[3][lane]);
+    if (j.tops) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            j.tops[to + e] = max(max(red_top[0][lane][e], red_top[1][lane][e]), max(red_top[2][lane][e], red_top[3][lane][e]));
     }
-    if (j.tops) j.tops[(size_t)unit * j.cols + c] = top;
 }
 
 // ------------------------------------------------------------------------------------------------ layouts
@@ -318,6 +350,7 @@ unsigned row_threads(size_t steps) { return steps > 512 ? 1024 : steps > 256 ? 5
 // The side of the tiles: large ones where they fill the chip and groups are long enough for them on average.
 size_t tile_for(size_t G, size_t M, size_t N, size_t K)
 {
+    if (getenv("G_TILE")) return strtoull(getenv("G_TILE"), 0, 10);
     const size_t rows = ceil_div(M, (size_t)kBig) + G / 2, tiles = rows * ceil_div(N, (size_t)kBig);
     return K >= 128 && M >= 384 * G && N >= 512 && tiles >= (size_t)num_cus() * 2 / 3 ? kBig : kSmall;
 }
@@ -326,12 +359,15 @@ size_t tile_for(size_t G, size_t M, size_t N, size_t K)
 
 namespace dopt {
 
+static size_t tune(const char *k, size_t d) { const char *v = getenv(k); return v ? strtoull(v, 0, 10) : d; }
 bool groups_wide_takes(size_t G, size_t M, size_t N, size_t K)
 {
+    if (getenv("G_WIDE")) return tune("G_WIDE", 0);
     return K >= 128 && N >= 128 && M >= 64 * G && M * N * K >= (size_t)900000000;
 }
 bool groups_wide_takes_grad(size_t G, size_t M, size_t N, size_t K)
 {
+    if (getenv("G_WIDE")) return tune("G_WIDE", 0);
     return K >= 128 && N >= 128 && M >= 64 * G && M * N * K >= (size_t)900000000;
 }
 
@@ -368,7 +404,7 @@ int groups_wide(const GroupLayer &l, const float *x, const float *w, const float
 int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
 {
     const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, steps = ceil_div(N, (size_t)16);
-    const size_t tile = std::min(tile_for(G, M, K, N), dw ? G * ceil_div(N, (size_t)kBig) * ceil_div(K, (size_t)kBig) >= (size_t)num_cus() ? (size_t)kBig : (size_t)kSmall : (size_t)kBig);
+    const size_t tile = getenv("G_TILE") ? strtoull(getenv("G_TILE"), 0, 10) : std::min(tile_for(G, M, K, N), dw ? G * ceil_div(N, (size_t)kBig) * ceil_div(K, (size_t)kBig) >= (size_t)num_cus() ? (size_t)kBig : (size_t)kSmall : (size_t)kBig);
     const size_t mtiles = most_units(M, G, shift_of_tile(tile)), rows = mtiles * tile, padded_n = padded_to(N, tile), padded_k = padded_to(K, tile);
     const size_t ktiles = padded_k / tile, wtiles = padded_n / tile * ktiles, units = most_units(M, G, kStepShift);
     int shift = kStepShift;   // rows of a run of sums and largest magnitudes: every tile of a turned layout reads all of a group's
