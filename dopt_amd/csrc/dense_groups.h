@@ -18,9 +18,12 @@ bool groups_wide_takes_grad(size_t G, size_t M, size_t N, size_t K);   // dx and
 int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
 // dy and pre give dz, which is written where there is an activation; any result may be null.
 int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
+// dz (which may be null) of N >= 4 columns, and the sums (null too) of runs of 2^shift rows of a group.
+int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const float *pre, float *dz, float *sums);
 
-// dense_groups.hip: dbias from the sums of runs of 2^shift rows of a group.
+// dense_groups.hip: dbias from the sums of runs of 2^shift rows of a group; dw from the matrices of such parts, of which an empty group has one of zeros.
 int groups_fold(const GroupLayer &l, int shift, const float *sums, float *dbias);
+int groups_join(const GroupLayer &l, int shift, const float *parts, float *dw);
 
 constexpr unsigned kGridRow = 65535;   // units along the second side of a grid; more go to the third
 __device__ __forceinline__ unsigned unit_id() { return blockIdx.z * kGridRow + blockIdx.y; }

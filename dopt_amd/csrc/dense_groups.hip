@@ -46,41 +46,85 @@ __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(GroupLayer l,
                                                        nullptr, 0, nullptr, 0, nullptr, (int)blockIdx.x, 0, 0, l.K, red, ep);
 }
 
-// dx = dz w: a tile of 32 rows of a group by 32 of the K columns.
+// The gradients in one launch, each by its own workgroups: dx = dz w, a tile of 32 rows of a group by 32 of the K columns; dw = dz^T x over
+// 2^shift rows of a group, a tile of 32 of the N rows by 32 of the K columns, which wait for groups_join_k in `parts` where a
+// group is several such parts; dbias from the sums of runs of rows, 32 columns of a group by sixteen lanes.
+struct SmallGrads {
+    const float *dz, *x, *w, *sums;
+    float *dx, *dw, *parts, *dbias;   // parts: or null
+    int slice, shift;
+    unsigned dx_tiles, dw_tiles, fold_tiles;           // side by side, multiples of eight: a tile of columns stays on one XCD
+    size_t dx_blocks, dw_blocks, fold_blocks;
+};
+
 template <bool kCut>
-__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dx_k(GroupLayer l, int kslice, const float *dz, const float *w, float *dx)
+__device__ __forceinline__ void small_dx(const GroupLayer &l, const SmallGrads &g, unsigned tile, unsigned unit, SmallSums *red)
 {
-    __shared__ SmallSums red[kSmallWaves];
-    const int k0 = (int)blockIdx.x * 32;
+    const int k0 = (int)tile * 32;
     if (k0 >= l.K) return;
-    const Segment s = find_unit<true>(l.q, kTileShift, unit_id());
+    const Segment s = find_unit<true>(l.q, kTileShift, unit);
     if (s.group < 0) return;
     const size_t row = s.begin + ((size_t)s.unit << kTileShift);
     const int rows = (int)min(s.end - row, (size_t)32);
     if (s.group == (int)l.q.G) {
         for (int i = threadIdx.x; i < 32 * rows; i += 64 * kSmallWaves)
-            if (k0 + (i & 31) < l.K) dx[(row + (i >> 5)) * l.K + k0 + (i & 31)] = 0.0f;
+            if (k0 + (i & 31) < l.K) g.dx[(row + (i >> 5)) * l.K + k0 + (i & 31)] = 0.0f;
         return;
     }
-    sgemm_small_body<false, false, kCut>(rows, l.K, l.N, l.N, l.K, kslice, dz + row * l.N, w + (size_t)s.group * l.N * l.K, dx + row * l.K, nullptr, 0,
-                                         nullptr, 0, nullptr, (int)blockIdx.x, 0, 0, l.N, red);
+    sgemm_small_body<false, false, kCut>(rows, l.K, l.N, l.N, l.K, g.slice, g.dz + row * l.N, g.w + (size_t)s.group * l.N * l.K, g.dx + row * l.K, nullptr,
+                                         0, nullptr, 0, nullptr, (int)tile, 0, 0, l.N, red);
 }
 
-// dw = dz^T x over 2^shift rows of a group: a tile of 32 of the N rows by 32 of the K columns.  Where a group is several such parts, they
-// wait for groups_join_k in `parts`, one matrix after the other.
-__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_dw_k(GroupLayer l, int shift, bool direct, const float *dz, const float *x, float *dw, float *parts)
+__device__ __forceinline__ void small_dw(const GroupLayer &l, const SmallGrads &g, unsigned tile, unsigned unit, SmallSums *red)
+{
+    const unsigned tiles = (unsigned)(l.K + 31) / 32, bx = tile % tiles, by = tile / tiles;
+    if ((int)by * 32 >= l.N) return;
+    const Segment s = find_unit<false, true>(l.q, g.shift, unit);
+    if (s.group < 0) return;
+    const size_t row = s.begin + ((size_t)s.unit << g.shift), matrix = (size_t)l.N * l.K;
+    const int rows = (int)min((size_t)s.end - row, (size_t)1 << g.shift);
+    const int kslice = ((rows + kSmallWaves - 1) / kSmallWaves + 7) / 8 * 8;
+    float *const to = g.parts ? g.parts + unit * matrix : g.dw + s.group * matrix;
+    sgemm_small_body<true, false, false>(l.N, l.K, rows, l.N, l.K, kslice, g.dz + row * l.N, g.x + row * l.K, to, nullptr, 0, nullptr, 0, nullptr, (int)bx,
+                                         (int)by, 0, rows, red);
+}
+
+// `lanes` lanes to a column, of 32 side by side; red: a value of each.
+__device__ __forceinline__ void fold_runs(const GroupLayer &l, int shift, const float *sums, float *dbias, unsigned tile, unsigned group, int lanes,
+                                          float (*red)[33])
+{
+    const int c = (int)tile * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
+    const Segment s = find_group(l.q, shift, group);
+    if (s.group < 0) return;
+    float all = 0.0f;
+    if (c < l.N) {
+        const float *const from = sums + (size_t)s.first * l.N + c;
+        for (unsigned i0 = (unsigned)lane; i0 < s.unit; i0 += 64 * lanes) {   // sums of 64 values each
+            float sum = 0.0f;
+#pragma unroll 4
+            for (unsigned i = i0; i < min(s.unit, i0 + 64 * lanes); i += lanes) sum += from[(size_t)i * l.N];
+            all += sum;
+        }
+    }
+    red[lane][threadIdx.x & 31] = all;
+    __syncthreads();
+    if (lane || c >= l.N) return;
+    for (int i = 1; i < lanes; i++) all += red[i][threadIdx.x];
+    dbias[(size_t)s.group * l.N + c] = all;
+}
+
+constexpr unsigned kRow = 1u << 22;   // workgroups of a row of such a grid
+template <bool kCut>
+__global__ __launch_bounds__(64 * kSmallWaves) void groups_small_grad_k(GroupLayer l, SmallGrads g)
 {
     __shared__ SmallSums red[kSmallWaves];
-    const unsigned tiles = (unsigned)(l.K + 31) / 32, bx = blockIdx.x % tiles, by = blockIdx.x / tiles;
-    if ((int)by * 32 >= l.N) return;
-    const Segment s = find_unit<false, true>(l.q, shift, unit_id());
-    if (s.group < 0) return;
-    const size_t row = s.begin + ((size_t)s.unit << shift), matrix = (size_t)l.N * l.K;
-    const int rows = (int)min((size_t)s.end - row, (size_t)1 << shift);
-    const int kslice = ((rows + kSmallWaves - 1) / kSmallWaves + 7) / 8 * 8;
-    float *const to = direct ? dw + s.group * matrix : parts + unit_id() * matrix;
-    sgemm_small_body<true, false, false>(l.N, l.K, rows, l.N, l.K, kslice, dz + row * l.N, x + row * l.K, to, nullptr, 0, nullptr, 0, nullptr, (int)bx,
-                                         (int)by, 0, rows, red);
+    size_t block = (size_t)blockIdx.y * kRow + blockIdx.x;
+    if (block < g.dx_blocks) return small_dx<kCut>(l, g, (unsigned)(block % g.dx_tiles), (unsigned)(block / g.dx_tiles), red);
+    block -= g.dx_blocks;
+    if (block < g.dw_blocks) return small_dw(l, g, (unsigned)(block % g.dw_tiles), (unsigned)(block / g.dw_tiles), red);
+    block -= g.dw_blocks;
+    if (block < g.fold_blocks)
+        fold_runs(l, kRunShift, g.sums, g.dbias, (unsigned)(block % g.fold_tiles), (unsigned)(block / g.fold_tiles), 2 * kSmallWaves, (float(*)[33])red);
 }
 // Adds a group's parts, of which an empty one has a matrix of zeros.
 __global__ __launch_bounds__(256) void groups_join_k(GroupLayer l, int shift, const float *parts, float *dw)
@@ -101,7 +145,7 @@ __global__ __launch_bounds__(256) void groups_join_k(GroupLayer l, int shift, co
     }
 }
 
-// dz (or null) of 64 rows of a group by 256 columns, and their sums.
+// dz (or null) of 64 rows of a group by 256 columns, and their sums, for fewer than four columns.
 __global__ __launch_bounds__(256) void groups_dz_k(GroupLayer l, int act, const float *dy, const float *pre, float *dz, float *sums)
 {
     const int c = (int)blockIdx.x * 256 + (int)threadIdx.x;
@@ -124,28 +168,11 @@ __global__ __launch_bounds__(256) void groups_dz_k(GroupLayer l, int act, const 
     });
     if (sums) sums[(size_t)unit_id() * l.N + c] = sum;
 }
-// dbias: 32 columns of a group by 32 lanes.
+// dbias by itself: 32 columns of a group by 32 lanes.
 __global__ __launch_bounds__(1024) void groups_fold_k(GroupLayer l, int shift, const float *sums, float *dbias)
 {
     __shared__ float red[32][33];
-    const int c = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
-    const Segment s = find_group(l.q, shift, unit_id());
-    if (s.group < 0) return;
-    float all = 0.0f;
-    if (c < l.N) {
-        const float *const from = sums + (size_t)s.first * l.N + c;
-        for (unsigned i0 = (unsigned)lane; i0 < s.unit; i0 += 64 * 32) {   // sums of 64 values each
-            float sum = 0.0f;
-#pragma unroll 4
-            for (unsigned i = i0; i < min(s.unit, i0 + 64 * 32); i += 32) sum += from[(size_t)i * l.N];
-            all += sum;
-        }
-    }
-    red[lane][threadIdx.x & 31] = all;
-    __syncthreads();
-    if (lane || c >= l.N) return;
-    for (int i = 1; i < 32; i++) all += red[i][threadIdx.x];
-    dbias[(size_t)s.group * l.N + c] = all;
+    fold_runs(l, shift, sums, dbias, blockIdx.x, unit_id(), 32, red);
 }
 
 __global__ __launch_bounds__(256) void groups_zero_k(size_t n, float *p)
@@ -196,6 +223,14 @@ namespace dopt {
 int groups_fold(const GroupLayer &l, int shift, const float *sums, float *dbias)
 {
     hipLaunchKernelGGL(groups_fold_k, grid_of(ceil_div((size_t)l.N, (size_t)32), l.q.G), dim3(1024), 0, stream(), l, shift, sums, dbias);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
+int groups_join(const GroupLayer &l, int shift, const float *parts, float *dw)
+{
+    const size_t matrix = (size_t)l.N * l.K;
+    hipLaunchKernelGGL(groups_join_k, grid_of(std::min(ceil_div(matrix, (size_t)256), (size_t)num_cus() * 8), l.q.G), dim3(256), 0, stream(), l, shift, parts, dw);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
@@ -269,22 +304,26 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
     float *const dz_to = dz_bytes ? (float *)scratch : nullptr, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
     const float *const dz = plain ? dy : dz_to;
     if (!plain || dbias) {
-        hipLaunchKernelGGL(groups_dz_k, grid_of(ceil_div(N, (size_t)256), runs), dim3(256), 0, stream(), l, act, dy, pre, dz_to, dbias ? sums : nullptr);
-        DOPT_LAUNCH_CHECK();
+        if (N >= 4) {
+            if (int rc = groups_dz(l, act, kRunShift, dy, pre, dz_to, dbias ? sums : nullptr)) return rc;
+        } else {
+            hipLaunchKernelGGL(groups_dz_k, grid_of(ceil_div(N, (size_t)256), runs), dim3(256), 0, stream(), l, act, dy, pre, dz_to, dbias ? sums : nullptr);
+            DOPT_LAUNCH_CHECK();
+        }
     }
-    if (dx) {
-        const dim3 grid = grid_of(ceil_div(K, (size_t)32), most_units(M, G + 2, kTileShift));
-        const int slice = (int)slice_of(N);
-        if (N % 4) hipLaunchKernelGGL(groups_small_dx_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, dz, w, dx);
-        else hipLaunchKernelGGL(groups_small_dx_k<false>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, dz, w, dx);
-    }
-    if (dw) {
-        hipLaunchKernelGGL(groups_small_dw_k, grid_of(tiles, dw_units), dim3(64 * kSmallWaves), 0, stream(), l, shift, direct, dz, x, dw, parts);
-        if (!direct)
-            hipLaunchKernelGGL(groups_join_k, grid_of(std::min(ceil_div(N * K, (size_t)256), (size_t)num_cus() * 8), G), dim3(256), 0, stream(), l, shift, parts, dw);
-    }
+    auto eights = [](size_t n) { return ceil_div(n, (size_t)8) * 8; };
+    SmallGrads g{dz, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, (int)slice_of(N), shift, (unsigned)eights(ceil_div(K, (size_t)32)),
+                 (unsigned)eights(tiles), (unsigned)eights(ceil_div(N, (size_t)32)), 0, 0, 0};
+    if (dx) g.dx_blocks = g.dx_tiles * most_units(M, G + 2, kTileShift);
+    if (dw) g.dw_blocks = g.dw_tiles * dw_units;
+    if (dbias) g.fold_blocks = g.fold_tiles * G;
+    const size_t blocks = g.dx_blocks + g.dw_blocks + g.fold_blocks;
+    DOPT_REQUIRE(blocks < ((size_t)1 << 37), "%s: dimensions too large", who);
+    const dim3 grid((unsigned)std::min(blocks, (size_t)kRow), (unsigned)ceil_div(blocks, (size_t)kRow));
+    if (dx && N % 4) hipLaunchKernelGGL(groups_small_grad_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, g);
+    else hipLaunchKernelGGL(groups_small_grad_k<false>, grid, dim3(64 * kSmallWaves), 0, stream(), l, g);
     DOPT_LAUNCH_CHECK();
-    return dbias ? groups_fold(l, kRunShift, sums, dbias) : DOPT_HIP_OK;
+    return dw && !direct ? groups_join(l, shift, parts, dw) : DOPT_HIP_OK;
 }
 
 }  // extern "C"

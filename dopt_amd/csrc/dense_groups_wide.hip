@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void groups_columns_k(Groups q, ColumnJobs job
                 sum[e] += v;
                 top[e] = max(top[e], magnitude(v));
             }
-            if (!kPlain) *(v4f_any *)(j.dz + i) = o;
+            if (!kPlain && j.dz) *(v4f_any *)(j.dz + i) = o;
         };
         int r = wave;
         for (; r + 12 < rows; r += 16) {
@@ -253,9 +253,10 @@ struct WeightsProduct {
     size_t N, K, dz_padded, x_padded;
     const char *dzp, *xp;
     const int *dzs, *xs;
-    float *dw;
+    float *dw, *parts;       // parts: of several for a group, a matrix each, where that is not null
     char *waiting;
     unsigned mtiles, ntiles;
+    int part_shift;          // of 2^part_shift rows
 };
 struct GroupProducts {
     RowsProduct rows;
@@ -269,7 +270,7 @@ struct GroupProducts {
 template <int kTile, bool kPasses>
 __global__ __launch_bounds__(2 * kTile, 2) void groups_product_k(Groups q, GroupProducts p)
 {
-    constexpr int kShift = kTile == kBig ? 8 : 7;
+    constexpr int kShift = kTile == kBig ? 8 : 7, kStages = 3;   // three workgroups of 128 x 128 to a CU: their numbers are rarely even
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const unsigned xcd = blockIdx.x & 7, place = blockIdx.x >> 3;
     if (place < p.rows_per) {
@@ -285,15 +286,24 @@ __global__ __launch_bounds__(2 * kTile, 2) void groups_product_k(Groups q, Group
                      r.xp + (size_t)s.first * (kTile / 32) * r.steps * 2048, r.wp + g * (r.padded / 32) * r.steps * 2048, r.xs + (size_t)s.first * kTile,
                      r.ws + g * r.padded, nullptr, nullptr, r.waiting, 0, 0, 0, 1};
         const DenseEpilogue ep{p.bias ? p.bias + g * r.N : nullptr, nullptr, p.pre ? p.pre + begin * r.N : nullptr, p.act, r.N};
-        wide_tile<kTile, kPasses>(z, ep, r.y + begin * r.N, s.unit, nt, 0, r.steps, id, lds);
+        wide_tile<kTile, kPasses, kStages>(z, ep, r.y + begin * r.N, s.unit, nt, 0, r.steps, id, lds);
         return;
     }
     const WeightsProduct &r = p.weights;
-    const unsigned tiles = r.mtiles * r.ntiles, of_xcd = (tiles + 7) / 8, at = place - p.rows_per, g = at / of_xcd, tile = xcd * of_xcd + at % of_xcd;
-    if (g >= q.G || tile >= tiles) return;
+    const unsigned tiles = r.mtiles * r.ntiles, of_xcd = (tiles + 7) / 8, at = place - p.rows_per, item = at / of_xcd, tile = xcd * of_xcd + at % of_xcd;
+    if (tile >= tiles) return;
     const unsigned mt = tile % r.mtiles, nt = tile / r.mtiles;
-    const Segment s = find_group(q, kStepShift, g);
-    float *const dw = r.dw + g * r.N * r.K;
+    unsigned group = item, part = 0;
+    if (r.parts) {
+        const Segment of = find_unit<false, true>(q, r.part_shift, item);
+        if (of.group < 0) return;
+        group = (unsigned)of.group;
+        part = of.unit;
+    }
+    if (group >= q.G) return;
+    const Segment s = find_group(q, kStepShift, group);
+    const size_t g = group;
+    float *const dw = r.parts ? r.parts + (size_t)item * r.N * r.K : r.dw + g * r.N * r.K;
     const size_t rows = s.end - s.begin;
     if (rows == 0) {
         const size_t m0 = (size_t)mt * kTile, n0 = (size_t)nt * kTile;
@@ -305,7 +315,12 @@ __global__ __launch_bounds__(2 * kTile, 2) void groups_product_k(Groups q, Group
     const Wide z{r.N, r.K, rows, steps, r.dz + (size_t)s.begin * r.N, r.x + (size_t)s.begin * r.K, 1, r.N, 1, r.K,
                  r.dzp + (r.dz_padded / 32) * block, r.xp + (r.x_padded / 32) * block, r.dzs + g * r.dz_padded, r.xs + g * r.x_padded, nullptr, nullptr,
                  r.waiting, 0, 0, 0, 1};
-    wide_tile<kTile, kPasses>(z, DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, r.K}, dw, mt, nt, 0, steps, g * tiles + tile, lds);
+    size_t from = 0, to = steps;
+    if (r.parts) {
+        from = (size_t)part << (r.part_shift - 4);
+        to = min(steps, from + ((size_t)1 << (r.part_shift - 4)));
+    }
+    wide_tile<kTile, kPasses, kStages>(z, DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, r.K}, dw, mt, nt, from, to, item * tiles + tile, lds);
 }
 
 // ------------------------------------------------------------------------------------------------ the host's side
@@ -329,10 +344,11 @@ template <int kTile, bool kPasses>
 int launch_tiles(const Groups &q, const GroupProducts &p)
 {
     static bool raised = false;
+    constexpr int lds = kLdsOf<kTile, 3>;
     const auto kernel = groups_product_k<kTile, kPasses>;
-    if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsOf<kTile>));
+    if (!raised) DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     raised = true;
-    hipLaunchKernelGGL(kernel, dim3(8 * (p.rows_per + p.weights_per)), dim3(2 * kTile), kLdsOf<kTile>, stream(), q, p);
+    hipLaunchKernelGGL(kernel, dim3(8 * (p.rows_per + p.weights_per)), dim3(2 * kTile), lds, stream(), q, p);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
@@ -360,6 +376,20 @@ size_t tile_for(size_t G, size_t M, size_t N, size_t K)
 namespace dopt {
 
 static size_t tune(const char *k, size_t d) { const char *v = getenv(k); return v ? strtoull(v, 0, 10) : d; }
+int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const float *pre, float *dz, float *sums)
+{
+    ColumnJobs jobs{};
+    const unsigned tiles = (unsigned)ceil_div((size_t)l.N, (size_t)256);
+    const size_t blocks = tiles * most_units(l.q.M, l.q.G, shift);
+    DOPT_REQUIRE(blocks < ((size_t)1 << 24), "dopt_hip_dense_groups_grad: dimensions too large");
+    jobs.j[0] = Columns{dy, pre, dz, sums, nullptr, l.N, act, tiles, 0, (unsigned)blocks};
+    jobs.n = 1;
+    jobs.shift = shift;
+    hipLaunchKernelGGL(groups_columns_k, dim3((unsigned)blocks), dim3(256), 0, stream(), l.q, jobs);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
 bool groups_wide_takes(size_t G, size_t M, size_t N, size_t K)
 {
     if (getenv("G_WIDE")) return tune("G_WIDE", 0);
@@ -410,7 +440,12 @@ int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float 
     int shift = kStepShift;   // rows of a run of sums and largest magnitudes: every tile of a turned layout reads all of a group's
     while ((M / G >> shift) > 64) shift++;
     const size_t runs = most_units(M, G, shift), w_runs = ceil_div(N, (size_t)kWeightRun);
-    const bool plain = act == DOPT_HIP_ACT_NONE, passes = (dx && steps > kPass) || (dw && M > kPass * 16);
+    // Few tiles of dw: a group's reduction in parts, whose matrices are written and read once more.
+    int part_shift = 13;
+    while (part_shift > 8 && most_units(M, G, part_shift) * wtiles < (size_t)num_cus() * (tile == kBig ? 1 : 2)) part_shift--;
+    const bool parted = dw && G * wtiles * 2 < (size_t)num_cus() * (tile == kBig ? 1 : 2) && M > (size_t)1 << part_shift;
+    const size_t items = parted ? most_units(M, G, part_shift) : G, most_rows = parted ? (size_t)1 << part_shift : M;
+    const bool plain = act == DOPT_HIP_ACT_NONE, passes = (dx && steps > kPass) || (dw && most_rows > kPass * 16);
     ColumnJobs jobs{};
     GroupLayout lay{};
     GroupProducts p{};
@@ -444,8 +479,9 @@ int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float 
             lay.across[1] = RowsAcross{x, K, padded_k, s.take(units * 64 * padded_k * 4), s.take<int>(G * padded_k), x_tops, shift,
                                        (unsigned)(units * (padded_k / 64))};
             p.weights = WeightsProduct{dz, x, N, K, padded_n, padded_k, lay.across[0].parts, lay.across[1].parts, lay.across[0].shift, lay.across[1].shift,
-                                       dw, passes ? s.take(G * wtiles * tile * tile * 4) : nullptr, (unsigned)(padded_n / tile), (unsigned)ktiles};
-            p.weights_per = (unsigned)(G * ceil_div(wtiles, (size_t)8));
+                                       dw, parted ? s.take<float>(items * N * K) : nullptr, passes ? s.take(items * wtiles * tile * tile * 4) : nullptr,
+                                       (unsigned)(padded_n / tile), (unsigned)ktiles, part_shift};
+            p.weights_per = (unsigned)(items * ceil_div(wtiles, (size_t)8));
         }
         return s.bytes;
     };
@@ -474,7 +510,8 @@ int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float 
     hipLaunchKernelGGL(groups_layout_k, dim3(lay.rows.blocks + lay.turned.blocks + lay.across[0].blocks + lay.across[1].blocks + lay.rest_blocks), dim3(256), 0,
                        stream(), l.q, lay);
     DOPT_LAUNCH_CHECK();
-    return launch_products(l.q, tile, passes, p);
+    if (int rc = launch_products(l.q, tile, passes, p)) return rc;
+    return parted ? groups_join(l, part_shift, p.weights.parts, dw) : DOPT_HIP_OK;
 }
 
 }  // namespace dopt

@@ -211,6 +211,7 @@ __device__ __forceinline__ void bring_both(const char *left, const char *right, 
 // Tiles of 256 x 256 by eight wavefronts of 128 x 64: the accumulators are half of the registers, and a stage, 32 KB, feeds 24 matrix
 // instructions of each.  The halves of the workgroup, which share the CU's four SIMDs, read and multiply in turn; three stages are on
 // their way.  (Reading and multiplying together, between one barrier per stage, took 908 us where this takes 815.)
+template <int>
 __device__ __forceinline__ void sums(const char *left, const char *right, int steps, int w, int lane, char *lds, v16f (&acc)[4][2])
 {
     const int wm = w >> 2, wn = w & 3;
@@ -244,10 +245,11 @@ __device__ __forceinline__ void sums(const char *left, const char *right, int st
     meet();
 }
 
-// Tiles of 128 x 128 by four of 64 x 64, two workgroups to a CU.
+// Tiles of 128 x 128 by four of 64 x 64, two workgroups to a CU with five stages, three with three.
+template <int kStages>
 __device__ __forceinline__ void sums(const char *left, const char *right, int steps, int w, int lane, char *lds, v16f (&acc)[2][2])
 {
-    pipeline<5, 16384, 4, 2, 2>(
+    pipeline<kStages, 16384, 4, 2, 2>(
         lds, steps, [&](int k, char *to) { bring_both(left, right, k, w, lane, 8192, to); },
         [&](const char *now, Side<2> &a, Side<2> &b) {
             a.read(now + (w >> 1) * 4096, lane);
@@ -279,13 +281,13 @@ __device__ __forceinline__ void waiting_sums(v16f (&acc)[MI][2], char *at, bool 
         }
 }
 
-template <int kTile>
-constexpr int kLdsOf = kTile == kBig ? 4 * 32768 : 5 * 16384;
+template <int kTile, int kStages = 5>
+constexpr int kLdsOf = kTile == kBig ? 4 * 32768 : kStages * 16384;
 
 // A tile (mt, nt) of a product, the blocks [from, to) of its reduction, to y.  place_of_tile: which place among those that wait is its.
 // kPasses: some part of a reduction is longer than a pass.  (The loop by itself, with its registers, takes 1.6 % of both gradients of
 // [1000 x 1777] from 1111 where it runs once.)
-template <int kTile, bool kPasses>
+template <int kTile, bool kPasses, int kStages = 5>
 __device__ __forceinline__ void wide_tile(const Wide &q, const DenseEpilogue &ep, float *y, unsigned mt, unsigned nt, size_t from, size_t to,
                                           unsigned place_of_tile, char *lds)
 {
@@ -303,14 +305,14 @@ __device__ __forceinline__ void wide_tile(const Wide &q, const DenseEpilogue &ep
         for (unsigned pass = 0;; pass++) {
             const size_t at = from + (to - from) * pass / passes, next = from + (to - from) * (pass + 1) / passes;
             zero_acc(acc);
-            sums(left + at * 2048, right + at * 2048, (int)(next - at), w, lane, lds, acc);
+            sums<kStages>(left + at * 2048, right + at * 2048, (int)(next - at), w, lane, lds, acc);
             if (passes == 1) break;
             waiting_sums(acc, waiting, pass > 0, pass + 1 < passes);
             if (pass + 1 == passes) break;
         }
     } else {
         zero_acc(acc);
-        sums(left + from * 2048, right + from * 2048, (int)(to - from), w, lane, lds, acc);
+        sums<kStages>(left + from * 2048, right + from * 2048, (int)(to - from), w, lane, lds, acc);
     }
 
     int *const shift = (int *)lds;
