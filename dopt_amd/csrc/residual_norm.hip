@@ -768,21 +768,29 @@ void with_form(const Form &f, F &&call)
     else call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 4>{}));
 }
 
-// How many workgroups of a kernel the chip holds at a time (0: the runtime does not say).  Asked once for each number of wavefronts.
-template <class K>
-size_t places_of(K kernel, unsigned threads, size_t lds)
+// How many workgroups of a kernel the chip holds at a time.  The runtime is asked once for each kernel and number of wavefronts, without the LDS that a
+// call adds: what that leaves room for is worked out, so that the answer never depends on the calls before.
+struct Places {
+    int of_cu[17];
+    size_t fixed[17];   // bytes of LDS of every launch
+};
+size_t places_of(Places &known, const void *kernel, unsigned threads, size_t lds)
 {
-    static size_t known[17] = {};
-    size_t &places = known[threads / 64];
-    if (!places) {
-        int of_cu = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&of_cu, reinterpret_cast<const void *>(kernel), (int)threads, lds) != hipSuccess) {
+    int &of_cu = known.of_cu[threads / 64];
+    size_t &fixed = known.fixed[threads / 64];
+    if (!of_cu) {
+        hipFuncAttributes a;
+        int n = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, (int)threads, 0) != hipSuccess || hipFuncGetAttributes(&a, kernel) != hipSuccess) {
             (void)hipGetLastError();
-            of_cu = 0;
+            n = 1;
+            a.sharedSizeBytes = 0;
         }
-        places = (size_t)num_cus() * (size_t)std::max(1, of_cu);
+        fixed = a.sharedSizeBytes;
+        of_cu = std::max(1, n);
     }
-    return places;
+    const size_t room = (size_t)160 * 1024 / std::max<size_t>(1, fixed + lds);
+    return (size_t)num_cus() * std::max<size_t>(1, std::min((size_t)of_cu, room));
 }
 
 struct Launch {
@@ -799,7 +807,8 @@ int grad_launch(unsigned threads, size_t lds, Launch *l)
         DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 159 * 1024));
         raised = true;
     }
-    *l = Launch{(const void *)kernel, threads, lds, places_of(kernel, threads, lds)};
+    static Places known{};
+    *l = Launch{(const void *)kernel, threads, lds, places_of(known, (const void *)kernel, threads, lds)};
     return DOPT_HIP_OK;
 }
 
@@ -886,7 +895,8 @@ int dopt_hip_residual_norm(const dopt_hip_residual_norm_desc *d, const float *x,
         with_form(form, [&](auto lanes, auto quads) {
             const auto kernel = join_k<lanes.value, quads.value>;
             // every workgroup loads the scales once: no more of them than run at a time, and as many rows for each
-            const size_t rounds = ceil_div(blocks, places_of(kernel, form.threads, 0));
+            static Places known{};
+            const size_t rounds = ceil_div(blocks, places_of(known, (const void *)kernel, form.threads, 0));
             hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(blocks, rounds)), dim3(form.threads), 0, stream(), n);
         });
     }

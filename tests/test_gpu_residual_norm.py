@@ -1,4 +1,8 @@
 """The residual norm and its gradient on the device against their float64 forms."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -7,6 +11,7 @@ from dopt_amd import capi, core, nnet, online, ops
 
 pytestmark = pytest.mark.gpu
 F32 = np.float32
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def _f(a):
@@ -224,6 +229,29 @@ def test_repeated_calls_give_the_same_bits():
     for _ in range(5):
         again = _check_backward(t, y, stats, "layer", "layer", 1.0)
         assert all(np.array_equal(first[k], again[k].numpy()) for k in first)
+
+
+_ORDER = """
+import hashlib, sys
+import numpy as np
+from dopt_amd import ops
+for cols in [int(c) for c in sys.argv[1:]]:
+    rows = 1 << 19 - cols.bit_length()
+    r = np.random.default_rng(cols)
+    x, b, dh = (ops.tensor(r.standard_normal((rows, cols), np.float32)) for _ in range(3))
+    gate, scale = ops.tensor(r.standard_normal((4, cols), np.float32)), ops.tensor(r.standard_normal(cols, np.float32))
+    y, h, stats = ops.residual_norm(x, b, gate, "none", None, None, "layer", scale, scale)
+    g = ops.residual_norm_grad(None, dh, y, b, stats, gate, "none", None, None, "layer", scale, scale)
+    out = b"".join(g[k].numpy().tobytes() for k in sorted(g))
+    print(cols, hashlib.sha256(out).hexdigest(), flush=True)
+"""
+
+
+def test_the_bits_do_not_depend_on_the_calls_before():
+    lengths = ["48", "128", "512", "1024", "2048", "4096"]
+    runs = [sorted(subprocess.run([sys.executable, "-c", _ORDER] + order, cwd=ROOT, capture_output=True, text=True, timeout=100, check=True)
+                   .stdout.splitlines()) for order in (lengths, lengths[::-1])]
+    assert len(runs[0]) == len(lengths) and runs[0] == runs[1]
 
 
 def test_sums_of_many_equal_rows():
