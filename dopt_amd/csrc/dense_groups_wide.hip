@@ -5,7 +5,6 @@
 // Rows of a group are laid out from a tile's boundary on, so that a tile holds rows of one group; the steps of dw's reductions from a boundary of
 // 64 rows on.  How many tiles there are is found on the device: an XCD takes an eighth of them, side by side.
 #include <algorithm>
-#include <cstdlib>
 
 #include "dense_groups.h"
 #include "dense_wide.h"
@@ -363,19 +362,27 @@ int shift_of_tile(size_t tile) { return tile == kBig ? 8 : 7; }
 // Threads of a workgroup that lays out rows of so many steps: in registers up to 1024.
 unsigned row_threads(size_t steps) { return steps > 512 ? 1024 : steps > 256 ? 512 : 256; }
 
-// The side of the tiles: large ones where they fill the chip and groups are long enough for them on average.
+// The side of the tiles: large ones for the largest products, of long groups (sixteen groups, [16384 x 4096] from 2048 steps: 1020 us, with small
+// ones 1035; four groups, [16384 x 1024] from 512: 133 and 106, gradients 279 and 285).
 size_t tile_for(size_t G, size_t M, size_t N, size_t K)
 {
-    if (getenv("G_TILE")) return strtoull(getenv("G_TILE"), 0, 10);
-    const size_t rows = ceil_div(M, (size_t)kBig) + G / 2, tiles = rows * ceil_div(N, (size_t)kBig);
-    return K >= 128 && M >= 384 * G && N >= 512 && tiles >= (size_t)num_cus() * 2 / 3 ? kBig : kSmall;
+    const size_t tiles = (ceil_div(M, (size_t)kBig) + G / 2) * ceil_div(N, (size_t)kBig);
+    return M >= 512 * G && M * N * K >= (size_t)30000000000 && tiles >= (size_t)num_cus() / 2 ? kBig : kSmall;
 }
+
+// What a product takes here and by the 32 x 32 tiles of dense_groups.hip, in us.  Here: launches, every byte that the layouts move, and the matrix
+// instructions over whole tiles (half of one more for each group).  There: launches, and operands that every tile reads by itself, from the L2; of
+// gradients also a workgroup for each tile of each group's dw.  Eight groups, here and there:
+//     [2048 x 512] from 512 37 28    [4096 x 512] from 512 39 46    [1024 x 1024] from 1024 51 45    [2048 x 1024] from 1024 56 77
+//     [256 x 4096] from 1024 85 65   [512 x 4096] from 1024 88 104   gradients [2048 x 512] from 512 59 56   [4096 x 512] 73 81
+//     [512 x 1024] from 1024 73 93   [1024 x 256] from 256 39 24
+double padded_rows(double G, double M) { return M + 64 * G; }
+double tiles32(double rows, double cols) { return (rows / 32 + 0.5) * ceil_div((size_t)cols, (size_t)32); }
 
 }  // namespace
 
 namespace dopt {
 
-static size_t tune(const char *k, size_t d) { const char *v = getenv(k); return v ? strtoull(v, 0, 10) : d; }
 int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const float *pre, float *dz, float *sums)
 {
     ColumnJobs jobs{};
@@ -390,15 +397,26 @@ int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const fl
     return DOPT_HIP_OK;
 }
 
+// A launch has fewer than 2^32 threads: the layouts' rows are four to a workgroup of at most 1024.
+static bool fits(size_t G, size_t M, size_t N, size_t K)
+{
+    const size_t most = (size_t)1 << 23;
+    return M + kBig * G < most && G * (N + K + 2 * kBig) < most && M / 64 * (ceil_div(N, (size_t)64) + ceil_div(K, (size_t)64)) < most;
+}
 bool groups_wide_takes(size_t G, size_t M, size_t N, size_t K)
 {
-    if (getenv("G_WIDE")) return tune("G_WIDE", 0);
-    return K >= 128 && N >= 128 && M >= 64 * G && M * N * K >= (size_t)900000000;
+    if (K < 128 || N < 128 || G == 0 || !fits(G, M, N, K)) return false;
+    const double g = (double)G, m = (double)M, n = (double)N, k = (double)K;
+    const double here = 29 + 8 * (m * k + g * n * k) / 5e6 + 6 * padded_rows(g, m) * n * k / 1.2e9;
+    return here < 5 + 256 * tiles32(m + 16 * g, n) * k / 6.8e6;
 }
 bool groups_wide_takes_grad(size_t G, size_t M, size_t N, size_t K)
 {
-    if (getenv("G_WIDE")) return tune("G_WIDE", 0);
-    return K >= 128 && N >= 128 && M >= 64 * G && M * N * K >= (size_t)900000000;
+    if (K < 128 || N < 128 || G == 0 || !fits(G, M, N, K)) return false;
+    const double g = (double)G, m = (double)M, n = (double)N, k = (double)K;
+    const double here = 36 + (28 * m * n + 16 * m * k + 16 * g * n * k) / 5e6 + 12 * padded_rows(g, m) * n * k / 1.2e9;
+    const double dw = tiles32(n, k);
+    return here < 10 + 256 * (tiles32(m + 16 * g, k) * n + dw * m) / 8e6 + 5e-3 * g * dw;
 }
 
 int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
@@ -426,7 +444,8 @@ int groups_wide(const GroupLayer &l, const float *x, const float *w, const float
     p.pre = pre;
     p.act = act;
     p.rows_per = (unsigned)ceil_div(mtiles * ntiles, (size_t)8);
-    hipLaunchKernelGGL(groups_layout_k, dim3(lay.rows.blocks + lay.weights.blocks + lay.rest_blocks), dim3(row_threads(steps)), 0, stream(), l.q, lay);
+    const unsigned threads = steps <= 128 ? 128 : row_threads(steps);   // (fewer wavefronts with more in flight: 4096 rows of 512 15.4 us, with 256 threads 18.8)
+    hipLaunchKernelGGL(groups_layout_k, dim3(lay.rows.blocks + lay.weights.blocks + lay.rest_blocks), dim3(threads), 0, stream(), l.q, lay);
     DOPT_LAUNCH_CHECK();
     return launch_products(l.q, tile, passes, p);
 }
@@ -434,7 +453,7 @@ int groups_wide(const GroupLayer &l, const float *x, const float *w, const float
 int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
 {
     const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, steps = ceil_div(N, (size_t)16);
-    const size_t tile = getenv("G_TILE") ? strtoull(getenv("G_TILE"), 0, 10) : std::min(tile_for(G, M, K, N), dw ? G * ceil_div(N, (size_t)kBig) * ceil_div(K, (size_t)kBig) >= (size_t)num_cus() ? (size_t)kBig : (size_t)kSmall : (size_t)kBig);
+    const size_t tile = dw && G * ceil_div(N, (size_t)kBig) * ceil_div(K, (size_t)kBig) < (size_t)num_cus() ? (size_t)kSmall : tile_for(G, M, K, N);
     const size_t mtiles = most_units(M, G, shift_of_tile(tile)), rows = mtiles * tile, padded_n = padded_to(N, tile), padded_k = padded_to(K, tile);
     const size_t ktiles = padded_k / tile, wtiles = padded_n / tile * ktiles, units = most_units(M, G, kStepShift);
     int shift = kStepShift;   // rows of a run of sums and largest magnitudes: every tile of a turned layout reads all of a group's
