@@ -21,9 +21,32 @@ int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float 
 // dz (which may be null) of N >= 4 columns, and the sums (null too) of runs of 2^shift rows of a group.
 int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const float *pre, float *dz, float *sums);
 
-// dense_groups.hip: dbias from the sums of runs of 2^shift rows of a group; dw from the matrices of such parts, of which an empty group has one of zeros.
-int groups_fold(const GroupLayer &l, int shift, const float *sums, float *dbias);
+// dense_groups.hip: dw from the matrices of parts of 2^shift rows of a group, of which an empty group has one of zeros.
 int groups_join(const GroupLayer &l, int shift, const float *parts, float *dw);
+
+// dbias from the sums of runs of 2^shift rows of a group: `lanes` lanes to a column, of 32 side by side; red: a value of each.
+__device__ __forceinline__ void fold_runs(const GroupLayer &l, int shift, const float *sums, float *dbias, unsigned tile, unsigned group, int lanes,
+                                          float (*red)[33])
+{
+    const int c = (int)tile * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
+    const Segment s = find_group(l.q, shift, group);
+    if (s.group < 0) return;
+    float all = 0.0f;
+    if (c < l.N) {
+        const float *const from = sums + (size_t)s.first * l.N + c;
+        for (unsigned i0 = (unsigned)lane; i0 < s.unit; i0 += 64 * lanes) {   // sums of 64 values each
+            float sum = 0.0f;
+#pragma unroll 4
+            for (unsigned i = i0; i < min(s.unit, i0 + 64 * lanes); i += lanes) sum += from[(size_t)i * l.N];
+            all += sum;
+        }
+    }
+    red[lane][threadIdx.x & 31] = all;
+    __syncthreads();
+    if (lane || c >= l.N) return;
+    for (int i = 1; i < lanes; i++) all += red[i][threadIdx.x];
+    dbias[(size_t)s.group * l.N + c] = all;
+}
 
 constexpr unsigned kGridRow = 65535;   // units along the second side of a grid; more go to the third
 __device__ __forceinline__ unsigned unit_id() { return blockIdx.z * kGridRow + blockIdx.y; }

@@ -89,30 +89,6 @@ __device__ __forceinline__ void small_dw(const GroupLayer &l, const SmallGrads &
                                          (int)by, 0, rows, red);
 }
 
-// `lanes` lanes to a column, of 32 side by side; red: a value of each.
-__device__ __forceinline__ void fold_runs(const GroupLayer &l, int shift, const float *sums, float *dbias, unsigned tile, unsigned group, int lanes,
-                                          float (*red)[33])
-{
-    const int c = (int)tile * 32 + (int)(threadIdx.x & 31), lane = (int)threadIdx.x >> 5;
-    const Segment s = find_group(l.q, shift, group);
-    if (s.group < 0) return;
-    float all = 0.0f;
-    if (c < l.N) {
-        const float *const from = sums + (size_t)s.first * l.N + c;
-        for (unsigned i0 = (unsigned)lane; i0 < s.unit; i0 += 64 * lanes) {   // sums of 64 values each
-            float sum = 0.0f;
-#pragma unroll 4
-            for (unsigned i = i0; i < min(s.unit, i0 + 64 * lanes); i += lanes) sum += from[(size_t)i * l.N];
-            all += sum;
-        }
-    }
-    red[lane][threadIdx.x & 31] = all;
-    __syncthreads();
-    if (lane || c >= l.N) return;
-    for (int i = 1; i < lanes; i++) all += red[i][threadIdx.x];
-    dbias[(size_t)s.group * l.N + c] = all;
-}
-
 constexpr unsigned kRow = 1u << 22;   // workgroups of a row of such a grid
 template <bool kCut>
 __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_grad_k(GroupLayer l, SmallGrads g)
@@ -168,13 +144,6 @@ __global__ __launch_bounds__(256) void groups_dz_k(GroupLayer l, int act, const 
     });
     if (sums) sums[(size_t)unit_id() * l.N + c] = sum;
 }
-// dbias by itself: 32 columns of a group by 32 lanes.
-__global__ __launch_bounds__(1024) void groups_fold_k(GroupLayer l, int shift, const float *sums, float *dbias)
-{
-    __shared__ float red[32][33];
-    fold_runs(l, shift, sums, dbias, blockIdx.x, unit_id(), 32, red);
-}
-
 __global__ __launch_bounds__(256) void groups_zero_k(size_t n, float *p)
 {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0.0f;
@@ -219,13 +188,6 @@ int apart(const char *who, const Span (&in)[I], const Span (&out)[O])
 }  // namespace
 
 namespace dopt {
-
-int groups_fold(const GroupLayer &l, int shift, const float *sums, float *dbias)
-{
-    hipLaunchKernelGGL(groups_fold_k, grid_of(ceil_div((size_t)l.N, (size_t)32), l.q.G), dim3(1024), 0, stream(), l, shift, sums, dbias);
-    DOPT_LAUNCH_CHECK();
-    return DOPT_HIP_OK;
-}
 
 int groups_join(const GroupLayer &l, int shift, const float *parts, float *dw)
 {

@@ -161,6 +161,11 @@ struct GroupLayout {
     WeightsJob weights;
     WeightsAcross turned;
     RowsAcross across[2];
+    // dbias of runs of 2^fold_shift rows, 32 columns to a block
+    const float *sums;
+    float *dbias;
+    int columns, fold_shift;
+    unsigned fold_tiles, fold_blocks;
     // rows of no group, of up to two results: cleared by so many blocks
     float *rest[2];
     size_t rest_cols[2];
@@ -230,6 +235,11 @@ __global__ __launch_bounds__(1024) void groups_layout_k(Groups q, GroupLayout l)
                         j.tops + (size_t)first_run * j.rows, (int)((K + ((size_t)1 << j.run_shift) - 1) >> j.run_shift), 0};
         return turn_tile(o, (size_t)(block % tiles) * 64, (size_t)s.unit * 64);
     }
+    if (block < l.fold_blocks) {
+        __shared__ float red[8][33];
+        return fold_runs(GroupLayer{q, l.columns, 0}, l.fold_shift, l.sums, l.dbias, block % l.fold_tiles, block / l.fold_tiles, 8, red);
+    }
+    block -= l.fold_blocks;
     for (int i = 0; i < 2; i++) clear_rest(q, l.rest[i], l.rest_cols[i], block, l.rest_blocks);
 }
 
@@ -513,21 +523,26 @@ int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float 
     for (int i = 0; i < jobs.n; i++) blocks += jobs.j[i].blocks;
     if (blocks) hipLaunchKernelGGL(groups_columns_k, dim3(blocks), dim3(256), 0, stream(), l.q, jobs);
     DOPT_LAUNCH_CHECK();
-    if (dbias)
-        if (int rc = groups_fold(l, shift, sums, dbias)) return rc;
-    if (!dx && !dw) return DOPT_HIP_OK;
+    if (dbias) {
+        lay.sums = sums;
+        lay.dbias = dbias;
+        lay.columns = (int)N;
+        lay.fold_shift = shift;
+        lay.fold_tiles = (unsigned)ceil_div(N, (size_t)32);
+        lay.fold_blocks = (unsigned)G * lay.fold_tiles;
+    }
     lay.rest[0] = dx;
     lay.rest_cols[0] = K;
     lay.rest_blocks = dx ? (unsigned)num_cus() : 0;
     const unsigned threads = row_threads(steps);
     if (dx && threads != 256) {   // rows by workgroups of their length, turned tiles by 256 threads
         GroupLayout alone = lay;
-        alone.turned.blocks = alone.across[0].blocks = alone.across[1].blocks = alone.rest_blocks = 0;
+        alone.turned.blocks = alone.across[0].blocks = alone.across[1].blocks = alone.fold_blocks = alone.rest_blocks = 0;
         hipLaunchKernelGGL(groups_layout_k, dim3(alone.rows.blocks), dim3(threads), 0, stream(), l.q, alone);
         lay.rows.blocks = 0;
     }
-    hipLaunchKernelGGL(groups_layout_k, dim3(lay.rows.blocks + lay.turned.blocks + lay.across[0].blocks + lay.across[1].blocks + lay.rest_blocks), dim3(256), 0,
-                       stream(), l.q, lay);
+    const unsigned all = lay.rows.blocks + lay.turned.blocks + lay.across[0].blocks + lay.across[1].blocks + lay.fold_blocks + lay.rest_blocks;
+    hipLaunchKernelGGL(groups_layout_k, dim3(all), dim3(256), 0, stream(), l.q, lay);
     DOPT_LAUNCH_CHECK();
     if (int rc = launch_products(l.q, tile, passes, p)) return rc;
     return parted ? groups_join(l, part_shift, p.weights.parts, dw) : DOPT_HIP_OK;
