@@ -411,7 +411,8 @@ int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const fl
 static bool fits(size_t G, size_t M, size_t N, size_t K)
 {
     const size_t most = (size_t)1 << 23;
-    return M + kBig * G < most && G * (N + K + 2 * kBig) < most && M / 64 * (ceil_div(N, (size_t)64) + ceil_div(K, (size_t)64)) < most;
+    return M + kBig * G < most && G * (N + K + 2 * kBig) < most && M / 64 * (ceil_div(N, (size_t)64) + ceil_div(K, (size_t)64)) < most &&
+           G * ceil_div(N, (size_t)64) * ceil_div(K, (size_t)64) < most;
 }
 bool groups_wide_takes(size_t G, size_t M, size_t N, size_t K)
 {

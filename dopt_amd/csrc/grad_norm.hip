@@ -39,6 +39,7 @@ struct Handle {
     Chunk *chunks = nullptr;
     double *parts = nullptr;    // a block's sum
     unsigned *arrived = nullptr;   // counts of them; zero between two calls
+    std::vector<dopt_hip_gradient_ref> refs;
 };
 
 // The workgroup's sum, in every thread.
@@ -175,6 +176,9 @@ int norm(const Handle *h, float most, float *result, const char *who)
 {
     DOPT_REQUIRE(result != nullptr, "%s: the result is null", who);
     DOPT_REQUIRE(most >= 0.0f, "%s: the largest norm is %g", who, (double)most);
+    for (const dopt_hip_gradient_ref &r : h->refs)
+        DOPT_REQUIRE(!overlaps(result, 2 * sizeof(float), r.g, r.n * sizeof(float)) && !overlaps(result, 2 * sizeof(float), r.out, r.n * sizeof(float)),
+                     "%s: the norm's place lies in a gradient", who);
     hipLaunchKernelGGL(gradient_squares_k, dim3(h->blocks), dim3(kBlock), 0, stream(), h->tensors, h->chunks, h->nchunks, h->parts, h->arrived, most, result);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
@@ -204,6 +208,7 @@ int dopt_hip_gradient_norm_create(int ntensors, const dopt_hip_gradient_ref *ref
     DOPT_ENSURE_INIT();
     Handle *h = new Handle();
     h->has_out = has_out;
+    h->refs.assign(refs, refs + ntensors);
     h->nchunks = chunks.size();
     h->blocks = (unsigned)std::max((size_t)1, std::min(chunks.size(), (size_t)num_cus() * 4));
     int rc = dopt_hip_malloc((void **)&h->parts, h->blocks * sizeof(double));

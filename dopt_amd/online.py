@@ -23,11 +23,15 @@ def _newbufs(variables):
     return [v.device_ptr()[0] for v in variables]
 
 
+def _check_norm(maxNorm):
+    if maxNorm is not None and not maxNorm >= 0:
+        raise ValueError("The largest norm is %r" % (maxNorm,))
+
+
 def clipped(grads, maxNorm):
     """The gradients times min(1, maxNorm / norm), norm the square root of the sum of all their squares; as they are where maxNorm
     is None.  A gradient that stands for several parameters counts for each.  No counterpart in the reference."""
-    if maxNorm is not None and not maxNorm >= 0:
-        raise ValueError("The largest norm is %r" % (maxNorm,))
+    _check_norm(maxNorm)
     if maxNorm is None or np.isinf(maxNorm) or not grads:
         return list(grads)
     total = None
@@ -169,6 +173,7 @@ class _Placeholder:
 
 class _FusedUpdater:
     def __init__(self, rule, outputs, wrt, projs, hyper, flags, maxNorm=None):
+        _check_norm(maxNorm)
         projs = projs or {}
         self.rule, self.hyper, self.outputs, self.wrt = rule, hyper, list(outputs), list(wrt)
         grads = grad(outputs[0], wrt)

@@ -115,6 +115,16 @@ def test_clipping_needs_places():
         ops.GradientNorm([ops.Tensor((4,), np.int32)])
 
 
+def test_the_norms_place_is_apart_from_the_gradients():
+    g, out = ops.tensor(np.arange(9, dtype=np.float32)), ops.Tensor((9,))
+    n = ops.GradientNorm([g], [out])
+    for t in (g, out):
+        for call in (n.norm, n.clip):
+            with pytest.raises(capi.HipError, match="lies in a gradient"):
+                call(1.0, out=t.view(7, (2,)))
+    assert not out.numpy().any() and np.array_equal(g.numpy(), np.arange(9))
+
+
 def test_repeated_calls_give_the_same_bits():
     grads = _gradients([1 << 20, 333, 70000], 4)
     n = ops.GradientNorm([ops.tensor(g) for g in grads])

@@ -47,3 +47,11 @@ def test_gradients_in_a_graph():
     for bad in (-1.0, float("nan")):
         with pytest.raises(ValueError, match="largest norm"):
             online.clipped(g, bad)
+
+
+@pytest.mark.parametrize("rule", ["fused_sgd", "fused_adam", "fused_amsgrad", "fused_muon"])
+def test_fused_updaters_refuse_a_norm_that_is_none(rule):
+    x = core.float32([3])
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="largest norm"):
+            getattr(online, rule)([core.sum(x * x)], [x], maxNorm=bad)
