@@ -12,17 +12,25 @@ struct GroupLayer {
     int N, K;   // of w_g [N, K]
 };
 
-// Large products, of two fp16 parts of each value.
-bool groups_wide_takes(size_t G, size_t M, size_t N, size_t K);        // y [M, N] from K steps
-bool groups_wide_takes_grad(size_t G, size_t M, size_t N, size_t K);   // dx and dw
+// The ways of such products besides the small ones' (dense_groups.hip): of two fp16 parts of each value that are made on the way (dense_groups_split.hip)
+// or laid out once (dense_groups_wide.hip).  What each takes of y [M, N] from K steps and of its gradients, in us, or infinity where it cannot.
+double groups_split_us(size_t G, size_t M, size_t N, size_t K);
+double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K);
+double groups_wide_us(size_t G, size_t M, size_t N, size_t K);
+double groups_wide_grad_us(size_t G, size_t M, size_t N, size_t K);
+int groups_split(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
 int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
 // dy and pre give dz, which is written where there is an activation; any result may be null.
+int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
 int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
 // dz (which may be null) of N >= 4 columns, and the sums (null too) of runs of 2^shift rows of a group.
 int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const float *pre, float *dz, float *sums);
 
 // dense_groups.hip: dw from the matrices of parts of 2^shift rows of a group, of which an empty group has one of zeros.
 int groups_join(const GroupLayer &l, int shift, const float *parts, float *dw);
+
+// Tiles of `side` rows and columns, half of one more for each group.
+inline double group_tiles(size_t G, size_t M, size_t N, size_t side) { return ((double)M / side + 0.5 * G) * ceil_div(N, side); }
 
 // dbias from the sums of runs of 2^shift rows of a group: `lanes` lanes to a column, of 32 side by side; red: a value of each.
 __device__ __forceinline__ void fold_runs(const GroupLayer &l, int shift, const float *sums, float *dbias, unsigned tile, unsigned group, int lanes,

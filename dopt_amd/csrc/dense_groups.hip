@@ -169,6 +169,22 @@ int check(const char *who, size_t G, size_t M, size_t N, size_t K, int act)
     return DOPT_HIP_OK;
 }
 
+// What the small products take, in us: launches, and operands that every tile of 32 x 32 reads by itself, from the L2; of gradients also a workgroup for each
+// tile of each group's dw.  The way that takes the least is taken.  Eight groups, small, split and wide:
+//     [64 x 512] from 512 7.4 10.7 29       [1024 x 512] from 512 19 13 36       [4096 x 512] from 512 46 28 39       [16384 x 512] from 512 156 79 70
+//     [1024 x 1024] from 1024 45 28 51      [8192 x 1024] from 1024 279 123 107  [512 x 4096] from 1024 104 50 85
+// and gradients
+//     [128 x 256] from 256 12 14 30         [1024 x 512] from 512 39 30 54       [4096 x 512] from 512 81 58 73       [16384 x 512] from 512 256 212 177
+//     [2048 x 1024] from 1024 171 87 90     [8192 x 1024] from 1024 436 301 221  [256 x 4096] from 1024 269 130 243
+double small_us(size_t G, size_t M, size_t N, size_t K) { return 5 + 256 * group_tiles(G, M, N, 32) * K / 6.8e6; }
+double small_grad_us(size_t G, size_t M, size_t N, size_t K)
+{
+    const double dw = ((double)N / 32 + 0.5) * ceil_div(K, (size_t)32);
+    return 10 + 256 * (group_tiles(G, M, K, 32) * N + dw * M) / 6.3e6 + 5e-3 * G * dw;
+}
+enum class Way { kSmall, kSplit, kWide };
+Way way_of(double small, double split, double wide) { return small <= std::min(split, wide) ? Way::kSmall : split <= wide ? Way::kSplit : Way::kWide; }
+
 size_t slice_of(size_t depth) { return ceil_div(ceil_div(depth, (size_t)kSmallWaves), (size_t)8) * 8; }
 
 struct Span {
@@ -214,7 +230,9 @@ int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const
     if (int rc = apart(who, in, results)) return rc;
     DOPT_ENSURE_INIT();
     const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
-    if (G > 0 && groups_wide_takes(G, M, N, K)) return groups_wide(l, x, w, bias, act, y, pre);
+    const Way way = way_of(small_us(G, M, N, K), groups_split_us(G, M, N, K), groups_wide_us(G, M, N, K));
+    if (G > 0 && way == Way::kSplit) return groups_split(l, x, w, bias, act, y, pre);
+    if (G > 0 && way == Way::kWide) return groups_wide(l, x, w, bias, act, y, pre);
     const dim3 grid = grid_of(ceil_div(N, (size_t)32), most_units(M, G + 2, kTileShift));
     const int slice = (int)slice_of(K);
     if (K % 4) hipLaunchKernelGGL(groups_small_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
@@ -248,7 +266,9 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
         return clear(dbias, G * N);
     }
     const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
-    if ((dx || dw) && groups_wide_takes_grad(G, M, N, K)) return groups_wide_grad(l, act, dy, pre, x, w, dx, dw, dbias);
+    const Way way = way_of(small_grad_us(G, M, N, K), groups_split_grad_us(G, M, N, K), groups_wide_grad_us(G, M, N, K));
+    if ((dx || dw) && way == Way::kSplit) return groups_split_grad(l, act, dy, pre, x, w, dx, dw, dbias);
+    if ((dx || dw) && way == Way::kWide) return groups_wide_grad(l, act, dy, pre, x, w, dx, dw, dbias);
     // Rows of a part of a group's reduction: at most 8192, 1024 for each wavefront, so that sums of one sign are not rounded the same way for
     // long; fewer where the tiles would not fill the chip (a part's matrix is written and read).
     const size_t tiles = ceil_div(N, (size_t)32) * ceil_div(K, (size_t)32);

@@ -1,0 +1,216 @@
+// Products of middle size of dense layers of groups: tiles of 64 x 64 whose operands become two fp16 parts on the way (split_tile.h), so that nothing is laid
+// out and read again in front of them.  Small enough a tile to have some thousand of them; a workgroup's teams share a reduction where there
+// are fewer than the chip holds.
+//
+// Bound by what a chunk of 32 steps costs where it is not the matrix instructions' 192 cycles: 110 vector instructions of each wavefront (450 cycles of a
+// SIMD), 300 cycles of LDS, and with few tiles the way from memory to the sums, some 0.9 us a chunk.  [16384 x 4096] from 2048 in sixteen groups
+// takes 830 cycles a chunk.  Tiles of 128 x 64 and 128 x 128 do more with a value that LDS holds, but leave two wavefronts to a SIMD, which hide less:
+// that product in 1270 and 1130 us for 1450, [1024 x 1024] from 1024 in eight groups in 38 and 53 for 32.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "dense_groups.h"
+#include "split_tile.h"
+
+namespace {
+
+using namespace dopt;
+
+constexpr int kTile = kSplitTile, kTileShift = 6;
+constexpr int kRunShift = 6;
+
+// y = act(x w^T + bias): a tile of rows of a group.
+template <int kTeams, bool kPasses>
+__global__ __launch_bounds__(256 * kTeams) void groups_split_k(GroupLayer l, const float *x, const float *w, const float *bias, float *y, float *pre, int act)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const unsigned n0 = blockIdx.x * kTile;
+    if (n0 >= (unsigned)l.N) return;
+    const Segment s = find_unit<true>(l.q, kTileShift, unit_id());
+    if (s.group < 0) return;
+    const size_t N = l.N, K = l.K;
+    if (s.group == (int)l.q.G) {
+        const size_t row = s.begin + ((size_t)s.unit << kTileShift);
+        const int rows = (int)min(s.end - row, (size_t)kTile);
+        for (int i = threadIdx.x; i < kTile * rows; i += 256 * kTeams) {
+            const unsigned c = n0 + i % kTile;
+            if (c >= N) continue;
+            const size_t at = (row + i / kTile) * N + c;
+            y[at] = 0.0f;
+            if (pre) pre[at] = 0.0f;
+        }
+        return;
+    }
+    const size_t begin = s.begin, g = (size_t)s.group;
+    const DenseEpilogue ep{bias ? bias + g * N : nullptr, nullptr, pre ? pre + begin * N : nullptr, act, N};
+    split_tile<kTeams, false, false, kPasses>(Matrix32{x + begin * K, K, s.end - s.begin}, Matrix32{w + g * N * K, K, (unsigned)N}, (unsigned)K,
+                                                s.unit << kTileShift, n0, ep, y + begin * N, lds);
+}
+
+// The gradients in one launch, as dense_groups.hip's: dx = dz w, dw = dz^T x over 2^shift rows of a group, dbias.
+struct SplitGrads {
+    const float *dz, *x, *w, *sums;
+    float *dx, *dw, *parts, *dbias;   // parts: or null
+    int shift;
+    unsigned dx_tiles, dw_tiles, fold_tiles;
+    size_t dx_blocks, dw_blocks, fold_blocks;
+};
+constexpr unsigned kRow = 1u << 22;   // workgroups of a row of the grid
+
+template <int kTeams, bool kPasses>
+__global__ __launch_bounds__(256 * kTeams) void groups_split_grad_k(GroupLayer l, SplitGrads g)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    size_t block = (size_t)blockIdx.y * kRow + blockIdx.x;
+    const size_t N = l.N, K = l.K;
+    if (block < g.dx_blocks) {
+        const unsigned k0 = (unsigned)(block % g.dx_tiles) * kTile;
+        if (k0 >= K) return;
+        const Segment s = find_unit<true>(l.q, kTileShift, (unsigned)(block / g.dx_tiles));
+        if (s.group < 0) return;
+        const size_t begin = s.begin;
+        if (s.group == (int)l.q.G) {
+            const size_t row = begin + ((size_t)s.unit << kTileShift);
+            const int rows = (int)min(s.end - row, (size_t)kTile);
+            for (int i = threadIdx.x; i < kTile * rows; i += 256 * kTeams)
+                if (k0 + i % kTile < K) g.dx[(row + i / kTile) * K + k0 + i % kTile] = 0.0f;
+            return;
+        }
+        return split_tile<kTeams, false, true, kPasses>(Matrix32{g.dz + begin * N, N, s.end - s.begin}, Matrix32{g.w + s.group * N * K, K, (unsigned)K},
+                                                          (unsigned)N, s.unit << kTileShift, k0,
+                                                          DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, g.dx + begin * K, lds);
+    }
+    block -= g.dx_blocks;
+    if (block < g.dw_blocks) {
+        const unsigned tile = (unsigned)(block % g.dw_tiles), unit = (unsigned)(block / g.dw_tiles), across = (unsigned)((K + kTile - 1) / kTile);
+        const unsigned k0 = tile % across * kTile, n0 = tile / across * kTile;
+        if (n0 >= N) return;
+        const Segment s = find_unit<false, true>(l.q, g.shift, unit);
+        if (s.group < 0) return;
+        const size_t row = s.begin + ((size_t)s.unit << g.shift);
+        const unsigned rows = (unsigned)min((size_t)s.end - row, (size_t)1 << g.shift);
+        float *const to = g.parts ? g.parts + unit * N * K : g.dw + s.group * N * K;
+        if (rows == 0) {
+            for (int i = threadIdx.x; i < kTile * kTile; i += 256 * kTeams)
+                if (n0 + i / kTile < N && k0 + i % kTile < K) to[(n0 + i / kTile) * K + k0 + i % kTile] = 0.0f;
+            return;
+        }
+        return split_tile<kTeams, true, true, kPasses>(Matrix32{g.dz + row * N, N, (unsigned)N}, Matrix32{g.x + row * K, K, (unsigned)K}, rows, n0, k0,
+                                                         DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, to, lds);
+    }
+    block -= g.dw_blocks;
+    if (block < g.fold_blocks)
+        fold_runs(l, kRunShift, g.sums, g.dbias, (unsigned)(block % g.fold_tiles), (unsigned)(block / g.fold_tiles), 8 * kTeams, (float(*)[33])lds);
+}
+
+constexpr int kLongestPart = 13;
+// Rows of a part of a group's reduction, as a shift: fewer where the tiles would not fill the chip (a part's matrix is written and read).
+int part_shift(size_t G, size_t M, size_t tiles)
+{
+    int shift = kLongestPart;
+    while (shift > 8 && most_units(M, G, shift) * tiles < (size_t)num_cus()) shift--;
+    return shift;
+}
+// Tiles of both products, and chunks of each.
+struct GradWork {
+    double dx_tiles, dx_chunks, dw_tiles, dw_chunks;
+    double chain() const { return std::max(dx_chunks, dw_chunks); }
+    // One workgroup's chunks take longer than all of them over the chip's: [1024 x 512] from 512 in eight groups with one team 31.2 us, with two 29.6,
+    // [2048 x 512] 38.9 and 40.9, [256 x 4096] from 1024 150 and 130, [1024 x 4096] 180 and 201.  (Four teams gain nothing further.)
+    bool few() const { return dx_tiles * dx_chunks + dw_tiles * dw_chunks < 1.5 * chain() * num_cus(); }
+};
+GradWork grad_work(size_t G, size_t M, size_t N, size_t K)
+{
+    const size_t tiles = ceil_div(N, (size_t)kTile) * ceil_div(K, (size_t)kTile);
+    const int shift = part_shift(G, M, tiles);
+    const double units = (size_t)1 << shift < M ? std::max((double)G, (double)M / ((size_t)1 << shift) + 0.5 * G) : (double)G;
+    return GradWork{group_tiles(G, M, K, kTile), (double)ceil_div(N, (size_t)kChunk), units * tiles, M / units / kChunk + 0.5};
+}
+
+template <auto kKernel, int kTeams>
+int allow()
+{
+    static bool raised = false;
+    if (kSplitLds<kTeams> >= 60 * 1024 && !raised)
+        DOPT_HIP_CHECK(hipFuncSetAttribute((const void *)kKernel, hipFuncAttributeMaxDynamicSharedMemorySize, kSplitLds<kTeams>));
+    raised = true;
+    return DOPT_HIP_OK;
+}
+template <class F>
+int with_teams(int teams, bool passes, F &&f)
+{
+    auto with = [&](auto n) { return passes ? f(n, std::true_type{}) : f(n, std::false_type{}); };
+    if (teams == 4) return with(std::integral_constant<int, 4>{});
+    if (teams == 2) return with(std::integral_constant<int, 2>{});
+    return with(std::integral_constant<int, 1>{});
+}
+
+}  // namespace
+
+namespace dopt {
+
+double groups_split_us(size_t G, size_t M, size_t N, size_t K)
+{
+    if (N < 32 || K < 32) return HUGE_VAL;
+    const double chunks = (double)ceil_div(K, (size_t)kChunk);
+    return 5 + chunks / 4 + 0.3 * group_tiles(G, M, N, kTile) * (chunks + 6) / num_cus() + 8.0 * M * N / 5e6;
+}
+double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K)
+{
+    if (N < 32 || K < 32) return HUGE_VAL;
+    const GradWork of = grad_work(G, M, N, K);
+    return 12 + 24.0 * M * N / 5e6 + (0.35 * of.dx_tiles * (of.dx_chunks + 18) + 0.22 * of.dw_tiles * (of.dw_chunks + 2.6)) / num_cus() + 0.43 * of.chain();
+}
+
+int groups_split(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
+{
+    const dim3 grid = grid_of(ceil_div((size_t)l.N, (size_t)kTile), most_units(l.q.M, l.q.G + 2, kTileShift));
+    // (workgroups and one, two, four teams: 160 18.9 14.0 12.7 us, 288 22.1 19.4 23.7, 544 28.0 30.0 36.4, reductions of 512 steps)
+    const double tiles = group_tiles(l.q.G, l.q.M, l.N, kTile);
+    const int teams = tiles <= num_cus() ? 4 : tiles <= 2 * num_cus() ? 2 : 1;
+    return with_teams(teams, l.K > (int)kPass * 16, [&](auto n, auto passes) {
+        constexpr auto kernel = groups_split_k<n.value, passes.value>;
+        if (int rc = allow<kernel, n.value>()) return rc;
+        hipLaunchKernelGGL(kernel, grid, dim3(256 * n.value), kSplitLds<n.value>, stream(), l, x, w, bias, y, pre, act);
+        DOPT_LAUNCH_CHECK();
+        return (int)DOPT_HIP_OK;
+    });
+}
+
+int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
+{
+    const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, tiles = ceil_div(N, (size_t)kTile) * ceil_div(K, (size_t)kTile);
+    const int shift = dw ? part_shift(G, M, tiles) : kLongestPart;
+    const bool direct = ((size_t)1 << shift) >= M, plain = act == DOPT_HIP_ACT_NONE;
+    const size_t dw_units = most_units(M, G, shift), runs = most_units(M, G, kRunShift), f = sizeof(float);
+    auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
+    const size_t dz_bytes = plain ? 0 : rounded(M * N * f), sum_bytes = dbias ? rounded(runs * N * f) : 0, part_bytes = dw && !direct ? dw_units * N * K * f : 0;
+    char *const scratch = dz_bytes + sum_bytes + part_bytes ? (char *)workspace(dz_bytes + sum_bytes + part_bytes) : nullptr;
+    if (dz_bytes + sum_bytes + part_bytes && !scratch) return DOPT_HIP_ERR_OOM;
+    float *const dz_to = plain ? nullptr : (float *)scratch, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
+    if (!plain || dbias)
+        if (int rc = groups_dz(l, act, kRunShift, dy, pre, dz_to, dbias ? sums : nullptr)) return rc;
+    auto eights = [](size_t n) { return ceil_div(n, (size_t)8) * 8; };
+    SplitGrads g{plain ? dy : dz_to, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, shift, (unsigned)eights(ceil_div(K, (size_t)kTile)),
+                 (unsigned)eights(tiles), (unsigned)eights(ceil_div(N, (size_t)32)), 0, 0, 0};
+    if (dx) g.dx_blocks = g.dx_tiles * most_units(M, G + 2, kTileShift);
+    if (dw) g.dw_blocks = g.dw_tiles * dw_units;
+    if (dbias) g.fold_blocks = g.fold_tiles * G;
+    const size_t blocks = g.dx_blocks + g.dw_blocks + g.fold_blocks;
+    DOPT_REQUIRE(blocks < ((size_t)1 << 37), "dopt_hip_dense_groups_grad: dimensions too large");
+    const dim3 grid((unsigned)std::min(blocks, (size_t)kRow), (unsigned)ceil_div(blocks, (size_t)kRow));
+    const bool passes = (dx && N > kPass * 16) || (dw && std::min(M, (size_t)1 << shift) > kPass * 16);
+    const int teams = grad_work(G, M, N, K).few() ? 2 : 1;
+    const int rc = with_teams(teams, passes, [&](auto n, auto passes) {
+        constexpr auto kernel = groups_split_grad_k<n.value, passes.value>;
+        if (int rc = allow<kernel, n.value>()) return rc;
+        hipLaunchKernelGGL(kernel, grid, dim3(256 * n.value), kSplitLds<n.value>, stream(), l, g);
+        DOPT_LAUNCH_CHECK();
+        return (int)DOPT_HIP_OK;
+    });
+    if (rc) return rc;
+    return dw && !direct ? groups_join(l, shift, parts, dw) : DOPT_HIP_OK;
+}
+
+}  // namespace dopt

@@ -5,6 +5,7 @@
 // Rows of a group are laid out from a tile's boundary on, so that a tile holds rows of one group; the steps of dw's reductions from a boundary of
 // 64 rows on.  How many tiles there are is found on the device: an XCD takes an eighth of them, side by side.
 #include <algorithm>
+#include <cmath>
 
 #include "dense_groups.h"
 #include "dense_wide.h"
@@ -380,15 +381,6 @@ size_t tile_for(size_t G, size_t M, size_t N, size_t K)
     return M >= 512 * G && M * N * K >= (size_t)30000000000 && tiles >= (size_t)num_cus() / 2 ? kBig : kSmall;
 }
 
-// What a product takes here and by the 32 x 32 tiles of dense_groups.hip, in us.  Here: launches, every byte that the layouts move, and the matrix
-// instructions over whole tiles (half of one more for each group).  There: launches, and operands that every tile reads by itself, from the L2; of
-// gradients also a workgroup for each tile of each group's dw.  Eight groups, here and there:
-//     [2048 x 512] from 512 37 28    [4096 x 512] from 512 39 46    [1024 x 1024] from 1024 51 45    [2048 x 1024] from 1024 56 77
-//     [256 x 4096] from 1024 85 65   [512 x 4096] from 1024 88 104   gradients [2048 x 512] from 512 59 56   [4096 x 512] 73 81
-//     [512 x 1024] from 1024 73 93   [1024 x 256] from 256 39 24
-double padded_rows(double G, double M) { return M + 64 * G; }
-double tiles32(double rows, double cols) { return (rows / 32 + 0.5) * ceil_div((size_t)cols, (size_t)32); }
-
 }  // namespace
 
 namespace dopt {
@@ -414,20 +406,18 @@ static bool fits(size_t G, size_t M, size_t N, size_t K)
     return M + kBig * G < most && G * (N + K + 2 * kBig) < most && M / 64 * (ceil_div(N, (size_t)64) + ceil_div(K, (size_t)64)) < most &&
            G * ceil_div(N, (size_t)64) * ceil_div(K, (size_t)64) < most;
 }
-bool groups_wide_takes(size_t G, size_t M, size_t N, size_t K)
+// Launches, every byte that the layouts move, and the matrix instructions over whole tiles (half of one more for each group).
+double groups_wide_us(size_t G, size_t M, size_t N, size_t K)
 {
-    if (K < 128 || N < 128 || G == 0 || !fits(G, M, N, K)) return false;
-    const double g = (double)G, m = (double)M, n = (double)N, k = (double)K;
-    const double here = 29 + 8 * (m * k + g * n * k) / 5e6 + 6 * padded_rows(g, m) * n * k / 1.2e9;
-    return here < 5 + 256 * tiles32(m + 16 * g, n) * k / 6.8e6;
+    if (K < 128 || N < 128 || !fits(G, M, N, K)) return HUGE_VAL;
+    const double m = (double)M, weights = (double)G * N * K;
+    return 29 + 8 * (m * K + weights) / 5e6 + 6 * (m + 64.0 * G) * N * K / 1.2e9;
 }
-bool groups_wide_takes_grad(size_t G, size_t M, size_t N, size_t K)
+double groups_wide_grad_us(size_t G, size_t M, size_t N, size_t K)
 {
-    if (K < 128 || N < 128 || G == 0 || !fits(G, M, N, K)) return false;
-    const double g = (double)G, m = (double)M, n = (double)N, k = (double)K;
-    const double here = 36 + (28 * m * n + 16 * m * k + 16 * g * n * k) / 5e6 + 12 * padded_rows(g, m) * n * k / 1.2e9;
-    const double dw = tiles32(n, k);
-    return here < 10 + 256 * (tiles32(m + 16 * g, k) * n + dw * m) / 8e6 + 5e-3 * g * dw;
+    if (K < 128 || N < 128 || !fits(G, M, N, K)) return HUGE_VAL;
+    const double m = (double)M, weights = (double)G * N * K;
+    return 36 + (28 * m * N + 16 * m * K + 16 * weights) / 5e6 + 12 * (m + 64.0 * G) * N * K / 1.2e9;
 }
 
 int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)

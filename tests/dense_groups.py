@@ -1,7 +1,8 @@
 """Dense layers of groups of rows in float64, one group after the other, with norm_dense_muon's bounds.
 
-Large products are formed from two fp16 parts of each value, scaled by its row: a value keeps 22 bits, or 2^-39 of its row's largest, and the
-product of two low parts is left out.  Three errors of 2^-22 of |a| |b| are under 2^-20 of it, and of the largest ones' 2 2^-39: `parts`
+Products that are not small are formed from two fp16 parts of each value, scaled by its row: a value keeps 22 bits, or 2^-38 of its row's largest (a
+scaled row's largest value so far is at least 2^13, and a low part is off by at most half of fp16's last place, 2^-25), and the product of two
+low parts is left out.  Three errors of 2^-22 of |a| |b| are under 2^-20 of it, and of the largest ones' 2 2^-38: `parts`
 adds those, which matter where a group has few rows (norm_dense_muon's bound shrinks with them)."""
 import numpy as np
 
@@ -18,7 +19,7 @@ def _of_parts(a, b):
     if not a.shape[1]:
         return 0.0
     a, b = np.abs(np.asarray(a, np.float64)), np.abs(np.asarray(b, np.float64))
-    return 2.0 ** -20 * (a @ b.T) + 2.0 ** -38 * a.shape[1] * np.outer(a.max(1), b.max(1))
+    return 2.0 ** -20 * (a @ b.T) + 2.0 ** -37 * a.shape[1] * np.outer(a.max(1), b.max(1))
 
 
 def forward(x, w, bias, offsets, name, parts=False):
