@@ -58,10 +58,16 @@ __device__ __forceinline__ void fold_runs(const GroupLayer &l, int shift, const 
 
 constexpr unsigned kGridRow = 65535;   // units along the second side of a grid; more go to the third
 __device__ __forceinline__ unsigned unit_id() { return blockIdx.z * kGridRow + blockIdx.y; }
-// x: as many as there are tiles side by side, a multiple of eight, so that a tile of columns - and what it reads of a weight - stays on one XCD
+// Workgroups for so many tiles side by side: a multiple of eight, so that a tile of columns - and what it reads of a weight - stays on one XCD, unless that
+// leaves XCDs with less to do or nothing.
+inline size_t abreast(size_t tiles)
+{
+    const size_t eights = ceil_div(tiles, (size_t)8) * 8;
+    return 5 * eights <= 6 * tiles ? eights : tiles;
+}
 inline dim3 grid_of(size_t tiles, size_t units)
 {
-    const size_t x = ceil_div(tiles, (size_t)8) * 8;
+    const size_t x = abreast(tiles);
     return dim3((unsigned)x, (unsigned)(units < kGridRow ? units : kGridRow), (unsigned)ceil_div(units, (size_t)kGridRow));
 }
 

@@ -56,7 +56,7 @@ struct SmallGrads {
     const float *dz, *x, *w, *sums;
     float *dx, *dw, *parts, *dbias;   // parts: or null
     int slice, shift;
-    unsigned dx_tiles, dw_tiles, fold_tiles;           // side by side, multiples of eight: a tile of columns stays on one XCD
+    unsigned dx_tiles, dw_tiles, fold_tiles;           // workgroups side by side
     size_t dx_blocks, dw_blocks, fold_blocks;
 };
 
@@ -172,18 +172,23 @@ int check(const char *who, size_t G, size_t M, size_t N, size_t K, int act)
     return DOPT_HIP_OK;
 }
 
-// What the small products take, in us: launches, and operands that every tile of 32 x 32 reads by itself, from the L2; of gradients also a workgroup for each
-// tile of each group's dw.  The way that takes the least is taken.  Eight groups, small, split and wide:
-//     [64 x 512] from 512 7.4 10.7 29       [1024 x 512] from 512 19 13 36       [4096 x 512] from 512 46 28 39       [16384 x 512] from 512 156 79 70
+// What the small products take, in us: launches, and operands that every tile of 32 x 32 reads by itself, rounds of tiles; of gradients their rows, and
+// a workgroup for each tile of each group's dw.  The way that takes the least is taken; the costs are fitted to 181 products and 119 gradients, where it
+// took within 10 % of the fastest way's time but for one product and four gradients.  Eight groups, small, split and wide:
+//     [64 x 512] from 512 7.4 10.7 29       [1024 x 512] from 512 19 13 36       [4096 x 512] from 512 46 28 39       [16384 x 512] from 512 156 77 70
 //     [1024 x 1024] from 1024 45 28 51      [8192 x 1024] from 1024 279 123 107  [512 x 4096] from 1024 104 50 85
 // and gradients
-//     [128 x 256] from 256 12 14 30         [1024 x 512] from 512 39 30 54       [4096 x 512] from 512 81 58 73       [16384 x 512] from 512 256 212 177
-//     [2048 x 1024] from 1024 171 87 90     [8192 x 1024] from 1024 436 301 221  [256 x 4096] from 1024 269 130 243
-double small_us(size_t G, size_t M, size_t N, size_t K) { return 5 + 256 * group_tiles(G, M, N, 32) * K / 6.8e6; }
+//     [128 x 256] from 256 12 14 30         [1024 x 512] from 512 39 29 54       [4096 x 512] from 512 81 57 73       [16384 x 512] from 512 256 211 177
+//     [2048 x 1024] from 1024 171 86 90     [8192 x 1024] from 1024 436 298 221  [256 x 4096] from 1024 269 130 243
+double small_us(size_t G, size_t M, size_t N, size_t K)
+{
+    const double rounds = group_tiles(G, M, N, 32) / num_cus();
+    return 5 + 0.0101 * K * (rounds > 1 ? rounds + 0.5 : std::max(rounds, 0.65));
+}
 double small_grad_us(size_t G, size_t M, size_t N, size_t K)
 {
-    const double dw = ((double)N / 32 + 0.5) * ceil_div(K, (size_t)32);
-    return 10 + 256 * (group_tiles(G, M, K, 32) * N + dw * M) / 6.3e6 + 5e-3 * G * dw;
+    const double m = (double)M, dw = ((double)N / 32 + 0.5) * ceil_div(K, (size_t)32);
+    return 10.8 + 1e-6 * (10 * m * K + 7 * m * N + 13 * (group_tiles(G, M, K, 32) * N + dw * m)) + 6.6e-3 * G * dw;
 }
 enum class Way { kSmall, kSplit, kWide };
 Way way_of(double small, double split, double wide) { return small <= std::min(split, wide) ? Way::kSmall : split <= wide ? Way::kSplit : Way::kWide; }
@@ -296,9 +301,8 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
             DOPT_LAUNCH_CHECK();
         }
     }
-    auto eights = [](size_t n) { return ceil_div(n, (size_t)8) * 8; };
-    SmallGrads g{dz, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, (int)slice_of(N), shift, (unsigned)eights(ceil_div(K, (size_t)32)),
-                 (unsigned)eights(tiles), (unsigned)eights(ceil_div(N, (size_t)32)), 0, 0, 0};
+    SmallGrads g{dz, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, (int)slice_of(N), shift, (unsigned)abreast(ceil_div(K, (size_t)32)),
+                 (unsigned)abreast(tiles), (unsigned)abreast(ceil_div(N, (size_t)32)), 0, 0, 0};
     if (dx) g.dx_blocks = g.dx_tiles * most_units(M, G + 2, kTileShift);
     if (dw) g.dw_blocks = g.dw_tiles * dw_units;
     if (dbias) g.fold_blocks = g.fold_tiles * G;

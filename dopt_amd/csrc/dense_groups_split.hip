@@ -152,15 +152,15 @@ namespace dopt {
 
 double groups_split_us(size_t G, size_t M, size_t N, size_t K)
 {
-    if (N < 32 || K < 32) return HUGE_VAL;
+    if (N < 4 || K < 4) return HUGE_VAL;   // (of no use, and sums of dz want four columns)
     const double chunks = (double)ceil_div(K, (size_t)kChunk);
     return 5 + chunks / 4 + 0.3 * group_tiles(G, M, N, kTile) * (chunks + 6) / num_cus() + 8.0 * M * N / 5e6;
 }
 double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K)
 {
-    if (N < 32 || K < 32) return HUGE_VAL;
+    if (N < 4 || K < 4) return HUGE_VAL;
     const GradWork of = grad_work(G, M, N, K);
-    return 12 + 24.0 * M * N / 5e6 + (0.35 * of.dx_tiles * (of.dx_chunks + 18) + 0.22 * of.dw_tiles * (of.dw_chunks + 2.6)) / num_cus() + 0.43 * of.chain();
+    return 11.5 + 3.4e-6 * M * N + (0.25 * of.dx_tiles * (of.dx_chunks + 18) + 0.44 * of.dw_tiles * (of.dw_chunks + 0.2)) / num_cus() + 0.57 * of.chain();
 }
 
 int groups_split(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
@@ -191,9 +191,8 @@ int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float
     float *const dz_to = plain ? nullptr : (float *)scratch, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
     if (!plain || dbias)
         if (int rc = groups_dz(l, act, kRunShift, dy, pre, dz_to, dbias ? sums : nullptr)) return rc;
-    auto eights = [](size_t n) { return ceil_div(n, (size_t)8) * 8; };
-    SplitGrads g{plain ? dy : dz_to, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, shift, (unsigned)eights(ceil_div(K, (size_t)kTile)),
-                 (unsigned)eights(tiles), (unsigned)eights(ceil_div(N, (size_t)32)), 0, 0, 0};
+    SplitGrads g{plain ? dy : dz_to, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, shift, (unsigned)abreast(ceil_div(K, (size_t)kTile)),
+                 (unsigned)abreast(tiles), (unsigned)abreast(ceil_div(N, (size_t)32)), 0, 0, 0};
     if (dx) g.dx_blocks = g.dx_tiles * most_units(M, G + 2, kTileShift);
     if (dw) g.dw_blocks = g.dw_tiles * dw_units;
     if (dbias) g.fold_blocks = g.fold_tiles * G;

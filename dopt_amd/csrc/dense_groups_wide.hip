@@ -422,7 +422,7 @@ double groups_wide_grad_us(size_t G, size_t M, size_t N, size_t K)
 {
     if (K < 128 || N < 128 || !fits(G, M, N, K)) return HUGE_VAL;
     const double m = (double)M, weights = (double)G * N * K;
-    return 36 + (28 * m * N + 16 * m * K + 16 * weights) / 5e6 + 12 * (m + 64.0 * G) * N * K / 1.2e9;
+    return 32.7 + 1e-6 * (9.9 * m * N + 4.5 * m * K + 3.9 * weights) + 3.5e-9 * (m + 64.0 * G) * N * K;
 }
 
 int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)

@@ -33,8 +33,9 @@ def _place(shape, up):
 
 
 def _parts(t):
-    """Whether the products may be of two fp16 parts: all but the small ones."""
-    return min(t["w"].shape[1:]) >= 32 and t["x"].size * t["w"].shape[1] >= 20000000
+    """Whether the products may be of two fp16 parts: all but the small ones, counted in whole tiles."""
+    (m, k), (g, n) = t["x"].shape, t["w"].shape[:2]
+    return max(m, 32 * g) * n * k >= 10000000
 
 
 def _check(t, name, up=ops.tensor, keep=True, bias=True):
@@ -234,7 +235,8 @@ def test_large(sizes, n, k):
 
 
 MIDDLE = [([9, 0, 170, 3, 110, 80, 14, 200], 512, 512), ([70, 600, 1, 333], 300, 1111), ([200, 31, 257, 64, 90], 777, 200), ([500], 1024, 1024),
-          ([3000, 100, 2500], 96, 130), ([16] * 64, 520, 260), ([1, 2, 3, 60], 2050, 1030)]
+          ([3000, 100, 2500], 96, 130), ([16] * 64, 520, 260), ([1, 2, 3, 60], 2050, 1030), ([6000, 900, 0, 2000], 12, 1561), ([5000, 1000], 5, 830),
+          ([7000], 31, 717), ([1200, 20, 4000], 48, 819)]
 
 
 @pytest.mark.parametrize("sizes,n,k", MIDDLE, ids=lambda v: "%dx%d" % (len(v), sum(v)) if isinstance(v, list) else str(v))
