@@ -968,8 +968,9 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     const size_t lds = (staged ? 3 + (teams > 1 ? teams : 0) : 2) * width * f;   // scales and what teams add, or sums
     Runs runs{0, (unsigned)d->rows, n.per_gate ? n.per_gate : (unsigned)std::max(d->rows, (size_t)1), 1, 0};
     Launch launch{nullptr, kBlock, 0, (size_t)num_cus() * 8};
-    // Gates of fewer rows than this go to teams as a whole.
-    const bool whole = d->gates && runs.per_gate < std::min(kWholeRows, 4 * teams);
+    // Gates of few rows go to teams as a whole where there are many of them, else to a workgroup each, whose teams share the rows: [1500 x 600]
+    // with 100 gates 19.6 us (as a whole 64), [2400 x 1500] with 200 33 (70), [2000 x 700] with 500 28 (27), [8000 x 600] with 1000 71 (51), with 4000 180 (50).
+    const bool whole = runs.per_gate < std::min(kWholeRows, 4 * teams) && d->gates > 2 * (size_t)num_cus();
     if (held) {
         int rc = DOPT_HIP_OK;
         with_form(form, [&](auto lanes, auto quads) {

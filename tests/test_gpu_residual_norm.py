@@ -105,6 +105,15 @@ def test_many_rows(rows, cols, gates):
     _check_backward(t, y, stats, post, pre, 0.9)
 
 
+@pytest.mark.parametrize("cols,per_gate", [(10, 15), (100, 3), (200, 7), (640, 5), (1500, 1), (1500, 3), (5000, 2), (9000, 3), (16390, 1)])
+def test_many_gates_of_few_rows(cols, per_gate):
+    """More gates than are shared by a workgroup's teams each."""
+    post, pre = KINDS[(cols + per_gate) % len(KINDS)]
+    t = _case(600 * per_gate, cols, 600, post, pre, cols)
+    y, stats = _check_forward(t, post, pre, 0.7)
+    _check_backward(t, y, stats, post, pre, 0.7)
+
+
 def test_rows_beyond_thirty_two_bits_of_values():
     """2^32 values and more: rows before and behind that border, of which the others are zero."""
     rows, cols = (1 << 21) + 5, 2048 + 4
