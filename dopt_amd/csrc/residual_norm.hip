@@ -18,7 +18,7 @@
 //
 // [16384 x 1024] forward 53 us (5.0 TB/s), backward 88 and 6 for the runs (4.3); [8192 x 4096] forward 99.6 (5.4); [4107 x 1111] with 37 gates backward 29 and 6;
 // one row of 512 3.4, a launch.  Rows of more than 8192 values leave a CU one workgroup, whose reads and writes take turns: [1024 x 16384] 92 forward, 174
-// backward (2.9 and 2.3 TB/s); beyond 16384 a fifth of the rate is left ([500 x 20000] 114 and 209).
+// backward (2.9 and 2.3 TB/s); beyond 16384 a fifth of the rate is left ([500 x 20000] 114 and 182).
 #include <algorithm>
 #include <type_traits>
 
@@ -991,13 +991,17 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
             runs.gates = (unsigned)(std::min(most, ceil_div(gates, launch.places * teams)) * teams);
             runs.count = (unsigned)ceil_div(gates, (size_t)runs.gates);
         } else {
-            // One to three rounds of all places, whichever leaves the fewest turns of a team; a workgroup's beginning and end cost some two of them.
+            // One to three rounds of all places, whichever leaves the fewest turns of a team; a workgroup's beginning and end cost some two of them.  Down to one
+            // row for a team: [1024 x 256] 11.2 us, with six rows 18, [256 x 1024] 14.2 and, with two, 16.8.  Long rows' columns eight at least: [500 x 20000]
+            // 182, with one 251.
             const size_t least = ceil_div((size_t)runs.per_gate, kTeamRows * teams);
-            const size_t most = ceil_div((size_t)runs.per_gate, (form.lanes ? 6 : 2) * teams);
+            const size_t most = ceil_div((size_t)runs.per_gate, held ? teams : (size_t)8);
             size_t best = 0;
             for (size_t rounds = 1; rounds <= 3; rounds++) {
-                const size_t splits = std::max(least, std::min(most, std::max((size_t)1, rounds * launch.places / gates)));
-                const size_t turns = ceil_div(gates * splits, launch.places) * (ceil_div(ceil_div((size_t)runs.per_gate, splits), teams) + 2);
+                size_t splits = std::max(least, std::min(most, std::max((size_t)1, rounds * launch.places / gates)));
+                const size_t of_team = ceil_div(ceil_div((size_t)runs.per_gate, splits), teams);
+                splits = std::max(least, ceil_div((size_t)runs.per_gate, of_team * teams));   // no more of them than so many rows need
+                const size_t turns = ceil_div(gates * splits, launch.places) * (of_team + 2);
                 if (best && turns >= best) continue;
                 best = turns;
                 runs.splits = (unsigned)splits;
