@@ -179,7 +179,7 @@ int check(const char *who, size_t G, size_t M, size_t N, size_t K, int act)
 //     [1024 x 1024] from 1024 45 28 51      [8192 x 1024] from 1024 279 123 107  [512 x 4096] from 1024 104 50 85
 // and gradients
 //     [128 x 256] from 256 12 14 30         [1024 x 512] from 512 39 29 54       [4096 x 512] from 512 81 57 73       [16384 x 512] from 512 256 211 177
-//     [2048 x 1024] from 1024 171 86 90     [8192 x 1024] from 1024 436 298 221  [256 x 4096] from 1024 269 130 243
+//     [2048 x 1024] from 1024 171 86 90     [8192 x 1024] from 1024 436 298 221  [256 x 4096] from 1024 269 110 243
 double small_us(size_t G, size_t M, size_t N, size_t K)
 {
     const double rounds = group_tiles(G, M, N, 32) / num_cus();

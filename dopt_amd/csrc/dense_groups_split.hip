@@ -44,11 +44,12 @@ __global__ __launch_bounds__(256 * kTeams) void groups_split_k(GroupLayer l, con
     }
     const size_t begin = s.begin, g = (size_t)s.group;
     const DenseEpilogue ep{bias ? bias + g * N : nullptr, nullptr, pre ? pre + begin * N : nullptr, act, N};
-    split_tile<kTeams, false, false, kPasses>(Matrix32{x + begin * K, K, s.end - s.begin}, Matrix32{w + g * N * K, K, (unsigned)N}, (unsigned)K,
+    split_tile<kTeams, true, false, false, kPasses>(Matrix32{x + begin * K, K, s.end - s.begin}, Matrix32{w + g * N * K, K, (unsigned)N}, (unsigned)K,
                                                 s.unit << kTileShift, n0, ep, y + begin * N, lds);
 }
 
-// The gradients in one launch, as dense_groups.hip's: dx = dz w, dw = dz^T x over 2^shift rows of a group, dbias.
+// The gradients in one launch, as dense_groups.hip's: dx = dz w, whose reduction is often the longer one and is shared by teams; dw = dz^T x over 2^shift rows of a
+// group, a tile for each team; dbias.
 struct SplitGrads {
     const float *dz, *x, *w, *sums;
     float *dx, *dw, *parts, *dbias;   // parts: or null
@@ -77,27 +78,28 @@ __global__ __launch_bounds__(256 * kTeams) void groups_split_grad_k(GroupLayer l
                 if (k0 + i % kTile < K) g.dx[(row + i / kTile) * K + k0 + i % kTile] = 0.0f;
             return;
         }
-        return split_tile<kTeams, false, true, kPasses>(Matrix32{g.dz + begin * N, N, s.end - s.begin}, Matrix32{g.w + s.group * N * K, K, (unsigned)K},
+        return split_tile<kTeams, true, false, true, kPasses>(Matrix32{g.dz + begin * N, N, s.end - s.begin}, Matrix32{g.w + s.group * N * K, K, (unsigned)K},
                                                           (unsigned)N, s.unit << kTileShift, k0,
                                                           DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, g.dx + begin * K, lds);
     }
     block -= g.dx_blocks;
     if (block < g.dw_blocks) {
-        const unsigned tile = (unsigned)(block % g.dw_tiles), unit = (unsigned)(block / g.dw_tiles), across = (unsigned)((K + kTile - 1) / kTile);
-        const unsigned k0 = tile % across * kTile, n0 = tile / across * kTile;
-        if (n0 >= N) return;
+        // a tile for each team
+        const unsigned first = (unsigned)(block % g.dw_tiles) * kTeams, unit = (unsigned)(block / g.dw_tiles), across = (unsigned)((K + kTile - 1) / kTile);
+        const unsigned tile = first + threadIdx.x / 256, k0 = tile % across * kTile, n0 = tile / across * kTile;
+        if (first / across * kTile >= N) return;
         const Segment s = find_unit<false, true>(l.q, g.shift, unit);
         if (s.group < 0) return;
         const size_t row = s.begin + ((size_t)s.unit << g.shift);
         const unsigned rows = (unsigned)min((size_t)s.end - row, (size_t)1 << g.shift);
         float *const to = g.parts ? g.parts + unit * N * K : g.dw + s.group * N * K;
         if (rows == 0) {
-            for (int i = threadIdx.x; i < kTile * kTile; i += 256 * kTeams)
+            for (int i = threadIdx.x & 255; i < kTile * kTile; i += 256)
                 if (n0 + i / kTile < N && k0 + i % kTile < K) to[(n0 + i / kTile) * K + k0 + i % kTile] = 0.0f;
             return;
         }
-        return split_tile<kTeams, true, true, kPasses>(Matrix32{g.dz + row * N, N, (unsigned)N}, Matrix32{g.x + row * K, K, (unsigned)K}, rows, n0, k0,
-                                                         DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, to, lds);
+        return split_tile<kTeams, false, true, true, kPasses>(Matrix32{g.dz + row * N, N, (unsigned)N}, Matrix32{g.x + row * K, K, (unsigned)K}, rows, n0, k0,
+                                                              DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, to, lds);
     }
     block -= g.dw_blocks;
     if (block < g.fold_blocks)
@@ -116,8 +118,8 @@ int part_shift(size_t G, size_t M, size_t tiles)
 struct GradWork {
     double dx_tiles, dx_chunks, dw_tiles, dw_chunks;
     double chain() const { return std::max(dx_chunks, dw_chunks); }
-    // One workgroup's chunks take longer than all of them over the chip's: [1024 x 512] from 512 in eight groups with one team 31.2 us, with two 29.6,
-    // [2048 x 512] 38.9 and 40.9, [256 x 4096] from 1024 150 and 130, [1024 x 4096] 180 and 201.  (Four teams gain nothing further.)
+    // One workgroup's chunks take longer than all of them over the chip: [1024 x 512] from 512 in eight groups with one team 31.4 us, with two 29.8, with
+    // four 35.3; [2048 x 512] 39 46 49; [256 x 4096] from 1024 151 110 113; [1024 x 4096] 179 177 191.
     bool few() const { return dx_tiles * dx_chunks + dw_tiles * dw_chunks < 1.5 * chain() * num_cus(); }
 };
 GradWork grad_work(size_t G, size_t M, size_t N, size_t K)
@@ -137,11 +139,12 @@ int allow()
     raised = true;
     return DOPT_HIP_OK;
 }
-template <class F>
+template <int kMost, class F>
 int with_teams(int teams, bool passes, F &&f)
 {
     auto with = [&](auto n) { return passes ? f(n, std::true_type{}) : f(n, std::false_type{}); };
-    if (teams == 4) return with(std::integral_constant<int, 4>{});
+    if constexpr (kMost == 4)
+        if (teams == 4) return with(std::integral_constant<int, 4>{});
     if (teams == 2) return with(std::integral_constant<int, 2>{});
     return with(std::integral_constant<int, 1>{});
 }
@@ -169,7 +172,7 @@ int groups_split(const GroupLayer &l, const float *x, const float *w, const floa
     // (workgroups and one, two, four teams: 160 18.9 14.0 12.7 us, 288 22.1 19.4 23.7, 544 28.0 30.0 36.4, reductions of 512 steps)
     const double tiles = group_tiles(l.q.G, l.q.M, l.N, kTile);
     const int teams = tiles <= num_cus() ? 4 : tiles <= 2 * num_cus() ? 2 : 1;
-    return with_teams(teams, l.K > (int)kPass * 16, [&](auto n, auto passes) {
+    return with_teams<4>(teams, l.K > (int)kPass * 16, [&](auto n, auto passes) {
         constexpr auto kernel = groups_split_k<n.value, passes.value>;
         if (int rc = allow<kernel, n.value>()) return rc;
         hipLaunchKernelGGL(kernel, grid, dim3(256 * n.value), kSplitLds<n.value>, stream(), l, x, w, bias, y, pre, act);
@@ -191,8 +194,9 @@ int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float
     float *const dz_to = plain ? nullptr : (float *)scratch, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
     if (!plain || dbias)
         if (int rc = groups_dz(l, act, kRunShift, dy, pre, dz_to, dbias ? sums : nullptr)) return rc;
+    const int teams = grad_work(G, M, N, K).few() ? 2 : 1;
     SplitGrads g{plain ? dy : dz_to, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, shift, (unsigned)abreast(ceil_div(K, (size_t)kTile)),
-                 (unsigned)abreast(tiles), (unsigned)abreast(ceil_div(N, (size_t)32)), 0, 0, 0};
+                 (unsigned)abreast(ceil_div(tiles, (size_t)teams)), (unsigned)abreast(ceil_div(N, (size_t)32)), 0, 0, 0};
     if (dx) g.dx_blocks = g.dx_tiles * most_units(M, G + 2, kTileShift);
     if (dw) g.dw_blocks = g.dw_tiles * dw_units;
     if (dbias) g.fold_blocks = g.fold_tiles * G;
@@ -200,8 +204,7 @@ int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float
     DOPT_REQUIRE(blocks < ((size_t)1 << 37), "dopt_hip_dense_groups_grad: dimensions too large");
     const dim3 grid((unsigned)std::min(blocks, (size_t)kRow), (unsigned)ceil_div(blocks, (size_t)kRow));
     const bool passes = (dx && N > kPass * 16) || (dw && std::min(M, (size_t)1 << shift) > kPass * 16);
-    const int teams = grad_work(G, M, N, K).few() ? 2 : 1;
-    const int rc = with_teams(teams, passes, [&](auto n, auto passes) {
+    const int rc = with_teams<2>(teams, passes, [&](auto n, auto passes) {
         constexpr auto kernel = groups_split_grad_k<n.value, passes.value>;
         if (int rc = allow<kernel, n.value>()) return rc;
         hipLaunchKernelGGL(kernel, grid, dim3(256 * n.value), kSplitLds<n.value>, stream(), l, g);

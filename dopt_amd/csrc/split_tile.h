@@ -122,32 +122,36 @@ struct Feed {
     }
 };
 
-// A tile of a result of ep.N columns; at least one step, row and column.
-template <int kTeams, bool kAcrossA, bool kAcrossB, bool kPasses>
+// A tile of a result of ep.N columns; at least one step, row and column.  The workgroup's teams share its reduction, or (kShare false) have a tile each, of
+// reductions that are as long: one that begins behind the last row or column is none.
+template <int kTeams, bool kShare, bool kAcrossA, bool kAcrossB, bool kPasses>
 __device__ __forceinline__ void split_tile(const Matrix32 &A, const Matrix32 &B, unsigned K, unsigned m0, unsigned n0, const DenseEpilogue &ep, float *y, char *lds)
 {
     constexpr int T = kSplitTile, kOfA = kSplitHalf / 2;
-    __shared__ int fell_of[kTeams][2][2 * T], shifts[kTeams][2 * T], moved_of[kTeams][2][4], odd[2 * T], any_odd;
+    constexpr int kSharing = kShare ? kTeams : 1, kTiles = kTeams / kSharing;
+    __shared__ int fell_of[kTeams][2][2 * T], shifts[kTeams][2 * T], moved_of[kTeams][2][4], odd_of[kTiles][2 * T], any_odd_of[kTiles];
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6 & 3, team = (int)threadIdx.x >> 8, wm = wave & 1, wn = wave >> 1;
     int(&fell)[2][2 * T] = fell_of[team], (&moved)[2][4] = moved_of[team];
     char *const of_team = lds + team * 2 * kSplitHalf;
-    if (threadIdx.x < 2 * T) odd[threadIdx.x] = 0;
-    if (threadIdx.x == 0) any_odd = 0;
+    const int tile = kShare ? 0 : team, shared = kShare ? team : 0, thread = (int)threadIdx.x & (256 * kSharing - 1);   // of the tile
+    int(&odd)[2 * T] = odd_of[tile], &any_odd = any_odd_of[tile];
+    if (thread < 2 * T) odd[thread] = 0;
+    if (thread == 0) any_odd = 0;
     Feed<kAcrossA> a;
     Feed<kAcrossB> b;
     a.begin(A, m0);
     b.begin(B, n0);
     v16f acc[1][1] = {}, all = {};
-    const unsigned chunks = (K + kChunk - 1) / kChunk, turns = (chunks + kTeams - 1) / kTeams;
+    const unsigned chunks = (K + kChunk - 1) / kChunk, turns = (chunks + kSharing - 1) / kSharing;
     auto load = [&](unsigned turn, auto parity) {
-        const unsigned c = turn * kTeams + team;
+        const unsigned c = turn * kSharing + shared;
         if (c >= chunks) return;
         a.template load<parity.value>(c * kChunk, K);
         b.template load<parity.value>(c * kChunk, K);
     };
     auto chunk = [&](unsigned turn, auto parity) {
         constexpr int P = decltype(parity)::value;
-        const bool live = kTeams == 1 || turn * kTeams + team < chunks;
+        const bool live = kSharing == 1 || turn * kSharing + shared < chunks;
         char *const to = of_team + P * kSplitHalf;
         if (live) {
             bool any = a.template put<P>(to, fell[P]);
@@ -201,7 +205,7 @@ __device__ __forceinline__ void split_tile(const Matrix32 &A, const Matrix32 &B,
     for (int e = 0; e < 16; e++) acc[0][0][e] = __builtin_ldexpf(acc[0][0][e], -(shifts[team][row_of(e)] + shifts[team][T + col]));
     // Teams add up their sums, a quarter or half of the rows each.
     float *const image = (float *)lds + ((int)threadIdx.x & 255);
-    if constexpr (kTeams > 1) {
+    if constexpr (kSharing > 1) {
 #pragma unroll
         for (int e = 0; e < 16; e++) image[(team * 16 + e) * 256] = acc[0][0][e];
         meet();
@@ -211,14 +215,14 @@ __device__ __forceinline__ void split_tile(const Matrix32 &A, const Matrix32 &B,
         with_activation(ep.act, [&](auto kind) {
             // (a loop, whose sums move down: less code to fetch)
 #pragma unroll 1
-            for (int t = team * (4 / kTeams); t < (team + 1) * (4 / kTeams); t++) {
+            for (int t = shared * (4 / kSharing); t < (shared + 1) * (4 / kSharing); t++) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float z = acc[0][0][e];
-                    if constexpr (kTeams > 1) {
+                    if constexpr (kSharing > 1) {
                         z = image[(4 * t + e) * 256];
 #pragma unroll
-                        for (int i = 1; i < kTeams; i++) z += image[(i * 16 + 4 * t + e) * 256];
+                        for (int i = 1; i < kSharing; i++) z += image[(i * 16 + 4 * t + e) * 256];
                     }
                     const int r = row_of(4 * t + e);
                     const unsigned m = m0 + r;
@@ -228,7 +232,7 @@ __device__ __forceinline__ void split_tile(const Matrix32 &A, const Matrix32 &B,
                     if (ep.pre) ep.pre[at] = z;
                     y[at] = act_value<kind.value>(z);
                 }
-                if constexpr (kTeams == 1) {
+                if constexpr (kSharing == 1) {
 #pragma unroll
                     for (int e = 0; e < 12; e++) acc[0][0][e] = acc[0][0][e + 4];
                 }
@@ -236,7 +240,7 @@ __device__ __forceinline__ void split_tile(const Matrix32 &A, const Matrix32 &B,
         });
     }
     if (!any_odd) return;
-    for (int i = threadIdx.x; i < T * T; i += 256 * kTeams) {
+    for (int i = thread; i < T * T; i += 256 * kSharing) {
         const unsigned m = m0 + i / T, n = n0 + i % T;
         if (m >= A.rows || n >= B.rows || !(odd[i / T] | odd[T + i % T])) continue;
         float s = 0.0f;
