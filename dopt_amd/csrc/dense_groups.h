@@ -1,6 +1,8 @@
 // What the kernels of dense layers of groups share (dense_groups.hip, dense_groups_wide.hip).
 #pragma once
 
+#include <cmath>
+
 #include "common.h"
 #include "dense.h"
 #include "groups.h"
@@ -29,8 +31,12 @@ int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const fl
 // dense_groups.hip: dw from the matrices of parts of 2^shift rows of a group, of which an empty group has one of zeros.
 int groups_join(const GroupLayer &l, int shift, const float *parts, float *dw);
 
+// Groups that have any of M rows which fall to them at random.
+inline double groups_with_rows(size_t G, size_t M) { return G * (1 - std::pow(1 - 1.0 / G, (double)M)); }
+// ... whose matrices come from memory at so many bytes a us.
+inline double weights_us(size_t G, size_t M, size_t N, size_t K, double rate) { return groups_with_rows(G, M) * N * K * 4 / rate; }
 // Tiles of `side` rows and columns, half of one more for each group.
-inline double group_tiles(size_t G, size_t M, size_t N, size_t side) { return ((double)M / side + 0.5 * G) * ceil_div(N, side); }
+inline double group_tiles(size_t G, size_t M, size_t N, size_t side) { return ((double)M / side + 0.5 * (G < M ? G : M)) * ceil_div(N, side); }
 
 // dbias from the sums of runs of 2^shift rows of a group: `lanes` lanes to a column, of 32 side by side; red: a value of each.
 __device__ __forceinline__ void fold_runs(const GroupLayer &l, int shift, const float *sums, float *dbias, unsigned tile, unsigned group, int lanes,

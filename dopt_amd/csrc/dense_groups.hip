@@ -7,9 +7,12 @@
 //
 // A workgroup finds its rows in the offsets itself: the grid has room for any sizes, workgroups beyond what there is end at once.
 //
-// Here are the small products: tiles of 32 x 32 by eight wavefronts that share the reduction, fp32 instructions, one launch forward, two backward.  Bound by a launch
-// and by what the tiles read from the L2: 64 rows in eight groups, [64 x 512] from 512, 7.2 us, of which the latency of a launch is 3.4 and w 1.6.
+// Here are the small products: tiles of 32 x 32 by eight wavefronts that share the reduction, fp32 instructions, one launch forward, two backward.  Bound by
+// a launch and by what the tiles read from the L2: 64 rows in eight groups, [64 x 512] from 512, 7.2 us, of which the latency of a launch is 3.4 and w 1.6.
+// And products of single rows, which w bounds: one row of [4096 x 4096] 15.0 us, 67 MB at 4.5 TB/s.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "dense_groups.h"
 #include "small_product.h"
@@ -19,6 +22,7 @@ namespace {
 using namespace dopt;
 
 constexpr int kTileShift = 5;    // rows of a tile: 32
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));   // sixteen bytes wherever they start
 constexpr int kRunShift = 6;     // rows that a thread adds up for dbias before it rounds to memory: 64
 typedef float SmallSums[32 * 33];
 
@@ -47,6 +51,97 @@ __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(GroupLayer l,
     const DenseEpilogue ep{bias ? bias + (size_t)s.group * l.N : nullptr, nullptr, pre ? pre + row * l.N : nullptr, act, (size_t)l.N};
     sgemm_small_body<false, true, kCut, DenseEpilogue>(rows, l.N, l.K, l.K, l.K, kslice, x + row * l.K, w + (size_t)s.group * l.N * l.K, y + row * l.N,
                                                        nullptr, 0, nullptr, 0, nullptr, (int)blockIdx.x, 0, 0, l.K, red, ep);
+}
+
+// The same for groups of a handful of rows, as when single tokens are served: up to R rows of a group by eight columns, two to a wavefront, whose lanes
+// read a row of w side by side, a kilobyte at a time, while x waits in LDS.  Bound by memory.  Sums of a lane are of 16 values, then of those, then of the lanes.
+template <int R>
+__global__ __launch_bounds__(256) void groups_few_k(GroupLayer l, const float *x, const float *w, const float *bias, float *y, float *pre, int act)
+{
+    constexpr int kColumns = 8, kChunk = 1024;
+    constexpr int kShift = R / 2;   // R: 1, 2 or 4
+    __shared__ __attribute__((aligned(16))) float rows_of[R][kChunk];
+    const int n0 = (int)blockIdx.x * kColumns;
+    if (n0 >= l.N) return;
+    const Segment s = find_unit<true>(l.q, kShift, unit_id());
+    if (s.group < 0) return;
+    const size_t row = s.begin + ((size_t)s.unit << kShift), N = l.N, K = l.K;
+    const int rows = (int)min(s.end - row, (size_t)R);
+    if (s.group == (int)l.q.G) {
+        for (int i = threadIdx.x; i < kColumns * rows; i += 256) {
+            const int c = n0 + i % kColumns;
+            if (c >= l.N) continue;
+            const size_t at = (row + i / kColumns) * N + c;
+            y[at] = 0.0f;
+            if (pre) pre[at] = 0.0f;
+        }
+        return;
+    }
+    const int lane = (int)threadIdx.x & 63, c0 = n0 + 2 * ((int)threadIdx.x >> 6);
+    const float *of[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) of[j] = w + (s.group * N + min(c0 + j, l.N - 1)) * K;
+    auto quad = [&](const float *p, size_t k) {   // zero beyond the row's end
+        if (k + 4 <= K) return *(const v4f_any *)(p + k);
+        v4f_any v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 3; e++)
+            if (k + e < K) v[e] = p[k + e];
+        return v;
+    };
+    v4f_any next[2][4];
+    auto fetch = [&](size_t k0) {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) next[j][t] = quad(of[j], k0 + 256 * t + 4 * lane);
+    };
+    float all[R][2] = {};
+    fetch(0);
+    for (size_t k0 = 0; k0 < K; k0 += kChunk) {
+        v4f_any own[2][4];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) own[j][t] = next[j][t];
+        if (k0) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const v4f_any v = r < rows ? quad(x + (row + r) * K, k0 + 4 * threadIdx.x) : v4f_any{0.0f, 0.0f, 0.0f, 0.0f};
+            *(v4f_any *)&rows_of[r][4 * threadIdx.x] = v;
+        }
+        __syncthreads();
+        if (k0 + kChunk < K) fetch(k0 + kChunk);
+        float part[R][2] = {};
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const v4f_any v = *(const v4f_any *)&rows_of[r][256 * t + 4 * lane];
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) part[r][j] = __builtin_fmaf(v[e], own[j][t][e], part[r][j]);
+            }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) all[r][j] += part[r][j];
+    }
+    float mine = 0.0f;   // lane 2 r + j has row r, column j
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            float v = all[r][j];
+#pragma unroll
+            for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
+            if (lane == 2 * r + j) mine = v;
+        }
+    const int r = lane >> 1, c = c0 + (lane & 1);
+    if (r >= rows || c >= l.N) return;
+    const DenseEpilogue ep{bias ? bias + s.group * N : nullptr, nullptr, pre ? pre + row * N : nullptr, act, N};
+    y[(row + r) * N + c] = ep(mine, r * N + c);
 }
 
 // The gradients in one launch, each by its own workgroups: dx = dz w, a tile of 32 rows of a group by 32 of the K columns; dw = dz^T x over
@@ -172,8 +267,8 @@ int check(const char *who, size_t G, size_t M, size_t N, size_t K, int act)
     return DOPT_HIP_OK;
 }
 
-// What the small products take, in us: launches, and operands that every tile of 32 x 32 reads by itself, rounds of tiles; of gradients their rows, and
-// a workgroup for each tile of each group's dw.  The way that takes the least is taken; the costs are fitted to 181 products and 119 gradients, where it
+// What the small products take, in us: launches, rounds of tiles of 32 x 32 that each read their operands, or all of w; of gradients their rows, and a
+// workgroup for each tile of each group's dw.  The way that takes the least is taken; the costs are fitted to 181 products and 119 gradients, where it
 // took within 10 % of the fastest way's time but for one product and four gradients.  Eight groups, small, split and wide:
 //     [64 x 512] from 512 7.4 10.7 29       [1024 x 512] from 512 19 13 36       [4096 x 512] from 512 46 28 39       [16384 x 512] from 512 156 77 70
 //     [1024 x 1024] from 1024 45 28 51      [8192 x 1024] from 1024 279 123 107  [512 x 4096] from 1024 104 50 85
@@ -182,16 +277,34 @@ int check(const char *who, size_t G, size_t M, size_t N, size_t K, int act)
 //     [2048 x 1024] from 1024 171 86 90     [8192 x 1024] from 1024 436 298 221  [256 x 4096] from 1024 269 110 243
 double small_us(size_t G, size_t M, size_t N, size_t K)
 {
-    const double rounds = group_tiles(G, M, N, 32) / num_cus();
-    return 5 + 0.0101 * K * (rounds > 1 ? rounds + 0.5 : std::max(rounds, 0.65));
+    const double rounds = group_tiles(G, M, N, 32) / num_cus(), least = G * N * K > (size_t)1 << 26 ? 1.2 : 0.75;   // (w that the last cache does not hold)
+    return 5 + std::max(0.0101 * K * std::max(rounds > 1 ? rounds + 0.5 : rounds, least), weights_us(G, M, N, K, 3.5e6));
 }
 double small_grad_us(size_t G, size_t M, size_t N, size_t K)
 {
     const double m = (double)M, dw = ((double)N / 32 + 0.5) * ceil_div(K, (size_t)32);
     return 10.8 + 1e-6 * (10 * m * K + 7 * m * N + 13 * (group_tiles(G, M, K, 32) * N + dw * m)) + 6.6e-3 * G * dw;
 }
-enum class Way { kSmall, kSplit, kWide };
-Way way_of(double small, double split, double wide) { return small <= std::min(split, wide) ? Way::kSmall : split <= wide ? Way::kSplit : Way::kWide; }
+// Rows of a group that groups_few_k takes at a time, and its time: w of the groups that have rows, or the products of whole units, and its chunks.  Eight groups,
+// it and the small products: one row of [4096 x 4096] 15.0 and 62.6 us (w alone 13.1), two 29 and 68, eight 61 and 98, 32 121 and 131, 64 171 and 132;
+// eight rows of [512 x 512] 5.4 and 6.0, of [4096 x 1024] 22.8 and 28.3, of 1024 from 4096 18.6 and 34.2.
+int few_rows(size_t G, size_t M)
+{
+    const size_t rows = std::min(M, ceil_div(3 * M, 2 * G));
+    return rows <= 1 ? 1 : rows <= 2 ? 2 : 4;
+}
+double few_us(size_t G, size_t M, size_t N, size_t K)
+{
+    const double rows = few_rows(G, M), chunks = (double)ceil_div(K, (size_t)1024), groups = groups_with_rows(G, M);
+    const double units = std::max(groups, M / rows + (rows > 1 ? 0.75 * (groups - 1) : 0.0));
+    return 1.1 * (4.9 + 0.4 * chunks + std::max(weights_us(G, M, N, K, 5.1e6), 0.3 * units * ceil_div(N, (size_t)8) * chunks * rows / num_cus()));
+}
+enum class Way { kFew, kSmall, kSplit, kWide };
+Way way_of(double few, double small, double split, double wide)
+{
+    const double least = std::min(std::min(few, small), std::min(split, wide));
+    return few == least ? Way::kFew : small == least ? Way::kSmall : split == least ? Way::kSplit : Way::kWide;
+}
 
 size_t slice_of(size_t depth) { return ceil_div(ceil_div(depth, (size_t)kSmallWaves), (size_t)8) * 8; }
 
@@ -238,9 +351,19 @@ int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const
     if (int rc = apart(who, in, results)) return rc;
     DOPT_ENSURE_INIT();
     const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
-    const Way way = way_of(small_us(G, M, N, K), groups_split_us(G, M, N, K), groups_wide_us(G, M, N, K));
-    if (G > 0 && way == Way::kSplit) return groups_split(l, x, w, bias, act, y, pre);
-    if (G > 0 && way == Way::kWide) return groups_wide(l, x, w, bias, act, y, pre);
+    const Way way = G == 0 ? Way::kSmall : way_of(few_us(G, M, N, K), small_us(G, M, N, K), groups_split_us(G, M, N, K), groups_wide_us(G, M, N, K));
+    if (way == Way::kSplit) return groups_split(l, x, w, bias, act, y, pre);
+    if (way == Way::kWide) return groups_wide(l, x, w, bias, act, y, pre);
+    if (way == Way::kFew) {
+        auto few = [&](auto rows) {
+            constexpr int R = decltype(rows)::value;
+            hipLaunchKernelGGL(groups_few_k<R>, grid_of(ceil_div(N, (size_t)8), most_units(M, G + 2, R / 2)), dim3(256), 0, stream(), l, x, w, bias, y, pre, act);
+            DOPT_LAUNCH_CHECK();
+            return (int)DOPT_HIP_OK;
+        };
+        const int rows = few_rows(G, M);
+        return rows == 4 ? few(std::integral_constant<int, 4>{}) : rows == 2 ? few(std::integral_constant<int, 2>{}) : few(std::integral_constant<int, 1>{});
+    }
     const dim3 grid = grid_of(ceil_div(N, (size_t)32), most_units(M, G + 2, kTileShift));
     const int slice = (int)slice_of(K);
     if (K % 4) hipLaunchKernelGGL(groups_small_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
@@ -274,7 +397,7 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
         return clear(dbias, G * N);
     }
     const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
-    const Way way = way_of(small_grad_us(G, M, N, K), groups_split_grad_us(G, M, N, K), groups_wide_grad_us(G, M, N, K));
+    const Way way = way_of(HUGE_VAL, small_grad_us(G, M, N, K), groups_split_grad_us(G, M, N, K), groups_wide_grad_us(G, M, N, K));
     if ((dx || dw) && way == Way::kSplit) return groups_split_grad(l, act, dy, pre, x, w, dx, dw, dbias);
     if ((dx || dw) && way == Way::kWide) return groups_wide_grad(l, act, dy, pre, x, w, dx, dw, dbias);
     // Rows of a part of a group's reduction: at most 8192, 1024 for each wavefront, so that sums of one sign are not rounded the same way for

@@ -157,7 +157,8 @@ double groups_split_us(size_t G, size_t M, size_t N, size_t K)
 {
     if (N < 4 || K < 4) return HUGE_VAL;   // (of no use, and sums of dz want four columns)
     const double chunks = (double)ceil_div(K, (size_t)kChunk);
-    return 5 + chunks / 4 + 0.3 * group_tiles(G, M, N, kTile) * (chunks + 6) / num_cus() + 8.0 * M * N / 5e6;
+    const double products = chunks / 4 + 0.3 * group_tiles(G, M, N, kTile) * (chunks + 6) / num_cus();
+    return 5 + std::max(products, weights_us(G, M, N, K, 4e6)) + 8.0 * M * N / 5e6;
 }
 double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K)
 {

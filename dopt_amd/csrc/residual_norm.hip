@@ -997,11 +997,11 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
             const size_t least = ceil_div((size_t)runs.per_gate, kTeamRows * teams);
             const size_t most = ceil_div((size_t)runs.per_gate, held ? teams : (size_t)8);
             size_t best = 0;
-            for (size_t rounds = 1; rounds <= 3; rounds++) {
+            for (size_t rounds = 0; rounds <= 3; rounds++) {   // (none: a run for each gate)
                 size_t splits = std::max(least, std::min(most, std::max((size_t)1, rounds * launch.places / gates)));
                 const size_t of_team = ceil_div(ceil_div((size_t)runs.per_gate, splits), teams);
                 splits = std::max(least, ceil_div((size_t)runs.per_gate, of_team * teams));   // no more of them than so many rows need
-                const size_t turns = ceil_div(gates * splits, launch.places) * (of_team + 2);
+                const size_t turns = ceil_div(gates * splits, launch.places) * (of_team + 2) + (gates * splits > 1 ? 4 : 0);   // (the runs' sums are a launch)
                 if (best && turns >= best) continue;
                 best = turns;
                 runs.splits = (unsigned)splits;

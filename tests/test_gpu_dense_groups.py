@@ -234,6 +234,27 @@ def test_large(sizes, n, k):
         _check(t, R.ACTS[(n + i) % 4], up=_off_grid if i else ops.tensor, keep=i == 0, bias=i == 0)
 
 
+FEW = [([0, 0, 1], 300, 4097), ([1], 10, 5), ([1, 0, 2, 0], 129, 2048), ([1] * 64, 40, 1030), ([3, 0, 1, 4], 515, 1027), ([0, 2, 0, 0, 0, 0, 0, 0], 9, 1),
+       ([7, 5, 9, 0, 6, 8], 33, 1500), ([0, 1, 0, 0, 0, 0, 1, 0], 1024, 4096), ([2], 1000, 1023), ([4] * 8, 70, 2051)]
+
+
+@pytest.mark.parametrize("sizes,n,k", FEW, ids=lambda v: "%dx%d" % (len(v), sum(v)) if isinstance(v, list) else str(v))
+def test_single_tokens(sizes, n, k):
+    for i, (before, after) in enumerate(((0, 0), (2, 3))):
+        t = _case(sizes, n, k, n + i, before, after)
+        _check(t, R.ACTS[(n + i) % 4], up=_off_grid if i else ops.tensor, keep=i == 0, bias=i == 0)
+
+
+def test_single_tokens_with_values_that_are_not_finite():
+    t = _case([1, 0, 2, 1], 40, 1500, 1)
+    clean = ops.dense_groups(*[ops.tensor(t[c]) for c in ("x", "w", "offsets")]).numpy()
+    t["x"][1, 1499], t["w"][2, 7, 3], t["w"][1], t["x"][3, 1024] = np.nan, np.inf, np.nan, -np.inf
+    y = ops.dense_groups(*[ops.tensor(t[c]) for c in ("x", "w", "offsets")]).numpy()
+    cols = np.delete(np.arange(40), 7)
+    assert np.isnan(y[1]).all() and np.isinf(y[2, 7]) and np.isinf(y[3]).all()
+    assert np.array_equal(y[0], clean[0]) and np.array_equal(y[2, cols], clean[2, cols])
+
+
 MIDDLE = [([9, 0, 170, 3, 110, 80, 14, 200], 512, 512), ([70, 600, 1, 333], 300, 1111), ([200, 31, 257, 64, 90], 777, 200), ([500], 1024, 1024),
           ([3000, 100, 2500], 96, 130), ([16] * 64, 520, 260), ([1, 2, 3, 60], 2050, 1030), ([6000, 900, 0, 2000], 12, 1561), ([5000, 1000], 5, 830),
           ([7000], 31, 717), ([1200, 20, 4000], 48, 819)]
