@@ -19,33 +19,69 @@ using namespace dopt;
 
 constexpr int kTile = kSplitTile, kTileShift = 6;
 constexpr int kRunShift = 6;
+constexpr unsigned kMostParts = 16;   // of a reduction of y
 
-// y = act(x w^T + bias): a tile of rows of a group.
+// y = act(x w^T + bias): a tile of rows of a group, over one of several parts of the reduction where there are few tiles; those wait in `parts`, [part][M][N].
+struct SplitForward {
+    const float *x, *w, *bias;
+    float *y, *pre, *parts;
+    int act;
+    unsigned tiles, count, steps;   // side by side; parts, and steps of each
+};
 template <int kTeams, bool kPasses>
-__global__ __launch_bounds__(256 * kTeams) void groups_split_k(GroupLayer l, const float *x, const float *w, const float *bias, float *y, float *pre, int act)
+__global__ __launch_bounds__(256 * kTeams) void groups_split_k(GroupLayer l, SplitForward f)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const unsigned n0 = blockIdx.x * kTile;
-    if (n0 >= (unsigned)l.N) return;
+    const unsigned part = blockIdx.x / f.tiles, n0 = blockIdx.x % f.tiles * kTile;
+    if (part >= f.count) return;
     const Segment s = find_unit<true>(l.q, kTileShift, unit_id());
     if (s.group < 0) return;
     const size_t N = l.N, K = l.K;
     if (s.group == (int)l.q.G) {
+        if (f.parts) return;
         const size_t row = s.begin + ((size_t)s.unit << kTileShift);
         const int rows = (int)min(s.end - row, (size_t)kTile);
         for (int i = threadIdx.x; i < kTile * rows; i += 256 * kTeams) {
             const unsigned c = n0 + i % kTile;
             if (c >= N) continue;
             const size_t at = (row + i / kTile) * N + c;
-            y[at] = 0.0f;
-            if (pre) pre[at] = 0.0f;
+            f.y[at] = 0.0f;
+            if (f.pre) f.pre[at] = 0.0f;
         }
         return;
     }
-    const size_t begin = s.begin, g = (size_t)s.group;
-    const DenseEpilogue ep{bias ? bias + g * N : nullptr, nullptr, pre ? pre + begin * N : nullptr, act, N};
-    split_tile<kTeams, true, false, false, kPasses>(Matrix32{x + begin * K, K, s.end - s.begin}, Matrix32{w + g * N * K, K, (unsigned)N}, (unsigned)K,
-                                                s.unit << kTileShift, n0, ep, y + begin * N, lds);
+    const size_t begin = s.begin, g = (size_t)s.group, from = (size_t)part * f.steps;
+    const Matrix32 rows{f.x + begin * K + from, K, s.end - s.begin}, columns{f.w + g * N * K + from, K, (unsigned)N};
+    DenseEpilogue ep{f.bias ? f.bias + g * N : nullptr, nullptr, f.pre ? f.pre + begin * N : nullptr, f.act, N};
+    float *to = f.y;
+    if (f.parts) {
+        ep = DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, N};
+        to = f.parts + part * (size_t)l.q.M * N;
+    }
+    split_tile<kTeams, true, false, false, kPasses>(rows, columns, (unsigned)min((size_t)f.steps, K - from), s.unit << kTileShift, n0, ep, to + begin * N, lds);
+}
+// Adds the parts, and the layer's end: a row of a group by 256 columns.  (All parts on their way at once: one after the other they took 20 us.)
+__global__ __launch_bounds__(256) void groups_end_k(GroupLayer l, SplitForward f)
+{
+    const size_t N = l.N, c = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if ((size_t)blockIdx.x * 256 >= N) return;
+    const Segment s = find_unit<true>(l.q, 0, unit_id());
+    if (s.group < 0 || c >= N) return;
+    const size_t at = ((size_t)s.begin + s.unit) * N + c, matrix = (size_t)l.q.M * N;
+    if (s.group == (int)l.q.G) {
+        f.y[at] = 0.0f;
+        if (f.pre) f.pre[at] = 0.0f;
+        return;
+    }
+    float part[kMostParts], z = 0.0f;
+#pragma unroll
+    for (unsigned p = 0; p < kMostParts; p++) part[p] = p < f.count ? f.parts[p * matrix + at] : 0.0f;
+#pragma unroll
+    for (unsigned p = 0; p < kMostParts; p++) z += part[p];
+    const DenseEpilogue ep{f.bias ? f.bias + s.group * N : nullptr, nullptr, f.pre, f.act, N};
+    z += ep.bias_of(c);
+    if (f.pre) f.pre[at] = z;
+    f.y[at] = ep.value(z);
 }
 
 // The gradients in one launch, as dense_groups.hip's: dx = dz w, whose reduction is often the longer one and is shared by teams; dw = dz^T x over 2^shift rows of a
@@ -130,6 +166,21 @@ GradWork grad_work(size_t G, size_t M, size_t N, size_t K)
     return GradWork{group_tiles(G, M, K, kTile), (double)ceil_div(N, (size_t)kChunk), units * tiles, M / units / kChunk + 0.5};
 }
 
+// A product's time, and in how many parts its reduction is the fastest: another launch, and the parts written and read.  One group, [108 x 367] from 2458 whole
+// 40 us (by the small products 31), in sixteen parts 15; four, [600 x 200] from 3986 57 (48) and 25, [3000 x 64] 50 (45) and 27.
+double forward_us(size_t G, size_t M, size_t N, size_t K, size_t *parts)
+{
+    const double chunks = (double)ceil_div(K, (size_t)kChunk), tiles = group_tiles(G, M, N, kTile);
+    double best = HUGE_VAL;
+    for (size_t p = 1; p == 1 || (p <= kMostParts && p <= chunks / 4); p *= 2) {
+        const double products = chunks / p / 4 + 0.3 * tiles * (chunks + 6 * p) / num_cus();
+        const double end = p > 1 ? 4.5 + 8.0 * p * M * N / 5e6 + 1e-3 * M * ceil_div(N, (size_t)256) : 0.0;
+        const double us = 5 + std::max(products, weights_us(G, M, N, K, 4e6)) + 8.0 * M * N / 5e6 + end;
+        if (us < best) best = us, *parts = p;
+    }
+    return best;
+}
+
 template <auto kKernel, int kTeams>
 int allow()
 {
@@ -156,9 +207,8 @@ namespace dopt {
 double groups_split_us(size_t G, size_t M, size_t N, size_t K)
 {
     if (N < 4 || K < 4) return HUGE_VAL;   // (of no use, and sums of dz want four columns)
-    const double chunks = (double)ceil_div(K, (size_t)kChunk);
-    const double products = chunks / 4 + 0.3 * group_tiles(G, M, N, kTile) * (chunks + 6) / num_cus();
-    return 5 + std::max(products, weights_us(G, M, N, K, 4e6)) + 8.0 * M * N / 5e6;
+    size_t parts;
+    return forward_us(G, M, N, K, &parts);
 }
 double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K)
 {
@@ -169,17 +219,26 @@ double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K)
 
 int groups_split(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
 {
-    const dim3 grid = grid_of(ceil_div((size_t)l.N, (size_t)kTile), most_units(l.q.M, l.q.G + 2, kTileShift));
+    const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, across = ceil_div(N, (size_t)kTile);
+    size_t parts;
+    forward_us(G, M, N, K, &parts);
+    SplitForward f{x, w, bias, y, pre, nullptr, act, (unsigned)across, (unsigned)parts, (unsigned)(ceil_div(ceil_div(K, (size_t)kChunk), parts) * kChunk)};
+    f.count = (unsigned)ceil_div(K, (size_t)f.steps);
+    if (parts > 1 && !(f.parts = (float *)workspace(f.count * M * N * sizeof(float)))) return DOPT_HIP_ERR_OOM;
     // (workgroups and one, two, four teams: 160 18.9 14.0 12.7 us, 288 22.1 19.4 23.7, 544 28.0 30.0 36.4, reductions of 512 steps)
-    const double tiles = group_tiles(l.q.G, l.q.M, l.N, kTile);
+    const double tiles = group_tiles(G, M, N, kTile) * parts;
     const int teams = tiles <= num_cus() ? 4 : tiles <= 2 * num_cus() ? 2 : 1;
-    return with_teams<4>(teams, l.K > (int)kPass * 16, [&](auto n, auto passes) {
+    const int rc = with_teams<4>(teams, f.steps > kPass * 16, [&](auto n, auto passes) {
         constexpr auto kernel = groups_split_k<n.value, passes.value>;
         if (int rc = allow<kernel, n.value>()) return rc;
-        hipLaunchKernelGGL(kernel, grid, dim3(256 * n.value), kSplitLds<n.value>, stream(), l, x, w, bias, y, pre, act);
+        hipLaunchKernelGGL(kernel, grid_of(across * f.count, most_units(M, G + 2, kTileShift)), dim3(256 * n.value), kSplitLds<n.value>, stream(), l, f);
         DOPT_LAUNCH_CHECK();
         return (int)DOPT_HIP_OK;
     });
+    if (rc || parts == 1) return rc;
+    hipLaunchKernelGGL(groups_end_k, grid_of(ceil_div(N, (size_t)256), most_units(M, G + 2, 0)), dim3(256), 0, stream(), l, f);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
 }
 
 int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
