@@ -268,8 +268,8 @@ int check(const char *who, size_t G, size_t M, size_t N, size_t K, int act)
 }
 
 // What the small products take, in us: launches, rounds of tiles of 32 x 32 that each read their operands, or all of w; of gradients their rows, and a
-// workgroup for each tile of each group's dw.  The way that takes the least is taken; the costs are fitted to 181 products and 119 gradients, where it
-// took within 10 % of the fastest way's time but for one product and four gradients.  Eight groups, small, split and wide:
+// workgroup for each tile of each group's dw.  The way that takes the least is taken; the costs are fitted to some 350 products and 120 gradients, of
+// which a dozen take more than 10 % longer than by the fastest way.  Eight groups, small, split and wide:
 //     [64 x 512] from 512 7.4 10.7 29       [1024 x 512] from 512 19 13 36       [4096 x 512] from 512 46 28 39       [16384 x 512] from 512 156 77 70
 //     [1024 x 1024] from 1024 45 28 51      [8192 x 1024] from 1024 279 123 107  [512 x 4096] from 1024 104 50 85
 // and gradients

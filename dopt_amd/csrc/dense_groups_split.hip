@@ -4,7 +4,7 @@
 //
 // With many tiles bound by what a CU takes in: 16 KB a chunk of 32 steps in 830 cycles, 47 GB/s (of which the matrix instructions need 192, 110 vector
 // instructions of each wavefront 450 and LDS 300): [16384 x 4096] from 2048 in sixteen groups 1450 us, dense_groups_wide.hip's 1030.  With few tiles by the
-// way from memory to the sums, some 0.9 us a chunk: [1024 x 1024] from 1024 in eight groups 29 us.  Tiles of 128 x 128, by four wavefronts (two to a SIMD) or
+// way from memory to the sums, some 0.9 us a chunk: [1024 x 1024] from 1024 in eight groups 28 us.  Tiles of 128 x 128, by four wavefronts (two to a SIMD) or
 // eight, take 1100 and 1090 us for the one and 53 and 42 for the other.
 #include <algorithm>
 #include <cmath>
@@ -170,12 +170,12 @@ GradWork grad_work(size_t G, size_t M, size_t N, size_t K)
 // 40 us (by the small products 31), in sixteen parts 15; four, [600 x 200] from 3986 57 (48) and 25, [3000 x 64] 50 (45) and 27.
 double forward_us(size_t G, size_t M, size_t N, size_t K, size_t *parts)
 {
-    const double chunks = (double)ceil_div(K, (size_t)kChunk), tiles = group_tiles(G, M, N, kTile);
+    const double chunks = (double)ceil_div(K, (size_t)kChunk), tiles = group_tiles(G, M, N, kTile), weights = weights_us(G, M, N, K, 4e6);
     double best = HUGE_VAL;
     for (size_t p = 1; p == 1 || (p <= kMostParts && p <= chunks / 4); p *= 2) {
         const double products = chunks / p / 4 + 0.3 * tiles * (chunks + 6 * p) / num_cus();
         const double end = p > 1 ? 4.5 + 8.0 * p * M * N / 5e6 + 1e-3 * M * ceil_div(N, (size_t)256) : 0.0;
-        const double us = 5 + std::max(products, weights_us(G, M, N, K, 4e6)) + 8.0 * M * N / 5e6 + end;
+        const double us = 5 + std::max(products, weights) + 8.0 * M * N / 5e6 + end;
         if (us < best) best = us, *parts = p;
     }
     return best;

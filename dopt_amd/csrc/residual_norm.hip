@@ -16,8 +16,8 @@
 // run of rows with the scales in LDS and the next rows on their way, and adds up the columns in registers: two sums for the branch's three results,
 // since dps, dpb and dgate follow from the sums of t zb and of t over a gate's rows.  A second launch adds the runs.  No atomics: every sum has one order.
 //
-// [16384 x 1024] forward 53 us (5.0 TB/s), backward 88 and 6 for the runs (4.3); [8192 x 4096] forward 99.6 (5.4); [4107 x 1111] with 37 gates backward 29 and 6;
-// one row of 512 3.4, a launch.  Rows of more than 8192 values leave a CU one workgroup, whose reads and writes take turns: [1024 x 16384] 92 forward, 174
+// [16384 x 1024] forward 53 us (5.0 TB/s), backward 88 and 6 for the runs (4.3); [8192 x 4096] forward 99.6 (5.4); [4107 x 1111] with 37 gates backward
+// 29 and 6; one row of 512 3.5, a launch; [256 x 1024] backward 14, [1024 x 256] 11: two launches, and the way of a row through both norms.  Rows of more than 8192 values leave a CU one workgroup, whose reads and writes take turns: [1024 x 16384] 92 forward, 174
 // backward (2.9 and 2.3 TB/s); beyond 16384 a fifth of the rate is left ([500 x 20000] 114 and 182).
 #include <algorithm>
 #include <type_traits>
