@@ -84,11 +84,13 @@ __global__ __launch_bounds__(256) void groups_end_k(GroupLayer l, SplitForward f
     f.y[at] = ep.value(z);
 }
 
-// The gradients in one launch, as dense_groups.hip's: dx = dz w, whose reduction is often the longer one and is shared by teams; dw = dz^T x over 2^shift rows of a
-// group, a tile for each team; dbias.
+// The gradients in one launch, as dense_groups.hip's: dx = dz w, whose reduction is often the longer one, is shared by teams and may be several parts
+// ([109 x 2573] from 1017 in five groups 75 -> 57 us); dw = dz^T x over 2^shift rows of a group, a tile for each team; dbias.
 struct SplitGrads {
     const float *dz, *x, *w, *sums;
-    float *dx, *dw, *parts, *dbias;   // parts: or null
+    float *dx, *dw, *parts, *dbias;   // parts: of dw, or null
+    float *dx_parts;                  // [part][M][K], or null
+    unsigned dx_across, dx_count, dx_steps;
     int shift;
     unsigned dx_tiles, dw_tiles, fold_tiles;
     size_t dx_blocks, dw_blocks, fold_blocks;
@@ -102,21 +104,24 @@ __global__ __launch_bounds__(256 * kTeams) void groups_split_grad_k(GroupLayer l
     size_t block = (size_t)blockIdx.y * kRow + blockIdx.x;
     const size_t N = l.N, K = l.K;
     if (block < g.dx_blocks) {
-        const unsigned k0 = (unsigned)(block % g.dx_tiles) * kTile;
-        if (k0 >= K) return;
+        const unsigned at = (unsigned)(block % g.dx_tiles), part = at / g.dx_across, k0 = at % g.dx_across * kTile;
+        if (part >= g.dx_count) return;
         const Segment s = find_unit<true>(l.q, kTileShift, (unsigned)(block / g.dx_tiles));
         if (s.group < 0) return;
-        const size_t begin = s.begin;
+        const size_t begin = s.begin, from = (size_t)part * g.dx_steps;
         if (s.group == (int)l.q.G) {
+            if (g.dx_parts) return;
             const size_t row = begin + ((size_t)s.unit << kTileShift);
             const int rows = (int)min(s.end - row, (size_t)kTile);
             for (int i = threadIdx.x; i < kTile * rows; i += 256 * kTeams)
                 if (k0 + i % kTile < K) g.dx[(row + i / kTile) * K + k0 + i % kTile] = 0.0f;
             return;
         }
-        return split_tile<kTeams, true, false, true, kPasses>(Matrix32{g.dz + begin * N, N, s.end - s.begin}, Matrix32{g.w + s.group * N * K, K, (unsigned)K},
-                                                          (unsigned)N, s.unit << kTileShift, k0,
-                                                          DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, g.dx + begin * K, lds);
+        float *const to = g.dx_parts ? g.dx_parts + part * (size_t)l.q.M * K : g.dx;
+        return split_tile<kTeams, true, false, true, kPasses>(Matrix32{g.dz + begin * N + from, N, s.end - s.begin},
+                                                              Matrix32{g.w + (s.group * N + from) * K, K, (unsigned)K},
+                                                              (unsigned)min((size_t)g.dx_steps, N - from), s.unit << kTileShift, k0,
+                                                              DenseEpilogue{nullptr, nullptr, nullptr, DOPT_HIP_ACT_NONE, K}, to + begin * K, lds);
     }
     block -= g.dx_blocks;
     if (block < g.dw_blocks) {
@@ -150,20 +155,39 @@ int part_shift(size_t G, size_t M, size_t tiles)
     while (shift > 8 && most_units(M, G, shift) * tiles < (size_t)num_cus()) shift--;
     return shift;
 }
+// Parts of [M, N] written and read by a launch of their own.
+double parts_us(size_t parts, size_t M, size_t N) { return 4.5 + 8.0 * parts * M * N / 5e6 + 1e-3 * M * ceil_div(N, (size_t)256); }
+
 // Tiles of both products, and chunks of each.
 struct GradWork {
-    double dx_tiles, dx_chunks, dw_tiles, dw_chunks;
+    double dx_tiles, dx_chunks, dw_tiles, dw_chunks;   // dx' chunks of a part
+    size_t parts;                                      // of dx' reductions
     double chain() const { return std::max(dx_chunks, dw_chunks); }
     // One workgroup's chunks take longer than all of them over the chip: [1024 x 512] from 512 in eight groups with one team 31.4 us, with two 29.8, with
     // four 35.3; [2048 x 512] 39 46 49; [256 x 4096] from 1024 151 110 113; [1024 x 4096] 179 177 191.
-    bool few() const { return dx_tiles * dx_chunks + dw_tiles * dw_chunks < 1.5 * chain() * num_cus(); }
+    bool few() const { return dx_tiles * parts * dx_chunks + dw_tiles * dw_chunks < 1.5 * chain() * num_cus(); }
+    double us() const
+    {
+        return (0.25 * dx_tiles * parts * (dx_chunks + 18) + 0.44 * dw_tiles * (dw_chunks + 0.2)) / num_cus() + 0.57 * chain();
+    }
 };
-GradWork grad_work(size_t G, size_t M, size_t N, size_t K)
+GradWork grad_work(size_t G, size_t M, size_t N, size_t K, double *total)
 {
     const size_t tiles = ceil_div(N, (size_t)kTile) * ceil_div(K, (size_t)kTile);
     const int shift = part_shift(G, M, tiles);
     const double units = (size_t)1 << shift < M ? std::max((double)G, (double)M / ((size_t)1 << shift) + 0.5 * G) : (double)G;
-    return GradWork{group_tiles(G, M, K, kTile), (double)ceil_div(N, (size_t)kChunk), units * tiles, M / units / kChunk + 0.5};
+    const double chunks = (double)ceil_div(N, (size_t)kChunk);
+    GradWork best{group_tiles(G, M, K, kTile), chunks, units * tiles, M / units / kChunk + 0.5, 1};
+    double least = best.us();
+    for (size_t p = 2; p <= kMostParts && p <= chunks / 4; p *= 2) {
+        GradWork w = best;
+        w.parts = p;
+        w.dx_chunks = chunks / p;
+        const double us = w.us() + parts_us(p, M, K);
+        if (us < least) least = us, best = w;
+    }
+    *total = least;
+    return best;
 }
 
 // A product's time, and in how many parts its reduction is the fastest: another launch, and the parts written and read.  One group, [108 x 367] from 2458 whole
@@ -174,8 +198,7 @@ double forward_us(size_t G, size_t M, size_t N, size_t K, size_t *parts)
     double best = HUGE_VAL;
     for (size_t p = 1; p == 1 || (p <= kMostParts && p <= chunks / 4); p *= 2) {
         const double products = chunks / p / 4 + 0.3 * tiles * (chunks + 6 * p) / num_cus();
-        const double end = p > 1 ? 4.5 + 8.0 * p * M * N / 5e6 + 1e-3 * M * ceil_div(N, (size_t)256) : 0.0;
-        const double us = 5 + std::max(products, weights) + 8.0 * M * N / 5e6 + end;
+        const double us = 5 + std::max(products, weights) + 8.0 * M * N / 5e6 + (p > 1 ? parts_us(p, M, N) : 0.0);
         if (us < best) best = us, *parts = p;
     }
     return best;
@@ -200,6 +223,13 @@ int with_teams(int teams, bool passes, F &&f)
     return with(std::integral_constant<int, 1>{});
 }
 
+int end_of_parts(const GroupLayer &l, const SplitForward &f)
+{
+    hipLaunchKernelGGL(groups_end_k, grid_of(ceil_div((size_t)l.N, (size_t)256), most_units(l.q.M, l.q.G + 2, 0)), dim3(256), 0, stream(), l, f);
+    DOPT_LAUNCH_CHECK();
+    return DOPT_HIP_OK;
+}
+
 }  // namespace
 
 namespace dopt {
@@ -213,8 +243,9 @@ double groups_split_us(size_t G, size_t M, size_t N, size_t K)
 double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K)
 {
     if (N < 4 || K < 4) return HUGE_VAL;
-    const GradWork of = grad_work(G, M, N, K);
-    return 11.5 + 3.4e-6 * M * N + (0.25 * of.dx_tiles * (of.dx_chunks + 18) + 0.44 * of.dw_tiles * (of.dw_chunks + 0.2)) / num_cus() + 0.57 * of.chain();
+    double products;
+    grad_work(G, M, N, K, &products);
+    return 11.5 + 3.4e-6 * M * N + products;
 }
 
 int groups_split(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
@@ -235,10 +266,7 @@ int groups_split(const GroupLayer &l, const float *x, const float *w, const floa
         DOPT_LAUNCH_CHECK();
         return (int)DOPT_HIP_OK;
     });
-    if (rc || parts == 1) return rc;
-    hipLaunchKernelGGL(groups_end_k, grid_of(ceil_div(N, (size_t)256), most_units(M, G + 2, 0)), dim3(256), 0, stream(), l, f);
-    DOPT_LAUNCH_CHECK();
-    return DOPT_HIP_OK;
+    return rc || parts == 1 ? rc : end_of_parts(l, f);
 }
 
 int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
@@ -246,24 +274,29 @@ int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float
     const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, tiles = ceil_div(N, (size_t)kTile) * ceil_div(K, (size_t)kTile);
     const int shift = dw ? part_shift(G, M, tiles) : kLongestPart;
     const bool direct = ((size_t)1 << shift) >= M, plain = act == DOPT_HIP_ACT_NONE;
-    const size_t dw_units = most_units(M, G, shift), runs = most_units(M, G, kRunShift), f = sizeof(float);
+    double unused;
+    const GradWork work = grad_work(G, M, N, K, &unused);
+    const size_t dw_units = most_units(M, G, shift), runs = most_units(M, G, kRunShift), f = sizeof(float), across = ceil_div(K, (size_t)kTile);
+    const size_t steps = ceil_div(ceil_div(N, (size_t)kChunk), dx ? work.parts : 1) * kChunk, count = ceil_div(N, steps);
     auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
-    const size_t dz_bytes = plain ? 0 : rounded(M * N * f), sum_bytes = dbias ? rounded(runs * N * f) : 0, part_bytes = dw && !direct ? dw_units * N * K * f : 0;
-    char *const scratch = dz_bytes + sum_bytes + part_bytes ? (char *)workspace(dz_bytes + sum_bytes + part_bytes) : nullptr;
-    if (dz_bytes + sum_bytes + part_bytes && !scratch) return DOPT_HIP_ERR_OOM;
-    float *const dz_to = plain ? nullptr : (float *)scratch, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
+    const size_t dz_bytes = plain ? 0 : rounded(M * N * f), sum_bytes = dbias ? rounded(runs * N * f) : 0, dx_bytes = count > 1 ? rounded(count * M * K * f) : 0;
+    const size_t part_bytes = dw && !direct ? dw_units * N * K * f : 0, bytes = dz_bytes + sum_bytes + dx_bytes + part_bytes;
+    char *const scratch = bytes ? (char *)workspace(bytes) : nullptr;
+    if (bytes && !scratch) return DOPT_HIP_ERR_OOM;
+    float *const dz_to = plain ? nullptr : (float *)scratch, *const sums = (float *)(scratch + dz_bytes);
+    float *const dx_parts = dx_bytes ? (float *)(scratch + dz_bytes + sum_bytes) : nullptr, *const parts = (float *)(scratch + dz_bytes + sum_bytes + dx_bytes);
     if (!plain || dbias)
         if (int rc = groups_dz(l, act, kRunShift, dy, pre, dz_to, dbias ? sums : nullptr)) return rc;
-    const int teams = grad_work(G, M, N, K).few() ? 2 : 1;
-    SplitGrads g{plain ? dy : dz_to, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, shift, (unsigned)abreast(ceil_div(K, (size_t)kTile)),
-                 (unsigned)abreast(ceil_div(tiles, (size_t)teams)), (unsigned)abreast(ceil_div(N, (size_t)32)), 0, 0, 0};
+    const int teams = work.few() ? 2 : 1;
+    SplitGrads g{plain ? dy : dz_to, x, w, sums, dx, dw, direct ? nullptr : parts, dbias, dx_parts, (unsigned)across, (unsigned)count, (unsigned)steps, shift,
+                 (unsigned)abreast(across * count), (unsigned)abreast(ceil_div(tiles, (size_t)teams)), (unsigned)abreast(ceil_div(N, (size_t)32)), 0, 0, 0};
     if (dx) g.dx_blocks = g.dx_tiles * most_units(M, G + 2, kTileShift);
     if (dw) g.dw_blocks = g.dw_tiles * dw_units;
     if (dbias) g.fold_blocks = g.fold_tiles * G;
     const size_t blocks = g.dx_blocks + g.dw_blocks + g.fold_blocks;
     DOPT_REQUIRE(blocks < ((size_t)1 << 37), "dopt_hip_dense_groups_grad: dimensions too large");
     const dim3 grid((unsigned)std::min(blocks, (size_t)kRow), (unsigned)ceil_div(blocks, (size_t)kRow));
-    const bool passes = (dx && N > kPass * 16) || (dw && std::min(M, (size_t)1 << shift) > kPass * 16);
+    const bool passes = (dx && steps > kPass * 16) || (dw && std::min(M, (size_t)1 << shift) > kPass * 16);
     const int rc = with_teams<2>(teams, passes, [&](auto n, auto passes) {
         constexpr auto kernel = groups_split_grad_k<n.value, passes.value>;
         if (int rc = allow<kernel, n.value>()) return rc;
@@ -272,6 +305,8 @@ int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float
         return (int)DOPT_HIP_OK;
     });
     if (rc) return rc;
+    if (dx_parts)
+        if (int rc = end_of_parts(GroupLayer{l.q, l.K, 0}, SplitForward{nullptr, nullptr, nullptr, dx, nullptr, dx_parts, DOPT_HIP_ACT_NONE, 0, (unsigned)count, 0})) return rc;
     return dw && !direct ? groups_join(l, shift, parts, dw) : DOPT_HIP_OK;
 }
 

@@ -257,7 +257,8 @@ def test_single_tokens_with_values_that_are_not_finite():
 
 MIDDLE = [([9, 0, 170, 3, 110, 80, 14, 200], 512, 512), ([70, 600, 1, 333], 300, 1111), ([200, 31, 257, 64, 90], 777, 200), ([500], 1024, 1024),
           ([3000, 100, 2500], 96, 130), ([16] * 64, 520, 260), ([1, 2, 3, 60], 2050, 1030), ([6000, 900, 0, 2000], 12, 1561), ([5000, 1000], 5, 830),
-          ([7000], 31, 717), ([1200, 20, 4000], 48, 819), ([108], 367, 2458), ([40, 0, 60, 1], 130, 5001), ([64, 64], 1024, 4096), ([300], 70, 20000)]
+          ([7000], 31, 717), ([1200, 20, 4000], 48, 819), ([108], 367, 2458), ([40, 0, 60, 1], 130, 5001), ([64, 64], 1024, 4096), ([300], 70, 20000),
+          ([5, 23, 13, 0, 46, 10], 2573, 1017), ([83, 190, 109, 13], 2857, 265), ([40], 9000, 70)]
 
 
 @pytest.mark.parametrize("sizes,n,k", MIDDLE, ids=lambda v: "%dx%d" % (len(v), sum(v)) if isinstance(v, list) else str(v))
@@ -281,7 +282,7 @@ def test_middle_with_offsets_of_any_value(offsets):
     _check(t, "silu")
 
 
-@pytest.mark.parametrize("sizes,n,k", [([150, 0, 250, 100], 300, 500), ([600, 900, 20, 800], 300, 500), ([20, 0, 30, 10], 150, 3000)])
+@pytest.mark.parametrize("sizes,n,k", [([150, 0, 250, 100], 300, 500), ([600, 900, 20, 800], 300, 500), ([20, 0, 30, 10], 150, 3000), ([20, 0, 30, 10], 2500, 150)])
 def test_middle_with_values_that_are_not_finite(sizes, n, k):
     """One NaN or infinity in a chunk at the end or the beginning of its reduction, in each operand: it reaches what depends on it alone, as a sum of
     products does."""
