@@ -9,6 +9,7 @@
 // cache's share included), the clipped gradients 44.8 behind it, which start with what the norm has read last; 670 thousand 5.0 and 3.4, a launch each.
 #include <algorithm>
 #include <cmath>
+#include <new>
 #include <vector>
 
 #include "common.h"
@@ -173,6 +174,29 @@ void release(Handle *h)
     delete h;
 }
 
+int fill(Handle *h, int n, const dopt_hip_gradient_ref *refs)
+{
+    std::vector<Tensor> tensors;
+    std::vector<Chunk> chunks;
+    for (int i = 0; i < n; i++) {
+        const dopt_hip_gradient_ref &r = refs[i];
+        if (r.n > 0 && !r.out) h->has_out = false;
+        tensors.push_back(Tensor{r.g, r.out, r.n, aligned16(r.g) && aligned16(r.out)});
+        for (size_t at = 0; at < r.n; at += kChunk) chunks.push_back(Chunk{(unsigned)i, at});
+    }
+    h->refs.assign(refs, refs + n);
+    h->nchunks = chunks.size();
+    h->blocks = (unsigned)std::max((size_t)1, std::min(chunks.size(), (size_t)num_cus() * 4));
+    int rc = dopt_hip_malloc((void **)&h->parts, h->blocks * sizeof(double));
+    if (!rc) rc = dopt_hip_malloc((void **)&h->arrived, (1 + ceil_div(h->blocks, kTeam)) * kApart * sizeof(unsigned));   // (zero-filled)
+    if (rc || chunks.empty()) return rc;
+    rc = dopt_hip_malloc((void **)&h->tensors, tensors.size() * sizeof(Tensor));
+    if (!rc) rc = dopt_hip_malloc((void **)&h->chunks, chunks.size() * sizeof(Chunk));
+    if (!rc) rc = dopt_hip_copy_h2d(h->tensors, tensors.data(), tensors.size() * sizeof(Tensor));
+    if (!rc) rc = dopt_hip_copy_h2d(h->chunks, chunks.data(), chunks.size() * sizeof(Chunk));
+    return rc;
+}
+
 int norm(const Handle *h, float most, float *result, const char *who)
 {
     DOPT_REQUIRE(result != nullptr, "%s: the result is null", who);
@@ -194,34 +218,22 @@ int dopt_hip_gradient_norm_create(int ntensors, const dopt_hip_gradient_ref *ref
     DOPT_REQUIRE(handle != nullptr, "dopt_hip_gradient_norm_create: handle is null");
     *handle = nullptr;
     DOPT_REQUIRE(ntensors >= 0 && (ntensors == 0 || refs), "dopt_hip_gradient_norm_create: bad tensor list");
-    std::vector<Tensor> tensors;
-    std::vector<Chunk> chunks;
-    bool has_out = true;
     for (int i = 0; i < ntensors; i++) {
-        const dopt_hip_gradient_ref &r = refs[i];
-        DOPT_REQUIRE(r.n == 0 || r.g, "dopt_hip_gradient_norm_create: tensor %d is null", i);
-        DOPT_REQUIRE(r.n < (size_t)1 << 40, "dopt_hip_gradient_norm_create: tensor %d is too large", i);
-        if (r.n > 0 && !r.out) has_out = false;
-        tensors.push_back(Tensor{r.g, r.out, r.n, aligned16(r.g) && aligned16(r.out)});
-        for (size_t at = 0; at < r.n; at += kChunk) chunks.push_back(Chunk{(unsigned)i, at});
+        DOPT_REQUIRE(refs[i].n == 0 || refs[i].g, "dopt_hip_gradient_norm_create: tensor %d is null", i);
+        DOPT_REQUIRE(refs[i].n < (size_t)1 << 40, "dopt_hip_gradient_norm_create: tensor %d is too large", i);
     }
-    DOPT_REQUIRE(!tangled(ntensors, refs), "dopt_hip_gradient_norm_create: a result overlaps another result or a gradient that is not its own");
-    DOPT_ENSURE_INIT();
-    Handle *h = new Handle();
-    h->has_out = has_out;
-    h->refs.assign(refs, refs + ntensors);
-    h->nchunks = chunks.size();
-    h->blocks = (unsigned)std::max((size_t)1, std::min(chunks.size(), (size_t)num_cus() * 4));
-    int rc = dopt_hip_malloc((void **)&h->parts, h->blocks * sizeof(double));
-    if (!rc) rc = dopt_hip_malloc((void **)&h->arrived, (1 + ceil_div(h->blocks, kTeam)) * kApart * sizeof(unsigned));   // (zero-filled)
-    if (!rc && !chunks.empty()) {
-        rc = dopt_hip_malloc((void **)&h->tensors, tensors.size() * sizeof(Tensor));
-        if (!rc) rc = dopt_hip_malloc((void **)&h->chunks, chunks.size() * sizeof(Chunk));
-        if (!rc) rc = dopt_hip_copy_h2d(h->tensors, tensors.data(), tensors.size() * sizeof(Tensor));
-        if (!rc) rc = dopt_hip_copy_h2d(h->chunks, chunks.data(), chunks.size() * sizeof(Chunk));
+    Handle *h = nullptr;
+    int rc;
+    try {
+        DOPT_REQUIRE(!tangled(ntensors, refs), "dopt_hip_gradient_norm_create: a result overlaps another result or a gradient that is not its own");
+        DOPT_ENSURE_INIT();
+        h = new Handle();
+        rc = fill(h, ntensors, refs);
+    } catch (const std::bad_alloc &) {
+        rc = fail(DOPT_HIP_ERR_OOM, "dopt_hip_gradient_norm_create: out of host memory");
     }
     if (rc) {
-        release(h);
+        if (h) release(h);
         return rc;
     }
     *handle = h;
