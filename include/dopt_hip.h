@@ -591,7 +591,11 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
      pre = x * w[g]^T + bias[g],  y = act(pre)
    x [M,K], w [G,N,K], bias [G,N] (may be null), y and pre (may be null) [M,N]; offsets holds G + 1 row numbers on the device.  A boundary
    counts as the largest one up to it, and as no more than M, whatever is there; rows in front of the first group and
-   behind the last one belong to none: y and pre are zero there.  No result may overlap an operand or the other one. */
+   behind the last one belong to none: y and pre are zero there.  No result may overlap an operand or the other one.  All but small
+   products and those of single rows (and the gradients of all but small ones) are formed from two fp16 parts of each value, scaled row by
+   row: a value keeps 22 bits, or 2^-38 of its row's largest one; infinities and NaN reach what fp32 would give them.  Workspace: large
+   products four bytes a value of both operands, long reductions over few tiles the result for each of up to sixteen parts; gradients dz, its
+   column sums by runs of rows, and dw for each part of a group's rows. */
 int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const int32_t *offsets, const float *x, const float *w,
                           const float *bias, float *y, float *pre);
 /* With dz = dy * act'(pre): dx = dz * w[g] [M,K], zero for rows of no group; dw[g] = dz^T * x [G,N,K] and dbias[g] = column sums of dz
