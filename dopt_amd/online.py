@@ -32,16 +32,16 @@ def clipped(grads, maxNorm):
     """The gradients times min(1, maxNorm / norm), norm the square root of the sum of all their squares; as they are where maxNorm
     is None.  A gradient that stands for several parameters counts for each.  No counterpart in the reference."""
     _check_norm(maxNorm)
-    if maxNorm is None or np.isinf(maxNorm) or not grads:
+    most = np.inf if maxNorm is None or maxNorm > float(np.finfo(np.float32).max) else float(maxNorm)
+    if np.isinf(most) or not grads:
         return list(grads)
     total = None
     for g in grads:
         s = core.sum(g * g)
         total = s if total is None else total + s
     norm = sqrt(total)
-    # (one where the norm is in bounds, whatever maxNorm / norm is there)
-    over = core.gt(norm, float32([], [maxNorm]))
-    factor = over * (float32([], [maxNorm]) / core.max(norm, float32([], [np.finfo(np.float32).tiny]))) + (1.0 - over)
+    # (one where the norm is in bounds; the divisor is never zero, and the quotient at most one)
+    factor = float32([], [most]) / core.max(norm, float32([], [max(most, np.finfo(np.float32).tiny)]))
     return [g * factor for g in grads]
 
 

@@ -1,9 +1,11 @@
 """The norm of a set of gradients and clipping: what is refused before the device is touched."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 from dopt_amd import capi, core, online
+from oracle import evaluator
 
 P = C.c_void_p
 
@@ -55,3 +57,31 @@ def test_fused_updaters_refuse_a_norm_that_is_none(rule):
     for bad in (-1.0, float("nan")):
         with pytest.raises(ValueError, match="largest norm"):
             getattr(online, rule)([core.sum(x * x)], [x], maxNorm=bad)
+
+
+def _clipped(values, most):
+    """The graph's gradients as the oracle's evaluator has them."""
+    g = [core.float32(v.shape) for v in values]
+    return evaluator.evaluate(online.clipped(g, most), dict(zip(g, values)))
+
+
+@pytest.mark.parametrize("most", [0.0, 1e-30, 1.0, 4.0, 5.0, 1e3, 3e38, 1e39])
+@pytest.mark.parametrize("value", [0.0, 1e-24])
+def test_a_norm_of_zero_in_a_graph(value, most):
+    """Gradients of a step without any stay what they are: their norm is in bounds wherever it is not the largest one that is nothing, and then what
+    is left of them is nothing as well."""
+    values = [np.full((3, 4), value, np.float32), np.full(5, -value, np.float32)]
+    for got, v in zip(_clipped(values, most), values):
+        assert np.isfinite(got).all()
+        if most >= 1.0 or not value:
+            assert np.array_equal(got, v)
+
+
+@pytest.mark.parametrize("most", [0.5, 5.0, 12.9, 13.1, 1e39])
+def test_norms_of_ordinary_size_in_a_graph(most):
+    """3, 4 and 12 of two gradients: the norm is 13.  The factor is off by the roundings of four squares, their three sums, the root, the quotient: under
+    nine halves of a last place, and the product's."""
+    values = [np.array([[3.0, 4.0]], np.float32), np.array([0.0, -12.0], np.float32)]
+    for got, v in zip(_clipped(values, most), values):
+        want = v.astype(np.float64) * min(1.0, most / 13.0)
+        assert np.abs(got - want).max() <= 10 * 2.0 ** -24 * 12 and (most < 13 or np.array_equal(got, v))
