@@ -30,18 +30,27 @@ def _check_norm(maxNorm):
 
 def clipped(grads, maxNorm):
     """The gradients times min(1, maxNorm / norm), norm the square root of the sum of all their squares; as they are where maxNorm
-    is None.  A gradient that stands for several parameters counts for each.  No counterpart in the reference."""
+    is None.  A gradient that stands for several parameters counts for each.  Of any size: the squares are those of the gradients over the
+    largest magnitude, so that none overflows and what vanishes is too small to count.  NaN for a norm that is NaN, zero for an infinite one.  No counterpart in
+    the reference."""
     _check_norm(maxNorm)
-    most = np.inf if maxNorm is None or maxNorm > float(np.finfo(np.float32).max) else float(maxNorm)
+    low, high = float(np.finfo(np.float32).tiny), float(np.finfo(np.float32).max)
+    most = np.inf if maxNorm is None or maxNorm > high else float(maxNorm)
     if np.isinf(most) or not grads:
         return list(grads)
-    total = None
+    top = total = None
     for g in grads:
-        s = core.sum(g * g)
+        t = core.maxElement(core.abs(g))   # (passes over NaN, which the squares keep)
+        top = t if top is None else core.max(top, t)
+    top = core.min(core.max(top, float32([], [low])), float32([], [high]))
+    for g in grads:
+        v = g / top
+        s = core.sum(v * v)
         total = s if total is None else total + s
-    norm = sqrt(total)
-    # (one where the norm is in bounds; the divisor is never zero, and the quotient at most one)
-    factor = float32([], [most]) / core.max(norm, float32([], [max(most, np.finfo(np.float32).tiny)]))
+    # Norm and bound over the largest magnitude; the bound is cut where no norm comes near, so that the quotient is one within bounds and
+    # its divisor never zero.
+    norm, bound = sqrt(total), core.min(float32([], [most]) / top, float32([], [1e30]))
+    factor = bound / core.max(norm, core.max(bound, float32([], [low])))
     return [g * factor for g in grads]
 
 

@@ -242,3 +242,38 @@ def test_sgd_moves_by_the_clipped_gradients():
         assert np.abs(a * float(factor) - b).max() <= 4 * np.abs(a).max() * 2.0 ** -24 + 2 * (np.abs(w).max() + np.abs(a).max()) * 2.0 ** -24
     total = np.sqrt(sum((m ** 2).sum() for m in moved[1])) / 0.05
     assert abs(total - 0.3) < 1e-4
+
+
+@pytest.mark.parametrize("most", [0.0, 1e-3, 1.0, 5.0])
+@pytest.mark.parametrize("size", [0.0, 1e-24, 1.0, 1e20, 1e37])
+def test_a_graph_clips_gradients_of_any_size(size, most):
+    """As tests/test_gradient_norm_cpu.py has it, compiled for the device, with the same bound for each result; and the fused updates' factor, which is formed in
+    64 bits and rounded once, is within 20 roundings of the graph's."""
+    r = np.random.default_rng(7)
+    values = [(size * r.uniform(-9, 9, s)).astype(F32) for s in ((3, 4), (5,), (2, 2, 2))]
+    norm = np.sqrt(sum((v.astype(np.float64) ** 2).sum() for v in values))
+    factor = 1.0 if norm <= most else most / norm
+    g = [core.float32(v.shape) for v in values]
+    got = core.evaluate(online.clipped(g, most), dict(zip(g, values)))
+    for a, v in zip(got, values):
+        want = v.astype(np.float64) * factor
+        assert np.isfinite(a).all()
+        assert (np.abs(a - want) <= 21 * 2.0 ** -24 * np.abs(want) + np.abs(v) * 2.0 ** -149 + 2.0 ** -149).all()
+    fused = float(ops.GradientNorm([ops.tensor(v) for v in values]).norm(most).numpy()[1])
+    for a, v in zip(got, values):
+        assert (np.abs(a - v.astype(np.float64) * fused) <= 22 * 2.0 ** -24 * np.abs(v) * fused + np.abs(v) * 2.0 ** -148 + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("rule", ["sgd", "adam", "amsgrad", "muon"])
+@pytest.mark.parametrize("most", [1.0, 5.0])
+def test_a_step_without_gradients_moves_nothing(rule, most):
+    """Zero gradients: both forms leave the parameters as they are, to the bit."""
+    for fused in (True, False):
+        w, x = core.float32([6, 5]), core.float32([6, 5])
+        start = np.random.default_rng(3).standard_normal((6, 5)).astype(F32)
+        w.set_value(start)
+        loss = core.sum(w * x, [0, 1]).reshape([])
+        up = getattr(online, ("fused_" if fused else "") + rule)([loss], [w], maxNorm=most)
+        for _ in range(2):
+            up({x: ops.tensor(np.zeros((6, 5), F32))})
+        assert np.array_equal(w.value, start)

@@ -85,3 +85,28 @@ def test_norms_of_ordinary_size_in_a_graph(most):
     for got, v in zip(_clipped(values, most), values):
         want = v.astype(np.float64) * min(1.0, most / 13.0)
         assert np.abs(got - want).max() <= 10 * 2.0 ** -24 * 12 and (most < 13 or np.array_equal(got, v))
+
+
+@pytest.mark.parametrize("most", [0.0, 1e-25, 1e-3, 1.0, 5.0, 1e18, 1e22])
+@pytest.mark.parametrize("size", [1e-44, 1e-38, 1e-30, 1e-24, 1e-19, 1.0, 1e18, 1e20, 1e37])
+def test_gradients_of_any_size_in_a_graph(size, most):
+    """Against the definition in 64 bits.  A square over the largest one is off by three roundings of values over the largest, the sums of under thirty
+    values by thirty, the root halves that: the norm is within 18 roundings, the quotients add two, the product one.  A quotient or product
+    below the smallest normal number is off by up to 2^-149."""
+    r = np.random.default_rng(7)
+    values = [(size * r.uniform(-9, 9, s)).astype(np.float32) for s in ((3, 4), (5,), (2, 2, 2))]
+    norm = np.sqrt(sum((v.astype(np.float64) ** 2).sum() for v in values))
+    factor = 1.0 if norm <= most else most / norm
+    for got, v in zip(_clipped(values, most), values):
+        want = v.astype(np.float64) * factor
+        assert np.isfinite(got).all()
+        assert (np.abs(got - want) <= 21 * 2.0 ** -24 * np.abs(want) + np.abs(v) * 2.0 ** -149 + 2.0 ** -149).all()
+
+
+def test_gradients_that_are_not_finite_in_a_graph():
+    ordinary = np.array([1.0, -2.0], np.float32)
+    for most in (0.5, 5.0):
+        got = _clipped([ordinary, np.array([np.inf, 3.0], np.float32)], most)
+        assert not got[0].any() and np.isnan(got[1][0]) and got[1][1] == 0
+        got = _clipped([ordinary, np.array([np.nan, 3.0], np.float32)], most)
+        assert np.isnan(got[0]).all() and np.isnan(got[1]).all()
