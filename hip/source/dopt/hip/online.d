@@ -15,7 +15,8 @@
     nnet/lipschitz.d) runs as a second small plan after the kernel; one that also reads this batch's activations (the
     max-gain projections) can only be ordered correctly inside a single plan, so use $(D dopt.online) for those.
 
-    All of them clip the gradients to the norm $(D maxNorm) of them all, if that is finite; $(D dopt.online) has nothing of the kind.
+    All of them clip the gradients to the norm $(D maxNorm) of them all, if that is finite, and refuse one that is negative or
+    NaN; $(D dopt.online) has nothing of the kind.
 
     Written where no D compiler exists: never compiled.
 */
@@ -42,6 +43,8 @@ private class FusedUpdater
 {
     this(Rule rule, Operation[] outputs, Operation[] wrt, Projection[Operation] projs, float maxNorm)
     {
+        enforce(maxNorm >= 0, "the largest norm of the gradients has to be zero or more");   //(NaN is not)
+
         mRule = rule;
         mMaxNorm = maxNorm;
         mOutputs = outputs.dup;
