@@ -33,6 +33,7 @@ constexpr int kBlock = 256;          // of teams within a wavefront
 constexpr size_t kHeld = 16384;      // values of a row that a workgroup holds at most
 constexpr size_t kWholeRows = 16;    // of a gate
 constexpr size_t kTeamRows = 128;    // rows that a team adds up at most: sums of more values that are alike are rounded the same way for long
+constexpr size_t kMostRuns = (size_t)1 << 22;   // workgroups of a launch, which has fewer than 2^32 threads
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));   // sixteen bytes wherever they start
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int 
     }
     const int teams = team.teams();
     const unsigned mine = alike<kWaves>(team.index());
-    unsigned r = kWhole ? from + mine * runs.per_gate : from + mine;   // (beyond the rows by fewer than 2^12: 32 bits hold it)
+    unsigned r = kWhole ? from + mine * runs.per_gate : from + mine;   // (beyond the rows by fewer than 2^16: 32 bits hold it)
     unsigned left = runs.per_gate;   // kWhole: rows of this gate that are left
     const unsigned turns = kWhole ? (runs.gates + teams - 1) / teams * runs.per_gate : (to - from + teams - 1) / teams;
     auto fetch = [&](unsigned row, Row<Q> &v) {   // (a team without a row keeps the others company)
@@ -970,7 +971,8 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     Launch launch{nullptr, kBlock, 0, (size_t)num_cus() * 8};
     // Gates of few rows go to teams as a whole where there are many of them, else to a workgroup each, whose teams share the rows: [1500 x 600]
     // with 100 gates 19.6 us (as a whole 64), [2400 x 1500] with 200 33 (70), [2000 x 700] with 500 28 (27), [8000 x 600] with 1000 71 (51), with 4000 180 (50).
-    const bool whole = runs.per_gate < std::min(kWholeRows, 4 * teams) && d->gates > 2 * (size_t)num_cus();
+    // So do the gates of any number of rows where a launch has no workgroup for each (a team then adds up a whole gate, of at most 511 rows).
+    const bool whole = (runs.per_gate < std::min(kWholeRows, 4 * teams) && d->gates > 2 * (size_t)num_cus()) || d->gates >= kMostRuns;
     if (held) {
         int rc = DOPT_HIP_OK;
         with_form(form, [&](auto lanes, auto quads) {
@@ -1010,7 +1012,7 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
         }
     }
     const size_t blocks = runs.count;
-    DOPT_REQUIRE(blocks < (size_t)1 << 22, "%s: dimensions too large", who);
+    DOPT_REQUIRE(blocks < kMostRuns, "%s: dimensions too large", who);
     const bool gate_sums = dgate && !runs.gates && (runs.splits > 1 || d->rows == 0);
     const size_t to_add = blocks == 1 ? 0 : kinds;   // (one run's sums are the results)
     const size_t sums = (to_add + gate_sums) * blocks * row, means = held ? 0 : ceil_div(d->rows * sizeof(Means), (size_t)256) * 256;

@@ -114,6 +114,39 @@ def test_many_gates_of_few_rows(cols, per_gate):
     _check_backward(t, y, stats, post, pre, 0.7)
 
 
+@pytest.mark.parametrize("per_gate,cols", [(16, 2), (40, 1)])
+def test_gates_beyond_the_workgroups_of_a_launch(per_gate, cols):
+    """2^22 gates of more rows than a workgroup takes several gates of.  Single rows and gates as the definition has them at some thousand places; the scale's and
+    bias' gradients over all rows: a gate's rows and up to eight gates by a team, at most 48 teams, runs of those by 32 lanes in pieces of 64 are under 256
+    additions that follow each other."""
+    gates = 1 << 22
+    rows = gates * per_gate
+    r = np.random.default_rng(per_gate)
+    branch, dy = (r.standard_normal((rows, cols), F32) for _ in range(2))
+    branch += F32(0.5)
+    gate, scale = r.standard_normal((gates, cols), F32), _f(1 + 0.2 * r.standard_normal(cols))
+    d = [ops.tensor(a) for a in (dy, branch, gate, scale)]
+    y, _, stats = ops.residual_norm(None, d[1], d[2], "rms", d[3])
+    got = ops.residual_norm_grad(d[0], None, None, d[1], stats, d[2], "rms", d[3], out={n: ops.Tensor(s) for n, s in (
+        ("dbranch", (rows, cols)), ("dgate", (gates, cols)), ("dpost_scale", (cols,)))})
+    y, stats, got = y.numpy(), stats.numpy(), {k: v.numpy() for k, v in got.items()}
+    some = np.unique(np.r_[0, gates - 1, r.integers(0, gates, 3000)])
+    at = (some[:, None] * per_gate + np.arange(per_gate)).reshape(-1)
+    v = dict(dict.fromkeys(R.NAMES), post_scale=scale)
+    want = R.forward(None, branch[at], gate[some], "rms", "none", v, 1.0, 1e-5)
+    R_close(y[at], want["y"], "y")
+    R_close(stats[at], want["stats"], "stats")
+    want = R.backward(dy[at], None, None, branch[at], gate[some], stats[at], "rms", "none", v, 1.0)
+    R_close(got["dbranch"][at], want["dbranch"], "dbranch")
+    R_close(got["dgate"][some], want["dgate"], "dgate")
+    total = size = 0.0
+    for g in range(0, gates, 1 << 18):
+        s = slice(g * per_gate, (g + (1 << 18)) * per_gate)
+        q = dy[s].astype(np.float64) * branch[s] * stats[s, None] * np.repeat(gate[g:g + (1 << 18)], per_gate, 0)
+        total, size = total + q.sum(0), size + np.abs(q).sum(0)
+    R_close(got["dpost_scale"], (total, (256 + 8) * 2.0 ** -24 * size), "dpost_scale")
+
+
 def test_rows_beyond_thirty_two_bits_of_values():
     """2^32 values and more: rows before and behind that border, of which the others are zero."""
     rows, cols = (1 << 21) + 5, 2048 + 4
