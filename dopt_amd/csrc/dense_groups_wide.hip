@@ -42,15 +42,17 @@ struct ColumnJobs {
     int n, shift, w_rows;
 };
 constexpr int kWeightRun = 256;
+constexpr unsigned kColumnsRow = 1u << 22;   // workgroups of a row of the grid
 
 __global__ __launch_bounds__(256) void groups_columns_k(Groups q, ColumnJobs jobs)
 {
     __shared__ v4f_any red_sum[4][64];
     __shared__ unsigned red_top[4][64][4];
-    unsigned block = blockIdx.x;
+    unsigned block = blockIdx.y * kColumnsRow + blockIdx.x;
     int which = 0;
     while (which + 1 < jobs.n && block >= jobs.j[which].blocks) block -= jobs.j[which++].blocks;
     const Columns &j = jobs.j[which];
+    if (block >= j.blocks) return;   // (behind the end of the grid's last row)
     const unsigned unit = block / j.tiles;
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     const int c = min((int)(block % j.tiles) * 256 + 4 * lane, j.cols - 4);
@@ -373,6 +375,13 @@ int launch_products(const Groups &q, size_t tile, bool passes, const GroupProduc
     return passes ? launch_tiles<kSmall, true>(q, p) : launch_tiles<kSmall, false>(q, p);
 }
 
+// A row of workgroups has fewer than 2^32 threads.
+void launch_columns(const Groups &q, const ColumnJobs &jobs, size_t blocks)
+{
+    const dim3 grid((unsigned)std::min(blocks, (size_t)kColumnsRow), (unsigned)ceil_div(blocks, (size_t)kColumnsRow));
+    hipLaunchKernelGGL(groups_columns_k, grid, dim3(256), 0, stream(), q, jobs);
+}
+
 int shift_of_tile(size_t tile) { return tile == kBig ? 8 : 7; }
 
 // Threads of a workgroup that lays out rows of so many steps: in registers up to 1024.
@@ -395,11 +404,11 @@ int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const fl
     ColumnJobs jobs{};
     const unsigned tiles = (unsigned)ceil_div((size_t)l.N, (size_t)256);
     const size_t blocks = tiles * most_units(l.q.M, l.q.G, shift);
-    DOPT_REQUIRE(blocks < ((size_t)1 << 24), "dopt_hip_dense_groups_grad: dimensions too large");
+    DOPT_REQUIRE(blocks < ((size_t)1 << 32), "dopt_hip_dense_groups_grad: dimensions too large");
     jobs.j[0] = Columns{dy, pre, dz, sums, nullptr, l.N, act, tiles, 0, (unsigned)blocks};
     jobs.n = 1;
     jobs.shift = shift;
-    hipLaunchKernelGGL(groups_columns_k, dim3((unsigned)blocks), dim3(256), 0, stream(), l.q, jobs);
+    launch_columns(l.q, jobs, blocks);
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
@@ -517,7 +526,7 @@ int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float 
     jobs.w_rows = (int)N;
     unsigned blocks = 0;
     for (int i = 0; i < jobs.n; i++) blocks += jobs.j[i].blocks;
-    if (blocks) hipLaunchKernelGGL(groups_columns_k, dim3(blocks), dim3(256), 0, stream(), l.q, jobs);
+    if (blocks) launch_columns(l.q, jobs, blocks);
     DOPT_LAUNCH_CHECK();
     if (dbias) {
         lay.sums = sums;

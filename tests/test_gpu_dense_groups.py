@@ -432,3 +432,25 @@ def test_large_in_a_recorded_plan():
         plan.execute(args, rets)
         assert all(np.array_equal(r.numpy(), w) for r, w in zip(rets, want))
     assert plan.stats()["kernels"] and plan.recordings()["replays"] > 0
+
+
+@pytest.mark.parametrize("k", [1, 4])
+def test_gradients_of_more_rows_than_two_to_the_thirty(k):
+    """As many rows as the forward pass takes.  All but some rows are zero, so that sums have a term for each of those alone."""
+    m, n = (1 << 30) + 64, 4
+    offsets = np.array([0, (1 << 29) + 7, (1 << 30) + 40], np.int32)
+    places = [0, 5, (1 << 29) + 6, (1 << 29) + 7, (1 << 30) - 1, 1 << 30, (1 << 30) + 39, (1 << 30) + 40, m - 1]
+    r = np.random.default_rng(k)
+    dy_of, x_of = _f(r.standard_normal((len(places), n))), _f(r.standard_normal((len(places), k)))
+    w = _f(r.standard_normal((2, n, k)))
+    dy, x, dx = ops.Tensor((m, n)), ops.Tensor((m, k)), ops.Tensor((m, k))
+    for p, a, b in zip(places, dy_of, x_of):
+        dy.view(p * n, (n,)).set(a)
+        x.view(p * k, (k,)).set(b)
+        dx.view(p * k, (k,)).set(np.full(k, 7, F32))
+    _, dw, db = ops.dense_groups_grad(dy, x, ops.tensor(w), ops.tensor(offsets), dx=dx)
+    at = [0, 3, 7]   # places of the groups; the last two belong to none
+    want = D.backward(dy_of, x_of, w, None, at, "none", True)
+    R.close(np.stack([dx.view(p * k, (k,)).numpy() for p in places]), want[0], "dx")
+    R.close(dw.numpy(), want[1], "dw")
+    R.close(db.numpy(), want[2], "dbias")
