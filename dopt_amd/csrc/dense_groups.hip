@@ -26,8 +26,9 @@ typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));   // sixt
 constexpr int kRunShift = 6;     // rows that a thread adds up for dbias before it rounds to memory: 64
 typedef float SmallSums[32 * 33];
 
-// y = act(x w^T + bias): a tile of 32 rows of a group by 32 columns.
-template <bool kCut>
+// y = act(x w^T + bias): a tile of 32 rows of a group by 32 columns.  kLong: a wavefront has more than 1024 steps, which are added in parts of so many; in
+// one accumulator 2^20 equal products of one sign were off by 1e-3 of their sum.
+template <bool kCut, bool kLong>
 __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(GroupLayer l, int kslice, const float *x, const float *w, const float *bias, float *y,
                                                                     float *pre, int act)
 {
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_k(GroupLayer l,
         return;
     }
     const DenseEpilogue ep{bias ? bias + (size_t)s.group * l.N : nullptr, nullptr, pre ? pre + row * l.N : nullptr, act, (size_t)l.N};
-    sgemm_small_body<false, true, kCut, DenseEpilogue>(rows, l.N, l.K, l.K, l.K, kslice, x + row * l.K, w + (size_t)s.group * l.N * l.K, y + row * l.N,
+    sgemm_small_body<false, true, kCut, DenseEpilogue, kLong>(rows, l.N, l.K, l.K, l.K, kslice, x + row * l.K, w + (size_t)s.group * l.N * l.K, y + row * l.N,
                                                        nullptr, 0, nullptr, 0, nullptr, (int)blockIdx.x, 0, 0, l.K, red, ep);
 }
 
@@ -155,7 +156,7 @@ struct SmallGrads {
     size_t dx_blocks, dw_blocks, fold_blocks;
 };
 
-template <bool kCut>
+template <bool kCut, bool kLong>
 __device__ __forceinline__ void small_dx(const GroupLayer &l, const SmallGrads &g, unsigned tile, unsigned unit, SmallSums *red)
 {
     const int k0 = (int)tile * 32;
@@ -169,8 +170,8 @@ __device__ __forceinline__ void small_dx(const GroupLayer &l, const SmallGrads &
             if (k0 + (i & 31) < l.K) g.dx[(row + (i >> 5)) * l.K + k0 + (i & 31)] = 0.0f;
         return;
     }
-    sgemm_small_body<false, false, kCut>(rows, l.K, l.N, l.N, l.K, g.slice, g.dz + row * l.N, g.w + (size_t)s.group * l.N * l.K, g.dx + row * l.K, nullptr,
-                                         0, nullptr, 0, nullptr, (int)tile, 0, 0, l.N, red);
+    sgemm_small_body<false, false, kCut, NoEpilogue, kLong>(rows, l.K, l.N, l.N, l.K, g.slice, g.dz + row * l.N, g.w + (size_t)s.group * l.N * l.K,
+                                                            g.dx + row * l.K, nullptr, 0, nullptr, 0, nullptr, (int)tile, 0, 0, l.N, red);
 }
 
 __device__ __forceinline__ void small_dw(const GroupLayer &l, const SmallGrads &g, unsigned tile, unsigned unit, SmallSums *red)
@@ -188,12 +189,12 @@ __device__ __forceinline__ void small_dw(const GroupLayer &l, const SmallGrads &
 }
 
 constexpr unsigned kRow = 1u << 22;   // workgroups of a row of such a grid
-template <bool kCut>
+template <bool kCut, bool kLong>
 __global__ __launch_bounds__(64 * kSmallWaves) void groups_small_grad_k(GroupLayer l, SmallGrads g)
 {
     __shared__ SmallSums red[kSmallWaves];
     size_t block = (size_t)blockIdx.y * kRow + blockIdx.x;
-    if (block < g.dx_blocks) return small_dx<kCut>(l, g, (unsigned)(block % g.dx_tiles), (unsigned)(block / g.dx_tiles), red);
+    if (block < g.dx_blocks) return small_dx<kCut, kLong>(l, g, (unsigned)(block % g.dx_tiles), (unsigned)(block / g.dx_tiles), red);
     block -= g.dx_blocks;
     if (block < g.dw_blocks) return small_dw(l, g, (unsigned)(block % g.dw_tiles), (unsigned)(block / g.dw_tiles), red);
     block -= g.dw_blocks;
@@ -307,6 +308,13 @@ Way way_of(double few, double small, double split, double wide)
 }
 
 size_t slice_of(size_t depth) { return ceil_div(ceil_div(depth, (size_t)kSmallWaves), (size_t)8) * 8; }
+// Calls with a reduction's kinds: its rows are no whole quads; a wavefront's share is longer than a part.
+template <class F>
+void with_reduction(size_t depth, F &&f)
+{
+    auto with = [&](auto cut) { slice_of(depth) > (size_t)kSmallPart ? f(cut, std::true_type{}) : f(cut, std::false_type{}); };
+    depth % 4 ? with(std::true_type{}) : with(std::false_type{});
+}
 
 struct Span {
     const void *p;
@@ -366,8 +374,9 @@ int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const
     }
     const dim3 grid = grid_of(ceil_div(N, (size_t)32), most_units(M, G + 2, kTileShift));
     const int slice = (int)slice_of(K);
-    if (K % 4) hipLaunchKernelGGL(groups_small_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
-    else hipLaunchKernelGGL(groups_small_k<false>, grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
+    with_reduction(K, [&](auto cut, auto is_long) {
+        hipLaunchKernelGGL((groups_small_k<cut.value, is_long.value>), grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
+    });
     DOPT_LAUNCH_CHECK();
     return DOPT_HIP_OK;
 }
@@ -432,8 +441,9 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
     const size_t blocks = g.dx_blocks + g.dw_blocks + g.fold_blocks;
     DOPT_REQUIRE(blocks < ((size_t)1 << 37), "%s: dimensions too large", who);
     const dim3 grid((unsigned)std::min(blocks, (size_t)kRow), (unsigned)ceil_div(blocks, (size_t)kRow));
-    if (dx && N % 4) hipLaunchKernelGGL(groups_small_grad_k<true>, grid, dim3(64 * kSmallWaves), 0, stream(), l, g);
-    else hipLaunchKernelGGL(groups_small_grad_k<false>, grid, dim3(64 * kSmallWaves), 0, stream(), l, g);
+    with_reduction(dx ? N : 0, [&](auto cut, auto is_long) {
+        hipLaunchKernelGGL((groups_small_grad_k<cut.value, is_long.value>), grid, dim3(64 * kSmallWaves), 0, stream(), l, g);
+    });
     DOPT_LAUNCH_CHECK();
     return dw && !direct ? groups_join(l, shift, parts, dw) : DOPT_HIP_OK;
 }

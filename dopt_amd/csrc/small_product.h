@@ -48,8 +48,10 @@ __device__ __forceinline__ float small_value(const float (&v)[4], int e, int kk,
     return kKContig && kCut && e > 0 ? (kk + e < k_end ? v[e] : 0.0f) : v[e];
 }
 
-// kCut: a k-contiguous operand's rows are no whole quads.
-template <bool kTA, bool kTB, bool kCut, class E = NoEpilogue>
+// kCut: a k-contiguous operand's rows are no whole quads.  kLong: a wavefront's share of the reduction may be longer than kSmallPart; each
+// such part has an accumulator of its own then.
+constexpr int kSmallPart = 1024;
+template <bool kTA, bool kTB, bool kCut, class E = NoEpilogue, bool kLong = false>
 __device__ __forceinline__ void sgemm_small_body(int M, int N, int K, int lda, int ldb, int kslice, const float *A,
                                                  const float *B, float *C, const float *colbias, int bias_shift,
                                                  const float *rowvec, int relu, const float *mask, int bx, int by, int k0, int k1,
@@ -83,16 +85,29 @@ __device__ __forceinline__ void sgemm_small_body(int M, int N, int K, int lda, i
     // load in flight at the top of the loop), then the steps left over, whose operands are in their registers or on
     // their way already.
     const int whole = nsteps / kSmallDepth * kSmallDepth;
-    for (int s = 0; s < whole; s += kSmallDepth) {
+    auto rounds = [&](int from, int to) {
+        for (int s = from; s < to; s += kSmallDepth) {
 #pragma unroll
-        for (int j = 0; j < kSmallDepth; j++) {
+            for (int j = 0; j < kSmallDepth; j++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(value_a(j, s, e), value_b(j, s, e), acc, 0, 0, 0);
-            const int kk = k_begin + 8 * (s + j + kSmallDepth) + 4 * half;   // this register set's next step
-            small_load<!kTA>(rsa, abase, apitch, kk, k_end, a[j]);
-            small_load<kTB>(rsb, bbase, bpitch, kk, k_end, b[j]);
-            __builtin_amdgcn_sched_barrier(0);   // keep each refill behind its own step: sunk to the loop's end, all of them are waited for at once
+                for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(value_a(j, s, e), value_b(j, s, e), acc, 0, 0, 0);
+                const int kk = k_begin + 8 * (s + j + kSmallDepth) + 4 * half;   // this register set's next step
+                small_load<!kTA>(rsa, abase, apitch, kk, k_end, a[j]);
+                small_load<kTB>(rsb, bbase, bpitch, kk, k_end, b[j]);
+                __builtin_amdgcn_sched_barrier(0);   // keep each refill behind its own step: sunk to the loop's end, all of them are waited for at once
+            }
         }
+    };
+    v16f parts = {};
+    if constexpr (kLong) {
+        constexpr int kPart = kSmallPart / 8;   // steps
+        for (int s = 0; s < whole; s += kPart) {
+            rounds(s, min(whole, s + kPart));
+            parts += acc;
+            acc = v16f{};
+        }
+    } else {
+        rounds(0, whole);
     }
 #pragma unroll
     for (int j = 0; j < kSmallDepth - 1; j++)
@@ -101,7 +116,7 @@ __device__ __forceinline__ void sgemm_small_body(int M, int N, int K, int lda, i
             for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(value_a(j, whole, e), value_b(j, whole, e), acc, 0, 0, 0);
         }
 #pragma unroll
-    for (int v = 0; v < 16; v++) red[wave][acc_row(v, lane) * 33 + r] = acc[v];
+    for (int v = 0; v < 16; v++) red[wave][acc_row(v, lane) * 33 + r] = kLong ? parts[v] + acc[v] : acc[v];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; i++) {

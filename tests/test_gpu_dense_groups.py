@@ -454,3 +454,22 @@ def test_gradients_of_more_rows_than_two_to_the_thirty(k):
     R.close(np.stack([dx.view(p * k, (k,)).numpy() for p in places]), want[0], "dx")
     R.close(dw.numpy(), want[1], "dw")
     R.close(db.numpy(), want[2], "dbias")
+
+
+@pytest.mark.parametrize("n", [70001, 1 << 20])
+def test_many_equal_values_of_a_row(n):
+    """dx of layers of so many columns and two inputs: products of 0.1 and one.  At most 1024 of them follow each other, whose sums of one sign are off by half
+    of that many roundings, then up to 128 such sums and eight wavefronts'."""
+    dy, w = np.full((40, n), 0.1, F32), np.ones((2, n, 2), F32)
+    offsets = ops.tensor(np.array([0, 33, 40], np.int32))
+    dx = ops.Tensor((40, 2))
+    capi.check(capi.load().dopt_hip_dense_groups_grad(2, 40, n, 2, 0, offsets.ptr, ops.tensor(dy).ptr, None, None, ops.tensor(w).ptr, dx.ptr, None, None))
+    assert np.abs(dx.numpy() / (n * np.float64(F32(0.1))) - 1).max() <= 600 * R.E
+
+
+def test_many_equal_values_of_a_long_reduction():
+    """The same forward, of rows enough that they go by tiles."""
+    m, n, k = 7000, 2, 65536
+    x, w = np.full((m, k), 0.1, F32), np.ones((1, n, k), F32)
+    y = ops.dense_groups(ops.tensor(x), ops.tensor(w), ops.tensor(np.array([0, m], np.int32)))
+    assert np.abs(y.numpy() / (k * np.float64(F32(0.1))) - 1).max() <= 600 * R.E
