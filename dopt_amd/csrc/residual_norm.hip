@@ -364,7 +364,7 @@ template <int kLanes, int Q, bool kWhole, int kThreads>
 __global__ __launch_bounds__(kThreads) void join_grad_k(Grads g, Runs runs, int waves)
 {
     constexpr bool kStaged = kLanes || Q < 4;
-    constexpr bool kAhead = kLanes ? Q <= 2 : kThreads <= 768;   // the next row is on its way while one is worked on
+    constexpr bool kAhead = kLanes || kThreads <= 768;   // the next row is on its way while one is worked on
     constexpr bool kWaves = kLanes == 0 || kLanes == 64;
     constexpr bool kSumsInLds = !kLanes && Q == 4;               // those of dh: the registers hold the others
     __shared__ float red[64];
@@ -762,16 +762,19 @@ Form form_of(size_t cols, bool back)
     }
     return Form{0, 4, quads <= 256 * 12 ? 768u : 1024u};
 }
-template <class F>
+template <bool kBack, class F>
 void with_form(const Form &f, F &&call)
 {
     auto c = [](auto v) { return v; };
     if (f.lanes == 16) call(c(std::integral_constant<int, 16>{}), c(std::integral_constant<int, 1>{}));
     else if (f.lanes == 32) call(c(std::integral_constant<int, 32>{}), c(std::integral_constant<int, 1>{}));
     else if (f.lanes == 64 && f.quads == 1) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 1>{}));
-    else if (f.lanes == 64 && f.quads == 2) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 2>{}));
-    else if (f.lanes == 64) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 4>{}));
-    else if (f.quads == 2) call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 2>{}));
+    else if (f.lanes == 64) {
+        if constexpr (!kBack) {
+            if (f.quads == 2) call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 2>{}));
+            else call(c(std::integral_constant<int, 64>{}), c(std::integral_constant<int, 4>{}));
+        }
+    } else if (f.quads == 2) call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 2>{}));
     else call(c(std::integral_constant<int, 0>{}), c(std::integral_constant<int, 4>{}));
 }
 
@@ -899,7 +902,7 @@ int dopt_hip_residual_norm(const dopt_hip_residual_norm_desc *d, const float *x,
     } else {
         const Form form = form_of(d->cols, false);
         const size_t blocks = form.lanes ? ceil_div(d->rows, (size_t)(kBlock / form.lanes)) : d->rows;
-        with_form(form, [&](auto lanes, auto quads) {
+        with_form<false>(form, [&](auto lanes, auto quads) {
             const auto kernel = join_k<lanes.value, quads.value>;
             // every workgroup loads the scales once: no more of them than run at a time, and as many rows for each
             static Places known{};
@@ -975,7 +978,7 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     const bool whole = (runs.per_gate < std::min(kWholeRows, 4 * teams) && d->gates > 2 * (size_t)num_cus()) || d->gates >= kMostRuns;
     if (held) {
         int rc = DOPT_HIP_OK;
-        with_form(form, [&](auto lanes, auto quads) {
+        with_form<true>(form, [&](auto lanes, auto quads) {
             auto with = [&](auto most) {
                 rc = whole ? grad_launch<lanes.value, quads.value, true, most.value>(threads, lds, &launch)
                            : grad_launch<lanes.value, quads.value, false, most.value>(threads, lds, &launch);

@@ -1,6 +1,7 @@
 """The residual norm: what is refused before the device is touched, what the graph operation is, and its float64 form against
 differences."""
 import ctypes as C
+import re
 
 import numpy as np
 import pytest
@@ -131,3 +132,9 @@ def test_gradient_against_differences(post, pre, gates):
         up[name], down[name] = v + step * d, v - step * d
         slope, want = (loss(up) - loss(down)) / (2 * step), float((g * d).sum())
         assert abs(slope - want) <= 1e-6 * (1 + np.abs(g * d).sum()), (name, slope, want)
+
+
+def test_the_library_holds_no_gradient_that_no_call_reaches():
+    """A wavefront's lanes have one quad of a row backward; longer rows go to whole wavefronts."""
+    names = set(re.findall(rb"join_grad_kILi(\d+)ELi(\d+)E", open(capi.LIB_PATH, "rb").read()))
+    assert names == {(b"16", b"1"), (b"32", b"1"), (b"64", b"1"), (b"0", b"2"), (b"0", b"4")}
