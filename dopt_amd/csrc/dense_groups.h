@@ -20,11 +20,11 @@ double groups_split_us(size_t G, size_t M, size_t N, size_t K);
 double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K);
 double groups_wide_us(size_t G, size_t M, size_t N, size_t K);
 double groups_wide_grad_us(size_t G, size_t M, size_t N, size_t K);
-int groups_split(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
-int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
+int groups_split(GroupLayer l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
+int groups_wide(GroupLayer l, const float *x, const float *w, const float *bias, int act, float *y, float *pre);
 // dy and pre give dz, which is written where there is an activation; any result may be null.
-int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
-int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
+int groups_split_grad(GroupLayer l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
+int groups_wide_grad(GroupLayer l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias);
 // dz (which may be null) of N >= 4 columns, and the sums (null too) of runs of 2^shift rows of a group.
 int groups_dz(const GroupLayer &l, int act, int shift, const float *dy, const float *pre, float *dz, float *sums);
 

@@ -243,6 +243,39 @@ __global__ __launch_bounds__(256) void groups_dz_k(GroupLayer l, int act, const 
     });
     if (sums) sums[(size_t)unit_id() * l.N + c] = sum;
 }
+// The fronts of a kind of units by a workgroup of sixteen wavefronts, sixteen pieces at a time.
+struct FrontKinds {
+    Units kind[kMostFronts];
+};
+__global__ __launch_bounds__(1024) void groups_fronts_k(Groups q, FrontKinds kinds, Front *fronts)
+{
+    __shared__ unsigned ends[16], counts[16];
+    const Units kind = kinds.kind[blockIdx.x];
+    Front *const to = fronts + (size_t)blockIdx.x * q.pieces;
+    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = segments_of(q, kind.rest);
+    unsigned units = 0, bound = first_row(q, kind.rest);
+    for (unsigned base = 0; base < count; base += 1024) {
+        const unsigned s = base + threadIdx.x;
+        unsigned end = wave_scan(end_of(q, kind.rest, s), [](unsigned a, unsigned b) { return max(a, b); });
+        if (lane == 63) ends[wave] = end;
+        __syncthreads();
+        unsigned before = bound;   // where what lies in front of the wavefront's piece ends
+        for (unsigned i = 0; i < wave; i++) before = max(before, ends[i]);
+        for (unsigned i = 0; i < 16; i++) bound = max(bound, ends[i]);
+        end = max(end, before);
+        unsigned begin = (unsigned)__shfl_up((int)end, 1, 64);
+        if (lane == 0) begin = before;
+        const unsigned n = s < count ? units_of(begin, end, kind.shift, kind.all) : 0;
+        const unsigned upto = wave_scan(n, [](unsigned a, unsigned b) { return a + b; });
+        if (lane == 63) counts[wave] = upto;
+        __syncthreads();
+        unsigned in_front = units;
+        for (unsigned i = 0; i < wave; i++) in_front += counts[i];
+        for (unsigned i = 0; i < 16; i++) units += counts[i];
+        if (lane == 0 && s < count) to[s / 64] = Front{in_front, before};
+        __syncthreads();
+    }
+}
 __global__ __launch_bounds__(256) void groups_zero_k(size_t n, float *p)
 {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0.0f;
@@ -334,6 +367,31 @@ int apart(const char *who, const Span (&in)[I], const Span (&out)[O])
 
 namespace dopt {
 
+int groups_scratch(Groups *q, std::initializer_list<Units> units, size_t bytes, char **scratch)
+{
+    const size_t pieces = ceil_div((size_t)q->G + 2, (size_t)64), kinds = q->G > kNoFronts ? units.size() : 0;
+    const size_t front_bytes = ceil_div(kinds * pieces * sizeof(Front), (size_t)256) * 256;
+    *scratch = nullptr;
+    if (front_bytes + bytes == 0) return DOPT_HIP_OK;
+    char *const at = (char *)workspace(front_bytes + bytes);
+    if (!at) return DOPT_HIP_ERR_OOM;
+    *scratch = at + front_bytes;
+    if (!kinds) return DOPT_HIP_OK;
+    DOPT_REQUIRE(kinds <= kMostFronts, "dopt_hip_dense_groups: more kinds of units than there are places for");
+    FrontKinds all{};
+    q->pieces = (unsigned)pieces;
+    for (int &key : q->keys) key = -1;
+    size_t i = 0;
+    for (const Units &u : units) {
+        all.kind[i] = u;
+        q->keys[i++] = u.key();
+    }
+    hipLaunchKernelGGL(groups_fronts_k, dim3((unsigned)kinds), dim3(1024), 0, stream(), *q, all, (Front *)at);
+    DOPT_LAUNCH_CHECK();
+    q->fronts = (const Front *)at;
+    return DOPT_HIP_OK;
+}
+
 int groups_join(const GroupLayer &l, int shift, const float *parts, float *dw)
 {
     const size_t matrix = (size_t)l.N * l.K;
@@ -358,13 +416,15 @@ int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const
     const Span results[] = {{y, out}, {pre, out}};
     if (int rc = apart(who, in, results)) return rc;
     DOPT_ENSURE_INIT();
-    const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    char *scratch;
     const Way way = G == 0 ? Way::kSmall : way_of(few_us(G, M, N, K), small_us(G, M, N, K), groups_split_us(G, M, N, K), groups_wide_us(G, M, N, K));
     if (way == Way::kSplit) return groups_split(l, x, w, bias, act, y, pre);
     if (way == Way::kWide) return groups_wide(l, x, w, bias, act, y, pre);
     if (way == Way::kFew) {
         auto few = [&](auto rows) {
             constexpr int R = decltype(rows)::value;
+            if (int rc = groups_scratch(&l.q, {Units{R / 2, true, false}}, 0, &scratch)) return rc;
             hipLaunchKernelGGL(groups_few_k<R>, grid_of(ceil_div(N, (size_t)8), most_units(M, G + 2, R / 2)), dim3(256), 0, stream(), l, x, w, bias, y, pre, act);
             DOPT_LAUNCH_CHECK();
             return (int)DOPT_HIP_OK;
@@ -374,6 +434,7 @@ int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const
     }
     const dim3 grid = grid_of(ceil_div(N, (size_t)32), most_units(M, G + 2, kTileShift));
     const int slice = (int)slice_of(K);
+    if (int rc = groups_scratch(&l.q, {Units{kTileShift, true, false}}, 0, &scratch)) return rc;
     with_reduction(K, [&](auto cut, auto is_long) {
         hipLaunchKernelGGL((groups_small_k<cut.value, is_long.value>), grid, dim3(64 * kSmallWaves), 0, stream(), l, slice, x, w, bias, y, pre, act);
     });
@@ -405,7 +466,7 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
         if (int rc = clear(dw, G * N * K)) return rc;
         return clear(dbias, G * N);
     }
-    const GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
+    GroupLayer l{Groups{offsets, (unsigned)G, (unsigned)M}, (int)N, (int)K};
     const Way way = way_of(HUGE_VAL, small_grad_us(G, M, N, K), groups_split_grad_us(G, M, N, K), groups_wide_grad_us(G, M, N, K));
     if ((dx || dw) && way == Way::kSplit) return groups_split_grad(l, act, dy, pre, x, w, dx, dw, dbias);
     if ((dx || dw) && way == Way::kWide) return groups_wide_grad(l, act, dy, pre, x, w, dx, dw, dbias);
@@ -421,8 +482,10 @@ int dopt_hip_dense_groups_grad(size_t G, size_t M, size_t N, size_t K, int act, 
     const bool plain = act == DOPT_HIP_ACT_NONE;
     const size_t dz_bytes = plain || !(dx || dw) ? 0 : rounded(M * N * f), sum_bytes = dbias ? rounded(runs * N * f) : 0,
                  part_bytes = dw && !direct ? dw_units * N * K * f : 0;
-    char *const scratch = dz_bytes + sum_bytes + part_bytes ? (char *)workspace(dz_bytes + sum_bytes + part_bytes) : nullptr;
-    if (dz_bytes + sum_bytes + part_bytes && !scratch) return DOPT_HIP_ERR_OOM;
+    char *scratch;
+    if (int rc = groups_scratch(&l.q, {Units{kTileShift, true, false}, Units{kRunShift, false, false}, Units{shift, false, true}},
+                                dz_bytes + sum_bytes + part_bytes, &scratch))
+        return rc;
     float *const dz_to = dz_bytes ? (float *)scratch : nullptr, *const sums = (float *)(scratch + dz_bytes), *const parts = (float *)(scratch + dz_bytes + sum_bytes);
     const float *const dz = plain ? dy : dz_to;
     if (!plain || dbias) {

@@ -248,14 +248,16 @@ double groups_split_grad_us(size_t G, size_t M, size_t N, size_t K)
     return 11.5 + 3.4e-6 * M * N + products;
 }
 
-int groups_split(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
+int groups_split(GroupLayer l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
 {
     const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, across = ceil_div(N, (size_t)kTile);
     size_t parts;
     forward_us(G, M, N, K, &parts);
     SplitForward f{x, w, bias, y, pre, nullptr, act, (unsigned)across, (unsigned)parts, (unsigned)(ceil_div(ceil_div(K, (size_t)kChunk), parts) * kChunk)};
     f.count = (unsigned)ceil_div(K, (size_t)f.steps);
-    if (parts > 1 && !(f.parts = (float *)workspace(f.count * M * N * sizeof(float)))) return DOPT_HIP_ERR_OOM;
+    char *scratch;
+    if (int rc = groups_scratch(&l.q, {Units{kTileShift, true, false}, Units{0, true, false}}, parts > 1 ? f.count * M * N * sizeof(float) : 0, &scratch)) return rc;
+    if (parts > 1) f.parts = (float *)scratch;
     // (workgroups and one, two, four teams: 160 18.9 14.0 12.7 us, 288 22.1 19.4 23.7, 544 28.0 30.0 36.4, reductions of 512 steps)
     const double tiles = group_tiles(G, M, N, kTile) * parts;
     const int teams = tiles <= num_cus() ? 4 : tiles <= 2 * num_cus() ? 2 : 1;
@@ -269,7 +271,7 @@ int groups_split(const GroupLayer &l, const float *x, const float *w, const floa
     return rc || parts == 1 ? rc : end_of_parts(l, f);
 }
 
-int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
+int groups_split_grad(GroupLayer l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
 {
     const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, tiles = ceil_div(N, (size_t)kTile) * ceil_div(K, (size_t)kTile);
     const int shift = dw ? part_shift(G, M, tiles) : kLongestPart;
@@ -281,8 +283,9 @@ int groups_split_grad(const GroupLayer &l, int act, const float *dy, const float
     auto rounded = [](size_t bytes) { return ceil_div(bytes, (size_t)256) * 256; };
     const size_t dz_bytes = plain ? 0 : rounded(M * N * f), sum_bytes = dbias ? rounded(runs * N * f) : 0, dx_bytes = count > 1 ? rounded(count * M * K * f) : 0;
     const size_t part_bytes = dw && !direct ? dw_units * N * K * f : 0, bytes = dz_bytes + sum_bytes + dx_bytes + part_bytes;
-    char *const scratch = bytes ? (char *)workspace(bytes) : nullptr;
-    if (bytes && !scratch) return DOPT_HIP_ERR_OOM;
+    char *scratch;
+    if (int rc = groups_scratch(&l.q, {Units{kTileShift, true, false}, Units{kRunShift, false, false}, Units{shift, false, true}, Units{0, true, false}}, bytes, &scratch))
+        return rc;
     float *const dz_to = plain ? nullptr : (float *)scratch, *const sums = (float *)(scratch + dz_bytes);
     float *const dx_parts = dx_bytes ? (float *)(scratch + dz_bytes + sum_bytes) : nullptr, *const parts = (float *)(scratch + dz_bytes + sum_bytes + dx_bytes);
     if (!plain || dbias)

@@ -20,6 +20,7 @@ namespace {
 using namespace dopt;
 
 constexpr int kStepShift = 6;   // rows of a tile of the turned operands' layout
+constexpr Units kRests{31, true, true};   // a unit for each group, and for the rows in front of them and behind
 
 // A group that these offsets leave empty, whatever came before (others may be empty as well).
 __device__ __forceinline__ bool surely_empty(const Groups &q, unsigned g) { return q.offsets[g + 1] <= q.offsets[g]; }
@@ -183,7 +184,7 @@ struct GroupLayout {
 __device__ __forceinline__ void clear_rest(const Groups &q, float *p, size_t cols, unsigned block, unsigned blocks)
 {
     if (!p) return;
-    const Segment front = find_unit<true, true>(q, 31, 0), back = find_unit<true, true>(q, 31, q.G + 1);   // (a unit for each)
+    const Segment front = find_unit<kRests.rest, kRests.all>(q, kRests.shift, 0), back = find_unit<kRests.rest, kRests.all>(q, kRests.shift, q.G + 1);
     const size_t first = front.end, n = first + (back.end - back.begin);
     for (size_t i = (size_t)block * blockDim.x + threadIdx.x; i < n * cols; i += (size_t)blocks * blockDim.x)
         p[i < first * cols ? i : i + (back.begin - first) * cols] = 0.0f;
@@ -434,7 +435,7 @@ double groups_wide_grad_us(size_t G, size_t M, size_t N, size_t K)
     return 32.7 + 1e-6 * (9.9 * m * N + 4.5 * m * K + 3.9 * weights) + 3.5e-9 * (m + 64.0 * G) * N * K;
 }
 
-int groups_wide(const GroupLayer &l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
+int groups_wide(GroupLayer l, const float *x, const float *w, const float *bias, int act, float *y, float *pre)
 {
     const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, steps = ceil_div(K, (size_t)16), tile = tile_for(G, M, N, K);
     const size_t mtiles = most_units(M, G, shift_of_tile(tile)), rows = mtiles * tile, padded = padded_to(N, tile), ntiles = padded / tile;
@@ -448,8 +449,8 @@ int groups_wide(const GroupLayer &l, const float *x, const float *w, const float
                              passes ? s.take(mtiles * ntiles * tile * tile * 4) : nullptr, (unsigned)ntiles};
         return s.bytes;
     };
-    char *const scratch = (char *)workspace(plan(Scratch{nullptr}));
-    if (!scratch) return DOPT_HIP_ERR_OOM;
+    char *scratch;
+    if (int rc = groups_scratch(&l.q, {Units{shift_of_tile(tile), false, false}, kRests}, plan(Scratch{nullptr}), &scratch)) return rc;
     plan(Scratch{scratch});
     lay.rest[0] = y;
     lay.rest[1] = pre;
@@ -465,7 +466,7 @@ int groups_wide(const GroupLayer &l, const float *x, const float *w, const float
     return launch_products(l.q, tile, passes, p);
 }
 
-int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
+int groups_wide_grad(GroupLayer l, int act, const float *dy, const float *pre, const float *x, const float *w, float *dx, float *dw, float *dbias)
 {
     const size_t G = l.q.G, M = l.q.M, N = l.N, K = l.K, steps = ceil_div(N, (size_t)16);
     const size_t tile = dw && G * ceil_div(N, (size_t)kBig) * ceil_div(K, (size_t)kBig) < (size_t)num_cus() ? (size_t)kSmall : tile_for(G, M, K, N);
@@ -519,8 +520,10 @@ int groups_wide_grad(const GroupLayer &l, int act, const float *dy, const float 
         }
         return s.bytes;
     };
-    char *const scratch = (char *)workspace(plan(Scratch{nullptr}));
-    if (!scratch) return DOPT_HIP_ERR_OOM;
+    char *scratch;
+    if (int rc = groups_scratch(&l.q, {Units{shift_of_tile(tile), false, false}, Units{kStepShift, false, false}, Units{shift, false, false},
+                                       Units{part_shift, false, true}, kRests}, plan(Scratch{nullptr}), &scratch))
+        return rc;
     plan(Scratch{scratch});
     jobs.shift = shift;
     jobs.w_rows = (int)N;

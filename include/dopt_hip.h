@@ -595,7 +595,7 @@ int dopt_hip_dense_act_grad(size_t M, size_t N, size_t K, int act, const float *
    products and those of single rows (and the gradients of all but small ones) are formed from two fp16 parts of each value, scaled row by
    row: a value keeps 22 bits, or 2^-38 of its row's largest one; infinities and NaN reach what fp32 would give them.  Workspace: large
    products four bytes a value of both operands, long reductions over few tiles the result for each of up to sixteen parts; gradients dz, its
-   column sums by runs of rows, and dw for each part of a group's rows. */
+   column sums by runs of rows, and dw for each part of a group's rows; more than 256 groups up to 40 bytes for every 64 of them. */
 int dopt_hip_dense_groups(size_t G, size_t M, size_t N, size_t K, int act, const int32_t *offsets, const float *x, const float *w,
                           const float *bias, float *y, float *pre);
 /* With dz = dy * act'(pre): dx = dz * w[g] [M,K], zero for rows of no group; dw[g] = dz^T * x [G,N,K] and dbias[g] = column sums of dz

@@ -473,3 +473,78 @@ def test_many_equal_values_of_a_long_reduction():
     x, w = np.full((m, k), 0.1, F32), np.ones((1, n, k), F32)
     y = ops.dense_groups(ops.tensor(x), ops.tensor(w), ops.tensor(np.array([0, m], np.int32)))
     assert np.abs(y.numpy() / (k * np.float64(F32(0.1))) - 1).max() <= 600 * R.E
+
+
+def _spread(g, m, seed):
+    """Sizes of g groups with m rows in all, of which every third on average has none."""
+    r = np.random.default_rng(seed)
+    weight = r.random(g) * (r.random(g) < 0.67)
+    weight[g // 2] += 1
+    return np.bincount(np.searchsorted(np.cumsum(weight / weight.sum()), r.random(m) * 0.999999), minlength=g)
+
+
+# more than 256 groups, whose searches begin at a piece of 64: sizes of single rows, small, split and wide products and gradients
+@pytest.mark.parametrize("g,m,n,k", [(257, 700, 33, 20), (300, 50, 300, 2000), (300, 3000, 40, 60), (300, 5000, 200, 3000), (257, 60000, 192, 128), (257, 100000, 128, 1024),
+                                     (4096, 4000, 24, 64), (5000, 20000, 64, 64), (70000, 50000, 16, 16), (1 << 20, 5000, 4, 4), (1 << 20, 5000, 3, 2)])
+@pytest.mark.parametrize("falling", [False, True])
+def test_long_lists_of_groups(g, m, n, k, falling):
+    """Groups at borders of pieces, the last ones and some others against their definition; what has no rows, or no group, is zero."""
+    before, after = 37, 70
+    t = _case(_spread(g, m, g + m), n, k, 11, before, after)
+    m = len(t["x"])
+    name = R.ACTS[n % 4]
+    if falling:   # (rows of the next group that does not fall)
+        r = np.random.default_rng(5)
+        low = r.choice(np.arange(1, g), g // 5, replace=False)
+        t["offsets"][low] -= r.integers(0, m, g // 5).astype(np.int32)
+    at = D.bounds(t["offsets"], m)
+    d = {key: ops.tensor(v) for key, v in t.items()}
+    y, pre = _place((m, n), ops.tensor), _place((m, n), ops.tensor)
+    ops.dense_groups(d["x"], d["w"], d["offsets"], d["bias"], name, out=y, pre=pre)
+    plain = name == "none"
+    grads = ops.dense_groups_grad(d["dy"], d["x"], d["w"], d["offsets"], None if plain else d["pre"], name, dx=_place((m, k), ops.tensor),
+                                  dw=_place((g, n, k), ops.tensor), dbias=_place((g, n), ops.tensor))
+    y, pre, dx, dw, db = (v.numpy() for v in (y, pre) + tuple(grads))
+    sizes = np.diff(at)
+    some = np.random.default_rng(1).choice(np.flatnonzero(sizes), min(30, np.count_nonzero(sizes)), replace=False)
+    border = [b for b in (0, 1, 62, 63, 64, 65, 127, 128, 1023, 1024, 4095, 4096, 65535, 65536, g - 66, g - 2, g - 1) if 0 <= b < g]
+    for i in sorted(set(some) | set(border)):
+        s, one, local = slice(at[i], at[i + 1]), slice(i, i + 1), [0, sizes[i]]
+        if not sizes[i]:
+            continue
+        of = {key: t[key][s] for key in ("x", "dy", "pre")}
+        want = D.forward(of["x"], t["w"][one], t["bias"][one], local, name, True)
+        R.close(y[s], want[0], "y of group %d" % i)
+        R.close(pre[s], want[1], "pre of group %d" % i)
+        want = D.backward(of["dy"], of["x"], t["w"][one], None if plain else of["pre"], local, name, True)
+        for a, b, what in zip((dx[s], dw[one], db[one]), want, ("dx", "dw", "dbias")):
+            R.close(a, b, "%s of group %d" % (what, i))
+    assert not dw[sizes == 0].any() and not db[sizes == 0].any()
+    for a in (y, pre, dx):
+        assert not a[:at[0]].any() and not a[at[-1]:].any()
+
+
+@pytest.mark.parametrize("flags", FLAGS)
+def test_long_lists_in_a_graph(flags):
+    """As test_in_a_graph, of 300 groups whose sizes change from step to step."""
+    n, k, g, m = 20, 30, 300, 900
+    t = _case(_spread(g, m, 3), n, k, 5)
+    f = {key: core.float32(t[key].shape) for key in ("x", "w", "bias", "dy")}
+    o = core.int32(t["offsets"].shape)
+    y = core.denseGroups(f["x"], f["w"], o, f["bias"], "gelu")
+    outputs = [y] + core.grad(core.sum(y * f["dy"], [0, 1]).reshape([]), [f[key] for key in ("x", "w", "bias")])
+    plan = core.compile(outputs, flags)
+    rets = [ops.Tensor(v.shape) for v in outputs]
+    args = {f[key]: ops.tensor(t[key]) for key in f}
+    args[o] = ops.tensor(t["offsets"])
+    for seed in (3, 4, 5, 3):
+        t["offsets"] = np.concatenate([[0], np.cumsum(_spread(g, m, seed))]).astype(np.int32)
+        args[o].set(t["offsets"])
+        plan.execute(args, rets)
+        p = ops.Tensor((m, n))
+        want = [ops.dense_groups(args[f["x"]], args[f["w"]], args[o], args[f["bias"]], "gelu", pre=p)]
+        want += ops.dense_groups_grad(args[f["dy"]], args[f["x"]], args[f["w"]], args[o], p, "gelu")
+        for a, b in zip(rets, want):
+            assert np.array_equal(a.numpy().reshape(b.shape), b.numpy())
+        (whole, bound), _ = D.forward(t["x"], t["w"], t["bias"], t["offsets"], "gelu", True)
+        R.close(rets[0].numpy(), (whole, bound), "y")
