@@ -483,8 +483,9 @@ def _spread(g, m, seed):
     return np.bincount(np.searchsorted(np.cumsum(weight / weight.sum()), r.random(m) * 0.999999), minlength=g)
 
 
-# more than 256 groups, whose searches begin at a piece of 64: sizes of single rows, small, split and wide products and gradients
-@pytest.mark.parametrize("g,m,n,k", [(257, 700, 33, 20), (300, 50, 300, 2000), (300, 3000, 40, 60), (300, 5000, 200, 3000), (257, 60000, 192, 128), (257, 100000, 128, 1024),
+# more than a piece of 64 groups, and more than 256, whose searches begin at a piece: sizes of single rows, small, split and wide products and gradients
+@pytest.mark.parametrize("g,m,n,k", [(100, 700, 33, 20), (100, 50, 300, 2000), (100, 2000, 100, 200), (100, 30000, 320, 128), (100, 40000, 128, 1024),
+                                     (257, 700, 33, 20), (300, 50, 300, 2000), (300, 3000, 40, 60), (300, 5000, 200, 3000), (257, 60000, 192, 128), (257, 100000, 128, 1024),
                                      (4096, 4000, 24, 64), (5000, 20000, 64, 64), (70000, 50000, 16, 16), (1 << 20, 5000, 4, 4), (1 << 20, 5000, 3, 2)])
 @pytest.mark.parametrize("falling", [False, True])
 def test_long_lists_of_groups(g, m, n, k, falling):
