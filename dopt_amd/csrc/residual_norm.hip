@@ -33,7 +33,7 @@ constexpr int kBlock = 256;          // of teams within a wavefront
 constexpr size_t kHeld = 16384;      // values of a row that a workgroup holds at most
 constexpr size_t kWholeRows = 16;    // of a gate
 constexpr size_t kTeamRows = 128;    // rows that a team adds up at most: sums of more values that are alike are rounded the same way for long
-constexpr size_t kMostRuns = (size_t)1 << 22;   // workgroups of a launch, which has fewer than 2^32 threads
+constexpr size_t kMostRuns = (size_t)1 << 22, kMostColumns = (size_t)1 << 24;   // workgroups of a launch, which has fewer than 2^32 threads
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));   // sixteen bytes wherever they start
@@ -974,8 +974,10 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
     Launch launch{nullptr, kBlock, 0, (size_t)num_cus() * 8};
     // Gates of few rows go to teams as a whole where there are many of them, else to a workgroup each, whose teams share the rows: [1500 x 600]
     // with 100 gates 19.6 us (as a whole 64), [2400 x 1500] with 200 33 (70), [2000 x 700] with 500 28 (27), [8000 x 600] with 1000 71 (51), with 4000 180 (50).
-    // So do the gates of any number of rows where a launch has no workgroup for each (a team then adds up a whole gate, of at most 511 rows).
-    const bool whole = (runs.per_gate < std::min(kWholeRows, 4 * teams) && d->gates > 2 * (size_t)num_cus()) || d->gates >= kMostRuns;
+    // So do the gates of any number of rows where a launch has no workgroups for each (a team then adds up a whole gate, of at most 511 rows).
+    const size_t column_tiles = ceil_div(d->cols, (size_t)kBlock);
+    const bool whole = (runs.per_gate < std::min(kWholeRows, 4 * teams) && d->gates > 2 * (size_t)num_cus()) ||
+                       (held ? d->gates >= kMostRuns : d->gates * column_tiles >= kMostColumns);
     if (held) {
         int rc = DOPT_HIP_OK;
         with_form<true>(form, [&](auto lanes, auto quads) {
@@ -1035,9 +1037,8 @@ int dopt_hip_residual_norm_grad(const dopt_hip_residual_norm_desc *d, const floa
         DOPT_HIP_CHECK(hipLaunchKernel(launch.kernel, dim3((unsigned)blocks), dim3(launch.threads), arguments, launch.lds, stream()));
     } else if (d->rows) {
         hipLaunchKernelGGL(join_grad_long_k, dim3((unsigned)std::min(d->rows, (size_t)num_cus() * 8)), dim3(kLong), 0, stream(), g, (Means *)scratch);
-        const size_t tiles = ceil_div(d->cols, (size_t)kBlock);
-        DOPT_REQUIRE(tiles * runs.count < (size_t)1 << 24, "%s: dimensions too large", who);
-        if (kinds || dgate) hipLaunchKernelGGL(join_columns_k, dim3((unsigned)(tiles * runs.count)), dim3(kBlock), 0, stream(), g, runs, (const Means *)scratch);
+        DOPT_REQUIRE(column_tiles * runs.count < kMostColumns, "%s: dimensions too large", who);
+        if (kinds || dgate) hipLaunchKernelGGL(join_columns_k, dim3((unsigned)(column_tiles * runs.count)), dim3(kBlock), 0, stream(), g, runs, (const Means *)scratch);
         DOPT_LAUNCH_CHECK();
     }
     Fold fold{};

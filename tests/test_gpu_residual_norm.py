@@ -147,6 +147,25 @@ def test_gates_beyond_the_workgroups_of_a_launch(per_gate, cols):
     R_close(got["dpost_scale"], (total, (256 + 8) * 2.0 ** -24 * size), "dpost_scale")
 
 
+def test_gates_of_long_rows_beyond_the_workgroups_of_a_launch():
+    """As many gates of four rows, of 65 workgroups' columns each, as a launch has no workgroups for.  All but some rows are zero; the gradient of y, the branch and the gate
+    lie in the same memory."""
+    gates, cols = (1 << 24) // 65 + 1, 16640
+    big, dgate = ops.Tensor((4 * gates, cols)), ops.Tensor((gates, cols))
+    r = np.random.default_rng(2)
+    places = [0, 31, 32, 1000, gates - 1]
+    values = _f(r.standard_normal((len(places), 4, cols)))
+    for p, v in zip(places, values):
+        big.view(4 * p * cols, (4, cols)).set(v)
+        dgate.view(p * cols, (cols,)).set(v[0])
+    dgate.view(5 * cols, (cols,)).set(values[0, 0])
+    ops.residual_norm_grad(big, None, None, big, None, big.view(0, (gates, cols)), out={"dgate": dgate})
+    for p, v in zip(places, values):   # three sums of four squares
+        want = (v.astype(np.float64) ** 2).sum(0)
+        R_close(dgate.view(p * cols, (cols,)).numpy(), (want, 8 * 2.0 ** -24 * want), "dgate")
+    assert not dgate.view(5 * cols, (cols,)).numpy().any()
+
+
 def test_rows_beyond_thirty_two_bits_of_values():
     """2^32 values and more: rows before and behind that border, of which the others are zero."""
     rows, cols = (1 << 21) + 5, 2048 + 4
